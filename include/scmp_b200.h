@@ -203,6 +203,125 @@ SCMP_API int scmp_scale_residual(float *out, const float *x, const float *y, con
 SCMP_API int scmp_split_qkv(const void *qkv, int64_t B, int64_t N, int64_t H, int64_t D,
                             int elem_bytes, void *q, void *k, void *vt, void *stream);
 
+/* ---- Microscaled 4-bit floating point (no reference counterpart: the
+ * deterministic 4-bit product that the SC estimates stand next to).
+ * An operand [rows, K] becomes e2m1 codes with one scale per block along K:
+ *   SCMP_MXFP4  blocks of 32, scale 2^E (e8m0), E = floor(log2 max|x|) - 2, at
+ *               least -127; scale_exp must be 0
+ *   SCMP_NVFP4  blocks of 16, scale s (e4m3) = max|x| / (6 * 2^scale_exp)
+ *               rounded to nearest even and at most 448; the block's step is
+ *               s * 2^scale_exp (a power of two per tensor, so that no rounding
+ *               but the codes' own enters)
+ * and each code is x / step rounded to nearest even among 0, .5, 1, 1.5, 2, 3,
+ * 4, 6, saturating.  A block that holds a NaN or an infinity stands for NaNs.
+ * Buffers (16-byte aligned; sizes from scmp_mx_data_size / scmp_mx_scale_size,
+ * 0 on bad sizes):
+ *   data    [rows][ceil32(K) / 2] bytes, element 2i in the low nibble of byte i
+ *   scales  [ceil(rows / 128)][ceil(blocks / 4)][512] bytes, scale of row r and
+ *           block b at (r % 32) * 16 + (r / 32 % 4) * 4 + b % 4 of its atom
+ * Element types are enum scmp_dtype.  Asynchronous on `stream`. */
+enum scmp_mx_format { SCMP_MXFP4 = 0, SCMP_NVFP4 = 1 };
+enum scmp_dtype { SCMP_F32 = 0, SCMP_BF16 = 1, SCMP_F16 = 2 };
+SCMP_API size_t scmp_mx_data_size(int64_t rows, int64_t K, int fmt);
+SCMP_API size_t scmp_mx_scale_size(int64_t rows, int64_t K, int fmt);
+/* x: rows of K elements, `ld` elements apart (ld >= K). */
+SCMP_API int scmp_mx_quantize(const void *x, int dtype, int64_t rows, int64_t K, int64_t ld,
+                              int fmt, int scale_exp, void *data, void *scales, void *stream);
+/* out [rows][K]: the values that the codes stand for, rounded to `dtype`. */
+SCMP_API int scmp_mx_dequantize(const void *data, const void *scales, int64_t rows, int64_t K,
+                                int fmt, int scale_exp, void *out, int dtype, void *stream);
+/* out [M, N] = A B^T (+ bias [N]) for quantised A [M, K] and B [N, K] of one
+ * format: fp32 sums, rounded once to out_dtype.  scale_exp is the sum of the
+ * two operands' tensor exponents. */
+typedef struct scmp_mx_matmul_args {
+  int32_t abi_version; /* must be SCMP_ABI_VERSION */
+  int32_t fmt;         /* enum scmp_mx_format */
+  const void *a, *a_scales, *b, *b_scales;
+  int64_t M, N, K;
+  int32_t scale_exp;
+  int32_t bias_dtype;
+  const void *bias; /* nullable [N] */
+  void *out;
+  int32_t out_dtype;
+  int32_t reserved;
+} scmp_mx_matmul_args;
+SCMP_API int scmp_mx_matmul(const scmp_mx_matmul_args *args, void *stream);
+
+/* ---- Gated residual add with the norms around it (the `x + ls1(attn(...))`
+ * and `norm2(x)` steps of the block forward of cls/sc_attention_patch.py:459-636,
+ * with the gate and the norm behind the branch that other transformer blocks
+ * have).  Row-major [rows, C], C <= 8192:
+ *   z = y, or N(y) post_weight + post_bias
+ *   r = x + z gamma gate     rounded to dtype
+ *   h = N(r) weight + bias
+ * N(v) = (v - mean) / sqrt(var + eps), with rms != 0 v / sqrt(mean v^2 + eps).
+ * y NULL: h = N(x) weight + bias and r is not written.  bias, gamma, gate,
+ * post_weight, post_bias are nullable; gate [rows / rows_per_gate, C].
+ * Parameters are of x's type or fp32 (param_dtype).  h is of x's type, or fp32
+ * with h_f32.  mx_data and mx_scales (nullable) receive h's 4-bit codes in
+ * mx_fmt, straight from the fp32 values (scale_exp 0); that takes rows whose
+ * C * element size is a multiple of 16 bytes and 16-byte aligned pointers.
+ * stats (nullable) float [2][rows][2] receives mean and 1 / deviation of r
+ * and, with post_weight, of y, for the backward pass.  One launch. */
+typedef struct scmp_norm_args {
+  int32_t abi_version;
+  int32_t dtype, param_dtype;
+  int32_t rms;
+  const void *x, *y, *weight, *bias, *gamma, *gate, *post_weight, *post_bias;
+  void *r, *h;
+  float *stats;
+  void *mx_data, *mx_scales;
+  int64_t rows, C, rows_per_gate;
+  float eps;
+  int32_t h_f32, mx_fmt, reserved;
+} scmp_norm_args;
+SCMP_API int scmp_residual_norm(const scmp_norm_args *args, void *stream);
+/* Gradients of the above from dr and dh (each nullable: zero): dx, dy and the
+ * parameters' (each nullable: not wanted), with the stats of the forward pass
+ * and its r (x where y was NULL).  Deterministic.  The workspace holds partial column
+ * sums; scmp_residual_norm_bwd_workspace gives its size.  One to three
+ * launches. */
+typedef struct scmp_norm_bwd_args {
+  int32_t abi_version;
+  int32_t dtype, param_dtype;
+  int32_t rms;
+  const void *r, *y, *dr, *dh, *weight, *gamma, *gate, *post_weight, *post_bias;
+  const float *stats;
+  void *dx, *dy, *dweight, *dbias, *dgamma, *dgate, *dpost_weight, *dpost_bias;
+  void *workspace;
+  size_t workspace_bytes;
+  int64_t rows, C, rows_per_gate;
+} scmp_norm_bwd_args;
+SCMP_API size_t scmp_residual_norm_bwd_workspace(int64_t rows, int64_t C, int64_t rows_per_gate);
+SCMP_API int scmp_residual_norm_bwd(const scmp_norm_bwd_args *args, void *stream);
+
+/* ---- scmp_split_qkv with multi-axis rotary positions on q and k (EVA-type
+ * blocks turn q and k by (height, width) before the matmuls that
+ * det/sc_patch/sc_matmul.py:67-195 replaces).  qkv [B, N, H + 2 Hk, D] -> q [B, H, N, D],
+ * k [B, Hk, N, D] and v [B, Hk, N, D] or, v_transposed, [B, Hk, D, N].  Axis a
+ * turns dims[a] elements (even; one axis after the other from element 0, the
+ * rest of the head is copied) as dims[a] / 2 pairs, (2i, 2i + 1) interleaved or
+ * (i, i + dims[a] / 2); pair i of a token at coordinate c = pos[token][a] by
+ * table_a[c][i] = {cos, sin}.  table holds the axes' [sizes[a]][dims[a] / 2]
+ * pairs one after the other.  A negative coordinate leaves that axis's pairs
+ * as they are, one past the table gives NaN.  pos [N, axes], or [B, N, axes]
+ * with pos_batched.  inverse: the gradient, from q, k, v (their gradients) to
+ * qkv, turning back.  D even, <= 256.  One launch. */
+#define SCMP_MAX_AXES 4
+typedef struct scmp_rotary_args {
+  int32_t abi_version;
+  int32_t dtype;
+  void *qkv, *q, *k, *v;
+  const float *table;
+  const int32_t *pos;
+  int64_t B, N, H, Hk, D;
+  int32_t axes;
+  int32_t dims[SCMP_MAX_AXES], sizes[SCMP_MAX_AXES];
+  int32_t pos_batched, interleaved, v_transposed, inverse;
+  int32_t reserved[3];
+} scmp_rotary_args;
+SCMP_API int scmp_split_qkv_rotary(const scmp_rotary_args *args, void *stream);
+
 /* Message of the last failure on this thread ("" if none). */
 SCMP_API const char *scmp_last_error(void);
 

@@ -22,6 +22,10 @@ STATUS_NAMES = {
 GRANULARITY = {"per_row": 0, "per_head": 1, "per_tensor": 2}
 MODE = {"bipolar": 0, "unipolar": 1}
 ENGINE = {"auto": 0, "popc": 1, "tcgen05": 2}
+MX_FORMAT = {"mxfp4": 0, "nvfp4": 1}
+MX_BLOCK = {"mxfp4": 32, "nvfp4": 16}
+DTYPE = {"torch.float32": 0, "torch.bfloat16": 1, "torch.float16": 2}  # enum scmp_dtype
+MAX_AXES = 4  # SCMP_MAX_AXES
 IO_A_BF16, IO_B_BF16, IO_OUT_BF16, IO_B_PACKED, IO_A_QUANT = 1, 2, 4, 8, 16  # io_flags bits
 
 EXPORTED_SYMBOLS = (
@@ -42,6 +46,15 @@ EXPORTED_SYMBOLS = (
     "scmp_softmax_quantize",
     "scmp_bias_gelu",
     "scmp_scale_residual",
+    "scmp_mx_data_size",
+    "scmp_mx_scale_size",
+    "scmp_mx_quantize",
+    "scmp_mx_dequantize",
+    "scmp_mx_matmul",
+    "scmp_residual_norm",
+    "scmp_residual_norm_bwd_workspace",
+    "scmp_residual_norm_bwd",
+    "scmp_split_qkv_rotary",
 )
 
 
@@ -75,6 +88,58 @@ class MatmulArgs(ctypes.Structure):
         ("workspace", ctypes.c_void_p),
         ("workspace_bytes", ctypes.c_size_t),
     ]
+
+
+class MxMatmulArgs(ctypes.Structure):
+    """Mirror of ``scmp_mx_matmul_args``."""
+    _fields_ = [
+        ("abi_version", ctypes.c_int32),
+        ("fmt", ctypes.c_int32),
+        ("a", ctypes.c_void_p),
+        ("a_scales", ctypes.c_void_p),
+        ("b", ctypes.c_void_p),
+        ("b_scales", ctypes.c_void_p),
+        ("M", ctypes.c_int64),
+        ("N", ctypes.c_int64),
+        ("K", ctypes.c_int64),
+        ("scale_exp", ctypes.c_int32),
+        ("bias_dtype", ctypes.c_int32),
+        ("bias", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("out_dtype", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
+class NormArgs(ctypes.Structure):
+    """Mirror of ``scmp_norm_args``."""
+    _fields_ = [(n, ctypes.c_int32) for n in ("abi_version", "dtype", "param_dtype", "rms")] + [
+        (n, ctypes.c_void_p) for n in ("x", "y", "weight", "bias", "gamma", "gate", "post_weight",
+                                       "post_bias", "r", "h", "stats", "mx_data", "mx_scales")] + [
+        (n, ctypes.c_int64) for n in ("rows", "C", "rows_per_gate")] + [
+        ("eps", ctypes.c_float)] + [(n, ctypes.c_int32) for n in ("h_f32", "mx_fmt", "reserved")]
+
+
+class NormBwdArgs(ctypes.Structure):
+    """Mirror of ``scmp_norm_bwd_args``."""
+    _fields_ = [(n, ctypes.c_int32) for n in ("abi_version", "dtype", "param_dtype", "rms")] + [
+        (n, ctypes.c_void_p) for n in ("r", "y", "dr", "dh", "weight", "gamma", "gate",
+                                       "post_weight", "post_bias", "stats", "dx", "dy", "dweight",
+                                       "dbias", "dgamma", "dgate", "dpost_weight", "dpost_bias",
+                                       "workspace")] + [
+        ("workspace_bytes", ctypes.c_size_t)] + [
+        (n, ctypes.c_int64) for n in ("rows", "C", "rows_per_gate")]
+
+
+class RotaryArgs(ctypes.Structure):
+    """Mirror of ``scmp_rotary_args``."""
+    _fields_ = [("abi_version", ctypes.c_int32), ("dtype", ctypes.c_int32)] + [
+        (n, ctypes.c_void_p) for n in ("qkv", "q", "k", "v", "table", "pos")] + [
+        (n, ctypes.c_int64) for n in ("B", "N", "H", "Hk", "D")] + [
+        ("axes", ctypes.c_int32), ("dims", ctypes.c_int32 * MAX_AXES),
+        ("sizes", ctypes.c_int32 * MAX_AXES)] + [
+        (n, ctypes.c_int32) for n in ("pos_batched", "interleaved", "v_transposed", "inverse")] + [
+        ("reserved", ctypes.c_int32 * 3)]
 
 
 class EngineError(RuntimeError):
@@ -143,6 +208,21 @@ def load() -> ctypes.CDLL:
                                                                     ctypes.c_int64,
                                                                     ctypes.c_void_p]
         lib.scmp_scale_residual.restype = ctypes.c_int
+        i32, i64, ptr = ctypes.c_int, ctypes.c_int64, ctypes.c_void_p
+        for name in ("scmp_mx_data_size", "scmp_mx_scale_size"):
+            getattr(lib, name).argtypes = [i64, i64, i32]
+            getattr(lib, name).restype = ctypes.c_size_t
+        lib.scmp_mx_quantize.argtypes = [ptr, i32, i64, i64, i64, i32, i32, ptr, ptr, ptr]
+        lib.scmp_mx_quantize.restype = ctypes.c_int
+        lib.scmp_mx_dequantize.argtypes = [ptr, ptr, i64, i64, i32, i32, ptr, i32, ptr]
+        lib.scmp_mx_dequantize.restype = ctypes.c_int
+        for name, args in (("scmp_mx_matmul", MxMatmulArgs), ("scmp_residual_norm", NormArgs),
+                           ("scmp_residual_norm_bwd", NormBwdArgs),
+                           ("scmp_split_qkv_rotary", RotaryArgs)):
+            getattr(lib, name).argtypes = [ctypes.POINTER(args), ptr]
+            getattr(lib, name).restype = ctypes.c_int
+        lib.scmp_residual_norm_bwd_workspace.argtypes = [i64, i64, i64]
+        lib.scmp_residual_norm_bwd_workspace.restype = ctypes.c_size_t
         lib.scmp_debug_set_wait_limit.argtypes = [ctypes.c_uint64]
         lib.scmp_debug_set_wait_limit.restype = ctypes.c_int
         lib.scmp_debug_hold_producers.argtypes = [ctypes.c_int]

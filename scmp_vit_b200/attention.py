@@ -14,6 +14,8 @@ numerics per slice, but without their host loops:
 """
 from __future__ import annotations
 
+import ctypes
+import math
 from typing import Callable, Optional
 
 import torch
@@ -368,6 +370,136 @@ def split_qkv(qkv: torch.Tensor, num_heads: int):
     _lib.check(_lib.load().scmp_split_qkv(src.data_ptr(), B, N, H, D, src.element_size(),
                                           q.data_ptr(), k.data_ptr(), vt.data_ptr(), stream))
     return q, k, vt.transpose(-1, -2)
+
+
+class RotaryAxes(nn.Module):
+    """Rotary positions along several axes (e.g. height and width, or time,
+    height and width): axis ``a`` turns ``dims[a]`` elements of every head
+    (even; one axis after the other from element 0, the rest stays), pair ``i``
+    of a token at coordinate ``c`` by the angle
+    ``c * scales[a] * base ** (-2 i / dims[a])``.
+
+    Holds cos and sin of every coordinate below ``sizes[a]``, computed in 64
+    bits and kept in fp32 (the bits are stored as integers, so that a cast of
+    the model leaves them alone); moves with ``.to(device)``.  Pairs are
+    ``(2i, 2i + 1)`` when ``interleaved``, else ``(i, i + dims[a] / 2)`` inside
+    the axis's section."""
+
+    def __init__(self, dims, sizes, *, base: float = 10000.0, scales=None,
+                 interleaved: bool = True, device=None):
+        super().__init__()
+        from . import _lib
+        dims, sizes = [int(d) for d in dims], [int(n) for n in sizes]
+        scales = [1.0] * len(dims) if scales is None else [float(f) for f in scales]
+        if not 1 <= len(dims) <= _lib.MAX_AXES or len(sizes) != len(dims) or len(
+                scales) != len(dims):
+            raise ValueError(f"one to {_lib.MAX_AXES} axes with a size and a scale each, got "
+                             f"dims {dims}, sizes {sizes}, scales {scales}")
+        if any(d < 2 or d % 2 for d in dims) or any(n < 1 for n in sizes):
+            raise ValueError(f"dims must be even and positive, sizes positive: {dims}, {sizes}")
+        if not base > 0:
+            raise ValueError(f"base must be positive, got {base}")
+        self.dims, self.sizes, self.interleaved = dims, sizes, bool(interleaved)
+        parts = []
+        for d, n, f in zip(dims, sizes, scales):
+            freq = torch.exp(torch.arange(0, d, 2, dtype=torch.float64, device=device)
+                             * (-math.log(base) / d))
+            angle = torch.arange(n, dtype=torch.float64, device=device)[:, None] * f * freq
+            parts.append(torch.stack([angle.cos(), angle.sin()], -1).float().reshape(-1))
+        self.register_buffer("table_bits", torch.cat(parts).view(torch.int32), persistent=False)
+
+    def extra_repr(self) -> str:
+        return f"dims={self.dims}, sizes={self.sizes}, interleaved={self.interleaved}"
+
+
+def _rotary_launch(qkv, q, k, v, axes: RotaryAxes, table, pos, v_transposed: bool, inverse: bool):
+    """One ``scmp_split_qkv_rotary`` call on contiguous storages."""
+    from . import _lib
+    B, H, N, D = q.shape
+    a = _lib.RotaryArgs()
+    a.abi_version = _lib.ABI_VERSION
+    a.dtype = _lib.DTYPE[str(qkv.dtype)]
+    a.qkv, a.q, a.k, a.v = (t.data_ptr() for t in (qkv, q, k, v))
+    a.table, a.pos = table.data_ptr(), pos.data_ptr()
+    a.B, a.N, a.H, a.Hk, a.D = B, N, H, k.shape[1], D
+    a.axes = len(axes.dims)
+    for i, (d, n) in enumerate(zip(axes.dims, axes.sizes)):
+        a.dims[i], a.sizes[i] = d, n
+    a.pos_batched = int(pos.dim() == 3)
+    a.interleaved, a.v_transposed, a.inverse = axes.interleaved, v_transposed, inverse
+    with torch.cuda.device(qkv.device):
+        stream = torch.cuda.current_stream(qkv.device).cuda_stream
+        _lib.check(_lib.load().scmp_split_qkv_rotary(ctypes.byref(a), ctypes.c_void_p(stream)))
+
+
+class _SplitQkvRotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, qkv, pos, table, axes, H, Hk, transpose_v):
+        B, N, width = qkv.shape
+        D = width // (H + 2 * Hk)
+        src = qkv.contiguous()
+        q = qkv.new_empty(B, H, N, D)
+        k = qkv.new_empty(B, Hk, N, D)
+        v = qkv.new_empty(B, Hk, D, N) if transpose_v else qkv.new_empty(B, Hk, N, D)
+        _rotary_launch(src, q, k, v, axes, table, pos, transpose_v, False)
+        ctx.axes, ctx.shape = axes, (B, N, width)
+        # the table itself: axes that move to another device in between leave
+        # this call's gradient alone
+        ctx.save_for_backward(pos, table)
+        return q, k, v.transpose(-1, -2) if transpose_v else v
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dq, dk, dv):
+        pos, table = ctx.saved_tensors
+        # v's gradient in whichever of its two layouts it comes
+        transposed = not dv.is_contiguous() and dv.transpose(-1, -2).is_contiguous()
+        dv = dv if transposed else dv.contiguous()
+        dq, dk = dq.contiguous(), dk.contiguous()
+        grad = dq.new_empty(ctx.shape)
+        _rotary_launch(grad, dq, dk, dv, ctx.axes, table, pos, transposed, True)
+        return grad, None, None, None, None, None, None
+
+
+def split_qkv_rotary(qkv: torch.Tensor, num_heads: int, axes: RotaryAxes, pos: torch.Tensor, *,
+                     num_kv_heads: Optional[int] = None, transpose_v: bool = True):
+    """``split_qkv`` with q and k turned by their tokens' positions, in one
+    engine pass: ``qkv`` [B, N, (H + 2 Hk) D] -> q [B, H, N, D], k and v
+    [B, Hk, N, D] (``num_kv_heads`` Hk: shared k/v heads; default H).
+
+    ``pos`` int32 [N, axes] or [B, N, axes]: the tokens' coordinates.  A
+    negative one leaves the token as it is along that axis (class and register
+    tokens); one at or past ``axes.sizes`` gives NaN.  ``transpose_v`` returns
+    v as the transposed view of a contiguous [B, Hk, D, N], the layout that the
+    Attn@V engine call reads, else contiguous.  fp32, bf16 or fp16; rotated in
+    fp32 and rounded once, everything else copied bit for bit.
+    Differentiable (once) in ``qkv``."""
+    H = int(num_heads)
+    Hk = H if num_kv_heads is None else int(num_kv_heads)
+    if not qkv.is_cuda:
+        raise RuntimeError("split_qkv_rotary runs on the CUDA engine only (no CPU path); "
+                           f"got {qkv.device}")
+    if qkv.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        raise TypeError(f"qkv must be float32, bfloat16 or float16, got {qkv.dtype}")
+    if H < 1 or Hk < 1 or H % Hk:
+        raise ValueError(f"num_heads={H} must be a positive multiple of num_kv_heads={Hk}")
+    if qkv.dim() != 3 or qkv.shape[-1] % (H + 2 * Hk):
+        raise ValueError(f"qkv must be [B, N, (H + 2 Hk) D], got {tuple(qkv.shape)} for H={H}, "
+                         f"Hk={Hk}")
+    B, N, width = qkv.shape
+    D = width // (H + 2 * Hk)
+    if D < 2 or D % 2 or D > 256 or sum(axes.dims) > D:
+        raise ValueError(f"the head size must be even, at most 256 and hold the axes' dims "
+                         f"{axes.dims}, got {D}")
+    n_axes = len(axes.dims)
+    if (pos.dtype != torch.int32 or pos.device != qkv.device
+            or tuple(pos.shape) not in ((N, n_axes), (B, N, n_axes))):
+        raise ValueError(f"pos must be int32 [{N}, {n_axes}] or [{B}, {N}, {n_axes}] on "
+                         f"{qkv.device}, got {pos.dtype} {tuple(pos.shape)} {pos.device}")
+    if axes.table_bits.device != qkv.device:
+        raise ValueError(f"axes are on {axes.table_bits.device}, qkv on {qkv.device}")
+    return _SplitQkvRotary.apply(qkv, pos.contiguous(), axes.table_bits, axes, H, Hk,
+                                 bool(transpose_v))
 
 
 def make_sc_attention_forward(sc_prec: int, sc_av: bool, sc_qk: bool = True,

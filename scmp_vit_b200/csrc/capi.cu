@@ -371,6 +371,8 @@ QuantPlane plane_of(const OperandLayout &o, unsigned char *ws) {
 }  // namespace
 
 void set_last_error(const char *msg) { g_last_error = msg ? msg : ""; }
+void add_launches(uint64_t n) { count_launches(n); }
+unsigned int *device_error_word() { return engine_error_ptr(); }
 
 void *current_context() {
   using GetCurrent = int (*)(void **);

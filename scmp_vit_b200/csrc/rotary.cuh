@@ -1,0 +1,24 @@
+// Arguments of the rotary qkv split (rotary.cu).
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "../../include/scmp_b200.h"
+
+namespace scmp {
+
+struct RotaryParams {
+  void *qkv;         // [B, N, H + 2 Hk, D]
+  void *q, *k, *v;   // [B, H, N, D], [B, Hk, N, D], and v the same or [B, Hk, D, N]
+  const float2 *table;
+  const int32_t *pos;  // [N, axes] or [B, N, axes]
+  int64_t B, N, H, Hk;
+  int D, axes, pairs;  // pairs: rotated pairs of a head
+  int dims[SCMP_MAX_AXES], sizes[SCMP_MAX_AXES], first_pair[SCMP_MAX_AXES];
+  int64_t table_at[SCMP_MAX_AXES];  // first entry of each axis
+  bool pos_batched, interleaved, v_transposed, inverse;
+};
+cudaError_t launch_rotary(const RotaryParams &p, int dtype, cudaStream_t s);
+
+}  // namespace scmp

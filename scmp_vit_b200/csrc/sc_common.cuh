@@ -192,6 +192,10 @@ int tc_ksplit(const GemmProblem &P, int64_t m_rows, int64_t n_rows);
 
 // Message of the last failure on this thread (capi.cu).
 void set_last_error(const char *msg);
+// Launch counter and sticky device error word (NULL if it cannot be resolved)
+// of the whole library (capi.cu).
+void add_launches(uint64_t n);
+unsigned int *device_error_word();
 
 // Driver context current on this thread (NULL if none or unknown).  A device
 // symbol's address belongs to the context that loaded the module, so the

@@ -1,0 +1,401 @@
+"""Microscaled 4-bit floating point: quantisation byte for byte against a
+search over the representable values in 64 bits, the product against the
+64-bit product of the dequantised operands, and the refusals."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+from scmp_vit_b200 import _lib, mx
+
+E2M1 = np.array([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0])
+E4M3 = np.array([i * 2.0 ** -9 for i in range(8)]
+                + [(1 + m / 8) * 2.0 ** e for e in range(-6, 9) for m in range(8)])[:127]
+FMTS = ("mxfp4", "nvfp4")
+DTYPES = (torch.float32, torch.bfloat16, torch.float16)
+
+
+def nearest(v, grid):
+    """Index of the nearest grid entry (ascending), the even one between two."""
+    hi = np.searchsorted((grid[1:] + grid[:-1]) / 2, v, side="right")
+    lo = np.searchsorted((grid[1:] + grid[:-1]) / 2, v, side="left")
+    return np.where((lo != hi) & (lo % 2 == 1), hi, lo)
+
+
+def quantize_ref(x, fmt, scale_exp=0):
+    """(element codes [rows, kp], scale codes [rows, kp / block], values [rows, K])."""
+    x = np.asarray(x, dtype=np.float64)
+    rows, K = x.shape
+    block = _lib.MX_BLOCK[fmt]
+    kp = -(-K // 32) * 32
+    v = np.zeros((rows, kp))
+    v[:, :K] = x
+    v = v.reshape(rows, -1, block)
+    with np.errstate(invalid="ignore"):
+        bad = ~np.isfinite(v).all(-1)
+        v = np.where(bad[..., None], 0.0, v)
+        amax = np.abs(v).max(-1)
+    if fmt == "mxfp4":
+        _, e = np.frexp(amax)  # amax = m 2^e, m in [1/2, 1)
+        e = np.maximum(np.where(amax > 0, e - 3, -127), -127)
+        scale, step = e + 127, 2.0 ** e.astype(np.float64)
+    else:
+        scale = nearest(np.minimum(amax / 2.0 ** scale_exp / 6, 448.0), E4M3)
+        step = E4M3[scale] * 2.0 ** scale_exp
+    mag = np.where(step[..., None] > 0, np.abs(v) / np.where(step > 0, step, 1)[..., None], 0)
+    code = nearest(mag, E2M1)
+    value = E2M1[code] * step[..., None] * np.where(np.signbit(v), -1, 1)
+    value[bad] = np.nan
+    code = code + 8 * np.signbit(v)
+    code[bad] = 0
+    scale = np.where(bad, 0xFF if fmt == "mxfp4" else 0x7F, scale)
+    return code.reshape(rows, kp), scale, value.reshape(rows, kp)[:, :K]
+
+
+def pack_ref(code, scale):
+    """The bytes of the documented layout."""
+    rows, nb = scale.shape
+    data = (code[:, 0::2] | code[:, 1::2] << 4).astype(np.uint8)
+    groups = -(-nb // 4)
+    out = np.zeros((-(-rows // 128), groups, 512), dtype=np.uint8)
+    r, b = np.meshgrid(np.arange(rows), np.arange(nb), indexing="ij")
+    out[r // 128, b // 4, r % 32 * 16 + r // 32 % 4 * 4 + b % 4] = scale
+    return data.reshape(-1), out.reshape(-1)
+
+
+# ------------------------------------------------------------ CPU: refusals
+
+def test_sizes():
+    lib = _lib.load()
+    for fmt, code in _lib.MX_FORMAT.items():
+        for rows, K in ((0, 5), (1, 1), (128, 32), (129, 33), (257, 1024)):
+            kp = -(-K // 32) * 32
+            assert lib.scmp_mx_data_size(rows, K, code) == rows * kp // 2
+            groups = -(-kp // (4 * _lib.MX_BLOCK[fmt]))
+            assert lib.scmp_mx_scale_size(rows, K, code) == -(-rows // 128) * groups * 512
+    for rows, K, code in ((-1, 4, 0), (4, 0, 0), (4, 4, 2), (1 << 31, 4, 0), (4, 1 << 31, 1)):
+        assert lib.scmp_mx_data_size(rows, K, code) == 0
+        assert lib.scmp_mx_scale_size(rows, K, code) == 0
+
+
+def test_struct_layouts_match_the_header():
+    assert ctypes.sizeof(_lib.MxMatmulArgs) == 8 + 32 + 24 + 8 + 16 + 8
+    assert ctypes.sizeof(_lib.NormArgs) == 16 + 13 * 8 + 24 + 16
+    assert ctypes.sizeof(_lib.NormBwdArgs) == 16 + 19 * 8 + 8 + 24
+    assert ctypes.sizeof(_lib.RotaryArgs) == 8 + 48 + 40 + 4 + 32 + 16 + 12
+
+
+@pytest.mark.parametrize("args,msg", [
+    (dict(fmt=7), "format"),
+    (dict(rows=-1), "shape"),
+    (dict(K=0), "shape"),
+    (dict(dtype=3), "dtype"),
+    (dict(ld=7), "ld"),
+    (dict(fmt=0, scale_exp=1), "scale_exp"),
+    (dict(fmt=1, scale_exp=121), "scale_exp"),
+    (dict(x=0), "non-NULL"),
+    (dict(data=0), "non-NULL"),
+    (dict(data=24), "aligned"),
+    (dict(scales=8), "aligned"),
+])
+def test_quantize_refusals(args, msg):
+    a = dict(x=16, dtype=0, rows=4, K=8, ld=8, fmt=0, scale_exp=0, data=16, scales=16)
+    a.update(args)
+    lib = _lib.load()
+    assert lib.scmp_mx_quantize(a["x"], a["dtype"], a["rows"], a["K"], a["ld"], a["fmt"],
+                                a["scale_exp"], a["data"], a["scales"], None) == -1
+    assert msg in _lib.last_error()
+
+
+@pytest.mark.parametrize("args,msg", [
+    (dict(abi_version=9), "abi_version"),
+    (dict(fmt=2), "format"),
+    (dict(M=-1), "shape"),
+    (dict(K=0), "shape"),
+    (dict(scale_exp=3), "scale_exp"),
+    (dict(out_dtype=5), "dtype"),
+    (dict(bias=16, bias_dtype=4), "dtype"),
+    (dict(a=None), "non-NULL"),
+    (dict(out=None), "non-NULL"),
+    (dict(b_scales=8), "aligned"),
+])
+def test_matmul_refusals(args, msg):
+    a = _lib.MxMatmulArgs()
+    a.abi_version, a.M, a.N, a.K = _lib.ABI_VERSION, 4, 4, 32
+    a.a = a.a_scales = a.b = a.b_scales = a.out = 16
+    for k, v in args.items():
+        setattr(a, k, v)
+    assert _lib.load().scmp_mx_matmul(ctypes.byref(a), None) == -1
+    assert msg in _lib.last_error()
+
+
+def test_python_refusals_on_cpu():
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        mx.mx_quantize(torch.zeros(4, 32))
+    with pytest.raises(ValueError, match="format"):
+        mx.mx_quantize(torch.zeros(4, 32), "fp4")
+    with pytest.raises(TypeError, match="float32"):
+        mx.mx_quantize(torch.zeros(4, 32, dtype=torch.int32))
+    with pytest.raises(TypeError, match="MXTensor"):
+        mx.mx_matmul(torch.zeros(4, 32), torch.zeros(4, 32))
+    with pytest.raises(ValueError, match="contiguous bytes"):
+        mx.MXTensor(torch.zeros(3, dtype=torch.uint8), torch.zeros(512, dtype=torch.uint8),
+                    (4, 32), "mxfp4")
+
+
+# ------------------------------------------------------------ GPU: quantise
+
+def special_rows(K):
+    """Rows that borders, ends of ranges and odd values decide."""
+    g = torch.Generator().manual_seed(K)
+    rows = [torch.zeros(K), torch.full((K,), -0.0), torch.full((K,), 1e-45),
+            torch.full((K,), 3.0e38), torch.randn(K, generator=g) * 1e-40,
+            torch.randn(K, generator=g) * 2.0 ** -125, torch.randn(K, generator=g) * 1e37]
+    ties = torch.tensor([6.0, 0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, -0.25, -0.75, -1.25, -1.75,
+                         -2.5, -3.5, -5.0, 0.5])
+    for s in (1.0, 1.125, 0.8125, 2.0 ** -9, 448.0, 7.0):  # e4m3 steps; 7 makes mxfp4 saturate
+        rows.append((ties.repeat(K // 16 + 1) * s)[:K])
+    for bad in (float("inf"), float("-inf"), float("nan")):
+        r = torch.randn(K, generator=g)
+        r[K // 2] = bad
+        rows.append(r)
+    return torch.stack(rows)
+
+
+def check_quantize(x, fmt, scale_exp=0):
+    q = mx.mx_quantize(x, fmt, scale_exp=scale_exp)
+    values = q.dequantize(torch.float32)
+    torch.cuda.synchronize()
+    x2 = x.detach().cpu().reshape(-1, x.shape[-1])
+    code, scale, value = quantize_ref(x2.double().numpy(), fmt, scale_exp)
+    data, scales = pack_ref(code, scale)
+    assert np.array_equal(q.data.cpu().numpy(), data)
+    assert np.array_equal(q.scales.cpu().numpy(), scales)
+    got = values.cpu().double().numpy().reshape(value.shape)
+    assert np.array_equal(got, value, equal_nan=True)
+    return q
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("rows,K", [(1, 1), (1, 32), (2, 31), (3, 33), (130, 64), (5, 257),
+                                    (129, 100), (257, 1024), (4, 4104), (33, 520)])
+def test_quantize_bytes(cuda_device, fmt, rows, K):
+    g = torch.Generator().manual_seed(rows * 1000 + K)
+    for dtype in DTYPES:
+        x = torch.randn(rows, K, generator=g) * torch.exp(3 * torch.randn(rows, 1, generator=g))
+        check_quantize(x.to(dtype).to(cuda_device), fmt)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt,scale_exp", [("mxfp4", 0), ("nvfp4", 0), ("nvfp4", -11),
+                                           ("nvfp4", 5), ("nvfp4", 120), ("nvfp4", -120)])
+@pytest.mark.parametrize("K", [16, 47, 256])
+def test_quantize_special_values(cuda_device, fmt, scale_exp, K):
+    x = special_rows(K).to(cuda_device)
+    check_quantize(x, fmt, scale_exp)
+    check_quantize(x.to(torch.bfloat16), fmt, scale_exp)
+    check_quantize(x.to(torch.float16), fmt, scale_exp)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FMTS)
+def test_quantize_strides_and_shapes(cuda_device, fmt):
+    x = torch.randn(6, 40, 96, generator=torch.Generator().manual_seed(1)).to(cuda_device)
+    check_quantize(x, fmt)
+    check_quantize(x[:, ::3, 1:65], fmt)               # strided rows at an odd offset
+    check_quantize(x[:, :, ::2], fmt)                  # strided elements
+    check_quantize(x.transpose(0, 2), fmt)
+    check_quantize(x[0, :1].expand(5, 96), fmt)        # one row five times
+    check_quantize(x[2, 3], fmt)                       # one dimension
+    empty = mx.mx_quantize(x[:0], fmt)
+    assert empty.shape == (0, 40, 96) and empty.dequantize().shape == (0, 40, 96)
+    r = mx.mx_quantize(x, fmt).reshape(-1, 96)
+    assert r.shape == (240, 96)
+    assert torch.equal(r.dequantize(), mx.mx_quantize(x, fmt).dequantize().reshape(240, 96))
+    with pytest.raises(ValueError, match="last dimension"):
+        r.reshape(96, 240)
+
+
+@pytest.mark.gpu
+def test_values_fit_the_types_they_came_from(cuda_device):
+    """Two significant bits (mxfp4) or six (nvfp4): exact in 16-bit types."""
+    for fmt in FMTS:
+        for dtype in DTYPES:
+            x = torch.randn(64, 96, generator=torch.Generator().manual_seed(2)).to(dtype)
+            q = mx.mx_quantize(x.to(cuda_device), fmt)
+            assert torch.equal(q.dequantize().float(), q.dequantize(torch.float32))
+
+
+# ------------------------------------------------------------- GPU: product
+
+def product_bound(a, b, y, out_dtype):
+    """|error| allowed for fp32 sums of exact products in any order, each
+    addition off by at most one unit in the last place (2^-23 of the running
+    magnitude, itself at most sum |a||b|), plus the final rounding."""
+    K = a.shape[-1]
+    return (K + 2) * 2.0 ** -23 * (a.abs() @ b.abs().t() + y.abs()) + \
+        torch.finfo(out_dtype).eps / 2 * y.abs()
+
+
+def check_product(a, w, fmt, dtype, bias=None, w_exp=0):
+    qa = mx.mx_quantize(a, fmt)
+    qw = mx.mx_quantize(w, fmt, scale_exp=w_exp)
+    y = mx.mx_matmul(a, qw, bias=bias, out_dtype=dtype)
+    y2 = mx.mx_matmul(qa, qw, bias=bias, out_dtype=dtype)
+    torch.cuda.synchronize()
+    assert _lib.engine_status() == 0
+    va = qa.dequantize(torch.float32).double().reshape(-1, a.shape[-1])
+    vw = qw.dequantize(torch.float32).double()
+    ref = va @ vw.t()
+    if bias is not None:
+        ref = ref + bias.double()
+    bound = product_bound(va, vw, ref, dtype)
+    if dtype == torch.float16:
+        ref = ref.clamp(-65504, 65504)
+    for got in (y, y2):
+        assert got.dtype == dtype and got.shape == (*a.shape[:-1], w.shape[0])
+        err = (got.double().reshape(ref.shape) - ref).abs()
+        assert bool((err <= bound).all()), (err / bound).max()
+    return y
+
+
+SHAPES = [(1, 1, 1), (1, 48, 32), (3, 5, 7), (2, 130, 96), (7, 64, 4104), (17, 200, 64),
+          (33, 257, 100), (127, 128, 128), (129, 257, 260), (257, 1024, 1024), (200, 511, 352),
+          (193, 264, 544), (385, 520, 2080), (64, 4096, 1024), (600, 96, 40), (1500, 300, 288)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("M,N,K", SHAPES)
+def test_matmul(cuda_device, fmt, M, N, K):
+    g = torch.Generator().manual_seed(M + N + K)
+    a = (torch.randn(M, K, generator=g) * torch.exp(torch.randn(M, 1, generator=g)))
+    w = torch.randn(N, K, generator=g) * 0.05
+    bias = torch.randn(N, generator=g)
+    exp = -12 if fmt == "nvfp4" else 0
+    for dtype in DTYPES:
+        check_product(a.to(dtype).to(cuda_device), w.to(cuda_device), fmt, dtype,
+                      bias.to(dtype).to(cuda_device), exp)
+    check_product(a.to(cuda_device), w.to(cuda_device), fmt, torch.float32, None, exp)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("M,N,K", [(1, 96, 96), (5, 40, 200), (300, 256, 160)])
+def test_matmul_not_finite(cuda_device, fmt, M, N, K):
+    """A block that is not finite makes its own row (column) NaN and leaves
+    every other output as it is."""
+    g = torch.Generator().manual_seed(9)
+    a, w = torch.randn(M, K, generator=g), torch.randn(N, K, generator=g)
+    clean = mx.mx_matmul(a.to(cuda_device), mx.mx_quantize(w.to(cuda_device), fmt))
+    a[M // 2, K - 1] = float("inf")
+    w[3, 0] = float("nan")
+    got = mx.mx_matmul(a.to(cuda_device), mx.mx_quantize(w.to(cuda_device), fmt))
+    assert bool(got[M // 2].isnan().all()) and bool(got[:, 3].isnan().all())
+    keep_m = torch.arange(M) != M // 2
+    keep_n = torch.arange(N) != 3
+    assert torch.equal(got[keep_m][:, keep_n], clean[keep_m][:, keep_n])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [1, 4, 40, 300])
+def test_matmul_wide_scales(cuda_device, M):
+    """Blocks of one row many powers of two apart: the largest decides."""
+    g = torch.Generator().manual_seed(5)
+    a, w = torch.randn(M, 256, generator=g), torch.randn(80, 256, generator=g)
+    a[:, :32] *= 2.0 ** 40
+    w[:, 32:64] *= 2.0 ** -60
+    check_product(a.to(cuda_device), w.to(cuda_device), "mxfp4", torch.float32)
+
+
+@pytest.mark.gpu
+def test_matmul_empty_and_out(cuda_device):
+    w = mx.mx_quantize(torch.randn(24, 64, device=cuda_device))
+    x = torch.randn(3, 5, 64, device=cuda_device)
+    assert mx.mx_matmul(x[:0], w).shape == (0, 5, 24)
+    none = mx.mx_quantize(torch.zeros(0, 64, device=cuda_device))
+    assert mx.mx_matmul(x, none).shape == (3, 5, 0)
+    # an output one element off 16-byte alignment, with guards on both sides
+    buf = torch.full((3 * 5 * 24 + 2,), 7.0, dtype=torch.bfloat16, device=cuda_device)
+    out = buf[1:-1].view(3, 5, 24)
+    assert mx.mx_matmul(x, w, out=out) is out
+    ref = mx.mx_matmul(x, w, out_dtype=torch.bfloat16)
+    assert torch.equal(out, ref) and buf[0] == 7 and buf[-1] == 7
+
+
+@pytest.mark.gpu
+def test_matmul_repeats_bit_for_bit(cuda_device):
+    """A call made again gives the same bits."""
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn(700, 512, generator=g).to(cuda_device)
+    w = mx.mx_quantize(torch.randn(384, 512, generator=g).to(cuda_device))
+    full = mx.mx_matmul(x, w)
+    assert torch.equal(full, mx.mx_matmul(x, w))
+
+
+@pytest.mark.gpu
+def test_python_refusals(cuda_device):
+    w = mx.mx_quantize(torch.randn(24, 64, device=cuda_device))
+    x = torch.randn(4, 64, device=cuda_device)
+    with pytest.raises(ValueError, match="inner-dim"):
+        mx.mx_matmul(x[:, :32], w)
+    with pytest.raises(ValueError, match="formats"):
+        mx.mx_matmul(mx.mx_quantize(x, "nvfp4"), w)
+    with pytest.raises(ValueError, match="bias"):
+        mx.mx_matmul(x, w, bias=torch.zeros(23, device=cuda_device))
+    with pytest.raises(TypeError, match="bias"):
+        mx.mx_matmul(x, w, bias=torch.zeros(24, device=cuda_device, dtype=torch.float64))
+    with pytest.raises(TypeError, match="out"):
+        mx.mx_matmul(x, w, out_dtype=torch.float64)
+    with pytest.raises(ValueError, match="out must"):
+        mx.mx_matmul(x, w, out=torch.empty(4, 23, device=cuda_device))
+    with pytest.raises(ValueError, match="devices"):
+        mx.mx_matmul(x.cpu(), w)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        mx.mx_matmul(x.clone().requires_grad_(), w)
+    with torch.no_grad():
+        mx.mx_matmul(x.clone().requires_grad_(), w)
+    with pytest.raises(_lib.EngineError, match="scale_exp"):
+        mx.mx_quantize(x, "mxfp4", scale_exp=2)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FMTS)
+def test_linear(cuda_device, fmt):
+    lin = torch.nn.Linear(96, 72).to(cuda_device)
+    m = mx.MXLinear(lin, fmt)
+    x = torch.randn(2, 11, 96, device=cuda_device)
+    ref = mx.mx_matmul(x, mx.mx_quantize(lin.weight.detach(), fmt, scale_exp=m.scale_exp),
+                       bias=lin.bias.detach())
+    assert torch.equal(m(x), ref)
+    assert torch.equal(m(mx.mx_quantize(x, fmt)), ref)
+    again = mx.MXLinear(torch.nn.Linear(96, 72).to(cuda_device), fmt)
+    again.load_state_dict(m.state_dict())
+    again.scale_exp = m.scale_exp
+    assert torch.equal(again(x), ref)
+
+
+@pytest.mark.gpu
+def test_streams_and_graph(cuda_device):
+    """A call on a side stream, and one captured and replayed on new inputs."""
+    g = torch.Generator().manual_seed(4)
+    w = mx.mx_quantize(torch.randn(160, 128, generator=g).to(cuda_device))
+    xs = [torch.randn(m, 128, generator=g).to(cuda_device) for m in (1, 300)]
+    for x in xs:
+        ref = mx.mx_matmul(x, w)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            got = mx.mx_matmul(x, w)
+        side.synchronize()
+        assert torch.equal(got, ref)
+        static = x.clone()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = mx.mx_matmul(static, w)
+        static.copy_(x * 2 + 1)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, mx.mx_matmul(x * 2 + 1, w))
