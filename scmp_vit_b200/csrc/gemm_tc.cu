@@ -31,6 +31,7 @@
 #include <vector>
 
 #include "sc_common.cuh"
+#include "tc_ptx.cuh"
 
 namespace scmp {
 namespace {
@@ -41,16 +42,6 @@ constexpr int kStages = 3;
 constexpr int kProducerWarps = 16;
 constexpr int kProducers = 32 * kProducerWarps;
 constexpr int kThreads = 32 + kProducers;
-constexpr unsigned long long kTimeoutNs = 2000000000ull;  // default limit: 2 s per wait
-
-// Limit of every bounded pipeline wait on this device (ns; kTimeoutNs unless
-// scmp_debug_set_wait_limit changed it).  Read on the slow path only.
-__device__ unsigned long long g_wait_limit_ns = kTimeoutNs;
-// Test hook for the give-up path (scmp_debug_hold_producers): while set, the
-// operand producers of the e2m1 kernels first wait on g_hold_release, which
-// nothing ever sets, so the pipeline waits of their CTA run out.
-__device__ int g_hold_producers = 0;
-__device__ int g_hold_release = 0;
 
 template <int BN>
 struct TcCfg {
@@ -120,89 +111,8 @@ __device__ __forceinline__ TileCoord tile_coord(const TcParams &prm, int64_t til
   return t;
 }
 
-// ------------------------------------------------------------ PTX helpers
+// ------------------------------------------------------------ MMA (kind::i8)
 
-__device__ __forceinline__ uint32_t smem_u32(const void *p) {
-  return (uint32_t)__cvta_generic_to_shared(p);
-}
-__device__ __forceinline__ unsigned long long now_ns() {
-  unsigned long long t;
-  asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
-  return t;
-}
-__device__ __forceinline__ void mbar_init(uint64_t *bar, uint32_t count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count));
-}
-__device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
-  asm volatile("mbarrier.arrive.release.cta.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar))
-               : "memory");
-}
-__device__ __forceinline__ bool mbar_try_wait(uint64_t *bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n.reg .pred p;\n"
-      "mbarrier.try_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2;\n"
-      "selp.u32 %0, 1, 0, p;\n}\n"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-// Bounded wait: false when it gave up (timeout or another thread aborted).
-// The limit is re-read on every slow iteration rather than held in registers
-// across the loop (waits sit where the producers hold the most live state).
-__device__ __forceinline__ unsigned long long wait_limit() {
-  return *reinterpret_cast<volatile unsigned long long *>(&g_wait_limit_ns);
-}
-__device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity, volatile int *abort) {
-  if (mbar_try_wait(bar, parity)) return true;
-  const unsigned long long t0 = now_ns();
-  while (true) {
-    if (mbar_try_wait(bar, parity)) return true;
-    if (*abort) return false;
-    if (now_ns() - t0 > wait_limit()) {
-      *abort = 1;
-      return false;
-    }
-  }
-}
-// Wait for this thread's own tensor-core work to complete before its TMEM is
-// freed: ignores the abort word (MMAs already issued always complete) and
-// gives up only after kTimeoutNs.
-__device__ __forceinline__ void mbar_wait_own(uint64_t *bar, uint32_t parity) {
-  if (mbar_try_wait(bar, parity)) return;
-  const unsigned long long t0 = now_ns();
-  while (!mbar_try_wait(bar, parity) && now_ns() - t0 <= kTimeoutNs) {
-  }
-}
-// Test hook: with g_hold_producers set, wait on a flag that nothing sets until
-// the wait limit runs out (or the CTA aborts); false = give up.
-__device__ __forceinline__ bool producers_released(volatile int *abort) {
-  if (!*reinterpret_cast<volatile int *>(&g_hold_producers)) return true;
-  const unsigned long long t0 = now_ns();
-  while (!*reinterpret_cast<volatile int *>(&g_hold_release)) {
-    if (*abort) return false;
-    if (now_ns() - t0 > wait_limit()) {
-      *abort = 1;
-      return false;
-    }
-  }
-  return true;
-}
-__device__ __forceinline__ void fence_async_smem() {
-  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-}
-__device__ __forceinline__ void tc_fence_before() {
-  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-}
-__device__ __forceinline__ void tc_fence_after() {
-  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-}
-__device__ __forceinline__ void tc_commit(uint64_t *bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-                   smem_u32(bar))
-               : "memory");
-}
 __device__ __forceinline__ void tc_mma_i8(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc,
                                           uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -210,61 +120,6 @@ __device__ __forceinline__ void tc_mma_i8(uint32_t tmem_d, uint64_t adesc, uint6
       "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n}\n" ::"r"(tmem_d),
       "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
       : "memory");
-}
-// ---- CTA pairs (cta_group::2): the even CTA of a 2-CTA cluster issues the
-// MMAs for both; every other wait on a peer is an mbarrier with a bound.
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-// shared::cluster address of `addr` (a shared::cta address) in CTA `rank`
-__device__ __forceinline__ uint32_t mapa_shared(uint32_t addr, uint32_t rank) {
-  uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-  return r;
-}
-// Cluster-scope release: issued only by threads with no global loads in
-// flight (a release waits for them), never by the producers per k-block.
-__device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr)
-               : "memory");
-}
-__device__ __forceinline__ bool mbar_try_wait_cl(uint64_t *bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n.reg .pred p;\n"
-      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
-      "selp.u32 %0, 1, 0, p;\n}\n"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-// Bounded wait with cluster-scope acquire (arrivals from the peer CTA).
-__device__ __forceinline__ bool mbar_wait_cl(uint64_t *bar, uint32_t parity, volatile int *abort) {
-  if (mbar_try_wait_cl(bar, parity)) return true;
-  const unsigned long long t0 = now_ns();
-  while (true) {
-    if (mbar_try_wait_cl(bar, parity)) return true;
-    if (*abort) return false;
-    if (now_ns() - t0 > wait_limit()) {
-      *abort = 1;
-      return false;
-    }
-  }
-}
-// mbar_wait_own with cluster-scope acquire (pair MMAs arrive from the pair).
-__device__ __forceinline__ void mbar_wait_own_cl(uint64_t *bar, uint32_t parity) {
-  if (mbar_try_wait_cl(bar, parity)) return;
-  const unsigned long long t0 = now_ns();
-  while (!mbar_try_wait_cl(bar, parity) && now_ns() - t0 <= kTimeoutNs) {
-  }
-}
-// Both CTAs of the pair reach this point (every path to it is bounded).
-__device__ __forceinline__ void cluster_sync_all() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::
-                   : "memory");
 }
 __device__ __forceinline__ void tc_mma_i8_pair(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc,
                                                uint32_t idesc, uint32_t accumulate) {
@@ -274,130 +129,6 @@ __device__ __forceinline__ void tc_mma_i8_pair(uint32_t tmem_d, uint64_t adesc, 
       "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-// Completion of this thread's pair MMAs arrives on `bar` in both CTAs (the
-// barrier sits at the same shared-memory offset in each).
-__device__ __forceinline__ void tc_commit_pair_both(uint64_t *bar) {
-  asm volatile(
-      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
-      "[%0], %1;" ::"r"(smem_u32(bar)),
-      "h"((unsigned short)3)
-      : "memory");
-}
-__device__ __forceinline__ void tc_commit_pair_local(uint64_t *bar) {
-  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-                   smem_u32(bar))
-               : "memory");
-}
-// ---- TMA (prepacked b): a plain 2-D tiled load into this CTA's shared
-// memory, completing bytes on an mbarrier (no multicast).
-__device__ __forceinline__ void mbar_arrive_expect_tx(uint64_t *bar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)),
-               "r"(bytes)
-               : "memory");
-}
-__device__ __forceinline__ void tma_load_2d(uint32_t smem_dst, const CUtensorMap *map, int x, int y,
-                                            uint64_t *bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
-      "%3}], [%4];" ::"r"(smem_dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(smem_u32(bar))
-      : "memory");
-}
-// L2 prefetch of one tensor-map tile of this GPU's memory (no shared memory,
-// no multicast): the prepacked-b loader asks for a k-block some stages
-// before its load, so that the load finds it in L2.
-__device__ __forceinline__ void tma_prefetch_l2_2d(const CUtensorMap *map, int x, int y) {
-  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];" ::"l"(
-                   reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y)
-               : "memory");
-}
-__device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c,
-                                             uint32_t d) {
-  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c),
-               "r"(d)
-               : "memory");
-}
-__device__ __forceinline__ uint4 ld_shared_v4(uint32_t addr) {
-  uint4 v;
-  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "r"(addr));
-  return v;
-}
-__device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
-  uint32_t r;
-  asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(sel));
-  return r;
-}
-
-// 32 consecutive TMEM columns of this warp's 32 lanes (lane i -> row i).
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]),
-        "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]),
-        "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]),
-        "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]),
-        "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
-      : "r"(taddr));
-}
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]),
-        "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]),
-        "=r"(v[14]), "=r"(v[15])
-      : "r"(taddr));
-}
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
-      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
-      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
-      "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]),
-      "r"(v[15])
-      : "memory");
-}
-
-__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&v)[8]) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]),
-                 "=r"(v[6]), "=r"(v[7])
-               : "r"(taddr));
-}
-__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&v)[8]) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(
-                   taddr),
-               "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]),
-               "r"(v[7])
-               : "memory");
-}
-
-// K-major, 128-byte-swizzled UMMA shared-memory descriptor: 8-row atoms of
-// 128 B (1024 B apart), version 1, layout SWIZZLE_128B.
-__device__ __forceinline__ uint64_t smem_desc_sw128(uint32_t addr) {
-  uint64_t d = 0;
-  d |= (uint64_t)((addr & 0x3FFFFu) >> 4);        // start address
-  d |= (uint64_t)1 << 16;                          // leading byte offset (unused here)
-  d |= (uint64_t)(1024u >> 4) << 32;               // stride byte offset: 8 rows x 128 B
-  d |= (uint64_t)1 << 46;                          // descriptor version (sm_100)
-  d |= (uint64_t)2 << 61;                          // SWIZZLE_128B
-  return d;
-}
-
-// The descriptor of addr + bytes from that of addr: the start-address field
-// holds (addr & 0x3FFFF) >> 4 in 14 bits, so adding bytes >> 4 is exact while
-// addr + bytes stays below 256 KB and bytes is a multiple of 16 (every tile
-// offset here).  One 64-bit add instead of rebuilding the descriptor: the
-// MMA thread shares its SM sub-partition with busy producer warps, and its
-// instructions per stage are on the tensor pipe's critical path.
-__device__ __forceinline__ uint64_t desc_add(uint64_t desc, uint32_t bytes) {
-  return desc + (uint64_t)(bytes >> 4);
-}
-
 // Instruction descriptor: s8 x s8 -> s32, K-major A and B, M = 128, N = BN.
 template <int BN>
 __host__ __device__ constexpr uint32_t idesc_i8() {
@@ -2524,20 +2255,6 @@ cudaError_t launch_bn(TcParams prm, int sms, cudaStream_t s) {
   return cudaGetLastError();
 }
 
-PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
-  static std::once_flag once;
-  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-  std::call_once(once, [] {
-    void *p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) ==
-            cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
-  });
-  return fn;
-}
-
 template <int LG, bool kPackedB>
 cudaError_t launch_pair_v(TcParams prm, int dev, const CUtensorMap &tmap, cudaStream_t s) {
   auto kern = gemm_tc_pair_kernel<LG, kPackedB>;
@@ -2999,9 +2716,11 @@ cudaError_t launch_gemm_tc(const GemmProblem &P, int64_t m_rows, int64_t n_rows,
 }
 
 namespace {
-template <typename T>
-int set_device_word(const T &symbol, const T &value, const char *what) {
-  const cudaError_t e = cudaMemcpyToSymbol(symbol, &value, sizeof(T));
+// Sets this file's word and the 4-bit product's.
+template <typename T, typename Mx>
+int set_device_word(const T &symbol, const T &value, Mx mx, const char *what) {
+  cudaError_t e = cudaMemcpyToSymbol(symbol, &value, sizeof(T));
+  if (e == cudaSuccess) e = mx(value);
   if (e != cudaSuccess) {
     char buf[200];
     snprintf(buf, sizeof(buf), "%s: %s", what, cudaGetErrorString(e));
@@ -3018,7 +2737,7 @@ int debug_set_wait_limit(uint64_t ns) {
     return SCMP_EINVAL;
   }
   const unsigned long long v = ns;
-  return set_device_word(g_wait_limit_ns, v, "setting the wait limit");
+  return set_device_word(g_wait_limit_ns, v, mx_set_wait_limit, "setting the wait limit");
 }
 
 cudaError_t launch_probe_mma_mxf4(int n, int iters, int blocks, unsigned int *error,
@@ -3047,7 +2766,7 @@ cudaError_t launch_probe_mma_mxf4(int n, int iters, int blocks, unsigned int *er
 
 int debug_hold_producers(int on) {
   const int v = on ? 1 : 0;
-  return set_device_word(g_hold_producers, v, "setting the producer hold");
+  return set_device_word(g_hold_producers, v, mx_hold_producers, "setting the producer hold");
 }
 
 }  // namespace scmp

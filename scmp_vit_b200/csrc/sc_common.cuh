@@ -236,6 +236,9 @@ cudaError_t cached_symbol_address(SymbolCache (&cache)[kMaxCachedDevices], std::
 // (synchronous; SCMP_OK or an SCMP_E* code).
 int debug_set_wait_limit(uint64_t ns);
 int debug_hold_producers(int on);
+// The same words of the 4-bit product's kernels (mx_matmul.cu).
+cudaError_t mx_set_wait_limit(unsigned long long ns);
+cudaError_t mx_hold_producers(int on);
 // e2m1 MMA-rate probe (kind::mxf4, M = 128 x N = n x K = 64, n = 64 or 256):
 // `blocks` CTAs each issue 4 * iters MMAs; bit 0 of *error = a wait gave up.
 cudaError_t launch_probe_mma_mxf4(int n, int iters, int blocks, unsigned int *error,

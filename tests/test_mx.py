@@ -399,3 +399,28 @@ def test_streams_and_graph(cuda_device):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, mx.mx_matmul(x * 2 + 1, w))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FMTS)
+def test_matmul_bounded_wait_gives_up_and_recovers(cuda_device, fmt):
+    """With the loaders held on a flag that nothing sets, every wait runs out
+    after its (shortened) limit, the launch returns and says so, and the next
+    call on the same context is right."""
+    g = torch.Generator().manual_seed(8)
+    a, w = torch.randn(300, 320, generator=g), torch.randn(300, 320, generator=g)
+    a, w = a.to(cuda_device), w.to(cuda_device)
+    qa, qw = mx.mx_quantize(a, fmt), mx.mx_quantize(w, fmt)
+    torch.cuda.synchronize()
+    _lib.engine_status(reset=True)
+    _lib.set_wait_limit(20_000_000)
+    _lib.hold_producers(True)
+    try:
+        mx.mx_matmul(qa, qw)
+        torch.cuda.synchronize()
+        status = _lib.engine_status(reset=True)
+    finally:
+        _lib.hold_producers(False)
+        _lib.set_wait_limit(2_000_000_000)
+    assert status & 1
+    check_product(a, w, fmt, torch.float32)
