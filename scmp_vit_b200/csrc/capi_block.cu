@@ -213,8 +213,7 @@ int scmp_residual_norm(const scmp_norm_args *args, void *stream) {
 size_t scmp_residual_norm_bwd_workspace(int64_t rows, int64_t C, int64_t rows_per_gate) {
   if (rows <= 0 || C <= 0 || C > kNormMaxC || rows_per_gate <= 0 || rows % rows_per_gate != 0)
     return 0;
-  const NormBwdPlan plan = norm_bwd_plan(rows, rows / rows_per_gate, C);
-  return (size_t)(plan.part_floats + plan.sum_floats) * sizeof(float);
+  return (size_t)norm_bwd_floats(rows, rows / rows_per_gate, C) * sizeof(float);
 }
 
 int scmp_residual_norm_bwd(const scmp_norm_bwd_args *args, void *stream) {
@@ -265,13 +264,13 @@ int scmp_residual_norm_bwd(const scmp_norm_bwd_args *args, void *stream) {
   p.rms = x.rms != 0;
   p.part_needed = x.dweight || x.dbias || x.dgamma || x.dgate || x.dpost_weight || x.dpost_bias;
   if (p.part_needed) {
-    const NormBwdPlan plan = norm_bwd_plan(p.rows, p.groups, p.C);
-    const size_t need = (size_t)(plan.part_floats + plan.sum_floats) * sizeof(float);
+    const size_t need = (size_t)norm_bwd_floats(p.rows, p.groups, p.C) * sizeof(float);
     if (!x.workspace || x.workspace_bytes < need)
       return fail(SCMP_EWORKSPACE, "workspace needs %zu bytes, got %zu", need,
                   x.workspace ? x.workspace_bytes : (size_t)0);
+    // the groups' sums lie behind the larger of the two plans' partials
     p.part = static_cast<float *>(x.workspace);
-    p.sums = p.part + plan.part_floats;
+    p.sums = p.part + need / sizeof(float) - (p.groups > 1 ? p.groups * 4 * p.C : 0);
   }
   if (!aligned({x.stats, x.workspace}, 8))
     return fail(SCMP_EINVAL, "stats and workspace must be 8-byte aligned");

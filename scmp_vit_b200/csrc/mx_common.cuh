@@ -29,6 +29,20 @@ template <> __device__ __forceinline__ __half from_f32<__half>(float v) {
   return __float2half_rn(v);
 }
 
+// n / d for n < 2^32 by a multiplication and shifts (round-up method of Granlund
+// and Montgomery: m = ceil(2^(32 + s) / d) - 2^32, s = ceil(log2 d)).
+struct FastDiv {
+  uint32_t d, m, s;
+  explicit FastDiv(uint32_t div) : d(div), m(0), s(0) {
+    while ((1ull << s) < d) ++s;
+    m = (uint32_t)(((1ull << 32) * ((1ull << s) - d)) / d + 1);
+  }
+  __device__ __forceinline__ uint32_t quotient(uint32_t n) const {
+    const uint32_t t = __umulhi(n, m);
+    return s ? (t + ((n - t) >> 1)) >> (s - 1) : n;
+  }
+};
+
 // Two elements packed in a 32-bit word (16-bit types).
 template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t w);
 template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w) {
@@ -135,20 +149,32 @@ __device__ __forceinline__ float e8m0_value(uint32_t code) {
 constexpr uint32_t kMxNan = 0xFF;  // e8m0 NaN
 constexpr uint32_t kNvNan = 0x7F;  // e4m3 NaN
 
-// One lane's eight consecutive values of a block whose largest magnitude is
-// amax: the block's scale code and the eight element codes.
+// Magnitudes are compared as integers, the sign bit cleared: their order is the
+// numbers' and every NaN lies above the infinities.
+template <int N> __device__ __forceinline__ uint32_t max_bits(const float *v) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) m = max(m, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+  return m;
+}
+
+// One lane's eight consecutive values of a block whose largest magnitude has
+// the bits `amax`: the block's scale code and the eight element codes.
 //   mxfp4: scale 2^E, E = floor(log2 amax) - 2 (never below -127), read off
 //   amax's exponent field; x * 2^-E is exact wherever it decides a code.
-//   nvfp4: scale s = e4m3(amax * 2^-e / 6), code of the IEEE quotient
-//   x * 2^-e / s.  s has 4 significant bits, so a value on a border between two
-//   codes divides to exactly that border and no other value rounds onto it:
-//   the codes are those of the exact quotient.
+//   nvfp4: scale s = e4m3(amax * 2^-e / 6), code of the correctly rounded
+//   quotient x * 2^-e / s, from s's correctly rounded reciprocal with one
+//   correction by the remainder (Markstein 1990).  s has 4 significant bits, so
+//   a value on a border between two codes divides to exactly that border and
+//   no other value rounds onto it: the codes are those of the exact quotient.
 // A NaN or an infinity in the block: the NaN scale, element codes 0.
-template <int kFmt>
-__device__ __forceinline__ uint32_t mx_encode8(const float *x, float amax, float inv_exp,
+// kExp: nvfp4 with e != 0; x * 2^-e may then leave fp32's range, and is held to
+// a magnitude that saturates under every scale.
+template <int kFmt, bool kExp>
+__device__ __forceinline__ uint32_t mx_encode8(const float *x, uint32_t amax, float inv_exp,
                                                uint32_t *codes) {
-  const uint32_t field = __float_as_uint(amax) >> 23;  // amax >= 0 or NaN
-  const bool bad = (field & 0xFFu) == 0xFFu;
+  const uint32_t field = amax >> 23;
+  const bool bad = field == 0xFFu;
   float q[8];
   uint32_t scale;
   if (kFmt == SCMP_MXFP4) {
@@ -157,22 +183,21 @@ __device__ __forceinline__ uint32_t mx_encode8(const float *x, float amax, float
 #pragma unroll
     for (int i = 0; i < 8; ++i) q[i] = x[i] * inv;
   } else {
-    scale = e4m3_code(__fdiv_rn(amax * inv_exp, 6.0f));
-    const float s = e4m3_value(scale);
+    const float a = __uint_as_float(amax);
+    scale = e4m3_code(__fdiv_rn(kExp ? a * inv_exp : a, 6.0f));
+    const float s = e4m3_value(scale), r = scale ? __frcp_rn(s) : 0.0f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) q[i] = scale ? __fdiv_rn(x[i] * inv_exp, s) : x[i] * 0.0f;
+    for (int i = 0; i < 8; ++i) {
+      float v = x[i];
+      if (kExp) v = fminf(fmaxf(v * inv_exp, -1e30f), 1e30f);
+      const float y = v * r;
+      q[i] = copysignf(__fmaf_rn(__fmaf_rn(-y, s, v), r, y), v);  // -0 stays -0
+    }
     if (bad) scale = kNvNan;
   }
   const uint32_t c = e2m1x8(q);
   *codes = bad ? 0u : c;
   return scale;
-}
-
-// Largest of two magnitudes; a NaN stays.
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
 }
 
 // --------------------------------------------------------------- launchers

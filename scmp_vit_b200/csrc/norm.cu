@@ -13,20 +13,39 @@
 namespace scmp {
 namespace {
 
-// Columns of lane `lane` of warp `w` (of the `G` that share a row), chunk j.
+// A row is dealt to G warps: chunk j (of V consecutive columns per lane) of warp
+// w starts at column ((j G + w) 32 + lane) V.
 template <int V> __device__ __forceinline__ int col_of(int j, int G, int w, int lane) {
   return ((j * G + w) * 32 + lane) * V;
 }
 
-// V consecutive elements at p (16-byte pieces when V > 1).
-template <typename T, int V> __device__ __forceinline__ void load_v(const T *p, float *v) {
-  if (V == 1) {
-    v[0] = to_f32(*p);
-  } else {
+// V consecutive elements, as loaded: 16-byte pieces, or one element (V = 1).
+template <typename T, int V> struct Pack {
+  static constexpr int kN = V * (int)sizeof(T) / 16;
+  uint4 u[kN];
+  __device__ __forceinline__ void zero() {
 #pragma unroll
-    for (int i = 0; i < V; i += kVec16<T>)
-      unpack16<T>(__ldg(reinterpret_cast<const uint4 *>(p + i)), v + i);
+    for (int i = 0; i < kN; ++i) u[i] = make_uint4(0, 0, 0, 0);
   }
+  __device__ __forceinline__ void load(const T *p) {
+#pragma unroll
+    for (int i = 0; i < kN; ++i) u[i] = __ldg(reinterpret_cast<const uint4 *>(p) + i);
+  }
+  __device__ __forceinline__ void get(float *v) const {
+#pragma unroll
+    for (int i = 0; i < kN; ++i) unpack16<T>(u[i], v + i * kVec16<T>);
+  }
+};
+template <typename T> struct Pack<T, 1> {
+  T u;
+  __device__ __forceinline__ void zero() { u = from_f32<T>(0.0f); }
+  __device__ __forceinline__ void load(const T *p) { u = *p; }
+  __device__ __forceinline__ void get(float *v) const { v[0] = to_f32(u); }
+};
+template <typename T, int V> __device__ __forceinline__ void load_v(const T *p, float *v) {
+  Pack<T, V> q;
+  q.load(p);
+  q.get(v);
 }
 template <typename T, int V> __device__ __forceinline__ void store_v(T *p, const float *v) {
   if (V == 1) {
@@ -46,34 +65,45 @@ __device__ __forceinline__ float2 warp_sum(float2 v) {
   }
   return v;
 }
-
-// Sums over the warps of a row.  Two buffers in turn: a warp writes one again
-// only after the barrier that follows every read of it.
-struct RowSum {
-  float2 *buf;  // [2][warps of the block]
-  int warps, first, G, turn;
-  __device__ __forceinline__ float2 operator()(float2 v) {
-    v = warp_sum(v);
-    if (G == 1) return v;
-    float2 *b = buf + turn * warps;
-    turn ^= 1;
-    if ((threadIdx.x & 31) == 0) b[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = make_float2(0.f, 0.f);
-    for (int i = 0; i < G; ++i) {
-      v.x += b[first + i].x;
-      v.y += b[first + i].y;
-    }
-    return v;
-  }
-  __device__ __forceinline__ float operator()(float v) {
-    return (*this)(make_float2(v, 0.f)).x;
-  }
-};
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
+  return v;
+}
 
 constexpr int kMaxWarps = 16;
 
-// v (valid where in(j)) -> N(v) and its statistics.
+// Sums over the G warps of a row slot, which meet at a barrier of their own.
+// Two buffers in turn: a warp writes one again only after the barrier that
+// follows every read of it.
+struct RowSum {
+  float2 *buf;  // this slot's warps in [2][kMaxWarps]
+  int G, w, barrier, turn;
+  __device__ RowSum(float2 *all, int G_, int slot, int w_)
+      : buf(all + slot * G_), G(G_), w(w_), barrier(1 + slot), turn(0) {}
+  __device__ __forceinline__ float2 meet(float2 v) {
+    float2 *b = buf + turn * kMaxWarps;
+    turn ^= 1;
+    if ((threadIdx.x & 31) == 0) b[w] = v;
+    asm volatile("bar.sync %0, %1;" ::"r"(barrier), "r"(G * 32) : "memory");
+    v = make_float2(0.f, 0.f);
+    for (int i = 0; i < G; ++i) {
+      v.x += b[i].x;
+      v.y += b[i].y;
+    }
+    return v;
+  }
+  __device__ __forceinline__ float2 operator()(float2 v) {
+    v = warp_sum(v);
+    return G == 1 ? v : meet(v);
+  }
+  __device__ __forceinline__ float operator()(float v) {
+    v = warp_sum(v);
+    return G == 1 ? v : meet(make_float2(v, 0.f)).x;
+  }
+};
+
+// v (0 past the row, where in(j) is false) -> N(v) and its statistics.
 template <int NV, int V, typename In>
 __device__ __forceinline__ float2 normalise(float (&v)[NV][V], const In &in, RowSum &sum,
                                             float inv_c, float eps, bool rms) {
@@ -83,7 +113,7 @@ __device__ __forceinline__ float2 normalise(float (&v)[NV][V], const In &in, Row
 #pragma unroll
     for (int j = 0; j < NV; ++j)
 #pragma unroll
-      for (int i = 0; i < V; ++i) s += v[j][i];  // 0 past the row
+      for (int i = 0; i < V; ++i) s += v[j][i];
     mean = sum(s) * inv_c;
   }
   float q = 0.f;
@@ -109,15 +139,13 @@ __device__ __forceinline__ void store_mx(const NormParams &p, const float *v, in
                                          int lane) {
   constexpr int kBlock = kFmt == SCMP_MXFP4 ? 32 : 16;
   constexpr int kLanes = kBlock / V;
-  float amax = 0.f, v8[8];
+  float v8[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) v8[i] = i < V ? v[i] : 0.f;
+  uint32_t amax = max_bits<V>(v), codes;
 #pragma unroll
-  for (int i = 0; i < V; ++i) amax = max_nan(amax, fabsf(v[i]));
-#pragma unroll
-  for (int o = 1; o < kLanes; o <<= 1) amax = max_nan(amax, __shfl_xor_sync(~0u, amax, o));
-  uint32_t codes;
-  const uint32_t scale = mx_encode8<kFmt>(v8, amax, 1.0f, &codes);
+  for (int o = 1; o < kLanes; o <<= 1) amax = max(amax, __shfl_xor_sync(~0u, amax, o));
+  const uint32_t scale = mx_encode8<kFmt, false>(v8, amax, 1.0f, &codes);
   if (row < p.rows && col < p.kp) {
     uint8_t *d = p.mx_data + row * (p.kp >> 1) + (col >> 1);
     if (V == 8)
@@ -125,61 +153,65 @@ __device__ __forceinline__ void store_mx(const NormParams &p, const float *v, in
     else
       *reinterpret_cast<uint16_t *>(d) = (uint16_t)codes;
   }
-  uint32_t word = 0;
-#pragma unroll
-  for (int b = 0; b < 4; ++b)
-    word |= __shfl_sync(~0u, scale, (lane & ~(4 * kLanes - 1)) + b * kLanes) << (8 * b);
-  const int64_t g = col / (4 * kBlock);
-  if ((lane & (4 * kLanes - 1)) == 0 && g < p.groups)
-    *reinterpret_cast<uint32_t *>(p.mx_scales + mx_scale_word(row, g, p.groups)) = word;
+  const int blk = col / kBlock;
+  if ((lane & (kLanes - 1)) == 0 && (blk >> 2) < p.groups)
+    p.mx_scales[mx_scale_word(row, blk >> 2, p.groups) + (blk & 3)] = (uint8_t)scale;
 }
 
-// G warps per row, 32 elements per lane.
-template <typename T, typename P, int V>
-__global__ void __launch_bounds__(32 * kMaxWarps)
+// E elements per lane.  E = 8 (rows of up to 2048 in 16-byte pieces: 8 warps a
+// block) keeps a row's chain of instructions short and 64 warps on an SM; longer
+// or unaligned rows take E = 32.
+template <typename T, typename P, int V, int E>
+__global__ void __launch_bounds__(256)
     residual_norm_kernel(const __grid_constant__ NormParams p) {
-  constexpr int NV = 32 / V;
+  constexpr int NV = E / V;
   __shared__ float2 buf[2 * kMaxWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int G = p.warps_per_row, w = warp % G;
-  RowSum sum{buf, (int)(blockDim.x >> 5), warp - w, G, 0};
-  const int64_t row = (int64_t)blockIdx.x * (blockDim.x / (32 * G)) + warp / G;
+  const int G = p.warps_per_row, slot = warp / G, w = warp - slot * G;
+  RowSum sum(buf, G, slot, w);
+  const int64_t row = (int64_t)blockIdx.x * (blockDim.x / (32 * G)) + slot;
   const bool live = row < p.rows;
   const int C = p.C;
   const float inv_c = 1.0f / (float)C;
-  const auto in = [&](int j) { return col_of<V>(j, G, w, lane) < C; };
+  const auto in = [&](int j) { return live && col_of<V>(j, G, w, lane) < C; };
   const int64_t at = row * C;
 
-  float r[NV][V], z[NV][V];
+  Pack<T, V> x[NV], y[NV];
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     const int c = col_of<V>(j, G, w, lane);
-#pragma unroll
-    for (int i = 0; i < V; ++i) r[j][i] = z[j][i] = 0.f;
-    if (live && c < C) {
-      load_v<T, V>(static_cast<const T *>(p.x) + at + c, r[j]);
-      if (p.y) load_v<T, V>(static_cast<const T *>(p.y) + at + c, z[j]);
-    }
+    x[j].zero();
+    y[j].zero();
+    if (!in(j)) continue;
+    x[j].load(static_cast<const T *>(p.x) + at + c);
+    if (p.y) y[j].load(static_cast<const T *>(p.y) + at + c);
   }
+  float r[NV][V];
   if (p.y) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) y[j].get(r[j]);
     if (p.post_weight) {
-      const float2 st = normalise<NV, V>(z, in, sum, inv_c, p.eps, p.rms);
+      const float2 st = normalise<NV, V>(r, in, sum, inv_c, p.eps, p.rms);
       if (p.stats && live && w == 0 && lane == 0) p.stats[p.rows + row] = st;
     }
     const int64_t gate_at = p.gate && live ? row / p.rows_per_gate * C : 0;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int c = col_of<V>(j, G, w, lane);
-      if (!live || c >= C) continue;
+      if (!in(j)) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) r[j][i] = 0.f;
+        continue;
+      }
       float f[V], g[V];
       if (p.post_weight) {
         load_v<P, V>(static_cast<const P *>(p.post_weight) + c, f);
 #pragma unroll
-        for (int i = 0; i < V; ++i) z[j][i] *= f[i];
+        for (int i = 0; i < V; ++i) r[j][i] *= f[i];
         if (p.post_bias) {
           load_v<P, V>(static_cast<const P *>(p.post_bias) + c, f);
 #pragma unroll
-          for (int i = 0; i < V; ++i) z[j][i] += f[i];
+          for (int i = 0; i < V; ++i) r[j][i] += f[i];
         }
       }
 #pragma unroll
@@ -190,20 +222,24 @@ __global__ void __launch_bounds__(32 * kMaxWarps)
 #pragma unroll
         for (int i = 0; i < V; ++i) f[i] *= g[i];
       }
+      x[j].get(g);
       // r is rounded to its type once, and the norm sees the rounded value: the
       // one that the next block and the backward pass read
 #pragma unroll
       for (int i = 0; i < V; ++i)
-        r[j][i] = to_f32(from_f32<T>(__fmaf_rn(z[j][i], f[i], r[j][i])));
+        r[j][i] = to_f32(from_f32<T>(__fmaf_rn(r[j][i], f[i], g[i])));
       store_v<T, V>(static_cast<T *>(p.r) + at + c, r[j]);
     }
+  } else {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) x[j].get(r[j]);
   }
   const float2 st = normalise<NV, V>(r, in, sum, inv_c, p.eps, p.rms);
   if (p.stats && live && w == 0 && lane == 0) p.stats[row] = st;
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     const int c = col_of<V>(j, G, w, lane);
-    if (live && c < C) {
+    if (in(j)) {
       float f[V];
       load_v<P, V>(static_cast<const P *>(p.weight) + c, f);
 #pragma unroll
@@ -230,30 +266,81 @@ __global__ void __launch_bounds__(32 * kMaxWarps)
 }
 
 // ---------------------------------------------------------------- backward
-// Rows of one gate group (all rows without a gate) are dealt to `per_group`
-// row slots; a slot is G warps with 16 elements per lane, a block holds a few
-// slots of one group.  Column sums stay in registers over a slot's rows, are
-// added over the block's slots in shared memory in a fixed order and written
-// as partials [group][block][part][C]; a second kernel adds those in order, so
-// the result does not depend on timing.
+// Rows of one gate group (all rows without a gate) are dealt to row slots of G
+// warps; a block holds a few slots of one group.  While a row is worked on, the
+// slot's next row is on its way into registers.  Column sums stay in registers
+// over a slot's rows, are added over the block's slots in shared memory in a
+// fixed order and written as partials [group][block][part][C]; a second kernel
+// adds those in order, so the result does not depend on timing.
 //   parts: 0 sum dh n   1 sum dh   2 sum g z (no post norm) or sum g m   3 sum g
-template <typename T, typename P, int V, bool kPost>
-__global__ void __launch_bounds__(32 * kMaxWarps)
+// E = 8 elements per lane for rows of up to 2048 in 16-byte pieces, else 16.
+template <typename T, int V, int NV> struct BwdRow {
+  Pack<T, V> r[NV], y[NV], dr[NV], dh[NV];
+  float2 st, st_y;
+};
+template <typename T, int V, int NV>
+__device__ __forceinline__ void load_row(const NormBwdParams &p, int64_t row, bool live, int G,
+                                         int w, int lane, bool post, BwdRow<T, V, NV> &q) {
+  q.st = q.st_y = make_float2(0.f, 0.f);
+  if (live) {
+    q.st = p.stats[row];
+    if (post) q.st_y = p.stats[p.rows + row];
+  }
+  const int64_t at = row * p.C;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int c = col_of<V>(j, G, w, lane);
+    q.r[j].zero();
+    q.y[j].zero();
+    q.dr[j].zero();
+    q.dh[j].zero();
+    if (!live || c >= p.C) continue;
+    q.r[j].load(static_cast<const T *>(p.r) + at + c);
+    if (p.dh) q.dh[j].load(static_cast<const T *>(p.dh) + at + c);
+    if (p.dr) q.dr[j].load(static_cast<const T *>(p.dr) + at + c);
+    if (p.y) q.y[j].load(static_cast<const T *>(p.y) + at + c);
+  }
+}
+
+template <typename T, typename P, int V, int E, bool kPost, int kThreads>
+__global__ void __launch_bounds__(kThreads, 1)
     residual_norm_bwd_kernel(const __grid_constant__ NormBwdParams p) {
-  constexpr int NV = 16 / V;
+  constexpr int NV = E / V;
   constexpr int kParts = kPost ? 4 : 3;
   __shared__ float2 buf[2 * kMaxWarps];
   extern __shared__ float part_smem[];  // [C], blocks of several slots
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int G = p.warps_per_row, w = warp % G, slot = warp / G;
+  const int G = p.warps_per_row, slot = warp / G, w = warp - slot * G;
   const int slots = blockDim.x / (32 * G);
-  RowSum sum{buf, (int)(blockDim.x >> 5), warp - w, G, 0};
+  RowSum sum(buf, G, slot, w);
   const int C = p.C;
   const float inv_c = 1.0f / (float)C;
   const int64_t group = blockIdx.x / p.blocks_per_group;
-  const int64_t first = (blockIdx.x % p.blocks_per_group) * slots + slot;
   const int64_t stride = p.blocks_per_group * slots;
+  const int64_t row0 = group * p.rows_per_group;
 
+  // the parameters of this lane's columns stay the same over the rows
+  float wt[NV][V], sc[NV][V], pw[kPost ? NV : 1][V];
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int c = col_of<V>(j, G, w, lane);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      wt[j][i] = 0.f;
+      sc[j][i] = 1.f;
+      if (kPost) pw[kPost ? j : 0][i] = 0.f;
+    }
+    if (c >= C) continue;
+    load_v<P, V>(static_cast<const P *>(p.weight) + c, wt[j]);
+    if (p.gamma) load_v<P, V>(static_cast<const P *>(p.gamma) + c, sc[j]);
+    if (p.gate) {
+      float g[V];
+      load_v<P, V>(static_cast<const P *>(p.gate) + group * C + c, g);
+#pragma unroll
+      for (int i = 0; i < V; ++i) sc[j][i] *= g[i];
+    }
+    if (kPost) load_v<P, V>(static_cast<const P *>(p.post_weight) + c, pw[kPost ? j : 0]);
+  }
   float acc[kParts][NV][V];
 #pragma unroll
   for (int k = 0; k < kParts; ++k)
@@ -262,44 +349,27 @@ __global__ void __launch_bounds__(32 * kMaxWarps)
 #pragma unroll
       for (int i = 0; i < V; ++i) acc[k][j][i] = 0.f;
 
-  // every slot of a block runs the same number of rounds: the row sums meet at
-  // block barriers
-  const int64_t rounds = (p.rows_per_group + stride - 1) / stride;
-  for (int64_t t = 0; t < rounds; ++t) {
-    const int64_t in_group = first + t * stride;
-    const bool live = in_group < p.rows_per_group;
-    const int64_t row = group * p.rows_per_group + in_group;
-    const int64_t at = row * C;
-    float n[NV][V], g[NV][V], dn[NV][V], y[NV][V];
-    float2 st = make_float2(0.f, 0.f), st_y = st;
-    if (live) {
-      st = p.stats[row];
-      if (kPost) st_y = p.stats[p.rows + row];
-    }
+  int64_t i_row = (blockIdx.x % p.blocks_per_group) * slots + slot;
+  BwdRow<T, V, NV> next;
+  load_row<T, V, NV>(p, row0 + i_row, i_row < p.rows_per_group, G, w, lane, kPost, next);
+  for (; i_row < p.rows_per_group; i_row += stride) {
+    const BwdRow<T, V, NV> q = next;
+    load_row<T, V, NV>(p, row0 + i_row + stride, i_row + stride < p.rows_per_group, G, w, lane,
+                       kPost, next);
+    const int64_t at = (row0 + i_row) * C;
+    float n[NV][V], dn[NV][V];
     float2 s = make_float2(0.f, 0.f);
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int c = col_of<V>(j, G, w, lane);
-#pragma unroll
-      for (int i = 0; i < V; ++i) n[j][i] = g[j][i] = dn[j][i] = y[j][i] = 0.f;
-      if (!live || c >= C) continue;
-      load_v<T, V>(static_cast<const T *>(p.r) + at + c, n[j]);
-      if (p.dh) load_v<T, V>(static_cast<const T *>(p.dh) + at + c, dn[j]);
-      if (p.dr) load_v<T, V>(static_cast<const T *>(p.dr) + at + c, g[j]);
-      if (p.y) load_v<T, V>(static_cast<const T *>(p.y) + at + c, y[j]);
-    }
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int c = col_of<V>(j, G, w, lane);
-      if (!live || c >= C) continue;
-      float f[V];
-      load_v<P, V>(static_cast<const P *>(p.weight) + c, f);
+      const bool in = col_of<V>(j, G, w, lane) < C;
+      q.r[j].get(n[j]);
+      q.dh[j].get(dn[j]);
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        n[j][i] = (n[j][i] - st.x) * st.y;
+        n[j][i] = in ? (n[j][i] - q.st.x) * q.st.y : 0.f;
         acc[0][j][i] = __fmaf_rn(dn[j][i], n[j][i], acc[0][j][i]);
         acc[1][j][i] += dn[j][i];
-        dn[j][i] *= f[i];
+        dn[j][i] *= wt[j][i];
         s.x += dn[j][i];
         s.y = __fmaf_rn(dn[j][i], n[j][i], s.y);
       }
@@ -307,43 +377,35 @@ __global__ void __launch_bounds__(32 * kMaxWarps)
     s = sum(s);
     const float mean_dn = p.rms ? 0.f : s.x * inv_c, mean_dnn = s.y * inv_c;
     float2 s2 = make_float2(0.f, 0.f);
-    const int64_t gate_at = group * C;
+    float m[kPost ? NV : 1][V];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int c = col_of<V>(j, G, w, lane);
-      if (!live || c >= C) continue;
+      float g[V], y[V];
+      q.dr[j].get(g);
+      q.y[j].get(y);
 #pragma unroll
       for (int i = 0; i < V; ++i)
-        g[j][i] = __fmaf_rn(st.y, __fmaf_rn(-n[j][i], mean_dnn, dn[j][i] - mean_dn), g[j][i]);
-      if (p.dx) store_v<T, V>(static_cast<T *>(p.dx) + at + c, g[j]);
-      if (!p.y) continue;
-      float f[V], e[V];
-#pragma unroll
-      for (int i = 0; i < V; ++i) f[i] = 1.0f;
-      if (p.gamma) load_v<P, V>(static_cast<const P *>(p.gamma) + c, f);
-      if (p.gate) {
-        load_v<P, V>(static_cast<const P *>(p.gate) + gate_at + c, e);
-#pragma unroll
-        for (int i = 0; i < V; ++i) f[i] *= e[i];
-      }
+        g[i] = __fmaf_rn(q.st.y, __fmaf_rn(-n[j][i], mean_dnn, dn[j][i] - mean_dn), g[i]);
+      if (p.dx && c < C) store_v<T, V>(static_cast<T *>(p.dx) + at + c, g);
       if (kPost) {
-        load_v<P, V>(static_cast<const P *>(p.post_weight) + c, e);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          y[j][i] = (y[j][i] - st_y.x) * st_y.y;
-          acc[2][j][i] = __fmaf_rn(g[j][i], y[j][i], acc[2][j][i]);
-          acc[kParts - 1][j][i] += g[j][i];
-          dn[j][i] = g[j][i] * f[i] * e[i];
+          const float mi = c < C ? (y[i] - q.st_y.x) * q.st_y.y : 0.f;
+          m[kPost ? j : 0][i] = mi;
+          acc[2][j][i] = __fmaf_rn(g[i], mi, acc[2][j][i]);
+          acc[kParts - 1][j][i] += g[i];
+          dn[j][i] = g[i] * sc[j][i] * pw[kPost ? j : 0][i];
           s2.x += dn[j][i];
-          s2.y = __fmaf_rn(dn[j][i], y[j][i], s2.y);
+          s2.y = __fmaf_rn(dn[j][i], mi, s2.y);
         }
       } else {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          acc[2][j][i] = __fmaf_rn(g[j][i], y[j][i], acc[2][j][i]);
-          dn[j][i] = g[j][i] * f[i];
+          acc[2][j][i] = __fmaf_rn(g[i], y[i], acc[2][j][i]);
+          g[i] *= sc[j][i];
         }
-        if (p.dy) store_v<T, V>(static_cast<T *>(p.dy) + at + c, dn[j]);
+        if (p.dy && c < C) store_v<T, V>(static_cast<T *>(p.dy) + at + c, g);
       }
     }
     if (kPost) {
@@ -352,10 +414,10 @@ __global__ void __launch_bounds__(32 * kMaxWarps)
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         const int c = col_of<V>(j, G, w, lane);
-        if (!live || c >= C || !p.dy) continue;
+        if (c >= C || !p.dy) continue;
 #pragma unroll
         for (int i = 0; i < V; ++i)
-          dn[j][i] = st_y.y * __fmaf_rn(-y[j][i], mean_dmm, dn[j][i] - mean_dm);
+          dn[j][i] = q.st_y.y * __fmaf_rn(-m[kPost ? j : 0][i], mean_dmm, dn[j][i] - mean_dm);
         store_v<T, V>(static_cast<T *>(p.dy) + at + c, dn[j]);
       }
     }
@@ -364,7 +426,7 @@ __global__ void __launch_bounds__(32 * kMaxWarps)
   float *out = p.part + (int64_t)blockIdx.x * 4 * C;
 #pragma unroll
   for (int k = 0; k < kParts; ++k) {
-    for (int q = slots - 1; q > 0; --q) {  // slot q adds to what q + 1.. left; slot 0 writes
+    for (int q = slots - 1; q > 0; --q) {  // the slots add up, from the last to the first
       __syncthreads();
       if (slot == q) {
 #pragma unroll
@@ -423,40 +485,45 @@ __device__ __forceinline__ void write_totals(const NormBwdParams &p, int c,
     if (out[k]) static_cast<P *>(out[k])[c] = from_f32<P>(total[k]);
 }
 
-// Block (32 columns, gate group): 32 warps share the group's partials.  With
-// one group it finishes; else it leaves the group's sums for the kernel below.
+// Block (8 columns, gate group): 128 threads per column share the group's
+// partials.  With one group it finishes; else it leaves the group's sums for the
+// kernel below.
 template <typename P>
 __global__ void __launch_bounds__(1024) norm_bwd_sum_kernel(
     const __grid_constant__ NormBwdParams p) {
-  __shared__ float s[4][32][33];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int cols = (p.C + 31) / 32;
-  const int c = (int)(blockIdx.x % cols) * 32 + lane;
+  __shared__ float s[4][32][8];
+  const int cols = (p.C + 7) / 8;
+  const int ci = threadIdx.x & 7, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int c = (int)(blockIdx.x % cols) * 8 + ci;
   const int64_t group = blockIdx.x / cols;
   const int parts = p.post_weight ? 4 : 3;
   float v[4] = {0.f, 0.f, 0.f, 0.f};
   if (c < p.C)
-    for (int64_t b = warp; b < p.blocks_per_group; b += 32) {
+    for (int64_t b = threadIdx.x >> 3; b < p.blocks_per_group; b += 128) {
       const float *src = p.part + (group * p.blocks_per_group + b) * 4 * p.C + c;
-      for (int k = 0; k < parts; ++k) v[k] += src[(int64_t)k * p.C];
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (k < parts) v[k] += src[(int64_t)k * p.C];
     }
 #pragma unroll
-  for (int k = 0; k < 4; ++k) s[k][warp][lane] = v[k];
+  for (int k = 0; k < 4; ++k) {
+    v[k] += __shfl_xor_sync(~0u, v[k], 8);
+    v[k] += __shfl_xor_sync(~0u, v[k], 16);
+    if (lane < 8) s[k][warp][ci] = v[k];
+  }
   __syncthreads();
-  if (warp < 4) {
-    float t = 0.f;
-    for (int i = 0; i < 32; ++i) t += s[warp][i][lane];
-    if (p.groups > 1 && c < p.C) p.sums[(group * 4 + warp) * p.C + c] = t;
-    s[warp][0][lane] = t;  // read above by this thread alone
+  if (threadIdx.x >= 8 || c >= p.C) return;
+  float one[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    one[k] = 0.f;
+    for (int i = 0; i < 32; ++i) one[k] += s[k][i][ci];
+    if (p.groups > 1) p.sums[(group * 4 + k) * p.C + c] = one[k];
   }
   if (p.groups > 1) return;
-  __syncthreads();
-  if (warp == 0 && c < p.C) {
-    const float one[4] = {s[0][0][lane], s[1][0][lane], s[2][0][lane], s[3][0][lane]};
-    float total[5] = {0.f, 0.f, 0.f, 0.f, 0.f};
-    add_group<P>(p, 0, c, one, total);
-    write_totals<P>(p, c, total);
-  }
+  float total[5] = {0.f, 0.f, 0.f, 0.f, 0.f};
+  add_group<P>(p, 0, c, one, total);
+  write_totals<P>(p, c, total);
 }
 
 template <typename P>
@@ -488,67 +555,84 @@ __global__ void __launch_bounds__(1024) norm_bwd_groups_kernel(
 
 // --------------------------------------------------------------- dispatch
 
+// Elements per lane: 8 for rows of up to 2048 in 16-byte pieces.
+bool short_rows(int64_t C, bool vec) { return vec && C <= 2048; }
+
 template <typename T, typename P>
 cudaError_t forward(NormParams p, bool vec, cudaStream_t s) {
   constexpr int V = kVec16<T>;
-  const int G = (p.C + 1023) / 1024;  // 32 elements per lane
-  const int rows_per_block = G >= 4 ? 1 : 4 / G;
+  const bool small = short_rows(p.C, vec);
+  const int G = small ? (p.C + 255) / 256 : (p.C + 1023) / 1024;
+  const int slots = 8 / G;
   p.warps_per_row = G;
   const int64_t rows = p.mx_data ? (p.rows + 127) / 128 * 128 : p.rows;
-  const int64_t blocks = (rows + rows_per_block - 1) / rows_per_block;
-  const int threads = 32 * G * rows_per_block;
-  if (vec)
-    residual_norm_kernel<T, P, V><<<(unsigned)blocks, threads, 0, s>>>(p);
+  const unsigned blocks = (unsigned)((rows + slots - 1) / slots);
+  const int threads = 32 * G * slots;
+  if (small)
+    residual_norm_kernel<T, P, V, 8><<<blocks, threads, 0, s>>>(p);
+  else if (vec)
+    residual_norm_kernel<T, P, V, 32><<<blocks, threads, 0, s>>>(p);
   else
-    residual_norm_kernel<T, P, 1><<<(unsigned)blocks, threads, 0, s>>>(p);
+    residual_norm_kernel<T, P, 1, 32><<<blocks, threads, 0, s>>>(p);
   return cudaGetLastError();
 }
 
-template <typename T, typename P, int V>
-cudaError_t backward_v(const NormBwdParams &p, const NormBwdPlan &plan, cudaStream_t s) {
+template <typename T, typename P, int V, int E, int kThreads>
+cudaError_t backward_e(const NormBwdParams &p, const NormBwdPlan &plan, cudaStream_t s) {
   const size_t smem = plan.slots > 1 ? (size_t)p.C * sizeof(float) : 0;
   const unsigned blocks = (unsigned)(p.groups * p.blocks_per_group);
   const int threads = 32 * plan.warps_per_row * plan.slots;
   if (p.post_weight)
-    residual_norm_bwd_kernel<T, P, V, true><<<blocks, threads, smem, s>>>(p);
+    residual_norm_bwd_kernel<T, P, V, E, true, kThreads><<<blocks, threads, smem, s>>>(p);
   else
-    residual_norm_bwd_kernel<T, P, V, false><<<blocks, threads, smem, s>>>(p);
+    residual_norm_bwd_kernel<T, P, V, E, false, kThreads><<<blocks, threads, smem, s>>>(p);
   return cudaGetLastError();
 }
 
 template <typename T, typename P>
 cudaError_t backward(NormBwdParams p, bool vec, cudaStream_t s, int *launches) {
-  const NormBwdPlan plan = norm_bwd_plan(p.rows, p.groups, p.C);
+  const NormBwdPlan plan = norm_bwd_plan(p.rows, p.groups, p.C, vec);
   p.warps_per_row = plan.warps_per_row;
   p.blocks_per_group = plan.blocks_per_group;
   p.rows_per_group = p.rows / p.groups;
   if (!p.part_needed) p.part = nullptr;
-  cudaError_t e = vec ? backward_v<T, P, kVec16<T>>(p, plan, s) : backward_v<T, P, 1>(p, plan, s);
+  // (blocks of 512 threads leave 128 registers a thread, too few for 16
+  // elements: they serve the rows that need them)
+  constexpr int V = kVec16<T>;
+  cudaError_t e = short_rows(p.C, vec)    ? backward_e<T, P, V, 8, 256>(p, plan, s)
+                  : vec && p.C <= 8 * 512 ? backward_e<T, P, V, 16, 256>(p, plan, s)
+                  : vec                   ? backward_e<T, P, V, 16, 512>(p, plan, s)
+                                          : backward_e<T, P, 1, 16, 512>(p, plan, s);
   *launches = 1;
   if (e != cudaSuccess || !p.part) return e;
-  const unsigned cols = (unsigned)((p.C + 31) / 32);
-  norm_bwd_sum_kernel<P><<<(unsigned)(cols * p.groups), 1024, 0, s>>>(p);
+  norm_bwd_sum_kernel<P><<<(unsigned)((p.C + 7) / 8 * p.groups), 1024, 0, s>>>(p);
   ++*launches;
   if ((e = cudaGetLastError()) != cudaSuccess || p.groups == 1) return e;
-  norm_bwd_groups_kernel<P><<<cols, 1024, 0, s>>>(p);
+  norm_bwd_groups_kernel<P><<<(unsigned)((p.C + 31) / 32), 1024, 0, s>>>(p);
   ++*launches;
   return cudaGetLastError();
 }
 
 }  // namespace
 
-// Slots of 16 elements per lane, about 8 warps a block, and two blocks on each
-// of the 148 SMs in all (at least one block per gate group).
-NormBwdPlan norm_bwd_plan(int64_t rows, int64_t groups, int64_t C) {
+// About 8 warps a block (16 for long rows) and three blocks on each of the 148
+// SMs in all, at least one per gate group.
+NormBwdPlan norm_bwd_plan(int64_t rows, int64_t groups, int64_t C, bool vec) {
   NormBwdPlan plan;
-  plan.warps_per_row = (int)((C + 511) / 512);
+  plan.warps_per_row = (int)(short_rows(C, vec) ? (C + 255) / 256 : (C + 511) / 512);
   plan.slots = plan.warps_per_row >= 8 ? 1 : 8 / plan.warps_per_row;
   const int64_t per_group = (rows / groups + plan.slots - 1) / plan.slots;
-  const int64_t want = (2 * 148 + groups - 1) / groups;
+  const int64_t want = (3 * 148 + groups - 1) / groups;
   plan.blocks_per_group = want < per_group ? want : per_group;
   plan.part_floats = groups * plan.blocks_per_group * 4 * C;
   plan.sum_floats = groups > 1 ? groups * 4 * C : 0;
   return plan;
+}
+
+int64_t norm_bwd_floats(int64_t rows, int64_t groups, int64_t C) {
+  const NormBwdPlan a = norm_bwd_plan(rows, groups, C, true);
+  const NormBwdPlan b = norm_bwd_plan(rows, groups, C, false);
+  return (a.part_floats > b.part_floats ? a.part_floats : b.part_floats) + a.sum_floats;
 }
 
 cudaError_t launch_residual_norm(const NormParams &p, int dtype, int param_dtype, bool vec,
