@@ -316,9 +316,10 @@ int scmp_split_qkv_rotary(const scmp_rotary_args *args, void *stream) {
   }
   if (2 * p.pairs > x.D) return fail(SCMP_EINVAL, "the axes' dims exceed the head size");
   if (x.B == 0 || x.N == 0) return SCMP_OK;
-  // 2^31 blocks of at least one token each
-  if (x.N > kMaxRows || x.B > kMaxRows / x.N)
-    return fail(SCMP_EUNSUPPORTED, "split_qkv_rotary takes up to 2^31 - 1 tokens");
+  // pieces of a head row are counted in 32 bits
+  if (x.N > UINT32_MAX / x.D || x.B > UINT32_MAX / x.D / x.N)
+    return fail(SCMP_EUNSUPPORTED, "split_qkv_rotary takes up to 2^32 - 1 elements per head, got "
+                "B=%lld N=%lld D=%lld tokens", (long long)x.B, (long long)x.N, (long long)x.D);
   if (!x.qkv || !x.q || !x.k || !x.v || !x.table || !x.pos)
     return fail(SCMP_EINVAL, "qkv, q, k, v, table and pos must be non-NULL");
   if (!aligned({x.table}, 8)) return fail(SCMP_EINVAL, "table must be 8-byte aligned");

@@ -4,7 +4,15 @@
 //     u' = u cos t - v sin t,  v' = v cos t + u sin t,  t = c scale_a base^(-2 i / d_a)
 // cos and sin come from a table per axis (rows = coordinates), built in 64 bits
 // where far coordinates need them; the backward pass turns by -t.
+//
+// A thread owns a piece of a token's head (16 bytes, else 8 bytes or one element
+// where sizes or pointers ask for it) and walks the heads: its cos and sin stay in
+// registers, every access of a warp covers whole head rows, and a few heads are
+// in flight at a time.  v with its dimensions and tokens exchanged goes through
+// a shared-memory tile in blocks of its own, in the same launch.  HBM-bound.
 #include "rotary.cuh"
+
+#include <cstring>
 
 #include "mx_common.cuh"
 
@@ -12,108 +20,258 @@ namespace scmp {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kTile = 32;  // tokens per block
+constexpr int kAtOnce = 4;  // heads in flight per thread
+constexpr int kTile = 64;   // tokens of a transposed tile
 
-// cos and sin of every pair of a tile's tokens in shared memory, [kTile][pairs].
-// A negative coordinate leaves the token's pairs of that axis as they are; one
-// past the table's end makes them NaN rather than read there.
-__device__ __forceinline__ void stage_angles(const RotaryParams &p, int64_t b, int64_t t0, int nt,
-                                             float2 *cs) {
-  const int pairs = p.pairs;
-  for (int i = threadIdx.x; i < nt * pairs; i += kThreads) {
-    const int t = i / pairs, q = i % pairs;
-    int a = 0;
-    while (a + 1 < p.axes && q >= p.first_pair[a + 1]) ++a;
-    const int c = p.pos[((p.pos_batched ? b * p.N : 0) + t0 + t) * p.axes + a];
-    const int half = p.dims[a] >> 1;
-    float2 v = make_float2(1.0f, 0.0f);
-    if (c >= p.sizes[a])
-      v = make_float2(__uint_as_float(0x7FC00000u), __uint_as_float(0x7FC00000u));
-    else if (c >= 0)
-      v = p.table[p.table_at[a] + (int64_t)c * half + (q - p.first_pair[a])];
-    if (p.inverse) v.y = -v.y;
-    cs[i] = v;
+// cos and sin (signed for this direction) of pair q of a token; false: the
+// pair stays as it is.  A negative coordinate leaves the axis, one past the
+// table's end gives NaN rather than a read there.
+__device__ __forceinline__ bool angle_of(const RotaryParams &p, int64_t token, int a, int i,
+                                         float2 &cs) {
+  const int c = p.pos[token * p.axes + a];
+  if (c < 0) return false;
+  cs = make_float2(__uint_as_float(0x7FC00000u), __uint_as_float(0x7FC00000u));
+  if (c < p.sizes[a]) cs = p.table[p.table_at[a] + (int64_t)c * (p.dims[a] >> 1) + i];
+  return true;
+}
+
+// V elements as loaded: 16 or 8 bytes, or one element.
+template <typename T, int V> struct Piece {
+  static constexpr int kWords = V * (int)sizeof(T) / 4;
+  uint32_t u[kWords];
+  __device__ __forceinline__ void load(const T *p) {
+    if (kWords == 4)
+      *reinterpret_cast<uint4 *>(u) = *reinterpret_cast<const uint4 *>(p);
+    else
+      *reinterpret_cast<uint2 *>(u) = *reinterpret_cast<const uint2 *>(p);
   }
-}
-
-// Element index of the first and second member of pair q inside a head.
-__device__ __forceinline__ int2 pair_at(const RotaryParams &p, int q) {
-  int a = 0;
-  while (a + 1 < p.axes && q >= p.first_pair[a + 1]) ++a;
-  const int i = q - p.first_pair[a], base = 2 * p.first_pair[a];
-  return p.interleaved ? make_int2(base + 2 * i, base + 2 * i + 1)
-                       : make_int2(base + i, base + i + (p.dims[a] >> 1));
-}
-
-// One pair per thread; any alignment.
-template <typename T, bool kBackward>
-__global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant__ RotaryParams p) {
-  extern __shared__ float2 cs[];
-  const int64_t tiles = (p.N + kTile - 1) / kTile;
-  const int64_t b = blockIdx.x / tiles, t0 = blockIdx.x % tiles * kTile;
-  const int nt = (int)(p.N - t0 < kTile ? p.N - t0 : kTile);
-  stage_angles(p, b, t0, nt, cs);
-  __syncthreads();
-  const int D = p.D, half = D / 2;  // pairs, then the rest of the head two by two
-  const int64_t heads = p.H + 2 * p.Hk;
-  for (int64_t i = threadIdx.x; i < nt * heads * half; i += kThreads) {
-    const int q = (int)(i % half);
-    const int64_t h = i / half % heads;
-    const int t = (int)(i / (half * heads));
-    const int64_t n = t0 + t;
-    int2 e = make_int2(2 * q, 2 * q + 1);
-    float2 turn = make_float2(1.0f, 0.0f);
-    if (h < p.H + p.Hk && q < p.pairs) {
-      e = pair_at(p, q);
-      turn = cs[t * p.pairs + q];
-    }
-    const int64_t fused = ((b * p.N + n) * heads + h) * D;
-    T *head;
-    int64_t step = 1;
-    if (h < p.H) {
-      head = static_cast<T *>(p.q) + ((b * p.H + h) * p.N + n) * D;
-    } else if (h < p.H + p.Hk) {
-      head = static_cast<T *>(p.k) + ((b * p.Hk + h - p.H) * p.N + n) * D;
-    } else if (p.v_transposed) {
-      head = static_cast<T *>(p.v) + (b * p.Hk + h - p.H - p.Hk) * D * p.N + n;
-      step = p.N;
-    } else {
-      head = static_cast<T *>(p.v) + ((b * p.Hk + h - p.H - p.Hk) * p.N + n) * D;
-    }
-    T *fu = static_cast<T *>(p.qkv) + fused + e.x, *fv = static_cast<T *>(p.qkv) + fused + e.y;
-    T *hu = head + e.x * step, *hv = head + e.y * step;
-    if (h >= p.H + p.Hk || q >= p.pairs) {  // copied bit for bit
-      if (kBackward) {
-        *fu = *hu;
-        *fv = *hv;
+  __device__ __forceinline__ void store(T *p) const {
+    if (kWords == 4)
+      *reinterpret_cast<uint4 *>(p) = *reinterpret_cast<const uint4 *>(u);
+    else
+      *reinterpret_cast<uint2 *>(p) = *reinterpret_cast<const uint2 *>(u);
+  }
+  __device__ __forceinline__ void get(float *v) const {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) {
+      if constexpr (sizeof(T) == 4) {
+        v[i] = __uint_as_float(u[i]);
       } else {
-        *hu = *fu;
-        *hv = *fv;
+        const float2 f = unpack2<T>(u[i]);
+        v[2 * i] = f.x;
+        v[2 * i + 1] = f.y;
       }
-      continue;
     }
-    const float u = to_f32(kBackward ? *hu : *fu), v = to_f32(kBackward ? *hv : *fv);
-    const T ru = from_f32<T>(__fmaf_rn(u, turn.x, -v * turn.y));
-    const T rv = from_f32<T>(__fmaf_rn(v, turn.x, u * turn.y));
-    if (kBackward) {
-      *fu = ru;
-      *fv = rv;
+  }
+  // word i from its elements v
+  static __device__ __forceinline__ uint32_t word(const float *v, int i) {
+    if constexpr (sizeof(T) == 4)
+      return __float_as_uint(v[i]);
+    else
+      return pack2<T>(v[2 * i], v[2 * i + 1]);
+  }
+};
+template <typename T> struct Piece<T, 1> {
+  T u[1];
+  __device__ __forceinline__ void load(const T *p) { u[0] = *p; }
+  __device__ __forceinline__ void store(T *p) const { *p = u[0]; }
+};
+
+// Element e of a head: its axis, pair, partner and whether it is the pair's
+// second member; false past the axes.
+__device__ __forceinline__ bool place(const RotaryParams &p, int e, int &a, int &i, int &partner,
+                                      bool &second) {
+  if (e >= 2 * p.pairs) return false;
+  a = 0;
+  while (a + 1 < p.axes && e >= 2 * p.first_pair[a + 1]) ++a;
+  const int o = e - 2 * p.first_pair[a], half = p.dims[a] >> 1;
+  if (p.interleaved) {
+    i = o >> 1;
+    second = o & 1;
+    partner = e ^ 1;
+  } else {
+    second = o >= half;
+    i = second ? o - half : o;
+    partner = second ? e - half : e + half;
+  }
+  return true;
+}
+
+// x turned: x cos + partner (-+ sin); words that stay are x's bits.
+template <typename T, int V, bool kInterleaved>
+__device__ __forceinline__ Piece<T, V> turned(const Piece<T, V> &x, const Piece<T, V> &o,
+                                              const float (&c)[V], const float (&s)[V],
+                                              uint32_t mask) {
+  Piece<T, V> r;
+  if constexpr (V == 1) {
+    r.u[0] = mask ? from_f32<T>(__fmaf_rn(to_f32(x.u[0]), c[0], to_f32(o.u[0]) * s[0])) : x.u[0];
+  } else {
+    float v[V], w[V];
+    x.get(v);
+    if (kInterleaved) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) w[i] = v[i ^ 1];
     } else {
-      *hu = ru;
-      *hv = rv;
+      o.get(w);
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = __fmaf_rn(v[i], c[i], w[i] * s[i]);
+    constexpr int kPer = 4 / (int)sizeof(T);  // elements per word: a pair's, or one
+#pragma unroll
+    for (int i = 0; i < V / kPer; ++i)
+      r.u[i] = (mask >> (i * kPer)) & 1 ? Piece<T, V>::word(v, i) : x.u[i];
+  }
+  return r;
+}
+
+template <typename T, int V, bool kInterleaved, bool kBackward>
+__device__ __forceinline__ void turn_heads(const RotaryParams &p, uint32_t block) {
+  const int per = p.D / V;  // pieces of a head row
+  const uint32_t id = (block / p.splits) * kThreads + threadIdx.x;  // of B N per pieces
+  const uint32_t tok = p.per.quotient(id);
+  if (tok >= (uint32_t)(p.B * p.N)) return;
+  const uint32_t b = p.tokens.quotient(tok), n = tok - b * (uint32_t)p.N;
+  const int e0 = (int)(id - tok * per) * V;
+  const int heads = (int)(p.H + 2 * p.Hk), turning = (int)(p.H + p.Hk);
+  const int all = p.v_transposed ? turning : heads;
+  const int first = (int)(block % p.splits) * p.heads_per;
+  const int last = first + p.heads_per < all ? first + p.heads_per : all;
+
+  float c[V], s[V];
+  uint32_t mask = 0;
+  int partner = e0;
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    int a, i, o;
+    bool second = false;
+    float2 cs = make_float2(1.0f, 0.0f);
+    if (place(p, e0 + j, a, i, o, second)) {
+      if (angle_of(p, p.pos_batched ? tok : n, a, i, cs)) mask |= 1u << j;
+      if (j == 0) partner = o;
+    }
+    c[j] = cs.x;
+    s[j] = second != kBackward ? cs.y : -cs.y;  // the first member subtracts
+  }
+  const bool fetch = (!kInterleaved || V == 1) && mask != 0;
+
+  T *const fused = static_cast<T *>(p.qkv) + (int64_t)tok * heads * p.D;
+  for (int h0 = first; h0 < last; h0 += kAtOnce) {
+    Piece<T, V> x[kAtOnce], o[kAtOnce];
+    T *to[kAtOnce], *from[kAtOnce];
+#pragma unroll
+    for (int q = 0; q < kAtOnce; ++q) {
+      const int h = h0 + q < last ? h0 + q : last - 1;
+      T *base;
+      int hh = h;
+      int64_t count = p.H;
+      if (h < p.H) {
+        base = static_cast<T *>(p.q);
+      } else {
+        base = static_cast<T *>(h < turning ? p.k : p.v);
+        hh = h - (int)(h < turning ? p.H : turning);
+        count = p.Hk;
+      }
+      T *const head = base + (((int64_t)b * count + hh) * p.N + n) * p.D;
+      T *const row = fused + (int64_t)h * p.D;
+      from[q] = kBackward ? head : row;
+      to[q] = kBackward ? row : head;
+      x[q].load(from[q] + e0);
+      if (fetch && h < turning) o[q].load(from[q] + partner);
+    }
+#pragma unroll
+    for (int q = 0; q < kAtOnce; ++q) {
+      if (h0 + q >= last) break;
+      if (mask != 0 && h0 + q < turning)
+        turned<T, V, kInterleaved>(x[q], o[q], c, s, mask).store(to[q] + e0);
+      else
+        x[q].store(to[q] + e0);
     }
   }
 }
 
-template <typename T>
-cudaError_t launch(const RotaryParams &p, cudaStream_t s) {
-  const int64_t blocks = p.B * ((p.N + kTile - 1) / kTile);
-  const size_t smem = (size_t)kTile * p.pairs * sizeof(float2);  // <= 32 KB (D <= 256)
-  if (p.inverse)
-    rotary_kernel<T, true><<<(unsigned)blocks, kThreads, smem, s>>>(p);
+// v of one head, kTile tokens: token rows of the fused tensor <-> [D, N].
+template <typename T, bool kBackward>
+__device__ __forceinline__ void transpose_tile(const RotaryParams &p, uint32_t block, T *tile) {
+  const uint32_t tiles = (uint32_t)((p.N + kTile - 1) / kTile);
+  const int64_t bh = block / tiles, b = bh / p.Hk, h = bh % p.Hk;
+  const int64_t t0 = (int64_t)(block % tiles) * kTile;
+  const int nt = (int)(p.N - t0 < kTile ? p.N - t0 : kTile);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, D = p.D, ld = D + 1;
+  const int64_t heads = p.H + 2 * p.Hk;
+  T *const fused = static_cast<T *>(p.qkv) + ((b * p.N + t0) * heads + p.H + p.Hk + h) * D;
+  T *const flat = static_cast<T *>(p.v) + bh * D * p.N + t0;
+  if (kBackward) {
+    for (int d = warp; d < D; d += 8)
+      for (int t = lane; t < nt; t += 32) tile[t * ld + d] = flat[d * p.N + t];
+  } else {
+    for (int t = warp; t < nt; t += 8)
+      for (int d = lane; d < D; d += 32) tile[t * ld + d] = fused[t * heads * D + d];
+  }
+  __syncthreads();
+  if (kBackward) {
+    for (int t = warp; t < nt; t += 8)
+      for (int d = lane; d < D; d += 32) fused[t * heads * D + d] = tile[t * ld + d];
+  } else {
+    for (int d = warp; d < D; d += 8)
+      for (int t = lane; t < nt; t += 32) flat[d * p.N + t] = tile[t * ld + d];
+  }
+}
+
+template <typename T, int V, bool kInterleaved, bool kBackward>
+__global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant__ RotaryParams p) {
+  extern __shared__ __align__(16) unsigned char smem[];
+  if (blockIdx.x < p.turn_blocks)
+    turn_heads<T, V, kInterleaved, kBackward>(p, blockIdx.x);
   else
-    rotary_kernel<T, false><<<(unsigned)blocks, kThreads, smem, s>>>(p);
+    transpose_tile<T, kBackward>(p, blockIdx.x - p.turn_blocks, reinterpret_cast<T *>(smem));
+}
+
+template <typename T, int V, bool kInterleaved>
+cudaError_t launch_v(RotaryParams p, cudaStream_t s) {
+  p.per = FastDiv((uint32_t)(p.D / V));
+  p.tokens = FastDiv((uint32_t)p.N);
+  const int all = (int)(p.H + p.Hk + (p.v_transposed ? 0 : p.Hk));
+  const int64_t token_blocks = (p.B * p.N * (p.D / V) + kThreads - 1) / kThreads;
+  // as many heads per thread as leave six blocks for each of the 148 SMs
+  const int64_t fit = all * token_blocks / (148 * 6);
+  p.heads_per = (int)(fit < 1 ? 1 : fit > all ? all : fit);
+  p.splits = (uint32_t)((all + p.heads_per - 1) / p.heads_per);
+  const int64_t turn = token_blocks * p.splits;
+  const int64_t tiles = p.v_transposed ? p.B * p.Hk * ((p.N + kTile - 1) / kTile) : 0;
+  if (turn + tiles > INT32_MAX) return cudaErrorInvalidConfiguration;
+  p.turn_blocks = (uint32_t)turn;
+  const size_t smem = p.v_transposed ? (size_t)kTile * (p.D + 1) * sizeof(T) : 0;  // <= 66 KB
+  auto kern = p.inverse ? rotary_kernel<T, V, kInterleaved, true>
+                        : rotary_kernel<T, V, kInterleaved, false>;
+  if (smem > 48 * 1024) {
+    const cudaError_t e =
+        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return e;
+  }
+  kern<<<(unsigned)(turn + tiles), kThreads, smem, s>>>(p);
   return cudaGetLastError();
+}
+
+// Whether pieces of V elements divide every head row and, with the two members
+// of a pair half a section apart, every half section (a piece's partners are
+// then a piece).  (t, h, w) sections of 16, 24, 24 take 8 bytes of 16-bit types.
+template <typename T, int V> bool pieces(const RotaryParams &p) {
+  const uintptr_t at = reinterpret_cast<uintptr_t>(p.qkv) | reinterpret_cast<uintptr_t>(p.q) |
+                       reinterpret_cast<uintptr_t>(p.k) | reinterpret_cast<uintptr_t>(p.v);
+  bool ok = p.D % V == 0 && at % (V * sizeof(T)) == 0;
+  if (!p.interleaved)
+    for (int a = 0; a < p.axes; ++a) ok = ok && (p.dims[a] / 2) % V == 0;
+  return ok;
+}
+template <typename T, bool kInterleaved>
+cudaError_t launch_order(const RotaryParams &p, cudaStream_t s) {
+  constexpr int V = kVec16<T>;
+  if (pieces<T, V>(p)) return launch_v<T, V, kInterleaved>(p, s);
+  if (pieces<T, V / 2>(p)) return launch_v<T, V / 2, kInterleaved>(p, s);
+  return launch_v<T, 1, kInterleaved>(p, s);
+}
+template <typename T> cudaError_t launch(const RotaryParams &p, cudaStream_t s) {
+  return p.interleaved ? launch_order<T, true>(p, s) : launch_order<T, false>(p, s);
 }
 
 }  // namespace

@@ -5,6 +5,7 @@
 #include <stdint.h>
 
 #include "../../include/scmp_b200.h"
+#include "mx_common.cuh"
 
 namespace scmp {
 
@@ -18,6 +19,11 @@ struct RotaryParams {
   int dims[SCMP_MAX_AXES], sizes[SCMP_MAX_AXES], first_pair[SCMP_MAX_AXES];
   int64_t table_at[SCMP_MAX_AXES];  // first entry of each axis
   bool pos_batched, interleaved, v_transposed, inverse;
+  // set by the launcher: pieces per head row, tokens per sample, the blocks that
+  // turn heads (each a split of them) in front of the transposed tiles
+  FastDiv per{1}, tokens{1};
+  int heads_per;
+  uint32_t splits, turn_blocks;
 };
 cudaError_t launch_rotary(const RotaryParams &p, int dtype, cudaStream_t s);
 
