@@ -246,6 +246,12 @@ typedef struct scmp_mx_matmul_args {
   int32_t reserved;
 } scmp_mx_matmul_args;
 SCMP_API int scmp_mx_matmul(const scmp_mx_matmul_args *args, void *stream);
+/* The same for an A that is not quantised yet: x, M rows of K elements of
+ * x_dtype, `ld` elements apart, quantised (nvfp4: with tensor exponent 0, so
+ * scale_exp is B's) into the buffers at args->a and args->a_scales, which the
+ * call writes. */
+SCMP_API int scmp_mx_linear(const void *x, int x_dtype, int64_t ld,
+                            const scmp_mx_matmul_args *args, void *stream);
 
 /* ---- Gated residual add with the norms around it (the `x + ls1(attn(...))`
  * and `norm2(x)` steps of the block forward of cls/sc_attention_patch.py:459-636,

@@ -1,0 +1,33 @@
+"""Calls into the engine library on a tensor's device and current stream."""
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+
+DTYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # enum scmp_dtype
+
+try:  # the stream's handle without a Stream object around it
+    _raw_stream = torch._C._cuda_getCurrentRawStream
+except AttributeError:  # a CPU build of torch
+    def _raw_stream(index: int) -> int:
+        return torch.cuda.current_stream(index).cuda_stream
+
+
+def call(fn, index: int, *args) -> None:
+    """``fn(*args, stream)`` on CUDA device ``index`` and its current stream;
+    raises on a non-zero status."""
+    if torch.cuda.current_device() == index:
+        status = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            status = fn(*args, _raw_stream(index))
+    if status:
+        _lib.check(status)
+
+
+def dtype_code(dtype: torch.dtype, what: str) -> int:
+    code = DTYPE.get(dtype)
+    if code is None:
+        raise TypeError(f"{what} must be float32, bfloat16 or float16, got {dtype}")
+    return code

@@ -51,6 +51,7 @@ EXPORTED_SYMBOLS = (
     "scmp_mx_quantize",
     "scmp_mx_dequantize",
     "scmp_mx_matmul",
+    "scmp_mx_linear",
     "scmp_residual_norm",
     "scmp_residual_norm_bwd_workspace",
     "scmp_residual_norm_bwd",
@@ -216,6 +217,8 @@ def load() -> ctypes.CDLL:
         lib.scmp_mx_quantize.restype = ctypes.c_int
         lib.scmp_mx_dequantize.argtypes = [ptr, ptr, i64, i64, i32, i32, ptr, i32, ptr]
         lib.scmp_mx_dequantize.restype = ctypes.c_int
+        lib.scmp_mx_linear.argtypes = [ptr, i32, i64, ctypes.POINTER(MxMatmulArgs), ptr]
+        lib.scmp_mx_linear.restype = ctypes.c_int
         for name, args in (("scmp_mx_matmul", MxMatmulArgs), ("scmp_residual_norm", NormArgs),
                            ("scmp_residual_norm_bwd", NormBwdArgs),
                            ("scmp_split_qkv_rotary", RotaryArgs)):

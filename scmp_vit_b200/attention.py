@@ -22,6 +22,7 @@ import torch
 import torch.nn as nn
 
 from . import sc_linear as _scl
+from ._call import DTYPE, call
 from .mp import (
     AdaptiveMPConfig,
     AutoMPBudgetLogger,
@@ -400,6 +401,9 @@ class RotaryAxes(nn.Module):
         if not base > 0:
             raise ValueError(f"base must be positive, got {base}")
         self.dims, self.sizes, self.interleaved = dims, sizes, bool(interleaved)
+        pad = [0] * (_lib.MAX_AXES - len(dims))
+        self.c_dims = (ctypes.c_int32 * _lib.MAX_AXES)(*dims, *pad)
+        self.c_sizes = (ctypes.c_int32 * _lib.MAX_AXES)(*sizes, *pad)
         parts = []
         for d, n, f in zip(dims, sizes, scales):
             freq = torch.exp(torch.arange(0, d, 2, dtype=torch.float64, device=device)
@@ -416,37 +420,31 @@ def _rotary_launch(qkv, q, k, v, axes: RotaryAxes, table, pos, v_transposed: boo
     """One ``scmp_split_qkv_rotary`` call on contiguous storages."""
     from . import _lib
     B, H, N, D = q.shape
-    a = _lib.RotaryArgs()
-    a.abi_version = _lib.ABI_VERSION
-    a.dtype = _lib.DTYPE[str(qkv.dtype)]
-    a.qkv, a.q, a.k, a.v = (t.data_ptr() for t in (qkv, q, k, v))
-    a.table, a.pos = table.data_ptr(), pos.data_ptr()
-    a.B, a.N, a.H, a.Hk, a.D = B, N, H, k.shape[1], D
-    a.axes = len(axes.dims)
-    for i, (d, n) in enumerate(zip(axes.dims, axes.sizes)):
-        a.dims[i], a.sizes[i] = d, n
-    a.pos_batched = int(pos.dim() == 3)
-    a.interleaved, a.v_transposed, a.inverse = axes.interleaved, v_transposed, inverse
-    with torch.cuda.device(qkv.device):
-        stream = torch.cuda.current_stream(qkv.device).cuda_stream
-        _lib.check(_lib.load().scmp_split_qkv_rotary(ctypes.byref(a), ctypes.c_void_p(stream)))
+    args = _lib.RotaryArgs(
+        _lib.ABI_VERSION, DTYPE[qkv.dtype], qkv.data_ptr(), q.data_ptr(), k.data_ptr(),
+        v.data_ptr(), table.data_ptr(), pos.data_ptr(), B, N, H, k.shape[1], D, len(axes.dims),
+        axes.c_dims, axes.c_sizes, pos.dim() == 3, axes.interleaved, v_transposed, inverse)
+    call(_lib.load().scmp_split_qkv_rotary, qkv.get_device(), args)
+
+
+def _split_rotary(src, pos, table, axes, H, Hk, transpose_v):
+    B, N, width = src.shape
+    D = width // (H + 2 * Hk)
+    q = src.new_empty(B, H, N, D)
+    k = src.new_empty(B, Hk, N, D)
+    v = src.new_empty(B, Hk, D, N) if transpose_v else src.new_empty(B, Hk, N, D)
+    _rotary_launch(src, q, k, v, axes, table, pos, transpose_v, False)
+    return q, k, v.transpose(-1, -2) if transpose_v else v
 
 
 class _SplitQkvRotary(torch.autograd.Function):
     @staticmethod
     def forward(ctx, qkv, pos, table, axes, H, Hk, transpose_v):
-        B, N, width = qkv.shape
-        D = width // (H + 2 * Hk)
-        src = qkv.contiguous()
-        q = qkv.new_empty(B, H, N, D)
-        k = qkv.new_empty(B, Hk, N, D)
-        v = qkv.new_empty(B, Hk, D, N) if transpose_v else qkv.new_empty(B, Hk, N, D)
-        _rotary_launch(src, q, k, v, axes, table, pos, transpose_v, False)
-        ctx.axes, ctx.shape = axes, (B, N, width)
+        ctx.axes, ctx.shape = axes, qkv.shape
         # the table itself: axes that move to another device in between leave
         # this call's gradient alone
         ctx.save_for_backward(pos, table)
-        return q, k, v.transpose(-1, -2) if transpose_v else v
+        return _split_rotary(qkv.contiguous(), pos, table, axes, H, Hk, transpose_v)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -488,18 +486,22 @@ def split_qkv_rotary(qkv: torch.Tensor, num_heads: int, axes: RotaryAxes, pos: t
                          f"Hk={Hk}")
     B, N, width = qkv.shape
     D = width // (H + 2 * Hk)
+    index = qkv.get_device()
     if D < 2 or D % 2 or D > 256 or sum(axes.dims) > D:
         raise ValueError(f"the head size must be even, at most 256 and hold the axes' dims "
                          f"{axes.dims}, got {D}")
     n_axes = len(axes.dims)
-    if (pos.dtype != torch.int32 or pos.device != qkv.device
+    if (pos.dtype != torch.int32 or pos.get_device() != index
             or tuple(pos.shape) not in ((N, n_axes), (B, N, n_axes))):
         raise ValueError(f"pos must be int32 [{N}, {n_axes}] or [{B}, {N}, {n_axes}] on "
                          f"{qkv.device}, got {pos.dtype} {tuple(pos.shape)} {pos.device}")
-    if axes.table_bits.device != qkv.device:
-        raise ValueError(f"axes are on {axes.table_bits.device}, qkv on {qkv.device}")
-    return _SplitQkvRotary.apply(qkv, pos.contiguous(), axes.table_bits, axes, H, Hk,
-                                 bool(transpose_v))
+    table = axes.table_bits
+    if table.get_device() != index:
+        raise ValueError(f"axes are on {table.device}, qkv on {qkv.device}")
+    pos, transpose_v = pos.contiguous(), bool(transpose_v)
+    if torch.is_grad_enabled() and qkv.requires_grad:
+        return _SplitQkvRotary.apply(qkv, pos, table, axes, H, Hk, transpose_v)
+    return _split_rotary(qkv.contiguous(), pos, table, axes, H, Hk, transpose_v)
 
 
 def make_sc_attention_forward(sc_prec: int, sc_av: bool, sc_qk: bool = True,

@@ -143,6 +143,17 @@ int scmp_mx_matmul(const scmp_mx_matmul_args *args, void *stream) {
   return SCMP_OK;
 }
 
+int scmp_mx_linear(const void *x, int x_dtype, int64_t ld, const scmp_mx_matmul_args *args,
+                   void *stream) {
+  set_last_error("");
+  if (!args) return fail(SCMP_EINVAL, "args is NULL");
+  if (args->M == 0 || args->N == 0) return scmp_mx_matmul(args, stream);
+  const int rc = scmp_mx_quantize(x, x_dtype, args->M, args->K, ld, args->fmt, 0,
+                                  const_cast<void *>(args->a), const_cast<void *>(args->a_scales),
+                                  stream);
+  return rc != SCMP_OK ? rc : scmp_mx_matmul(args, stream);
+}
+
 int scmp_residual_norm(const scmp_norm_args *args, void *stream) {
   set_last_error("");
   if (!args) return fail(SCMP_EINVAL, "args is NULL");

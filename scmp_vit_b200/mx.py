@@ -20,7 +20,6 @@ refused.  There is no CPU path: CPU tensors raise.
 """
 from __future__ import annotations
 
-import ctypes
 import math
 from typing import Optional, Sequence, Union
 
@@ -28,15 +27,9 @@ import torch
 import torch.nn as nn
 
 from . import _lib
+from ._call import call, dtype_code
 
 __all__ = ["MXTensor", "mx_quantize", "mx_matmul", "MXLinear", "tensor_scale_exp"]
-
-
-def _dtype_code(dtype: torch.dtype, what: str) -> int:
-    code = _lib.DTYPE.get(str(dtype))
-    if code is None:
-        raise TypeError(f"{what} must be float32, bfloat16 or float16, got {dtype}")
-    return code
 
 
 def _check_fmt(fmt: str) -> str:
@@ -46,49 +39,71 @@ def _check_fmt(fmt: str) -> str:
 
 
 def _no_grad_wanted(name: str, *tensors) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError(f"{name} has no gradient; call it under torch.no_grad() or on "
-                           "detached inputs")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError(f"{name} has no gradient; call it under torch.no_grad() or on "
+                                   "detached inputs")
 
 
-def _stream(dev: torch.device) -> ctypes.c_void_p:
-    return ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
+def _sizes(rows: int, K: int, fmt: str):
+    """Bytes of codes and of scales (``scmp_mx_data_size``, ``scmp_mx_scale_size``)."""
+    kp = (K + 31) // 32 * 32
+    groups = -(-kp // (4 * _lib.MX_BLOCK[fmt]))
+    return rows * kp // 2, (rows + 127) // 128 * groups * 512
 
 
 class MXTensor:
     """A quantised tensor ``[..., K]``: codes and block scales on the GPU.
 
-    ``data`` and ``scales`` have the layout of ``scmp_mx_quantize`` (rows are
-    the leading dimensions flattened); ``dtype`` is the type of the tensor it
-    was made from, which products of it come out in by default."""
+    ``data`` and ``scales`` (uint8) have the layout of ``scmp_mx_quantize``
+    (rows are the leading dimensions flattened); ``dtype`` is the type of the
+    tensor it was made from, which products of it come out in by default."""
+
+    __slots__ = ("shape", "rows", "fmt", "scale_exp", "dtype", "_data", "_scales", "_buf",
+                 "data_ptr", "scales_ptr", "index")
 
     def __init__(self, data: torch.Tensor, scales: torch.Tensor, shape: Sequence[int], fmt: str,
                  scale_exp: int = 0, dtype: torch.dtype = torch.float32):
-        self.data = data
-        self.scales = scales
-        self.shape = torch.Size(shape)
-        self.fmt = _check_fmt(fmt)
-        self.scale_exp = int(scale_exp)
-        self.dtype = dtype
-        lib = _lib.load()
-        rows, K = self.rows, self.shape[-1]
-        for t, size, what in ((data, lib.scmp_mx_data_size(rows, K, _lib.MX_FORMAT[fmt]), "data"),
-                              (scales, lib.scmp_mx_scale_size(rows, K, _lib.MX_FORMAT[fmt]),
-                               "scales")):
+        shape = torch.Size(shape)
+        want = _sizes(math.prod(shape[:-1]), shape[-1], _check_fmt(fmt))
+        for t, size, what in ((data, want[0], "data"), (scales, want[1], "scales")):
             if t.dtype != torch.uint8 or not t.is_contiguous() or t.numel() != size:
-                raise ValueError(f"{what} must be {size} contiguous bytes for {tuple(self.shape)}")
+                raise ValueError(f"{what} must be {size} contiguous bytes for {tuple(shape)}")
+        if data.device != scales.device:
+            raise ValueError(f"data on {data.device}, scales on {scales.device}")
+        if data.data_ptr() % 16 or scales.data_ptr() % 16:
+            raise ValueError("data and scales must be 16-byte aligned")
+        self._set(data, scales, None, data.data_ptr(), scales.data_ptr(), data.get_device(), shape,
+                  fmt, scale_exp, dtype)
+
+    def _set(self, data, scales, buf, data_ptr, scales_ptr, index, shape, fmt, scale_exp, dtype):
+        self._data, self._scales, self._buf = data, scales, buf
+        self.data_ptr, self.scales_ptr, self.index = data_ptr, scales_ptr, index
+        self.shape, self.fmt, self.scale_exp, self.dtype = shape, fmt, int(scale_exp), dtype
+        self.rows = math.prod(shape[:-1])
+        return self
 
     @property
-    def rows(self) -> int:
-        return math.prod(self.shape[:-1])
+    def data(self) -> torch.Tensor:
+        if self._data is None:
+            self._data = self._buf[:_sizes(self.rows, self.shape[-1], self.fmt)[0]]
+        return self._data
+
+    @property
+    def scales(self) -> torch.Tensor:
+        if self._scales is None:
+            at = self.scales_ptr - self.data_ptr
+            self._scales = self._buf[at:at + _sizes(self.rows, self.shape[-1], self.fmt)[1]]
+        return self._scales
 
     @property
     def device(self) -> torch.device:
-        return self.data.device
+        return (self._data if self._buf is None else self._buf).device
 
     @property
     def is_cuda(self) -> bool:
-        return self.data.is_cuda
+        return self.index >= 0
 
     def dim(self) -> int:
         return len(self.shape)
@@ -99,22 +114,20 @@ class MXTensor:
         shape = torch.empty(self.shape, device="meta").reshape(*shape).shape
         if shape[-1] != self.shape[-1]:
             raise ValueError("an MXTensor keeps its last dimension")
-        return MXTensor(self.data, self.scales, shape, self.fmt, self.scale_exp, self.dtype)
+        return MXTensor.__new__(MXTensor)._set(
+            self._data, self._scales, self._buf, self.data_ptr, self.scales_ptr, self.index, shape,
+            self.fmt, self.scale_exp, self.dtype)
 
-    @torch.no_grad()
     def dequantize(self, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
         """The values that the codes stand for, ``[..., K]`` (default: the
         type the tensor was made from; exact in it unless they leave its range)."""
         dtype = self.dtype if dtype is None else dtype
-        code = _dtype_code(dtype, "dtype")
-        if not self.is_cuda:
+        code = dtype_code(dtype, "dtype")
+        if self.index < 0:
             raise RuntimeError("dequantize runs on the CUDA engine only (no CPU path)")
         out = torch.empty(self.shape, dtype=dtype, device=self.device)
-        with torch.cuda.device(self.device):
-            _lib.check(_lib.load().scmp_mx_dequantize(
-                self.data.data_ptr(), self.scales.data_ptr(), self.rows, self.shape[-1],
-                _lib.MX_FORMAT[self.fmt], self.scale_exp, out.data_ptr(), code,
-                _stream(self.device)))
+        call(_lib.load().scmp_mx_dequantize, self.index, self.data_ptr, self.scales_ptr, self.rows,
+             self.shape[-1], _lib.MX_FORMAT[self.fmt], self.scale_exp, out.data_ptr(), code)
         return out
 
     def __repr__(self) -> str:
@@ -122,25 +135,36 @@ class MXTensor:
                 f"scale_exp={self.scale_exp}, dtype={self.dtype}, device={self.device})")
 
 
-def mx_empty(shape: Sequence[int], fmt: str, device: torch.device, dtype: torch.dtype,
+def mx_empty(shape: torch.Size, fmt: str, device: torch.device, dtype: torch.dtype,
              scale_exp: int = 0) -> MXTensor:
-    """An MXTensor whose codes and scales are still to be written."""
-    lib = _lib.load()
-    rows, K = math.prod(shape[:-1]), shape[-1]
-    code = _lib.MX_FORMAT[_check_fmt(fmt)]
-    data = torch.empty(lib.scmp_mx_data_size(rows, K, code), dtype=torch.uint8, device=device)
-    scales = torch.empty(lib.scmp_mx_scale_size(rows, K, code), dtype=torch.uint8, device=device)
-    return MXTensor(data, scales, shape, fmt, scale_exp, dtype)
+    """An MXTensor whose codes and scales (one allocation) are still to be written."""
+    data, scales = _sizes(math.prod(shape[:-1]), shape[-1], _check_fmt(fmt))
+    at = (data + 255) & ~255
+    buf = torch.empty(at + scales, dtype=torch.uint8, device=device)
+    ptr = buf.data_ptr()
+    return MXTensor.__new__(MXTensor)._set(None, None, buf, ptr, ptr + at, buf.get_device(), shape,
+                                           fmt, scale_exp, dtype)
 
 
-def _as_rows(x: torch.Tensor) -> torch.Tensor:
-    """``[rows, K]`` with contiguous rows a fixed distance apart (a view where
-    the strides allow it)."""
+def _rows_of(x: torch.Tensor):
+    """(x or a copy of it, row distance) with contiguous rows a fixed distance apart."""
     K = x.shape[-1]
-    x2 = x.reshape(-1, K)
-    if K > 1 and x2.stride(1) != 1 or x2.shape[0] > 1 and x2.stride(0) < K:
+    if x.is_contiguous():
+        return x, K
+    x2 = x.detach().reshape(-1, K)
+    if (K > 1 and x2.stride(1) != 1) or (x2.shape[0] > 1 and x2.stride(0) < K):
         x2 = x2.contiguous()
-    return x2
+    return x2, (x2.stride(0) if x2.shape[0] > 1 else K)
+
+
+def _check_input(x: torch.Tensor, name: str) -> int:
+    code = dtype_code(x.dtype, "x")
+    if not x.is_cuda:
+        raise RuntimeError(f"{name} runs on the CUDA engine only (no CPU path); got {x.device}")
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"{name} needs a last dimension of at least 1, got {tuple(x.shape)}")
+    _no_grad_wanted(name, x)
+    return code
 
 
 def mx_quantize(x: torch.Tensor, fmt: str = "mxfp4", *, scale_exp: int = 0) -> MXTensor:
@@ -148,21 +172,12 @@ def mx_quantize(x: torch.Tensor, fmt: str = "mxfp4", *, scale_exp: int = 0) -> M
     its last dimension.  ``scale_exp`` is nvfp4's power-of-two tensor scale
     (``tensor_scale_exp`` gives the one that suits a tensor; 0 suits normalised
     activations)."""
-    fmt = _check_fmt(fmt)
-    code = _dtype_code(x.dtype, "x")
-    if not x.is_cuda:
-        raise RuntimeError(f"mx_quantize runs on the CUDA engine only (no CPU path); got {x.device}")
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise ValueError(f"mx_quantize needs a last dimension of at least 1, got {tuple(x.shape)}")
-    _no_grad_wanted("mx_quantize", x)
+    _check_fmt(fmt)
+    code = _check_input(x, "mx_quantize")
     out = mx_empty(x.shape, fmt, x.device, x.dtype, scale_exp)
-    x2 = _as_rows(x.detach()) if out.rows else x
-    K = x.shape[-1]
-    ld = x2.stride(0) if out.rows > 1 else K
-    with torch.cuda.device(x.device):
-        _lib.check(_lib.load().scmp_mx_quantize(
-            x2.data_ptr(), code, out.rows, K, ld, _lib.MX_FORMAT[fmt], int(scale_exp),
-            out.data.data_ptr(), out.scales.data_ptr(), _stream(x.device)))
+    x, ld = _rows_of(x)
+    call(_lib.load().scmp_mx_quantize, out.index, x.data_ptr(), code, out.rows, out.shape[-1], ld,
+         _lib.MX_FORMAT[fmt], out.scale_exp, out.data_ptr, out.scales_ptr)
     return out
 
 
@@ -173,46 +188,52 @@ def mx_matmul(a: Union[torch.Tensor, MXTensor], b: MXTensor, *,
     ``[..., N]``: the exact products of the 4-bit values summed in fp32, the
     bias added, rounded once to ``out_dtype`` (default: a's type).  A plain
     ``a`` is quantised to ``b``'s format first (nvfp4 with tensor scale 1)."""
-    if not isinstance(b, MXTensor) or b.dim() != 2:
+    if not isinstance(b, MXTensor) or len(b.shape) != 2:
         raise TypeError("b must be a 2-D MXTensor [N, K]")
-    if not isinstance(a, MXTensor):
-        if a.device != b.device:
-            raise ValueError(f"operands on different devices: {a.device} vs {b.device}")
-        if a.dim() < 1 or a.shape[-1] != b.shape[-1]:
-            raise ValueError(f"inner-dim mismatch: a {tuple(a.shape)}, b {tuple(b.shape)}")
-        a = mx_quantize(a, b.fmt)
-    if a.device != b.device or not b.is_cuda:
-        raise ValueError(f"operands on different devices or on the CPU: {a.device} vs {b.device}")
-    if a.fmt != b.fmt:
-        raise ValueError(f"operands of different formats: {a.fmt} vs {b.fmt}")
+    if b.index < 0:
+        raise RuntimeError("mx_matmul runs on the CUDA engine only (no CPU path)")
     N, K = b.shape
-    if a.shape[-1] != K:
+    plain = not isinstance(a, MXTensor)
+    index = a.get_device() if plain else a.index
+    if index != b.index:
+        raise ValueError(f"operands on different devices: {a.device} vs {b.device}")
+    if len(a.shape) < 1 or a.shape[-1] != K:
         raise ValueError(f"inner-dim mismatch: a {tuple(a.shape)}, b {tuple(b.shape)}")
-    _no_grad_wanted("mx_matmul", bias)
-    shape = (*a.shape[:-1], N)
+    if plain:
+        x_code = _check_input(a, "mx_matmul")
+        qa = mx_empty(a.shape, b.fmt, a.device, a.dtype)
+    elif a.fmt != b.fmt:
+        raise ValueError(f"operands of different formats: {a.fmt} vs {b.fmt}")
+    else:
+        qa = a
+    shape = (*qa.shape[:-1], N)
     if out is None:
-        out = torch.empty(shape, dtype=a.dtype if out_dtype is None else out_dtype, device=b.device)
-    elif (tuple(out.shape) != shape or not out.is_contiguous() or out.device != b.device
-          or out_dtype not in (None, out.dtype)):
-        raise ValueError(f"out must be contiguous {shape} on {b.device} of out_dtype")
-    _no_grad_wanted("mx_matmul", out)
-    args = _lib.MxMatmulArgs()
-    args.abi_version = _lib.ABI_VERSION
-    args.fmt = _lib.MX_FORMAT[b.fmt]
-    args.a, args.a_scales = a.data.data_ptr(), a.scales.data_ptr()
-    args.b, args.b_scales = b.data.data_ptr(), b.scales.data_ptr()
-    args.M, args.N, args.K = a.rows, N, K
-    args.scale_exp = a.scale_exp + b.scale_exp
+        dtype = qa.dtype if out_dtype is None else out_dtype
+        out_code = dtype_code(dtype, "out")
+        out = torch.empty(shape, dtype=dtype, device=b.device)
+    else:
+        if (tuple(out.shape) != shape or not out.is_contiguous() or out.get_device() != index
+                or out_dtype not in (None, out.dtype)):
+            raise ValueError(f"out must be contiguous {shape} on {b.device} of out_dtype")
+        out_code = dtype_code(out.dtype, "out")
+    bias_code, bias_ptr = 0, None
     if bias is not None:
-        if bias.shape != (N,) or bias.device != b.device:
-            raise ValueError(f"bias must be [{N}] on {b.device}, got {tuple(bias.shape)}")
-        args.bias_dtype = _dtype_code(bias.dtype, "bias")
-        bias = bias.detach().contiguous()
-        args.bias = bias.data_ptr()
-    args.out_dtype = _dtype_code(out.dtype, "out")
-    args.out = out.data_ptr()
-    with torch.cuda.device(b.device):
-        _lib.check(_lib.load().scmp_mx_matmul(ctypes.byref(args), _stream(b.device)))
+        if bias.shape != (N,) or bias.get_device() != index:
+            raise ValueError(f"bias must be [{N}] on {b.device}, got {tuple(bias.shape)} on "
+                             f"{bias.device}")
+        bias_code = dtype_code(bias.dtype, "bias")
+        _no_grad_wanted("mx_matmul", bias)
+        bias = bias if bias.is_contiguous() else bias.detach().contiguous()
+        bias_ptr = bias.data_ptr()
+    _no_grad_wanted("mx_matmul", out)
+    args = _lib.MxMatmulArgs(_lib.ABI_VERSION, _lib.MX_FORMAT[b.fmt], qa.data_ptr, qa.scales_ptr,
+                             b.data_ptr, b.scales_ptr, qa.rows, N, K, qa.scale_exp + b.scale_exp,
+                             bias_code, bias_ptr, out.data_ptr(), out_code, 0)
+    if plain:
+        x, ld = _rows_of(a)
+        call(_lib.load().scmp_mx_linear, index, x.data_ptr(), x_code, ld, args)
+    else:
+        call(_lib.load().scmp_mx_matmul, index, args)
     return out
 
 
@@ -243,14 +264,16 @@ class MXLinear(nn.Module):
         self.fmt = fmt
         self.scale_exp = exp
         self.out_features, self.in_features = w.shape
-        self.register_buffer("data", q.data)
-        self.register_buffer("scales", q.scales)
+        self.register_buffer("data", q.data.clone())
+        self.register_buffer("scales", q.scales.clone())
         bias = linear.bias
         self.register_buffer("bias", None if bias is None else bias.detach().clone())
 
     def quantized_weight(self) -> MXTensor:
-        return MXTensor(self.data, self.scales, (self.out_features, self.in_features), self.fmt,
-                        self.scale_exp)
+        return MXTensor.__new__(MXTensor)._set(
+            self.data, self.scales, None, self.data.data_ptr(), self.scales.data_ptr(),
+            self.data.get_device(), torch.Size((self.out_features, self.in_features)), self.fmt,
+            self.scale_exp, torch.float32)
 
     def forward(self, x: Union[torch.Tensor, MXTensor]) -> torch.Tensor:
         return mx_matmul(x, self.quantized_weight(), bias=self.bias)

@@ -22,6 +22,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from ._call import DTYPE, call
 from .attention import make_sc_attention_forward
 from .head_aligned_comp import HeadAlignedSCLinear
 from .mp import SeededRandomMPConfig, quantile_counts, set_current_block_idx
@@ -88,129 +89,114 @@ def scale_residual(x: torch.Tensor, y: torch.Tensor, gamma: torch.Tensor,
     return out
 
 
-def _norm_inputs(x, y, weight, norm_bias, kind, gamma, gate, post_weight, post_bias):
-    """Checks ``residual_norm``'s arguments; returns the parameters' type."""
+_NORM_TYPES = (torch.float32, torch.bfloat16, torch.float16)
+
+
+def _check_norm(x, y, weight, norm_bias, kind, eps, gamma, gate, post_weight, post_bias) -> None:
+    """Refuses what ``residual_norm`` does not take."""
     if kind not in ("layer", "rms"):
         raise ValueError(f"unknown norm kind {kind!r}")
+    if not (isinstance(eps, (int, float)) and eps >= 0):
+        raise ValueError(f"eps must be >= 0, got {eps!r}")
     if not x.is_cuda:
         raise RuntimeError(f"residual_norm runs on the CUDA engine only (no CPU path); got {x.device}")
-    if x.dtype not in (torch.float32, torch.bfloat16, torch.float16):
-        raise TypeError(f"x must be float32, bfloat16 or float16, got {x.dtype}")
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise ValueError(f"x needs a last dimension of at least 1, got {tuple(x.shape)}")
-    C = x.shape[-1]
+    dtype = x.dtype
+    if dtype not in _NORM_TYPES:
+        raise TypeError(f"x must be float32, bfloat16 or float16, got {dtype}")
+    shape = x.shape
+    if not shape or not 1 <= shape[-1] <= 8192:
+        raise ValueError(f"residual_norm takes rows of 1 to 8192 values, got {tuple(shape)}")
+    index = x.get_device()
     if y is None:
         if gamma is not None or gate is not None or post_weight is not None:
             raise ValueError("gamma, gate and post_weight scale y, which is None")
-    elif y.shape != x.shape or y.dtype != x.dtype or y.device != x.device:
+    elif y.shape != shape or y.dtype != dtype or y.get_device() != index:
         raise ValueError(f"y must match x: {tuple(y.shape)} {y.dtype} {y.device} vs "
-                         f"{tuple(x.shape)} {x.dtype} {x.device}")
+                         f"{tuple(shape)} {dtype} {x.device}")
     if post_bias is not None and post_weight is None:
         raise ValueError("post_bias without post_weight")
-    param_dtype = weight.dtype
-    if param_dtype not in (x.dtype, torch.float32):
-        raise TypeError(f"parameters must be {x.dtype} or float32, got {param_dtype}")
+    param_dtype, row = weight.dtype, shape[-1:]
+    if param_dtype != dtype and param_dtype != torch.float32:
+        raise TypeError(f"parameters must be {dtype} or float32, got {param_dtype}")
     for name, p in (("weight", weight), ("norm_bias", norm_bias), ("gamma", gamma),
                     ("post_weight", post_weight), ("post_bias", post_bias)):
-        if p is None:
-            continue
-        if p.shape != (C,) or p.device != x.device or p.dtype != param_dtype:
-            raise ValueError(f"{name} must be [{C}] of {param_dtype} on {x.device}, got "
+        if p is not None and (p.shape != row or p.dtype != param_dtype or p.get_device() != index):
+            raise ValueError(f"{name} must be {list(row)} of {param_dtype} on {x.device}, got "
                              f"{tuple(p.shape)} {p.dtype} {p.device}")
-    if gate is not None and (x.dim() < 2 or gate.shape != (x.shape[0], C)
-                             or gate.device != x.device or gate.dtype != param_dtype):
-        raise ValueError(f"gate must be [x.shape[0], {C}] of {param_dtype} on {x.device}, got "
-                         f"{tuple(gate.shape)} {gate.dtype} {gate.device}")
-    return param_dtype
+    if gate is not None and (len(shape) < 2 or gate.shape != (shape[0], shape[-1])
+                             or gate.dtype != param_dtype or gate.get_device() != index):
+        raise ValueError(f"gate must be [x.shape[0], {shape[-1]}] of {param_dtype} on {x.device}, "
+                         f"got {tuple(gate.shape)} {gate.dtype} {gate.device}")
 
 
 def _ptr(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
 
 
-def _norm_launch(x, y, weight, norm_bias, gamma, gate, post_weight, post_bias, kind, eps, *,
+def _dense(t: Optional[torch.Tensor]):
+    return t if t is None or t.is_contiguous() else t.detach().contiguous()
+
+
+def _norm_launch(x, y, weight, norm_bias, gamma, gate, post_weight, post_bias, kind, eps,
                  stats=None, h=None, mx=None):
     """One ``scmp_residual_norm`` call on contiguous tensors; returns r (None without y)."""
-    import ctypes
-
     from . import _lib
-    r = torch.empty_like(x) if y is not None else None
+    r = None if y is None else torch.empty_like(x)
     C = x.shape[-1]
-    a = _lib.NormArgs()
-    a.abi_version = _lib.ABI_VERSION
-    a.dtype, a.param_dtype = _lib.DTYPE[str(x.dtype)], _lib.DTYPE[str(weight.dtype)]
-    a.rms = int(kind == "rms")
-    for name, t in (("x", x), ("y", y), ("weight", weight), ("bias", norm_bias), ("gamma", gamma),
-                    ("gate", gate), ("post_weight", post_weight), ("post_bias", post_bias),
-                    ("r", r), ("h", h), ("stats", stats)):
-        setattr(a, name, _ptr(t))
-    if mx is not None:
-        a.mx_data, a.mx_scales = mx.data.data_ptr(), mx.scales.data_ptr()
-        a.mx_fmt = _lib.MX_FORMAT[mx.fmt]
-    a.rows, a.C = x.numel() // C, C
-    a.rows_per_gate = 0 if gate is None else a.rows // max(1, x.shape[0])
-    a.eps = float(eps)
-    a.h_f32 = int(h is not None and h.dtype == torch.float32)
-    with torch.cuda.device(x.device):
-        _lib.check(_lib.load().scmp_residual_norm(ctypes.byref(a), _stream(x)))
+    rows = x.numel() // C
+    args = _lib.NormArgs(
+        _lib.ABI_VERSION, DTYPE[x.dtype], DTYPE[weight.dtype], kind == "rms", x.data_ptr(),
+        _ptr(y), weight.data_ptr(), _ptr(norm_bias), _ptr(gamma), _ptr(gate), _ptr(post_weight),
+        _ptr(post_bias), _ptr(r), _ptr(h), _ptr(stats), None if mx is None else mx.data_ptr,
+        None if mx is None else mx.scales_ptr, rows, C,
+        0 if gate is None else rows // max(1, x.shape[0]), eps,
+        h is not None and h.dtype == torch.float32,
+        0 if mx is None else _lib.MX_FORMAT[mx.fmt], 0)
+    call(_lib.load().scmp_residual_norm, x.get_device(), args)
     return r
 
 
 class _ResidualNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, y, weight, norm_bias, gamma, gate, post_weight, post_bias, kind, eps):
-        x, y = x.contiguous(), None if y is None else y.contiguous()
-        params = [None if p is None else p.contiguous()
-                  for p in (weight, norm_bias, gamma, gate, post_weight, post_bias)]
-        rows = x.numel() // x.shape[-1]
-        stats = torch.empty(2 if post_weight is not None else 1, rows, 2, dtype=torch.float32,
-                            device=x.device)
+        t = [_dense(v) for v in (x, y, weight, norm_bias, gamma, gate, post_weight, post_bias)]
+        x = t[0]
+        stats = torch.empty(2 if post_weight is not None else 1, x.numel() // x.shape[-1], 2,
+                            dtype=torch.float32, device=x.device)
         h = torch.empty_like(x)
-        r = _norm_launch(x, y, *params, kind, eps, stats=stats, h=h)
+        r = _norm_launch(*t, kind, eps, stats, h)
         ctx.kind = kind
-        ctx.save_for_backward(x if r is None else r, y, stats, *params)
+        ctx.save_for_backward(x if r is None else r, t[1], stats, *t[2:])
         ctx.set_materialize_grads(False)
         return h if r is None else (r, h)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, *grads):
-        import ctypes
-
         from . import _lib
         r, y, stats, weight, norm_bias, gamma, gate, post_weight, post_bias = ctx.saved_tensors
         dr, dh = grads if y is not None else (None, grads[0])
-        want = ctx.needs_input_grad[:8]
+        leaves = (r, y, weight, norm_bias, gamma, gate, post_weight, post_bias)
         if r.numel() == 0 or (dr is None and dh is None):
-            leaves = (r, y, weight, norm_bias, gamma, gate, post_weight, post_bias)
             return tuple(torch.zeros_like(t) if w and t is not None else None
-                         for w, t in zip(want, leaves)) + (None, None)
-        dr, dh = (None if g is None else g.contiguous() for g in (dr, dh))
+                         for w, t in zip(ctx.needs_input_grad, leaves)) + (None, None)
+        dr, dh = _dense(dr), _dense(dh)
         out = [torch.empty_like(t) if w and t is not None else None
-               for w, t in zip(want, (r, y, weight, norm_bias, gamma, gate, post_weight,
-                                      post_bias))]
+               for w, t in zip(ctx.needs_input_grad, leaves)]
         C = r.shape[-1]
         rows = r.numel() // C
-        a = _lib.NormBwdArgs()
-        a.abi_version = _lib.ABI_VERSION
-        a.dtype, a.param_dtype = _lib.DTYPE[str(r.dtype)], _lib.DTYPE[str(weight.dtype)]
-        a.rms = int(ctx.kind == "rms")
-        names = ("r", "y", "dr", "dh", "weight", "gamma", "gate", "post_weight", "post_bias",
-                 "stats", "dx", "dy", "dweight", "dbias", "dgamma", "dgate", "dpost_weight",
-                 "dpost_bias")
-        tensors = (r, y, dr, dh, weight, gamma, gate, post_weight, post_bias, stats, *out)
-        for name, t in zip(names, tensors):
-            setattr(a, name, _ptr(t))
-        a.rows, a.C = rows, C
-        a.rows_per_gate = rows if gate is None else rows // r.shape[0]
+        per_gate = rows if gate is None else rows // r.shape[0]
         lib = _lib.load()
-        ws = None
+        ws, size = None, 0
         if any(t is not None for t in out[2:]):
-            size = lib.scmp_residual_norm_bwd_workspace(rows, C, a.rows_per_gate)
+            size = lib.scmp_residual_norm_bwd_workspace(rows, C, per_gate)
             ws = torch.empty(size, dtype=torch.uint8, device=r.device)
-            a.workspace, a.workspace_bytes = ws.data_ptr(), size
-        with torch.cuda.device(r.device):
-            _lib.check(lib.scmp_residual_norm_bwd(ctypes.byref(a), _stream(r)))
+        args = _lib.NormBwdArgs(
+            _lib.ABI_VERSION, DTYPE[r.dtype], DTYPE[weight.dtype], ctx.kind == "rms", r.data_ptr(),
+            _ptr(y), _ptr(dr), _ptr(dh), weight.data_ptr(), _ptr(gamma), _ptr(gate),
+            _ptr(post_weight), _ptr(post_bias), stats.data_ptr(), *[_ptr(t) for t in out], _ptr(ws),
+            size, rows, C, per_gate)
+        call(lib.scmp_residual_norm_bwd, r.get_device(), args)
         return (*out, None, None)
 
 
@@ -239,32 +225,28 @@ def residual_norm(x: torch.Tensor, y: Optional[torch.Tensor], weight: torch.Tens
     returns ``h`` as an ``MXTensor`` quantised from its fp32 values (nvfp4 with
     tensor scale 1) for ``mx_matmul``; that form has no gradient.  The sums
     differ from ``F.layer_norm``'s in their order, so the bits may too."""
-    _norm_inputs(x, y, weight, norm_bias, kind, gamma, gate, post_weight, post_bias)
-    if not (isinstance(eps, (int, float)) and eps >= 0):
-        raise ValueError(f"eps must be >= 0, got {eps!r}")
-    if x.shape[-1] > 8192:
-        raise ValueError(f"residual_norm takes rows of up to 8192 values, got {x.shape[-1]}")
+    _check_norm(x, y, weight, norm_bias, kind, eps, gamma, gate, post_weight, post_bias)
     leaves = (x, y, weight, norm_bias, gamma, gate, post_weight, post_bias)
-    if quantize is None and torch.is_grad_enabled() and any(
-            t is not None and t.requires_grad for t in leaves):
+    if torch.is_grad_enabled() and any([t is not None and t.requires_grad for t in leaves]):
+        if quantize is not None:
+            raise RuntimeError("residual_norm with quantize has no gradient; call it under "
+                               "torch.no_grad() or on detached inputs")
         out = _ResidualNorm.apply(*leaves, kind, eps)
         return (x, out) if y is None else out
-    from . import mx as _mx
-    _mx._no_grad_wanted("residual_norm with quantize", *leaves)
-    t = [None if v is None else v.detach().contiguous() for v in leaves]
+    t = [_dense(v) for v in leaves]
     if quantize is None:
         h = torch.empty_like(t[0])
-        r = _norm_launch(*t, kind, eps, h=h)
+        r = _norm_launch(*t, kind, eps, None, h)
         return (x if r is None else r), h
+    from . import mx as _mx
     _mx._check_fmt(quantize)
-    rows_vec = x.shape[-1] * x.element_size() % 16 == 0 and not any(
-        v is not None and v.data_ptr() % 16 for v in t)
-    if rows_vec or x.numel() == 0:
+    if x.numel() == 0 or (x.shape[-1] * x.element_size() % 16 == 0 and not any(
+            [v is not None and v.data_ptr() % 16 for v in t])):
         q = _mx.mx_empty(x.shape, quantize, x.device, x.dtype)
-        r = _norm_launch(*t, kind, eps, mx=q)
+        r = _norm_launch(*t, kind, eps, None, None, q)
     else:  # odd rows: through h's fp32 values, the same codes in two launches
         h = torch.empty(x.shape, dtype=torch.float32, device=x.device)
-        r = _norm_launch(*t, kind, eps, h=h)
+        r = _norm_launch(*t, kind, eps, None, h)
         q = _mx.mx_quantize(h, quantize)
         q.dtype = x.dtype
     return (x if r is None else r), q
