@@ -158,109 +158,129 @@ __device__ __forceinline__ void store_mx(const NormParams &p, const float *v, in
     p.mx_scales[mx_scale_word(row, blk >> 2, p.groups) + (blk & 3)] = (uint8_t)scale;
 }
 
-// E elements per lane.  E = 8 (rows of up to 2048 in 16-byte pieces: 8 warps a
-// block) keeps a row's chain of instructions short and 64 warps on an SM; longer
-// or unaligned rows take E = 32.
+// E elements per lane, by the shape (rows x columns, bf16 unless fp32, us):
+//   E = 8   one row per slot, up to 2048 columns: a short chain per row and 48
+//           warps an SM.  Few rows (257 x 1024: 3.3, E = 16 3.5), fp32 (16448 x
+//           1024: 49.7 = a copy's rate, E = 16 57.9), short rows (16448 x 200:
+//           9.1, E = 16 10.7)
+//   E = 16  slots walk rows, and once a row's x and y are used the next one is on
+//           its way into their registers.  Many rows (16448 x 1024: 30.6, E = 8
+//           42.1)
+//   E = 32  the same for rows of over 4096 columns, or not in 16-byte pieces
 template <typename T, typename P, int V, int E>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, E == 16 ? 3 : 1)
     residual_norm_kernel(const __grid_constant__ NormParams p) {
+  constexpr bool kWalk = E > 8;
   constexpr int NV = E / V;
   __shared__ float2 buf[2 * kMaxWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int G = p.warps_per_row, slot = warp / G, w = warp - slot * G;
+  const int slots = blockDim.x / (32 * G);
   RowSum sum(buf, G, slot, w);
-  const int64_t row = (int64_t)blockIdx.x * (blockDim.x / (32 * G)) + slot;
-  const bool live = row < p.rows;
   const int C = p.C;
   const float inv_c = 1.0f / (float)C;
-  const auto in = [&](int j) { return live && col_of<V>(j, G, w, lane) < C; };
-  const int64_t at = row * C;
+  const auto in_row = [&](int j) { return col_of<V>(j, G, w, lane) < C; };
 
   Pack<T, V> x[NV], y[NV];
+  const auto load = [&](int64_t row) {
+    const bool live = row < p.rows;
+    const int64_t at = row * C;
 #pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    const int c = col_of<V>(j, G, w, lane);
-    x[j].zero();
-    y[j].zero();
-    if (!in(j)) continue;
-    x[j].load(static_cast<const T *>(p.x) + at + c);
-    if (p.y) y[j].load(static_cast<const T *>(p.y) + at + c);
-  }
-  float r[NV][V];
-  if (p.y) {
-#pragma unroll
-    for (int j = 0; j < NV; ++j) y[j].get(r[j]);
-    if (p.post_weight) {
-      const float2 st = normalise<NV, V>(r, in, sum, inv_c, p.eps, p.rms);
-      if (p.stats && live && w == 0 && lane == 0) p.stats[p.rows + row] = st;
+    for (int j = 0; j < NV; ++j) {
+      x[j].zero();
+      y[j].zero();
+      if (!live || !in_row(j)) continue;
+      const int c = col_of<V>(j, G, w, lane);
+      x[j].load(static_cast<const T *>(p.x) + at + c);
+      if (p.y) y[j].load(static_cast<const T *>(p.y) + at + c);
     }
-    const int64_t gate_at = p.gate && live ? row / p.rows_per_gate * C : 0;
+  };
+  // (rows past the last one, up to a multiple of 128, exist for 4-bit scales)
+  const int64_t stride = (int64_t)gridDim.x * slots;
+  int64_t row = (int64_t)blockIdx.x * slots + slot;
+  load(row);
+  for (; row < p.row_end; row = kWalk ? row + stride : p.row_end) {
+    const bool live = row < p.rows;
+    const auto in = [&](int j) { return live && in_row(j); };
+    const int64_t at = row * C;
+    float r[NV][V];
+    if (p.y) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) y[j].get(r[j]);
+      if (p.post_weight) {
+        const float2 st = normalise<NV, V>(r, in, sum, inv_c, p.eps, p.rms);
+        if (p.stats && live && w == 0 && lane == 0) p.stats[p.rows + row] = st;
+      }
+      const int64_t gate_at = p.gate && live ? row / p.rows_per_gate * C : 0;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        const int c = col_of<V>(j, G, w, lane);
+        if (!in(j)) {
+#pragma unroll
+          for (int i = 0; i < V; ++i) r[j][i] = 0.f;
+          continue;
+        }
+        float f[V], g[V];
+        if (p.post_weight) {
+          load_v<P, V>(static_cast<const P *>(p.post_weight) + c, f);
+#pragma unroll
+          for (int i = 0; i < V; ++i) r[j][i] *= f[i];
+          if (p.post_bias) {
+            load_v<P, V>(static_cast<const P *>(p.post_bias) + c, f);
+#pragma unroll
+            for (int i = 0; i < V; ++i) r[j][i] += f[i];
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i) f[i] = 1.0f;
+        if (p.gamma) load_v<P, V>(static_cast<const P *>(p.gamma) + c, f);
+        if (p.gate) {
+          load_v<P, V>(static_cast<const P *>(p.gate) + gate_at + c, g);
+#pragma unroll
+          for (int i = 0; i < V; ++i) f[i] *= g[i];
+        }
+        x[j].get(g);
+        // r is rounded to its type once, and the norm sees the rounded value:
+        // the one that the next block and the backward pass read
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          r[j][i] = to_f32(from_f32<T>(__fmaf_rn(r[j][i], f[i], g[i])));
+        store_v<T, V>(static_cast<T *>(p.r) + at + c, r[j]);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) x[j].get(r[j]);
+    }
+    if (kWalk) load(row + stride);
+    const float2 st = normalise<NV, V>(r, in, sum, inv_c, p.eps, p.rms);
+    if (p.stats && live && w == 0 && lane == 0) p.stats[row] = st;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int c = col_of<V>(j, G, w, lane);
-      if (!in(j)) {
+      if (in(j)) {
+        float f[V], g[V];
+        load_v<P, V>(static_cast<const P *>(p.weight) + c, f);
+        if (p.bias) {
+          load_v<P, V>(static_cast<const P *>(p.bias) + c, g);
 #pragma unroll
-        for (int i = 0; i < V; ++i) r[j][i] = 0.f;
-        continue;
-      }
-      float f[V], g[V];
-      if (p.post_weight) {
-        load_v<P, V>(static_cast<const P *>(p.post_weight) + c, f);
+          for (int i = 0; i < V; ++i) r[j][i] = __fmaf_rn(r[j][i], f[i], g[i]);
+        } else {
 #pragma unroll
-        for (int i = 0; i < V; ++i) r[j][i] *= f[i];
-        if (p.post_bias) {
-          load_v<P, V>(static_cast<const P *>(p.post_bias) + c, f);
-#pragma unroll
-          for (int i = 0; i < V; ++i) r[j][i] += f[i];
+          for (int i = 0; i < V; ++i) r[j][i] *= f[i];
+        }
+        if (p.h) {
+          if (p.h_f32)
+            store_v<float, V>(static_cast<float *>(p.h) + at + c, r[j]);
+          else
+            store_v<T, V>(static_cast<T *>(p.h) + at + c, r[j]);
         }
       }
-#pragma unroll
-      for (int i = 0; i < V; ++i) f[i] = 1.0f;
-      if (p.gamma) load_v<P, V>(static_cast<const P *>(p.gamma) + c, f);
-      if (p.gate) {
-        load_v<P, V>(static_cast<const P *>(p.gate) + gate_at + c, g);
-#pragma unroll
-        for (int i = 0; i < V; ++i) f[i] *= g[i];
-      }
-      x[j].get(g);
-      // r is rounded to its type once, and the norm sees the rounded value: the
-      // one that the next block and the backward pass read
-#pragma unroll
-      for (int i = 0; i < V; ++i)
-        r[j][i] = to_f32(from_f32<T>(__fmaf_rn(r[j][i], f[i], g[i])));
-      store_v<T, V>(static_cast<T *>(p.r) + at + c, r[j]);
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < NV; ++j) x[j].get(r[j]);
-  }
-  const float2 st = normalise<NV, V>(r, in, sum, inv_c, p.eps, p.rms);
-  if (p.stats && live && w == 0 && lane == 0) p.stats[row] = st;
-#pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    const int c = col_of<V>(j, G, w, lane);
-    if (in(j)) {
-      float f[V];
-      load_v<P, V>(static_cast<const P *>(p.weight) + c, f);
-#pragma unroll
-      for (int i = 0; i < V; ++i) r[j][i] *= f[i];
-      if (p.bias) {
-        load_v<P, V>(static_cast<const P *>(p.bias) + c, f);
-#pragma unroll
-        for (int i = 0; i < V; ++i) r[j][i] += f[i];
-      }
-      if (p.h) {
-        if (p.h_f32)
-          store_v<float, V>(static_cast<float *>(p.h) + at + c, r[j]);
+      if (V > 1 && p.mx_data) {
+        if (p.fmt == SCMP_MXFP4)
+          store_mx<SCMP_MXFP4, V>(p, r[j], row, c, lane);
         else
-          store_v<T, V>(static_cast<T *>(p.h) + at + c, r[j]);
+          store_mx<SCMP_NVFP4, V>(p, r[j], row, c, lane);
       }
-    }
-    if (V > 1 && p.mx_data) {
-      if (p.fmt == SCMP_MXFP4)
-        store_mx<SCMP_MXFP4, V>(p, r[j], row, c, lane);
-      else
-        store_mx<SCMP_NVFP4, V>(p, r[j], row, c, lane);
     }
   }
 }
@@ -303,7 +323,7 @@ __device__ __forceinline__ void load_row(const NormBwdParams &p, int64_t row, bo
 }
 
 template <typename T, typename P, int V, int E, bool kPost, int kThreads>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kThreads, E == 8 ? 2 : 1)
     residual_norm_bwd_kernel(const __grid_constant__ NormBwdParams p) {
   constexpr int NV = E / V;
   constexpr int kParts = kPost ? 4 : 3;
@@ -485,7 +505,7 @@ __device__ __forceinline__ void write_totals(const NormBwdParams &p, int c,
     if (out[k]) static_cast<P *>(out[k])[c] = from_f32<P>(total[k]);
 }
 
-// Block (8 columns, gate group): 128 threads per column share the group's
+// Block (8 columns, gate group): 32 or 128 threads per column share the group's
 // partials.  With one group it finishes; else it leaves the group's sums for the
 // kernel below.
 template <typename P>
@@ -499,7 +519,7 @@ __global__ void __launch_bounds__(1024) norm_bwd_sum_kernel(
   const int parts = p.post_weight ? 4 : 3;
   float v[4] = {0.f, 0.f, 0.f, 0.f};
   if (c < p.C)
-    for (int64_t b = threadIdx.x >> 3; b < p.blocks_per_group; b += 128) {
+    for (int64_t b = threadIdx.x >> 3; b < p.blocks_per_group; b += blockDim.x >> 3) {
       const float *src = p.part + (group * p.blocks_per_group + b) * 4 * p.C + c;
 #pragma unroll
       for (int k = 0; k < 4; ++k)
@@ -517,7 +537,7 @@ __global__ void __launch_bounds__(1024) norm_bwd_sum_kernel(
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     one[k] = 0.f;
-    for (int i = 0; i < 32; ++i) one[k] += s[k][i][ci];
+    for (int i = 0; i < (int)(blockDim.x >> 5); ++i) one[k] += s[k][i][ci];
     if (p.groups > 1) p.sums[(group * 4 + k) * p.C + c] = one[k];
   }
   if (p.groups > 1) return;
@@ -555,26 +575,29 @@ __global__ void __launch_bounds__(1024) norm_bwd_groups_kernel(
 
 // --------------------------------------------------------------- dispatch
 
-// Elements per lane: 8 for rows of up to 2048 in 16-byte pieces.
+// Backward: elements per lane, 8 for rows of up to 2048 in 16-byte pieces.
 bool short_rows(int64_t C, bool vec) { return vec && C <= 2048; }
 
-template <typename T, typename P>
-cudaError_t forward(NormParams p, bool vec, cudaStream_t s) {
-  constexpr int V = kVec16<T>;
-  const bool small = short_rows(p.C, vec);
-  const int G = small ? (p.C + 255) / 256 : (p.C + 1023) / 1024;
-  const int slots = 8 / G;
+template <typename T, typename P, int V, int E>
+cudaError_t forward_e(NormParams p, cudaStream_t s) {
+  const int G = (p.C + 32 * E - 1) / (32 * E), slots = 8 / G, threads = 32 * G * slots;
   p.warps_per_row = G;
-  const int64_t rows = p.mx_data ? (p.rows + 127) / 128 * 128 : p.rows;
-  const unsigned blocks = (unsigned)((rows + slots - 1) / slots);
-  const int threads = 32 * G * slots;
-  if (small)
-    residual_norm_kernel<T, P, V, 8><<<blocks, threads, 0, s>>>(p);
-  else if (vec)
-    residual_norm_kernel<T, P, V, 32><<<blocks, threads, 0, s>>>(p);
-  else
-    residual_norm_kernel<T, P, 1, 32><<<blocks, threads, 0, s>>>(p);
+  p.row_end = p.mx_data ? (p.rows + 127) / 128 * 128 : p.rows;
+  const int64_t blocks = (p.row_end + slots - 1) / slots;
+  // walking slots: the blocks that 148 SMs hold at once
+  const int64_t most = E == 8 ? blocks : 148 * ((E == 16 ? 768 : 512) / threads);
+  residual_norm_kernel<T, P, V, E>
+      <<<(unsigned)(blocks < most ? blocks : most), threads, 0, s>>>(p);
   return cudaGetLastError();
+}
+
+template <typename T, typename P>
+cudaError_t forward(const NormParams &p, bool vec, cudaStream_t s) {
+  constexpr int V = kVec16<T>;
+  if (!vec) return forward_e<T, P, 1, 32>(p, s);
+  if (p.C <= 256 || (p.C <= 2048 && (sizeof(T) == 4 || p.rows <= 148 * 8)))
+    return forward_e<T, P, V, 8>(p, s);
+  return p.C <= 4096 ? forward_e<T, P, V, 16>(p, s) : forward_e<T, P, V, 32>(p, s);
 }
 
 template <typename T, typename P, int V, int E, int kThreads>
@@ -605,7 +628,8 @@ cudaError_t backward(NormBwdParams p, bool vec, cudaStream_t s, int *launches) {
                                           : backward_e<T, P, 1, 16, 512>(p, plan, s);
   *launches = 1;
   if (e != cudaSuccess || !p.part) return e;
-  norm_bwd_sum_kernel<P><<<(unsigned)((p.C + 7) / 8 * p.groups), 1024, 0, s>>>(p);
+  norm_bwd_sum_kernel<P><<<(unsigned)((p.C + 7) / 8 * p.groups),
+                           p.blocks_per_group > 64 ? 1024 : 256, 0, s>>>(p);
   ++*launches;
   if ((e = cudaGetLastError()) != cudaSuccess || p.groups == 1) return e;
   norm_bwd_groups_kernel<P><<<(unsigned)((p.C + 31) / 32), 1024, 0, s>>>(p);
@@ -615,15 +639,19 @@ cudaError_t backward(NormBwdParams p, bool vec, cudaStream_t s, int *launches) {
 
 }  // namespace
 
-// About 8 warps a block (16 for long rows) and three blocks on each of the 148
-// SMs in all, at least one per gate group.
+// About 8 warps a block (16 for long rows), and as many blocks as the 148 SMs
+// hold at once: two of 256 threads and 128 registers, or one (a block more would
+// start when the others end: 16400 x 1408 in 16 gate groups 168 us instead of
+// 103).  At least one block per gate group.
 NormBwdPlan norm_bwd_plan(int64_t rows, int64_t groups, int64_t C, bool vec) {
   NormBwdPlan plan;
-  plan.warps_per_row = (int)(short_rows(C, vec) ? (C + 255) / 256 : (C + 511) / 512);
+  const bool small = short_rows(C, vec);
+  plan.warps_per_row = (int)(small ? (C + 255) / 256 : (C + 511) / 512);
   plan.slots = plan.warps_per_row >= 8 ? 1 : 8 / plan.warps_per_row;
+  const int64_t resident = 148 * (small ? 512 / (32 * plan.warps_per_row * plan.slots) : 1);
   const int64_t per_group = (rows / groups + plan.slots - 1) / plan.slots;
-  const int64_t want = (3 * 148 + groups - 1) / groups;
-  plan.blocks_per_group = want < per_group ? want : per_group;
+  const int64_t share = resident / groups > 1 ? resident / groups : 1;
+  plan.blocks_per_group = share < per_group ? share : per_group;
   plan.part_floats = groups * plan.blocks_per_group * 4 * C;
   plan.sum_floats = groups > 1 ? groups * 4 * C : 0;
   return plan;

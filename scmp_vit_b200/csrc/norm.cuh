@@ -23,6 +23,7 @@ struct NormParams {
   bool rms, h_f32;
   int fmt;
   int warps_per_row;  // set by the launcher
+  int64_t row_end;    // rows that have output: all, or whole atoms of 4-bit scales
 };
 
 struct NormBwdParams {
