@@ -504,13 +504,35 @@ def split_qkv_rotary(qkv: torch.Tensor, num_heads: int, axes: RotaryAxes, pos: t
     return _split_rotary(qkv.contiguous(), pos, table, axes, H, Hk, transpose_v)
 
 
+class GridRotary(nn.Module):
+    """The positions of an image's (or clip's) patches on their grid, behind
+    ``prefix`` tokens without one (the class token): the head's dimensions in
+    equal sections per axis, as EVA-type blocks turn them."""
+
+    def __init__(self, grid, head_dim: int, *, base: float = 10000.0, prefix: int = 1,
+                 interleaved: bool = True):
+        super().__init__()
+        grid = [int(n) for n in grid]
+        section = head_dim // len(grid) // 2 * 2
+        self.axes = RotaryAxes([section] * len(grid), grid, base=base, interleaved=interleaved)
+        at = torch.meshgrid(*[torch.arange(n) for n in grid], indexing="ij")
+        pos = torch.stack([a.reshape(-1) for a in at], -1)
+        pos = torch.cat([pos.new_full((prefix, len(grid)), -1), pos])
+        self.register_buffer("pos", pos.to(torch.int32), persistent=False)
+
+    def split(self, qkv: torch.Tensor, num_heads: int, *, transpose_v: bool = True):
+        """``split_qkv_rotary`` of a projection output with these positions."""
+        return split_qkv_rotary(qkv, num_heads, self.axes, self.pos, transpose_v=transpose_v)
+
+
 def make_sc_attention_forward(sc_prec: int, sc_av: bool, sc_qk: bool = True,
                               qk_mp_cfg: MPConfig | None = None,
                               av_mp_cfg: MPConfig | None = None, *,
                               av_mode: str = "bipolar", cfg_for: Optional[CfgFor] = None):
     """``forward(self, x)`` for a DINOv2-style attention module with
     ``qkv``, ``proj``, ``proj_drop``, ``num_heads``, ``scale`` attributes
-    (same signature and numerics as ``cls/sc_attention_patch.py:248-328``)."""
+    (same signature and numerics as ``cls/sc_attention_patch.py:248-328``).
+    A ``rope`` attribute (``GridRotary``) turns q and k before Q@K^T."""
     do_av = sc_av
 
     def forward(self, x, attn_bias=None):
@@ -518,7 +540,10 @@ def make_sc_attention_forward(sc_prec: int, sc_av: bool, sc_qk: bool = True,
         H = self.num_heads
         D = C // H
         qkv = self.qkv(x)
-        if qkv.is_cuda and qkv.element_size() in (2, 4) and B * H <= 65535 and D <= 256:
+        rope = getattr(self, "rope", None)
+        if rope is not None:
+            q, k, v = rope.split(qkv, H)
+        elif qkv.is_cuda and qkv.element_size() in (2, 4) and B * H <= 65535 and D <= 256:
             q, k, v = split_qkv(qkv, H)
         else:
             q, k, v = torch.unbind(qkv.reshape(B, N, 3, H, D), 2)

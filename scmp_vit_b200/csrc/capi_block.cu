@@ -49,6 +49,40 @@ int check_exp(int fmt, int e, int limit) {
   return SCMP_OK;
 }
 
+// A product's arguments; `codes`: A's buffers are needed.
+int check_product(const scmp_mx_matmul_args *args, bool codes, MxProduct &p) {
+  if (!args) return fail(SCMP_EINVAL, "args is NULL");
+  const scmp_mx_matmul_args &x = *args;
+  if (x.abi_version != SCMP_ABI_VERSION)
+    return fail(SCMP_EINVAL, "abi_version %d != %d", x.abi_version, SCMP_ABI_VERSION);
+  int rc;
+  if ((rc = check_mx(x.M, x.K, x.fmt)) != SCMP_OK || (rc = check_mx(x.N, x.K, x.fmt)) != SCMP_OK ||
+      (rc = check_exp(x.fmt, x.scale_exp, kMaxScaleExp)) != SCMP_OK)
+    return rc;
+  if (!known_dtype(x.out_dtype) || (x.bias && !known_dtype(x.bias_dtype)))
+    return fail(SCMP_EINVAL, "unknown dtype (out %d, bias %d)", x.out_dtype, x.bias_dtype);
+  if (x.M > 0 && x.N > 0) {
+    if ((codes && (!x.a || !x.a_scales)) || !x.b || !x.b_scales || !x.out)
+      return fail(SCMP_EINVAL, "a, b, their scales and out must be non-NULL");
+    if (!aligned({x.a, x.a_scales, x.b, x.b_scales}, 16))
+      return fail(SCMP_EINVAL, "a, b and their scales must be 16-byte aligned");
+  }
+  p.a = static_cast<const uint8_t *>(x.a);
+  p.a_scales = static_cast<const uint8_t *>(x.a_scales);
+  p.b = static_cast<const uint8_t *>(x.b);
+  p.b_scales = static_cast<const uint8_t *>(x.b_scales);
+  p.M = x.M;
+  p.N = x.N;
+  p.K = x.K;
+  p.fmt = x.fmt;
+  p.alpha = ldexpf(1.0f, x.scale_exp);
+  p.bias = x.bias;
+  p.bias_dtype = x.bias_dtype;
+  p.out = x.out;
+  p.out_dtype = x.out_dtype;
+  return SCMP_OK;
+}
+
 }  // namespace
 }  // namespace scmp
 
@@ -76,12 +110,11 @@ int scmp_mx_quantize(const void *x, int dtype, int64_t rows, int64_t K, int64_t 
   if (!x || !data || !scales) return fail(SCMP_EINVAL, "x, data and scales must be non-NULL");
   if (!aligned({data, scales}, 16))
     return fail(SCMP_EINVAL, "data and scales must be 16-byte aligned");
-  int launches = 0;
   const cudaError_t e = launch_mx_quantize(
       x, dtype, ld, mx_layout(rows, K, fmt), fmt, scale_exp, static_cast<uint8_t *>(data),
-      static_cast<uint8_t *>(scales), static_cast<cudaStream_t>(stream), &launches);
+      static_cast<uint8_t *>(scales), static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return cuda_fail(e, "mx_quantize launch");
-  add_launches((uint64_t)launches);
+  add_launches(1);
   return SCMP_OK;
 }
 
@@ -105,41 +138,20 @@ int scmp_mx_dequantize(const void *data, const void *scales, int64_t rows, int64
 
 int scmp_mx_matmul(const scmp_mx_matmul_args *args, void *stream) {
   set_last_error("");
-  if (!args) return fail(SCMP_EINVAL, "args is NULL");
-  const scmp_mx_matmul_args &x = *args;
-  if (x.abi_version != SCMP_ABI_VERSION)
-    return fail(SCMP_EINVAL, "abi_version %d != %d", x.abi_version, SCMP_ABI_VERSION);
-  int rc;
-  if ((rc = check_mx(x.M, x.K, x.fmt)) != SCMP_OK || (rc = check_mx(x.N, x.K, x.fmt)) != SCMP_OK ||
-      (rc = check_exp(x.fmt, x.scale_exp, kMaxScaleExp)) != SCMP_OK)
-    return rc;
-  if (!known_dtype(x.out_dtype) || (x.bias && !known_dtype(x.bias_dtype)))
-    return fail(SCMP_EINVAL, "unknown dtype (out %d, bias %d)", x.out_dtype, x.bias_dtype);
-  if (x.M == 0 || x.N == 0) return SCMP_OK;
-  if (!x.a || !x.a_scales || !x.b || !x.b_scales || !x.out)
-    return fail(SCMP_EINVAL, "a, b, their scales and out must be non-NULL");
-  if (!aligned({x.a, x.a_scales, x.b, x.b_scales}, 16))
-    return fail(SCMP_EINVAL, "a, b and their scales must be 16-byte aligned");
-  unsigned int *err = device_error_word();
-  if (!err) return fail(SCMP_ECUDA, "cannot resolve the engine error word");
   MxProduct p{};
-  p.a = static_cast<const uint8_t *>(x.a);
-  p.a_scales = static_cast<const uint8_t *>(x.a_scales);
-  p.b = static_cast<const uint8_t *>(x.b);
-  p.b_scales = static_cast<const uint8_t *>(x.b_scales);
-  p.M = x.M;
-  p.N = x.N;
-  p.K = x.K;
-  p.fmt = x.fmt;
-  p.alpha = ldexpf(1.0f, x.scale_exp);
-  p.bias = x.bias;
-  p.bias_dtype = x.bias_dtype;
-  p.out = x.out;
-  p.out_dtype = x.out_dtype;
-  int launches = 0;
-  const cudaError_t e = launch_mx_matmul(p, err, static_cast<cudaStream_t>(stream), &launches);
+  const int rc = check_product(args, true, p);
+  if (rc != SCMP_OK || p.M == 0 || p.N == 0) return rc;
+  auto s = static_cast<cudaStream_t>(stream);
+  cudaError_t e;
+  if (mx_thin(p.M, p.K)) {
+    e = launch_mx_thin(p, nullptr, 0, 0, s);
+  } else {
+    unsigned int *err = device_error_word();
+    if (!err) return fail(SCMP_ECUDA, "cannot resolve the engine error word");
+    e = launch_mx_matmul(p, err, s);
+  }
   if (e != cudaSuccess) return cuda_fail(e, "mx_matmul launch");
-  add_launches((uint64_t)launches);
+  add_launches(1);
   return SCMP_OK;
 }
 
@@ -147,10 +159,22 @@ int scmp_mx_linear(const void *x, int x_dtype, int64_t ld, const scmp_mx_matmul_
                    void *stream) {
   set_last_error("");
   if (!args) return fail(SCMP_EINVAL, "args is NULL");
-  if (args->M == 0 || args->N == 0) return scmp_mx_matmul(args, stream);
-  const int rc = scmp_mx_quantize(x, x_dtype, args->M, args->K, ld, args->fmt, 0,
-                                  const_cast<void *>(args->a), const_cast<void *>(args->a_scales),
-                                  stream);
+  const bool thin = mx_thin(args->M, args->K);
+  MxProduct p{};
+  int rc = check_product(args, !thin, p);
+  if (rc != SCMP_OK) return rc;
+  if (!known_dtype(x_dtype)) return fail(SCMP_EINVAL, "unknown dtype %d", x_dtype);
+  if (ld < p.K) return fail(SCMP_EINVAL, "ld=%lld below K=%lld", (long long)ld, (long long)p.K);
+  if (p.M == 0 || p.N == 0) return SCMP_OK;
+  if (!x) return fail(SCMP_EINVAL, "x must be non-NULL");
+  if (thin) {
+    const cudaError_t e = launch_mx_thin(p, x, x_dtype, ld, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return cuda_fail(e, "mx_linear launch");
+    add_launches(1);
+    return SCMP_OK;
+  }
+  rc = scmp_mx_quantize(x, x_dtype, p.M, p.K, ld, p.fmt, 0, const_cast<uint8_t *>(p.a),
+                        const_cast<uint8_t *>(p.a_scales), stream);
   return rc != SCMP_OK ? rc : scmp_mx_matmul(args, stream);
 }
 

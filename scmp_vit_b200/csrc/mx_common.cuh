@@ -203,8 +203,7 @@ __device__ __forceinline__ uint32_t mx_encode8(const float *x, uint32_t amax, fl
 // --------------------------------------------------------------- launchers
 
 cudaError_t launch_mx_quantize(const void *x, int dtype, int64_t ld, const MxLayout &l, int fmt,
-                               int scale_exp, uint8_t *data, uint8_t *scales, cudaStream_t s,
-                               int *launches);
+                               int scale_exp, uint8_t *data, uint8_t *scales, cudaStream_t s);
 cudaError_t launch_mx_dequantize(const uint8_t *data, const uint8_t *scales, const MxLayout &l,
                                  int fmt, int scale_exp, void *out, int dtype, cudaStream_t s);
 
@@ -218,7 +217,10 @@ struct MxProduct {
   void *out;  // [M, N] row-major
   int out_dtype;
 };
-cudaError_t launch_mx_matmul(const MxProduct &p, unsigned int *error, cudaStream_t s,
-                             int *launches);
+cudaError_t launch_mx_matmul(const MxProduct &p, unsigned int *error, cudaStream_t s);
+// A few rows (mx_thin): x quantised in the same launch, or NULL with p.a's codes.
+bool mx_thin(int64_t M, int64_t K);
+cudaError_t launch_mx_thin(const MxProduct &p, const void *x, int x_dtype, int64_t ld,
+                           cudaStream_t s);
 
 }  // namespace scmp

@@ -474,9 +474,6 @@ cudaError_t launch(MxTiles t, int64_t kp, int64_t groups, cudaStream_t s) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
-  if ((e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                (int)Cfg::kSmem)) != cudaSuccess)
-    return e;
   cudaLaunchConfig_t cfg = {};
   cfg.blockDim = dim3(kThreads, 1, 1);
   cfg.dynamicSmemBytes = Cfg::kSmem;
@@ -485,6 +482,9 @@ cudaError_t launch(MxTiles t, int64_t kp, int64_t groups, cudaStream_t s) {
   static int max_clusters[kMaxCachedDevices] = {};
   int clusters = dev < kMaxCachedDevices ? max_clusters[dev] : 0;
   if (clusters <= 0) {
+    if ((e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                  (int)Cfg::kSmem)) != cudaSuccess)
+      return e;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = 2;
@@ -529,9 +529,7 @@ cudaError_t launch_typed(const MxTiles &t, int64_t kp, int64_t groups, cudaStrea
 
 }  // namespace
 
-cudaError_t launch_mx_matmul(const MxProduct &p, unsigned int *error, cudaStream_t s,
-                             int *launches) {
-  *launches = 1;
+cudaError_t launch_mx_matmul(const MxProduct &p, unsigned int *error, cudaStream_t s) {
   const MxLayout l = mx_layout(p.M, p.K, p.fmt);
   MxTiles t{};
   t.p = p;

@@ -252,9 +252,7 @@ cudaError_t dequantize(const uint8_t *data, const uint8_t *scales, const MxLayou
 }  // namespace
 
 cudaError_t launch_mx_quantize(const void *x, int dtype, int64_t ld, const MxLayout &l, int fmt,
-                               int scale_exp, uint8_t *data, uint8_t *scales, cudaStream_t s,
-                               int *launches) {
-  *launches = 1;
+                               int scale_exp, uint8_t *data, uint8_t *scales, cudaStream_t s) {
   const bool mx = fmt == SCMP_MXFP4;
   if (dtype == SCMP_F32)
     return mx ? quantize<float, SCMP_MXFP4>(x, ld, l, scale_exp, data, scales, s)

@@ -199,16 +199,20 @@ def mx_matmul(a: Union[torch.Tensor, MXTensor], b: MXTensor, *,
         raise ValueError(f"operands on different devices: {a.device} vs {b.device}")
     if len(a.shape) < 1 or a.shape[-1] != K:
         raise ValueError(f"inner-dim mismatch: a {tuple(a.shape)}, b {tuple(b.shape)}")
+    qa = a
     if plain:
         x_code = _check_input(a, "mx_matmul")
-        qa = mx_empty(a.shape, b.fmt, a.device, a.dtype)
+        rows = a.numel() // K
+        # a few rows are quantised inside the product's own launch
+        thin = rows <= _lib.MX_THIN_ROWS and K <= _lib.MX_THIN_K
+        qa = None if thin else mx_empty(a.shape, b.fmt, a.device, a.dtype)
     elif a.fmt != b.fmt:
         raise ValueError(f"operands of different formats: {a.fmt} vs {b.fmt}")
     else:
-        qa = a
-    shape = (*qa.shape[:-1], N)
+        rows = a.rows
+    shape = (*a.shape[:-1], N)
     if out is None:
-        dtype = qa.dtype if out_dtype is None else out_dtype
+        dtype = a.dtype if out_dtype is None else out_dtype
         out_code = dtype_code(dtype, "out")
         out = torch.empty(shape, dtype=dtype, device=b.device)
     else:
@@ -226,9 +230,11 @@ def mx_matmul(a: Union[torch.Tensor, MXTensor], b: MXTensor, *,
         bias = bias if bias.is_contiguous() else bias.detach().contiguous()
         bias_ptr = bias.data_ptr()
     _no_grad_wanted("mx_matmul", out)
-    args = _lib.MxMatmulArgs(_lib.ABI_VERSION, _lib.MX_FORMAT[b.fmt], qa.data_ptr, qa.scales_ptr,
-                             b.data_ptr, b.scales_ptr, qa.rows, N, K, qa.scale_exp + b.scale_exp,
-                             bias_code, bias_ptr, out.data_ptr(), out_code, 0)
+    args = _lib.MxMatmulArgs(
+        _lib.ABI_VERSION, _lib.MX_FORMAT[b.fmt], None if qa is None else qa.data_ptr,
+        None if qa is None else qa.scales_ptr, b.data_ptr, b.scales_ptr, rows, N, K,
+        b.scale_exp if plain else a.scale_exp + b.scale_exp, bias_code, bias_ptr, out.data_ptr(),
+        out_code, 0)
     if plain:
         x, ld = _rows_of(a)
         call(_lib.load().scmp_mx_linear, index, x.data_ptr(), x_code, ld, args)

@@ -8,6 +8,12 @@ class with ``fc1`` / ``fc2``; and a 1000-way head on the concatenation of the
 CLS token and the mean patch token (2048 -> 1000).  Weights are random
 (seeded); there are no checkpoints in this environment.
 
+With ``rope`` the attention turns q and k by the patches' (height, width), as
+EVA-type blocks do.  ``patch_vit_mx`` puts the linears in microscaled 4 bits
+instead (``mx.MXLinear``, the deterministic counterpart of the SC linears), and
+``set_fused_norm`` runs the blocks' residual adds and norms in one pass each,
+with gradients.
+
 ``patch_vit`` installs the SC operators per block: ``qkv_proj`` /
 ``out_proj`` / ``mlp_fc1`` / ``mlp_fc2`` as ``SCLinear``, Q@K^T and Attn@V
 through the batched attention core, optional per-block pools (e.g. an
@@ -23,9 +29,10 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from ._call import DTYPE, call
-from .attention import make_sc_attention_forward
+from .attention import GridRotary, make_sc_attention_forward
 from .head_aligned_comp import HeadAlignedSCLinear
 from .mp import SeededRandomMPConfig, quantile_counts, set_current_block_idx
+from .mx import MXLinear
 from .sc_linear import PackedWeights, SCLinear, _get_config, sc_linear_rows
 
 
@@ -55,6 +62,19 @@ def set_fused_glue(flag: bool) -> None:
     """Turn the fused fp32 block glue on or off (results are identical)."""
     global FUSED_GLUE
     FUSED_GLUE = bool(flag)
+
+
+# Whether the blocks run a residual add and the norm behind it in one pass
+# (residual_norm), in training too.  The sums' order differs from
+# nn.LayerNorm's, so this is off unless asked for; blocks with 4-bit linears
+# always do.
+FUSED_NORM = False
+
+
+def set_fused_norm(flag: bool) -> None:
+    """Turn the blocks' fused residual adds and norms on or off."""
+    global FUSED_NORM
+    FUSED_NORM = bool(flag)
 
 
 def _stream(t: torch.Tensor):
@@ -277,12 +297,16 @@ class Attention(nn.Module):
         self.proj = nn.Linear(dim, dim)
         self.attn_drop = nn.Identity()
         self.proj_drop = nn.Identity()
+        self.rope: Optional[GridRotary] = None  # positions of q and k, if the model has them
 
     def forward(self, x, attn_bias=None):
         B, N, C = x.shape
         H = self.num_heads
-        qkv = self.qkv(x).reshape(B, N, 3, H, C // H).permute(2, 0, 3, 1, 4)
-        q, k, v = qkv.unbind(0)
+        if self.rope is not None:
+            q, k, v = self.rope.split(self.qkv(x), H, transpose_v=False)
+        else:
+            qkv = self.qkv(x).reshape(B, N, 3, H, C // H).permute(2, 0, 3, 1, 4)
+            q, k, v = qkv.unbind(0)
         out = F.scaled_dot_product_attention(q, k, v)
         return self.proj_drop(self.proj(out.transpose(1, 2).reshape(B, N, C)))
 
@@ -310,6 +334,8 @@ class Block(nn.Module):
 
     def forward(self, x):
         set_current_block_idx(self.block_idx)
+        if self._fused_norm_applies(x):
+            return self._forward_fused_norm(x)
         if self._fused_glue_applies(x):
             return self._forward_fused_glue(x)
         y = x + self.ls1(self.attn(self.norm1(x)))
@@ -317,6 +343,37 @@ class Block(nn.Module):
         if self.comp is not None:
             y = y + self.comp(x).to(y.dtype)
         return y
+
+    def _fused_norm_applies(self, x: torch.Tensor) -> bool:
+        qkv, fc1 = getattr(self.attn, "qkv", None), getattr(self.mlp, "fc1", None)
+        if not (FUSED_NORM or type(qkv) is MXLinear or type(fc1) is MXLinear):
+            return False
+        norms = (self.norm1, self.norm2)
+        return (x.is_cuda and x.dtype in _NORM_TYPES and x.shape[-1] <= 8192
+                and type(self.ls1) is LayerScale
+                and all(type(n) is nn.LayerNorm and n.weight is not None and n.bias is not None
+                        and n.weight.dtype in (x.dtype, torch.float32) for n in norms)
+                and self.ls1.gamma.dtype == self.norm2.weight.dtype)
+
+    def _forward_fused_norm(self, x):
+        """The forward above with each norm in the pass of the residual add in
+        front of it; a norm whose reader is a 4-bit linear writes codes only."""
+        def norm(n, reader, y=None, gamma=None):
+            # (the reader of a patched block that is not a 4-bit linear, or any
+            # reader while gradients are recorded, takes values)
+            fmt = reader.fmt if type(reader) is MXLinear and not torch.is_grad_enabled() else None
+            return residual_norm(x, y, n.weight, n.bias, eps=n.eps, gamma=gamma, quantize=fmt)
+
+        _, h = norm(self.norm1, self.attn.qkv)
+        a = self.attn(h)
+        y, h = norm(self.norm2, getattr(self.mlp, "fc1", None), a, self.ls1.gamma)
+        u = self.mlp(h)
+        e = None if self.comp is None else self.comp(x).to(y.dtype)
+        if self._fused_glue_applies(y):
+            return scale_residual(y, u.contiguous(), self.ls2.gamma, out=y,
+                                  extra=None if e is None else e.contiguous())
+        y = y + self.ls2(u)
+        return y if e is None else y + e
 
     def _fused_glue_applies(self, x: torch.Tensor) -> bool:
         return (FUSED_GLUE and x.is_cuda and x.dtype == torch.float32 and x.is_contiguous()
@@ -350,7 +407,8 @@ class Block(nn.Module):
 
 class Backbone(nn.Module):
     def __init__(self, img: int = 224, patch: int = 14, dim: int = 1024, depth: int = 24,
-                 heads: int = 16, hidden: int = 4096, ls_init: float = 1.0):
+                 heads: int = 16, hidden: int = 4096, ls_init: float = 1.0, rope: bool = False,
+                 rope_base: float = 10000.0):
         super().__init__()
         self.patch_embed = nn.Conv2d(3, dim, kernel_size=patch, stride=patch)
         n = (img // patch) ** 2
@@ -359,6 +417,10 @@ class Backbone(nn.Module):
         self.blocks = nn.ModuleList([Block(dim, heads, hidden, ls_init) for _ in range(depth)])
         for i, b in enumerate(self.blocks):
             b.block_idx = i
+        if rope:
+            grid = GridRotary((img // patch, img // patch), dim // heads, base=rope_base)
+            for b in self.blocks:
+                b.attn.rope = grid
         self.norm = nn.LayerNorm(dim, eps=1e-6)
 
     def forward(self, x):
@@ -495,4 +557,28 @@ def patch_vit(model: ViTClassifier, sc_prec: int, ops: Iterable[str] = ("qk", "a
             blk.comp = HeadAlignedSCLinear(lin, p, n_heads=attn.num_heads,
                                            cfg_override=cfg_for(head_dim, p))
             stats["comp"] += 1
+    return stats
+
+
+MX_OPS = ("qkv_proj", "out_proj", "mlp_fc1", "mlp_fc2")
+
+
+def patch_vit_mx(model: ViTClassifier, ops: Iterable[str] = MX_OPS, *,
+                 fmt: str = "mxfp4") -> dict:
+    """Put the named linears of every block (the op names of ``patch_vit``) in
+    microscaled 4 bits: ``mx.MXLinear`` from the present weights, which must be
+    on the GPU.  The norms in front of qkv_proj and mlp_fc1 then write their
+    codes.  Inference only."""
+    ops = set(ops)
+    unknown = ops - set(MX_OPS)
+    if unknown:
+        raise ValueError(f"unknown ops {sorted(unknown)} (of {MX_OPS})")
+    where = {"qkv_proj": ("attn", "qkv"), "out_proj": ("attn", "proj"), "mlp_fc1": ("mlp", "fc1"),
+             "mlp_fc2": ("mlp", "fc2")}
+    stats = {op: 0 for op in MX_OPS}
+    for blk in model.backbone.blocks:
+        for op in ops:
+            owner = getattr(blk, where[op][0])
+            setattr(owner, where[op][1], MXLinear(getattr(owner, where[op][1]), fmt))
+            stats[op] += 1
     return stats
