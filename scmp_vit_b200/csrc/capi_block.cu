@@ -26,7 +26,7 @@ int cuda_fail(cudaError_t e, const char *what) {
   return fail(SCMP_ECUDA, "%s: %s", what, cudaGetErrorString(e));
 }
 
-constexpr int64_t kMaxRows = INT32_MAX;  // tensor-map and grid coordinates
+constexpr int64_t kMaxRows = INT32_MAX - 1023;  // a tile's coordinates stay 32-bit
 constexpr int kMaxScaleExp = 120;        // 2^+-e and its reciprocal are normal fp32 numbers
 
 bool known_dtype(int d) { return d >= SCMP_F32 && d <= SCMP_F16; }
@@ -297,15 +297,12 @@ int scmp_residual_norm_bwd(const scmp_norm_bwd_args *args, void *stream) {
   p.groups = x.gate ? x.rows / x.rows_per_gate : 1;
   p.C = (int)x.C;
   p.rms = x.rms != 0;
-  p.part_needed = x.dweight || x.dbias || x.dgamma || x.dgate || x.dpost_weight || x.dpost_bias;
-  if (p.part_needed) {
+  if (x.dweight || x.dbias || x.dgamma || x.dgate || x.dpost_weight || x.dpost_bias) {
     const size_t need = (size_t)norm_bwd_floats(p.rows, p.groups, p.C) * sizeof(float);
     if (!x.workspace || x.workspace_bytes < need)
       return fail(SCMP_EWORKSPACE, "workspace needs %zu bytes, got %zu", need,
                   x.workspace ? x.workspace_bytes : (size_t)0);
-    // the groups' sums lie behind the larger of the two plans' partials
     p.part = static_cast<float *>(x.workspace);
-    p.sums = p.part + need / sizeof(float) - (p.groups > 1 ? p.groups * 4 * p.C : 0);
   }
   if (!aligned({x.stats, x.workspace}, 8))
     return fail(SCMP_EINVAL, "stats and workspace must be 8-byte aligned");

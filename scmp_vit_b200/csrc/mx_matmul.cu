@@ -18,6 +18,8 @@
 // Warps: 0 loads, 1 issues MMAs (even CTA), 2 owns the tensor memory, 4-19 run
 // the epilogue.  Every wait is bounded: a wait that gives up raises the error
 // word and the pair drains.
+#include <atomic>
+
 #include "mx_common.cuh"
 #include "tc_ptx.cuh"
 
@@ -474,29 +476,28 @@ cudaError_t launch(MxTiles t, int64_t kp, int64_t groups, cudaStream_t s) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
-  cudaLaunchConfig_t cfg = {};
-  cfg.blockDim = dim3(kThreads, 1, 1);
-  cfg.dynamicSmemBytes = Cfg::kSmem;
-  cfg.stream = s;
+  // (an attribute of the function in the current context, so set in every call)
+  if ((e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                (int)Cfg::kSmem)) != cudaSuccess)
+    return e;
   // one cluster per resident pair slot (persistent tiles)
-  static int max_clusters[kMaxCachedDevices] = {};
-  int clusters = dev < kMaxCachedDevices ? max_clusters[dev] : 0;
+  static std::atomic<int> max_clusters[kMaxCachedDevices];
+  int clusters = dev < kMaxCachedDevices ? max_clusters[dev].load(std::memory_order_relaxed) : 0;
   if (clusters <= 0) {
-    if ((e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                  (int)Cfg::kSmem)) != cudaSuccess)
-      return e;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = 2;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(2, 1, 1);
+    cfg.blockDim = dim3(kThreads, 1, 1);
+    cfg.dynamicSmemBytes = Cfg::kSmem;
+    cfg.stream = s;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    cfg.gridDim = dim3(2, 1, 1);
     if ((e = cudaOccupancyMaxActiveClusters(&clusters, kern, &cfg)) != cudaSuccess) return e;
     if (clusters <= 0) return cudaErrorInvalidConfiguration;
-    if (dev < kMaxCachedDevices) max_clusters[dev] = clusters;
-    cfg.attrs = nullptr;
-    cfg.numAttrs = 0;
+    if (dev < kMaxCachedDevices) max_clusters[dev].store(clusters, std::memory_order_relaxed);
   }
   t.tiles_f = (uint32_t)((t.p.N + 255) / 256);
   t.nt = tile_rows(t.p.M, t.tiles_f, clusters);

@@ -618,7 +618,7 @@ cudaError_t backward(NormBwdParams p, bool vec, cudaStream_t s, int *launches) {
   p.warps_per_row = plan.warps_per_row;
   p.blocks_per_group = plan.blocks_per_group;
   p.rows_per_group = p.rows / p.groups;
-  if (!p.part_needed) p.part = nullptr;
+  p.sums = p.part ? p.part + plan.part_floats : nullptr;
   // (blocks of 512 threads leave 128 registers a thread, too few for 16
   // elements: they serve the rows that need them)
   constexpr int V = kVec16<T>;
@@ -628,6 +628,12 @@ cudaError_t backward(NormBwdParams p, bool vec, cudaStream_t s, int *launches) {
                                           : backward_e<T, P, 1, 16, 512>(p, plan, s);
   *launches = 1;
   if (e != cudaSuccess || !p.part) return e;
+  if (p.groups > 1 && p.blocks_per_group == 1) {
+    p.sums = p.part;  // one block per group: its partials are the group's sums
+    norm_bwd_groups_kernel<P><<<(unsigned)((p.C + 31) / 32), 1024, 0, s>>>(p);
+    ++*launches;
+    return cudaGetLastError();
+  }
   norm_bwd_sum_kernel<P><<<(unsigned)((p.C + 7) / 8 * p.groups),
                            p.blocks_per_group > 64 ? 1024 : 256, 0, s>>>(p);
   ++*launches;
@@ -653,14 +659,15 @@ NormBwdPlan norm_bwd_plan(int64_t rows, int64_t groups, int64_t C, bool vec) {
   const int64_t share = resident / groups > 1 ? resident / groups : 1;
   plan.blocks_per_group = share < per_group ? share : per_group;
   plan.part_floats = groups * plan.blocks_per_group * 4 * C;
-  plan.sum_floats = groups > 1 ? groups * 4 * C : 0;
+  plan.sum_floats = groups > 1 && plan.blocks_per_group > 1 ? groups * 4 * C : 0;
   return plan;
 }
 
 int64_t norm_bwd_floats(int64_t rows, int64_t groups, int64_t C) {
   const NormBwdPlan a = norm_bwd_plan(rows, groups, C, true);
   const NormBwdPlan b = norm_bwd_plan(rows, groups, C, false);
-  return (a.part_floats > b.part_floats ? a.part_floats : b.part_floats) + a.sum_floats;
+  return (a.part_floats > b.part_floats ? a.part_floats : b.part_floats) +
+         (a.sum_floats > b.sum_floats ? a.sum_floats : b.sum_floats);
 }
 
 cudaError_t launch_residual_norm(const NormParams &p, int dtype, int param_dtype, bool vec,

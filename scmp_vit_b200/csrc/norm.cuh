@@ -32,10 +32,11 @@ struct NormBwdParams {
   const float2 *stats;
   void *dx, *dy;  // nullable
   void *dweight, *dbias, *dgamma, *dgate, *dpost_weight, *dpost_bias;  // nullable
-  float *part, *sums;  // see NormBwdPlan
+  float *part;  // nullable (no parameter gradient wanted), see NormBwdPlan
+  float *sums;  // set by the launcher
   int64_t rows, groups;
   int C;
-  bool rms, part_needed;
+  bool rms;
   int64_t rows_per_group, blocks_per_group;  // set by the launcher, as below
   int warps_per_row;
 };

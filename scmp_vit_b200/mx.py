@@ -275,6 +275,15 @@ class MXLinear(nn.Module):
         bias = linear.bias
         self.register_buffer("bias", None if bias is None else bias.detach().clone())
 
+    def get_extra_state(self):
+        return {"fmt": self.fmt, "scale_exp": self.scale_exp}
+
+    def set_extra_state(self, state):
+        # (the format fixes the buffers' sizes and was chosen with them)
+        if state["fmt"] != self.fmt:
+            raise ValueError(f"saved in {state['fmt']}, this module is {self.fmt}")
+        self.scale_exp = int(state["scale_exp"])
+
     def quantized_weight(self) -> MXTensor:
         return MXTensor.__new__(MXTensor)._set(
             self.data, self.scales, None, self.data.data_ptr(), self.scales.data_ptr(),

@@ -74,7 +74,8 @@ def test_sizes():
             assert lib.scmp_mx_data_size(rows, K, code) == rows * kp // 2
             groups = -(-kp // (4 * _lib.MX_BLOCK[fmt]))
             assert lib.scmp_mx_scale_size(rows, K, code) == -(-rows // 128) * groups * 512
-    for rows, K, code in ((-1, 4, 0), (4, 0, 0), (4, 4, 2), (1 << 31, 4, 0), (4, 1 << 31, 1)):
+    for rows, K, code in ((-1, 4, 0), (4, 0, 0), (4, 4, 2), (1 << 31, 4, 0), (4, 1 << 31, 1),
+                          ((1 << 31) - 1, 4, 0)):
         assert lib.scmp_mx_data_size(rows, K, code) == 0
         assert lib.scmp_mx_scale_size(rows, K, code) == 0
 
@@ -105,6 +106,29 @@ def test_quantize_refusals(args, msg):
     lib = _lib.load()
     assert lib.scmp_mx_quantize(a["x"], a["dtype"], a["rows"], a["K"], a["ld"], a["fmt"],
                                 a["scale_exp"], a["data"], a["scales"], None) == -1
+    assert msg in _lib.last_error()
+
+
+@pytest.mark.parametrize("args,msg", [
+    (dict(x_dtype=3), "dtype"),
+    (dict(ld=31), "ld"),
+    (dict(x=None), "non-NULL"),
+    (dict(M=5, a=None), "non-NULL"),       # past the rows that need no buffers
+    (dict(K=6400, ld=6400, a=None), "non-NULL"),
+    (dict(fmt=1, scale_exp=200), "scale_exp"),
+])
+def test_linear_refusals(args, msg):
+    a = _lib.MxMatmulArgs()
+    a.abi_version, a.M, a.N, a.K = _lib.ABI_VERSION, 4, 4, 32
+    a.a = a.a_scales = a.b = a.b_scales = a.out = 16
+    call = dict(x=16, x_dtype=0, ld=32)
+    for k, v in args.items():
+        if k in call:
+            call[k] = v
+        else:
+            setattr(a, k, v)
+    assert _lib.load().scmp_mx_linear(call["x"], call["x_dtype"], call["ld"], ctypes.byref(a),
+                                      None) == -1
     assert msg in _lib.last_error()
 
 
@@ -261,7 +285,8 @@ def check_product(a, w, fmt, dtype, bias=None, w_exp=0):
     return y
 
 
-SHAPES = [(1, 1, 1), (1, 48, 32), (3, 5, 7), (2, 130, 96), (7, 64, 4104), (17, 200, 64),
+SHAPES = [(1, 1, 1), (1, 48, 32), (3, 5, 7), (2, 130, 96), (1, 300, 6144), (2, 9, 6145),
+          (4, 1030, 1025), (5, 64, 96), (7, 64, 4104), (16, 40, 64), (32, 40, 64), (17, 200, 64),
           (33, 257, 100), (127, 128, 128), (129, 257, 260), (257, 1024, 1024), (200, 511, 352),
           (193, 264, 544), (385, 520, 2080), (64, 4096, 1024), (600, 96, 40), (1500, 300, 288)]
 
@@ -326,6 +351,22 @@ def test_matmul_empty_and_out(cuda_device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("M,K", [(1, 130), (3, 200), (4, 4100), (70, 130)])
+def test_matmul_strided_rows(cuda_device, fmt, M, K):
+    """Rows a distance apart, at offsets off every alignment; a transposed bias."""
+    g = torch.Generator().manual_seed(6)
+    big = torch.randn(M, K + 37, generator=g).to(cuda_device)
+    w = mx.mx_quantize(torch.randn(48, K, generator=g).to(cuda_device), fmt)
+    bias = torch.randn(48, 2, generator=g).to(cuda_device)[:, 1]
+    for dtype in DTYPES:
+        for at in (0, 1, 8):
+            a = big.to(dtype)[:, at:at + K]
+            assert torch.equal(mx.mx_matmul(a, w, bias=bias),
+                               mx.mx_matmul(a.clone(), w, bias=bias.clone()))
+
+
+@pytest.mark.gpu
 def test_matmul_repeats_bit_for_bit(cuda_device):
     """A call made again gives the same bits."""
     g = torch.Generator().manual_seed(3)
@@ -373,8 +414,10 @@ def test_linear(cuda_device, fmt):
     assert torch.equal(m(mx.mx_quantize(x, fmt)), ref)
     again = mx.MXLinear(torch.nn.Linear(96, 72).to(cuda_device), fmt)
     again.load_state_dict(m.state_dict())
-    again.scale_exp = m.scale_exp
     assert torch.equal(again(x), ref)
+    other = mx.MXLinear(torch.nn.Linear(96, 72).to(cuda_device), FMTS[1 - FMTS.index(fmt)])
+    with pytest.raises((ValueError, RuntimeError)):
+        other.load_state_dict(m.state_dict())
 
 
 @pytest.mark.gpu

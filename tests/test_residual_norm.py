@@ -159,7 +159,7 @@ def test_workspace_sizes():
     size = _lib.load().scmp_residual_norm_bwd_workspace
     assert size(0, 8, 1) == 0 and size(4, 0, 1) == 0 and size(4, 8, 3) == 0
     assert size(4, 8, 4) >= 4 * 8 * 4
-    assert size(6, 8, 2) >= (3 + 3) * 4 * 8 * 4
+    assert size(6, 8, 2) >= 3 * 4 * 8 * 4
 
 
 def test_python_refusals_on_cpu():
@@ -388,7 +388,8 @@ def test_backward_fp32_parameters(cuda_device, dtype):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("rows", [(64, 257, 256), (300, 2, 72), (1, 5000, 24)])
+@pytest.mark.parametrize("rows", [(64, 257, 256), (300, 2, 72), (1, 5000, 24), (700, 1, 40),
+                                  (297, 5, 1408), (2, 3000, 1032)])
 def test_backward_many_rows_and_repeats(cuda_device, rows):
     """More rows than slots, more gate groups than blocks; the same bits again."""
     t, kind = make(rows, torch.float32, cuda_device, grad=True, gate=True)

@@ -79,9 +79,14 @@ def test_patched_model_is_its_calls(cuda_device, fmt, dtype):
 @pytest.mark.gpu
 def test_linears_alone_and_beside_sc(cuda_device):
     """Some linears in 4 bits, the attention through SC, positions on."""
-    m = small(cuda_device, rope=True)
-    vit.patch_vit(m, 8, ("qk", "av"))
-    vit.patch_vit_mx(m, ("mlp_fc1",))
+    for ops in (("mlp_fc1",), ("qkv_proj", "mlp_fc2"), vit.MX_OPS):
+        m = small(cuda_device, rope=True)
+        vit.patch_vit(m, 8, ("qk", "av"))
+        vit.patch_vit_mx(m, ops)
+        check_beside_sc(m, cuda_device)
+
+
+def check_beside_sc(m, cuda_device):
     x = torch.randn(2, 3, 56, 56, generator=torch.Generator().manual_seed(3)).to(cuda_device)
     with torch.no_grad():
         a, b = m(x), m(x)
