@@ -98,6 +98,9 @@ __device__ __forceinline__ void copy_scales(uint32_t taddr, uint64_t desc) {
 __device__ __forceinline__ uint64_t scale_desc(uint32_t addr) {
   return (uint64_t)((addr & 0x3FFFFu) >> 4) | (uint64_t)(128u >> 4) << 32 | (uint64_t)1 << 46;
 }
+__device__ __forceinline__ void grid_dependency_wait() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
 __device__ __forceinline__ bool elect_one() {
   uint32_t ok;
   asm volatile(
@@ -224,6 +227,9 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
   cluster_sync_all();  // both CTAs' barriers and tensor memory exist
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  // All of the above may run while the kernel in front of this one in the stream
+  // ends; global memory is touched from here on only.
+  grid_dependency_wait();
   const uint32_t cluster = blockIdx.x >> 1, clusters = gridDim.x >> 1;
   const uint32_t smem0 = smem_u32(smem);
 
@@ -517,8 +523,17 @@ cudaError_t launch(MxTiles t, int64_t kp, int64_t groups, cudaStream_t s) {
       (t.tma_out && !encode_out(&omap, t.p.out, t.p.M, t.p.N)))
     return cudaErrorInvalidValue;
   const unsigned grid = t.tiles < (uint32_t)clusters ? t.tiles : (unsigned)clusters;
-  kern<<<2 * grid, kThreads, Cfg::kSmem, s>>>(t, wmap, xmap, wsmap, xsmap, omap);
-  return cudaGetLastError();
+  cudaLaunchAttribute early[1];
+  early[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2 * grid, 1, 1);
+  cfg.blockDim = dim3(kThreads, 1, 1);
+  cfg.dynamicSmemBytes = Cfg::kSmem;
+  cfg.stream = s;
+  cfg.attrs = early;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, t, wmap, xmap, wsmap, xsmap, omap);
 }
 
 template <int kFmt>

@@ -75,6 +75,8 @@ __global__ void __launch_bounds__(kThreads)
   constexpr int kLanes = kFmt == SCMP_MXFP4 ? 4 : 2;   // lanes per block
   constexpr int kGroups = 8 / kLanes;                  // scale groups per chunk
   __shared__ __align__(16) T deal[kVec ? 8 : kThreads * 8];
+  // (a product behind this launch may set up as SMs become free)
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int lane = threadIdx.x & 31;
   T *const buf = deal + (kVec ? 0 : (threadIdx.x >> 5) * 256);
   const uint32_t warps = gridDim.x * (kThreads / 32);
