@@ -208,10 +208,10 @@ SCMP_API int scmp_split_qkv(const void *qkv, int64_t B, int64_t N, int64_t H, in
  * An operand [rows, K] becomes e2m1 codes with one scale per block along K:
  *   SCMP_MXFP4  blocks of 32, scale 2^E (e8m0), E = floor(log2 max|x|) - 2, at
  *               least -127; scale_exp must be 0
- *   SCMP_NVFP4  blocks of 16, scale s (e4m3) = max|x| / (6 * 2^scale_exp)
- *               rounded to nearest even and at most 448; the block's step is
- *               s * 2^scale_exp (a power of two per tensor, so that no rounding
- *               but the codes' own enters)
+ *   SCMP_NVFP4  blocks of 16, scale s (e4m3) = max|x| / 2^scale_exp times the fp32
+ *               number nearest 1/6 (an fp32 product), rounded to nearest even and
+ *               at most 448; the block's step is s * 2^scale_exp (a power of two
+ *               per tensor, so that no rounding but the codes' own enters)
  * and each code is x / step rounded to nearest even among 0, .5, 1, 1.5, 2, 3,
  * 4, 6, saturating.  A block that holds a NaN or an infinity stands for NaNs.
  * Buffers (16-byte aligned; sizes from scmp_mx_data_size / scmp_mx_scale_size,

@@ -162,7 +162,7 @@ template <int N> __device__ __forceinline__ uint32_t max_bits(const float *v) {
 // the bits `amax`: the block's scale code and the eight element codes.
 //   mxfp4: scale 2^E, E = floor(log2 amax) - 2 (never below -127), read off
 //   amax's exponent field; x * 2^-E is exact wherever it decides a code.
-//   nvfp4: scale s = e4m3(amax * 2^-e / 6), code of the correctly rounded
+//   nvfp4: scale s = e4m3(amax * 2^-e * fl(1/6)), code of the correctly rounded
 //   quotient x * 2^-e / s, from s's correctly rounded reciprocal with one
 //   correction by the remainder (Markstein 1990).  s has 4 significant bits, so
 //   a value on a border between two codes divides to exactly that border and
@@ -184,7 +184,7 @@ __device__ __forceinline__ uint32_t mx_encode8(const float *x, uint32_t amax, fl
     for (int i = 0; i < 8; ++i) q[i] = x[i] * inv;
   } else {
     const float a = __uint_as_float(amax);
-    scale = e4m3_code(__fdiv_rn(kExp ? a * inv_exp : a, 6.0f));
+    scale = e4m3_code((kExp ? a * inv_exp : a) * (1.0f / 6.0f));
     const float s = e4m3_value(scale), r = scale ? __frcp_rn(s) : 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {

@@ -7,9 +7,9 @@ deterministic 4-bit linear that an SC linear is compared with.
 * ``mx_quantize(x, fmt)`` -> ``MXTensor``: e2m1 codes with one scale per block
   of the last dimension.  ``"mxfp4"``: blocks of 32, power-of-two scales
   ``2^(floor(log2 max|x|) - 2)``.  ``"nvfp4"``: blocks of 16, e4m3 scales
-  ``max|x| / 6`` under a power-of-two tensor scale ``2^scale_exp``.  Codes are
-  rounded to nearest even and saturate at 6.  A block with a NaN or an
-  infinity stands for NaNs.
+  ``max|x| * fl32(1/6)`` under a power-of-two tensor scale ``2^scale_exp``.
+  Codes are rounded to nearest even and saturate at 6.  A block with a NaN or
+  an infinity stands for NaNs.
 * ``MXTensor.dequantize()``: the values that the codes stand for.
 * ``mx_matmul(a, b)``: ``a @ b^T`` (+ bias) with fp32 sums; ``a`` may be a
   plain tensor, which is quantised to ``b``'s format on the way in.

@@ -41,7 +41,10 @@ def quantize_ref(x, fmt, scale_exp=0):
         e = np.maximum(np.where(amax > 0, e - 3, -127), -127)
         scale, step = e + 127, 2.0 ** e.astype(np.float64)
     else:
-        scale = nearest(np.minimum(amax / 2.0 ** scale_exp / 6, 448.0), E4M3)
+        # a sixth in fp32: the scale is a choice, and this product is its definition
+        with np.errstate(over="ignore"):
+            sixth = (amax / 2.0 ** scale_exp).astype(np.float32) * np.float32(1 / 6)
+        scale = nearest(np.minimum(sixth.astype(np.float64), 448.0), E4M3)
         step = E4M3[scale] * 2.0 ** scale_exp
     mag = np.where(step[..., None] > 0, np.abs(v) / np.where(step > 0, step, 1)[..., None], 0)
     code = nearest(mag, E2M1)
