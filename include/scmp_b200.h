@@ -219,7 +219,9 @@ SCMP_API int scmp_split_qkv(const void *qkv, int64_t B, int64_t N, int64_t H, in
  *   data    [rows][ceil32(K) / 2] bytes, element 2i in the low nibble of byte i
  *   scales  [ceil(rows / 128)][ceil(blocks / 4)][512] bytes, scale of row r and
  *           block b at (r % 32) * 16 + (r / 32 % 4) * 4 + b % 4 of its atom
- * Element types are enum scmp_dtype.  Asynchronous on `stream`. */
+ * Element types are enum scmp_dtype; pointers are aligned to their elements, and
+ * outputs share no memory with inputs, here and in the two sections below.
+ * Asynchronous on `stream`. */
 enum scmp_mx_format { SCMP_MXFP4 = 0, SCMP_NVFP4 = 1 };
 enum scmp_dtype { SCMP_F32 = 0, SCMP_BF16 = 1, SCMP_F16 = 2 };
 SCMP_API size_t scmp_mx_data_size(int64_t rows, int64_t K, int fmt);

@@ -14,7 +14,6 @@ numerics per slice, but without their host loops:
 """
 from __future__ import annotations
 
-import ctypes
 import math
 from typing import Callable, Optional
 
@@ -402,8 +401,7 @@ class RotaryAxes(nn.Module):
             raise ValueError(f"base must be positive, got {base}")
         self.dims, self.sizes, self.interleaved = dims, sizes, bool(interleaved)
         pad = [0] * (_lib.MAX_AXES - len(dims))
-        self.c_dims = (ctypes.c_int32 * _lib.MAX_AXES)(*dims, *pad)
-        self.c_sizes = (ctypes.c_int32 * _lib.MAX_AXES)(*sizes, *pad)
+        self.c_dims, self.c_sizes = (*dims, *pad), (*sizes, *pad)  # as the C struct takes them
         parts = []
         for d, n, f in zip(dims, sizes, scales):
             freq = torch.exp(torch.arange(0, d, 2, dtype=torch.float64, device=device)

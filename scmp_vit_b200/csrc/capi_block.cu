@@ -31,10 +31,16 @@ constexpr int kMaxScaleExp = 120;        // 2^+-e and its reciprocal are normal 
 
 bool known_dtype(int d) { return d >= SCMP_F32 && d <= SCMP_F16; }
 int64_t dtype_bytes(int d) { return d == SCMP_F32 ? 4 : 2; }
-bool aligned(std::initializer_list<const void *> ptrs, uintptr_t to) {
+bool aligned(std::initializer_list<const void *> ptrs, int64_t to) {
   uintptr_t a = 0;
   for (const void *p : ptrs) a |= reinterpret_cast<uintptr_t>(p);
-  return (a & (to - 1)) == 0;
+  return (a & (uintptr_t)(to - 1)) == 0;
+}
+int check_elements(std::initializer_list<const void *> ptrs, int dtype) {
+  if (!aligned(ptrs, dtype_bytes(dtype)))
+    return fail(SCMP_EINVAL, "a pointer is not aligned to its elements of %lld bytes",
+                (long long)dtype_bytes(dtype));
+  return SCMP_OK;
 }
 
 int check_mx(int64_t rows, int64_t K, int fmt) {
@@ -66,6 +72,9 @@ int check_product(const scmp_mx_matmul_args *args, bool codes, MxProduct &p) {
       return fail(SCMP_EINVAL, "a, b, their scales and out must be non-NULL");
     if (!aligned({x.a, x.a_scales, x.b, x.b_scales}, 16))
       return fail(SCMP_EINVAL, "a, b and their scales must be 16-byte aligned");
+    if ((rc = check_elements({x.out}, x.out_dtype)) != SCMP_OK ||
+        (x.bias && (rc = check_elements({x.bias}, x.bias_dtype)) != SCMP_OK))
+      return rc;
   }
   p.a = static_cast<const uint8_t *>(x.a);
   p.a_scales = static_cast<const uint8_t *>(x.a_scales);
@@ -110,6 +119,7 @@ int scmp_mx_quantize(const void *x, int dtype, int64_t rows, int64_t K, int64_t 
   if (!x || !data || !scales) return fail(SCMP_EINVAL, "x, data and scales must be non-NULL");
   if (!aligned({data, scales}, 16))
     return fail(SCMP_EINVAL, "data and scales must be 16-byte aligned");
+  if ((rc = check_elements({x}, dtype)) != SCMP_OK) return rc;
   const cudaError_t e = launch_mx_quantize(
       x, dtype, ld, mx_layout(rows, K, fmt), fmt, scale_exp, static_cast<uint8_t *>(data),
       static_cast<uint8_t *>(scales), static_cast<cudaStream_t>(stream));
@@ -128,6 +138,7 @@ int scmp_mx_dequantize(const void *data, const void *scales, int64_t rows, int64
   if (!out || !data || !scales) return fail(SCMP_EINVAL, "data, scales and out must be non-NULL");
   if (!aligned({data, scales}, 16))
     return fail(SCMP_EINVAL, "data and scales must be 16-byte aligned");
+  if ((rc = check_elements({out}, dtype)) != SCMP_OK) return rc;
   const cudaError_t e = launch_mx_dequantize(
       static_cast<const uint8_t *>(data), static_cast<const uint8_t *>(scales),
       mx_layout(rows, K, fmt), fmt, scale_exp, out, dtype, static_cast<cudaStream_t>(stream));
@@ -167,6 +178,7 @@ int scmp_mx_linear(const void *x, int x_dtype, int64_t ld, const scmp_mx_matmul_
   if (ld < p.K) return fail(SCMP_EINVAL, "ld=%lld below K=%lld", (long long)ld, (long long)p.K);
   if (p.M == 0 || p.N == 0) return SCMP_OK;
   if (!x) return fail(SCMP_EINVAL, "x must be non-NULL");
+  if ((rc = check_elements({x}, x_dtype)) != SCMP_OK) return rc;
   if (thin) {
     const cudaError_t e = launch_mx_thin(p, x, x_dtype, ld, static_cast<cudaStream_t>(stream));
     if (e != cudaSuccess) return cuda_fail(e, "mx_linear launch");
@@ -203,6 +215,12 @@ int scmp_residual_norm(const scmp_norm_args *args, void *stream) {
                 (long long)x.rows, (long long)x.rows_per_gate);
   if (!x.mx_data != !x.mx_scales)
     return fail(SCMP_EINVAL, "mx_data and mx_scales go together");
+  int rc;
+  if ((rc = check_elements({x.x, x.y, x.r}, x.dtype)) != SCMP_OK ||
+      (rc = check_elements({x.h}, x.h_f32 ? SCMP_F32 : x.dtype)) != SCMP_OK ||
+      (rc = check_elements({x.weight, x.bias, x.gamma, x.gate, x.post_weight, x.post_bias},
+                           x.param_dtype)) != SCMP_OK)
+    return rc;
   NormParams p{};
   p.x = x.x;
   p.y = x.y;
@@ -274,6 +292,12 @@ int scmp_residual_norm_bwd(const scmp_norm_bwd_args *args, void *stream) {
   if (x.gate && (x.rows_per_gate <= 0 || x.rows % x.rows_per_gate != 0))
     return fail(SCMP_EINVAL, "rows=%lld is not a multiple of rows_per_gate=%lld",
                 (long long)x.rows, (long long)x.rows_per_gate);
+  int rc;
+  if ((rc = check_elements({x.r, x.y, x.dr, x.dh, x.dx, x.dy}, x.dtype)) != SCMP_OK ||
+      (rc = check_elements({x.weight, x.gamma, x.gate, x.post_weight, x.post_bias, x.dweight,
+                            x.dbias, x.dgamma, x.dgate, x.dpost_weight, x.dpost_bias},
+                           x.param_dtype)) != SCMP_OK)
+    return rc;
   NormBwdParams p{};
   p.r = x.r;
   p.y = x.y;
@@ -354,7 +378,10 @@ int scmp_split_qkv_rotary(const scmp_rotary_args *args, void *stream) {
                 "B=%lld N=%lld D=%lld tokens", (long long)x.B, (long long)x.N, (long long)x.D);
   if (!x.qkv || !x.q || !x.k || !x.v || !x.table || !x.pos)
     return fail(SCMP_EINVAL, "qkv, q, k, v, table and pos must be non-NULL");
-  if (!aligned({x.table}, 8)) return fail(SCMP_EINVAL, "table must be 8-byte aligned");
+  if (!aligned({x.table}, 8) || !aligned({x.pos}, 4))
+    return fail(SCMP_EINVAL, "table must be 8-byte and pos 4-byte aligned");
+  const int rc = check_elements({x.qkv, x.q, x.k, x.v}, x.dtype);
+  if (rc != SCMP_OK) return rc;
   p.qkv = x.qkv;
   p.q = x.q;
   p.k = x.k;

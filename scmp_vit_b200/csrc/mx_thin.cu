@@ -48,6 +48,17 @@ template <int kFmt> __device__ __forceinline__ float scale_value(uint32_t code) 
 __device__ __forceinline__ __half2 as_half2(uint32_t w) {
   return *reinterpret_cast<const __half2 *>(&w);
 }
+// Smaller and larger of two scales, a NaN if either is one.
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 // Sum of eight products, exact in fp16 until the two halves meet in fp32.
 __device__ __forceinline__ float dot8(const uint4 &w, const uint4 &x) {
   __half2 a = __hmul2(as_half2(w.x), as_half2(x.x));
@@ -176,8 +187,8 @@ __global__ void __launch_bounds__(kThreads)
           const float *sx = scales + m * blocks + k / kBlock;
           const float lo = dot8(c[0], v[0]) + dot8(c[1], v[quarter]);
           const float hi = dot8(c[2], v[2 * quarter]) + dot8(c[3], v[3 * quarter]);
-          if (kFmt == SCMP_MXFP4)
-            acc[m] = __fmaf_rn((lo + hi) * s.s0, sx[0], acc[m]);
+          if (kFmt == SCMP_MXFP4)  // the smaller scale first: nothing leaves fp32's range on the way
+            acc[m] = __fmaf_rn((lo + hi) * min_nan(s.s0, sx[0]), max_nan(s.s0, sx[0]), acc[m]);
           else
             acc[m] = __fmaf_rn(lo * s.s0, sx[0], __fmaf_rn(hi * s.s1, sx[1], acc[m]));
         }

@@ -108,6 +108,11 @@ class MXTensor:
     def dim(self) -> int:
         return len(self.shape)
 
+    def __reduce__(self):
+        # copies and loaded tensors are other memory: no address is carried over
+        return MXTensor, (self.data, self.scales, tuple(self.shape), self.fmt, self.scale_exp,
+                          self.dtype)
+
     def reshape(self, *shape) -> "MXTensor":
         """The same codes under other leading dimensions; the last one stays."""
         shape = shape[0] if len(shape) == 1 and not isinstance(shape[0], int) else shape
@@ -155,6 +160,15 @@ def _rows_of(x: torch.Tensor):
     if (K > 1 and x2.stride(1) != 1) or (x2.shape[0] > 1 and x2.stride(0) < K):
         x2 = x2.contiguous()
     return x2, (x2.stride(0) if x2.shape[0] > 1 else K)
+
+
+def _overlap(out: torch.Tensor, t: torch.Tensor) -> bool:
+    """Whether contiguous ``out`` and ``t`` (its span, where strided) share bytes."""
+    if t.numel() == 0 or out.numel() == 0:
+        return False
+    span = sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1
+    start, end = out.data_ptr(), out.data_ptr() + out.numel() * out.element_size()
+    return t.data_ptr() < end and start < t.data_ptr() + span * t.element_size()
 
 
 def _check_input(x: torch.Tensor, name: str) -> int:
@@ -211,15 +225,20 @@ def mx_matmul(a: Union[torch.Tensor, MXTensor], b: MXTensor, *,
     else:
         rows = a.rows
     shape = (*a.shape[:-1], N)
-    if out is None:
+    given = out is not None
+    if not given:
         dtype = a.dtype if out_dtype is None else out_dtype
         out_code = dtype_code(dtype, "out")
         out = torch.empty(shape, dtype=dtype, device=b.device)
     else:
+        _no_grad_wanted("mx_matmul", out)
         if (tuple(out.shape) != shape or not out.is_contiguous() or out.get_device() != index
                 or out_dtype not in (None, out.dtype)):
             raise ValueError(f"out must be contiguous {shape} on {b.device} of out_dtype")
         out_code = dtype_code(out.dtype, "out")
+        for t in (a if plain else None, bias):
+            if t is not None and _overlap(out, t):
+                raise ValueError("out shares memory with an input")
     bias_code, bias_ptr = 0, None
     if bias is not None:
         if bias.shape != (N,) or bias.get_device() != index:
@@ -229,7 +248,6 @@ def mx_matmul(a: Union[torch.Tensor, MXTensor], b: MXTensor, *,
         _no_grad_wanted("mx_matmul", bias)
         bias = bias if bias.is_contiguous() else bias.detach().contiguous()
         bias_ptr = bias.data_ptr()
-    _no_grad_wanted("mx_matmul", out)
     args = _lib.MxMatmulArgs(
         _lib.ABI_VERSION, _lib.MX_FORMAT[b.fmt], None if qa is None else qa.data_ptr,
         None if qa is None else qa.scales_ptr, b.data_ptr, b.scales_ptr, rows, N, K,
@@ -240,6 +258,8 @@ def mx_matmul(a: Union[torch.Tensor, MXTensor], b: MXTensor, *,
         call(_lib.load().scmp_mx_linear, index, x.data_ptr(), x_code, ld, args)
     else:
         call(_lib.load().scmp_mx_matmul, index, args)
+    if given:
+        torch.autograd.graph.increment_version(out)  # a write in place, as autograd counts them
     return out
 
 

@@ -1,7 +1,9 @@
 """Microscaled 4-bit floating point: quantisation byte for byte against a
 search over the representable values in 64 bits, the product against the
 64-bit product of the dequantised operands, and the refusals."""
+import copy
 import ctypes
+import pickle
 
 import numpy as np
 import pytest
@@ -102,6 +104,8 @@ def test_struct_layouts_match_the_header():
     (dict(data=0), "non-NULL"),
     (dict(data=24), "aligned"),
     (dict(scales=8), "aligned"),
+    (dict(x=18), "aligned to its elements"),
+    (dict(x=17, dtype=1), "aligned to its elements"),
 ])
 def test_quantize_refusals(args, msg):
     a = dict(x=16, dtype=0, rows=4, K=8, ld=8, fmt=0, scale_exp=0, data=16, scales=16)
@@ -119,6 +123,7 @@ def test_quantize_refusals(args, msg):
     (dict(M=5, a=None), "non-NULL"),       # past the rows that need no buffers
     (dict(K=6400, ld=6400, a=None), "non-NULL"),
     (dict(fmt=1, scale_exp=200), "scale_exp"),
+    (dict(x=18), "aligned to its elements"),
 ])
 def test_linear_refusals(args, msg):
     a = _lib.MxMatmulArgs()
@@ -146,6 +151,8 @@ def test_linear_refusals(args, msg):
     (dict(a=None), "non-NULL"),
     (dict(out=None), "non-NULL"),
     (dict(b_scales=8), "aligned"),
+    (dict(out=18), "aligned to its elements"),
+    (dict(bias=17, bias_dtype=2), "aligned to its elements"),
 ])
 def test_matmul_refusals(args, msg):
     a = _lib.MxMatmulArgs()
@@ -155,6 +162,20 @@ def test_matmul_refusals(args, msg):
         setattr(a, k, v)
     assert _lib.load().scmp_mx_matmul(ctypes.byref(a), None) == -1
     assert msg in _lib.last_error()
+
+
+def test_copies_are_tensors_of_their_own():
+    """A copied or loaded MXTensor points at its own bytes, not at the first one's."""
+    q = mx.mx_empty(torch.Size((5, 40)), "nvfp4", torch.device("cpu"), torch.bfloat16, 3)
+    q.data.copy_(torch.arange(q.data.numel()) % 251)
+    q.scales.copy_(torch.arange(q.scales.numel()) % 127)
+    for c in (copy.deepcopy(q), pickle.loads(pickle.dumps(q))):
+        assert c.data_ptr == c.data.data_ptr() and c.scales_ptr == c.scales.data_ptr()
+        assert c.data_ptr != q.data_ptr and c.scales_ptr != q.scales_ptr
+        assert torch.equal(c.data, q.data) and torch.equal(c.scales, q.scales)
+        assert (c.shape, c.rows, c.fmt, c.scale_exp, c.dtype) == ((5, 40), 5, "nvfp4", 3,
+                                                                   torch.bfloat16)
+    assert copy.copy(q).data_ptr == q.data_ptr
 
 
 def test_python_refusals_on_cpu():
@@ -336,6 +357,39 @@ def test_matmul_wide_scales(cuda_device, M):
     a[:, :32] *= 2.0 ** 40
     w[:, 32:64] *= 2.0 ** -60
     check_product(a.to(cuda_device), w.to(cuda_device), "mxfp4", torch.float32)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [1, 3, 4, 40, 300])
+@pytest.mark.parametrize("big,small", [(2.0 ** 120, 2.0 ** -110), (2.0 ** -110, 2.0 ** 120)])
+def test_matmul_scales_that_meet(cuda_device, M, big, small):
+    """Scales near both ends of fp32 whose products are ordinary numbers: no step
+    on the way overflows."""
+    g = torch.Generator().manual_seed(8)
+    a, w = torch.randn(M, 256, generator=g) * big, torch.randn(80, 256, generator=g) * small
+    check_product(a.to(cuda_device), w.to(cuda_device), "mxfp4", torch.float32)
+
+
+@pytest.mark.gpu
+def test_matmul_out_counts_as_a_write(cuda_device):
+    """autograd notices that a tensor it saved was written, and out that shares
+    memory with an input is refused."""
+    w = mx.mx_quantize(torch.randn(64, 64, device=cuda_device))
+    leaf = torch.randn(3, 64, device=cuda_device, requires_grad=True)
+    out = torch.randn(3, 64, device=cuda_device)
+    y = (leaf * out).sum()
+    with torch.no_grad():
+        mx.mx_matmul(leaf, w, out=out)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    buf = torch.randn(7, 64, device=cuda_device)
+    with pytest.raises(ValueError, match="shares memory"):
+        mx.mx_matmul(buf[:3], w, out=buf[:3])
+    with pytest.raises(ValueError, match="shares memory"):
+        mx.mx_matmul(buf[:3], w, out=buf[2:5])
+    with pytest.raises(ValueError, match="shares memory"):
+        mx.mx_matmul(buf[:3], w, out=buf[4:7], bias=buf[6])
+    assert torch.equal(mx.mx_matmul(buf[:3], w, out=buf[3:6]), mx.mx_matmul(buf[:3], w))
 
 
 @pytest.mark.gpu

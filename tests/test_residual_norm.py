@@ -125,6 +125,9 @@ def norm_args(**kw):
     (dict(mx_data=16, mx_scales=16, mx_fmt=2), -1, "format"),
     (dict(mx_data=16, mx_scales=16, C=7), -4, "16-byte"),
     (dict(mx_data=16, mx_scales=16, x=20), -4, "16-byte"),
+    (dict(x=18), -1, "aligned to its elements"),
+    (dict(dtype=1, weight=17, param_dtype=1), -1, "aligned to its elements"),
+    (dict(dtype=1, h=18, h_f32=1), -1, "aligned to its elements"),
 ])
 def test_forward_refusals(kw, code, msg):
     assert _lib.load().scmp_residual_norm(ctypes.byref(norm_args(**kw)), None) == code
@@ -143,6 +146,8 @@ def test_forward_refusals(kw, code, msg):
     (dict(y=16, gate=16, rows_per_gate=3), -1, "rows_per_gate"),
     (dict(dweight=16), -3, "workspace"),
     (dict(dweight=16, workspace=16, workspace_bytes=4), -3, "workspace"),
+    (dict(dx=18), -1, "aligned to its elements"),
+    (dict(dbias=18), -1, "aligned to its elements"),
 ])
 def test_backward_refusals(kw, code, msg):
     a = _lib.NormBwdArgs()

@@ -2,14 +2,16 @@
 values, gradient, layouts and refusals.  A turned element is one product and
 one fused multiply-add of fp32 numbers whose cos and sin are rounded once:
 off by at most 3 2^-24 (|u| + |v|), plus its type's half step."""
+import copy
 import ctypes
 import math
+import pickle
 
 import pytest
 import torch
 
 from scmp_vit_b200 import _lib
-from scmp_vit_b200.attention import RotaryAxes, split_qkv, split_qkv_rotary
+from scmp_vit_b200.attention import GridRotary, RotaryAxes, split_qkv, split_qkv_rotary
 
 DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 U = 2.0 ** -24
@@ -63,6 +65,8 @@ def close(got, ref, mag):
     (dict(dims=(8, 10)), -1, "exceed"),
     (dict(pos=None), -1, "non-NULL"),
     (dict(table=12), -1, "aligned"),
+    (dict(pos=18), -1, "aligned"),
+    (dict(k=18), -1, "aligned to its elements"),
     (dict(B=1 << 20, N=1 << 20), -4, "tokens"),
 ])
 def test_refusals(kw, code, msg):
@@ -93,6 +97,15 @@ def test_python_refusals_on_cpu():
     axes = RotaryAxes([8, 8], [4, 4])
     with pytest.raises(RuntimeError, match="no CPU path"):
         split_qkv_rotary(torch.zeros(1, 2, 96), 2, axes, torch.zeros(2, 2, dtype=torch.int32))
+
+
+def test_copies():
+    """Modules with positions are copied and pickled like others."""
+    rope = GridRotary((3, 2), 8)
+    for c in (copy.deepcopy(rope), pickle.loads(pickle.dumps(rope))):
+        assert c.axes.dims == [4, 4] and c.axes.sizes == [3, 2]
+        assert torch.equal(c.axes.table_bits, rope.axes.table_bits)
+        assert torch.equal(c.pos, rope.pos)
 
 
 def test_table():
