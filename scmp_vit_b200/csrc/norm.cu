@@ -56,20 +56,55 @@ template <typename T, int V> __device__ __forceinline__ void store_v(T *p, const
       *reinterpret_cast<uint4 *>(p + i) = pack16<T>(v + i);
   }
 }
-
-__device__ __forceinline__ float2 warp_sum(float2 v) {
+// The same, and v becomes the rounded values.
+template <typename T, int V> __device__ __forceinline__ void store_rounded(T *p, float *v) {
+  if (V == 1) {
+    const T t = from_f32<T>(v[0]);
+    *p = t;
+    v[0] = to_f32(t);
+  } else {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    v.x += __shfl_xor_sync(~0u, v.x, o);
-    v.y += __shfl_xor_sync(~0u, v.y, o);
+    for (int i = 0; i < V; i += kVec16<T>) {
+      const uint4 u = pack16<T>(v + i);
+      *reinterpret_cast<uint4 *>(p + i) = u;
+      unpack16<T>(u, v + i);
+    }
   }
-  return v;
 }
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
-  return v;
+
+// Two fp32 operations in one instruction: rows of 16-bit types are bound by
+// instructions, not by HBM.
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n.reg .b64 a, b;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\n"
+      "add.rn.f32x2 a, a, b;\nmov.b64 {%0, %1}, a;\n}\n"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
 }
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n.reg .b64 a, b;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\n"
+      "mul.rn.f32x2 a, a, b;\nmov.b64 {%0, %1}, a;\n}\n"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{\n.reg .b64 a, b, c;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nmov.b64 c, {%6, %7};\n"
+      "fma.rn.f32x2 a, a, b, c;\nmov.b64 {%0, %1}, a;\n}\n"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
+// The E values of a lane, chunk j's V from element j V on, as pairs.
+template <int E> struct Values {
+  float2 p[E / 2];
+  __device__ __forceinline__ float *at(int e) { return reinterpret_cast<float *>(p) + e; }
+};
 
 constexpr int kMaxWarps = 16;
 
@@ -77,58 +112,76 @@ constexpr int kMaxWarps = 16;
 // Two buffers in turn: a warp writes one again only after the barrier that
 // follows every read of it.
 struct RowSum {
-  float2 *buf;  // this slot's warps in [2][kMaxWarps]
+  float2 *buf;  // this slot's warps in [2][kMaxWarps], an even number (the last may be 0)
   int G, w, barrier, turn;
   __device__ RowSum(float2 *all, int G_, int slot, int w_)
-      : buf(all + slot * G_), G(G_), w(w_), barrier(1 + slot), turn(0) {}
-  __device__ __forceinline__ float2 meet(float2 v) {
-    float2 *b = buf + turn * kMaxWarps;
+      : buf(all + slot * ((G_ + 1) & ~1)), G(G_), w(w_), barrier(1 + slot), turn(0) {
+    if ((G & 1) && w == 0 && (threadIdx.x & 31) == 0)
+      buf[G] = buf[kMaxWarps + G] = make_float2(0.f, 0.f);
+  }
+  __device__ __forceinline__ float2 meet() {
+    const float4 *b = reinterpret_cast<const float4 *>(buf + turn * kMaxWarps);
     turn ^= 1;
-    if ((threadIdx.x & 31) == 0) b[w] = v;
     asm volatile("bar.sync %0, %1;" ::"r"(barrier), "r"(G * 32) : "memory");
-    v = make_float2(0.f, 0.f);
-    for (int i = 0; i < G; ++i) {
-      v.x += b[i].x;
-      v.y += b[i].y;
+    float2 v = make_float2(0.f, 0.f);
+    const auto add = [&](int i) {
+      if (2 * i >= G) return;
+      const float4 f = b[i];
+      v.x += f.x;
+      v.y += f.y;
+      v.x += f.z;
+      v.y += f.w;
+    };
+#pragma unroll
+    for (int i = 0; i < 4; ++i) add(i);
+    if (G > 8) {
+#pragma unroll
+      for (int i = 4; i < kMaxWarps / 2; ++i) add(i);
     }
     return v;
   }
+  // (half the lanes go on with x, the others with y)
   __device__ __forceinline__ float2 operator()(float2 v) {
-    v = warp_sum(v);
-    return G == 1 ? v : meet(v);
+    const bool hi = threadIdx.x & 16;
+    float a = hi ? v.y : v.x;
+    a += __shfl_xor_sync(~0u, hi ? v.x : v.y, 16);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) a += __shfl_xor_sync(~0u, a, o);
+    if (G == 1) return make_float2(__shfl_sync(~0u, a, 0), __shfl_sync(~0u, a, 16));
+    if ((threadIdx.x & 15) == 0)
+      reinterpret_cast<float *>(buf + turn * kMaxWarps + w)[hi ? 1 : 0] = a;
+    return meet();
   }
   __device__ __forceinline__ float operator()(float v) {
-    v = warp_sum(v);
-    return G == 1 ? v : meet(make_float2(v, 0.f)).x;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
+    if (G == 1) return v;
+    if ((threadIdx.x & 31) == 0) buf[turn * kMaxWarps + w] = make_float2(v, 0.f);
+    return meet().x;
   }
 };
 
 // v (0 past the row, where in(j) is false) -> N(v) and its statistics.
-template <int NV, int V, typename In>
-__device__ __forceinline__ float2 normalise(float (&v)[NV][V], const In &in, RowSum &sum,
-                                            float inv_c, float eps, bool rms) {
+template <int V, int E, typename In>
+__device__ __forceinline__ float2 normalise(Values<E> &v, const In &in, RowSum &sum, float inv_c,
+                                            float eps, bool rms) {
   float mean = 0.f;
   if (!rms) {
-    float s = 0.f;
+    float2 s = make_float2(0.f, 0.f);
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
+    for (int i = 0; i < E / 2; ++i) s = add2(s, v.p[i]);
+    mean = sum(s.x + s.y) * inv_c;
 #pragma unroll
-      for (int i = 0; i < V; ++i) s += v[j][i];
-    mean = sum(s) * inv_c;
+    for (int i = 0; i < E / 2; ++i)  // (what lies past the row stays 0)
+      v.p[i] = add2(v.p[i], make_float2(in(2 * i / V) ? -mean : 0.f,
+                                        in((2 * i + 1) / V) ? -mean : 0.f));
   }
-  float q = 0.f;
+  float2 q = make_float2(0.f, 0.f);
 #pragma unroll
-  for (int j = 0; j < NV; ++j)
+  for (int i = 0; i < E / 2; ++i) q = fma2(v.p[i], v.p[i], q);
+  const float rstd = 1.0f / sqrtf(__fmaf_rn(sum(q.x + q.y), inv_c, eps));
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      v[j][i] = in(j) ? v[j][i] - mean : 0.f;
-      q = __fmaf_rn(v[j][i], v[j][i], q);
-    }
-  const float rstd = 1.0f / sqrtf(__fmaf_rn(sum(q), inv_c, eps));
-#pragma unroll
-  for (int j = 0; j < NV; ++j)
-#pragma unroll
-    for (int i = 0; i < V; ++i) v[j][i] *= rstd;
+  for (int i = 0; i < E / 2; ++i) v.p[i] = mul2(v.p[i], both(rstd));
   return make_float2(mean, rstd);
 }
 
@@ -172,7 +225,7 @@ __global__ void __launch_bounds__(256, E == 16 ? 3 : 1)
     residual_norm_kernel(const __grid_constant__ NormParams p) {
   constexpr bool kWalk = E > 8;
   constexpr int NV = E / V;
-  __shared__ float2 buf[2 * kMaxWarps];
+  __shared__ __align__(16) float2 buf[2 * kMaxWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int G = p.warps_per_row, slot = warp / G, w = warp - slot * G;
   const int slots = blockDim.x / (32 * G);
@@ -203,83 +256,114 @@ __global__ void __launch_bounds__(256, E == 16 ? 3 : 1)
     const bool live = row < p.rows;
     const auto in = [&](int j) { return live && in_row(j); };
     const int64_t at = row * C;
-    float r[NV][V];
+    Values<E> r;
     if (p.y) {
 #pragma unroll
-      for (int j = 0; j < NV; ++j) y[j].get(r[j]);
+      for (int j = 0; j < NV; ++j) y[j].get(r.at(j * V));
       if (p.post_weight) {
-        const float2 st = normalise<NV, V>(r, in, sum, inv_c, p.eps, p.rms);
+        const float2 st = normalise<V, E>(r, in, sum, inv_c, p.eps, p.rms);
         if (p.stats && live && w == 0 && lane == 0) p.stats[p.rows + row] = st;
       }
-      const int64_t gate_at = p.gate && live ? row / p.rows_per_gate * C : 0;
+      const int64_t gate_at = p.gate && live ? (int64_t)p.per_gate.quotient((uint32_t)row) * C : 0;
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         const int c = col_of<V>(j, G, w, lane);
+        float *const rj = r.at(j * V);
         if (!in(j)) {
 #pragma unroll
-          for (int i = 0; i < V; ++i) r[j][i] = 0.f;
+          for (int i = 0; i < V; ++i) rj[i] = 0.f;
           continue;
         }
-        float f[V], g[V];
+        constexpr int N2 = V > 1 ? V / 2 : 1;
+        float2 z[N2], f[N2], g[N2];
+        const auto load2 = [&](const void *src, int64_t at, float2 *to) {
+          if (V == 1) to[0].y = 0.f;
+          load_v<P, V>(static_cast<const P *>(src) + at, &to[0].x);
+        };
+#pragma unroll
+        for (int i = 0; i < N2; ++i)
+          z[i] = make_float2(rj[2 * i], V > 1 ? rj[2 * i + (V > 1)] : 0.f);
         if (p.post_weight) {
-          load_v<P, V>(static_cast<const P *>(p.post_weight) + c, f);
-#pragma unroll
-          for (int i = 0; i < V; ++i) r[j][i] *= f[i];
+          load2(p.post_weight, c, f);
           if (p.post_bias) {
-            load_v<P, V>(static_cast<const P *>(p.post_bias) + c, f);
+            load2(p.post_bias, c, g);
 #pragma unroll
-            for (int i = 0; i < V; ++i) r[j][i] += f[i];
+            for (int i = 0; i < N2; ++i) z[i] = add2(mul2(z[i], f[i]), g[i]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < N2; ++i) z[i] = mul2(z[i], f[i]);
           }
         }
 #pragma unroll
-        for (int i = 0; i < V; ++i) f[i] = 1.0f;
-        if (p.gamma) load_v<P, V>(static_cast<const P *>(p.gamma) + c, f);
+        for (int i = 0; i < N2; ++i) f[i] = both(1.0f);
+        if (p.gamma) load2(p.gamma, c, f);
         if (p.gate) {
-          load_v<P, V>(static_cast<const P *>(p.gate) + gate_at + c, g);
+          load2(p.gate, gate_at + c, g);
 #pragma unroll
-          for (int i = 0; i < V; ++i) f[i] *= g[i];
+          for (int i = 0; i < N2; ++i) f[i] = mul2(f[i], g[i]);
         }
-        x[j].get(g);
+        x[j].get(&g[0].x);
+        if (V == 1) g[0].y = 0.f;
+#pragma unroll
+        for (int i = 0; i < N2; ++i) {
+          z[i] = fma2(z[i], f[i], g[i]);
+          rj[2 * i] = z[i].x;
+          if (V > 1) rj[2 * i + (V > 1)] = z[i].y;
+        }
         // r is rounded to its type once, and the norm sees the rounded value:
         // the one that the next block and the backward pass read
-#pragma unroll
-        for (int i = 0; i < V; ++i)
-          r[j][i] = to_f32(from_f32<T>(__fmaf_rn(r[j][i], f[i], g[i])));
-        store_v<T, V>(static_cast<T *>(p.r) + at + c, r[j]);
+        store_rounded<T, V>(static_cast<T *>(p.r) + at + c, rj);
       }
     } else {
 #pragma unroll
-      for (int j = 0; j < NV; ++j) x[j].get(r[j]);
+      for (int j = 0; j < NV; ++j) x[j].get(r.at(j * V));
     }
     if (kWalk) load(row + stride);
-    const float2 st = normalise<NV, V>(r, in, sum, inv_c, p.eps, p.rms);
+    const float2 st = normalise<V, E>(r, in, sum, inv_c, p.eps, p.rms);
     if (p.stats && live && w == 0 && lane == 0) p.stats[row] = st;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int c = col_of<V>(j, G, w, lane);
+      float *const rj = r.at(j * V);
       if (in(j)) {
-        float f[V], g[V];
-        load_v<P, V>(static_cast<const P *>(p.weight) + c, f);
-        if (p.bias) {
-          load_v<P, V>(static_cast<const P *>(p.bias) + c, g);
+        constexpr int N2 = V > 1 ? V / 2 : 1;
+        float2 z[N2], f[N2], g[N2];
+        const auto load2 = [&](const void *src, float2 *to) {
+          if (V == 1) to[0].y = 0.f;
+          load_v<P, V>(static_cast<const P *>(src) + c, &to[0].x);
+        };
 #pragma unroll
-          for (int i = 0; i < V; ++i) r[j][i] = __fmaf_rn(r[j][i], f[i], g[i]);
+        for (int i = 0; i < N2; ++i)
+          z[i] = make_float2(rj[2 * i], V > 1 ? rj[2 * i + (V > 1)] : 0.f);
+        load2(p.weight, f);
+        if (p.bias) {
+          load2(p.bias, g);
+#pragma unroll
+          for (int i = 0; i < N2; ++i) z[i] = fma2(z[i], f[i], g[i]);
         } else {
 #pragma unroll
-          for (int i = 0; i < V; ++i) r[j][i] *= f[i];
+          for (int i = 0; i < N2; ++i) z[i] = mul2(z[i], f[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < N2; ++i) {
+          rj[2 * i] = z[i].x;
+          if (V > 1) rj[2 * i + (V > 1)] = z[i].y;
         }
         if (p.h) {
           if (p.h_f32)
-            store_v<float, V>(static_cast<float *>(p.h) + at + c, r[j]);
+            store_v<float, V>(static_cast<float *>(p.h) + at + c, rj);
           else
-            store_v<T, V>(static_cast<T *>(p.h) + at + c, r[j]);
+            store_v<T, V>(static_cast<T *>(p.h) + at + c, rj);
         }
+      } else {  // (0 times a deviation's reciprocal that is infinite)
+#pragma unroll
+        for (int i = 0; i < V; ++i) rj[i] = 0.f;
       }
       if (V > 1 && p.mx_data) {
         if (p.fmt == SCMP_MXFP4)
-          store_mx<SCMP_MXFP4, V>(p, r[j], row, c, lane);
+          store_mx<SCMP_MXFP4, V>(p, rj, row, c, lane);
         else
-          store_mx<SCMP_NVFP4, V>(p, r[j], row, c, lane);
+          store_mx<SCMP_NVFP4, V>(p, rj, row, c, lane);
       }
     }
   }
@@ -287,48 +371,48 @@ __global__ void __launch_bounds__(256, E == 16 ? 3 : 1)
 
 // ---------------------------------------------------------------- backward
 // Rows of one gate group (all rows without a gate) are dealt to row slots of G
-// warps; a block holds a few slots of one group.  While a row is worked on, the
-// slot's next row is on its way into registers.  Column sums stay in registers
+// warps; a block holds a few slots of one group.  Column sums stay in registers
 // over a slot's rows, are added over the block's slots in shared memory in a
 // fixed order and written as partials [group][block][part][C]; a second kernel
 // adds those in order, so the result does not depend on timing.
 //   parts: 0 sum dh n   1 sum dh   2 sum g z (no post norm) or sum g m   3 sum g
 // E = 8 elements per lane for rows of up to 2048 in 16-byte pieces, else 16.
-template <typename T, int V, int NV> struct BwdRow {
-  Pack<T, V> r[NV], y[NV], dr[NV], dh[NV];
-  float2 st, st_y;
+//
+// A slot's next rows are on their way into a ring of stages in shared memory,
+// each thread copying what it will read itself.
+template <typename T, int V, int E, int kThreads> struct BwdCfg {
+  static constexpr int kPieces = E * (int)sizeof(T) / 16;  // 16-byte pieces per array and lane
+  static constexpr int kStages = V == 1 ? 0
+                                 : E == 8 || kThreads == 256 ? (sizeof(T) == 2 ? 4 : 3)
+                                                             : (sizeof(T) == 2 ? 3 : 0);
+  // bytes per thread and stage; each warp's two statistics behind them
+  static constexpr int kStageBytes = 4 * kPieces * 16;
 };
-template <typename T, int V, int NV>
-__device__ __forceinline__ void load_row(const NormBwdParams &p, int64_t row, bool live, int G,
-                                         int w, int lane, bool post, BwdRow<T, V, NV> &q) {
-  q.st = q.st_y = make_float2(0.f, 0.f);
-  if (live) {
-    q.st = p.stats[row];
-    if (post) q.st_y = p.stats[p.rows + row];
-  }
-  const int64_t at = row * p.C;
-#pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    const int c = col_of<V>(j, G, w, lane);
-    q.r[j].zero();
-    q.y[j].zero();
-    q.dr[j].zero();
-    q.dh[j].zero();
-    if (!live || c >= p.C) continue;
-    q.r[j].load(static_cast<const T *>(p.r) + at + c);
-    if (p.dh) q.dh[j].load(static_cast<const T *>(p.dh) + at + c);
-    if (p.dr) q.dr[j].load(static_cast<const T *>(p.dr) + at + c);
-    if (p.y) q.y[j].load(static_cast<const T *>(p.y) + at + c);
-  }
+__device__ __forceinline__ void copy_async16(void *dst, const void *src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                   (uint32_t)__cvta_generic_to_shared(dst)),
+               "l"(src)
+               : "memory");
+}
+__device__ __forceinline__ void copy_async8(void *dst, const void *src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(
+                   (uint32_t)__cvta_generic_to_shared(dst)),
+               "l"(src)
+               : "memory");
 }
 
 template <typename T, typename P, int V, int E, bool kPost, int kThreads>
 __global__ void __launch_bounds__(kThreads, E == 8 ? 2 : 1)
     residual_norm_bwd_kernel(const __grid_constant__ NormBwdParams p) {
+  using Cfg = BwdCfg<T, V, E, kThreads>;
   constexpr int NV = E / V;
   constexpr int kParts = kPost ? 4 : 3;
-  __shared__ float2 buf[2 * kMaxWarps];
-  extern __shared__ float part_smem[];  // [C], blocks of several slots
+  constexpr int kStages = Cfg::kStages, kPieces = Cfg::kPieces;
+  constexpr bool kHeld = !(kPost && E == 8);  // parameters in registers, else in shared memory
+  __shared__ __align__(16) float2 buf[2 * kMaxWarps];
+  __shared__ float2 stat_ring[kStages > 0 ? kStages : 1][kMaxWarps][2];
+  extern __shared__ __align__(16) unsigned char smem[];
+  float *const part_smem = reinterpret_cast<float *>(smem);  // [C], once the rows are done
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int G = p.warps_per_row, slot = warp / G, w = warp - slot * G;
   const int slots = blockDim.x / (32 * G);
@@ -339,110 +423,211 @@ __global__ void __launch_bounds__(kThreads, E == 8 ? 2 : 1)
   const int64_t stride = p.blocks_per_group * slots;
   const int64_t row0 = group * p.rows_per_group;
 
-  // the parameters of this lane's columns stay the same over the rows
-  float wt[NV][V], sc[NV][V], pw[kPost ? NV : 1][V];
-#pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    const int c = col_of<V>(j, G, w, lane);
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      wt[j][i] = 0.f;
-      sc[j][i] = 1.f;
-      if (kPost) pw[kPost ? j : 0][i] = 0.f;
-    }
-    if (c >= C) continue;
-    load_v<P, V>(static_cast<const P *>(p.weight) + c, wt[j]);
-    if (p.gamma) load_v<P, V>(static_cast<const P *>(p.gamma) + c, sc[j]);
-    if (p.gate) {
-      float g[V];
-      load_v<P, V>(static_cast<const P *>(p.gate) + group * C + c, g);
-#pragma unroll
-      for (int i = 0; i < V; ++i) sc[j][i] *= g[i];
-    }
-    if (kPost) load_v<P, V>(static_cast<const P *>(p.post_weight) + c, pw[kPost ? j : 0]);
-  }
-  float acc[kParts][NV][V];
-#pragma unroll
-  for (int k = 0; k < kParts; ++k)
-#pragma unroll
-    for (int j = 0; j < NV; ++j)
-#pragma unroll
-      for (int i = 0; i < V; ++i) acc[k][j][i] = 0.f;
-
-  int64_t i_row = (blockIdx.x % p.blocks_per_group) * slots + slot;
-  BwdRow<T, V, NV> next;
-  load_row<T, V, NV>(p, row0 + i_row, i_row < p.rows_per_group, G, w, lane, kPost, next);
-  for (; i_row < p.rows_per_group; i_row += stride) {
-    const BwdRow<T, V, NV> q = next;
-    load_row<T, V, NV>(p, row0 + i_row + stride, i_row + stride < p.rows_per_group, G, w, lane,
-                       kPost, next);
-    const int64_t at = (row0 + i_row) * C;
-    float n[NV][V], dn[NV][V];
-    float2 s = make_float2(0.f, 0.f);
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const bool in = col_of<V>(j, G, w, lane) < C;
-      q.r[j].get(n[j]);
-      q.dh[j].get(dn[j]);
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        n[j][i] = in ? (n[j][i] - q.st.x) * q.st.y : 0.f;
-        acc[0][j][i] = __fmaf_rn(dn[j][i], n[j][i], acc[0][j][i]);
-        acc[1][j][i] += dn[j][i];
-        dn[j][i] *= wt[j][i];
-        s.x += dn[j][i];
-        s.y = __fmaf_rn(dn[j][i], n[j][i], s.y);
+  // [stage][array][piece][thread], then the parameters in shared memory
+  uint4 *const ring = reinterpret_cast<uint4 *>(smem) + threadIdx.x;
+  const int per_array = kPieces * (int)blockDim.x, per_stage = 4 * per_array;
+  const T *const array[4] = {static_cast<const T *>(p.r), static_cast<const T *>(p.dh),
+                             static_cast<const T *>(p.dr), static_cast<const T *>(p.y)};
+  const auto fetch = [&](int64_t i_row, int stage) {
+    if (i_row < p.rows_per_group) {
+      const int64_t row = row0 + i_row;
+      if (lane == 0) {
+        copy_async8(&stat_ring[stage][warp][0], p.stats + row);
+        if (kPost) copy_async8(&stat_ring[stage][warp][1], p.stats + p.rows + row);
       }
-    }
-    s = sum(s);
-    const float mean_dn = p.rms ? 0.f : s.x * inv_c, mean_dnn = s.y * inv_c;
-    float2 s2 = make_float2(0.f, 0.f);
-    float m[kPost ? NV : 1][V];
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int c = col_of<V>(j, G, w, lane);
-      float g[V], y[V];
-      q.dr[j].get(g);
-      q.y[j].get(y);
-#pragma unroll
-      for (int i = 0; i < V; ++i)
-        g[i] = __fmaf_rn(q.st.y, __fmaf_rn(-n[j][i], mean_dnn, dn[j][i] - mean_dn), g[i]);
-      if (p.dx && c < C) store_v<T, V>(static_cast<T *>(p.dx) + at + c, g);
-      if (kPost) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float mi = c < C ? (y[i] - q.st_y.x) * q.st_y.y : 0.f;
-          m[kPost ? j : 0][i] = mi;
-          acc[2][j][i] = __fmaf_rn(g[i], mi, acc[2][j][i]);
-          acc[kParts - 1][j][i] += g[i];
-          dn[j][i] = g[i] * sc[j][i] * pw[kPost ? j : 0][i];
-          s2.x += dn[j][i];
-          s2.y = __fmaf_rn(dn[j][i], mi, s2.y);
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          acc[2][j][i] = __fmaf_rn(g[i], y[i], acc[2][j][i]);
-          g[i] *= sc[j][i];
-        }
-        if (p.dy && c < C) store_v<T, V>(static_cast<T *>(p.dy) + at + c, g);
-      }
-    }
-    if (kPost) {
-      s2 = sum(s2);
-      const float mean_dm = p.rms ? 0.f : s2.x * inv_c, mean_dmm = s2.y * inv_c;
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         const int c = col_of<V>(j, G, w, lane);
-        if (c >= C || !p.dy) continue;
+        if (c >= C) continue;
 #pragma unroll
-        for (int i = 0; i < V; ++i)
-          dn[j][i] = q.st_y.y * __fmaf_rn(-m[kPost ? j : 0][i], mean_dmm, dn[j][i] - mean_dm);
-        store_v<T, V>(static_cast<T *>(p.dy) + at + c, dn[j]);
+        for (int a = 0; a < 4; ++a) {
+          if (!array[a]) continue;
+          const T *src = array[a] + row * C + c;
+          uint4 *dst = ring + stage * per_stage + a * per_array + j * (kPieces / NV) * blockDim.x;
+#pragma unroll
+          for (int k = 0; k < kPieces / NV; ++k)
+            copy_async16(dst + k * blockDim.x, src + k * kVec16<T>);
+        }
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  // V elements of an array's chunk j in this stage (or straight from memory)
+  const auto get = [&](int a, int j, int stage, int64_t at, float *v) {
+    if constexpr (kStages > 0) {
+      const uint4 *src = ring + stage * per_stage + a * per_array + j * (kPieces / NV) * blockDim.x;
+#pragma unroll
+      for (int k = 0; k < kPieces / NV; ++k) unpack16<T>(src[k * blockDim.x], v + k * kVec16<T>);
+    } else {
+      const int c = col_of<V>(j, G, w, lane);
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[i] = 0.f;
+      if (c < C && array[a]) load_v<T, V>(array[a] + at + c, v);
+    }
+  };
+  if constexpr (kStages > 0) {
+    // what no copy writes (columns past the row, arrays that are not there) is 0
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int a = 0; a < 4; ++a)
+        if (col_of<V>(j, G, w, lane) >= C || !array[a])
+          for (int s = 0; s < kStages; ++s)
+            for (int k = 0; k < kPieces / NV; ++k)
+              ring[s * per_stage + a * per_array + (j * (kPieces / NV) + k) * blockDim.x] =
+                  make_uint4(0, 0, 0, 0);
+  }
+  int64_t i_row = (blockIdx.x % p.blocks_per_group) * slots + slot;
+#pragma unroll
+  for (int s = 0; s + 1 < kStages; ++s) fetch(i_row + s * stride, s);
+
+  // the parameters of this lane's columns stay the same over the rows: weight
+  // and gamma gate (times post_weight)
+  float wt[kHeld ? NV : 1][V], sc[kHeld ? NV : 1][V];
+  float4 *const held = reinterpret_cast<float4 *>(smem) + kStages * 4 * kPieces * blockDim.x +
+                       w * (E / 4) * 32 + lane;
+  const int plane = G * (E / 4) * 32;
+  if (kHeld || slot == 0) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int c = col_of<V>(j, G, w, lane), k = kHeld ? j : 0;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        wt[k][i] = 0.f;
+        sc[k][i] = kPost ? 0.f : 1.f;
+      }
+      if (c < C) {
+        float f[V];
+        load_v<P, V>(static_cast<const P *>(p.weight) + c, wt[k]);
+        if (kPost) load_v<P, V>(static_cast<const P *>(p.post_weight) + c, sc[k]);
+        if (p.gamma) {
+          load_v<P, V>(static_cast<const P *>(p.gamma) + c, f);
+#pragma unroll
+          for (int i = 0; i < V; ++i) sc[k][i] *= f[i];
+        }
+        if (p.gate) {
+          load_v<P, V>(static_cast<const P *>(p.gate) + group * C + c, f);
+#pragma unroll
+          for (int i = 0; i < V; ++i) sc[k][i] *= f[i];
+        }
+      }
+      if constexpr (!kHeld) {
+#pragma unroll
+        for (int i = 0; i < V; i += 4) {
+          float4 *const to = held + (j * V + i) / 4 * 32;
+          to[0] = make_float4(wt[0][i], wt[0][i + 1], wt[0][i + 2], wt[0][i + 3]);
+          to[plane] = make_float4(sc[0][i], sc[0][i + 1], sc[0][i + 2], sc[0][i + 3]);
+        }
       }
     }
   }
+  if (!kHeld) __syncthreads();
+  const auto param = [&](int which, int j, float *v) {
+    if constexpr (kHeld) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[i] = which ? sc[j][i] : wt[j][i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; i += 4) {
+        const float4 f = held[which * plane + (j * V + i) / 4 * 32];
+        v[i] = f.x;
+        v[i + 1] = f.y;
+        v[i + 2] = f.z;
+        v[i + 3] = f.w;
+      }
+    }
+  };
+  Values<E> acc[kParts];
+#pragma unroll
+  for (int k = 0; k < kParts; ++k)
+#pragma unroll
+    for (int i = 0; i < E / 2; ++i) acc[k].p[i] = make_float2(0.f, 0.f);
+
+  int stage = 0;
+  for (; i_row < p.rows_per_group; i_row += stride) {
+    const int64_t row = row0 + i_row, at = row * C;
+    float2 st, st_y = make_float2(0.f, 0.f);
+    if constexpr (kStages > 0) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(kStages > 1 ? kStages - 2 : 0) : "memory");
+      __syncwarp();  // lane 0 fetched the statistics
+      st = stat_ring[stage][warp][0];
+      if (kPost) st_y = stat_ring[stage][warp][1];
+      __syncwarp();
+      // into the stage that the row before this one was read from
+      fetch(i_row + (kStages - 1) * stride, stage == 0 ? kStages - 1 : stage - 1);
+    } else {
+      st = p.stats[row];
+      if (kPost) st_y = p.stats[p.rows + row];
+    }
+    const auto in = [&](int j) { return col_of<V>(j, G, w, lane) < C; };
+    Values<E> n, dn, f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      get(0, j, stage, at, n.at(j * V));
+      get(1, j, stage, at, dn.at(j * V));
+      param(0, j, f.at(j * V));
+    }
+    float2 s = make_float2(0.f, 0.f), t = s;  // pairs of sums of dn and of dn n
+#pragma unroll
+    for (int i = 0; i < E / 2; ++i) {
+      const float2 mean = make_float2(in(2 * i / V) ? -st.x : 0.f, in((2 * i + 1) / V) ? -st.x : 0.f);
+      n.p[i] = mul2(add2(n.p[i], mean), both(st.y));
+      acc[0].p[i] = fma2(dn.p[i], n.p[i], acc[0].p[i]);
+      acc[1].p[i] = add2(acc[1].p[i], dn.p[i]);
+      dn.p[i] = mul2(dn.p[i], f.p[i]);
+      s = add2(s, dn.p[i]);
+      t = fma2(dn.p[i], n.p[i], t);
+    }
+    s = sum(make_float2(s.x + s.y, t.x + t.y));
+    const float2 mean_dn = both(p.rms ? 0.f : -s.x * inv_c), mean_dnn = both(-s.y * inv_c);
+    Values<E> g, y;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      get(2, j, stage, at, g.at(j * V));
+      get(3, j, stage, at, y.at(j * V));
+      param(1, j, f.at(j * V));
+    }
+#pragma unroll
+    for (int i = 0; i < E / 2; ++i)
+      g.p[i] = fma2(both(st.y), fma2(n.p[i], mean_dnn, add2(dn.p[i], mean_dn)), g.p[i]);
+    const auto store = [&](void *to, Values<E> &v) {
+      if (!to) return;
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+        if (in(j)) store_v<T, V>(static_cast<T *>(to) + at + col_of<V>(j, G, w, lane), v.at(j * V));
+    };
+    store(p.dx, g);
+    if (kPost) {
+      s = t = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < E / 2; ++i) {
+        const float2 mean =
+            make_float2(in(2 * i / V) ? -st_y.x : 0.f, in((2 * i + 1) / V) ? -st_y.x : 0.f);
+        y.p[i] = mul2(add2(y.p[i], mean), both(st_y.y));
+        acc[2].p[i] = fma2(g.p[i], y.p[i], acc[2].p[i]);
+        acc[kParts - 1].p[i] = add2(acc[kParts - 1].p[i], g.p[i]);
+        g.p[i] = mul2(g.p[i], f.p[i]);
+        s = add2(s, g.p[i]);
+        t = fma2(g.p[i], y.p[i], t);
+      }
+      s = sum(make_float2(s.x + s.y, t.x + t.y));
+      const float2 mean_dm = both(p.rms ? 0.f : -s.x * inv_c), mean_dmm = both(-s.y * inv_c);
+#pragma unroll
+      for (int i = 0; i < E / 2; ++i)
+        g.p[i] = mul2(both(st_y.y), fma2(y.p[i], mean_dmm, add2(g.p[i], mean_dm)));
+    } else {
+#pragma unroll
+      for (int i = 0; i < E / 2; ++i) {
+        acc[2].p[i] = fma2(g.p[i], y.p[i], acc[2].p[i]);
+        g.p[i] = mul2(g.p[i], f.p[i]);
+      }
+    }
+    store(p.dy, g);
+    if (kStages > 0) stage = stage + 1 == kStages ? 0 : stage + 1;
+  }
+  if (kStages > 0) asm volatile("cp.async.wait_all;" ::: "memory");
   if (!p.part) return;
+  if (kStages > 0) __syncthreads();  // the ring's place is taken by the sums
   float *out = p.part + (int64_t)blockIdx.x * 4 * C;
 #pragma unroll
   for (int k = 0; k < kParts; ++k) {
@@ -455,7 +640,7 @@ __global__ void __launch_bounds__(kThreads, E == 8 ? 2 : 1)
           if (c >= C) continue;
 #pragma unroll
           for (int i = 0; i < V; ++i) {
-            float v = acc[k][j][i];
+            float v = acc[k].at(j * V)[i];
             if (q < slots - 1) v += part_smem[c + i];
             part_smem[c + i] = v;
           }
@@ -470,7 +655,7 @@ __global__ void __launch_bounds__(kThreads, E == 8 ? 2 : 1)
         if (c >= C) continue;
 #pragma unroll
         for (int i = 0; i < V; ++i)
-          out[(int64_t)k * C + c + i] = acc[k][j][i] + (slots > 1 ? part_smem[c + i] : 0.f);
+          out[(int64_t)k * C + c + i] = acc[k].at(j * V)[i] + (slots > 1 ? part_smem[c + i] : 0.f);
       }
     }
   }
@@ -582,6 +767,7 @@ template <typename T, typename P, int V, int E>
 cudaError_t forward_e(NormParams p, cudaStream_t s) {
   const int G = (p.C + 32 * E - 1) / (32 * E), slots = 8 / G, threads = 32 * G * slots;
   p.warps_per_row = G;
+  p.per_gate = FastDiv((uint32_t)p.rows_per_gate);
   p.row_end = p.mx_data ? (p.rows + 127) / 128 * 128 : p.rows;
   const int64_t blocks = (p.row_end + slots - 1) / slots;
   // walking slots: the blocks that 148 SMs hold at once
@@ -600,16 +786,27 @@ cudaError_t forward(const NormParams &p, bool vec, cudaStream_t s) {
   return p.C <= 4096 ? forward_e<T, P, V, 16>(p, s) : forward_e<T, P, V, 32>(p, s);
 }
 
+template <typename T, typename P, int V, int E, int kThreads, bool kPost>
+cudaError_t backward_post(const NormBwdParams &p, const NormBwdPlan &plan, cudaStream_t s) {
+  using Cfg = BwdCfg<T, V, E, kThreads>;
+  auto kern = residual_norm_bwd_kernel<T, P, V, E, kPost, kThreads>;
+  const int threads = 32 * plan.warps_per_row * plan.slots;
+  size_t smem = (size_t)Cfg::kStages * Cfg::kStageBytes * threads;
+  if (kPost && E == 8) smem += (size_t)plan.warps_per_row * 32 * E * 2 * sizeof(float);
+  const size_t sums = plan.slots > 1 ? (size_t)p.C * sizeof(float) : 0;
+  if (smem < sums) smem = sums;
+  if (smem > 48 * 1024) {
+    const cudaError_t e =
+        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return e;
+  }
+  kern<<<(unsigned)(p.groups * p.blocks_per_group), threads, smem, s>>>(p);
+  return cudaGetLastError();
+}
 template <typename T, typename P, int V, int E, int kThreads>
 cudaError_t backward_e(const NormBwdParams &p, const NormBwdPlan &plan, cudaStream_t s) {
-  const size_t smem = plan.slots > 1 ? (size_t)p.C * sizeof(float) : 0;
-  const unsigned blocks = (unsigned)(p.groups * p.blocks_per_group);
-  const int threads = 32 * plan.warps_per_row * plan.slots;
-  if (p.post_weight)
-    residual_norm_bwd_kernel<T, P, V, E, true, kThreads><<<blocks, threads, smem, s>>>(p);
-  else
-    residual_norm_bwd_kernel<T, P, V, E, false, kThreads><<<blocks, threads, smem, s>>>(p);
-  return cudaGetLastError();
+  return p.post_weight ? backward_post<T, P, V, E, kThreads, true>(p, plan, s)
+                       : backward_post<T, P, V, E, kThreads, false>(p, plan, s);
 }
 
 template <typename T, typename P>

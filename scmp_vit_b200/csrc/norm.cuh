@@ -5,6 +5,7 @@
 #include <stdint.h>
 
 #include "../../include/scmp_b200.h"
+#include "mx_common.cuh"
 
 namespace scmp {
 
@@ -23,6 +24,7 @@ struct NormParams {
   bool rms, h_f32;
   int fmt;
   int warps_per_row;  // set by the launcher
+  FastDiv per_gate{1};  // rows_per_gate
   int64_t row_end;    // rows that have output: all, or whole atoms of 4-bit scales
 };
 
