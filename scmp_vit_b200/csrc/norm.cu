@@ -213,13 +213,17 @@ __device__ __forceinline__ void store_mx(const NormParams &p, const float *v, in
 
 // E elements per lane, by the shape (rows x columns, bf16 unless fp32, us):
 //   E = 8   one row per slot, up to 2048 columns: a short chain per row and 48
-//           warps an SM.  Few rows (257 x 1024: 3.3, E = 16 3.5), fp32 (16448 x
-//           1024: 49.7 = a copy's rate, E = 16 57.9), short rows (16448 x 200:
-//           9.1, E = 16 10.7)
+//           warps an SM.  Few rows (257 x 1024: 3.2, E = 16 3.5), fp32 rows that
+//           fill blocks of eight warps (16448 x 1024: 49.6 = a copy's rate, E = 16
+//           57.9; 8200 x 2048: 50.3, 54.2), rows of one warp (16448 x 200: 9.4,
+//           E = 16 10.7)
 //   E = 16  slots walk rows, and once a row's x and y are used the next one is on
-//           its way into their registers.  Many rows (16448 x 1024: 30.6, E = 8
-//           42.1)
+//           its way into their registers.  Many rows (16448 x 1024: 27.1, E = 8
+//           42.1; fp32 16400 x 1408: 69.9, E = 8 79.4, with a post norm 85.6, 111)
 //   E = 32  the same for rows of over 4096 columns, or not in 16-byte pieces
+// 16-bit rows are bound by instructions: two fp32 operations per instruction, the
+// gate's row by a multiplication and sums over lanes in half the shuffles took
+// 16400 x 1408 with gates and a post norm from 57 to 46 us.
 template <typename T, typename P, int V, int E>
 __global__ void __launch_bounds__(256, E == 16 ? 3 : 1)
     residual_norm_kernel(const __grid_constant__ NormParams p) {
@@ -379,7 +383,13 @@ __global__ void __launch_bounds__(256, E == 16 ? 3 : 1)
 // E = 8 elements per lane for rows of up to 2048 in 16-byte pieces, else 16.
 //
 // A slot's next rows are on their way into a ring of stages in shared memory,
-// each thread copying what it will read itself.
+// each thread copying what it will read itself (no barrier), which leaves the
+// registers to the sums; with a post norm the parameters stay there too.  bf16
+// 16448 x 1024: 39 us (5.2 TB/s), in registers one row ahead 45; fp32 73 (5.5);
+// 16400 x 1408 with gates and a post norm bf16 80 us, 102 with registers and
+// single operations, instructions (two meetings of a row's warps) its bound; fp32
+// 105 (5.3 TB/s), 201.  Rows not in 16-byte pieces, and fp32 rows of over 4096
+// columns, whose ring would not fit, load as they go.
 template <typename T, int V, int E, int kThreads> struct BwdCfg {
   static constexpr int kPieces = E * (int)sizeof(T) / 16;  // 16-byte pieces per array and lane
   static constexpr int kStages = V == 1 ? 0
@@ -781,7 +791,8 @@ template <typename T, typename P>
 cudaError_t forward(const NormParams &p, bool vec, cudaStream_t s) {
   constexpr int V = kVec16<T>;
   if (!vec) return forward_e<T, P, 1, 32>(p, s);
-  if (p.C <= 256 || (p.C <= 2048 && (sizeof(T) == 4 || p.rows <= 148 * 8)))
+  const int G = (p.C + 255) / 256;  // warps per row at E = 8
+  if (p.C <= 256 || (G <= 8 && ((sizeof(T) == 4 && 8 % G == 0) || p.rows <= 148 * 8)))
     return forward_e<T, P, V, 8>(p, s);
   return p.C <= 4096 ? forward_e<T, P, V, 16>(p, s) : forward_e<T, P, V, 32>(p, s);
 }
