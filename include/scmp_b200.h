@@ -251,8 +251,9 @@ SCMP_API int scmp_mx_matmul(const scmp_mx_matmul_args *args, void *stream);
 /* The same for an A that is not quantised yet: x, M rows of K elements of
  * x_dtype, `ld` elements apart, quantised on the way in (nvfp4: with tensor
  * exponent 0, so scale_exp is B's).  args->a and args->a_scales are buffers for
- * its codes that the call writes; up to SCMP_MX_THIN_ROWS rows of up to
- * SCMP_MX_THIN_K values need none (NULL) and take one launch. */
+ * its codes that the call may write; up to SCMP_MX_THIN_ROWS rows of up to
+ * SCMP_MX_THIN_K values need none (NULL) and then take one launch, which is the
+ * faster way for short weights (with buffers the call chooses). */
 #define SCMP_MX_THIN_ROWS 4
 #define SCMP_MX_THIN_K 6144
 SCMP_API int scmp_mx_linear(const void *x, int x_dtype, int64_t ld,

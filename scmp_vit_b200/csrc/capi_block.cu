@@ -154,7 +154,7 @@ int scmp_mx_matmul(const scmp_mx_matmul_args *args, void *stream) {
   if (rc != SCMP_OK || p.M == 0 || p.N == 0) return rc;
   auto s = static_cast<cudaStream_t>(stream);
   cudaError_t e;
-  if (mx_thin(p.M, p.K)) {
+  if (mx_thin(p.M, p.N, p.K)) {
     e = launch_mx_thin(p, nullptr, 0, 0, s);
   } else {
     unsigned int *err = device_error_word();
@@ -170,7 +170,7 @@ int scmp_mx_linear(const void *x, int x_dtype, int64_t ld, const scmp_mx_matmul_
                    void *stream) {
   set_last_error("");
   if (!args) return fail(SCMP_EINVAL, "args is NULL");
-  const bool thin = mx_thin(args->M, args->K);
+  const bool thin = args->a ? mx_thin(args->M, args->N, args->K) : mx_thin_fits(args->M, args->K);
   MxProduct p{};
   int rc = check_product(args, !thin, p);
   if (rc != SCMP_OK) return rc;

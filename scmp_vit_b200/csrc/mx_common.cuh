@@ -218,8 +218,10 @@ struct MxProduct {
   int out_dtype;
 };
 cudaError_t launch_mx_matmul(const MxProduct &p, unsigned int *error, cudaStream_t s);
-// A few rows (mx_thin): x quantised in the same launch, or NULL with p.a's codes.
-bool mx_thin(int64_t M, int64_t K);
+// A few rows: x quantised in the same launch, or NULL with p.a's codes.  Which
+// products that launch can take, and where it is faster than quantise + tiles.
+bool mx_thin_fits(int64_t M, int64_t K);
+bool mx_thin(int64_t M, int64_t N, int64_t K);
 cudaError_t launch_mx_thin(const MxProduct &p, const void *x, int x_dtype, int64_t ld,
                            cudaStream_t s);
 

@@ -7,8 +7,8 @@
 // codes, i.e. a block of 32 (mxfp4) or two of 16 (nvfp4).  Products of e2m1
 // values are multiples of 1/4 up to 36: eight of them add up exactly in fp16,
 // which the four accumulators per block rely on; block sums and scales are fp32.
-// One row, [4096, 1024]: 3.7 us (quantise + tensor-core tiles 8.0); four rows 6.1
-// (8.0), [4096, 4096] 15.6 (11.8), [1024, 1024] 3.8 (7.2); eight rows are slower.
+// One row, [4096, 1024]: 4.3 us (quantise + tensor-core tiles 6.7); mx_thin has
+// the sizes where it pays.
 #include "mx_common.cuh"
 
 namespace scmp {
@@ -245,7 +245,18 @@ cudaError_t launch_f(const MxProduct &p, const void *x, int x_dtype, int64_t ld,
 
 }  // namespace
 
-bool mx_thin(int64_t M, int64_t K) { return M <= SCMP_MX_THIN_ROWS && K <= SCMP_MX_THIN_K; }
+bool mx_thin_fits(int64_t M, int64_t K) { return M <= SCMP_MX_THIN_ROWS && K <= SCMP_MX_THIN_K; }
+
+// With k = K / 1024 and n = N / 1024 this launch takes about 2 + k n (0.25 +
+// 0.17 M) + 0.25 M k us, quantise + tensor-core tiles 4.6 + 1.25 k.  mxfp4, [N, K]
+// and rows, this / the other (us):
+//   [1024, 1024]  1: 2.6 / 6.0   4: 3.8 / 6.0     [4096, 1024]  1: 4.3 / 6.7   4: 6.9 / 6.7
+//   [1024, 4096]  1: 5.7 / 9.8   4: 9.6 / 9.8     [4096, 4096]  1: 7.5 / 10.0  2: 11.6 / 10.0
+//   [16384, 1024] 1: 9.1 / 7.4                    [6144, 6144]  1: 15.0 / 12.2
+bool mx_thin(int64_t M, int64_t N, int64_t K) {
+  return mx_thin_fits(M, K) &&
+         K / 1024.0 * (N / 1024.0 * (1 + 0.7 * M) + (double)M - 5) < 12;
+}
 
 cudaError_t launch_mx_thin(const MxProduct &p, const void *x, int x_dtype, int64_t ld,
                            cudaStream_t s) {

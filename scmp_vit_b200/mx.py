@@ -162,6 +162,13 @@ def _rows_of(x: torch.Tensor):
     return x2, (x2.stride(0) if x2.shape[0] > 1 else K)
 
 
+def _thin(rows: int, N: int, K: int) -> bool:
+    """Whether a few rows are quantised inside the product's own launch, which
+    needs no buffers (the engine's rule for products of codes)."""
+    return (rows <= _lib.MX_THIN_ROWS and K <= _lib.MX_THIN_K
+            and K / 1024 * (N / 1024 * (1 + 0.7 * rows) + rows - 5) < 12)
+
+
 def _overlap(out: torch.Tensor, t: torch.Tensor) -> bool:
     """Whether contiguous ``out`` and ``t`` (its span, where strided) share bytes."""
     if t.numel() == 0 or out.numel() == 0:
@@ -217,9 +224,7 @@ def mx_matmul(a: Union[torch.Tensor, MXTensor], b: MXTensor, *,
     if plain:
         x_code = _check_input(a, "mx_matmul")
         rows = a.numel() // K
-        # a few rows are quantised inside the product's own launch
-        thin = rows <= _lib.MX_THIN_ROWS and K <= _lib.MX_THIN_K
-        qa = None if thin else mx_empty(a.shape, b.fmt, a.device, a.dtype)
+        qa = None if _thin(rows, N, K) else mx_empty(a.shape, b.fmt, a.device, a.dtype)
     elif a.fmt != b.fmt:
         raise ValueError(f"operands of different formats: {a.fmt} vs {b.fmt}")
     else:

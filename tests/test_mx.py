@@ -360,6 +360,34 @@ def test_matmul_wide_scales(cuda_device, M):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("M,N,K", [(1, 16390, 1024), (2, 4104, 2048), (4, 4096, 1024)])
+def test_few_rows_long_weight(cuda_device, fmt, M, N, K):
+    """Few rows of a long weight go through the tensor-core tiles; without
+    buffers for their codes the one launch takes them all the same."""
+    g = torch.Generator().manual_seed(10)
+    a, w = torch.randn(M, K, generator=g).to(cuda_device), torch.randn(N, K, generator=g)
+    w = w.to(cuda_device)
+    y = check_product(a, w, fmt, torch.float32)
+    q, qa = mx.mx_quantize(w, fmt), mx.mx_quantize(a, fmt)
+    launches = _lib.kernel_launches()
+    mx.mx_matmul(a, q)
+    assert _lib.kernel_launches() - launches == 2
+    out = torch.empty(M, N, device=cuda_device)
+    args = _lib.MxMatmulArgs(_lib.ABI_VERSION, _lib.MX_FORMAT[fmt], None, None, q.data_ptr,
+                             q.scales_ptr, M, N, K, 0, 0, None, out.data_ptr(), 0, 0)
+    launches = _lib.kernel_launches()
+    _lib.check(_lib.load().scmp_mx_linear(
+        a.data_ptr(), 0, K, ctypes.byref(args),
+        ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)))
+    assert _lib.kernel_launches() - launches == 1
+    va, vw = (t.dequantize().double() for t in (qa, q))
+    ref = va @ vw.t()
+    for got in (y, out):
+        assert bool(((got.double() - ref).abs() <= product_bound(va, vw, ref, got.dtype)).all())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("M", [1, 3, 4, 40, 300])
 @pytest.mark.parametrize("big,small", [(2.0 ** 120, 2.0 ** -110), (2.0 ** -110, 2.0 ** 120)])
 def test_matmul_scales_that_meet(cuda_device, M, big, small):
