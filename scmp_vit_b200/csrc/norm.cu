@@ -806,7 +806,7 @@ cudaError_t backward_post(const NormBwdParams &p, const NormBwdPlan &plan, cudaS
   if (kPost && E == 8) smem += (size_t)plan.warps_per_row * 32 * E * 2 * sizeof(float);
   const size_t sums = plan.slots > 1 ? (size_t)p.C * sizeof(float) : 0;
   if (smem < sums) smem = sums;
-  if (smem > 48 * 1024) {
+  if (smem > 44 * 1024) {  // (48 KB without asking, the kernel's own arrays included)
     const cudaError_t e =
         cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;

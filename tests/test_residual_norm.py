@@ -5,6 +5,9 @@ Tolerances carry magnitudes through the formulas: a fp32 sum of C terms is off
 by at most (C + 8) 2^-24 of the sum of their magnitudes, whatever its order,
 and a value rounded to its type by half a step of it."""
 import ctypes
+import pathlib
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -471,6 +474,22 @@ def test_gradient_against_differences(cuda_device):
         A = (cr.abs() * r.detach().double().abs()).sum() + (ch.abs() * (
             h.detach().double().abs() + 3)).sum()
         assert abs(diff - dot) <= A * ((48 + 16) * U / e + 8 * e * e), (k, diff, dot)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("C", [768, 1408])
+def test_backward_first_call_of_a_process(cuda_device, C):
+    """A kernel's first launch asks for the shared memory that it needs, whatever
+    the size of later ones."""
+    code = ("import torch\n"
+            "from scmp_vit_b200.vit import residual_norm\n"
+            f"x = torch.randn(64, {C}, device='cuda').bfloat16().requires_grad_()\n"
+            f"w = torch.ones({C}, device='cuda').bfloat16()\n"
+            "_, h = residual_norm(x, x.detach(), w)\n"
+            "h.sum().backward()\n"
+            "assert bool(x.grad.isfinite().all())\n")
+    root = pathlib.Path(__file__).resolve().parent.parent
+    subprocess.run([sys.executable, "-c", code], check=True, cwd=root, timeout=120)
 
 
 @pytest.mark.gpu
