@@ -214,8 +214,10 @@ cudaError_t launch(const MxProduct &p, const void *x, int64_t ld, const MxLayout
   auto kern = mx_thin_kernel<T, kFmt, kCodes, kM>;
   const size_t smem = (size_t)p.M * l.kp * 2 + (size_t)p.M * (l.kp / l.block) * 4;
   if (smem > 48 * 1024) {
-    const cudaError_t e =
-        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    // (always the most that this kernel uses: calls at the same time agree on it)
+    const cudaError_t e = cudaFuncSetAttribute(
+        kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+        kM * (SCMP_MX_THIN_K * 2 + SCMP_MX_THIN_K / (kFmt == SCMP_MXFP4 ? 32 : 16) * 4));
     if (e != cudaSuccess) return e;
   }
   const bool vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && ld * (int)sizeof(T) % 16 == 0;

@@ -807,8 +807,11 @@ cudaError_t backward_post(const NormBwdParams &p, const NormBwdPlan &plan, cudaS
   const size_t sums = plan.slots > 1 ? (size_t)p.C * sizeof(float) : 0;
   if (smem < sums) smem = sums;
   if (smem > 44 * 1024) {  // (48 KB without asking, the kernel's own arrays included)
+    // (always the most that this kernel uses: calls at the same time agree on it)
+    constexpr size_t kMost = (size_t)Cfg::kStages * Cfg::kStageBytes * kThreads +
+                             (kPost && E == 8 ? kThreads * E * 2 * sizeof(float) : 0);
     const cudaError_t e =
-        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMost);
     if (e != cudaSuccess) return e;
   }
   kern<<<(unsigned)(p.groups * p.blocks_per_group), threads, smem, s>>>(p);

@@ -301,8 +301,9 @@ cudaError_t launch_v(RotaryParams p, cudaStream_t s) {
   auto kern = p.inverse ? rotary_kernel<T, V, kInterleaved, true>
                         : rotary_kernel<T, V, kInterleaved, false>;
   if (smem > 48 * 1024) {
-    const cudaError_t e =
-        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    // (always the most that this kernel uses: calls at the same time agree on it)
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               (kTile + 2) * 256 * (int)sizeof(T));
     if (e != cudaSuccess) return e;
   }
   kern<<<(unsigned)(turn + tiles), kThreads, smem, s>>>(p);

@@ -8,6 +8,7 @@ import ctypes
 import pathlib
 import subprocess
 import sys
+import threading
 
 import pytest
 import torch
@@ -490,6 +491,40 @@ def test_backward_first_call_of_a_process(cuda_device, C):
             "assert bool(x.grad.isfinite().all())\n")
     root = pathlib.Path(__file__).resolve().parent.parent
     subprocess.run([sys.executable, "-c", code], check=True, cwd=root, timeout=120)
+
+
+@pytest.mark.gpu
+def test_calls_at_the_same_time(cuda_device):
+    """Threads with sizes and streams of their own give the bits of one thread."""
+    def step(C):
+        g = torch.Generator().manual_seed(C)
+        t = [torch.randn(300, C, generator=g).bfloat16().to(cuda_device).requires_grad_()
+             for _ in range(2)]
+        w = torch.randn(C, generator=g).bfloat16().to(cuda_device).requires_grad_()
+        r, h = vit.residual_norm(*t, w, post_weight=w)
+        return torch.autograd.grad((r, h), (*t, w), (r.detach(), h.detach()))
+
+    sizes = (768, 1408, 2048, 1024)
+    want = {C: step(C) for C in sizes}
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(C):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(30):
+                    got = step(C)
+                    torch.cuda.current_stream().synchronize()
+                    assert all(torch.equal(x, y) for x, y in zip(got, want[C]))
+        except BaseException as e:  # seen by the test's own thread
+            failed.append((C, e))
+
+    threads = [threading.Thread(target=work, args=(C,)) for C in sizes]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
 
 
 @pytest.mark.gpu
