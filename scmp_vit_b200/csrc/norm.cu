@@ -13,10 +13,13 @@
 namespace scmp {
 namespace {
 
-// A row is dealt to G warps: chunk j (of V consecutive columns per lane) of warp
-// w starts at column ((j G + w) 32 + lane) V.
-template <int V> __device__ __forceinline__ int col_of(int j, int G, int w, int lane) {
-  return ((j * G + w) * 32 + lane) * V;
+// A row is dealt to G warps: chunk j (of NV, each V consecutive columns per lane)
+// of warp w starts at column ((j G + w) 32 + lane) V.  Single elements: at (w NV +
+// j) 32 + lane, so that a lane's columns are a constant distance apart (with the
+// order above, computing their addresses took rows of 1001 elements to 132 us
+// forward and 334 backward, at 16448 rows of bf16).
+template <int V, int NV> __device__ __forceinline__ int col_of(int j, int G, int w, int lane) {
+  return V == 1 ? (w * NV + j) * 32 + lane : ((j * G + w) * 32 + lane) * V;
 }
 
 // V consecutive elements, as loaded: 16-byte pieces, or one element (V = 1).
@@ -56,19 +59,13 @@ template <typename T, int V> __device__ __forceinline__ void store_v(T *p, const
       *reinterpret_cast<uint4 *>(p + i) = pack16<T>(v + i);
   }
 }
-// The same, and v becomes the rounded values.
+// 16-byte pieces stored, and v becomes the rounded values.
 template <typename T, int V> __device__ __forceinline__ void store_rounded(T *p, float *v) {
-  if (V == 1) {
-    const T t = from_f32<T>(v[0]);
-    *p = t;
-    v[0] = to_f32(t);
-  } else {
 #pragma unroll
-    for (int i = 0; i < V; i += kVec16<T>) {
-      const uint4 u = pack16<T>(v + i);
-      *reinterpret_cast<uint4 *>(p + i) = u;
-      unpack16<T>(u, v + i);
-    }
+  for (int i = 0; i < V; i += kVec16<T>) {
+    const uint4 u = pack16<T>(v + i);
+    *reinterpret_cast<uint4 *>(p + i) = u;
+    unpack16<T>(u, v + i);
   }
 }
 
@@ -236,7 +233,7 @@ __global__ void __launch_bounds__(256, E == 16 ? 3 : 1)
   RowSum sum(buf, G, slot, w);
   const int C = p.C;
   const float inv_c = 1.0f / (float)C;
-  const auto in_row = [&](int j) { return col_of<V>(j, G, w, lane) < C; };
+  const auto in_row = [&](int j) { return col_of<V, NV>(j, G, w, lane) < C; };
 
   Pack<T, V> x[NV], y[NV];
   const auto load = [&](int64_t row) {
@@ -247,7 +244,7 @@ __global__ void __launch_bounds__(256, E == 16 ? 3 : 1)
       x[j].zero();
       y[j].zero();
       if (!live || !in_row(j)) continue;
-      const int c = col_of<V>(j, G, w, lane);
+      const int c = col_of<V, NV>(j, G, w, lane);
       x[j].load(static_cast<const T *>(p.x) + at + c);
       if (p.y) y[j].load(static_cast<const T *>(p.y) + at + c);
     }
@@ -271,9 +268,12 @@ __global__ void __launch_bounds__(256, E == 16 ? 3 : 1)
       const int64_t gate_at = p.gate && live ? (int64_t)p.per_gate.quotient((uint32_t)row) * C : 0;
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        const int c = col_of<V>(j, G, w, lane);
+        // (single elements past the row go along, reading its last parameters,
+        // rather than branch)
+        const bool ok = in(j);
+        const int c0 = col_of<V, NV>(j, G, w, lane), c = V > 1 || c0 < C ? c0 : C - 1;
         float *const rj = r.at(j * V);
-        if (!in(j)) {
+        if (V > 1 && !ok) {
 #pragma unroll
           for (int i = 0; i < V; ++i) rj[i] = 0.f;
           continue;
@@ -316,7 +316,13 @@ __global__ void __launch_bounds__(256, E == 16 ? 3 : 1)
         }
         // r is rounded to its type once, and the norm sees the rounded value:
         // the one that the next block and the backward pass read
-        store_rounded<T, V>(static_cast<T *>(p.r) + at + c, rj);
+        if (V == 1) {
+          const T t = from_f32<T>(rj[0]);
+          if (ok) static_cast<T *>(p.r)[at + c] = t;
+          rj[0] = ok ? to_f32(t) : 0.f;
+        } else {
+          store_rounded<T, V>(static_cast<T *>(p.r) + at + c, rj);
+        }
       }
     } else {
 #pragma unroll
@@ -327,9 +333,10 @@ __global__ void __launch_bounds__(256, E == 16 ? 3 : 1)
     if (p.stats && live && w == 0 && lane == 0) p.stats[row] = st;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int c = col_of<V>(j, G, w, lane);
+      const bool ok = in(j);
+      const int c0 = col_of<V, NV>(j, G, w, lane), c = V > 1 || c0 < C ? c0 : C - 1;
       float *const rj = r.at(j * V);
-      if (in(j)) {
+      if (V == 1 || ok) {
         constexpr int N2 = V > 1 ? V / 2 : 1;
         float2 z[N2], f[N2], g[N2];
         const auto load2 = [&](const void *src, float2 *to) {
@@ -353,7 +360,7 @@ __global__ void __launch_bounds__(256, E == 16 ? 3 : 1)
           rj[2 * i] = z[i].x;
           if (V > 1) rj[2 * i + (V > 1)] = z[i].y;
         }
-        if (p.h) {
+        if (p.h && ok) {
           if (p.h_f32)
             store_v<float, V>(static_cast<float *>(p.h) + at + c, rj);
           else
@@ -418,7 +425,7 @@ __global__ void __launch_bounds__(kThreads, E == 8 ? 2 : 1)
   constexpr int NV = E / V;
   constexpr int kParts = kPost ? 4 : 3;
   constexpr int kStages = Cfg::kStages, kPieces = Cfg::kPieces;
-  constexpr bool kHeld = !(kPost && E == 8);  // parameters in registers, else in shared memory
+  constexpr bool kHeld = !(kPost && E == 8 && V > 1);  // parameters in registers, else in shared memory
   __shared__ __align__(16) float2 buf[2 * kMaxWarps];
   __shared__ float2 stat_ring[kStages > 0 ? kStages : 1][kMaxWarps][2];
   extern __shared__ __align__(16) unsigned char smem[];
@@ -447,7 +454,7 @@ __global__ void __launch_bounds__(kThreads, E == 8 ? 2 : 1)
       }
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        const int c = col_of<V>(j, G, w, lane);
+        const int c = col_of<V, NV>(j, G, w, lane);
         if (c >= C) continue;
 #pragma unroll
         for (int a = 0; a < 4; ++a) {
@@ -469,10 +476,12 @@ __global__ void __launch_bounds__(kThreads, E == 8 ? 2 : 1)
 #pragma unroll
       for (int k = 0; k < kPieces / NV; ++k) unpack16<T>(src[k * blockDim.x], v + k * kVec16<T>);
     } else {
-      const int c = col_of<V>(j, G, w, lane);
-#pragma unroll
-      for (int i = 0; i < V; ++i) v[i] = 0.f;
-      if (c < C && array[a]) load_v<T, V>(array[a] + at + c, v);
+      // (the raw element is what the predicate guards: no branch per element)
+      const int c = col_of<V, NV>(j, G, w, lane);
+      Pack<T, V> q;
+      q.zero();
+      if (c < C && array[a]) q.load(array[a] + at + c);
+      q.get(v);
     }
   };
   if constexpr (kStages > 0) {
@@ -481,7 +490,7 @@ __global__ void __launch_bounds__(kThreads, E == 8 ? 2 : 1)
     for (int j = 0; j < NV; ++j)
 #pragma unroll
       for (int a = 0; a < 4; ++a)
-        if (col_of<V>(j, G, w, lane) >= C || !array[a])
+        if (col_of<V, NV>(j, G, w, lane) >= C || !array[a])
           for (int s = 0; s < kStages; ++s)
             for (int k = 0; k < kPieces / NV; ++k)
               ring[s * per_stage + a * per_array + (j * (kPieces / NV) + k) * blockDim.x] =
@@ -500,7 +509,7 @@ __global__ void __launch_bounds__(kThreads, E == 8 ? 2 : 1)
   if (kHeld || slot == 0) {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int c = col_of<V>(j, G, w, lane), k = kHeld ? j : 0;
+      const int c = col_of<V, NV>(j, G, w, lane), k = kHeld ? j : 0;
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         wt[k][i] = 0.f;
@@ -569,7 +578,7 @@ __global__ void __launch_bounds__(kThreads, E == 8 ? 2 : 1)
       st = p.stats[row];
       if (kPost) st_y = p.stats[p.rows + row];
     }
-    const auto in = [&](int j) { return col_of<V>(j, G, w, lane) < C; };
+    const auto in = [&](int j) { return col_of<V, NV>(j, G, w, lane) < C; };
     Values<E> n, dn, f;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
@@ -604,7 +613,7 @@ __global__ void __launch_bounds__(kThreads, E == 8 ? 2 : 1)
       if (!to) return;
 #pragma unroll
       for (int j = 0; j < NV; ++j)
-        if (in(j)) store_v<T, V>(static_cast<T *>(to) + at + col_of<V>(j, G, w, lane), v.at(j * V));
+        if (in(j)) store_v<T, V>(static_cast<T *>(to) + at + col_of<V, NV>(j, G, w, lane), v.at(j * V));
     };
     store(p.dx, g);
     if (kPost) {
@@ -646,7 +655,7 @@ __global__ void __launch_bounds__(kThreads, E == 8 ? 2 : 1)
       if (slot == q) {
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-          const int c = col_of<V>(j, G, w, lane);
+          const int c = col_of<V, NV>(j, G, w, lane);
           if (c >= C) continue;
 #pragma unroll
           for (int i = 0; i < V; ++i) {
@@ -661,7 +670,7 @@ __global__ void __launch_bounds__(kThreads, E == 8 ? 2 : 1)
     if (slot == 0) {
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        const int c = col_of<V>(j, G, w, lane);
+        const int c = col_of<V, NV>(j, G, w, lane);
         if (c >= C) continue;
 #pragma unroll
         for (int i = 0; i < V; ++i)
@@ -770,8 +779,8 @@ __global__ void __launch_bounds__(1024) norm_bwd_groups_kernel(
 
 // --------------------------------------------------------------- dispatch
 
-// Backward: elements per lane, 8 for rows of up to 2048 in 16-byte pieces.
-bool short_rows(int64_t C, bool vec) { return vec && C <= 2048; }
+// Backward: 8 elements per lane for rows of up to 2048.
+bool short_rows(int64_t C) { return C <= 2048; }
 
 template <typename T, typename P, int V, int E>
 cudaError_t forward_e(NormParams p, cudaStream_t s) {
@@ -790,7 +799,10 @@ cudaError_t forward_e(NormParams p, cudaStream_t s) {
 template <typename T, typename P>
 cudaError_t forward(const NormParams &p, bool vec, cudaStream_t s) {
   constexpr int V = kVec16<T>;
-  if (!vec) return forward_e<T, P, 1, 32>(p, s);
+  if (!vec)
+    return p.C <= 2048   ? forward_e<T, P, 1, 8>(p, s)
+           : p.C <= 4096 ? forward_e<T, P, 1, 16>(p, s)
+                         : forward_e<T, P, 1, 32>(p, s);
   const int G = (p.C + 255) / 256;  // warps per row at E = 8
   if (p.C <= 256 || (G <= 8 && ((sizeof(T) == 4 && 8 % G == 0) || p.rows <= 148 * 8)))
     return forward_e<T, P, V, 8>(p, s);
@@ -803,13 +815,13 @@ cudaError_t backward_post(const NormBwdParams &p, const NormBwdPlan &plan, cudaS
   auto kern = residual_norm_bwd_kernel<T, P, V, E, kPost, kThreads>;
   const int threads = 32 * plan.warps_per_row * plan.slots;
   size_t smem = (size_t)Cfg::kStages * Cfg::kStageBytes * threads;
-  if (kPost && E == 8) smem += (size_t)plan.warps_per_row * 32 * E * 2 * sizeof(float);
+  if (kPost && E == 8 && V > 1) smem += (size_t)plan.warps_per_row * 32 * E * 2 * sizeof(float);
   const size_t sums = plan.slots > 1 ? (size_t)p.C * sizeof(float) : 0;
   if (smem < sums) smem = sums;
   if (smem > 44 * 1024) {  // (48 KB without asking, the kernel's own arrays included)
     // (always the most that this kernel uses: calls at the same time agree on it)
     constexpr size_t kMost = (size_t)Cfg::kStages * Cfg::kStageBytes * kThreads +
-                             (kPost && E == 8 ? kThreads * E * 2 * sizeof(float) : 0);
+                             (kPost && E == 8 && V > 1 ? kThreads * E * 2 * sizeof(float) : 0);
     const cudaError_t e =
         cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMost);
     if (e != cudaSuccess) return e;
@@ -833,10 +845,15 @@ cudaError_t backward(NormBwdParams p, bool vec, cudaStream_t s, int *launches) {
   // (blocks of 512 threads leave 128 registers a thread, too few for 16
   // elements: they serve the rows that need them)
   constexpr int V = kVec16<T>;
-  cudaError_t e = short_rows(p.C, vec)    ? backward_e<T, P, V, 8, 256>(p, plan, s)
-                  : vec && p.C <= 8 * 512 ? backward_e<T, P, V, 16, 256>(p, plan, s)
-                  : vec                   ? backward_e<T, P, V, 16, 512>(p, plan, s)
-                                          : backward_e<T, P, 1, 16, 512>(p, plan, s);
+  cudaError_t e;
+  if (vec)
+    e = short_rows(p.C)    ? backward_e<T, P, V, 8, 256>(p, plan, s)
+        : p.C <= 8 * 512 ? backward_e<T, P, V, 16, 256>(p, plan, s)
+                         : backward_e<T, P, V, 16, 512>(p, plan, s);
+  else
+    e = short_rows(p.C)    ? backward_e<T, P, 1, 8, 256>(p, plan, s)
+        : p.C <= 8 * 512 ? backward_e<T, P, 1, 16, 256>(p, plan, s)
+                         : backward_e<T, P, 1, 16, 512>(p, plan, s);
   *launches = 1;
   if (e != cudaSuccess || !p.part) return e;
   if (p.groups > 1 && p.blocks_per_group == 1) {
@@ -862,7 +879,7 @@ cudaError_t backward(NormBwdParams p, bool vec, cudaStream_t s, int *launches) {
 // 103).  At least one block per gate group.
 NormBwdPlan norm_bwd_plan(int64_t rows, int64_t groups, int64_t C, bool vec) {
   NormBwdPlan plan;
-  const bool small = short_rows(C, vec);
+  const bool small = short_rows(C);
   plan.warps_per_row = (int)(small ? (C + 255) / 256 : (C + 511) / 512);
   plan.slots = plan.warps_per_row >= 8 ? 1 : 8 / plan.warps_per_row;
   const int64_t resident = 148 * (small ? 512 / (32 * plan.warps_per_row * plan.slots) : 1);
