@@ -217,12 +217,15 @@ __device__ __forceinline__ void store_mx(const NormParams &p, const float *v, in
 //   E = 16  slots walk rows, and once a row's x and y are used the next one is on
 //           its way into their registers.  Many rows (16448 x 1024: 27.1, E = 8
 //           42.1; fp32 16400 x 1408: 69.9, E = 8 79.4, with a post norm 85.6, 111)
-//   E = 32  the same for rows of over 4096 columns, or not in 16-byte pieces
+//   E = 32  the same for rows of over 4096 columns
+// Rows not in 16-byte pieces go one element at a time: E = 8 up to 2048 columns
+// (16448 x 1001: 67 us, E = 16 71; fp32 69, 99), E = 16 up to 4096, two blocks an
+// SM rather than three, which spill (6400 x 2501: 73, 82).
 // 16-bit rows are bound by instructions: two fp32 operations per instruction, the
 // gate's row by a multiplication and sums over lanes in half the shuffles took
 // 16400 x 1408 with gates and a post norm from 57 to 46 us.
 template <typename T, typename P, int V, int E>
-__global__ void __launch_bounds__(256, E == 16 ? 3 : 1)
+__global__ void __launch_bounds__(256, E == 16 ? (V == 1 ? 2 : 3) : 1)
     residual_norm_kernel(const __grid_constant__ NormParams p) {
   constexpr bool kWalk = E > 8;
   constexpr int NV = E / V;
@@ -790,7 +793,7 @@ cudaError_t forward_e(NormParams p, cudaStream_t s) {
   p.row_end = p.mx_data ? (p.rows + 127) / 128 * 128 : p.rows;
   const int64_t blocks = (p.row_end + slots - 1) / slots;
   // walking slots: the blocks that 148 SMs hold at once
-  const int64_t most = E == 8 ? blocks : 148 * ((E == 16 ? 768 : 512) / threads);
+  const int64_t most = E == 8 ? blocks : 148 * ((E == 16 && V > 1 ? 768 : 512) / threads);
   residual_norm_kernel<T, P, V, E>
       <<<(unsigned)(blocks < most ? blocks : most), threads, 0, s>>>(p);
   return cudaGetLastError();
