@@ -12,18 +12,32 @@ try:  # the stream's handle without a Stream object around it
 except AttributeError:  # a CPU build of torch
     def _raw_stream(index: int) -> int:
         return torch.cuda.current_stream(index).cuda_stream
+try:  # (the tensors of a call exist, so the device is initialised)
+    _current_device = torch._C._cuda_getDevice
+except AttributeError:
+    _current_device = torch.cuda.current_device
 
 
 def call(fn, index: int, *args) -> None:
     """``fn(*args, stream)`` on CUDA device ``index`` and its current stream;
     raises on a non-zero status."""
-    if torch.cuda.current_device() == index:
+    if _current_device() == index:
         status = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
             status = fn(*args, _raw_stream(index))
     if status:
         _lib.check(status)
+
+
+def once_differentiable(backward):
+    """``torch.autograd.function.once_differentiable``, entered only where a
+    gradient of the gradient is being recorded."""
+    recorded = torch.autograd.function.once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return (recorded if torch.is_grad_enabled() else backward)(ctx, *grads)
+    return run
 
 
 def dtype_code(dtype: torch.dtype, what: str) -> int:

@@ -6,6 +6,7 @@ no fallback: if it is missing or fails to load, every SC call raises.
 from __future__ import annotations
 
 import ctypes
+import struct
 import threading
 from pathlib import Path
 
@@ -143,6 +144,14 @@ class RotaryArgs(ctypes.Structure):
         ("reserved", ctypes.c_int32 * 3)]
 
 
+# The same layouts as packers: a call's arguments as bytes cost a quarter of a
+# Structure's (None is 0 there, so pointers come as integers).
+PACK_MX_MATMUL = struct.Struct("2i4P3q2i2P2i")
+PACK_NORM = struct.Struct("4i13P3qf3i")
+PACK_NORM_BWD = struct.Struct("4i19PN3q")
+PACK_ROTARY = struct.Struct("2i6P5q16i")
+
+
 class EngineError(RuntimeError):
     """A non-zero status returned by the engine."""
 
@@ -217,12 +226,12 @@ def load() -> ctypes.CDLL:
         lib.scmp_mx_quantize.restype = ctypes.c_int
         lib.scmp_mx_dequantize.argtypes = [ptr, ptr, i64, i64, i32, i32, ptr, i32, ptr]
         lib.scmp_mx_dequantize.restype = ctypes.c_int
-        lib.scmp_mx_linear.argtypes = [ptr, i32, i64, ctypes.POINTER(MxMatmulArgs), ptr]
+        # (their argument structs: byref of a Structure, or packed bytes)
+        lib.scmp_mx_linear.argtypes = [ptr, i32, i64, ptr, ptr]
         lib.scmp_mx_linear.restype = ctypes.c_int
-        for name, args in (("scmp_mx_matmul", MxMatmulArgs), ("scmp_residual_norm", NormArgs),
-                           ("scmp_residual_norm_bwd", NormBwdArgs),
-                           ("scmp_split_qkv_rotary", RotaryArgs)):
-            getattr(lib, name).argtypes = [ctypes.POINTER(args), ptr]
+        for name in ("scmp_mx_matmul", "scmp_residual_norm", "scmp_residual_norm_bwd",
+                     "scmp_split_qkv_rotary"):
+            getattr(lib, name).argtypes = [ptr, ptr]
             getattr(lib, name).restype = ctypes.c_int
         lib.scmp_residual_norm_bwd_workspace.argtypes = [i64, i64, i64]
         lib.scmp_residual_norm_bwd_workspace.restype = ctypes.c_size_t

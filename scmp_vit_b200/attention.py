@@ -21,7 +21,7 @@ import torch
 import torch.nn as nn
 
 from . import sc_linear as _scl
-from ._call import DTYPE, call
+from ._call import DTYPE, call, once_differentiable
 from .mp import (
     AdaptiveMPConfig,
     AutoMPBudgetLogger,
@@ -418,10 +418,11 @@ def _rotary_launch(qkv, q, k, v, axes: RotaryAxes, table, pos, v_transposed: boo
     """One ``scmp_split_qkv_rotary`` call on contiguous storages."""
     from . import _lib
     B, H, N, D = q.shape
-    args = _lib.RotaryArgs(
+    args = _lib.PACK_ROTARY.pack(
         _lib.ABI_VERSION, DTYPE[qkv.dtype], qkv.data_ptr(), q.data_ptr(), k.data_ptr(),
         v.data_ptr(), table.data_ptr(), pos.data_ptr(), B, N, H, k.shape[1], D, len(axes.dims),
-        axes.c_dims, axes.c_sizes, pos.dim() == 3, axes.interleaved, v_transposed, inverse)
+        *axes.c_dims, *axes.c_sizes, pos.dim() == 3, axes.interleaved, v_transposed, inverse,
+        0, 0, 0)
     call(_lib.load().scmp_split_qkv_rotary, qkv.get_device(), args)
 
 
@@ -445,7 +446,7 @@ class _SplitQkvRotary(torch.autograd.Function):
         return _split_rotary(qkv.contiguous(), pos, table, axes, H, Hk, transpose_v)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @once_differentiable
     def backward(ctx, dq, dk, dv):
         pos, table = ctx.saved_tensors
         # v's gradient in whichever of its two layouts it comes

@@ -38,6 +38,13 @@ def _check_fmt(fmt: str) -> str:
     return fmt
 
 
+def _check_exp(scale_exp: int) -> int:
+    exp = int(scale_exp)
+    if not -1024 <= exp <= 1024:  # (the engine has the formats' own limits)
+        raise ValueError(f"scale_exp {scale_exp} is out of range")
+    return exp
+
+
 def _no_grad_wanted(name: str, *tensors) -> None:
     if torch.is_grad_enabled():
         for t in tensors:
@@ -75,12 +82,12 @@ class MXTensor:
         if data.data_ptr() % 16 or scales.data_ptr() % 16:
             raise ValueError("data and scales must be 16-byte aligned")
         self._set(data, scales, None, data.data_ptr(), scales.data_ptr(), data.get_device(), shape,
-                  fmt, scale_exp, dtype)
+                  fmt, _check_exp(scale_exp), dtype)
 
     def _set(self, data, scales, buf, data_ptr, scales_ptr, index, shape, fmt, scale_exp, dtype):
         self._data, self._scales, self._buf = data, scales, buf
         self.data_ptr, self.scales_ptr, self.index = data_ptr, scales_ptr, index
-        self.shape, self.fmt, self.scale_exp, self.dtype = shape, fmt, int(scale_exp), dtype
+        self.shape, self.fmt, self.scale_exp, self.dtype = shape, fmt, scale_exp, dtype
         self.rows = math.prod(shape[:-1])
         return self
 
@@ -195,7 +202,7 @@ def mx_quantize(x: torch.Tensor, fmt: str = "mxfp4", *, scale_exp: int = 0) -> M
     activations)."""
     _check_fmt(fmt)
     code = _check_input(x, "mx_quantize")
-    out = mx_empty(x.shape, fmt, x.device, x.dtype, scale_exp)
+    out = mx_empty(x.shape, fmt, x.device, x.dtype, _check_exp(scale_exp))
     x, ld = _rows_of(x)
     call(_lib.load().scmp_mx_quantize, out.index, x.data_ptr(), code, out.rows, out.shape[-1], ld,
          _lib.MX_FORMAT[fmt], out.scale_exp, out.data_ptr, out.scales_ptr)
@@ -244,7 +251,7 @@ def mx_matmul(a: Union[torch.Tensor, MXTensor], b: MXTensor, *,
         for t in (a if plain else None, bias):
             if t is not None and _overlap(out, t):
                 raise ValueError("out shares memory with an input")
-    bias_code, bias_ptr = 0, None
+    bias_code, bias_ptr = 0, 0
     if bias is not None:
         if bias.shape != (N,) or bias.get_device() != index:
             raise ValueError(f"bias must be [{N}] on {b.device}, got {tuple(bias.shape)} on "
@@ -253,9 +260,9 @@ def mx_matmul(a: Union[torch.Tensor, MXTensor], b: MXTensor, *,
         _no_grad_wanted("mx_matmul", bias)
         bias = bias if bias.is_contiguous() else bias.detach().contiguous()
         bias_ptr = bias.data_ptr()
-    args = _lib.MxMatmulArgs(
-        _lib.ABI_VERSION, _lib.MX_FORMAT[b.fmt], None if qa is None else qa.data_ptr,
-        None if qa is None else qa.scales_ptr, b.data_ptr, b.scales_ptr, rows, N, K,
+    args = _lib.PACK_MX_MATMUL.pack(
+        _lib.ABI_VERSION, _lib.MX_FORMAT[b.fmt], 0 if qa is None else qa.data_ptr,
+        0 if qa is None else qa.scales_ptr, b.data_ptr, b.scales_ptr, rows, N, K,
         b.scale_exp if plain else a.scale_exp + b.scale_exp, bias_code, bias_ptr, out.data_ptr(),
         out_code, 0)
     if plain:

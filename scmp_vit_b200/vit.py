@@ -22,13 +22,14 @@ LFSR-16 pool seeded per block) and optional head-aligned compensation
 """
 from __future__ import annotations
 
+import functools
 from typing import Callable, Dict, Iterable, Optional
 
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from ._call import DTYPE, call
+from ._call import DTYPE, call, once_differentiable
 from .attention import GridRotary, make_sc_attention_forward
 from .head_aligned_comp import HeadAlignedSCLinear
 from .mp import SeededRandomMPConfig, quantile_counts, set_current_block_idx
@@ -149,8 +150,8 @@ def _check_norm(x, y, weight, norm_bias, kind, eps, gamma, gate, post_weight, po
                          f"got {tuple(gate.shape)} {gate.dtype} {gate.device}")
 
 
-def _ptr(t: Optional[torch.Tensor]):
-    return None if t is None else t.data_ptr()
+def _ptr(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
 def _dense(t: Optional[torch.Tensor]):
@@ -164,16 +165,23 @@ def _norm_launch(x, y, weight, norm_bias, gamma, gate, post_weight, post_bias, k
     r = None if y is None else torch.empty_like(x)
     C = x.shape[-1]
     rows = x.numel() // C
-    args = _lib.NormArgs(
+    args = _lib.PACK_NORM.pack(
         _lib.ABI_VERSION, DTYPE[x.dtype], DTYPE[weight.dtype], kind == "rms", x.data_ptr(),
         _ptr(y), weight.data_ptr(), _ptr(norm_bias), _ptr(gamma), _ptr(gate), _ptr(post_weight),
-        _ptr(post_bias), _ptr(r), _ptr(h), _ptr(stats), None if mx is None else mx.data_ptr,
-        None if mx is None else mx.scales_ptr, rows, C,
+        _ptr(post_bias), _ptr(r), _ptr(h), _ptr(stats), 0 if mx is None else mx.data_ptr,
+        0 if mx is None else mx.scales_ptr, rows, C,
         0 if gate is None else rows // max(1, x.shape[0]), eps,
         h is not None and h.dtype == torch.float32,
         0 if mx is None else _lib.MX_FORMAT[mx.fmt], 0)
     call(_lib.load().scmp_residual_norm, x.get_device(), args)
     return r
+
+
+@functools.lru_cache(maxsize=256)
+def _norm_bwd_workspace(rows: int, C: int, rows_per_gate: int) -> int:
+    """Bytes, a function of the sizes alone."""
+    from . import _lib
+    return _lib.load().scmp_residual_norm_bwd_workspace(rows, C, rows_per_gate)
 
 
 class _ResidualNorm(torch.autograd.Function):
@@ -191,7 +199,7 @@ class _ResidualNorm(torch.autograd.Function):
         return h if r is None else (r, h)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @once_differentiable
     def backward(ctx, *grads):
         from . import _lib
         r, y, stats, weight, norm_bias, gamma, gate, post_weight, post_bias = ctx.saved_tensors
@@ -209,9 +217,9 @@ class _ResidualNorm(torch.autograd.Function):
         lib = _lib.load()
         ws, size = None, 0
         if any(t is not None for t in out[2:]):
-            size = lib.scmp_residual_norm_bwd_workspace(rows, C, per_gate)
+            size = _norm_bwd_workspace(rows, C, per_gate)
             ws = torch.empty(size, dtype=torch.uint8, device=r.device)
-        args = _lib.NormBwdArgs(
+        args = _lib.PACK_NORM_BWD.pack(
             _lib.ABI_VERSION, DTYPE[r.dtype], DTYPE[weight.dtype], ctx.kind == "rms", r.data_ptr(),
             _ptr(y), _ptr(dr), _ptr(dh), weight.data_ptr(), _ptr(gamma), _ptr(gate),
             _ptr(post_weight), _ptr(post_bias), stats.data_ptr(), *[_ptr(t) for t in out], _ptr(ws),

@@ -85,6 +85,23 @@ def test_sizes():
         assert lib.scmp_mx_scale_size(rows, K, code) == 0
 
 
+@pytest.mark.parametrize("pack,cls", [
+    (_lib.PACK_MX_MATMUL, _lib.MxMatmulArgs), (_lib.PACK_NORM, _lib.NormArgs),
+    (_lib.PACK_NORM_BWD, _lib.NormBwdArgs), (_lib.PACK_ROTARY, _lib.RotaryArgs)])
+def test_packed_arguments_are_the_structs(pack, cls):
+    a, values, n = cls(), [], 0
+    for name, kind in cls._fields_:
+        for i in range(getattr(kind, "_length_", 0) or 1):
+            n += 1
+            v = n / 4 if kind is ctypes.c_float else n
+            values.append(v)
+            if hasattr(kind, "_length_"):
+                getattr(a, name)[i] = v
+            else:
+                setattr(a, name, v)
+    assert pack.pack(*values) == bytes(a)
+
+
 def test_struct_layouts_match_the_header():
     assert ctypes.sizeof(_lib.MxMatmulArgs) == 8 + 32 + 24 + 8 + 16 + 8
     assert ctypes.sizeof(_lib.NormArgs) == 16 + 13 * 8 + 24 + 16
@@ -183,6 +200,9 @@ def test_python_refusals_on_cpu():
         mx.mx_quantize(torch.zeros(4, 32))
     with pytest.raises(ValueError, match="format"):
         mx.mx_quantize(torch.zeros(4, 32), "fp4")
+    with pytest.raises(ValueError, match="scale_exp"):
+        mx.MXTensor(torch.zeros(64, dtype=torch.uint8), torch.zeros(512, dtype=torch.uint8),
+                    (4, 32), "nvfp4", 1 << 32)
     with pytest.raises(TypeError, match="float32"):
         mx.mx_quantize(torch.zeros(4, 32, dtype=torch.int32))
     with pytest.raises(TypeError, match="MXTensor"):
