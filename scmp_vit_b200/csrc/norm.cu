@@ -390,7 +390,7 @@ __global__ void __launch_bounds__(256, E == 16 ? (V == 1 ? 2 : 3) : 1)
 // fixed order and written as partials [group][block][part][C]; a second kernel
 // adds those in order, so the result does not depend on timing.
 //   parts: 0 sum dh n   1 sum dh   2 sum g z (no post norm) or sum g m   3 sum g
-// E = 8 elements per lane for rows of up to 2048 in 16-byte pieces, else 16.
+// E = 8 elements per lane for rows of up to 2048, else 16.
 //
 // A slot's next rows are on their way into a ring of stages in shared memory,
 // each thread copying what it will read itself (no barrier), which leaves the
@@ -840,7 +840,7 @@ cudaError_t backward_e(const NormBwdParams &p, const NormBwdPlan &plan, cudaStre
 
 template <typename T, typename P>
 cudaError_t backward(NormBwdParams p, bool vec, cudaStream_t s, int *launches) {
-  const NormBwdPlan plan = norm_bwd_plan(p.rows, p.groups, p.C, vec);
+  const NormBwdPlan plan = norm_bwd_plan(p.rows, p.groups, p.C);
   p.warps_per_row = plan.warps_per_row;
   p.blocks_per_group = plan.blocks_per_group;
   p.rows_per_group = p.rows / p.groups;
@@ -878,9 +878,9 @@ cudaError_t backward(NormBwdParams p, bool vec, cudaStream_t s, int *launches) {
 
 // About 8 warps a block (16 for long rows), and as many blocks as the 148 SMs
 // hold at once: two of 256 threads and 128 registers, or one (a block more would
-// start when the others end: 16400 x 1408 in 16 gate groups 168 us instead of
-// 103).  At least one block per gate group.
-NormBwdPlan norm_bwd_plan(int64_t rows, int64_t groups, int64_t C, bool vec) {
+// start when the others end: at 16400 x 1408 in 16 gate groups that took 1.6 times
+// as long).  At least one block per gate group.
+NormBwdPlan norm_bwd_plan(int64_t rows, int64_t groups, int64_t C) {
   NormBwdPlan plan;
   const bool small = short_rows(C);
   plan.warps_per_row = (int)(small ? (C + 255) / 256 : (C + 511) / 512);
@@ -895,10 +895,8 @@ NormBwdPlan norm_bwd_plan(int64_t rows, int64_t groups, int64_t C, bool vec) {
 }
 
 int64_t norm_bwd_floats(int64_t rows, int64_t groups, int64_t C) {
-  const NormBwdPlan a = norm_bwd_plan(rows, groups, C, true);
-  const NormBwdPlan b = norm_bwd_plan(rows, groups, C, false);
-  return (a.part_floats > b.part_floats ? a.part_floats : b.part_floats) +
-         (a.sum_floats > b.sum_floats ? a.sum_floats : b.sum_floats);
+  const NormBwdPlan plan = norm_bwd_plan(rows, groups, C);
+  return plan.part_floats + plan.sum_floats;
 }
 
 cudaError_t launch_residual_norm(const NormParams &p, int dtype, int param_dtype, bool vec,

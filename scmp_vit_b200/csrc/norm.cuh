@@ -48,8 +48,8 @@ struct NormBwdPlan {
   int64_t blocks_per_group;
   int64_t part_floats, sum_floats;  // workspace
 };
-NormBwdPlan norm_bwd_plan(int64_t rows, int64_t groups, int64_t C, bool vec);
-// Floats of workspace that either alignment can need.
+NormBwdPlan norm_bwd_plan(int64_t rows, int64_t groups, int64_t C);
+// Floats of workspace.
 int64_t norm_bwd_floats(int64_t rows, int64_t groups, int64_t C);
 
 constexpr int64_t kNormMaxC = 8192;  // 16 warps of 16 elements per lane
