@@ -189,7 +189,7 @@ class _ResidualNorm(torch.autograd.Function):
     def forward(ctx, x, y, weight, norm_bias, gamma, gate, post_weight, post_bias, kind, eps):
         t = [_dense(v) for v in (x, y, weight, norm_bias, gamma, gate, post_weight, post_bias)]
         x = t[0]
-        stats = torch.empty(2 if post_weight is not None else 1, x.numel() // x.shape[-1], 2,
+        stats = torch.empty(x.numel() // x.shape[-1] * (2 if post_weight is None else 4),
                             dtype=torch.float32, device=x.device)
         h = torch.empty_like(x)
         r = _norm_launch(*t, kind, eps, stats, h)
