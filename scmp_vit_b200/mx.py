@@ -215,7 +215,8 @@ def mx_matmul(a: Union[torch.Tensor, MXTensor], b: MXTensor, *,
     """``a @ b^T`` (+ ``bias``) for ``a`` ``[..., K]`` and ``b`` ``[N, K]`` ->
     ``[..., N]``: the exact products of the 4-bit values summed in fp32, the
     bias added, rounded once to ``out_dtype`` (default: a's type).  A plain
-    ``a`` is quantised to ``b``'s format first (nvfp4 with tensor scale 1)."""
+    ``a`` is quantised to ``b``'s format first (nvfp4 with tensor scale 1).
+    ``out`` is contiguous and shares no memory with ``a`` or ``bias``."""
     if not isinstance(b, MXTensor) or len(b.shape) != 2:
         raise TypeError("b must be a 2-D MXTensor [N, K]")
     if b.index < 0:
