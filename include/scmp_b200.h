@@ -291,7 +291,7 @@ SCMP_API int scmp_residual_norm(const scmp_norm_args *args, void *stream);
 /* Gradients of the above from dr and dh (each nullable: zero): dx, dy and the
  * parameters' (each nullable: not wanted), with the stats of the forward pass
  * and its r (x where y was NULL).  Deterministic.  The workspace holds partial column
- * sums; scmp_residual_norm_bwd_workspace gives its size.  One to three
+ * sums; scmp_residual_norm_bwd_workspace gives its size.  One or two
  * launches. */
 typedef struct scmp_norm_bwd_args {
   int32_t abi_version;

@@ -396,7 +396,7 @@ __global__ void __launch_bounds__(256, E == 16 ? (V == 1 ? 2 : 3) : 1)
 // each thread copying what it will read itself (no barrier), which leaves the
 // registers to the sums; with a post norm the parameters stay there too.  bf16
 // 16448 x 1024: 39 us (5.2 TB/s), in registers one row ahead 45; fp32 73 (5.5);
-// 16400 x 1408 with gates and a post norm bf16 80 us, 102 with registers and
+// 16400 x 1408 with gates and a post norm bf16 76 us, 102 with registers and
 // single operations, instructions (two meetings of a row's warps) its bound; fp32
 // 105 (5.3 TB/s), 201.  Rows not in 16-byte pieces, and fp32 rows of over 4096
 // columns, whose ring would not fit, load as they go.
@@ -712,26 +712,29 @@ __device__ __forceinline__ void write_totals(const NormBwdParams &p, int c,
     if (out[k]) static_cast<P *>(out[k])[c] = from_f32<P>(total[k]);
 }
 
-// Block (8 columns, gate group): 32 or 128 threads per column share the group's
-// partials.  With one group it finishes; else it leaves the group's sums for the
-// kernel below.
+// The four sums of a group's partials, blocks first, first + step, ... of column c.
+__device__ __forceinline__ void add_partials(const NormBwdParams &p, int64_t group, int first,
+                                             int step, int c, int parts, float (&v)[4]) {
+#pragma unroll 4
+  for (int64_t b = first; b < p.blocks_per_group; b += step) {
+    const float *src = p.part + (group * p.blocks_per_group + b) * 4 * p.C + c;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (k < parts) v[k] += __ldg(src + (int64_t)k * p.C);
+  }
+}
+
+// One gate group: a block takes 8 columns, 32 or 128 threads per column share the
+// partials.
 template <typename P>
 __global__ void __launch_bounds__(1024) norm_bwd_sum_kernel(
     const __grid_constant__ NormBwdParams p) {
   __shared__ float s[4][32][8];
-  const int cols = (p.C + 7) / 8;
   const int ci = threadIdx.x & 7, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int c = (int)(blockIdx.x % cols) * 8 + ci;
-  const int64_t group = blockIdx.x / cols;
-  const int parts = p.post_weight ? 4 : 3;
+  const int c = (int)blockIdx.x * 8 + ci;
   float v[4] = {0.f, 0.f, 0.f, 0.f};
   if (c < p.C)
-    for (int64_t b = threadIdx.x >> 3; b < p.blocks_per_group; b += blockDim.x >> 3) {
-      const float *src = p.part + (group * p.blocks_per_group + b) * 4 * p.C + c;
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (k < parts) v[k] += src[(int64_t)k * p.C];
-    }
+    add_partials(p, 0, threadIdx.x >> 3, blockDim.x >> 3, c, p.post_weight ? 4 : 3, v);
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     v[k] += __shfl_xor_sync(~0u, v[k], 8);
@@ -745,39 +748,64 @@ __global__ void __launch_bounds__(1024) norm_bwd_sum_kernel(
   for (int k = 0; k < 4; ++k) {
     one[k] = 0.f;
     for (int i = 0; i < (int)(blockDim.x >> 5); ++i) one[k] += s[k][i][ci];
-    if (p.groups > 1) p.sums[(group * 4 + k) * p.C + c] = one[k];
   }
-  if (p.groups > 1) return;
   float total[5] = {0.f, 0.f, 0.f, 0.f, 0.f};
   add_group<P>(p, 0, c, one, total);
   write_totals<P>(p, c, total);
 }
 
+// Several gate groups: a block takes 8 columns, of whose 64 or 128 threads each
+// `p.share` (a power of two) share a group's partials; the groups' gradients are
+// added over the threads.  Both sums are trees of a fixed shape.  (In two kernels,
+// the groups' sums through memory: 64 groups of 1024 columns 19 us, now 7; 16384
+// groups 313, now 180.)
 template <typename P>
 __global__ void __launch_bounds__(1024) norm_bwd_groups_kernel(
     const __grid_constant__ NormBwdParams p) {
-  __shared__ float s[5][32][33];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int c = blockIdx.x * 32 + lane;
+  __shared__ float s[5][128][8];
+  const int ci = threadIdx.x & 7, t = threadIdx.x >> 3;
+  const int c = (int)blockIdx.x * 8 + ci, parts = p.post_weight ? 4 : 3;
+  const int share = p.share, sub = t & (share - 1);
   float total[5] = {0.f, 0.f, 0.f, 0.f, 0.f};
-  if (c < p.C)
-    for (int64_t g = warp; g < p.groups; g += 32) {
-      float one[4];
+  if (share == 1) {
+    if (c < p.C) {
+#pragma unroll 4
+      for (int64_t g = t; g < p.groups; g += blockDim.x >> 3) {
+        float one[4] = {0.f, 0.f, 0.f, 0.f};
+        add_partials(p, g, 0, 1, c, parts, one);
+        add_group<P>(p, g, c, one, total);
+      }
+    }
+  } else {  // (share x groups threads or more)
+    const int64_t g = t / share;
+    const bool live = c < p.C && g < p.groups;
+    float one[4] = {0.f, 0.f, 0.f, 0.f};
+    if (live) add_partials(p, g, sub, share, c, parts, one);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) one[k] = p.sums[(g * 4 + k) * p.C + c];
-      add_group<P>(p, g, c, one, total);
+    for (int k = 0; k < 4; ++k) s[k][t][ci] = one[k];
+    for (int o = share >> 1; o > 0; o >>= 1) {
+      __syncthreads();
+      if (sub < o)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) s[k][t][ci] += s[k][t + o][ci];
     }
 #pragma unroll
-  for (int k = 0; k < 5; ++k) s[k][warp][lane] = total[k];
-  __syncthreads();
-  if (warp == 0 && c < p.C) {
-#pragma unroll
-    for (int k = 0; k < 5; ++k) {
-      total[k] = 0.f;
-      for (int i = 0; i < 32; ++i) total[k] += s[k][i][lane];
-    }
-    write_totals<P>(p, c, total);
+    for (int k = 0; k < 4; ++k) one[k] = s[k][t][ci];
+    if (live && sub == 0) add_group<P>(p, g, c, one, total);
+    __syncthreads();
   }
+#pragma unroll
+  for (int k = 0; k < 5; ++k) s[k][t][ci] = total[k];
+  for (int o = (int)blockDim.x >> 4; o > 0; o >>= 1) {
+    __syncthreads();
+    if (t < o)
+#pragma unroll
+      for (int k = 0; k < 5; ++k) s[k][t][ci] += s[k][t + o][ci];
+  }
+  if (t > 0 || c >= p.C) return;
+#pragma unroll
+  for (int k = 0; k < 5; ++k) total[k] = s[k][0][ci];
+  write_totals<P>(p, c, total);
 }
 
 // --------------------------------------------------------------- dispatch
@@ -844,7 +872,6 @@ cudaError_t backward(NormBwdParams p, bool vec, cudaStream_t s, int *launches) {
   p.warps_per_row = plan.warps_per_row;
   p.blocks_per_group = plan.blocks_per_group;
   p.rows_per_group = p.rows / p.groups;
-  p.sums = p.part ? p.part + plan.part_floats : nullptr;
   // (blocks of 512 threads leave 128 registers a thread, too few for 16
   // elements: they serve the rows that need them)
   constexpr int V = kVec16<T>;
@@ -859,17 +886,16 @@ cudaError_t backward(NormBwdParams p, bool vec, cudaStream_t s, int *launches) {
                          : backward_e<T, P, 1, 16, 512>(p, plan, s);
   *launches = 1;
   if (e != cudaSuccess || !p.part) return e;
-  if (p.groups > 1 && p.blocks_per_group == 1) {
-    p.sums = p.part;  // one block per group: its partials are the group's sums
-    norm_bwd_groups_kernel<P><<<(unsigned)((p.C + 31) / 32), 1024, 0, s>>>(p);
-    ++*launches;
-    return cudaGetLastError();
+  const unsigned blocks = (unsigned)((p.C + 7) / 8);
+  if (p.groups == 1) {
+    norm_bwd_sum_kernel<P><<<blocks, p.blocks_per_group > 64 ? 1024 : 256, 0, s>>>(p);
+  } else {
+    // (up to 64 groups: blocks of 512 threads, several to an SM)
+    const int threads = p.groups <= 64 ? 512 : 1024;
+    p.share = 1;
+    while (2 * p.share * p.groups <= threads / 8) p.share *= 2;
+    norm_bwd_groups_kernel<P><<<blocks, threads, 0, s>>>(p);
   }
-  norm_bwd_sum_kernel<P><<<(unsigned)((p.C + 7) / 8 * p.groups),
-                           p.blocks_per_group > 64 ? 1024 : 256, 0, s>>>(p);
-  ++*launches;
-  if ((e = cudaGetLastError()) != cudaSuccess || p.groups == 1) return e;
-  norm_bwd_groups_kernel<P><<<(unsigned)((p.C + 31) / 32), 1024, 0, s>>>(p);
   ++*launches;
   return cudaGetLastError();
 }
@@ -890,13 +916,11 @@ NormBwdPlan norm_bwd_plan(int64_t rows, int64_t groups, int64_t C) {
   const int64_t share = resident / groups > 1 ? resident / groups : 1;
   plan.blocks_per_group = share < per_group ? share : per_group;
   plan.part_floats = groups * plan.blocks_per_group * 4 * C;
-  plan.sum_floats = groups > 1 && plan.blocks_per_group > 1 ? groups * 4 * C : 0;
   return plan;
 }
 
 int64_t norm_bwd_floats(int64_t rows, int64_t groups, int64_t C) {
-  const NormBwdPlan plan = norm_bwd_plan(rows, groups, C);
-  return plan.part_floats + plan.sum_floats;
+  return norm_bwd_plan(rows, groups, C).part_floats;
 }
 
 cudaError_t launch_residual_norm(const NormParams &p, int dtype, int param_dtype, bool vec,

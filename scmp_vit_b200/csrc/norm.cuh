@@ -35,18 +35,17 @@ struct NormBwdParams {
   void *dx, *dy;  // nullable
   void *dweight, *dbias, *dgamma, *dgate, *dpost_weight, *dpost_bias;  // nullable
   float *part;  // nullable (no parameter gradient wanted), see NormBwdPlan
-  float *sums;  // set by the launcher
   int64_t rows, groups;
   int C;
   bool rms;
   int64_t rows_per_group, blocks_per_group;  // set by the launcher, as below
-  int warps_per_row;
+  int warps_per_row, share;
 };
 
 struct NormBwdPlan {
   int warps_per_row, slots;  // slots: rows a block works on at a time
   int64_t blocks_per_group;
-  int64_t part_floats, sum_floats;  // workspace
+  int64_t part_floats;  // workspace
 };
 NormBwdPlan norm_bwd_plan(int64_t rows, int64_t groups, int64_t C);
 // Floats of workspace.
