@@ -83,10 +83,30 @@ def _stream(t: torch.Tensor):
     return ctypes.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
 
 
+def _check_glue(like: torch.Tensor, **tensors) -> None:
+    """The glue kernels take fp32 CUDA tensors, contiguous and of one shape, and
+    per-column parameters; anything else would be read past its end."""
+    if not like.is_cuda:
+        raise RuntimeError(f"the fused block glue runs on the CUDA engine only (no CPU path); "
+                           f"got {like.device}")
+    if not like.dim():
+        raise ValueError("the fused block glue takes rows [..., C]")
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if t.dtype != torch.float32:
+            raise TypeError(f"{name} must be float32, got {t.dtype}")
+        want = like.shape[-1:] if name in ("gamma", "bias") else like.shape
+        if t.shape != want or t.device != like.device or not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous {list(want)} on {like.device}, got "
+                             f"{tuple(t.shape)} strides {t.stride()} on {t.device}")
+
+
 def bias_gelu_(t: torch.Tensor, bias: torch.Tensor) -> torch.Tensor:
     """``t = gelu(t + bias)`` in place (fp32 CUDA ``[..., C]``, exact GELU):
     the bias add and torch's erf-form GELU in one pass, same bits."""
     from . import _lib
+    _check_glue(t, t=t, bias=bias)
     C = t.shape[-1]
     _lib.check(_lib.load().scmp_bias_gelu(t.data_ptr(), bias.data_ptr(), t.numel() // C, C,
                                           _stream(t)))
@@ -101,6 +121,7 @@ def scale_residual(x: torch.Tensor, y: torch.Tensor, gamma: torch.Tensor,
     unfused bias and a compensation term, in one pass; each step rounded as
     the separate torch ops round it.  ``out`` may be ``x`` or ``y``."""
     from . import _lib
+    _check_glue(x, x=x, y=y, gamma=gamma, bias=bias, extra=extra, out=out)
     C = x.shape[-1]
     out = torch.empty_like(x) if out is None else out
     _lib.check(_lib.load().scmp_scale_residual(
@@ -377,7 +398,7 @@ class Block(nn.Module):
         y, h = norm(self.norm2, getattr(self.mlp, "fc1", None), a, self.ls1.gamma)
         u = self.mlp(h)
         e = None if self.comp is None else self.comp(x).to(y.dtype)
-        if self._fused_glue_applies(y):
+        if self._fused_glue_applies(y) and u.dtype == torch.float32:
             return scale_residual(y, u.contiguous(), self.ls2.gamma, out=y,
                                   extra=None if e is None else e.contiguous())
         y = y + self.ls2(u)
@@ -385,16 +406,21 @@ class Block(nn.Module):
 
     def _fused_glue_applies(self, x: torch.Tensor) -> bool:
         return (FUSED_GLUE and x.is_cuda and x.dtype == torch.float32 and x.is_contiguous()
-                and not torch.is_grad_enabled() and type(self.ls1) is LayerScale
-                and type(self.ls2) is LayerScale)
+                and not torch.is_grad_enabled() and not torch.is_autocast_enabled("cuda")
+                and all(type(ls) is LayerScale and ls.gamma.dtype == torch.float32
+                        for ls in (self.ls1, self.ls2)))
 
     def _forward_fused_glue(self, x: torch.Tensor) -> torch.Tensor:
         """The forward above with its fp32 elementwise steps on the engine:
         ``x + ls1(a)`` in one pass, fc1's bias with the GELU, fc2's bias with
         ``ls2``, the residual add and the compensation term in another (the
-        matmuls stay cuBLAS fp32).  Bit-identical to the unfused forward."""
-        a = self.attn(self.norm1(x)).contiguous()
-        y = scale_residual(x, a, self.ls1.gamma)
+        matmuls stay cuBLAS fp32).  Bit-identical to the unfused forward.  A
+        branch in another type is added as there."""
+        a = self.attn(self.norm1(x))
+        if a.dtype == torch.float32:
+            y = scale_residual(x, a.contiguous(), self.ls1.gamma)
+        else:
+            y = x + self.ls1(a)
         h = self.norm2(y)
         mlp = self.mlp
         ub = None
@@ -406,6 +432,9 @@ class Block(nn.Module):
             ub = mlp.fc2.bias
         else:
             u = mlp(h)
+            if u.dtype != torch.float32:
+                y = y + self.ls2(u)
+                return y if self.comp is None else y + self.comp(x).to(y.dtype)
         e = None
         if self.comp is not None:
             e = self.comp(x).to(torch.float32).contiguous()
