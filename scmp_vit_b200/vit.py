@@ -378,7 +378,9 @@ class Block(nn.Module):
         if not (FUSED_NORM or type(qkv) is MXLinear or type(fc1) is MXLinear):
             return False
         norms = (self.norm1, self.norm2)
+        # (autocast keeps a 16-bit x's norms and residual in fp32, which r would not)
         return (x.is_cuda and x.dtype in _NORM_TYPES and x.shape[-1] <= 8192
+                and (x.dtype == torch.float32 or not torch.is_autocast_enabled("cuda"))
                 and type(self.ls1) is LayerScale
                 and all(type(n) is nn.LayerNorm and n.weight is not None and n.bias is not None
                         and n.weight.dtype in (x.dtype, torch.float32) for n in norms)
@@ -395,7 +397,12 @@ class Block(nn.Module):
 
         _, h = norm(self.norm1, self.attn.qkv)
         a = self.attn(h)
-        y, h = norm(self.norm2, getattr(self.mlp, "fc1", None), a, self.ls1.gamma)
+        if torch.promote_types(a.dtype, x.dtype) == x.dtype:
+            # (under autocast the branch comes in 16 bits: as wide as the sum it joins)
+            y, h = norm(self.norm2, getattr(self.mlp, "fc1", None), a.to(x.dtype), self.ls1.gamma)
+        else:
+            y = x + self.ls1(a)
+            h = self.norm2(y)
         u = self.mlp(h)
         e = None if self.comp is None else self.comp(x).to(y.dtype)
         if self._fused_glue_applies(y) and u.dtype == torch.float32:

@@ -208,3 +208,86 @@ def test_fused_norm_off_keeps_the_bits(cuda_device):
         assert torch.equal(m(x), a)
     # the fused norms differ in the order of their sums only (see above)
     assert (a - b).abs().max() <= 40 * (256 + 16) * U * a.abs().max()
+
+
+def block_in_autocast(blk, x, ops=()):
+    """A block's forward from the public calls, its branch widened to x's type."""
+    def norm(n, y=None, gamma=None, fmt=None):
+        return vit.residual_norm(x, y, n.weight, n.bias, eps=n.eps, gamma=gamma, quantize=fmt)
+
+    _, h = norm(blk.norm1, fmt="mxfp4" if "qkv_proj" in ops else None)
+    a = blk.attn(h)
+    assert a.dtype == torch.bfloat16 and x.dtype == torch.float32
+    y, h = norm(blk.norm2, a.float(), blk.ls1.gamma, "mxfp4" if "mlp_fc1" in ops else None)
+    return y + blk.ls2(blk.mlp(h))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ops", [("mlp_fc1",), ("qkv_proj", "mlp_fc2"), vit.MX_OPS])
+def test_4bit_linears_under_autocast(cuda_device, ops):
+    """The residual stream is fp32, the attention's output bf16."""
+    m = small(cuda_device)
+    vit.patch_vit_mx(m, ops)
+    x = torch.randn(2, 17, 128, generator=torch.Generator().manual_seed(6)).to(cuda_device)
+    with torch.no_grad(), torch.autocast("cuda", torch.bfloat16):
+        for blk in m.backbone.blocks:
+            got, want = blk(x), block_in_autocast(blk, x, ops)
+            assert got.dtype == torch.float32 and torch.equal(got, want)
+            x = got
+        assert bool(m(torch.randn(2, 3, 56, 56, device=cuda_device)).isfinite().all())
+
+
+@pytest.mark.gpu
+def test_fused_norm_training_under_autocast(cuda_device):
+    """The switch in mixed precision: a step's output and gradients are those of
+    the calls made one by one, in the same types as without it."""
+    from torch.nn.attention import SDPBackend, sdpa_kernel
+    m = small(cuda_device, rope=True)
+    blk = m.backbone.blocks[0]
+    g = torch.Generator().manual_seed(7)
+    x = torch.randn(2, 17, 128, generator=g).to(cuda_device).requires_grad_()
+    t = torch.randn(2, 17, 128, generator=g).to(cuda_device)
+    leaves = [x, *blk.parameters()]
+    with sdpa_kernel(SDPBackend.MATH):
+        with torch.autocast("cuda", torch.bfloat16):
+            plain = blk(x)
+            want = block_in_autocast(blk, x)
+            vit.set_fused_norm(True)
+            try:
+                got = blk(x)
+                wide = blk(x.detach().bfloat16())
+            finally:
+                vit.set_fused_norm(False)
+        assert got.dtype == plain.dtype == wide.dtype == torch.float32
+        assert torch.equal(got, want)
+        grads = [torch.autograd.grad((o * t).sum(), leaves) for o in (got, want)]
+    for a, b in zip(*grads):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_fused_norm_beside_a_wider_branch(cuda_device):
+    """A 16-bit block whose attention returns fp32 adds it as torch does."""
+    class Wide(torch.nn.Module):
+        def __init__(self, inner):
+            super().__init__()
+            self.inner, self.qkv = inner, inner.qkv
+
+        def forward(self, x):
+            return self.inner(x).float()
+
+    m = small(cuda_device, torch.bfloat16)
+    blk = m.backbone.blocks[0]
+    blk.attn, blk.norm2 = Wide(blk.attn), blk.norm2.float()
+    blk.mlp, blk.ls1 = blk.mlp.float(), blk.ls1.float()
+    x = torch.randn(2, 17, 128, device=cuda_device).bfloat16()
+    with torch.no_grad():
+        _, h = vit.residual_norm(x, None, blk.norm1.weight, blk.norm1.bias, eps=blk.norm1.eps)
+        y = x + blk.ls1(blk.attn(h))
+        want = y + blk.ls2(blk.mlp(blk.norm2(y)))
+        vit.set_fused_norm(True)
+        try:
+            got = blk(x)
+        finally:
+            vit.set_fused_norm(False)
+    assert got.dtype == torch.float32 and torch.equal(got, want)
