@@ -531,7 +531,8 @@ def make_sc_attention_forward(sc_prec: int, sc_av: bool, sc_qk: bool = True,
     """``forward(self, x)`` for a DINOv2-style attention module with
     ``qkv``, ``proj``, ``proj_drop``, ``num_heads``, ``scale`` attributes
     (same signature and numerics as ``cls/sc_attention_patch.py:248-328``).
-    A ``rope`` attribute (``GridRotary``) turns q and k before Q@K^T."""
+    A ``rope`` attribute that is a ``GridRotary`` turns q and k before Q@K^T;
+    what other modules keep under that name is left alone."""
     do_av = sc_av
 
     def forward(self, x, attn_bias=None):
@@ -540,7 +541,7 @@ def make_sc_attention_forward(sc_prec: int, sc_av: bool, sc_qk: bool = True,
         D = C // H
         qkv = self.qkv(x)
         rope = getattr(self, "rope", None)
-        if rope is not None:
+        if isinstance(rope, GridRotary):
             q, k, v = rope.split(qkv, H)
         elif qkv.is_cuda and qkv.element_size() in (2, 4) and B * H <= 65535 and D <= 256:
             q, k, v = split_qkv(qkv, H)

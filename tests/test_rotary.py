@@ -11,7 +11,8 @@ import pytest
 import torch
 
 from scmp_vit_b200 import _lib
-from scmp_vit_b200.attention import GridRotary, RotaryAxes, split_qkv, split_qkv_rotary
+from scmp_vit_b200.attention import (GridRotary, RotaryAxes, make_sc_attention_forward, split_qkv,
+                                     split_qkv_rotary)
 
 DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 U = 2.0 ** -24
@@ -298,3 +299,33 @@ def test_python_refusals(cuda_device):
             split_qkv_rotary(*args, **kw)
     with pytest.raises(TypeError, match="float32"):
         split_qkv_rotary(x.double(), 2, axes, pos)
+
+
+def test_sc_attention_leaves_a_foreign_rope_alone():
+    """Attention modules of other models keep an embedding, a function or a flag
+    under that name and turn q and k themselves, or elsewhere."""
+    class Attn(torch.nn.Module):
+        def __init__(self, rope):
+            super().__init__()
+            self.num_heads, self.scale, self.rope = 2, 0.5, rope
+            self.qkv, self.proj = torch.nn.Linear(8, 24), torch.nn.Linear(8, 8)
+            self.proj_drop = torch.nn.Identity()
+
+    x = torch.randn(2, 3, 8, generator=torch.Generator().manual_seed(1))
+    forward = make_sc_attention_forward(8, False, sc_qk=False)
+    torch.manual_seed(0)
+    want = forward(Attn(None), x)
+    for rope in (lambda q: q, True, torch.nn.Embedding(3, 4), "axial"):
+        torch.manual_seed(0)
+        m = Attn(None)
+        m.rope = rope
+        assert torch.equal(forward(m, x), want)
+
+
+def test_sc_attention_refuses_positions_on_the_cpu():
+    torch.manual_seed(0)
+    from scmp_vit_b200.vit import Attention
+    m = Attention(8, 2)
+    m.rope = GridRotary((1, 2), 4)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        make_sc_attention_forward(8, False, sc_qk=False)(m, torch.zeros(2, 3, 8))
