@@ -331,8 +331,9 @@ class Attention(nn.Module):
     def forward(self, x, attn_bias=None):
         B, N, C = x.shape
         H = self.num_heads
-        if self.rope is not None:
-            q, k, v = self.rope.split(self.qkv(x), H, transpose_v=False)
+        rope = getattr(self, "rope", None)  # (a module saved whole by an earlier version has none)
+        if rope is not None:
+            q, k, v = rope.split(self.qkv(x), H, transpose_v=False)
         else:
             qkv = self.qkv(x).reshape(B, N, 3, H, C // H).permute(2, 0, 3, 1, 4)
             q, k, v = qkv.unbind(0)

@@ -3,6 +3,7 @@ residual adds with their norms and 4-bit linears in a small ViT, bit for bit
 against the same calls made one by one, and the fused norms' training step
 against 64 bits."""
 import copy
+import pickle
 
 import pytest
 import torch
@@ -291,3 +292,13 @@ def test_fused_norm_beside_a_wider_branch(cuda_device):
         finally:
             vit.set_fused_norm(False)
     assert got.dtype == torch.float32 and torch.equal(got, want)
+
+
+def test_modules_saved_before_positions_run():
+    """An attention module pickled whole by an earlier version has no ``rope``."""
+    attn = vit.Attention(16, 2)
+    x = torch.randn(2, 5, 16, generator=torch.Generator().manual_seed(1))
+    want = attn(x)
+    del attn.rope
+    assert torch.equal(attn(x), want)
+    assert torch.equal(pickle.loads(pickle.dumps(attn))(x), want)
