@@ -396,7 +396,7 @@ class Block(nn.Module):
             fmt = reader.fmt if type(reader) is MXLinear and not torch.is_grad_enabled() else None
             return residual_norm(x, y, n.weight, n.bias, eps=n.eps, gamma=gamma, quantize=fmt)
 
-        _, h = norm(self.norm1, self.attn.qkv)
+        _, h = norm(self.norm1, getattr(self.attn, "qkv", None))
         a = self.attn(h)
         if torch.promote_types(a.dtype, x.dtype) == x.dtype:
             # (under autocast the branch comes in 16 bits: as wide as the sum it joins)
