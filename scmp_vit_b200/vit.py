@@ -73,7 +73,9 @@ FUSED_NORM = False
 
 
 def set_fused_norm(flag: bool) -> None:
-    """Turn the blocks' fused residual adds and norms on or off."""
+    """Turn the blocks' fused residual adds and norms on or off.  A block with
+    hooks on its norms or its first layer scale, which one pass would not call,
+    keeps the separate ones."""
     global FUSED_NORM
     FUSED_NORM = bool(flag)
 
@@ -129,6 +131,13 @@ def scale_residual(x: torch.Tensor, y: torch.Tensor, gamma: torch.Tensor,
         gamma.data_ptr(), None if extra is None else extra.data_ptr(), x.numel() // C, C,
         _stream(x)))
     return out
+
+
+def _watched(*modules: Optional[nn.Module]) -> bool:
+    """Whether hooks watch the modules' calls."""
+    return bool(torch.nn.modules.module._has_any_global_hook()) or any(
+        m is not None and bool(m._forward_hooks or m._forward_pre_hooks or m._backward_hooks
+                               or m._backward_pre_hooks) for m in modules)
 
 
 _NORM_TYPES = (torch.float32, torch.bfloat16, torch.float16)
@@ -385,22 +394,27 @@ class Block(nn.Module):
                 and type(self.ls1) is LayerScale
                 and all(type(n) is nn.LayerNorm and n.weight is not None and n.bias is not None
                         and n.weight.dtype in (x.dtype, torch.float32) for n in norms)
-                and self.ls1.gamma.dtype == self.norm2.weight.dtype)
+                and self.ls1.gamma.dtype == self.norm2.weight.dtype
+                and not _watched(*norms, self.ls1))
 
     def _forward_fused_norm(self, x):
         """The forward above with each norm in the pass of the residual add in
-        front of it; a norm whose reader is a 4-bit linear writes codes only."""
-        def norm(n, reader, y=None, gamma=None):
-            # (the reader of a patched block that is not a 4-bit linear, or any
-            # reader while gradients are recorded, takes values)
-            fmt = reader.fmt if type(reader) is MXLinear and not torch.is_grad_enabled() else None
+        front of it; a norm whose reader is a 4-bit linear writes codes only
+        (``attn`` or ``mlp`` then get an ``MXTensor``)."""
+        def norm(n, owner, name, y=None, gamma=None):
+            # (the reader of a patched block that is not a 4-bit linear, one whose
+            # input a hook sees, or any reader while gradients are recorded, takes
+            # values)
+            reader = getattr(owner, name, None)
+            fmt = reader.fmt if (type(reader) is MXLinear and not torch.is_grad_enabled()
+                                 and not _watched(owner, reader)) else None
             return residual_norm(x, y, n.weight, n.bias, eps=n.eps, gamma=gamma, quantize=fmt)
 
-        _, h = norm(self.norm1, getattr(self.attn, "qkv", None))
+        _, h = norm(self.norm1, self.attn, "qkv")
         a = self.attn(h)
         if torch.promote_types(a.dtype, x.dtype) == x.dtype:
             # (under autocast the branch comes in 16 bits: as wide as the sum it joins)
-            y, h = norm(self.norm2, getattr(self.mlp, "fc1", None), a.to(x.dtype), self.ls1.gamma)
+            y, h = norm(self.norm2, self.mlp, "fc1", a.to(x.dtype), self.ls1.gamma)
         else:
             y = x + self.ls1(a)
             h = self.norm2(y)
@@ -613,7 +627,8 @@ def patch_vit_mx(model: ViTClassifier, ops: Iterable[str] = MX_OPS, *,
     """Put the named linears of every block (the op names of ``patch_vit``) in
     microscaled 4 bits: ``mx.MXLinear`` from the present weights, which must be
     on the GPU.  The norms in front of qkv_proj and mlp_fc1 then write their
-    codes.  Inference only."""
+    codes, except where a hook watches the norm or the module that reads them.
+    Inference only."""
     ops = set(ops)
     unknown = ops - set(MX_OPS)
     if unknown:

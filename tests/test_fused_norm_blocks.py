@@ -41,3 +41,61 @@ def test_attention_without_a_qkv_linear(calls):
         want = y + blk.ls2(blk.mlp(blk.norm2(y)))
         assert torch.equal(blk(x), want)
     assert calls == [None, None]
+
+
+def patched(monkeypatch):
+    """Every linear in 4 bits, as modules that take values and codes alike."""
+    blk, x = block()
+
+    class Linear4(torch.nn.Linear):
+        fmt = "mxfp4"
+
+    monkeypatch.setattr(vit, "MXLinear", Linear4)
+    for owner, name in ((blk.attn, "qkv"), (blk.mlp, "fc1")):
+        getattr(owner, name).__class__ = Linear4
+    return blk, x
+
+
+def test_hooks_see_every_module_they_watch(calls):
+    """A block whose norms or layer scale are watched calls them as modules."""
+    blk, x = block()
+    with torch.no_grad():
+        want = blk(x)
+        assert calls == [None, None]
+        for m in (blk.norm1, blk.norm2, blk.ls1):
+            for register in ("register_forward_hook", "register_forward_pre_hook"):
+                fired = []
+                handle = getattr(m, register)(lambda *a: fired.append(1))
+                assert torch.equal(blk(x), want) and fired == [1]
+                handle.remove()
+        fired = []
+        handle = torch.nn.modules.module.register_module_forward_hook(
+            lambda m, *a: fired.append(m))
+        blk(x)
+        handle.remove()
+        assert {blk.norm1, blk.norm2, blk.ls1} <= set(fired)
+    assert calls == [None, None]
+    fired = []
+    handle = blk.norm2.register_full_backward_hook(lambda *a: fired.append(1))
+    blk(x.requires_grad_()).sum().backward()
+    handle.remove()
+    assert fired == [1] and calls == [None, None]
+
+
+def test_codes_only_where_nobody_watches(calls, monkeypatch):
+    blk, x = patched(monkeypatch)
+    with torch.no_grad():
+        blk(x)
+        assert calls == ["mxfp4", "mxfp4"]
+        for m, want in ((blk.attn, [None, "mxfp4"]), (blk.attn.qkv, [None, "mxfp4"]),
+                        (blk.mlp, ["mxfp4", None]), (blk.mlp.fc1, ["mxfp4", None])):
+            for register in ("register_forward_hook", "register_forward_pre_hook"):
+                del calls[:]
+                fired = []
+                handle = getattr(m, register)(lambda m, a, *out: fired.append(type(a[0])))
+                blk(x)
+                handle.remove()
+                assert calls == want and fired == [torch.Tensor]
+        del calls[:]
+        blk(x)
+        assert calls == ["mxfp4", "mxfp4"]
