@@ -2,6 +2,7 @@
 from __future__ import annotations
 
 import torch
+import torch.autograd.forward_ad as _forward_ad
 
 from . import _lib
 
@@ -28,6 +29,14 @@ def call(fn, index: int, *args) -> None:
             status = fn(*args, _raw_stream(index))
     if status:
         _lib.check(status)
+
+
+def has_tangent(tensors) -> bool:
+    """Whether one of the tensors (or None) is a dual one of forward-mode
+    differentiation, which ``requires_grad`` and the grad mode do not show."""
+    if getattr(_forward_ad, "_current_level", 0) < 0:  # outside every dual level: the usual case
+        return False
+    return any([t is not None and _forward_ad.unpack_dual(t).tangent is not None for t in tensors])
 
 
 def once_differentiable(backward):

@@ -21,7 +21,7 @@ import torch
 import torch.nn as nn
 
 from . import sc_linear as _scl
-from ._call import DTYPE, call, once_differentiable
+from ._call import DTYPE, call, has_tangent, once_differentiable
 from .mp import (
     AdaptiveMPConfig,
     AutoMPBudgetLogger,
@@ -470,7 +470,7 @@ def split_qkv_rotary(qkv: torch.Tensor, num_heads: int, axes: RotaryAxes, pos: t
     v as the transposed view of a contiguous [B, Hk, D, N], the layout that the
     Attn@V engine call reads, else contiguous.  fp32, bf16 or fp16; rotated in
     fp32 and rounded once, everything else copied bit for bit.
-    Differentiable (once) in ``qkv``."""
+    Differentiable (once, backward) in ``qkv``."""
     H = int(num_heads)
     Hk = H if num_kv_heads is None else int(num_kv_heads)
     if not qkv.is_cuda:
@@ -498,7 +498,8 @@ def split_qkv_rotary(qkv: torch.Tensor, num_heads: int, axes: RotaryAxes, pos: t
     if table.get_device() != index:
         raise ValueError(f"axes are on {table.device}, qkv on {qkv.device}")
     pos, transpose_v = pos.contiguous(), bool(transpose_v)
-    if torch.is_grad_enabled() and qkv.requires_grad:
+    if has_tangent((qkv,)) or (torch.is_grad_enabled() and qkv.requires_grad):
+        # (a forward-mode tangent is refused there: the function has no jvp)
         return _SplitQkvRotary.apply(qkv, pos, table, axes, H, Hk, transpose_v)
     return _split_rotary(qkv.contiguous(), pos, table, axes, H, Hk, transpose_v)
 

@@ -27,7 +27,7 @@ import torch
 import torch.nn as nn
 
 from . import _lib
-from ._call import call, dtype_code
+from ._call import call, dtype_code, has_tangent
 
 __all__ = ["MXTensor", "mx_quantize", "mx_matmul", "MXLinear", "tensor_scale_exp"]
 
@@ -46,11 +46,11 @@ def _check_exp(scale_exp: int) -> int:
 
 
 def _no_grad_wanted(name: str, *tensors) -> None:
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                raise RuntimeError(f"{name} has no gradient; call it under torch.no_grad() or on "
-                                   "detached inputs")
+    recorded = torch.is_grad_enabled() and any([t is not None and t.requires_grad
+                                                for t in tensors])
+    if recorded or has_tangent(tensors):
+        raise RuntimeError(f"{name} has no gradient; call it under torch.no_grad() or on "
+                           "detached inputs")
 
 
 def _sizes(rows: int, K: int, fmt: str):

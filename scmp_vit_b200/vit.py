@@ -29,7 +29,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from ._call import DTYPE, call, once_differentiable
+from ._call import DTYPE, call, has_tangent, once_differentiable
 from .attention import GridRotary, make_sc_attention_forward
 from .head_aligned_comp import HeadAlignedSCLinear
 from .mp import SeededRandomMPConfig, quantile_counts, set_current_block_idx
@@ -279,13 +279,15 @@ def residual_norm(x: torch.Tensor, y: Optional[torch.Tensor], weight: torch.Tens
     float32, all optional but ``weight``.  ``y=None`` is the norm alone: ``r``
     is ``x``.
 
-    Differentiable (once) in every tensor.  ``quantize="mxfp4"`` or ``"nvfp4"``
+    Differentiable (once, backward) in every tensor.  ``quantize="mxfp4"`` or ``"nvfp4"``
     returns ``h`` as an ``MXTensor`` quantised from its fp32 values (nvfp4 with
     tensor scale 1) for ``mx_matmul``; that form has no gradient.  The sums
     differ from ``F.layer_norm``'s in their order, so the bits may too."""
     _check_norm(x, y, weight, norm_bias, kind, eps, gamma, gate, post_weight, post_bias)
     leaves = (x, y, weight, norm_bias, gamma, gate, post_weight, post_bias)
-    if torch.is_grad_enabled() and any([t is not None and t.requires_grad for t in leaves]):
+    if has_tangent(leaves) or (torch.is_grad_enabled() and any(
+            [t is not None and t.requires_grad for t in leaves])):
+        # (a forward-mode tangent is refused there: the function has no jvp)
         if quantize is not None:
             raise RuntimeError("residual_norm with quantize has no gradient; call it under "
                                "torch.no_grad() or on detached inputs")
