@@ -73,6 +73,9 @@ class MXTensor:
     def __init__(self, data: torch.Tensor, scales: torch.Tensor, shape: Sequence[int], fmt: str,
                  scale_exp: int = 0, dtype: torch.dtype = torch.float32):
         shape = torch.Size(shape)
+        if not shape or shape[-1] < 1 or min(shape) < 0:
+            raise ValueError("an MXTensor has a last dimension of at least 1 and none below 0, got "
+                             f"{tuple(shape)}")
         want = _sizes(math.prod(shape[:-1]), shape[-1], _check_fmt(fmt))
         for t, size, what in ((data, want[0], "data"), (scales, want[1], "scales")):
             if t.dtype != torch.uint8 or not t.is_contiguous() or t.numel() != size:

@@ -572,3 +572,14 @@ def test_matmul_bounded_wait_gives_up_and_recovers(cuda_device, fmt):
         _lib.set_wait_limit(2_000_000_000)
     assert status & 1
     check_product(a, w, fmt, torch.float32)
+
+
+# --------------------------------------------------- CPU: tensors and modules
+
+@pytest.mark.parametrize("shape", [(4, 0), (0, 0), (0,), (), (-4, 32), (2, -2, 32), (4, -32)])
+def test_tensor_refuses_shapes_without_columns(shape):
+    """A product would divide by the last dimension."""
+    data, scales = torch.zeros(0, dtype=torch.uint8), torch.zeros(0, dtype=torch.uint8)
+    with pytest.raises(ValueError, match="last dimension"):
+        mx.MXTensor(data, scales, shape, "mxfp4")
+    assert mx.MXTensor(data, scales, (0, 32), "mxfp4").rows == 0
