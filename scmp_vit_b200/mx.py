@@ -60,6 +60,16 @@ def _sizes(rows: int, K: int, fmt: str):
     return rows * kp // 2, (rows + 127) // 128 * groups * 512
 
 
+def _check_bytes(data: torch.Tensor, scales: torch.Tensor, sizes) -> None:
+    if (data.dtype == scales.dtype == torch.uint8 and (data.numel(), scales.numel()) == sizes
+            and data.is_contiguous() and scales.is_contiguous()):
+        return
+    for t, size, what in ((data, sizes[0], "data"), (scales, sizes[1], "scales")):
+        if t.dtype != torch.uint8 or not t.is_contiguous() or t.numel() != size:
+            raise ValueError(f"{what} must be {size} contiguous bytes, got {t.numel()} of {t.dtype}"
+                             f" with strides {t.stride()}")
+
+
 class MXTensor:
     """A quantised tensor ``[..., K]``: codes and block scales on the GPU.
 
@@ -76,10 +86,7 @@ class MXTensor:
         if not shape or shape[-1] < 1 or min(shape) < 0:
             raise ValueError("an MXTensor has a last dimension of at least 1 and none below 0, got "
                              f"{tuple(shape)}")
-        want = _sizes(math.prod(shape[:-1]), shape[-1], _check_fmt(fmt))
-        for t, size, what in ((data, want[0], "data"), (scales, want[1], "scales")):
-            if t.dtype != torch.uint8 or not t.is_contiguous() or t.numel() != size:
-                raise ValueError(f"{what} must be {size} contiguous bytes for {tuple(shape)}")
+        _check_bytes(data, scales, _sizes(math.prod(shape[:-1]), shape[-1], _check_fmt(fmt)))
         if data.device != scales.device:
             raise ValueError(f"data on {data.device}, scales on {scales.device}")
         if data.data_ptr() % 16 or scales.data_ptr() % 16:
@@ -321,10 +328,13 @@ class MXLinear(nn.Module):
         self.scale_exp = int(state["scale_exp"])
 
     def quantized_weight(self) -> MXTensor:
+        data, scales = self.data, self.scales
+        # (buffers can be assigned: a state dict's own tensors, of any kind)
+        _check_bytes(data, scales, _sizes(self.out_features, self.in_features, self.fmt))
         return MXTensor.__new__(MXTensor)._set(
-            self.data, self.scales, None, self.data.data_ptr(), self.scales.data_ptr(),
-            self.data.get_device(), torch.Size((self.out_features, self.in_features)), self.fmt,
-            self.scale_exp, torch.float32)
+            data, scales, None, data.data_ptr(), scales.data_ptr(), data.get_device(),
+            torch.Size((self.out_features, self.in_features)), self.fmt, self.scale_exp,
+            torch.float32)
 
     def forward(self, x: Union[torch.Tensor, MXTensor]) -> torch.Tensor:
         return mx_matmul(x, self.quantized_weight(), bias=self.bias)

@@ -583,3 +583,30 @@ def test_tensor_refuses_shapes_without_columns(shape):
     with pytest.raises(ValueError, match="last dimension"):
         mx.MXTensor(data, scales, shape, "mxfp4")
     assert mx.MXTensor(data, scales, (0, 32), "mxfp4").rows == 0
+
+
+def linear_on_cpu(monkeypatch, fmt="mxfp4"):
+    monkeypatch.setattr(mx, "mx_quantize", lambda w, fmt, scale_exp: mx.mx_empty(
+        w.shape, fmt, w.device, w.dtype, scale_exp))
+    return mx.MXLinear(torch.nn.Linear(96, 72), fmt)
+
+
+@pytest.mark.parametrize("name", ["data", "scales"])
+@pytest.mark.parametrize("change", [
+    lambda t: t.float(), lambda t: torch.zeros(1, dtype=torch.uint8).expand(t.shape),
+    lambda t: torch.cat([t, t])[::2],
+])
+def test_linear_refuses_buffers_of_another_kind(monkeypatch, name, change):
+    """``load_state_dict(assign=True)`` takes the given tensors themselves, of any
+    type and stride; the kernels would read them as the packed layout."""
+    m = linear_on_cpu(monkeypatch)
+    state = m.state_dict()
+    state[name] = change(state[name])
+    m.load_state_dict(state, assign=True)
+    with pytest.raises(ValueError, match="contiguous bytes"):
+        m.quantized_weight()
+    m.load_state_dict(linear_on_cpu(monkeypatch).state_dict(), assign=True)
+    assert m.quantized_weight().shape == (72, 96)
+    setattr(m, name, getattr(m, name)[:-16])
+    with pytest.raises(ValueError, match="contiguous bytes"):
+        m.quantized_weight()
