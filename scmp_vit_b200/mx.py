@@ -195,6 +195,13 @@ def _overlap(out: torch.Tensor, t: torch.Tensor) -> bool:
     return t.data_ptr() < end and start < t.data_ptr() + span * t.element_size()
 
 
+def _overlap_codes(out: torch.Tensor, q: "MXTensor") -> bool:
+    """The same for ``q``'s codes and scales."""
+    start, end = out.data_ptr(), out.data_ptr() + out.numel() * out.element_size()
+    sizes = _sizes(q.rows, q.shape[-1], q.fmt)
+    return any([p < end and start < p + n for p, n in zip((q.data_ptr, q.scales_ptr), sizes)])
+
+
 def _check_input(x: torch.Tensor, name: str) -> int:
     code = dtype_code(x.dtype, "x")
     if not x.is_cuda:
@@ -226,7 +233,7 @@ def mx_matmul(a: Union[torch.Tensor, MXTensor], b: MXTensor, *,
     ``[..., N]``: the exact products of the 4-bit values summed in fp32, the
     bias added, rounded once to ``out_dtype`` (default: a's type).  A plain
     ``a`` is quantised to ``b``'s format first (nvfp4 with tensor scale 1).
-    ``out`` is contiguous and shares no memory with ``a`` or ``bias``."""
+    ``out`` is contiguous and shares no memory with the operands or ``bias``."""
     if not isinstance(b, MXTensor) or len(b.shape) != 2:
         raise TypeError("b must be a 2-D MXTensor [N, K]")
     if b.index < 0:
@@ -259,9 +266,9 @@ def mx_matmul(a: Union[torch.Tensor, MXTensor], b: MXTensor, *,
                 or out_dtype not in (None, out.dtype)):
             raise ValueError(f"out must be contiguous {shape} on {b.device} of out_dtype")
         out_code = dtype_code(out.dtype, "out")
-        for t in (a if plain else None, bias):
-            if t is not None and _overlap(out, t):
-                raise ValueError("out shares memory with an input")
+        if ((_overlap if plain else _overlap_codes)(out, a) or _overlap_codes(out, b)
+                or (bias is not None and _overlap(out, bias))):
+            raise ValueError("out shares memory with an input")
     bias_code, bias_ptr = 0, 0
     if bias is not None:
         if bias.shape != (N,) or bias.get_device() != index:

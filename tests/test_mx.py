@@ -610,3 +610,28 @@ def test_linear_refuses_buffers_of_another_kind(monkeypatch, name, change):
     setattr(m, name, getattr(m, name)[:-16])
     with pytest.raises(ValueError, match="contiguous bytes"):
         m.quantized_weight()
+
+
+def test_out_shares_no_memory_with_codes(monkeypatch):
+    """Outputs written while codes are still read; refused before any launch."""
+    monkeypatch.setattr(torch.Tensor, "is_cuda", True)
+    monkeypatch.setattr(torch.Tensor, "get_device", lambda t: 0)
+    launched = []
+    monkeypatch.setattr(mx, "call", lambda *a: launched.append(a))
+    cpu = torch.device("cpu")
+    a = mx.mx_empty(torch.Size((256, 64)), "nvfp4", cpu, torch.bfloat16)
+    b = mx.mx_empty(torch.Size((16, 64)), "nvfp4", cpu, torch.bfloat16)
+    few = mx.mx_empty(torch.Size((16, 64)), "nvfp4", cpu, torch.bfloat16)
+    for x, q in ((a, a), (few, b)):
+        size = 2 * x.rows * 16
+        for part in (q.data, q.scales):
+            memory = torch.empty(0, dtype=torch.uint8).set_(part.untyped_storage())
+            at = min(part.storage_offset(), memory.numel() - size)
+            out = memory[at:at + size].view(torch.bfloat16).view(x.rows, 16)
+            with pytest.raises(ValueError, match="shares memory"):
+                mx.mx_matmul(x, b, out=out)
+    with pytest.raises(ValueError, match="shares memory"):
+        mx.mx_matmul(torch.zeros(16, 64).bfloat16(), b, out=out)
+    assert launched == []
+    out = torch.empty(256, 16, dtype=torch.bfloat16)
+    assert mx.mx_matmul(a, b, out=out) is out and len(launched) == 1
