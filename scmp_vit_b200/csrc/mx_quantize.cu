@@ -150,7 +150,7 @@ __global__ void __launch_bounds__(kThreads)
       if (kFmt == SCMP_MXFP4)
         s = sc[i] == kMxNan ? __uint_as_float(0x7FC00000u) : e8m0_value(sc[i]);
       else
-        s = e4m3_value(sc[i]) * exp_value;
+        s = e4m3_value(sc[i]);
       float v[V];
 #pragma unroll
       for (int j = 0; j < V / 2; ++j) {
@@ -162,6 +162,12 @@ __global__ void __launch_bounds__(kThreads)
         const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h2));
         v[2 * j] = f.x * s;
         v[2 * j + 1] = f.y * s;
+        if (kFmt == SCMP_NVFP4) {
+          // last, since a scale times the tensor's may leave fp32's range where
+          // the value, a zero's for one, does not
+          v[2 * j] *= exp_value;
+          v[2 * j + 1] *= exp_value;
+        }
       }
       T *dst = out + r * K + ki;
       if (kVec) {

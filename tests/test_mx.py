@@ -635,3 +635,25 @@ def test_out_shares_no_memory_with_codes(monkeypatch):
     assert launched == []
     out = torch.empty(256, 16, dtype=torch.bfloat16)
     assert mx.mx_matmul(a, b, out=out) is out and len(launched) == 1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scale_exp", [120, 119, 0, -120])
+def test_dequantize_ends_of_the_range(cuda_device, scale_exp):
+    """Every scale code under the largest and smallest tensor scales: the values
+    that fp32 holds are exact, zero codes are zero whatever their scale."""
+    code = np.tile(np.arange(16), (128, 2))                # a row: two blocks of all codes
+    scale = np.stack([np.arange(128), np.arange(128)[::-1]], 1)  # 0x7F is NaN
+    data, scales = pack_ref(code, scale)
+    q = mx.MXTensor(torch.from_numpy(data).to(cuda_device),
+                    torch.from_numpy(scales).to(cuda_device), (128, 32), "nvfp4", scale_exp)
+    value = np.append(E4M3, np.nan)[scale] * 2.0 ** scale_exp
+    ref = np.repeat(value, 16, 1) * E2M1[code % 8] * np.where(code < 8, 1, -1)
+    ref = torch.from_numpy(ref)
+    for dtype in DTYPES:
+        got = q.dequantize(dtype).cpu()
+        want = ref.to(torch.float32).to(dtype)
+        assert torch.equal(got.isnan(), want.isnan())
+        assert torch.equal(got.nan_to_num(nan=0.0, posinf=None, neginf=None),
+                           want.nan_to_num(nan=0.0, posinf=None, neginf=None))
+        assert torch.equal(got.isinf(), want.isinf())
