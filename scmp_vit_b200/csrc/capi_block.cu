@@ -358,19 +358,18 @@ int scmp_split_qkv_rotary(const scmp_rotary_args *args, void *stream) {
   if (x.axes < 1 || x.axes > SCMP_MAX_AXES)
     return fail(SCMP_EINVAL, "axes must be 1 to %d, got %d", SCMP_MAX_AXES, x.axes);
   RotaryParams p{};
-  int64_t at = 0;
+  int64_t at = 0, turned = 0;
   for (int a = 0; a < x.axes; ++a) {
     if (x.dims[a] < 2 || x.dims[a] > x.D || x.dims[a] % 2 != 0 || x.sizes[a] < 1)
       return fail(SCMP_EINVAL, "axis %d: dims %d (even, >= 2), size %d (>= 1)", a, x.dims[a],
                   x.sizes[a]);
     p.dims[a] = x.dims[a];
     p.sizes[a] = x.sizes[a];
-    p.first_pair[a] = p.pairs;
     p.table_at[a] = at;
-    p.pairs += x.dims[a] / 2;
+    turned += x.dims[a];
     at += (int64_t)x.sizes[a] * (x.dims[a] / 2);
   }
-  if (2 * p.pairs > x.D) return fail(SCMP_EINVAL, "the axes' dims exceed the head size");
+  if (turned > x.D) return fail(SCMP_EINVAL, "the axes' dims exceed the head size");
   if (x.B == 0 || x.N == 0) return SCMP_OK;
   // pieces of a head row are counted in 32 bits
   if (x.N > UINT32_MAX / x.D || x.B > UINT32_MAX / x.D / x.N)

@@ -15,8 +15,8 @@ struct RotaryParams {
   const float2 *table;
   const int32_t *pos;  // [N, axes] or [B, N, axes]
   int64_t B, N, H, Hk;
-  int D, axes, pairs;  // pairs: rotated pairs of a head
-  int dims[SCMP_MAX_AXES], sizes[SCMP_MAX_AXES], first_pair[SCMP_MAX_AXES];
+  int D, axes;
+  int dims[SCMP_MAX_AXES], sizes[SCMP_MAX_AXES];
   int64_t table_at[SCMP_MAX_AXES];  // first entry of each axis
   bool pos_batched, interleaved, v_transposed, inverse;
   // set by the launcher: pieces per head row, tokens per sample, the blocks that
