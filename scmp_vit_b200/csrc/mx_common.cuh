@@ -29,6 +29,13 @@ template <> __device__ __forceinline__ __half from_f32<__half>(float v) {
   return __float2half_rn(v);
 }
 
+// Element i of an array of enum scmp_dtype.
+__device__ __forceinline__ float load_as_f32(const void *p, int dtype, int64_t i) {
+  if (dtype == SCMP_F32) return static_cast<const float *>(p)[i];
+  if (dtype == SCMP_BF16) return to_f32(static_cast<const __nv_bfloat16 *>(p)[i]);
+  return to_f32(static_cast<const __half *>(p)[i]);
+}
+
 // n / d for n < 2^32 by a multiplication and shifts (round-up method of Granlund
 // and Montgomery: m = ceil(2^(32 + s) / d) - 2^32, s = ceil(log2 d)).
 struct FastDiv {

@@ -162,12 +162,6 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap *map, int x, int 
       : "memory");
 }
 
-__device__ __forceinline__ float load_as_f32(const void *p, int dtype, int64_t i) {
-  if (dtype == SCMP_F32) return static_cast<const float *>(p)[i];
-  if (dtype == SCMP_BF16) return to_f32(static_cast<const __nv_bfloat16 *>(p)[i]);
-  return to_f32(static_cast<const __half *>(p)[i]);
-}
-
 // One row of 32 neighbouring features per lane, 32 activation rows in v: scaled,
 // with the bias, rounded, stored.  16-bit outputs whose pairs of features are
 // words (`words`: N even, out 4-byte aligned) go out as such: neighbouring lanes

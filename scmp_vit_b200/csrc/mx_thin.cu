@@ -17,11 +17,6 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kAhead = 2;  // 1024-value steps of a weight row in flight
 
-__device__ __forceinline__ float load_as_f32(const void *p, int dtype, int64_t i) {
-  if (dtype == SCMP_F32) return static_cast<const float *>(p)[i];
-  if (dtype == SCMP_BF16) return to_f32(static_cast<const __nv_bfloat16 *>(p)[i]);
-  return to_f32(static_cast<const __half *>(p)[i]);
-}
 __device__ __forceinline__ void store_as(void *p, int dtype, int64_t i, float v) {
   if (dtype == SCMP_F32)
     static_cast<float *>(p)[i] = v;
