@@ -365,6 +365,11 @@ SCMP_API int scmp_engine_status(int reset, unsigned int *flags);
  * synchronous and apply to the current device only. */
 SCMP_API int scmp_debug_set_wait_limit(uint64_t ns);
 SCMP_API int scmp_debug_hold_producers(int on);
+/* Which launch a 4-bit product [M, K] x [N, K]^T takes on a device that holds
+ * `pairs` CTA pairs at once: plan[0] = 1 for the one launch of few rows (with
+ * buffers for codes; 0: tiles), plan[1] = activation rows per tile, plan[2] =
+ * tiles.  Touches no device. */
+SCMP_API int scmp_debug_mx_plan(int64_t M, int64_t N, int64_t K, int pairs, int32_t *plan);
 
 /* Roofline probe (synchronous; allocates a small scratch buffer): runs a
  * register-only loop of one instruction class on every SM of the current

@@ -40,6 +40,7 @@ EXPORTED_SYMBOLS = (
     "scmp_probe_int_peak",
     "scmp_debug_set_wait_limit",
     "scmp_debug_hold_producers",
+    "scmp_debug_mx_plan",
     "scmp_prepack_b_size",
     "scmp_prepack_b",
     "scmp_split_qkv",
@@ -239,6 +240,8 @@ def load() -> ctypes.CDLL:
         lib.scmp_debug_set_wait_limit.restype = ctypes.c_int
         lib.scmp_debug_hold_producers.argtypes = [ctypes.c_int]
         lib.scmp_debug_hold_producers.restype = ctypes.c_int
+        lib.scmp_debug_mx_plan.argtypes = [i64, i64, i64, i32, ctypes.POINTER(ctypes.c_int32)]
+        lib.scmp_debug_mx_plan.restype = ctypes.c_int
         if lib.scmp_abi_version() != ABI_VERSION:
             raise RuntimeError(
                 f"engine ABI {lib.scmp_abi_version()} != expected {ABI_VERSION}")
@@ -269,6 +272,14 @@ def hold_producers(on: bool) -> None:
     """Test hook: make the e2m1 kernels' bounded waits run out (see
     ``scmp_debug_hold_producers`` in the header)."""
     check(load().scmp_debug_hold_producers(1 if on else 0))
+
+
+def mx_plan(M: int, N: int, K: int, pairs: int = 74) -> tuple:
+    """(one launch of few rows?, activation rows per tile, tiles) of a 4-bit
+    product on ``pairs`` CTA pairs; for tests that mean a certain variant."""
+    plan = (ctypes.c_int32 * 3)()
+    check(load().scmp_debug_mx_plan(int(M), int(N), int(K), int(pairs), plan))
+    return bool(plan[0]), plan[1], plan[2]
 
 
 def probe_int_peak(kind: int) -> float:

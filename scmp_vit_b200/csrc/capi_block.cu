@@ -190,6 +190,20 @@ int scmp_mx_linear(const void *x, int x_dtype, int64_t ld, const scmp_mx_matmul_
   return rc != SCMP_OK ? rc : scmp_mx_matmul(args, stream);
 }
 
+int scmp_debug_mx_plan(int64_t M, int64_t N, int64_t K, int pairs, int32_t *plan) {
+  set_last_error("");
+  int rc;
+  if ((rc = check_mx(M, K, SCMP_MXFP4)) != SCMP_OK || (rc = check_mx(N, K, SCMP_MXFP4)) != SCMP_OK)
+    return rc;
+  if (M == 0 || N == 0 || pairs < 1 || !plan)
+    return fail(SCMP_EINVAL, "mx_plan takes a product with outputs, pairs >= 1 and a plan");
+  const MxTilePlan tiles = mx_tile_plan(M, N, pairs);
+  plan[0] = mx_thin(M, N, K) ? 1 : 0;
+  plan[1] = tiles.nt;
+  plan[2] = (int32_t)tiles.tiles;
+  return SCMP_OK;
+}
+
 int scmp_residual_norm(const scmp_norm_args *args, void *stream) {
   set_last_error("");
   if (!args) return fail(SCMP_EINVAL, "args is NULL");

@@ -224,6 +224,12 @@ struct MxProduct {
   void *out;  // [M, N] row-major
   int out_dtype;
 };
+// Activation rows per tile and tiles of 256 weight rows x that, over `pairs`.
+struct MxTilePlan {
+  int nt;
+  uint32_t tiles_f, tiles;
+};
+MxTilePlan mx_tile_plan(int64_t M, int64_t N, int pairs);
 cudaError_t launch_mx_matmul(const MxProduct &p, unsigned int *error, cudaStream_t s);
 // A few rows: x quantised in the same launch, or NULL with p.a's codes.  Which
 // products that launch can take, and where it is faster than quantise + tiles.

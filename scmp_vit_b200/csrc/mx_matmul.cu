@@ -527,10 +527,10 @@ cudaError_t launch(MxTiles t, int64_t kp, int64_t groups, cudaStream_t s) {
     if (clusters <= 0) return cudaErrorInvalidConfiguration;
     if (dev < kMaxCachedDevices) max_clusters[dev].store(clusters, std::memory_order_relaxed);
   }
-  t.tiles_f = (uint32_t)((t.p.N + 255) / 256);
-  t.nt = tile_rows(t.p.M, t.tiles_f, clusters);
-  // (2^31 tiles of 256 x 64 outputs do not fit the memory)
-  t.tiles = t.tiles_f * (uint32_t)((t.p.M + t.nt - 1) / t.nt);
+  const MxTilePlan plan = mx_tile_plan(t.p.M, t.p.N, clusters);
+  t.tiles_f = plan.tiles_f;
+  t.nt = plan.nt;
+  t.tiles = plan.tiles;
   t.steps = (int)((kp + 255) / 256);
   t.mmas = (int)((kp + 63) / 64);
   t.xrows = t.nt > 128 ? 2 : 1;
@@ -566,6 +566,15 @@ cudaError_t launch_typed(const MxTiles &t, int64_t kp, int64_t groups, cudaStrea
 }
 
 }  // namespace
+
+MxTilePlan mx_tile_plan(int64_t M, int64_t N, int pairs) {
+  MxTilePlan plan;
+  plan.tiles_f = (uint32_t)((N + 255) / 256);
+  plan.nt = tile_rows(M, plan.tiles_f, pairs);
+  // (2^31 tiles of 256 x 64 outputs do not fit the memory)
+  plan.tiles = plan.tiles_f * (uint32_t)((M + plan.nt - 1) / plan.nt);
+  return plan;
+}
 
 cudaError_t launch_mx_matmul(const MxProduct &p, unsigned int *error, cudaStream_t s) {
   const MxLayout l = mx_layout(p.M, p.K, p.fmt);

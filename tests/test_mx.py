@@ -657,3 +657,131 @@ def test_dequantize_ends_of_the_range(cuda_device, scale_exp):
         assert torch.equal(got.nan_to_num(nan=0.0, posinf=None, neginf=None),
                            want.nan_to_num(nan=0.0, posinf=None, neginf=None))
         assert torch.equal(got.isinf(), want.isinf())
+
+
+# ------------------------------------- the variants that large calls take
+# Tiles: a pair of CTAs that goes from tile to tile uses its second accumulator,
+# hands accumulators back and carries the ring's phases on; 128 and 192 rows a
+# tile read scales of two row groups and store a second and a third piece.
+
+# M, N, K, rows per tile and tiles per pair (at least) on 74 pairs
+MANY_TILES = [(16448, 1040, 288, 192, 5),   # rows of whole 16-byte pieces: TMA stores
+              (20000, 1030, 96, 192, 7),    # two features a store
+              (12000, 2049, 544, 192, 7),   # one feature a store
+              (30000, 1040, 40, 192, 10),   # one stage a tile, mostly past K
+              (3000, 8200, 64, 192, 7),
+              (2000, 2056, 1100, 128, 1.9),
+              (1800, 4102, 64, 128, 3),
+              (1700, 4099, 2600, 128, 3),   # eleven stages a tile: the ring wraps inside it
+              (3500, 1000, 2600, 64, 2.9),
+              (800, 4101, 160, 64, 2.9),
+              (1300, 4100, 1024, 192, 1.6)]
+
+
+def test_many_tiles_are_many():
+    for M, N, K, nt, each in MANY_TILES:
+        few, rows, tiles = _lib.mx_plan(M, N, K)
+        assert not few and rows == nt and tiles >= 74 * each, (M, N, K, rows, tiles)
+
+
+def test_few_rows_rule():
+    """``mx._thin`` (no buffers asked for) is the engine's own rule."""
+    sizes = [*range(1, 200, 13), *range(200, 20000, 331), *(1024 * i for i in range(1, 40))]
+    for K in (1, 31, 32, 1000, 1024, 2048, 4096, 5000, 6143, 6144, 6145, 8192):
+        for M in range(1, 7):
+            for N in sizes:
+                assert mx._thin(M, N, K) == _lib.mx_plan(M, N, K)[0], (M, N, K)
+
+
+@pytest.mark.parametrize("M,N,K,pairs", [(0, 4, 4, 74), (4, 0, 4, 74), (4, 4, 0, 74),
+                                         (4, 4, 4, 0), (-1, 4, 4, 74)])
+def test_plan_refusals(M, N, K, pairs):
+    with pytest.raises(_lib.EngineError):
+        _lib.mx_plan(M, N, K, pairs)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("M,N,K", [s[:3] for s in MANY_TILES])
+def test_matmul_many_tiles(cuda_device, fmt, M, N, K):
+    g = torch.Generator().manual_seed(M + N + K)
+    a = torch.randn(M, K, generator=g) * torch.exp(torch.randn(M, 1, generator=g))
+    w = (torch.randn(N, K, generator=g) * 0.05).to(cuda_device)
+    bias = torch.randn(N, generator=g).to(cuda_device)
+    exp = -12 if fmt == "nvfp4" else 0
+    for dtype in DTYPES:
+        x = a.to(dtype).to(cuda_device)
+        y = check_product(x, w, fmt, dtype, bias.to(dtype), exp)
+        # a row's result does not depend on the rows around it, nor on its tile
+        q = mx.mx_quantize(w, fmt, scale_exp=exp)
+        for at in (0, M // 2 + 1, M - 70):
+            assert torch.equal(mx.mx_matmul(x[at:at + 70], q, bias=bias.to(dtype)), y[at:at + 70])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FMTS)
+def test_many_tiles_repeat_and_keep_to_their_rows(cuda_device, fmt):
+    """The same bits again, and guards around an output whose last tile is cut."""
+    M, N, K = 16449, 1040, 288
+    x = torch.randn(M, K, device=cuda_device).bfloat16()
+    w = mx.mx_quantize(torch.randn(N, K, device=cuda_device), fmt)
+    first = mx.mx_matmul(x, w)
+    for dtype, pad in ((torch.bfloat16, 64), (torch.bfloat16, 1), (torch.float32, 3)):
+        buf = torch.full((M * N + 2 * pad,), 7.0, dtype=dtype, device=cuda_device)
+        out = buf[pad:-pad].view(M, N)
+        mx.mx_matmul(x, w, out=out)
+        assert torch.equal(out.bfloat16(), first)
+        assert bool((buf[:pad] == 7).all()) and bool((buf[-pad:] == 7).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("rows,K,dtypes", [
+    (1300, 1056, DTYPES), (1300, 1057, DTYPES),   # four chunks a warp, whole and odd rows
+    (2600, 4104, DTYPES[1:2]),                    # several units a row
+    (19500, 520, DTYPES[:1]),                     # more units than warps
+])
+def test_quantize_bytes_many_rows(cuda_device, fmt, rows, K, dtypes):
+    g = torch.Generator().manual_seed(rows + K)
+    x = torch.randn(rows, K, generator=g) * torch.exp(3 * torch.randn(rows, 1, generator=g))
+    for dtype in dtypes:
+        q = check_quantize(x.to(dtype).to(cuda_device), fmt)
+        values = q.dequantize(torch.float32)      # (compared with the reference above)
+        for to in DTYPES[1:]:
+            # (fp16 inputs past their range are infinities: blocks of NaN)
+            assert torch.allclose(q.dequantize(to), values.to(to), rtol=0, atol=0, equal_nan=True)
+
+
+@pytest.mark.gpu
+def test_captured_product_behind_two_streams(cuda_device):
+    """A captured product whose operands come from two streams, with a copy
+    between them: it waits for all of them in every replay."""
+    g = torch.Generator().manual_seed(11)
+    a, w = (torch.randn(n, 256, generator=g).to(cuda_device) for n in (3000, 520))
+    src, wsrc, out = a.clone(), w.clone(), torch.empty(3000, 520, device=cuda_device)
+    side = torch.cuda.Stream()
+
+    def step():
+        main = torch.cuda.current_stream()
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            w.copy_(wsrc)
+            qw = mx.mx_quantize(w)
+        a.copy_(src)
+        qa = mx.mx_quantize(a)
+        main.wait_stream(side)
+        y = mx.mx_matmul(qa, qw, out=out)
+        out.mul_(2)
+        return mx.mx_matmul(qa, qw), y
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        plain, doubled = step()
+    for i in range(3):
+        src.copy_(torch.randn(3000, 256, generator=g))
+        wsrc.copy_(torch.randn(520, 256, generator=g))
+        graph.replay()
+        want = mx.mx_matmul(src, mx.mx_quantize(wsrc))
+        assert torch.equal(plain, want) and torch.equal(doubled, 2 * want)
