@@ -546,3 +546,102 @@ def test_backward_in_a_graph(cuda_device):
     ref = torch.autograd.grad(call(t, kind), leaves, (dr, dr))
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got, ref))
+
+
+# ------------------------------------- the variants that large calls take
+# Slots that walk: 16-bit rows, and fp32 rows of warps that do not fill a block,
+# from some 1200 rows on (148 SMs x 3 or 4 blocks x the rows of a block), the next
+# row's loads issued into the registers of the one at work.  Backward slots with
+# more rows than their ring has stages (148 x 1 or 2 blocks), and parameters read
+# again from shared memory.
+
+MANY = [(8, 600, 1024), (8, 601, 1408), (3, 700, 2504), (2, 900, 4104), (4, 700, 1001),
+        (3, 500, 2501), (2, 500, 4101), (5, 500, 200)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", [0, 3, 5, 6])
+@pytest.mark.parametrize("shape", MANY)
+def test_forward_many_rows(cuda_device, shape, form):
+    for dtype in DTYPES:
+        t, kind = make(shape, dtype, cuda_device, **FORMS[form])
+        r, h = call(t, kind)
+        check_forward(t, kind, r, h)
+        again = call(t, kind)
+        assert torch.equal(r, again[0]) and torch.equal(h, again[1])
+
+
+@pytest.mark.gpu
+def test_forward_of_a_training_batch(cuda_device):
+    for post in (False, True):
+        t, kind = make((16, 1025, 1408), torch.bfloat16, cuda_device, kind="rms", bias=False,
+                       gate=True, post=post)
+        check_forward(t, kind, *call(t, kind))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("shape", [(8, 600, 1024), (8, 601, 1408), (3, 700, 2504), (2, 900, 4104),
+                                   (5, 500, 200)])
+def test_quantized_output_many_rows(cuda_device, fmt, shape):
+    """Byte for byte the codes of the same pass's h in fp32, rows past the last
+    one (up to whole atoms of scales) included."""
+    for dtype in DTYPES:
+        for form in (dict(), dict(gate=True, post=True), dict(branch=False, kind="rms")):
+            t, kind = make(shape, dtype, cuda_device, **form)
+            r, q = call(t, kind, quantize=fmt)
+            h32 = torch.empty(shape, dtype=torch.float32, device=cuda_device)
+            r2 = vit._norm_launch(*[t[k] for k in NAMES], kind, EPS, None, h32)
+            ref = mx.mx_quantize(h32, fmt)
+            assert r is t["x"] if r2 is None else torch.equal(r, r2)
+            assert torch.equal(q.data, ref.data) and torch.equal(q.scales, ref.scales)
+            _, f = forward64(t, kind, r)
+            close(h32, f["h"], (shape[-1] + 16) * U * f["H"], "h in fp32")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("shape", [(2, 3, 7), (2, 70, 1025), (3, 90, 1001)])
+def test_quantized_output_of_odd_rows(cuda_device, fmt, shape):
+    """Rows in single elements deal their columns alike in every type: with the
+    rounded r widened, N(r) is computed from the same numbers in the same order,
+    so the codes are those of the fp32 call."""
+    for dtype in (torch.bfloat16, torch.float16):
+        t, kind = make(shape, dtype, cuda_device, gate=True, post=True)
+        r, q = call(t, kind, quantize=fmt)
+        t2 = {k: None for k in NAMES}
+        t2.update(x=r.float(), weight=t["weight"].float(), norm_bias=t["norm_bias"].float())
+        _, h = call(t2, kind)
+        ref = mx.mx_quantize(h, fmt)
+        assert q.dtype == dtype and q.shape == shape
+        assert torch.equal(q.data, ref.data) and torch.equal(q.scales, ref.scales)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", [0, 3, 4, 6])
+@pytest.mark.parametrize("shape", MANY)
+def test_backward_many_rows(cuda_device, shape, form):
+    for dtype in DTYPES:
+        t, kind = make(shape, dtype, cuda_device, grad=True, **FORMS[form])
+        r, h = call(t, kind)
+        g = torch.Generator().manual_seed(7)
+        dr = torch.randn(shape, generator=g).to(dtype).to(cuda_device)
+        dh = torch.randn(shape, generator=g).to(dtype).to(cuda_device)
+        check_grads(t, kind, r, h, dr if t["y"] is not None else None, dh)
+        r, h = call(t, kind)
+        leaves = [t[k] for k in NAMES if t[k] is not None]
+        outs, grads = ((h,), (dh,)) if t["y"] is None else ((r, h), (dr, dh))
+        first = torch.autograd.grad(outs, leaves, grads, retain_graph=True)
+        again = torch.autograd.grad(outs, leaves, grads)
+        assert all(torch.equal(a, b) for a, b in zip(first, again))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_many_rows_fp32_parameters(cuda_device, dtype):
+    for shape in ((8, 600, 1024), (2, 900, 4104), (4, 700, 1001)):
+        t, kind = make(shape, dtype, cuda_device, grad=True, gate=True, post=True,
+                       param_dtype=torch.float32)
+        r, h = call(t, kind)
+        check_forward(t, kind, r, h)
+        check_grads(t, kind, r, h, torch.randn_like(r), torch.randn_like(h))
