@@ -329,3 +329,47 @@ def test_sc_attention_refuses_positions_on_the_cpu():
     m.rope = GridRotary((1, 2), 4)
     with pytest.raises(RuntimeError, match="no CPU path"):
         make_sc_attention_forward(8, False, sc_qk=False)(m, torch.zeros(2, 3, 8))
+
+
+# ------------------------------------- the variants that large calls take
+
+LARGE = [  # B, H, Hk, D, dims, grid: a thread walks three heads or more, in batches of four
+    (16, 16, 16, 64, [32, 32], (16, 16)),
+    (24, 12, 4, 64, [16, 24, 24], (3, 9, 9)),
+    (120, 5, 5, 40, [20, 20], (13, 15)),
+    (16, 10, 2, 128, [44, 42, 42], (4, 8, 9)),
+    (30, 7, 7, 34, [30], (200,)),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("interleaved", [True, False])
+@pytest.mark.parametrize("case", range(len(LARGE)))
+def test_values_and_gradient_of_many_tokens(cuda_device, case, interleaved):
+    B, H, Hk, D, dims, grid = LARGE[case]
+    dev = cuda_device
+    pos = positions(grid, 1).to(dev)
+    N = pos.shape[0]
+    # the heads that one thread takes with the widest pieces, v in blocks of its own
+    widest = next(v for v in (8, 4, 2) if D % v == 0)
+    assert (H + Hk) * (B * N * (D // widest) // 256) // (148 * 6) >= 3
+    scales = [1.0, 0.5, 2.0][:len(dims)]
+    axes = RotaryAxes(dims, grid, base=1000.0, scales=scales, interleaved=interleaved, device=dev)
+    for dtype in DTYPES:
+        g = torch.Generator().manual_seed(case)
+        qkv = torch.randn(B, N, (H + 2 * Hk) * D, generator=g).to(dtype).to(dev).requires_grad_()
+        heads = qkv.detach().reshape(B, N, H + 2 * Hk, D).transpose(1, 2)
+        want = rotate64(heads[:, :H + Hk], dims, pos, 1000.0, scales, interleaved)
+        grad = torch.randn(heads.shape, generator=g).to(dtype).to(dev)
+        back = rotate64(grad[:, :H + Hk], dims, pos, 1000.0, scales, interleaved, -1)
+        for transpose_v in (True, False):
+            q, k, v = split_qkv_rotary(qkv, H, axes, pos, num_kv_heads=Hk, transpose_v=transpose_v)
+            close(torch.cat([q, k], 1).detach(), *want)
+            assert torch.equal(v, heads[:, H + Hk:])
+            dv = grad[:, H + Hk:]
+            if transpose_v:
+                dv = dv.transpose(-1, -2).contiguous().transpose(-1, -2)
+            (dqkv,) = torch.autograd.grad((q, k, v), (qkv,), (grad[:, :H], grad[:, H:H + Hk], dv))
+            dqkv = dqkv.reshape(B, N, H + 2 * Hk, D).transpose(1, 2)
+            close(dqkv[:, :H + Hk], *back)
+            assert torch.equal(dqkv[:, H + Hk:], dv)
