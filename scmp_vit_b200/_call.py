@@ -25,6 +25,8 @@ def call(fn, index: int, *args) -> None:
     if _current_device() == index:
         status = fn(*args, _raw_stream(index))
     else:
+        if index < 0:
+            raise RuntimeError("runs on the CUDA engine only (no CPU path)")
         with torch.cuda.device(index):
             status = fn(*args, _raw_stream(index))
     if status:

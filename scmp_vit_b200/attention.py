@@ -366,9 +366,8 @@ def split_qkv(qkv: torch.Tensor, num_heads: int):
     q = torch.empty(B, H, N, D, dtype=qkv.dtype, device=qkv.device)
     k = torch.empty_like(q)
     vt = torch.empty(B, H, D, N, dtype=qkv.dtype, device=qkv.device)
-    stream = torch.cuda.current_stream(qkv.device).cuda_stream
-    _lib.check(_lib.load().scmp_split_qkv(src.data_ptr(), B, N, H, D, src.element_size(),
-                                          q.data_ptr(), k.data_ptr(), vt.data_ptr(), stream))
+    call(_lib.load().scmp_split_qkv, src.get_device(), src.data_ptr(), B, N, H, D,
+         src.element_size(), q.data_ptr(), k.data_ptr(), vt.data_ptr())
     return q, k, vt.transpose(-1, -2)
 
 

@@ -80,11 +80,6 @@ def set_fused_norm(flag: bool) -> None:
     FUSED_NORM = bool(flag)
 
 
-def _stream(t: torch.Tensor):
-    import ctypes
-    return ctypes.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
-
-
 def _check_glue(like: torch.Tensor, **tensors) -> None:
     """The glue kernels take fp32 CUDA tensors, contiguous and of one shape, and
     per-column parameters; anything else would be read past its end."""
@@ -110,8 +105,8 @@ def bias_gelu_(t: torch.Tensor, bias: torch.Tensor) -> torch.Tensor:
     from . import _lib
     _check_glue(t, t=t, bias=bias)
     C = t.shape[-1]
-    _lib.check(_lib.load().scmp_bias_gelu(t.data_ptr(), bias.data_ptr(), t.numel() // C, C,
-                                          _stream(t)))
+    call(_lib.load().scmp_bias_gelu, t.get_device(), t.data_ptr(), bias.data_ptr(),
+         t.numel() // max(1, C), C)
     return t
 
 
@@ -126,10 +121,8 @@ def scale_residual(x: torch.Tensor, y: torch.Tensor, gamma: torch.Tensor,
     _check_glue(x, x=x, y=y, gamma=gamma, bias=bias, extra=extra, out=out)
     C = x.shape[-1]
     out = torch.empty_like(x) if out is None else out
-    _lib.check(_lib.load().scmp_scale_residual(
-        out.data_ptr(), x.data_ptr(), y.data_ptr(), None if bias is None else bias.data_ptr(),
-        gamma.data_ptr(), None if extra is None else extra.data_ptr(), x.numel() // C, C,
-        _stream(x)))
+    call(_lib.load().scmp_scale_residual, x.get_device(), out.data_ptr(), x.data_ptr(),
+         y.data_ptr(), _ptr(bias), gamma.data_ptr(), _ptr(extra), x.numel() // max(1, C), C)
     return out
 
 

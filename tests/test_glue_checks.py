@@ -2,32 +2,32 @@
 of one shape: other operands are refused, and a block whose branch comes in
 another type adds it the ordinary way.  The library call is replaced on the
 CPU, so nothing here reads memory that it should not."""
-import ctypes
-
 import pytest
 import torch
 
-from scmp_vit_b200 import _lib, vit
+from scmp_vit_b200 import _lib, attention, vit
 
 
 class Recorder:
-    """Stands for the library: counts its calls."""
+    """Stands for the library: keeps its calls' names and device indices."""
 
     def __init__(self):
-        self.calls = 0
+        self.made = []
 
     def __getattr__(self, name):
-        def run(*args):
-            self.calls += 1
-            return 0
-        return run
+        return name
+
+    @property
+    def calls(self):
+        return len(self.made)
 
 
 @pytest.fixture
 def lib(monkeypatch):
     rec = Recorder()
     monkeypatch.setattr(_lib, "load", lambda: rec)
-    monkeypatch.setattr(vit, "_stream", lambda t: ctypes.c_void_p(0))
+    for module in (vit, attention):
+        monkeypatch.setattr(module, "call", lambda fn, index, *args: rec.made.append((fn, index)))
     monkeypatch.setattr(torch.Tensor, "is_cuda", True)
     return rec
 
@@ -72,11 +72,23 @@ class Bf16Branch(torch.nn.Module):
         return self.inner(x).bfloat16()
 
 
+def test_calls_go_to_their_tensors_device(lib, monkeypatch):
+    """On the default stream, whose handle every device shares, a launch on the
+    current device would be given another device's memory."""
+    monkeypatch.setattr(torch.Tensor, "get_device", lambda t: 3)
+    vit.scale_residual(X, X.clone(), G)
+    vit.bias_gelu_(X.clone(), G)
+    attention.split_qkv(torch.zeros(2, 3, 24), 2)
+    assert lib.made == [("scmp_scale_residual", 3), ("scmp_bias_gelu", 3), ("scmp_split_qkv", 3)]
+
+
 def test_no_cpu_path():
     with pytest.raises(RuntimeError, match="no CPU path"):
         vit.scale_residual(X, X, G)
     with pytest.raises(RuntimeError, match="no CPU path"):
         vit.bias_gelu_(X, G)
+    with pytest.raises(RuntimeError):  # (a machine without a GPU says so itself)
+        attention.split_qkv(torch.zeros(2, 3, 24), 2)
 
 
 @pytest.mark.parametrize("where", ["attn", "mlp", "both"])
