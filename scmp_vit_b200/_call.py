@@ -36,7 +36,7 @@ def call(fn, index: int, *args) -> None:
 def has_tangent(tensors) -> bool:
     """Whether one of the tensors (or None) is a dual one of forward-mode
     differentiation, which ``requires_grad`` and the grad mode do not show."""
-    if getattr(_forward_ad, "_current_level", 0) < 0:  # outside every dual level: the usual case
+    if _forward_ad._current_level < 0:  # outside every dual level: the usual case
         return False
     return any([t is not None and _forward_ad.unpack_dual(t).tangent is not None for t in tensors])
 

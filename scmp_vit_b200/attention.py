@@ -20,6 +20,7 @@ from typing import Callable, Optional
 import torch
 import torch.nn as nn
 
+from . import _lib
 from . import sc_linear as _scl
 from ._call import DTYPE, call, has_tangent, once_differentiable
 from .mp import (
@@ -358,7 +359,6 @@ def split_qkv(qkv: torch.Tensor, num_heads: int):
     contiguous v^T [B, H, D, N]: the layouts the per-head Q@K^T and per-row
     Attn@V engine calls read without further copies.  One engine pass
     (``scmp_split_qkv``), bit-identical to unbind + transpose."""
-    from . import _lib
     B, N, C3 = qkv.shape
     H = num_heads
     D = C3 // (3 * H)
@@ -387,7 +387,6 @@ class RotaryAxes(nn.Module):
     def __init__(self, dims, sizes, *, base: float = 10000.0, scales=None,
                  interleaved: bool = True, device=None):
         super().__init__()
-        from . import _lib
         dims, sizes = [int(d) for d in dims], [int(n) for n in sizes]
         scales = [1.0] * len(dims) if scales is None else [float(f) for f in scales]
         if not 1 <= len(dims) <= _lib.MAX_AXES or len(sizes) != len(dims) or len(
@@ -415,7 +414,6 @@ class RotaryAxes(nn.Module):
 
 def _rotary_launch(qkv, q, k, v, axes: RotaryAxes, table, pos, v_transposed: bool, inverse: bool):
     """One ``scmp_split_qkv_rotary`` call on contiguous storages."""
-    from . import _lib
     B, H, N, D = q.shape
     args = _lib.PACK_ROTARY.pack(
         _lib.ABI_VERSION, DTYPE[qkv.dtype], qkv.data_ptr(), q.data_ptr(), k.data_ptr(),
@@ -497,7 +495,7 @@ def split_qkv_rotary(qkv: torch.Tensor, num_heads: int, axes: RotaryAxes, pos: t
     if table.get_device() != index:
         raise ValueError(f"axes are on {table.device}, qkv on {qkv.device}")
     pos, transpose_v = pos.contiguous(), bool(transpose_v)
-    if has_tangent((qkv,)) or (torch.is_grad_enabled() and qkv.requires_grad):
+    if (torch.is_grad_enabled() and qkv.requires_grad) or has_tangent((qkv,)):
         # (a forward-mode tangent is refused there: the function has no jvp)
         return _SplitQkvRotary.apply(qkv, pos, table, axes, H, Hk, transpose_v)
     return _split_rotary(qkv.contiguous(), pos, table, axes, H, Hk, transpose_v)

@@ -46,9 +46,11 @@ def _check_exp(scale_exp: int) -> int:
 
 
 def _no_grad_wanted(name: str, *tensors) -> None:
-    recorded = torch.is_grad_enabled() and any([t is not None and t.requires_grad
-                                                for t in tensors])
-    if recorded or has_tangent(tensors):
+    wanted = has_tangent(tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            wanted = wanted or (t is not None and t.requires_grad)
+    if wanted:
         raise RuntimeError(f"{name} has no gradient; call it under torch.no_grad() or on "
                            "detached inputs")
 
@@ -208,7 +210,6 @@ def _check_input(x: torch.Tensor, name: str) -> int:
         raise RuntimeError(f"{name} runs on the CUDA engine only (no CPU path); got {x.device}")
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f"{name} needs a last dimension of at least 1, got {tuple(x.shape)}")
-    _no_grad_wanted(name, x)
     return code
 
 
@@ -219,6 +220,7 @@ def mx_quantize(x: torch.Tensor, fmt: str = "mxfp4", *, scale_exp: int = 0) -> M
     activations)."""
     _check_fmt(fmt)
     code = _check_input(x, "mx_quantize")
+    _no_grad_wanted("mx_quantize", x)
     out = mx_empty(x.shape, fmt, x.device, x.dtype, _check_exp(scale_exp))
     x, ld = _rows_of(x)
     call(_lib.load().scmp_mx_quantize, out.index, x.data_ptr(), code, out.rows, out.shape[-1], ld,
@@ -254,6 +256,7 @@ def mx_matmul(a: Union[torch.Tensor, MXTensor], b: MXTensor, *,
         raise ValueError(f"operands of different formats: {a.fmt} vs {b.fmt}")
     else:
         rows = a.rows
+    _no_grad_wanted("mx_matmul", a if plain else None, bias, out)
     shape = (*a.shape[:-1], N)
     given = out is not None
     if not given:
@@ -261,7 +264,6 @@ def mx_matmul(a: Union[torch.Tensor, MXTensor], b: MXTensor, *,
         out_code = dtype_code(dtype, "out")
         out = torch.empty(shape, dtype=dtype, device=b.device)
     else:
-        _no_grad_wanted("mx_matmul", out)
         if (tuple(out.shape) != shape or not out.is_contiguous() or out.get_device() != index
                 or out_dtype not in (None, out.dtype)):
             raise ValueError(f"out must be contiguous {shape} on {b.device} of out_dtype")
@@ -275,7 +277,6 @@ def mx_matmul(a: Union[torch.Tensor, MXTensor], b: MXTensor, *,
             raise ValueError(f"bias must be [{N}] on {b.device}, got {tuple(bias.shape)} on "
                              f"{bias.device}")
         bias_code = dtype_code(bias.dtype, "bias")
-        _no_grad_wanted("mx_matmul", bias)
         bias = bias if bias.is_contiguous() else bias.detach().contiguous()
         bias_ptr = bias.data_ptr()
     args = _lib.PACK_MX_MATMUL.pack(

@@ -29,6 +29,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from . import _lib
 from ._call import DTYPE, call, has_tangent, once_differentiable
 from .attention import GridRotary, make_sc_attention_forward
 from .head_aligned_comp import HeadAlignedSCLinear
@@ -102,7 +103,6 @@ def _check_glue(like: torch.Tensor, **tensors) -> None:
 def bias_gelu_(t: torch.Tensor, bias: torch.Tensor) -> torch.Tensor:
     """``t = gelu(t + bias)`` in place (fp32 CUDA ``[..., C]``, exact GELU):
     the bias add and torch's erf-form GELU in one pass, same bits."""
-    from . import _lib
     _check_glue(t, t=t, bias=bias)
     C = t.shape[-1]
     call(_lib.load().scmp_bias_gelu, t.get_device(), t.data_ptr(), bias.data_ptr(),
@@ -117,7 +117,6 @@ def scale_residual(x: torch.Tensor, y: torch.Tensor, gamma: torch.Tensor,
     contiguous and of one shape): a block's layer-scaled residual add, with an
     unfused bias and a compensation term, in one pass; each step rounded as
     the separate torch ops round it.  ``out`` may be ``x`` or ``y``."""
-    from . import _lib
     _check_glue(x, x=x, y=y, gamma=gamma, bias=bias, extra=extra, out=out)
     C = x.shape[-1]
     out = torch.empty_like(x) if out is None else out
@@ -184,7 +183,6 @@ def _dense(t: Optional[torch.Tensor]):
 def _norm_launch(x, y, weight, norm_bias, gamma, gate, post_weight, post_bias, kind, eps,
                  stats=None, h=None, mx=None):
     """One ``scmp_residual_norm`` call on contiguous tensors; returns r (None without y)."""
-    from . import _lib
     r = None if y is None else torch.empty_like(x)
     C = x.shape[-1]
     rows = x.numel() // C
@@ -203,7 +201,6 @@ def _norm_launch(x, y, weight, norm_bias, gamma, gate, post_weight, post_bias, k
 @functools.lru_cache(maxsize=256)
 def _norm_bwd_workspace(rows: int, C: int, rows_per_gate: int) -> int:
     """Bytes, a function of the sizes alone."""
-    from . import _lib
     return _lib.load().scmp_residual_norm_bwd_workspace(rows, C, rows_per_gate)
 
 
@@ -224,7 +221,6 @@ class _ResidualNorm(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, *grads):
-        from . import _lib
         r, y, stats, weight, norm_bias, gamma, gate, post_weight, post_bias = ctx.saved_tensors
         dr, dh = grads if y is not None else (None, grads[0])
         leaves = (r, y, weight, norm_bias, gamma, gate, post_weight, post_bias)
@@ -278,8 +274,8 @@ def residual_norm(x: torch.Tensor, y: Optional[torch.Tensor], weight: torch.Tens
     differ from ``F.layer_norm``'s in their order, so the bits may too."""
     _check_norm(x, y, weight, norm_bias, kind, eps, gamma, gate, post_weight, post_bias)
     leaves = (x, y, weight, norm_bias, gamma, gate, post_weight, post_bias)
-    if has_tangent(leaves) or (torch.is_grad_enabled() and any(
-            [t is not None and t.requires_grad for t in leaves])):
+    if (torch.is_grad_enabled() and any([t is not None and t.requires_grad for t in leaves])
+            ) or has_tangent(leaves):
         # (a forward-mode tangent is refused there: the function has no jvp)
         if quantize is not None:
             raise RuntimeError("residual_norm with quantize has no gradient; call it under "
