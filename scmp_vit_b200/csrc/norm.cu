@@ -397,9 +397,10 @@ __global__ void __launch_bounds__(256, E == 16 ? (V == 1 ? 2 : 3) : 1)
 // registers to the sums; with a post norm the parameters stay there too.  bf16
 // 16448 x 1024: 39 us (5.2 TB/s), in registers one row ahead 45; fp32 73 (5.5);
 // 16400 x 1408 with gates and a post norm bf16 76 us, 102 with registers and
-// single operations, instructions (two meetings of a row's warps) its bound; fp32
-// 105 (5.3 TB/s), 201.  Rows not in 16-byte pieces, and fp32 rows of over 4096
-// columns, whose ring would not fit, load as they go.
+// single operations, when instructions bounded it; now 52 % of cycles issue and the
+// two meetings of a row's warps are left; fp32 105 (5.3 TB/s), 201.  Rows not in
+// 16-byte pieces, and fp32 rows of over 4096 columns, whose ring would not fit, load
+// as they go.
 template <typename T, int V, int E, int kThreads> struct BwdCfg {
   static constexpr int kPieces = E * (int)sizeof(T) / 16;  // 16-byte pieces per array and lane
   static constexpr int kStages = V == 1 ? 0
