@@ -33,10 +33,15 @@ def call(fn, index: int, *args) -> None:
         _lib.check(status)
 
 
+def in_dual_level() -> bool:
+    """Whether forward-mode derivatives are being taken."""
+    return _forward_ad._current_level >= 0
+
+
 def has_tangent(tensors) -> bool:
     """Whether one of the tensors (or None) is a dual one of forward-mode
     differentiation, which ``requires_grad`` and the grad mode do not show."""
-    if _forward_ad._current_level < 0:  # outside every dual level: the usual case
+    if not in_dual_level():
         return False
     return any([t is not None and _forward_ad.unpack_dual(t).tangent is not None for t in tensors])
 

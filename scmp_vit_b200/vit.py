@@ -30,7 +30,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from . import _lib
-from ._call import DTYPE, call, has_tangent, once_differentiable
+from ._call import DTYPE, call, has_tangent, in_dual_level, once_differentiable
 from .attention import GridRotary, make_sc_attention_forward
 from .head_aligned_comp import HeadAlignedSCLinear
 from .mp import SeededRandomMPConfig, quantile_counts, set_current_block_idx
@@ -386,7 +386,7 @@ class Block(nn.Module):
                 and all(type(n) is nn.LayerNorm and n.weight is not None and n.bias is not None
                         and n.weight.dtype in (x.dtype, torch.float32) for n in norms)
                 and self.ls1.gamma.dtype == self.norm2.weight.dtype
-                and not _watched(*norms, self.ls1))
+                and not in_dual_level() and not _watched(*norms, self.ls1))
 
     def _forward_fused_norm(self, x):
         """The forward above with each norm in the pass of the residual add in
@@ -420,6 +420,7 @@ class Block(nn.Module):
     def _fused_glue_applies(self, x: torch.Tensor) -> bool:
         return (FUSED_GLUE and x.is_cuda and x.dtype == torch.float32 and x.is_contiguous()
                 and not torch.is_grad_enabled() and not torch.is_autocast_enabled("cuda")
+                and not in_dual_level()
                 and all(type(ls) is LayerScale and ls.gamma.dtype == torch.float32
                         for ls in (self.ls1, self.ls2)))
 

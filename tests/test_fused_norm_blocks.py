@@ -2,6 +2,7 @@
 is replaced by its formula and CPU tensors pass for CUDA ones."""
 import pytest
 import torch
+import torch.autograd.forward_ad as fwAD
 import torch.nn.functional as F
 
 from scmp_vit_b200 import vit
@@ -99,3 +100,28 @@ def test_codes_only_where_nobody_watches(calls, monkeypatch):
         del calls[:]
         blk(x)
         assert calls == ["mxfp4", "mxfp4"]
+
+
+@pytest.mark.parametrize("glue", [False, True])
+def test_forward_mode_takes_the_separate_modules(calls, monkeypatch, glue):
+    """The fused steps have no forward-mode derivative; a block under one, or with
+    a dual parameter, is differentiated as the modules are."""
+    monkeypatch.setattr(vit, "FUSED_GLUE", glue)
+    monkeypatch.setattr(vit, "FUSED_NORM", not glue)
+    monkeypatch.setattr(vit, "call", lambda *a: calls.append(a))
+    blk, x = block()
+    blk.attn = torch.nn.Linear(32, 32)
+    t = torch.randn(x.shape, generator=torch.Generator().manual_seed(2))
+    with torch.no_grad(), fwAD.dual_level():
+        got = fwAD.unpack_dual(blk(fwAD.make_dual(x, t))).tangent
+        scaled = torch.func.functional_call(
+            blk, {"ls1.gamma": fwAD.make_dual(blk.ls1.gamma.detach(), torch.ones(32))}, (x,))
+        assert fwAD.unpack_dual(scaled).tangent is not None
+    assert calls == []
+    e = 2.0 ** -10
+    with torch.no_grad():
+        monkeypatch.setattr(vit, "FUSED_GLUE", False)
+        monkeypatch.setattr(vit, "FUSED_NORM", False)
+        diff = (blk.double()(x.double() + e * t) - blk(x.double() - e * t)) / (2 * e)
+    # differences are off by e^2 times the third derivative, of the order of the values
+    assert (got - diff).abs().max() <= 100 * e * e * diff.abs().max()
