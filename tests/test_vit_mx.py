@@ -302,3 +302,18 @@ def test_modules_saved_before_positions_run():
     del attn.rope
     assert torch.equal(attn(x), want)
     assert torch.equal(pickle.loads(pickle.dumps(attn))(x), want)
+
+
+@pytest.mark.gpu
+def test_beside_sc_under_autocast(cuda_device):
+    """4-bit linears, SC attention and fp32 linears under autocast: every branch is
+    joined in the residual's type, as without the fused norms."""
+    m = small(cuda_device, rope=True)
+    vit.patch_vit(m, 8, ("qk", "av"))
+    x = torch.randn(2, 3, 56, 56, generator=torch.Generator().manual_seed(3)).to(cuda_device)
+    with torch.no_grad(), torch.autocast("cuda", torch.bfloat16):
+        plain = m(x)
+        vit.patch_vit_mx(m, ("mlp_fc1", "mlp_fc2"))
+        a, b = m(x), m(x)
+    assert plain.dtype == a.dtype and bool(plain.isfinite().all())
+    assert torch.equal(a, b) and bool(a.isfinite().all())
