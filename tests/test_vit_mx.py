@@ -4,6 +4,7 @@ against the same calls made one by one, and the fused norms' training step
 against 64 bits."""
 import copy
 import pickle
+import threading
 
 import pytest
 import torch
@@ -317,3 +318,36 @@ def test_beside_sc_under_autocast(cuda_device):
         a, b = m(x), m(x)
     assert plain.dtype == a.dtype and bool(plain.isfinite().all())
     assert torch.equal(a, b) and bool(a.isfinite().all())
+
+
+@pytest.mark.gpu
+def test_models_at_the_same_time(cuda_device):
+    """Threads with models, formats and streams of their own, whose products, norms
+    and splits share the GPU, give the bits of one thread."""
+    jobs = []
+    for i, (fmt, dtype) in enumerate((("mxfp4", torch.float32), ("nvfp4", torch.bfloat16),
+                                      ("mxfp4", torch.bfloat16))):
+        m = small(cuda_device, dtype, rope=True)
+        vit.patch_vit_mx(m, fmt=fmt)
+        x = torch.randn(8 * (i + 1), 3, 56, 56, device=cuda_device).to(dtype)
+        with torch.no_grad():
+            jobs.append((m, x, m(x)))
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(m, x, want):
+        try:
+            with torch.no_grad(), torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    got = m(x)
+                    torch.cuda.current_stream().synchronize()
+                    assert torch.equal(got, want)
+        except BaseException as e:  # seen by the test's own thread
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=job) for job in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
