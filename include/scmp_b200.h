@@ -259,6 +259,90 @@ SCMP_API int scmp_mx_matmul(const scmp_mx_matmul_args *args, void *stream);
 SCMP_API int scmp_mx_linear(const void *x, int x_dtype, int64_t ld,
                             const scmp_mx_matmul_args *args, void *stream);
 
+/* ---- 8-bit floating point with a scale per block of 128 (no reference
+ * counterpart), for training and inference.  An operand [rows, K] becomes e4m3
+ * codes with one scale 2^E per block: E = the smallest integer from -127 on under
+ * which the block's largest magnitude is at most 448 2^E, the codes x 2^-E rounded to
+ * nearest even.  Blocks are 128 consecutive elements of a row, or, `square`, 128 x
+ * 128 elements (a weight and its transpose then have the same codes).  A block that
+ * holds a NaN or an infinity stands for NaNs.  Buffers (16-byte aligned; sizes from
+ * scmp_fp8_data_size / scmp_fp8_scale_size, 0 on bad sizes):
+ *   data    [rows][ceil16(K)] bytes, 0 past K
+ *   scales  [ceil(rows / 128)][ceil(blocks / 4)][512] bytes e8m0, the scale of row r
+ *           and block b at (r % 32) * 16 + (r / 32 % 4) * 4 + b % 4 of its atom
+ *           (a square's in each of its rows); 0 past K and past the last row
+ * Asynchronous on `stream`. */
+SCMP_API size_t scmp_fp8_data_size(int64_t rows, int64_t K);
+SCMP_API size_t scmp_fp8_scale_size(int64_t rows, int64_t K);
+/* x: rows of K elements, `ld` elements apart.  data / scales (nullable pair): its
+ * codes; t_data / t_scales (nullable pair): those of its transpose [K, rows],
+ * quantised along the rows of x (or the same squares).  One launch. */
+typedef struct scmp_fp8_quantize_args {
+  int32_t abi_version;
+  int32_t dtype;
+  const void *x;
+  int64_t rows, K, ld;
+  int32_t square, reserved;
+  void *data, *scales, *t_data, *t_scales;
+} scmp_fp8_quantize_args;
+SCMP_API int scmp_fp8_quantize(const scmp_fp8_quantize_args *args, void *stream);
+/* out [rows][K]: the values that the codes stand for, rounded to `dtype`. */
+SCMP_API int scmp_fp8_dequantize(const void *data, const void *scales, int64_t rows, int64_t K,
+                                 void *out, int dtype, void *stream);
+/* out [M, N] = A B^T (+ bias [N]) for quantised A [M, K] and B [N, K]: fp32 sums,
+ * rounded once to out_dtype. */
+typedef struct scmp_fp8_matmul_args {
+  int32_t abi_version;
+  int32_t bias_dtype;
+  const void *a, *a_scales, *b, *b_scales;
+  int64_t M, N, K;
+  const void *bias; /* nullable [N] */
+  void *out;
+  int32_t out_dtype;
+  int32_t reserved;
+} scmp_fp8_matmul_args;
+SCMP_API int scmp_fp8_matmul(const scmp_fp8_matmul_args *args, void *stream);
+/* The same for an A that is not quantised yet: x, M rows of K elements of x_dtype,
+ * `ld` elements apart.  args->a and args->a_scales are buffers for its codes that
+ * the call may write; up to SCMP_FP8_THIN_ROWS rows of up to SCMP_FP8_THIN_K values
+ * need none (NULL) and then take one launch (with buffers the call chooses). */
+#define SCMP_FP8_THIN_ROWS 4
+#define SCMP_FP8_THIN_K 6144
+SCMP_API int scmp_fp8_linear(const void *x, int x_dtype, int64_t ld,
+                             const scmp_fp8_matmul_args *args, void *stream);
+/* A linear's training step: y = Q(x) Q(W)^T + bias with x [M, K] quantised along its
+ * rows and W [N, K] in squares; y is of x's type.  saved_x and saved_weight
+ * (nullable: not wanted) receive the transposes' codes for the backward pass,
+ * scmp_fp8_train_saved_size(M, K) and (N, K) bytes.  The workspace
+ * (scmp_fp8_train_workspace, backward 0) holds codes.  Three launches. */
+typedef struct scmp_fp8_train_args {
+  int32_t abi_version;
+  int32_t dtype, weight_dtype, bias_dtype;
+  const void *x, *weight, *bias; /* bias nullable [N] */
+  void *y;
+  void *saved_x, *saved_weight;
+  void *workspace;
+  size_t workspace_bytes;
+  int64_t M, N, K, ld, weight_ld;
+} scmp_fp8_train_args;
+SCMP_API size_t scmp_fp8_train_saved_size(int64_t rows, int64_t K);
+SCMP_API size_t scmp_fp8_train_workspace(int64_t M, int64_t N, int64_t K, int backward);
+SCMP_API int scmp_fp8_train_forward(const scmp_fp8_train_args *args, void *stream);
+/* Its gradients from dy [M, N] of y's type, rows `ld` apart (each nullable: not
+ * wanted): dx [M, K] = Q(dy) Q(W), dy quantised along its rows; dweight [N, K] =
+ * Q(dy)^T Q(x), both quantised along their columns; dbias [N] = the column sums of dy
+ * (not quantised).  Deterministic.  Up to four launches. */
+typedef struct scmp_fp8_train_bwd_args {
+  int32_t abi_version;
+  int32_t dtype, weight_dtype, bias_dtype;
+  const void *dy, *saved_x, *saved_weight;
+  void *dx, *dweight, *dbias;
+  void *workspace;
+  size_t workspace_bytes;
+  int64_t M, N, K, ld;
+} scmp_fp8_train_bwd_args;
+SCMP_API int scmp_fp8_train_backward(const scmp_fp8_train_bwd_args *args, void *stream);
+
 /* ---- Gated residual add with the norms around it (the `x + ls1(attn(...))`
  * and `norm2(x)` steps of the block forward of cls/sc_attention_patch.py:459-636,
  * with the gate and the norm behind the branch that other transformer blocks
@@ -370,6 +454,9 @@ SCMP_API int scmp_debug_hold_producers(int on);
  * buffers for codes; 0: tiles), plan[1] = activation rows per tile, plan[2] =
  * tiles.  Touches no device. */
 SCMP_API int scmp_debug_mx_plan(int64_t M, int64_t N, int64_t K, int pairs, int32_t *plan);
+
+/* The same for an 8-bit product. */
+SCMP_API int scmp_debug_fp8_plan(int64_t M, int64_t N, int64_t K, int pairs, int32_t *plan);
 
 /* Roofline probe (synchronous; allocates a small scratch buffer): runs a
  * register-only loop of one instruction class on every SM of the current

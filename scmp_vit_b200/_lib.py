@@ -26,6 +26,8 @@ ENGINE = {"auto": 0, "popc": 1, "tcgen05": 2}
 MX_FORMAT = {"mxfp4": 0, "nvfp4": 1}
 MX_BLOCK = {"mxfp4": 32, "nvfp4": 16}
 MX_THIN_ROWS, MX_THIN_K = 4, 6144  # SCMP_MX_THIN_ROWS, SCMP_MX_THIN_K
+FP8_BLOCK = 128
+FP8_THIN_ROWS, FP8_THIN_K = 4, 6144  # SCMP_FP8_THIN_ROWS, SCMP_FP8_THIN_K
 MAX_AXES = 4  # SCMP_MAX_AXES
 IO_A_BF16, IO_B_BF16, IO_OUT_BF16, IO_B_PACKED, IO_A_QUANT = 1, 2, 4, 8, 16  # io_flags bits
 
@@ -58,6 +60,17 @@ EXPORTED_SYMBOLS = (
     "scmp_residual_norm_bwd_workspace",
     "scmp_residual_norm_bwd",
     "scmp_split_qkv_rotary",
+    "scmp_fp8_data_size",
+    "scmp_fp8_scale_size",
+    "scmp_fp8_quantize",
+    "scmp_fp8_dequantize",
+    "scmp_fp8_matmul",
+    "scmp_fp8_linear",
+    "scmp_fp8_train_saved_size",
+    "scmp_fp8_train_workspace",
+    "scmp_fp8_train_forward",
+    "scmp_fp8_train_backward",
+    "scmp_debug_fp8_plan",
 )
 
 
@@ -145,12 +158,54 @@ class RotaryArgs(ctypes.Structure):
         ("reserved", ctypes.c_int32 * 3)]
 
 
+class Fp8QuantizeArgs(ctypes.Structure):
+    """Mirror of ``scmp_fp8_quantize_args``."""
+    _fields_ = [("abi_version", ctypes.c_int32), ("dtype", ctypes.c_int32),
+                ("x", ctypes.c_void_p)] + [
+        (n, ctypes.c_int64) for n in ("rows", "K", "ld")] + [
+        ("square", ctypes.c_int32), ("reserved", ctypes.c_int32)] + [
+        (n, ctypes.c_void_p) for n in ("data", "scales", "t_data", "t_scales")]
+
+
+class Fp8MatmulArgs(ctypes.Structure):
+    """Mirror of ``scmp_fp8_matmul_args``."""
+    _fields_ = [("abi_version", ctypes.c_int32), ("bias_dtype", ctypes.c_int32)] + [
+        (n, ctypes.c_void_p) for n in ("a", "a_scales", "b", "b_scales")] + [
+        (n, ctypes.c_int64) for n in ("M", "N", "K")] + [
+        ("bias", ctypes.c_void_p), ("out", ctypes.c_void_p), ("out_dtype", ctypes.c_int32),
+        ("reserved", ctypes.c_int32)]
+
+
+class Fp8TrainArgs(ctypes.Structure):
+    """Mirror of ``scmp_fp8_train_args``."""
+    _fields_ = [(n, ctypes.c_int32) for n in ("abi_version", "dtype", "weight_dtype",
+                                              "bias_dtype")] + [
+        (n, ctypes.c_void_p) for n in ("x", "weight", "bias", "y", "saved_x", "saved_weight",
+                                       "workspace")] + [
+        ("workspace_bytes", ctypes.c_size_t)] + [
+        (n, ctypes.c_int64) for n in ("M", "N", "K", "ld", "weight_ld")]
+
+
+class Fp8TrainBwdArgs(ctypes.Structure):
+    """Mirror of ``scmp_fp8_train_bwd_args``."""
+    _fields_ = [(n, ctypes.c_int32) for n in ("abi_version", "dtype", "weight_dtype",
+                                              "bias_dtype")] + [
+        (n, ctypes.c_void_p) for n in ("dy", "saved_x", "saved_weight", "dx", "dweight", "dbias",
+                                       "workspace")] + [
+        ("workspace_bytes", ctypes.c_size_t)] + [
+        (n, ctypes.c_int64) for n in ("M", "N", "K", "ld")]
+
+
 # The same layouts as packers: a call's arguments as bytes cost a quarter of a
 # Structure's (None is 0 there, so pointers come as integers).
 PACK_MX_MATMUL = struct.Struct("2i4P3q2i2P2i")
 PACK_NORM = struct.Struct("4i13P3qf3i")
 PACK_NORM_BWD = struct.Struct("4i19PN3q")
 PACK_ROTARY = struct.Struct("2i6P5q16i")
+PACK_FP8_QUANTIZE = struct.Struct("2iP3q2i4P")
+PACK_FP8_MATMUL = struct.Struct("2i4P3q2P2i")
+PACK_FP8_TRAIN = struct.Struct("4i7PN5q")
+PACK_FP8_TRAIN_BWD = struct.Struct("4i7PN4q")
 
 
 class EngineError(RuntimeError):
@@ -230,8 +285,18 @@ def load() -> ctypes.CDLL:
         # (their argument structs: byref of a Structure, or packed bytes)
         lib.scmp_mx_linear.argtypes = [ptr, i32, i64, ptr, ptr]
         lib.scmp_mx_linear.restype = ctypes.c_int
+        for name in ("scmp_fp8_data_size", "scmp_fp8_scale_size", "scmp_fp8_train_saved_size"):
+            getattr(lib, name).argtypes = [i64, i64]
+            getattr(lib, name).restype = ctypes.c_size_t
+        lib.scmp_fp8_train_workspace.argtypes = [i64, i64, i64, i32]
+        lib.scmp_fp8_train_workspace.restype = ctypes.c_size_t
+        lib.scmp_fp8_dequantize.argtypes = [ptr, ptr, i64, i64, ptr, i32, ptr]
+        lib.scmp_fp8_dequantize.restype = ctypes.c_int
+        lib.scmp_fp8_linear.argtypes = [ptr, i32, i64, ptr, ptr]
+        lib.scmp_fp8_linear.restype = ctypes.c_int
         for name in ("scmp_mx_matmul", "scmp_residual_norm", "scmp_residual_norm_bwd",
-                     "scmp_split_qkv_rotary"):
+                     "scmp_split_qkv_rotary", "scmp_fp8_quantize", "scmp_fp8_matmul",
+                     "scmp_fp8_train_forward", "scmp_fp8_train_backward"):
             getattr(lib, name).argtypes = [ptr, ptr]
             getattr(lib, name).restype = ctypes.c_int
         lib.scmp_residual_norm_bwd_workspace.argtypes = [i64, i64, i64]
@@ -240,8 +305,9 @@ def load() -> ctypes.CDLL:
         lib.scmp_debug_set_wait_limit.restype = ctypes.c_int
         lib.scmp_debug_hold_producers.argtypes = [ctypes.c_int]
         lib.scmp_debug_hold_producers.restype = ctypes.c_int
-        lib.scmp_debug_mx_plan.argtypes = [i64, i64, i64, i32, ctypes.POINTER(ctypes.c_int32)]
-        lib.scmp_debug_mx_plan.restype = ctypes.c_int
+        for name in ("scmp_debug_mx_plan", "scmp_debug_fp8_plan"):
+            getattr(lib, name).argtypes = [i64, i64, i64, i32, ctypes.POINTER(ctypes.c_int32)]
+            getattr(lib, name).restype = ctypes.c_int
         if lib.scmp_abi_version() != ABI_VERSION:
             raise RuntimeError(
                 f"engine ABI {lib.scmp_abi_version()} != expected {ABI_VERSION}")
@@ -279,6 +345,13 @@ def mx_plan(M: int, N: int, K: int, pairs: int = 74) -> tuple:
     product on ``pairs`` CTA pairs; for tests that mean a certain variant."""
     plan = (ctypes.c_int32 * 3)()
     check(load().scmp_debug_mx_plan(int(M), int(N), int(K), int(pairs), plan))
+    return bool(plan[0]), plan[1], plan[2]
+
+
+def fp8_plan(M: int, N: int, K: int, pairs: int = 74) -> tuple:
+    """``mx_plan`` of an 8-bit product."""
+    plan = (ctypes.c_int32 * 3)()
+    check(load().scmp_debug_fp8_plan(int(M), int(N), int(K), int(pairs), plan))
     return bool(plan[0]), plan[1], plan[2]
 
 

@@ -1,0 +1,434 @@
+// Quantisation to 8-bit floating point with a scale per block of 128, and back.
+//
+// Rows alone: a warp takes 512 or 1024 columns of a row, a half-warp a block.
+// With the transpose, or in squares: a block of threads takes a 128 x 128 tile,
+// which it reads once; its columns' codes leave through shared memory as rows of
+// the transpose.  Both are bound by HBM (read once, written once or twice).
+#include "chunk.cuh"
+#include "fp8_common.cuh"
+
+namespace scmp {
+namespace {
+
+constexpr int kThreads = 256;
+
+// ------------------------------------------------------------ rows alone
+
+// A unit is kChunks x 256 columns of one row, one warp; a block's largest magnitude
+// is a maximum over 16 lanes, and a lane writes the scales of four blocks at once.
+template <typename T, bool kVec, int kChunks>
+__global__ void __launch_bounds__(kThreads)
+    fp8_rows_kernel(const T *__restrict__ x, int64_t ld, const __grid_constant__ Fp8Layout l,
+                    const __grid_constant__ FastDiv per_row, uint32_t units,
+                    uint8_t *__restrict__ data, uint8_t *__restrict__ scales) {
+  __shared__ __align__(16) T deal[kVec ? 8 : kThreads * 8];
+  // (a product behind this launch may set up as SMs become free)
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int lane = threadIdx.x & 31;
+  T *const buf = deal + (kVec ? 0 : (threadIdx.x >> 5) * 256);
+  const uint32_t warps = gridDim.x * (kThreads / 32);
+  for (uint64_t u = (blockIdx.x * kThreads + threadIdx.x) >> 5; u < units; u += warps) {
+    const uint32_t r = per_row.quotient((uint32_t)u);
+    const uint32_t chunk0 = ((uint32_t)u - r * per_row.d) * kChunks;
+    const int64_t k = (int64_t)chunk0 * 256 + lane * 8;
+    const bool live = r < l.rows;
+    const T *row = x + r * ld;
+    uint8_t *codes_at = data + r * l.kp + k;
+    Chunk<T, kVec> e[kChunks];
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i) e[i].load(row, (int64_t)(chunk0 + i) * 256, lane, l.K, live);
+    uint32_t word[kChunks / 2];  // this half-warp's two bytes of each scale word
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i) {
+      e[i].deal(buf, lane);
+      float v[8];
+      unpack16<T>(e[i].u[0], v);
+      if (sizeof(T) == 4) unpack16<T>(e[i].u[sizeof(T) / 4], v + 4);
+      uint32_t amax = max_bits8<T>(e[i].u[0], v);
+#pragma unroll
+      for (int o = 1; o < 16; o <<= 1) amax = max(amax, __shfl_xor_sync(~0u, amax, o));
+      const uint32_t b = 2 * (chunk0 + i) + (lane >> 4);
+      const uint32_t scale = live && b < l.blocks ? fp8_scale(amax) : 0u;
+      const float inv = fp8_inverse(scale);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] *= inv;
+      const uint2 codes =
+          make_uint2(e4m3x4(v[0], v[1], v[2], v[3]), e4m3x4(v[4], v[5], v[6], v[7]));
+      if (live && k + i * 256 < l.kp) *reinterpret_cast<uint2 *>(codes_at + i * 256) = codes;
+      const uint32_t both = scale | __shfl_xor_sync(~0u, scale, 16) << 8;  // (right in lane 0)
+      if (i % 2 == 0)
+        word[i / 2] = both;
+      else
+        word[i / 2] |= both << 16;
+    }
+#pragma unroll
+    for (int i = 0; i < kChunks / 2; ++i) {
+      const int64_t g = chunk0 / 2 + i;
+      if (lane == 0 && g < l.groups)
+        *reinterpret_cast<uint32_t *>(scales + mx_scale_word(r, g, l.groups)) = word[i];
+    }
+  }
+}
+
+// -------------------------------------------- tiles: both orders, or squares
+
+struct TileArgs {
+  Fp8Layout rows, cols;  // of x and of its transpose
+  int64_t ld;
+  uint8_t *data, *scales, *t_data, *t_scales;  // either pair nullable
+  float *column_sums;                          // nullable
+  FastDiv tiles_c{1};
+};
+
+// Pitch of a transposed row in shared memory: 8-byte stores of a warp (16 columns
+// 8 apart, 2 row groups) and 16-byte loads of neighbours both go without conflicts
+// beyond their size.
+constexpr int kTilePitch = 128 + 16;
+
+// Thread t holds rows 8 (t / 16) + i and columns 8 (t % 16) + j of the tile, i, j < 8.
+template <typename T, bool kVec, bool kSquare, bool kSums>
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : 3)
+    fp8_tile_kernel(const T *__restrict__ x, const __grid_constant__ TileArgs a) {
+  __shared__ __align__(16) uint8_t turned[128 * kTilePitch];
+  __shared__ uint32_t warp_max[8][128];
+  __shared__ float warp_sum[kSums ? 8 : 1][128];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int rg = threadIdx.x >> 4, piece = threadIdx.x & 15;
+  const uint32_t tile_row = a.tiles_c.quotient(blockIdx.x);
+  const int64_t tile_r = tile_row, tile_c = blockIdx.x - tile_row * a.tiles_c.d;
+  const int64_t r0 = tile_r * 128 + rg * 8, c0 = tile_c * 128 + piece * 8;
+  const int64_t rows = a.rows.rows, K = a.rows.K;
+
+  // the tile, as loaded
+  constexpr int kWords = 2 * (int)sizeof(T);  // of eight elements
+  uint32_t e[8][kWords];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const T *p = x + (r0 + i) * a.ld + c0;
+    if (kVec && r0 + i < rows && c0 + 8 <= K) {
+#pragma unroll
+      for (int h = 0; h < kWords / 4; ++h)
+        *reinterpret_cast<uint4 *>(&e[i][4 * h]) = __ldg(reinterpret_cast<const uint4 *>(p) + h);
+    } else {
+      T v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        v[j] = r0 + i < rows && c0 + j < K ? p[j] : from_f32<T>(0.0f);
+      memcpy(e[i], v, sizeof(v));
+    }
+  }
+  const auto values = [&](int i, float *v) {
+    unpack16<T>(*reinterpret_cast<const uint4 *>(&e[i][0]), v);
+    if (sizeof(T) == 4) unpack16<T>(*reinterpret_cast<const uint4 *>(&e[i][kWords - 4]), v + 4);
+  };
+
+  // largest magnitudes: of the thread's part of each row and each column
+  uint32_t row_max[8], col_max[8];
+  float sums[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    col_max[j] = 0;
+    sums[j] = 0.0f;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    float v[8];
+    values(i, v);
+    row_max[i] = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t bits = __float_as_uint(v[j]) & 0x7FFFFFFFu;
+      row_max[i] = max(row_max[i], bits);
+      col_max[j] = max(col_max[j], bits);
+      if (kSums) sums[j] += v[j];
+    }
+  }
+  uint32_t row_scale[8], col_scale[8];
+  if (kSquare) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, row_max[i]);
+    m = __reduce_max_sync(~0u, m);
+    if (lane == 0) warp_max[0][warp] = m;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 8; ++w) m = max(m, warp_max[0][w]);
+    const uint32_t s = fp8_scale(m);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) row_scale[i] = col_scale[i] = s;
+  } else {
+    if (a.data) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+#pragma unroll
+        for (int o = 1; o < 16; o <<= 1)
+          row_max[i] = max(row_max[i], __shfl_xor_sync(~0u, row_max[i], o));
+        row_scale[i] = fp8_scale(row_max[i]);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      col_max[j] = max(col_max[j], __shfl_xor_sync(~0u, col_max[j], 16));
+      if (kSums) sums[j] += __shfl_xor_sync(~0u, sums[j], 16);
+    }
+    if (lane < 16) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        warp_max[warp][piece * 8 + j] = col_max[j];
+        if (kSums) warp_sum[warp][piece * 8 + j] = sums[j];
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int w = 0; w < 8; ++w) m = max(m, warp_max[w][piece * 8 + j]);
+      col_scale[j] = fp8_scale(m);
+    }
+    if (kSums && threadIdx.x < 128 && tile_c * 128 + threadIdx.x < K) {
+      float t = 0.0f;
+#pragma unroll
+      for (int w = 0; w < 8; ++w) t += warp_sum[w][threadIdx.x];
+      a.column_sums[tile_r * K + tile_c * 128 + threadIdx.x] = t;
+    }
+  }
+
+  if (a.data) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float v[8];
+      values(i, v);
+      const float inv = fp8_inverse(row_scale[i]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] *= inv;
+      if (r0 + i < rows && c0 < a.rows.kp)
+        *reinterpret_cast<uint2 *>(a.data + (r0 + i) * a.rows.kp + c0) =
+            make_uint2(e4m3x4(v[0], v[1], v[2], v[3]), e4m3x4(v[4], v[5], v[6], v[7]));
+      if (piece == 0)
+        a.scales[fp8_scale_at(r0 + i, tile_c, a.rows.groups)] =
+            (uint8_t)(r0 + i < rows ? row_scale[i] : 0u);
+    }
+    // the last tile of a row also fills its last scale word
+    if (tile_c == a.rows.blocks - 1 && threadIdx.x < 128)
+      for (int64_t b = a.rows.blocks; b < a.rows.groups * 4; ++b)
+        a.scales[fp8_scale_at(tile_r * 128 + threadIdx.x, b, a.rows.groups)] = 0;
+  }
+  if (a.t_data) {
+    // column j's eight rows are eight neighbouring bytes of the transpose
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+      float u[8], w[8];
+      const float iu = fp8_inverse(col_scale[j]), iw = fp8_inverse(col_scale[j + 1]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        float v[8];
+        values(i, v);
+        u[i] = v[j] * iu;
+        w[i] = v[j + 1] * iw;
+      }
+      uint8_t *at = turned + (piece * 8 + j) * kTilePitch + rg * 8;
+      *reinterpret_cast<uint2 *>(at) =
+          make_uint2(e4m3x4(u[0], u[1], u[2], u[3]), e4m3x4(u[4], u[5], u[6], u[7]));
+      *reinterpret_cast<uint2 *>(at + kTilePitch) =
+          make_uint2(e4m3x4(w[0], w[1], w[2], w[3]), e4m3x4(w[4], w[5], w[6], w[7]));
+    }
+    if (rg == 0) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        a.t_scales[fp8_scale_at(c0 + j, tile_r, a.cols.groups)] =
+            (uint8_t)(c0 + j < K ? col_scale[j] : 0u);
+    }
+    if (tile_r == a.cols.blocks - 1 && threadIdx.x < 128)
+      for (int64_t b = a.cols.blocks; b < a.cols.groups * 4; ++b)
+        a.t_scales[fp8_scale_at(tile_c * 128 + threadIdx.x, b, a.cols.groups)] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int q = threadIdx.x + i * kThreads, c = q >> 3, m = (q & 7) * 16;
+      if (tile_c * 128 + c < K && tile_r * 128 + m < a.cols.kp)
+        *reinterpret_cast<uint4 *>(a.t_data + (tile_c * 128 + c) * a.cols.kp + tile_r * 128 + m) =
+            *reinterpret_cast<const uint4 *>(turned + c * kTilePitch + m);
+    }
+  }
+}
+
+// Sums of columns over the tiles' parts, in a fixed order.
+template <typename T>
+__global__ void __launch_bounds__(128)
+    fp8_sum_kernel(const float *__restrict__ sums, int64_t parts, int64_t K, T *__restrict__ out) {
+  // 32 columns, four threads each: part p of a column goes to thread p % 4
+  __shared__ float part[4][32];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int64_t c = (int64_t)blockIdx.x * 32 + lane;
+  float t = 0.0f;
+  if (c < K) {
+#pragma unroll 8
+    for (int64_t p = w; p < parts; p += 4) t += sums[p * K + c];
+  }
+  part[w][lane] = t;
+  __syncthreads();
+  if (w == 0 && c < K)
+    out[c] = from_f32<T>((part[0][lane] + part[1][lane]) + (part[2][lane] + part[3][lane]));
+}
+
+// ------------------------------------------------------------------- back
+
+// Eight (16-bit) or four (fp32) consecutive elements per lane and chunk of 32 lanes.
+template <typename T, int kChunks, bool kVec>
+__global__ void __launch_bounds__(kThreads)
+    fp8_values_kernel(const uint8_t *__restrict__ data, const uint8_t *__restrict__ scales,
+                      const __grid_constant__ Fp8Layout l, const __grid_constant__ FastDiv per_row,
+                      uint32_t units, T *__restrict__ out) {
+  constexpr int V = kVec16<T>;
+  __shared__ __align__(16) T deal[kVec ? 8 : kThreads * V];
+  const int lane = threadIdx.x & 31;
+  T *const buf = deal + (kVec ? 0 : (threadIdx.x >> 5) * 32 * V);
+  const uint32_t warps = gridDim.x * (kThreads / 32);
+  for (uint64_t u = (blockIdx.x * kThreads + threadIdx.x) >> 5; u < units; u += warps) {
+    const uint32_t r = per_row.quotient((uint32_t)u);
+    const int64_t k = ((int64_t)((uint32_t)u - r * per_row.d) * kChunks * 32 + lane) * V;
+    uint32_t codes[kChunks][V / 4], sc[kChunks];
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i) {
+      const int64_t ki = k + i * 32 * V;
+      sc[i] = 0;
+#pragma unroll
+      for (int j = 0; j < V / 4; ++j) codes[i][j] = 0;
+      if (ki < l.kp) {
+#pragma unroll
+        for (int j = 0; j < V / 4; ++j)
+          codes[i][j] = __ldg(reinterpret_cast<const uint32_t *>(data + r * l.kp + ki) + j);
+        sc[i] = __ldg(scales + fp8_scale_at(r, ki / kFp8Block, l.groups));
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i) {
+      const int64_t ki = k + i * 32 * V;
+      if (ki - lane * V >= l.K) break;
+      const float s = fp8_value_of_scale(sc[i]);
+      float v[V];
+#pragma unroll
+      for (int j = 0; j < V / 4; ++j) e4m3_values(codes[i][j], v + 4 * j);
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[j] *= s;
+      T *dst = out + r * l.K + ki;
+      if (kVec) {
+        if (ki < l.K) *reinterpret_cast<uint4 *>(dst) = pack16<T>(v);
+      } else {
+        *reinterpret_cast<uint4 *>(buf + lane * V) = pack16<T>(v);
+        __syncwarp();
+        const int64_t c = ki - lane * V + lane;  // a neighbour per lane
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          if (c + 32 * j < l.K) out[r * l.K + c + 32 * j] = buf[lane + 32 * j];
+        __syncwarp();
+      }
+    }
+  }
+}
+
+unsigned grid_for(uint32_t units) {
+  const int64_t b = ((int64_t)units + kThreads / 32 - 1) / (kThreads / 32);
+  return (unsigned)(b < 148 * 16 ? b : 148 * 16);
+}
+
+// (rows and their units stay below 2^32 for what fits the memory)
+template <typename T, bool kVec, int kChunks>
+cudaError_t rows_k(const Fp8Quantize &q, const Fp8Layout &l, cudaStream_t s) {
+  const FastDiv per_row((uint32_t)((l.kp + 256 * kChunks - 1) / (256 * kChunks)));
+  const uint32_t units = (uint32_t)((l.rows + 127) / 128 * 128) * per_row.d;
+  fp8_rows_kernel<T, kVec, kChunks><<<grid_for(units), kThreads, 0, s>>>(
+      static_cast<const T *>(q.x), q.ld, l, per_row, units, q.data, q.scales);
+  return cudaGetLastError();
+}
+template <typename T, bool kVec>
+cudaError_t tiles_k(const Fp8Quantize &q, cudaStream_t s) {
+  TileArgs a;
+  a.rows = fp8_layout(q.rows, q.K);
+  a.cols = fp8_layout(q.K, q.rows);
+  a.ld = q.ld;
+  a.data = q.data;
+  a.scales = q.scales;
+  a.t_data = q.t_data;
+  a.t_scales = q.t_scales;
+  a.column_sums = q.column_sums;
+  a.tiles_c = FastDiv((uint32_t)a.rows.blocks);
+  const int64_t tiles = a.rows.blocks * a.cols.blocks;
+  if (tiles > INT32_MAX) return cudaErrorInvalidConfiguration;
+  const unsigned grid = (unsigned)tiles;
+  const T *x = static_cast<const T *>(q.x);
+  if (q.square)
+    fp8_tile_kernel<T, kVec, true, false><<<grid, kThreads, 0, s>>>(x, a);
+  else if (q.column_sums)
+    fp8_tile_kernel<T, kVec, false, true><<<grid, kThreads, 0, s>>>(x, a);
+  else
+    fp8_tile_kernel<T, kVec, false, false><<<grid, kThreads, 0, s>>>(x, a);
+  return cudaGetLastError();
+}
+template <typename T> cudaError_t quantize(const Fp8Quantize &q, cudaStream_t s) {
+  const bool vec =
+      (reinterpret_cast<uintptr_t>(q.x) & 15) == 0 && (q.ld * (int64_t)sizeof(T)) % 16 == 0;
+  if (q.square || q.t_data || q.column_sums)
+    return vec ? tiles_k<T, true>(q, s) : tiles_k<T, false>(q, s);
+  const Fp8Layout l = fp8_layout(q.rows, q.K);
+  // four chunks in flight per warp; two for short rows and where there would be
+  // fewer than eight warps on each of the 148 SMs
+  const bool few = l.kp <= 512 || l.rows * ((l.kp + 1023) / 1024) < 148 * 8;
+  if (few) return vec ? rows_k<T, true, 2>(q, l, s) : rows_k<T, false, 2>(q, l, s);
+  return vec ? rows_k<T, true, 4>(q, l, s) : rows_k<T, false, 4>(q, l, s);
+}
+
+template <typename T, int kChunks, bool kVec>
+cudaError_t values_v(const uint8_t *data, const uint8_t *scales, const Fp8Layout &l, void *out,
+                     cudaStream_t s) {
+  constexpr int V = kVec16<T>;
+  const FastDiv per_row((uint32_t)((l.kp + 32 * V * kChunks - 1) / (32 * V * kChunks)));
+  const uint32_t units = (uint32_t)l.rows * per_row.d;
+  fp8_values_kernel<T, kChunks, kVec><<<grid_for(units), kThreads, 0, s>>>(
+      data, scales, l, per_row, units, static_cast<T *>(out));
+  return cudaGetLastError();
+}
+template <typename T>
+cudaError_t values_t(const uint8_t *data, const uint8_t *scales, const Fp8Layout &l, void *out,
+                     cudaStream_t s) {
+  const int64_t chunk = 32 * kVec16<T>;
+  const bool one = l.kp <= 2 * chunk || l.rows * ((l.kp + 4 * chunk - 1) / (4 * chunk)) < 148 * 8;
+  const bool vec = l.K % kVec16<T> == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+  if (vec)
+    return one ? values_v<T, 1, true>(data, scales, l, out, s)
+               : values_v<T, 4, true>(data, scales, l, out, s);
+  return one ? values_v<T, 1, false>(data, scales, l, out, s)
+             : values_v<T, 4, false>(data, scales, l, out, s);
+}
+
+}  // namespace
+
+cudaError_t launch_fp8_quantize(const Fp8Quantize &q, cudaStream_t s) {
+  if (q.dtype == SCMP_F32) return quantize<float>(q, s);
+  if (q.dtype == SCMP_BF16) return quantize<__nv_bfloat16>(q, s);
+  return quantize<__half>(q, s);
+}
+
+cudaError_t launch_fp8_dequantize(const uint8_t *data, const uint8_t *scales, const Fp8Layout &l,
+                                  void *out, int dtype, cudaStream_t s) {
+  if (dtype == SCMP_F32) return values_t<float>(data, scales, l, out, s);
+  if (dtype == SCMP_BF16) return values_t<__nv_bfloat16>(data, scales, l, out, s);
+  return values_t<__half>(data, scales, l, out, s);
+}
+
+cudaError_t launch_fp8_sum_columns(const float *sums, int64_t parts, int64_t K, void *out,
+                                   int dtype, cudaStream_t s) {
+  const unsigned grid = (unsigned)((K + 31) / 32);
+  if (dtype == SCMP_F32)
+    fp8_sum_kernel<float><<<grid, 128, 0, s>>>(sums, parts, K, static_cast<float *>(out));
+  else if (dtype == SCMP_BF16)
+    fp8_sum_kernel<__nv_bfloat16>
+        <<<grid, 128, 0, s>>>(sums, parts, K, static_cast<__nv_bfloat16 *>(out));
+  else
+    fp8_sum_kernel<__half><<<grid, 128, 0, s>>>(sums, parts, K, static_cast<__half *>(out));
+  return cudaGetLastError();
+}
+
+}  // namespace scmp

@@ -2716,11 +2716,12 @@ cudaError_t launch_gemm_tc(const GemmProblem &P, int64_t m_rows, int64_t n_rows,
 }
 
 namespace {
-// Sets this file's word and the 4-bit product's.
-template <typename T, typename Mx>
-int set_device_word(const T &symbol, const T &value, Mx mx, const char *what) {
+// Sets this file's word and those of the 4-bit and 8-bit products.
+template <typename T, typename Set>
+int set_device_word(const T &symbol, const T &value, Set mx, Set fp8, const char *what) {
   cudaError_t e = cudaMemcpyToSymbol(symbol, &value, sizeof(T));
   if (e == cudaSuccess) e = mx(value);
+  if (e == cudaSuccess) e = fp8(value);
   if (e != cudaSuccess) {
     char buf[200];
     snprintf(buf, sizeof(buf), "%s: %s", what, cudaGetErrorString(e));
@@ -2737,7 +2738,8 @@ int debug_set_wait_limit(uint64_t ns) {
     return SCMP_EINVAL;
   }
   const unsigned long long v = ns;
-  return set_device_word(g_wait_limit_ns, v, mx_set_wait_limit, "setting the wait limit");
+  return set_device_word(g_wait_limit_ns, v, mx_set_wait_limit, fp8_set_wait_limit,
+                         "setting the wait limit");
 }
 
 cudaError_t launch_probe_mma_mxf4(int n, int iters, int blocks, unsigned int *error,
@@ -2766,7 +2768,8 @@ cudaError_t launch_probe_mma_mxf4(int n, int iters, int blocks, unsigned int *er
 
 int debug_hold_producers(int on) {
   const int v = on ? 1 : 0;
-  return set_device_word(g_hold_producers, v, mx_hold_producers, "setting the producer hold");
+  return set_device_word(g_hold_producers, v, mx_hold_producers, fp8_hold_producers,
+                         "setting the producer hold");
 }
 
 }  // namespace scmp
