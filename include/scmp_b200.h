@@ -267,7 +267,7 @@ SCMP_API int scmp_mx_linear(const void *x, int x_dtype, int64_t ld,
  * 128 elements (a weight and its transpose then have the same codes).  A block that
  * holds a NaN or an infinity stands for NaNs.  Buffers (16-byte aligned; sizes from
  * scmp_fp8_data_size / scmp_fp8_scale_size, 0 on bad sizes):
- *   data    [rows][ceil16(K)] bytes, 0 past K
+ *   data    [rows][ceil128(K)] bytes, 0 past K
  *   scales  [ceil(rows / 128)][ceil(blocks / 4)][512] bytes e8m0, the scale of row r
  *           and block b at (r % 32) * 16 + (r / 32 % 4) * 4 + b % 4 of its atom
  *           (a square's in each of its rows); 0 past K and past the last row
@@ -455,7 +455,9 @@ SCMP_API int scmp_debug_hold_producers(int on);
  * tiles.  Touches no device. */
 SCMP_API int scmp_debug_mx_plan(int64_t M, int64_t N, int64_t K, int pairs, int32_t *plan);
 
-/* The same for an 8-bit product. */
+/* The same for an 8-bit product: plan[0] as above, plan[1] and plan[2] = rows of A
+ * per tile, in turn (plan[2] 0: all alike), plan[3] = units of 256 rows of B by
+ * the sum of the two. */
 SCMP_API int scmp_debug_fp8_plan(int64_t M, int64_t N, int64_t K, int pairs, int32_t *plan);
 
 /* Roofline probe (synchronous; allocates a small scratch buffer): runs a

@@ -349,10 +349,11 @@ def mx_plan(M: int, N: int, K: int, pairs: int = 74) -> tuple:
 
 
 def fp8_plan(M: int, N: int, K: int, pairs: int = 74) -> tuple:
-    """``mx_plan`` of an 8-bit product."""
-    plan = (ctypes.c_int32 * 3)()
+    """(one launch of few rows?, the rows of A per tile in turn (second 0: all
+    alike), units) of an 8-bit product on ``pairs`` CTA pairs."""
+    plan = (ctypes.c_int32 * 4)()
     check(load().scmp_debug_fp8_plan(int(M), int(N), int(K), int(pairs), plan))
-    return bool(plan[0]), plan[1], plan[2]
+    return bool(plan[0]), (plan[1], plan[2]), plan[3]
 
 
 def probe_int_peak(kind: int) -> float:

@@ -24,14 +24,13 @@ int multiply(const Fp8Product &p, bool may_be_thin, cudaStream_t s) {
   cudaError_t e;
   if (may_be_thin && fp8_thin(p.M, p.N, p.K)) {
     e = launch_fp8_thin(p, nullptr, 0, 0, s);
+    if (e == cudaSuccess) add_launches(1);
   } else {
     unsigned int *err = device_error_word();
     if (!err) return fail(SCMP_ECUDA, "cannot resolve the engine error word");
     e = launch_fp8_matmul(p, err, s);
   }
-  if (e != cudaSuccess) return cuda_fail(e, "fp8_matmul launch");
-  add_launches(1);
-  return SCMP_OK;
+  return e == cudaSuccess ? SCMP_OK : cuda_fail(e, "fp8_matmul launch");
 }
 
 // A product's arguments; `codes`: A's buffers are needed.
@@ -346,10 +345,11 @@ int scmp_debug_fp8_plan(int64_t M, int64_t N, int64_t K, int pairs, int32_t *pla
   if ((rc = check_operand(M, K)) != SCMP_OK || (rc = check_operand(N, K)) != SCMP_OK) return rc;
   if (M == 0 || N == 0 || pairs < 1 || !plan)
     return fail(SCMP_EINVAL, "fp8_plan takes a product with outputs, pairs >= 1 and a plan");
-  const Fp8TilePlan tiles = fp8_tile_plan(M, N, pairs);
+  const Fp8TilePlan tiles = fp8_tile_plan(M, N, K, pairs);
   plan[0] = fp8_thin(M, N, K) ? 1 : 0;
-  plan[1] = tiles.nt;
-  plan[2] = (int32_t)tiles.tiles;
+  plan[1] = tiles.w[0];
+  plan[2] = tiles.w[1];
+  plan[3] = (int32_t)tiles.units;
   return SCMP_OK;
 }
 

@@ -9,8 +9,8 @@ namespace scmp {
 constexpr int kFp8Block = 128;
 
 // Layout of a quantised [rows, K] operand.
-//   data:   [rows][kp] bytes, kp = K rounded up to 16 (what a tensor map asks of
-//           its strides); codes past K are 0.
+//   data:   [rows][kp] bytes, kp = K rounded up to 128, so that a tensor map sees
+//           rows of whole blocks; codes past K are 0.
 //   scales: [ceil(rows / 128)][groups][512] bytes, groups = ceil(ceil(K / 128) / 4),
 //           the scale of row r, block b in the order of the 4-bit formats' atoms
 //           (mx_scale_word): e8m0, 2^(code - 127).  A 128 x 128 block's scale
@@ -25,8 +25,8 @@ inline Fp8Layout fp8_layout(int64_t rows, int64_t K) {
   Fp8Layout l;
   l.rows = rows;
   l.K = K;
-  l.kp = (K + 15) / 16 * 16;
   l.blocks = (K + kFp8Block - 1) / kFp8Block;
+  l.kp = l.blocks * kFp8Block;
   l.groups = (l.blocks + 3) / 4;
   return l;
 }
@@ -111,11 +111,14 @@ struct Fp8Product {
   void *out;  // [M, N] row-major
   int out_dtype;
 };
+// Rows of a per tile: w[0] throughout, or w[0] and w[1] in turn.  A unit is 256
+// rows of b by the widths' sum.
 struct Fp8TilePlan {
-  int nt;                   // rows of a per tile
-  uint32_t tiles_f, tiles;  // tiles of 256 rows of b; all tiles
+  int w[2];
+  uint32_t tiles_f, units;  // tiles of 256 rows of b; units, those fastest
 };
-Fp8TilePlan fp8_tile_plan(int64_t M, int64_t N, int pairs);
+Fp8TilePlan fp8_tile_plan(int64_t M, int64_t N, int64_t K, int pairs);
+// (counts its launches)
 cudaError_t launch_fp8_matmul(const Fp8Product &p, unsigned int *error, cudaStream_t s);
 // A few rows: x quantised in the same launch, or NULL with p.a's codes.
 bool fp8_thin_fits(int64_t M, int64_t K);

@@ -5,14 +5,20 @@
 //
 // tcgen05.mma kind::mxf8f6f4 on CTA pairs (cta_group::2), which takes one e8m0
 // scale per 32 values of K: the four MMAs of a block of 128 read the same byte of
-// the scale word, and an atom of scales serves four blocks, i.e. four stages.  The
-// accumulator is never scaled by the CUDA cores, so the epilogue runs once per
-// tile.  256 rows of B are the accumulator's lanes (128 per CTA), `nt` rows of A
-// its columns: a lane owns one output feature and 32 lanes store 32 neighbouring
-// outputs.  A stage is one block of K: both operands' codes (128-byte rows,
-// 128-byte swizzle) by TMA, completing on the even CTA's barrier; every fourth one
-// brings the scales too.  Two accumulators of up to 192 columns alternate, so the
-// epilogue of one tile runs under the MMAs of the next.
+// the scale word, and an atom of scales serves four blocks.  The accumulator is
+// never scaled by the CUDA cores, so the epilogue runs once per tile.  256 rows of
+// B are the accumulator's lanes (128 per CTA), rows of A its columns: a lane owns
+// one output feature and 32 lanes store 32 neighbouring outputs.  A stage is two
+// blocks of K: both operands' codes (128-byte rows, 128-byte swizzle) by TMA,
+// completing on the even CTA's barrier; every other one brings the scales too.  (With
+// one block per stage the issuing warp, some 450 cycles of waits and descriptors a
+// stage, held a block to 270 ns at every width; with two 240 at 192 columns, 183 at
+// 128, 160 at 64, at full clocks.)
+//
+// Tensor memory holds an accumulator of 256 columns, one of 192 and the scales, so
+// that the epilogue of a tile runs under the MMAs of the next, and a pair takes its
+// tiles 256 and 192 rows of A wide in turn: fewer bytes per product than 192 alone.
+// Where that leaves pairs idle, tiles have one width (plan_of).
 //
 // Warps: 0 loads, 1 issues MMAs (even CTA), 2 owns the tensor memory, 4-19 run
 // the epilogue.  Every wait is bounded: a wait that gives up raises the error
@@ -28,43 +34,63 @@ namespace {
 
 constexpr int kThreads = 640;
 constexpr int kEpilogueWarps = 16;
-constexpr int kMaxNt = 192;  // rows of A per tile
-constexpr uint32_t kAccCols = kMaxNt;
-constexpr uint32_t kScaleCol = 2 * kAccCols;
+constexpr int kWide = 256, kNarrow = 192;  // rows of A: the accumulators' columns
+constexpr int kPerStage = 2;               // blocks of K per stage
+constexpr int kStages = 3;
+constexpr uint32_t kScaleCol = kWide + kNarrow;
+constexpr uint32_t kScaleCols = 4 + 12;  // of an atom of B, three of A
 
-template <typename T> struct Fp8Cfg {
-  static constexpr uint32_t kW = 128 * kRowBytes;         // a CTA's rows of B
-  static constexpr uint32_t kX = kMaxNt / 2 * kRowBytes;  // a CTA's rows of A
-  static constexpr uint32_t kStage = kW + kX;
-  static constexpr uint32_t kScales = 3 * 512;  // one row group of B, up to two of A
-  static constexpr uint32_t kScaleCols = 4 + 8;
-  // 16-bit outputs are stored through pieces of 32 rows x 32 features, one per
-  // epilogue warp
-  static constexpr uint32_t kPiece = sizeof(T) == 2 ? 2048 : 0;
-  static constexpr int kStages = 6;
-  static constexpr uint32_t kScalesAt = kStages * kStage;
-  static constexpr uint32_t kOutAt = kScalesAt + kStages * kScales;
-  static constexpr uint32_t kBarsAt = kOutAt + kEpilogueWarps * kPiece;
-  static constexpr size_t kSmem = (size_t)kBarsAt + 1024 /*align*/ + 256;
-  static_assert(kStage % 1024 == 0, "swizzle atoms stay aligned");
-  static_assert(kScaleCol + 2 * kScaleCols <= 512, "two sets of scales behind the accumulators");
-  static_assert(kSmem <= 227 * 1024, "shared memory per CTA");
-};
+constexpr uint32_t kW = 128 * kRowBytes;        // a CTA's rows of B, one block of K
+constexpr uint32_t kX = kWide / 2 * kRowBytes;  // a CTA's rows of A, at most
+constexpr uint32_t kStage = kPerStage * (kW + kX);
+constexpr uint32_t kScales = 4 * 512;  // one row group of B, up to three of A
+constexpr uint32_t kScalesAt = kStages * kStage;
+// 16-bit outputs are stored through pieces of 16 rows x 32 features, one per epilogue
+// warp (of 32 rows they do not fit; stored from registers instead, two rows of 64
+// bytes at a time, products of short K take 3% longer).
+constexpr int kPieceRows = 16;
+constexpr uint32_t kPiece = kPieceRows * 64;
+constexpr uint32_t kOutAt = kScalesAt + kStages * kScales;
+constexpr uint32_t kBarsAt = kOutAt + kEpilogueWarps * kPiece;
+constexpr size_t kSmem = (size_t)kBarsAt + 1024 /*align*/ + 256;
+static_assert(kStage % 1024 == 0, "swizzle atoms stay aligned");
+static_assert(kScaleCol + 2 * kScaleCols <= 512, "two sets of scales behind the accumulators");
+static_assert(kSmem <= 227 * 1024, "shared memory per CTA");
 
 struct Fp8Tiles {
   Fp8Product p;
-  int nt;                   // rows of A per tile (16, 32, 64, 128 or 192)
-  int xrows;                // row groups (of 128) that their scales touch: 1 or 2
-  uint32_t tiles_f, tiles;  // tiles of 256 rows of B; all tiles, those fastest
-  int steps;                // stages per tile
-  int mmas;                 // 32-value MMAs per tile
-  bool tma_out;             // 16-bit rows of whole 16-byte pieces: stored by TMA
-  bool words;               // else: 16-bit outputs are stored two features at a time
+  Fp8TilePlan plan;
+  int xrows;               // row groups (of 128) that a tile's scales of A touch, at most
+  int block0, blocks;      // blocks of K of this launch
+  int steps;               // stages per tile
+  bool tma_out;            // 16-bit rows of whole 16-byte pieces: stored by TMA
+  bool words;              // else: 16-bit outputs are stored two features at a time
+  bool add;                // fp32 outputs: added to what is there
   unsigned int *error;
 };
 
+// The tiles of a pair in order: f(first row of B, first row of A, which width,
+// accumulator) until it is false.
+template <typename F>
+__device__ __forceinline__ void for_tiles(const Fp8Tiles &t, F &&f) {
+  const uint32_t clusters = gridDim.x >> 1;
+  uint32_t it = 0;
+  for (uint32_t u = blockIdx.x >> 1; u < t.plan.units; u += clusters) {
+    const uint32_t q = u / t.plan.tiles_f;
+    const int f0 = (int)(u - q * t.plan.tiles_f) * 256;
+    int64_t n0 = (int64_t)q * (t.plan.w[0] + t.plan.w[1]);
+    for (int sub = 0; sub < 2; ++sub) {
+      if (t.plan.w[sub] == 0 || n0 >= t.p.M) break;
+      const uint32_t buf = t.plan.w[1] ? (uint32_t)sub : t.plan.w[0] > kNarrow ? 0u : it & 1u;
+      ++it;
+      if (!f(f0, (int)n0, sub, buf)) return;
+      n0 += t.plan.w[0];
+    }
+  }
+}
+
+// (of an MMA n columns wide; A and B e4m3: 0)
 __host__ __device__ constexpr uint32_t idesc(int n) {
-  // (A and B e4m3: 0)
   return ((uint32_t)(n >> 3) << 17)         // N
          | (1u << 23)                       // scales e8m0
          | ((uint32_t)(256 >> 4) << 24);    // M over the pair
@@ -85,30 +111,33 @@ __device__ __forceinline__ void mma_pair(uint32_t d, uint64_t a, uint64_t b, uin
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
     fp8_pair_kernel(const __grid_constant__ Fp8Tiles t, const __grid_constant__ CUtensorMap wmap,
-                   const __grid_constant__ CUtensorMap xmap,
-                   const __grid_constant__ CUtensorMap wsmap,
-                   const __grid_constant__ CUtensorMap xsmap,
-                   const __grid_constant__ CUtensorMap omap) {
-  using Cfg = Fp8Cfg<T>;
+                    const __grid_constant__ CUtensorMap xmap0,
+                    const __grid_constant__ CUtensorMap xmap1,
+                    const __grid_constant__ CUtensorMap wsmap,
+                    const __grid_constant__ CUtensorMap xsmap,
+                    const __grid_constant__ CUtensorMap omap) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char *smem = reinterpret_cast<unsigned char *>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t *full = reinterpret_cast<uint64_t *>(smem + Cfg::kBarsAt);
-  uint64_t *empty = full + Cfg::kStages;
-  uint64_t *tfull = empty + Cfg::kStages, *tempty = tfull + 2, *drain = tempty + 2;
+  uint64_t *full = reinterpret_cast<uint64_t *>(smem + kBarsAt);
+  uint64_t *empty = full + kStages;
+  uint64_t *tfull = empty + kStages, *tempty = tfull + 2, *drain = tempty + 2;
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
   volatile int *abort = reinterpret_cast<volatile int *>(tmem_slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
+  // one accumulator: all epilogue warps read it
+  const bool alone = t.plan.w[1] == 0 && t.plan.w[0] > kNarrow;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < Cfg::kStages; ++s) {
+    for (int s = 0; s < kStages; ++s) {
       mbar_init(&full[s], 1);   // even CTA: its loader, and both loaders' bytes
       mbar_init(&empty[s], 1);  // commit of the MMAs that read the stage
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&tfull[i], 1);
-      mbar_init(&tempty[i], kEpilogueWarps);  // even CTA: the accumulator's readers in both CTAs
+      // even CTA: the accumulator's readers in both CTAs
+      mbar_init(&tempty[i], alone ? 2 * kEpilogueWarps : kEpilogueWarps);
     }
     mbar_init(drain, 1);
     *abort = 0;
@@ -128,53 +157,55 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
   // All of the above may run while the kernel in front of this one in the stream
   // ends; global memory is touched from here on only.
   grid_dependency_wait();
-  const uint32_t cluster = blockIdx.x >> 1, clusters = gridDim.x >> 1;
   const uint32_t smem0 = smem_u32(smem);
 
   if (warp == 0) {
     // -------------------------------------------------------------- loader
     // (the whole warp walks the stages, one elected lane issues: see the MMA warp)
     const uint32_t bars = mapa_shared(smem_u32(full), 0);
-    // bytes of a stage over both CTAs, without and with scales; what lies past an
-    // operand's end arrives as zeros and counts too
-    const uint32_t bytes = 2 * (Cfg::kW + (uint32_t)t.nt / 2 * kRowBytes);
     const uint32_t scale_bytes = 2 * (1u + (uint32_t)t.xrows) * 512;
     int stage = 0;
     uint32_t phase = 0, issued = 0;
     bool ok = __all_sync(~0u, producers_released(abort));
-    for (uint32_t tile = cluster; tile < t.tiles && ok; tile += clusters) {
-      const int f0 = (int)(tile % t.tiles_f * 256 + rank * 128);
-      const int n0 = (int)(tile / t.tiles_f) * t.nt, half = n0 + (int)rank * (t.nt / 2);
+    if (ok) for_tiles(t, [&](int f0, int n0, int sub, uint32_t) {
+      const int w = t.plan.w[sub], half = n0 + (int)rank * (w / 2);
+      const CUtensorMap *xmap = sub ? &xmap1 : &xmap0;
+      // bytes of a stage over both CTAs; what lies past an operand's end arrives as
+      // zeros and counts too
+      const uint32_t bytes = 2 * kPerStage * (kW + (uint32_t)w / 2 * kRowBytes);
+      f0 += (int)rank * 128;
       for (int kb = 0; kb < t.steps; ++kb) {
         ok = warp_wait_cl(&empty[stage], phase ^ 1, abort);
-        if (!ok) break;
-        const uint32_t at = smem0 + stage * Cfg::kStage, bar = bars + 8u * (uint32_t)stage;
+        if (!ok) return false;
+        const uint32_t at = smem0 + stage * kStage, bar = bars + 8u * (uint32_t)stage;
+        const int block = t.block0 + kb * kPerStage;
         if (elect_one()) {
-          const bool first = (kb & 3) == 0;  // the block whose stage brings four blocks' scales
+          const bool first = kb % (4 / kPerStage) == 0;  // brings four blocks' scales
           if (rank == 0) mbar_arrive_expect_tx(&full[stage], first ? bytes + scale_bytes : bytes);
-          tma_pair_2d(at, &wmap, kb * (int)kRowBytes, f0, bar);
-          tma_pair_2d(at + Cfg::kW, &xmap, kb * (int)kRowBytes, half, bar);
+          tma_pair_3d(at, &wmap, 0, f0, block, bar);
+          tma_pair_3d(at + kPerStage * kW, xmap, 0, half, block, bar);
           if (first) {
-            const uint32_t sat = smem0 + Cfg::kScalesAt + stage * Cfg::kScales;
-            tma_pair_3d(sat, &wsmap, 0, kb >> 2, f0 >> 7, bar);
-            tma_pair_3d(sat + 512, &xsmap, 0, kb >> 2, n0 >> 7, bar);
+            const uint32_t sat = smem0 + kScalesAt + stage * kScales;
+            tma_pair_3d(sat, &wsmap, 0, block >> 2, f0 >> 7, bar);
+            tma_pair_3d(sat + 512, &xsmap, 0, block >> 2, n0 >> 7, bar);
           }
         }
         __syncwarp();
         ++issued;
-        if (++stage == Cfg::kStages) {
+        if (++stage == kStages) {
           stage = 0;
           phase ^= 1;
         }
       }
-    }
+      return true;
+    });
     // No CTA ends with copies in flight.  The even CTA sees every stage's bytes
     // arrive, and the odd one leaves after it (cluster barrier below).  When a
     // wait gave up, the odd CTA may have started copies for a stage that the
     // even one did not: it lets them land first (they take microseconds).
     if (rank == 0) {
-      for (uint32_t i = issued > Cfg::kStages ? issued - Cfg::kStages : 0; i < issued; ++i)
-        mbar_wait_own(&full[i % Cfg::kStages], i / Cfg::kStages & 1);
+      for (uint32_t i = issued > kStages ? issued - kStages : 0; i < issued; ++i)
+        mbar_wait_own(&full[i % kStages], i / kStages & 1);
     } else if (!ok) {
       const unsigned long long t0 = now_ns();
       while (now_ns() - t0 < 2000000ull) {
@@ -185,125 +216,127 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
     // the whole warp walks the stages and one elected lane issues: loop state
     // and descriptors stay warp-uniform, and so does what the instructions read
     int stage = 0;
-    uint32_t phase = 0, it = 0, set = 0;
+    uint32_t phase = 0, set = 0, uses[2] = {0, 0};
     const uint64_t desc0 = smem_desc_sw128(smem0);
-    const uint64_t sdesc0 = scale_desc(smem0 + Cfg::kScalesAt);
-    const uint32_t id0 = idesc(t.nt);
-    const bool two = t.xrows > 1;
-    bool ok = true;
-    for (uint32_t tile = cluster; tile < t.tiles && ok; tile += clusters, ++it) {
-      const uint32_t n0 = (uint32_t)(tile / t.tiles_f) * (uint32_t)t.nt;
-      const uint32_t buf = it & 1;
-      if (it >= 2) ok = warp_wait_cl(&tempty[buf], ((it >> 1) - 1) & 1, abort);
-      if (!ok) break;
+    const uint64_t sdesc0 = scale_desc(smem0 + kScalesAt);
+    for_tiles(t, [&](int, int n0, int sub, uint32_t buf) {
+      const uint32_t use = buf ? uses[1]++ : uses[0]++;
+      if (use > 0 && !warp_wait_cl(&tempty[buf], (use - 1) & 1, abort)) return false;
       tc_fence_after();
-      const uint32_t acc = tmem + buf * kAccCols;
-      int left = t.mmas;
-      for (int kb = 0; kb < t.steps; ++kb, left -= 4) {
-        ok = warp_wait_cl(&full[stage], phase, abort);
-        if (!ok) break;
+      const uint32_t acc = tmem + buf * kWide;
+      const uint32_t w = (uint32_t)t.plan.w[sub], id0 = idesc((int)w);
+      const uint32_t xblock = w / 2 * kRowBytes, offset = ((uint32_t)n0 & 127u) / 32;
+      for (int kb = 0; kb < t.steps; ++kb) {
+        if (!warp_wait_cl(&full[stage], phase, abort)) return false;
         tc_fence_after();
         // consecutive atoms of scales use two sets of columns in turn
-        if ((kb & 3) == 0) set ^= 1;
-        const uint32_t sw = tmem + kScaleCol + set * Cfg::kScaleCols, sx = sw + 4;
-        const uint64_t d = desc_add(desc0, (uint32_t)stage * Cfg::kStage);
-        const uint32_t sxo = sx + (n0 & 127u) / 32;
-        const uint32_t id = idesc_byte(id0, (uint32_t)kb & 3u);
+        const bool first = kb % (4 / kPerStage) == 0;
+        if (first) set ^= 1;
+        const uint32_t sw = tmem + kScaleCol + set * kScaleCols, sx = sw + 4;
+        const uint64_t d = desc_add(desc0, (uint32_t)stage * kStage);
+        const uint64_t dx = desc_add(d, kPerStage * kW);
         if (elect_one()) {
-          if ((kb & 3) == 0) {
-            const uint64_t ds = desc_add(sdesc0, (uint32_t)stage * Cfg::kScales);
+          if (first) {
+            const uint64_t ds = desc_add(sdesc0, (uint32_t)stage * kScales);
             copy_scales(sw, ds);
-            copy_scales(sx, desc_add(ds, 512));
-            if (two) copy_scales(sx + 4, desc_add(ds, 1024));
+            for (int i = 0; i < t.xrows; ++i)
+              copy_scales(sx + 4 * i, desc_add(ds, 512 + 512 * i));
           }
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk) {
-            if (kk >= left) break;  // past K
-            mma_pair(acc, desc_add(d, kk * 32), desc_add(d, Cfg::kW + kk * 32), id, sw, sxo,
-                     (kb > 0 || kk > 0) ? 1u : 0u);
+          for (int b = 0; b < kPerStage; ++b) {
+            if (b > 0 && kb * kPerStage + b >= t.blocks) break;  // past K
+            const uint32_t id = idesc_byte(id0, (uint32_t)(kb * kPerStage + b) & 3u);
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              mma_pair(acc, desc_add(d, b * kW + kk * 32), desc_add(dx, b * xblock + kk * 32), id,
+                       sw, sx + offset, (kb > 0 || b > 0 || kk > 0) ? 1u : 0u);
           }
           tc_commit_pair_both(&empty[stage]);
           if (kb == t.steps - 1) tc_commit_pair_both(&tfull[buf]);
         }
         __syncwarp();
-        if (++stage == Cfg::kStages) {
+        if (++stage == kStages) {
           stage = 0;
           phase ^= 1;
         }
       }
-    }
+      return true;
+    });
     if (elect_one()) {
       tc_commit_pair_local(drain);
       mbar_wait_own_cl(drain, 0);
     }
   } else if (warp >= 4) {
     // ------------------------------------------------------------ epilogue
-    // Eight warps per accumulator (two per 32 lanes, 32-column pieces in turn), so
+    // Eight warps per accumulator (two per 32 lanes, pieces of 32 columns in turn), so
     // that the tiles of the two accumulators are read and stored side by side.  An
     // accumulator's next tile waits for the last load from it: two pieces are
-    // loaded at once, one is stored to make room, the third is loaded and the
-    // accumulator handed back before the others are stored (after two stores: 42
-    // us for fc1 of 64 images in bf16, now 41).
-    const uint32_t buf = (uint32_t)(warp - 4) >> 3;
-    const uint32_t acc = tmem + ((uint32_t)((warp & 3) * 32) << 16) + buf * kAccCols;
-    const uint32_t to = mapa_shared(smem_u32(&tempty[buf]), 0);
-    const int first = ((warp - 4) >> 2 & 1) * 32;
+    // loaded at once and stored while the next are on their way.
+    const uint32_t mine = (uint32_t)(warp - 4) >> 3, half = (uint32_t)(warp - 4) >> 2 & 1;
+    const int first = (int)(alone ? 2 * mine + half : half) * 32, stride = alone ? 128 : 64;
     uint32_t turn = 0;
-    for (uint32_t tile = cluster + buf * clusters; tile < t.tiles; tile += 2 * clusters, ++turn) {
-      const int64_t f = (int64_t)(tile % t.tiles_f) * 256 + rank * 128 + (warp & 3) * 32 + lane;
-      const int64_t n0 = (int64_t)(tile / t.tiles_f) * t.nt;
-      const float bias = t.p.bias && f < t.p.N ? load_as_f32(t.p.bias, t.p.bias_dtype, f) : 0.0f;
+    for_tiles(t, [&](int f0, int n0, int sub, uint32_t buf) {
+      if (!alone && buf != mine) return true;
+      f0 += (int)rank * 128 + (warp & 3) * 32;
+      const int64_t f = f0 + lane;
+      const float bias =
+          t.p.bias && f < t.p.N ? load_as_f32(t.p.bias, t.p.bias_dtype, f) : 0.0f;
       const int64_t left = t.p.M - n0;
-      const int rows = left < t.nt ? (int)left : t.nt;
-      const int f0 = (int)(f - lane);
-      if (!warp_wait_cl(&tfull[buf], turn & 1, abort)) break;
+      const int w = t.plan.w[sub], rows = left < w ? (int)left : w;
+      if (!warp_wait_cl(&tfull[buf], turn++ & 1, abort)) return false;
       tc_fence_after();
+      const uint32_t acc = tmem + ((uint32_t)((warp & 3) * 32) << 16) + buf * kWide;
       const auto hand_back = [&] {
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) arrive_remote(to);
+        if (lane == 0) arrive_remote(mapa_shared(smem_u32(&tempty[buf]), 0));
       };
-      const auto store = [&](int j0, const uint32_t (&v)[32]) {
+      const auto store = [&](int j0, uint32_t (&v)[32]) {
         if (j0 >= rows || f0 >= t.p.N) return;
-        if (sizeof(T) == 2 && t.tma_out) {
-          // through shared memory; a TMA store clips what lies past M and N
-          asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-          __syncwarp();
-          uint16_t *piece =
-              reinterpret_cast<uint16_t *>(smem + Cfg::kOutAt + (warp - 4) * Cfg::kPiece);
+        if constexpr (sizeof(T) == 4) if (t.add && f < t.p.N) {
+          const float *out = static_cast<const float *>(t.p.out) + (int64_t)(n0 + j0) * t.p.N + f;
 #pragma unroll
-          for (int j = 0; j < 32; j += 2) {
-            uint32_t two = 0;
-            if constexpr (sizeof(T) == 2)
-              two = pack2<T>(__uint_as_float(v[j]) + bias,
-                             __uint_as_float(v[j + 1]) + bias);
-            piece[j * 32 + lane] = (uint16_t)two;
-            piece[(j + 1) * 32 + lane] = (uint16_t)(two >> 16);
-          }
-          fence_async_smem();
-          __syncwarp();
-          if (lane == 0) tma_store_2d(&omap, f0, (int)n0 + j0, smem_u32(piece));
-        } else if (j0 + 32 <= rows) {
-          store_chunk<T, true>(t.p, 1.0f, t.words, v, bias, n0 + j0, f, 32, lane);
-        } else {
-          store_chunk<T, false>(t.p, 1.0f, t.words, v, bias, n0 + j0, f, rows - j0, lane);
+          for (int j = 0; j < 32; ++j)
+            if (j0 + j < rows) v[j] = __float_as_uint(__uint_as_float(v[j]) + out[j * t.p.N]);
         }
+        if constexpr (sizeof(T) == 2) if (t.tma_out) {
+          // (a TMA store clips what lies past M and N)
+          uint16_t *piece = reinterpret_cast<uint16_t *>(smem + kOutAt + (warp - 4) * kPiece);
+#pragma unroll
+          for (int h = 0; h < 32; h += kPieceRows) {
+            asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < kPieceRows; j += 2) {
+              const uint32_t two = pack2<T>(__uint_as_float(v[h + j]) + bias,
+                                            __uint_as_float(v[h + j + 1]) + bias);
+              piece[j * 32 + lane] = (uint16_t)two;
+              piece[(j + 1) * 32 + lane] = (uint16_t)(two >> 16);
+            }
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0 && j0 + h < rows) tma_store_2d(&omap, f0, n0 + j0 + h, smem_u32(piece));
+          }
+          return;
+        }
+        if (j0 + 32 <= rows)
+          store_chunk<T, true>(t.p, 1.0f, t.words, v, bias, n0 + j0, f, 32, lane);
+        else
+          store_chunk<T, false>(t.p, 1.0f, t.words, v, bias, n0 + j0, f, rows - j0, lane);
       };
-      const bool third = first + 128 < t.nt;
       uint32_t v[2][32];
-      if (first < t.nt) tmem_ld32(acc + first, v[0]);
-      if (first + 64 < t.nt) tmem_ld32(acc + first + 64, v[1]);
-      asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-      if (!third) hand_back();
-      store(first, v[0]);
-      if (third) {
-        tmem_ld32(acc + first + 128, v[0]);
+      if (first >= w) hand_back();
+#pragma unroll 1
+      for (int j0 = first; j0 < w; j0 += 2 * stride) {
+        tmem_ld32(acc + j0, v[0]);
+        if (j0 + stride < w) tmem_ld32(acc + j0 + stride, v[1]);
         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-        hand_back();
+        if (j0 + 2 * stride >= w) hand_back();
+        store(j0, v[0]);
+        if (j0 + stride < w) store(j0 + stride, v[1]);
       }
-      store(first + 64, v[1]);
-      if (third) store(first + 128, v[0]);
-    }
+      return true;
+    });
     asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
   __syncwarp();
@@ -317,36 +350,74 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
   if (threadIdx.x == 0 && *abort) atomicOr(t.error, 1u);
 }
 
-// Activation rows per tile: one tile for up to 32 rows; else the width among
-// 64, 128 and 192 whose rounds of tiles over the CTA pairs cost least, a tile
-// costing its columns plus about 48 (its fixed part), the wider on a tie.
-// (Starts of tiles are multiples of 64 rows: the scale columns they begin at
-// are even.)
-int tile_rows(int64_t M, int64_t tiles_f, int clusters) {
-  if (M <= 16) return 16;
-  if (M <= 32) return 32;
-  int best = kMaxNt;
-  int64_t best_cost = -1;
-  for (int nt : {192, 128, 64}) {
-    const int64_t tiles = tiles_f * ((M + nt - 1) / nt);
-    const int64_t cost = (tiles + clusters - 1) / clusters * (nt + 48);
-    if (best_cost < 0 || cost < best_cost) {
-      best_cost = cost;
-      best = nt;
+// Codes as [blocks][rows][128 bytes], in boxes of a stage's blocks.
+bool encode_blocks(CUtensorMap *map, const uint8_t *data, int64_t rows, const Fp8Layout &l,
+                   uint32_t box_rows) {
+  PFN_cuTensorMapEncodeTiled_v12000 enc = tensor_map_encoder();
+  if (!enc) return false;
+  cuuint64_t gdim[3] = {kRowBytes, (cuuint64_t)rows, (cuuint64_t)l.blocks};
+  cuuint64_t gstride[2] = {(cuuint64_t)l.kp, kRowBytes};
+  cuuint32_t box[3] = {kRowBytes, box_rows, kPerStage};
+  cuuint32_t estride[3] = {1u, 1u, 1u};
+  return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<uint8_t *>(data), gdim, gstride,
+             box, estride, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// ns of one block of K for a tile `w` wide (measured at full clocks: 64 160, 128
+// 183, 192 240; 256 by its MMAs).
+double block_ns(int w) {
+  const double issue = 100 + 0.65 * w, math = 1.2 * w;
+  return issue > math ? issue : math;
+}
+// The same of a tile's part that no MMA hides.
+constexpr double kTileNs = 250, kAloneNs = 2000;
+
+// Widths: one tile for up to 32 rows; else what costs least among 64, 128 and 192
+// throughout, 256 alone, and 256 and 192 in turn, whose starts are all multiples of
+// 64 rows (the scale columns they begin at are even).
+Fp8TilePlan plan_of(int64_t M, int64_t N, int64_t blocks, int pairs) {
+  Fp8TilePlan best{};
+  best.tiles_f = (uint32_t)((N + 255) / 256);
+  best.units = best.tiles_f;
+  if (M <= 32) {
+    best.w[0] = M <= 16 ? 16 : 32;
+    return best;
+  }
+  constexpr int kWidths[5][2] = {{kWide, kNarrow}, {kNarrow, 0}, {128, 0}, {64, 0}, {kWide, 0}};
+  double best_ns = 0;
+  for (const auto &w : kWidths) {
+    const int pitch = w[0] + w[1];
+    const int64_t units = best.tiles_f * ((M + pitch - 1) / pitch);
+    double ns = blocks * block_ns(w[0]) + (w[0] > kNarrow && !w[1] ? kAloneNs : kTileNs);
+    if (w[1]) ns += blocks * block_ns(w[1]) + kTileNs;
+    ns *= (double)((units + pairs - 1) / pairs);
+    if (best.w[0] == 0 || ns < best_ns) {
+      best_ns = ns;
+      best.w[0] = w[0];
+      best.w[1] = w[1];
+      // (2^31 tiles of 256 x 64 outputs do not fit the memory)
+      best.units = (uint32_t)units;
     }
   }
   return best;
 }
 
+// fp32 outputs of long sums: the tensor core cuts its running sum's low bits off at
+// every MMA, which leaves a relative 3e-6 after 16384 values (1e-7 rounded), so
+// those go in launches of at most this many blocks that add up in the outputs (0.5e-6
+// at 4096 values).  16-bit outputs do not show it.
+constexpr int64_t kSumBlocks = 32;
+
 template <typename T> cudaError_t launch(Fp8Tiles t, const Fp8Layout &l, cudaStream_t s) {
-  using Cfg = Fp8Cfg<T>;
   auto kern = fp8_pair_kernel<T>;
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   // (an attribute of the function in the current context, so set in every call)
-  if ((e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                (int)Cfg::kSmem)) != cudaSuccess)
+  if ((e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem)) !=
+      cudaSuccess)
     return e;
   // one cluster per resident pair slot (persistent tiles)
   static std::atomic<int> max_clusters[kMaxCachedDevices];
@@ -359,7 +430,7 @@ template <typename T> cudaError_t launch(Fp8Tiles t, const Fp8Layout &l, cudaStr
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(2, 1, 1);
     cfg.blockDim = dim3(kThreads, 1, 1);
-    cfg.dynamicSmemBytes = Cfg::kSmem;
+    cfg.dynamicSmemBytes = kSmem;
     cfg.stream = s;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
@@ -367,46 +438,53 @@ template <typename T> cudaError_t launch(Fp8Tiles t, const Fp8Layout &l, cudaStr
     if (clusters <= 0) return cudaErrorInvalidConfiguration;
     if (dev < kMaxCachedDevices) max_clusters[dev].store(clusters, std::memory_order_relaxed);
   }
-  const Fp8TilePlan plan = fp8_tile_plan(t.p.M, t.p.N, clusters);
-  t.tiles_f = plan.tiles_f;
-  t.nt = plan.nt;
-  t.tiles = plan.tiles;
-  t.steps = (int)l.blocks;
-  t.mmas = (int)((l.kp + 31) / 32);
-  t.xrows = t.nt > 128 ? 2 : 1;
+  const int64_t launches =
+      sizeof(T) == 4 ? (l.blocks + kSumBlocks - 1) / kSumBlocks : 1;
+  const int64_t share = ((l.blocks + launches - 1) / launches + 3) / 4 * 4;  // whole scale atoms
+  t.plan = plan_of(t.p.M, t.p.N, launches > 1 ? share : l.blocks, clusters);
+  const int *w = t.plan.w;
+  t.xrows = w[0] > kNarrow ? 3 : w[0] > 128 ? 2 : 1;
   t.words = t.p.N % 2 == 0 && (reinterpret_cast<uintptr_t>(t.p.out) & 3) == 0;
   t.tma_out = sizeof(T) == 2 && t.p.N % 8 == 0 &&
               (reinterpret_cast<uintptr_t>(t.p.out) & 15) == 0;
-  CUtensorMap wmap, xmap, wsmap, xsmap, omap = {};
-  if (!encode_rows(&wmap, t.p.b, t.p.N, l.kp, 128) ||
-      !encode_rows(&xmap, t.p.a, t.p.M, l.kp, (uint32_t)t.nt / 2) ||
+  CUtensorMap wmap, xmap0, xmap1, wsmap, xsmap, omap = {};
+  if (!encode_blocks(&wmap, t.p.b, t.p.N, l, 128) ||
+      !encode_blocks(&xmap0, t.p.a, t.p.M, l, (uint32_t)w[0] / 2) ||
+      !encode_blocks(&xmap1, t.p.a, t.p.M, l, (uint32_t)(w[1] ? w[1] : w[0]) / 2) ||
       !encode_scales(&wsmap, t.p.b_scales, t.p.N, l.groups, 1, 1) ||
       !encode_scales(&xsmap, t.p.a_scales, t.p.M, l.groups, 1, (uint32_t)t.xrows) ||
-      (t.tma_out && !encode_out(&omap, t.p.out, t.p.M, t.p.N)))
+      (t.tma_out && !encode_out(&omap, t.p.out, t.p.M, t.p.N, kPieceRows)))
     return cudaErrorInvalidValue;
-  const unsigned grid = t.tiles < (uint32_t)clusters ? t.tiles : (unsigned)clusters;
+  const unsigned grid = t.plan.units < (uint32_t)clusters ? t.plan.units : (unsigned)clusters;
   cudaLaunchAttribute early[1];
   early[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   early[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(2 * grid, 1, 1);
   cfg.blockDim = dim3(kThreads, 1, 1);
-  cfg.dynamicSmemBytes = Cfg::kSmem;
+  cfg.dynamicSmemBytes = kSmem;
   cfg.stream = s;
   cfg.attrs = early;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kern, t, wmap, xmap, wsmap, xsmap, omap);
+  for (int64_t block = 0; block < l.blocks; block += share) {
+    t.block0 = (int)block;
+    t.blocks = (int)(l.blocks - block < share || launches == 1 ? l.blocks - block : share);
+    t.steps = (t.blocks + kPerStage - 1) / kPerStage;
+    t.add = block > 0;
+    if (t.add) t.p.bias = nullptr;
+    if ((e = cudaLaunchKernelEx(&cfg, kern, t, wmap, xmap0, xmap1, wsmap, xsmap, omap)) !=
+        cudaSuccess)
+      return e;
+    add_launches(1);
+    if (launches == 1) break;
+  }
+  return cudaSuccess;
 }
 
 }  // namespace
 
-Fp8TilePlan fp8_tile_plan(int64_t M, int64_t N, int pairs) {
-  Fp8TilePlan plan;
-  plan.tiles_f = (uint32_t)((N + 255) / 256);
-  plan.nt = tile_rows(M, plan.tiles_f, pairs);
-  // (2^31 tiles of 256 x 64 outputs do not fit the memory)
-  plan.tiles = plan.tiles_f * (uint32_t)((M + plan.nt - 1) / plan.nt);
-  return plan;
+Fp8TilePlan fp8_tile_plan(int64_t M, int64_t N, int64_t K, int pairs) {
+  return plan_of(M, N, (K + kFp8Block - 1) / kFp8Block, pairs);
 }
 
 cudaError_t launch_fp8_matmul(const Fp8Product &p, unsigned int *error, cudaStream_t s) {

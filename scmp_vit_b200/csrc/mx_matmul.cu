@@ -324,6 +324,20 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
   if (threadIdx.x == 0 && *abort) atomicOr(t.error, 1u);
 }
 
+bool encode_rows(CUtensorMap *map, const uint8_t *data, int64_t rows, int64_t row_bytes,
+                 uint32_t box_rows) {
+  PFN_cuTensorMapEncodeTiled_v12000 enc = tensor_map_encoder();
+  if (!enc) return false;
+  cuuint64_t gdim[2] = {(cuuint64_t)row_bytes, (cuuint64_t)rows};
+  cuuint64_t gstride[1] = {(cuuint64_t)row_bytes};
+  cuuint32_t box[2] = {kStepBytes, box_rows};
+  cuuint32_t estride[2] = {1u, 1u};
+  return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t *>(data), gdim, gstride,
+             box, estride, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 // Activation rows per tile: one tile for up to 32 rows; else the width among
 // 64, 128 and 192 whose rounds of tiles over the CTA pairs cost least, a tile
 // costing its columns plus about 48 (its fixed part), the wider on a tie.
@@ -390,7 +404,7 @@ cudaError_t launch(MxTiles t, int64_t kp, int64_t groups, cudaStream_t s) {
       !encode_rows(&xmap, t.p.a, t.p.M, kp / 2, (uint32_t)t.nt / 2) ||
       !encode_scales(&wsmap, t.p.b_scales, t.p.N, groups, Cfg::kGroups, 1) ||
       !encode_scales(&xsmap, t.p.a_scales, t.p.M, groups, Cfg::kGroups, (uint32_t)t.xrows) ||
-      (t.tma_out && !encode_out(&omap, t.p.out, t.p.M, t.p.N)))
+      (t.tma_out && !encode_out(&omap, t.p.out, t.p.M, t.p.N, 32)))
     return cudaErrorInvalidValue;
   const unsigned grid = t.tiles < (uint32_t)clusters ? t.tiles : (unsigned)clusters;
   cudaLaunchAttribute early[1];

@@ -121,20 +121,6 @@ __device__ __forceinline__ void store_chunk(const P &p, float alpha, bool words,
   }
 }
 
-bool encode_rows(CUtensorMap *map, const uint8_t *data, int64_t rows, int64_t row_bytes,
-                 uint32_t box_rows) {
-  PFN_cuTensorMapEncodeTiled_v12000 enc = tensor_map_encoder();
-  if (!enc) return false;
-  cuuint64_t gdim[2] = {(cuuint64_t)row_bytes, (cuuint64_t)rows};
-  cuuint64_t gstride[1] = {(cuuint64_t)row_bytes};
-  cuuint32_t box[2] = {kRowBytes, box_rows};
-  cuuint32_t estride[2] = {1u, 1u};
-  return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t *>(data), gdim, gstride,
-             box, estride, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-             CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 // Scale atoms [row groups][groups][512 bytes] in boxes of `box_groups` x `box_rows`.
 bool encode_scales(CUtensorMap *map, const uint8_t *scales, int64_t rows, int64_t groups,
                    uint32_t box_groups, uint32_t box_rows) {
@@ -150,13 +136,13 @@ bool encode_scales(CUtensorMap *map, const uint8_t *scales, int64_t rows, int64_
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// 16-bit outputs in pieces of 32 rows x 32 features.
-bool encode_out(CUtensorMap *map, void *out, int64_t rows, int64_t features) {
+// 16-bit outputs in pieces of 32 features.
+bool encode_out(CUtensorMap *map, void *out, int64_t rows, int64_t features, uint32_t box_rows) {
   PFN_cuTensorMapEncodeTiled_v12000 enc = tensor_map_encoder();
   if (!enc) return false;
   cuuint64_t gdim[2] = {(cuuint64_t)features, (cuuint64_t)rows};
   cuuint64_t gstride[1] = {(cuuint64_t)features * 2};
-  cuuint32_t box[2] = {32, 32};
+  cuuint32_t box[2] = {32, box_rows};
   cuuint32_t estride[2] = {1u, 1u};
   return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, out, gdim, gstride, box, estride,
              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,

@@ -40,7 +40,7 @@ BLOCKS = ("row", "square")
 
 def _sizes(rows: int, K: int) -> Tuple[int, int]:
     """Bytes of codes and of scales (``scmp_fp8_data_size``, ``scmp_fp8_scale_size``)."""
-    return rows * ((K + 15) // 16 * 16), (rows + 127) // 128 * ((K + 511) // 512) * 512
+    return rows * ((K + 127) // 128 * 128), (rows + 127) // 128 * ((K + 511) // 512) * 512
 
 
 class FP8Tensor:

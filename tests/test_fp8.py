@@ -45,7 +45,7 @@ def quantize_ref(x, blocks="row"):
     code = code + 128 * np.signbit(v)
     scale = np.broadcast_to(np.where(bad, 0xFF, e + 127), v.shape)[:, :, :, 0]
     flat = (nr * height, nb * 128)
-    kp = -(-K // 16) * 16
+    kp = nb * 128
     return (code.reshape(flat)[:rows, :kp], scale.reshape(-1, nb)[:rows],
             value.reshape(flat)[:rows, :K])
 
@@ -64,7 +64,7 @@ def test_sizes():
     lib = _lib.load()
     for rows, K in ((0, 5), (1, 1), (128, 32), (129, 513), (257, 1024)):
         data, scales = fp8._sizes(rows, K)
-        assert lib.scmp_fp8_data_size(rows, K) == data == rows * (-(-K // 16) * 16)
+        assert lib.scmp_fp8_data_size(rows, K) == data == rows * (-(-K // 128) * 128)
         assert lib.scmp_fp8_scale_size(rows, K) == scales == -(-rows // 128) * -(-K // 512) * 512
     for rows, K in ((-1, 4), (4, 0), (1 << 31, 4), (4, 1 << 31)):
         assert lib.scmp_fp8_data_size(rows, K) == lib.scmp_fp8_scale_size(rows, K) == 0
@@ -501,18 +501,40 @@ def test_product_ranges_and_nan(cuda_device, M):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("M,N,K,nt", [(16448, 1024, 640, 192), (9000, 1152, 1024, 128),
-                                      (1200, 3800, 500, 64), (760, 16384, 256, 192)])
-def test_product_many_tiles(cuda_device, M, N, K, nt):
-    """Several tiles per pair at every tile width, ragged ends; in squares of
-    sampled rows, since the 64-bit product is slow."""
+@pytest.mark.parametrize("M,N,K,widths,units", [
+    (16135, 952, 640, (256, 192), 148), (7299, 1817, 1100, (256, 192), 136),
+    (9000, 1152, 1024, (192, 0), 235), (16697, 80, 71, (128, 0), 131),
+    (788, 333, 1000, (64, 0), 26), (1024, 4096, 4300, (256, 0), 64)])
+def test_product_many_tiles(cuda_device, M, N, K, widths, units):
+    """Every choice of tile widths, several units per pair where it has them, and
+    ragged ends."""
+    assert _lib.fp8_plan(M, N, K)[1:] == (widths, units)
     g = torch.Generator().manual_seed(M)
     a = torch.randn(M, K, generator=g).to(torch.bfloat16).to(cuda_device)
     w = (torch.randn(N, K, generator=g) * 0.05).to(cuda_device)
+    bias = torch.randn(N, generator=g).to(cuda_device)
     qa, qw = fp8.fp8_quantize(a), fp8.fp8_quantize(w, "square")
     for dtype in (torch.float32, torch.bfloat16):
-        close(fp8.fp8_matmul(qa, qw, out_dtype=dtype), values(qa), values(qw))
-    assert _lib.fp8_plan(M, N, K)[1:] == (nt, -(-M // nt) * -(-N // 256))
+        close(fp8.fp8_matmul(qa, qw, bias=bias, out_dtype=dtype), values(qa), values(qw), bias)
+
+
+@pytest.mark.gpu
+def test_long_sums(cuda_device):
+    """fp32 outputs of long sums go in pieces that are rounded, not cut off: with
+    2^-24 per 4096 values and piece at most 8 of them (the tensor core's 128 adds of
+    32 products each cut at most 2^-23 of the running sum, and a quarter of that on
+    average is far from reached), against a root mean square over the outputs."""
+    g = torch.Generator().manual_seed(2)
+    a = torch.randn(300, 16500, generator=g).to(cuda_device)
+    w = torch.randn(520, 16500, generator=g).to(cuda_device)
+    bias = torch.randn(520, generator=g).to(cuda_device)
+    qa, qw = fp8.fp8_quantize(a), fp8.fp8_quantize(w)
+    before = _lib.kernel_launches()
+    y = fp8.fp8_matmul(qa, qw, bias=bias)
+    assert _lib.kernel_launches() - before == 5
+    ref = values(qa) @ values(qw).t() + bias.double()
+    assert float((y.double() - ref).norm() / ref.norm()) < 16 * 2.0 ** -24
+    close(y, values(qa), values(qw), bias)
 
 
 @pytest.mark.gpu
