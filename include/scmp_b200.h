@@ -418,6 +418,50 @@ typedef struct scmp_rotary_args {
 } scmp_rotary_args;
 SCMP_API int scmp_split_qkv_rotary(const scmp_rotary_args *args, void *stream);
 
+/* ---- The same split with every head's row of q and k normalised first (norms of
+ * queries and keys), and its gradients.  With u a row of D elements:
+ *   n = (u - mean) / sqrt(var + eps), rms != 0: u / sqrt(mean u^2 + eps)
+ *   t = n weight + bias               q_ and k_, [D] of x's type or fp32 (param_dtype)
+ * then turned as above; axes may be 0 (no positions, table and pos not read).
+ * split.inverse: the gradients, from q, k, v (their gradients) and x (the forward's
+ * qkv) to qkv, and to dq_weight, dk_weight, dq_bias, dk_bias (each nullable: not
+ * wanted), for which the workspace holds partial sums
+ * (scmp_split_qkv_norm_workspace).  Deterministic.  One launch, two with gradients of
+ * parameters. */
+typedef struct scmp_qknorm_args {
+  scmp_rotary_args split;
+  const void *x;
+  const void *q_weight, *k_weight, *q_bias, *k_bias; /* biases nullable */
+  void *dq_weight, *dk_weight, *dq_bias, *dk_bias;
+  void *workspace;
+  size_t workspace_bytes;
+  int32_t param_dtype, rms;
+  float eps;
+  int32_t reserved;
+} scmp_qknorm_args;
+SCMP_API int scmp_split_qkv_norm(const scmp_qknorm_args *args, void *stream);
+SCMP_API size_t scmp_split_qkv_norm_workspace(int64_t H, int64_t Hk, int64_t D);
+
+/* ---- Dropout from a counter-based generator, with no stored mask:
+ *   y[i] = residual[i] + (u_d < rint(p 2^32) ? 0 : x[i] / (1 - p)),  d = i / span
+ * rounded once; u_d is word d % 4 of Philox4x32-10 at the counter whose lower half is
+ * d / 4 and upper half offset, under the key seed.  span 1 is dropout, a sample's
+ * size stochastic depth.  The gradient of x is the same call on y's gradient without
+ * residual.  state (nullable, on the device): {seed, what is added to offset}, read by
+ * the kernel, so that a captured call draws anew when it changes; the argument seed
+ * is not used then.  residual nullable; y may be x or residual.  One launch. */
+typedef struct scmp_dropout_args {
+  int32_t abi_version;
+  int32_t dtype;
+  const void *x, *residual;
+  void *y;
+  const uint64_t *state;
+  int64_t n, span;
+  uint64_t seed, offset;
+  double p;
+} scmp_dropout_args;
+SCMP_API int scmp_dropout(const scmp_dropout_args *args, void *stream);
+
 /* Message of the last failure on this thread ("" if none). */
 SCMP_API const char *scmp_last_error(void);
 

@@ -71,6 +71,9 @@ EXPORTED_SYMBOLS = (
     "scmp_fp8_train_forward",
     "scmp_fp8_train_backward",
     "scmp_debug_fp8_plan",
+    "scmp_split_qkv_norm",
+    "scmp_split_qkv_norm_workspace",
+    "scmp_dropout",
 )
 
 
@@ -158,6 +161,24 @@ class RotaryArgs(ctypes.Structure):
         ("reserved", ctypes.c_int32 * 3)]
 
 
+class QkNormArgs(ctypes.Structure):
+    """Mirror of ``scmp_qknorm_args``."""
+    _fields_ = [("split", RotaryArgs)] + [
+        (n, ctypes.c_void_p) for n in ("x", "q_weight", "k_weight", "q_bias", "k_bias",
+                                       "dq_weight", "dk_weight", "dq_bias", "dk_bias",
+                                       "workspace")] + [
+        ("workspace_bytes", ctypes.c_size_t), ("param_dtype", ctypes.c_int32),
+        ("rms", ctypes.c_int32), ("eps", ctypes.c_float), ("reserved", ctypes.c_int32)]
+
+
+class DropoutArgs(ctypes.Structure):
+    """Mirror of ``scmp_dropout_args``."""
+    _fields_ = [("abi_version", ctypes.c_int32), ("dtype", ctypes.c_int32)] + [
+        (n, ctypes.c_void_p) for n in ("x", "residual", "y", "state")] + [
+        ("n", ctypes.c_int64), ("span", ctypes.c_int64), ("seed", ctypes.c_uint64),
+        ("offset", ctypes.c_uint64), ("p", ctypes.c_double)]
+
+
 class Fp8QuantizeArgs(ctypes.Structure):
     """Mirror of ``scmp_fp8_quantize_args``."""
     _fields_ = [("abi_version", ctypes.c_int32), ("dtype", ctypes.c_int32),
@@ -202,6 +223,8 @@ PACK_MX_MATMUL = struct.Struct("2i4P3q2i2P2i")
 PACK_NORM = struct.Struct("4i13P3qf3i")
 PACK_NORM_BWD = struct.Struct("4i19PN3q")
 PACK_ROTARY = struct.Struct("2i6P5q16i")
+PACK_QKNORM = struct.Struct("2i6P5q16i10PN2ifi")
+PACK_DROPOUT = struct.Struct("2i4P2q2Qd")
 PACK_FP8_QUANTIZE = struct.Struct("2iP3q2i4P")
 PACK_FP8_MATMUL = struct.Struct("2i4P3q2P2i")
 PACK_FP8_TRAIN = struct.Struct("4i7PN5q")
@@ -296,9 +319,12 @@ def load() -> ctypes.CDLL:
         lib.scmp_fp8_linear.restype = ctypes.c_int
         for name in ("scmp_mx_matmul", "scmp_residual_norm", "scmp_residual_norm_bwd",
                      "scmp_split_qkv_rotary", "scmp_fp8_quantize", "scmp_fp8_matmul",
-                     "scmp_fp8_train_forward", "scmp_fp8_train_backward"):
+                     "scmp_fp8_train_forward", "scmp_fp8_train_backward", "scmp_split_qkv_norm",
+                     "scmp_dropout"):
             getattr(lib, name).argtypes = [ptr, ptr]
             getattr(lib, name).restype = ctypes.c_int
+        lib.scmp_split_qkv_norm_workspace.argtypes = [i64, i64, i64]
+        lib.scmp_split_qkv_norm_workspace.restype = ctypes.c_size_t
         lib.scmp_residual_norm_bwd_workspace.argtypes = [i64, i64, i64]
         lib.scmp_residual_norm_bwd_workspace.restype = ctypes.c_size_t
         lib.scmp_debug_set_wait_limit.argtypes = [ctypes.c_uint64]

@@ -501,6 +501,146 @@ def split_qkv_rotary(qkv: torch.Tensor, num_heads: int, axes: RotaryAxes, pos: t
     return _split_rotary(qkv.contiguous(), pos, table, axes, H, Hk, transpose_v)
 
 
+def _norm_args(qkv, q, k, v, x, weights, pos, table, spec, inverse, v_transposed, grads=(0, 0, 0, 0),
+               workspace=0, workspace_bytes=0):
+    """One ``scmp_split_qkv_norm`` call on contiguous storages."""
+    axes, _, _, rms, eps, _ = spec
+    B, H, N, D = q.shape
+    qw, kw, qb, kb = weights
+    n_axes, dims, sizes, interleaved = (0, _NO_AXES, _NO_AXES, True) if axes is None else (
+        len(axes.dims), axes.c_dims, axes.c_sizes, axes.interleaved)
+    args = _lib.PACK_QKNORM.pack(
+        _lib.ABI_VERSION, DTYPE[qkv.dtype], qkv.data_ptr(), q.data_ptr(), k.data_ptr(),
+        v.data_ptr(), 0 if table is None else table.data_ptr(),
+        0 if pos is None else pos.data_ptr(), B, N, H, k.shape[1], D, n_axes, *dims, *sizes,
+        pos is not None and pos.dim() == 3, interleaved, v_transposed, inverse, 0, 0, 0,
+        0 if x is None else x.data_ptr(), qw.data_ptr(), kw.data_ptr(),
+        0 if qb is None else qb.data_ptr(), 0 if kb is None else kb.data_ptr(), *grads, workspace,
+        workspace_bytes, DTYPE[qw.dtype], rms, eps, 0)
+    call(_lib.load().scmp_split_qkv_norm, qkv.get_device(), args)
+
+
+_NO_AXES = (0,) * _lib.MAX_AXES
+
+
+def _split_norm(src, weights, pos, table, spec):
+    _, H, Hk, _, _, transpose_v = spec
+    B, N, width = src.shape
+    D = width // (H + 2 * Hk)
+    q = src.new_empty(B, H, N, D)
+    k = src.new_empty(B, Hk, N, D)
+    v = src.new_empty(B, Hk, D, N) if transpose_v else src.new_empty(B, Hk, N, D)
+    _norm_args(src, q, k, v, None, weights, pos, table, spec, False, transpose_v)
+    return q, k, v.transpose(-1, -2) if transpose_v else v
+
+
+class _SplitQkvNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, qkv, q_weight, k_weight, q_bias, k_bias, pos, table, spec):
+        src = qkv.contiguous()
+        weights = [t if t is None else t.contiguous()
+                   for t in (q_weight, k_weight, q_bias, k_bias)]
+        ctx.spec = spec
+        ctx.save_for_backward(src, *weights, pos, table)
+        return _split_norm(src, weights, pos, table, spec)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dq, dk, dv):
+        src, *weights, pos, table = ctx.saved_tensors
+        spec, wants = ctx.spec, ctx.needs_input_grad[1:5]
+        grad = torch.empty_like(src)
+        new = torch.zeros_like if src.numel() == 0 else torch.empty_like
+        params = [new(w) if want and w is not None else None for w, want in zip(weights, wants)]
+        if src.numel():
+            # v's gradient in whichever of its two layouts it comes
+            transposed = not dv.is_contiguous() and dv.transpose(-1, -2).is_contiguous()
+            dv = dv if transposed else dv.contiguous()
+            dq, dk = dq.contiguous(), dk.contiguous()
+            size, ws = 0, None
+            if any([t is not None for t in params]):
+                size = _lib.load().scmp_split_qkv_norm_workspace(dq.shape[1], dk.shape[1],
+                                                                 dq.shape[3])
+                ws = torch.empty(size, dtype=torch.uint8, device=src.device)
+            _norm_args(grad, dq, dk, dv, src, weights, pos, table, spec, True, transposed,
+                       [0 if t is None else t.data_ptr() for t in params],
+                       0 if ws is None else ws.data_ptr(), size)
+        return (grad if ctx.needs_input_grad[0] else None, *params, None, None, None)
+
+
+def split_qkv_norm(qkv: torch.Tensor, num_heads: int, q_weight: torch.Tensor,
+                   k_weight: torch.Tensor, q_bias: Optional[torch.Tensor] = None,
+                   k_bias: Optional[torch.Tensor] = None, *, kind: str = "rms",
+                   eps: float = 1e-6, axes: Optional[RotaryAxes] = None,
+                   pos: Optional[torch.Tensor] = None, num_kv_heads: Optional[int] = None,
+                   transpose_v: bool = True):
+    """``split_qkv_rotary`` with every head's row of q and k normalised first, in
+    the same engine pass::
+
+        n = u / sqrt(mean(u^2) + eps)                   kind "rms", over the D of a head
+        n = (u - mean(u)) / sqrt(var(u) + eps)          kind "layer"
+        q = turned(n * q_weight + q_bias)               k the same with its own
+
+    ``q_weight``, ``k_weight`` and the optional biases: ``[D]``, shared by the heads, of
+    qkv's type or float32, all of one type.  ``axes`` and ``pos`` as there, or both
+    None: norms alone.  Statistics and rotation in fp32, rounded once; v is copied
+    bit for bit.  Differentiable (once, backward) in ``qkv`` and the parameters, whose
+    gradients add up in a fixed order."""
+    H = int(num_heads)
+    Hk = H if num_kv_heads is None else int(num_kv_heads)
+    if kind not in ("layer", "rms"):
+        raise ValueError(f"unknown norm kind {kind!r}")
+    if not (isinstance(eps, (int, float)) and eps >= 0):
+        raise ValueError(f"eps must be >= 0, got {eps!r}")
+    if not qkv.is_cuda:
+        raise RuntimeError("split_qkv_norm runs on the CUDA engine only (no CPU path); "
+                           f"got {qkv.device}")
+    if qkv.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        raise TypeError(f"qkv must be float32, bfloat16 or float16, got {qkv.dtype}")
+    if H < 1 or Hk < 1 or H % Hk:
+        raise ValueError(f"num_heads={H} must be a positive multiple of num_kv_heads={Hk}")
+    if qkv.dim() != 3 or qkv.shape[-1] % (H + 2 * Hk):
+        raise ValueError(f"qkv must be [B, N, (H + 2 Hk) D], got {tuple(qkv.shape)} for H={H}, "
+                         f"Hk={Hk}")
+    B, N, width = qkv.shape
+    D = width // (H + 2 * Hk)
+    index = qkv.get_device()
+    n_axes = 0 if axes is None else len(axes.dims)
+    if D < 2 or D % 2 or D > 256 or (n_axes and sum(axes.dims) > D):
+        raise ValueError("the head size must be even, at most 256 and hold the axes' dims, "
+                         f"got {D}")
+    param_dtype = q_weight.dtype
+    if param_dtype != qkv.dtype and param_dtype != torch.float32:
+        raise TypeError(f"parameters must be {qkv.dtype} or float32, got {param_dtype}")
+    weights = (q_weight, k_weight, q_bias, k_bias)
+    for name, w in zip(("q_weight", "k_weight", "q_bias", "k_bias"), weights):
+        if w is None and "bias" in name:
+            continue
+        if w.shape != (D,) or w.dtype != param_dtype or w.get_device() != index:
+            raise ValueError(f"{name} must be [{D}] of {param_dtype} on {qkv.device}, got "
+                             f"{tuple(w.shape)} {w.dtype} {w.device}")
+    if (axes is None) != (pos is None):
+        raise ValueError("axes and pos go together")
+    table = None
+    if axes is not None:
+        if (pos.dtype != torch.int32 or pos.get_device() != index
+                or tuple(pos.shape) not in ((N, n_axes), (B, N, n_axes))):
+            raise ValueError(f"pos must be int32 [{N}, {n_axes}] or [{B}, {N}, {n_axes}] on "
+                             f"{qkv.device}, got {pos.dtype} {tuple(pos.shape)} {pos.device}")
+        table = axes.table_bits
+        if table.get_device() != index:
+            raise ValueError(f"axes are on {table.device}, qkv on {qkv.device}")
+        pos = pos.contiguous()
+    spec = (axes, H, Hk, kind == "rms", float(eps), bool(transpose_v))
+    leaves = (qkv, *weights)
+    if (torch.is_grad_enabled() and any([t is not None and t.requires_grad for t in leaves])
+            ) or has_tangent(leaves):
+        # (a forward-mode tangent is refused there: the function has no jvp)
+        return _SplitQkvNorm.apply(*leaves, pos, table, spec)
+    return _split_norm(qkv.contiguous(), [t if t is None else t.contiguous() for t in weights],
+                       pos, table, spec)
+
+
 class GridRotary(nn.Module):
     """The positions of an image's (or clip's) patches on their grid, behind
     ``prefix`` tokens without one (the class token): the head's dimensions in
@@ -522,6 +662,37 @@ class GridRotary(nn.Module):
         return split_qkv_rotary(qkv, num_heads, self.axes, self.pos, transpose_v=transpose_v)
 
 
+class QKNorm(nn.Module):
+    """The norms of queries and keys of an attention module, one weight (and, for
+    layer norms, bias) of the head's size each.  An attention module whose ``qk_norm``
+    attribute is one splits its projection output by it, its ``rope`` included."""
+
+    def __init__(self, head_dim: int, kind: str = "rms", *, eps: float = 1e-6,
+                 bias: Optional[bool] = None):
+        super().__init__()
+        if kind not in ("layer", "rms"):
+            raise ValueError(f"unknown norm kind {kind!r}")
+        self.kind, self.eps = kind, eps
+        self.q_weight = nn.Parameter(torch.ones(head_dim))
+        self.k_weight = nn.Parameter(torch.ones(head_dim))
+        bias = kind == "layer" if bias is None else bias
+        self.q_bias = nn.Parameter(torch.zeros(head_dim)) if bias else None
+        self.k_bias = nn.Parameter(torch.zeros(head_dim)) if bias else None
+
+    def split(self, qkv: torch.Tensor, num_heads: int, rope: Optional[GridRotary] = None, *,
+              num_kv_heads: Optional[int] = None, transpose_v: bool = True):
+        """``split_qkv_norm`` of a projection output, with ``rope``'s positions."""
+        return split_qkv_norm(qkv, num_heads, self.q_weight, self.k_weight, self.q_bias,
+                              self.k_bias, kind=self.kind, eps=self.eps,
+                              axes=None if rope is None else rope.axes,
+                              pos=None if rope is None else rope.pos, num_kv_heads=num_kv_heads,
+                              transpose_v=transpose_v)
+
+    def extra_repr(self) -> str:
+        return (f"{self.q_weight.numel()}, kind={self.kind!r}, eps={self.eps}, "
+                f"bias={self.q_bias is not None}")
+
+
 def make_sc_attention_forward(sc_prec: int, sc_av: bool, sc_qk: bool = True,
                               qk_mp_cfg: MPConfig | None = None,
                               av_mp_cfg: MPConfig | None = None, *,
@@ -529,8 +700,9 @@ def make_sc_attention_forward(sc_prec: int, sc_av: bool, sc_qk: bool = True,
     """``forward(self, x)`` for a DINOv2-style attention module with
     ``qkv``, ``proj``, ``proj_drop``, ``num_heads``, ``scale`` attributes
     (same signature and numerics as ``cls/sc_attention_patch.py:248-328``).
-    A ``rope`` attribute that is a ``GridRotary`` turns q and k before Q@K^T;
-    what other modules keep under that name is left alone."""
+    A ``rope`` attribute that is a ``GridRotary`` turns q and k before Q@K^T, a
+    ``qk_norm`` attribute that is a ``QKNorm`` normalises them before that; what
+    other modules keep under those names is left alone."""
     do_av = sc_av
 
     def forward(self, x, attn_bias=None):
@@ -538,8 +710,10 @@ def make_sc_attention_forward(sc_prec: int, sc_av: bool, sc_qk: bool = True,
         H = self.num_heads
         D = C // H
         qkv = self.qkv(x)
-        rope = getattr(self, "rope", None)
-        if isinstance(rope, GridRotary):
+        rope, qk_norm = getattr(self, "rope", None), getattr(self, "qk_norm", None)
+        if isinstance(qk_norm, QKNorm):
+            q, k, v = qk_norm.split(qkv, H, rope if isinstance(rope, GridRotary) else None)
+        elif isinstance(rope, GridRotary):
             q, k, v = rope.split(qkv, H)
         elif qkv.is_cuda and qkv.element_size() in (2, 4) and B * H <= 65535 and D <= 256:
             q, k, v = split_qkv(qkv, H)

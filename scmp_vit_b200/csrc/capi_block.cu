@@ -1,8 +1,12 @@
-// C ABI of the 4-bit block operators (declared in include/scmp_b200.h):
+// C ABI of the block operators but the 8-bit products (declared in include/scmp_b200.h):
 // argument checks, layouts and launches.
+#include <cmath>
+
 #include "capi_check.cuh"
 #include "mx_common.cuh"
 #include "norm.cuh"
+#include "dropout.cuh"
+#include "qknorm.cuh"
 #include "rotary.cuh"
 #include "sc_common.cuh"
 
@@ -57,6 +61,66 @@ int check_product(const scmp_mx_matmul_args *args, bool codes, MxProduct &p) {
   p.bias_dtype = x.bias_dtype;
   p.out = x.out;
   p.out_dtype = x.out_dtype;
+  return SCMP_OK;
+}
+
+// Shapes of a qkv split.
+int check_split(const char *what, int64_t B, int64_t N, int64_t H, int64_t Hk, int64_t D) {
+  if (B < 0 || N < 0 || H < 1 || Hk < 1 || D < 1 || H > 65535 || Hk > 65535)
+    return fail(SCMP_EINVAL, "bad shape B=%lld N=%lld H=%lld Hk=%lld D=%lld", (long long)B,
+                (long long)N, (long long)H, (long long)Hk, (long long)D);
+  if (H % Hk != 0) return fail(SCMP_EINVAL, "H must be a multiple of Hk");
+  if (D > 256 || D % 2 != 0)
+    return fail(SCMP_EUNSUPPORTED, "%s takes even head sizes up to 256, got %lld", what,
+                (long long)D);
+  return SCMP_OK;
+}
+
+// A split's arguments, with 0 (positions then are not read) to SCMP_MAX_AXES axes.
+int check_rotary(const char *what, const scmp_rotary_args &x, RotaryParams &p) {
+  int rc = check_split(what, x.B, x.N, x.H, x.Hk, x.D);
+  if (rc != SCMP_OK) return rc;
+  if (x.axes < 0 || x.axes > SCMP_MAX_AXES)
+    return fail(SCMP_EINVAL, "axes must be at most %d, got %d", SCMP_MAX_AXES, x.axes);
+  int64_t at = 0, turned = 0;
+  for (int a = 0; a < x.axes; ++a) {
+    if (x.dims[a] < 2 || x.dims[a] > x.D || x.dims[a] % 2 != 0 || x.sizes[a] < 1)
+      return fail(SCMP_EINVAL, "axis %d: dims %d (even, >= 2), size %d (>= 1)", a, x.dims[a],
+                  x.sizes[a]);
+    p.dims[a] = x.dims[a];
+    p.sizes[a] = x.sizes[a];
+    p.table_at[a] = at;
+    turned += x.dims[a];
+    at += (int64_t)x.sizes[a] * (x.dims[a] / 2);
+  }
+  if (turned > x.D) return fail(SCMP_EINVAL, "the axes' dims exceed the head size");
+  if (x.B == 0 || x.N == 0) return SCMP_OK;
+  // pieces of a head row are counted in 32 bits
+  if (x.N > UINT32_MAX / x.D || x.B > UINT32_MAX / x.D / x.N)
+    return fail(SCMP_EUNSUPPORTED, "%s takes up to 2^32 - 1 elements per head, got "
+                "B=%lld N=%lld D=%lld tokens", what, (long long)x.B, (long long)x.N,
+                (long long)x.D);
+  if (!x.qkv || !x.q || !x.k || !x.v || (x.axes > 0 && (!x.table || !x.pos)))
+    return fail(SCMP_EINVAL, "qkv, q, k, v, table and pos must be non-NULL");
+  if (!aligned({x.table}, 8) || !aligned({x.pos}, 4))
+    return fail(SCMP_EINVAL, "table must be 8-byte and pos 4-byte aligned");
+  if ((rc = check_elements({x.qkv, x.q, x.k, x.v}, x.dtype)) != SCMP_OK) return rc;
+  p.qkv = x.qkv;
+  p.q = x.q;
+  p.k = x.k;
+  p.v = x.v;
+  p.table = reinterpret_cast<const float2 *>(x.table);
+  p.pos = x.pos;
+  p.B = x.B;
+  p.N = x.N;
+  p.H = x.H;
+  p.Hk = x.Hk;
+  p.D = (int)x.D;
+  p.axes = x.axes;
+  p.pos_batched = x.pos_batched != 0;
+  p.interleaved = x.interleaved != 0;
+  p.v_transposed = x.v_transposed != 0;
+  p.inverse = x.inverse != 0;
   return SCMP_OK;
 }
 
@@ -330,57 +394,110 @@ int scmp_split_qkv_rotary(const scmp_rotary_args *args, void *stream) {
   if (x.abi_version != SCMP_ABI_VERSION)
     return fail(SCMP_EINVAL, "abi_version %d != %d", x.abi_version, SCMP_ABI_VERSION);
   if (!known_dtype(x.dtype)) return fail(SCMP_EINVAL, "unknown dtype %d", x.dtype);
-  if (x.B < 0 || x.N < 0 || x.H < 1 || x.Hk < 1 || x.D < 1 || x.H > 65535 || x.Hk > 65535)
-    return fail(SCMP_EINVAL, "bad shape B=%lld N=%lld H=%lld Hk=%lld D=%lld", (long long)x.B,
-                (long long)x.N, (long long)x.H, (long long)x.Hk, (long long)x.D);
-  if (x.H % x.Hk != 0) return fail(SCMP_EINVAL, "H must be a multiple of Hk");
-  if (x.D > 256 || x.D % 2 != 0)
-    return fail(SCMP_EUNSUPPORTED, "split_qkv_rotary takes even head sizes up to 256, got %lld",
-                (long long)x.D);
-  if (x.axes < 1 || x.axes > SCMP_MAX_AXES)
-    return fail(SCMP_EINVAL, "axes must be 1 to %d, got %d", SCMP_MAX_AXES, x.axes);
-  RotaryParams p{};
-  int64_t at = 0, turned = 0;
-  for (int a = 0; a < x.axes; ++a) {
-    if (x.dims[a] < 2 || x.dims[a] > x.D || x.dims[a] % 2 != 0 || x.sizes[a] < 1)
-      return fail(SCMP_EINVAL, "axis %d: dims %d (even, >= 2), size %d (>= 1)", a, x.dims[a],
-                  x.sizes[a]);
-    p.dims[a] = x.dims[a];
-    p.sizes[a] = x.sizes[a];
-    p.table_at[a] = at;
-    turned += x.dims[a];
-    at += (int64_t)x.sizes[a] * (x.dims[a] / 2);
+  if (x.axes < 1 || x.axes > SCMP_MAX_AXES) {
+    const int rc = check_split("split_qkv_rotary", x.B, x.N, x.H, x.Hk, x.D);
+    return rc != SCMP_OK
+               ? rc
+               : fail(SCMP_EINVAL, "axes must be 1 to %d, got %d", SCMP_MAX_AXES, x.axes);
   }
-  if (turned > x.D) return fail(SCMP_EINVAL, "the axes' dims exceed the head size");
-  if (x.B == 0 || x.N == 0) return SCMP_OK;
-  // pieces of a head row are counted in 32 bits
-  if (x.N > UINT32_MAX / x.D || x.B > UINT32_MAX / x.D / x.N)
-    return fail(SCMP_EUNSUPPORTED, "split_qkv_rotary takes up to 2^32 - 1 elements per head, got "
-                "B=%lld N=%lld D=%lld tokens", (long long)x.B, (long long)x.N, (long long)x.D);
-  if (!x.qkv || !x.q || !x.k || !x.v || !x.table || !x.pos)
-    return fail(SCMP_EINVAL, "qkv, q, k, v, table and pos must be non-NULL");
-  if (!aligned({x.table}, 8) || !aligned({x.pos}, 4))
-    return fail(SCMP_EINVAL, "table must be 8-byte and pos 4-byte aligned");
-  const int rc = check_elements({x.qkv, x.q, x.k, x.v}, x.dtype);
-  if (rc != SCMP_OK) return rc;
-  p.qkv = x.qkv;
-  p.q = x.q;
-  p.k = x.k;
-  p.v = x.v;
-  p.table = reinterpret_cast<const float2 *>(x.table);
-  p.pos = x.pos;
-  p.B = x.B;
-  p.N = x.N;
-  p.H = x.H;
-  p.Hk = x.Hk;
-  p.D = (int)x.D;
-  p.axes = x.axes;
-  p.pos_batched = x.pos_batched != 0;
-  p.interleaved = x.interleaved != 0;
-  p.v_transposed = x.v_transposed != 0;
-  p.inverse = x.inverse != 0;
+  RotaryParams p{};
+  int rc = check_rotary("split_qkv_rotary", x, p);
+  if (rc != SCMP_OK || x.B == 0 || x.N == 0) return rc;
   const cudaError_t e = launch_rotary(p, x.dtype, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return cuda_fail(e, "split_qkv_rotary launch");
+  add_launches(1);
+  return SCMP_OK;
+}
+
+int scmp_split_qkv_norm(const scmp_qknorm_args *args, void *stream) {
+  set_last_error("");
+  if (!args) return fail(SCMP_EINVAL, "args is NULL");
+  const scmp_rotary_args &x = args->split;
+  if (x.abi_version != SCMP_ABI_VERSION)
+    return fail(SCMP_EINVAL, "abi_version %d != %d", x.abi_version, SCMP_ABI_VERSION);
+  if (!known_dtype(x.dtype) ||
+      (args->param_dtype != x.dtype && args->param_dtype != SCMP_F32))
+    return fail(SCMP_EINVAL, "dtype %d with parameters of dtype %d", x.dtype, args->param_dtype);
+  if (!(args->eps >= 0.0f)) return fail(SCMP_EINVAL, "eps must be >= 0");
+  QkNormParams p{};
+  int rc = check_rotary("split_qkv_norm", x, p.r);
+  if (rc != SCMP_OK) return rc;
+  if (x.B == 0 || x.N == 0) return SCMP_OK;
+  if (!args->q_weight || !args->k_weight)
+    return fail(SCMP_EINVAL, "q_weight and k_weight must be non-NULL");
+  if ((rc = check_elements({args->q_weight, args->k_weight, args->q_bias, args->k_bias,
+                            args->dq_weight, args->dk_weight, args->dq_bias, args->dk_bias},
+                           args->param_dtype)) != SCMP_OK)
+    return rc;
+  p.weight[0] = args->q_weight;
+  p.weight[1] = args->k_weight;
+  p.bias[0] = args->q_bias;
+  p.bias[1] = args->k_bias;
+  p.param_dtype = args->param_dtype;
+  p.eps = args->eps;
+  p.rms = args->rms != 0;
+  auto s = static_cast<cudaStream_t>(stream);
+  void *const grads[4] = {args->dq_weight, args->dq_bias, args->dk_weight, args->dk_bias};
+  bool sums = false;
+  if (x.inverse) {
+    if (!args->x) return fail(SCMP_EINVAL, "x (the forward's qkv) must be non-NULL");
+    if ((rc = check_elements({args->x}, x.dtype)) != SCMP_OK) return rc;
+    p.x = args->x;
+    sums = grads[0] || grads[1] || grads[2] || grads[3];
+    if (sums) {
+      const size_t need = scmp_split_qkv_norm_workspace(x.H, x.Hk, x.D);
+      if (!args->workspace || args->workspace_bytes < need)
+        return fail(SCMP_EWORKSPACE, "workspace needs %zu bytes, got %zu", need,
+                    args->workspace ? args->workspace_bytes : (size_t)0);
+      if (!aligned({args->workspace}, 4))
+        return fail(SCMP_EINVAL, "workspace must be 4-byte aligned");
+      p.part = static_cast<float *>(args->workspace);
+    }
+  }
+  cudaError_t e = launch_qknorm(p, x.dtype, s);
+  if (e != cudaSuccess) return cuda_fail(e, "split_qkv_norm launch");
+  add_launches(1);
+  if (sums) {
+    if ((e = launch_qknorm_sum(p, grads, s)) != cudaSuccess)
+      return cuda_fail(e, "split_qkv_norm launch");
+    add_launches(1);
+  }
+  return SCMP_OK;
+}
+
+size_t scmp_split_qkv_norm_workspace(int64_t H, int64_t Hk, int64_t D) {
+  if (H < 1 || Hk < 1 || H > 65535 || Hk > 65535 || D < 1 || D > 256) return 0;
+  return (size_t)qknorm_bwd_blocks(H, Hk).qk * 2 * (size_t)D * sizeof(float);
+}
+
+int scmp_dropout(const scmp_dropout_args *args, void *stream) {
+  set_last_error("");
+  if (!args) return fail(SCMP_EINVAL, "args is NULL");
+  const scmp_dropout_args &x = *args;
+  if (x.abi_version != SCMP_ABI_VERSION)
+    return fail(SCMP_EINVAL, "abi_version %d != %d", x.abi_version, SCMP_ABI_VERSION);
+  if (!known_dtype(x.dtype)) return fail(SCMP_EINVAL, "unknown dtype %d", x.dtype);
+  if (x.n < 0 || x.span < 1)
+    return fail(SCMP_EINVAL, "bad sizes n=%lld span=%lld", (long long)x.n, (long long)x.span);
+  if (!(x.p >= 0.0 && x.p <= 1.0)) return fail(SCMP_EINVAL, "p must be within 0 and 1");
+  if (x.n == 0) return SCMP_OK;
+  if (!x.x || !x.y) return fail(SCMP_EINVAL, "x and y must be non-NULL");
+  const int rc = check_elements({x.x, x.residual, x.y}, x.dtype);
+  if (rc != SCMP_OK) return rc;
+  if (!aligned({x.state}, 8)) return fail(SCMP_EINVAL, "state must be 8-byte aligned");
+  DropoutParams p{};
+  p.x = x.x;
+  p.residual = x.residual;
+  p.y = x.y;
+  p.n = x.n;
+  p.span = x.span;
+  p.seed = x.seed;
+  p.offset = x.offset;
+  p.state = x.state;
+  p.threshold = (uint64_t)nearbyint(x.p * 4294967296.0);
+  p.scale = x.p < 1.0 ? (float)(1.0 / (1.0 - x.p)) : 0.0f;
+  const cudaError_t e = launch_dropout(p, x.dtype, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "dropout launch");
   add_launches(1);
   return SCMP_OK;
 }

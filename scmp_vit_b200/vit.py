@@ -9,10 +9,11 @@ CLS token and the mean patch token (2048 -> 1000).  Weights are random
 (seeded); there are no checkpoints in this environment.
 
 With ``rope`` the attention turns q and k by the patches' (height, width), as
-EVA-type blocks do.  ``patch_vit_mx`` puts the linears in microscaled 4 bits
-instead (``mx.MXLinear``, the deterministic counterpart of the SC linears), and
+EVA-type blocks do, with ``qk_norm`` it normalises them first.  ``patch_vit_mx``
+puts the linears in microscaled 4 bits instead (``mx.MXLinear``, the deterministic
+counterpart of the SC linears), ``patch_vit_fp8`` in 8 bits, for training too, and
 ``set_fused_norm`` runs the blocks' residual adds and norms in one pass each,
-with gradients.
+with gradients.  ``set_dropout`` gives the blocks dropout and stochastic depth.
 
 ``patch_vit`` installs the SC operators per block: ``qkv_proj`` /
 ``out_proj`` / ``mlp_fc1`` / ``mlp_fc2`` as ``SCLinear``, Q@K^T and Attn@V
@@ -31,7 +32,8 @@ import torch.nn.functional as F
 
 from . import _lib
 from ._call import DTYPE, call, has_tangent, in_dual_level, once_differentiable
-from .attention import GridRotary, make_sc_attention_forward
+from .attention import GridRotary, QKNorm, make_sc_attention_forward
+from .fp8 import FP8Linear
 from .head_aligned_comp import HeadAlignedSCLinear
 from .mp import SeededRandomMPConfig, quantile_counts, set_current_block_idx
 from .mx import MXLinear
@@ -301,6 +303,133 @@ def residual_norm(x: torch.Tensor, y: Optional[torch.Tensor], weight: torch.Tens
     return (x if r is None else r), q
 
 
+PER = ("element", "row", "sample")
+
+
+def _dropout_launch(x, residual, p, seed, offset, state, span):
+    """One ``scmp_dropout`` call on contiguous tensors."""
+    y = torch.empty_like(x)
+    args = _lib.PACK_DROPOUT.pack(_lib.ABI_VERSION, DTYPE[x.dtype], x.data_ptr(), _ptr(residual),
+                                  y.data_ptr(), _ptr(state), x.numel(), span, seed, offset, p)
+    call(_lib.load().scmp_dropout, x.get_device(), args)
+    return y
+
+
+class _Dropout(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, state, p, seed, offset, span):
+        ctx.draw = (p, seed, offset)
+        ctx.span = span
+        ctx.save_for_backward(state)
+        return _dropout_launch(_dense(x), _dense(residual), p, seed, offset, state, span)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        (state,) = ctx.saved_tensors
+        dx = None
+        if ctx.needs_input_grad[0]:
+            dx = _dropout_launch(_dense(dy), None, *ctx.draw, state, ctx.span)
+        return dx, dy if ctx.needs_input_grad[1] else None, None, None, None, None, None
+
+
+def dropout(x: torch.Tensor, p: float, seed, offset: int = 0, *, per: str = "element",
+            residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Dropout whose mask is never stored: ``x / (1 - p)`` where a draw is kept, 0
+    where it is dropped (whatever x holds there), ``+ residual``, in one pass, rounded
+    once.  ``per``: one draw per ``"element"``, per ``"row"`` (last dimension) or per
+    ``"sample"`` (first dimension: stochastic depth).
+
+    Draw ``d`` (counted in row-major order) is word ``d % 4`` of Philox4x32-10 under
+    the 64-bit key ``seed`` at the counter ``(d // 4, offset)``, and is dropped if it is
+    below ``round(p * 2^32)``: the same call draws the same mask, another ``offset``
+    another one.  ``seed`` may be an int64 tensor ``[seed, more]`` on x's device, which
+    the kernel reads (``more`` is added to ``offset``): a captured call then draws anew
+    when the tensor changes between replays.
+
+    ``x`` ``[..., C]`` and ``residual`` of one shape and type (float32, bfloat16,
+    float16), CUDA.  Differentiable (once, backward) in both: the backward pass draws
+    the mask again, so a seed tensor must still hold what it held."""
+    if per not in PER:
+        raise ValueError(f"unknown per {per!r} (one of {PER})")
+    if not 0.0 <= p <= 1.0:
+        raise ValueError(f"p must be within 0 and 1, got {p!r}")
+    if not x.is_cuda:
+        raise RuntimeError(f"dropout runs on the CUDA engine only (no CPU path); got {x.device}")
+    if x.dtype not in _NORM_TYPES:
+        raise TypeError(f"x must be float32, bfloat16 or float16, got {x.dtype}")
+    if not x.dim() and per != "element":
+        raise ValueError("rows and samples are of tensors with dimensions")
+    index = x.get_device()
+    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype
+                                 or residual.get_device() != index):
+        raise ValueError(f"residual must match x: {tuple(residual.shape)} {residual.dtype} "
+                         f"{residual.device} vs {tuple(x.shape)} {x.dtype} {x.device}")
+    state = None
+    if isinstance(seed, torch.Tensor):
+        if (seed.dtype != torch.int64 or seed.shape != (2,) or seed.get_device() != index
+                or not seed.is_contiguous()):
+            raise ValueError(f"a seed tensor is [seed, more], int64 and contiguous on {x.device}, "
+                             f"got {seed.dtype} {tuple(seed.shape)} {seed.device}")
+        state, seed = seed, 0
+    seed, offset = int(seed), int(offset)
+    if not (-1 << 63 <= seed < 1 << 64 and 0 <= offset < 1 << 64):
+        raise ValueError(f"seed and offset are 64-bit, got {seed} and {offset}")
+    n = x.numel()
+    span = 1
+    if per != "element" and n:
+        span = x.shape[-1] if per == "row" else n // x.shape[0]
+    seed &= (1 << 64) - 1
+    if (torch.is_grad_enabled() and (x.requires_grad or (
+            residual is not None and residual.requires_grad))) or has_tangent((x, residual)):
+        # (a forward-mode tangent is refused there: the function has no jvp)
+        return _Dropout.apply(x, residual, state, float(p), seed, offset, span)
+    return _dropout_launch(_dense(x), _dense(residual), float(p), seed, offset, state, span)
+
+
+class Dropout(nn.Module):
+    """``dropout`` in a model: in training every call takes the next mask, in
+    evaluation it passes through.  ``index`` tells the modules of a model apart, which
+    may then share ``seed``.  ``calls`` counts (and, set, repeats) the eager masks;
+    calls that a graph captures count on the device, so that every replay draws
+    masks of its own."""
+
+    def __init__(self, p: float, *, per: str = "element", seed: int = 0, index: int = 0):
+        super().__init__()
+        if per not in PER:
+            raise ValueError(f"unknown per {per!r} (one of {PER})")
+        if not 0.0 <= p <= 1.0:
+            raise ValueError(f"p must be within 0 and 1, got {p!r}")
+        if not 0 <= index < 1 << 16:
+            raise ValueError(f"index must be within 0 and 65535, got {index}")
+        self.p, self.per, self.seed, self.index, self.calls = float(p), per, int(seed), index, 0
+        self.register_buffer("state", torch.tensor([self.seed, 0]), persistent=False)
+
+    @property
+    def active(self) -> bool:
+        return self.training and self.p > 0
+
+    def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+        if not self.active:
+            return x if residual is None else residual + x
+        at = self.index << 48  # (its calls below 2^47, the captured ones above)
+        if x.is_cuda and torch.cuda.is_current_stream_capturing():
+            state = self.state.clone()
+            self.state[1:] += 1
+            return dropout(x, self.p, state, at + (1 << 47), per=self.per, residual=residual)
+        offset = at + self.calls
+        self.calls += 1
+        return dropout(x, self.p, self.seed, offset, per=self.per, residual=residual)
+
+    def extra_repr(self) -> str:
+        return f"p={self.p}, per={self.per!r}, seed={self.seed}, index={self.index}"
+
+
+def _active(m: Optional[nn.Module]) -> bool:
+    """Whether a module drops anything in this call."""
+    return m is not None and (type(m) is not Dropout or m.active) and type(m) is not nn.Identity
+
+
 def _plain_linear(m: nn.Module) -> bool:
     return (type(m) is nn.Linear and m.bias is not None and m.weight.dtype == torch.float32
             and m.weight.is_contiguous() and m.bias.is_contiguous())
@@ -312,9 +441,12 @@ class Mlp(nn.Module):
         self.fc1 = nn.Linear(dim, hidden)
         self.act = nn.GELU()
         self.fc2 = nn.Linear(hidden, dim)
+        self.drop = nn.Identity()
 
     def forward(self, x):
-        return _fp_linear(self.fc2, self.act(_fp_linear(self.fc1, x)))
+        y = _fp_linear(self.fc2, self.act(_fp_linear(self.fc1, x)))
+        drop = getattr(self, "drop", None)  # (a module saved whole by an earlier version has none)
+        return y if drop is None else drop(y)
 
 
 class Attention(nn.Module):
@@ -327,12 +459,16 @@ class Attention(nn.Module):
         self.attn_drop = nn.Identity()
         self.proj_drop = nn.Identity()
         self.rope: Optional[GridRotary] = None  # positions of q and k, if the model has them
+        self.qk_norm: Optional[QKNorm] = None   # and their norms
 
     def forward(self, x, attn_bias=None):
         B, N, C = x.shape
         H = self.num_heads
-        rope = getattr(self, "rope", None)  # (a module saved whole by an earlier version has none)
-        if rope is not None:
+        # (a module saved whole by an earlier version has neither)
+        rope, qk_norm = getattr(self, "rope", None), getattr(self, "qk_norm", None)
+        if qk_norm is not None:
+            q, k, v = qk_norm.split(self.qkv(x), H, rope, transpose_v=False)
+        elif rope is not None:
             q, k, v = rope.split(self.qkv(x), H, transpose_v=False)
         else:
             qkv = self.qkv(x).reshape(B, N, 3, H, C // H).permute(2, 0, 3, 1, 4)
@@ -360,6 +496,7 @@ class Block(nn.Module):
         self.mlp = Mlp(dim, hidden)
         self.ls2 = LayerScale(dim, ls_init)
         self.comp: Optional[nn.Module] = None  # head-aligned compensation, if installed
+        self.drop_path: Optional[Dropout] = None  # stochastic depth, if the model has it
         self.block_idx = 0
 
     def forward(self, x):
@@ -368,11 +505,20 @@ class Block(nn.Module):
             return self._forward_fused_norm(x)
         if self._fused_glue_applies(x):
             return self._forward_fused_glue(x)
-        y = x + self.ls1(self.attn(self.norm1(x)))
-        y = y + self.ls2(self.mlp(self.norm2(y)))
+        y = self._add(x, self.ls1(self.attn(self.norm1(x))))
+        y = self._add(y, self.ls2(self.mlp(self.norm2(y))))
         if self.comp is not None:
             y = y + self.comp(x).to(y.dtype)
         return y
+
+    def _add(self, x: torch.Tensor, branch: torch.Tensor) -> torch.Tensor:
+        """The residual add, with stochastic depth in the same pass where types allow."""
+        drop = getattr(self, "drop_path", None)
+        if not _active(drop):
+            return x + branch
+        if x.dtype == branch.dtype and type(drop) is Dropout:
+            return drop(branch, x)
+        return x + drop(branch)
 
     def _fused_norm_applies(self, x: torch.Tensor) -> bool:
         qkv, fc1 = getattr(self.attn, "qkv", None), getattr(self.mlp, "fc1", None)
@@ -401,8 +547,11 @@ class Block(nn.Module):
                                  and not _watched(owner, reader)) else None
             return residual_norm(x, y, n.weight, n.bias, eps=n.eps, gamma=gamma, quantize=fmt)
 
+        drop = getattr(self, "drop_path", None)
         _, h = norm(self.norm1, self.attn, "qkv")
         a = self.attn(h)
+        if _active(drop):  # (a sample's draw and the layer scale commute)
+            a = drop(a)
         if torch.promote_types(a.dtype, x.dtype) == x.dtype:
             # (under autocast the branch comes in 16 bits: as wide as the sum it joins)
             y, h = norm(self.norm2, self.mlp, "fc1", a.to(x.dtype), self.ls1.gamma)
@@ -411,6 +560,9 @@ class Block(nn.Module):
             h = self.norm2(y)
         u = self.mlp(h)
         e = None if self.comp is None else self.comp(x).to(y.dtype)
+        if _active(drop):
+            y = self._add(y, self.ls2(u))
+            return y if e is None else y + e
         if self._fused_glue_applies(y) and u.dtype == torch.float32:
             return scale_residual(y, u.contiguous(), self.ls2.gamma, out=y,
                                   extra=None if e is None else e.contiguous())
@@ -420,7 +572,7 @@ class Block(nn.Module):
     def _fused_glue_applies(self, x: torch.Tensor) -> bool:
         return (FUSED_GLUE and x.is_cuda and x.dtype == torch.float32 and x.is_contiguous()
                 and not torch.is_grad_enabled() and not torch.is_autocast_enabled("cuda")
-                and not in_dual_level()
+                and not in_dual_level() and not _active(getattr(self, "drop_path", None))
                 and all(type(ls) is LayerScale and ls.gamma.dtype == torch.float32
                         for ls in (self.ls1, self.ls2)))
 
@@ -439,7 +591,8 @@ class Block(nn.Module):
         mlp = self.mlp
         ub = None
         if (type(mlp) is Mlp and _plain_linear(mlp.fc1) and _plain_linear(mlp.fc2)
-                and type(mlp.act) is nn.GELU and mlp.act.approximate == "none"):
+                and type(mlp.act) is nn.GELU and mlp.act.approximate == "none"
+                and not _active(getattr(mlp, "drop", None))):
             h2 = h.reshape(-1, h.shape[-1])
             t = bias_gelu_(torch.mm(h2, mlp.fc1.weight.t()), mlp.fc1.bias)
             u = torch.mm(t, mlp.fc2.weight.t())
@@ -459,7 +612,7 @@ class Block(nn.Module):
 class Backbone(nn.Module):
     def __init__(self, img: int = 224, patch: int = 14, dim: int = 1024, depth: int = 24,
                  heads: int = 16, hidden: int = 4096, ls_init: float = 1.0, rope: bool = False,
-                 rope_base: float = 10000.0):
+                 rope_base: float = 10000.0, qk_norm: Optional[str] = None):
         super().__init__()
         self.patch_embed = nn.Conv2d(3, dim, kernel_size=patch, stride=patch)
         n = (img // patch) ** 2
@@ -472,6 +625,9 @@ class Backbone(nn.Module):
             grid = GridRotary((img // patch, img // patch), dim // heads, base=rope_base)
             for b in self.blocks:
                 b.attn.rope = grid
+        if qk_norm is not None:  # "rms" or "layer"
+            for b in self.blocks:
+                b.attn.qk_norm = QKNorm(dim // heads, qk_norm)
         self.norm = nn.LayerNorm(dim, eps=1e-6)
 
     def forward(self, x):
@@ -612,6 +768,22 @@ def patch_vit(model: ViTClassifier, sc_prec: int, ops: Iterable[str] = ("qk", "a
 
 
 MX_OPS = ("qkv_proj", "out_proj", "mlp_fc1", "mlp_fc2")
+_WHERE = {"qkv_proj": ("attn", "qkv"), "out_proj": ("attn", "proj"), "mlp_fc1": ("mlp", "fc1"),
+          "mlp_fc2": ("mlp", "fc2")}
+
+
+def _patch_linears(model: ViTClassifier, ops: Iterable[str], make: Callable) -> dict:
+    ops = set(ops)
+    unknown = ops - set(MX_OPS)
+    if unknown:
+        raise ValueError(f"unknown ops {sorted(unknown)} (of {MX_OPS})")
+    stats = {op: 0 for op in MX_OPS}
+    for blk in model.backbone.blocks:
+        for op in ops:
+            owner = getattr(blk, _WHERE[op][0])
+            setattr(owner, _WHERE[op][1], make(getattr(owner, _WHERE[op][1])))
+            stats[op] += 1
+    return stats
 
 
 def patch_vit_mx(model: ViTClassifier, ops: Iterable[str] = MX_OPS, *,
@@ -621,16 +793,30 @@ def patch_vit_mx(model: ViTClassifier, ops: Iterable[str] = MX_OPS, *,
     on the GPU.  The norms in front of qkv_proj and mlp_fc1 then write their
     codes, except where a hook watches the norm or the module that reads them.
     Inference only."""
-    ops = set(ops)
-    unknown = ops - set(MX_OPS)
-    if unknown:
-        raise ValueError(f"unknown ops {sorted(unknown)} (of {MX_OPS})")
-    where = {"qkv_proj": ("attn", "qkv"), "out_proj": ("attn", "proj"), "mlp_fc1": ("mlp", "fc1"),
-             "mlp_fc2": ("mlp", "fc2")}
-    stats = {op: 0 for op in MX_OPS}
-    for blk in model.backbone.blocks:
-        for op in ops:
-            owner = getattr(blk, where[op][0])
-            setattr(owner, where[op][1], MXLinear(getattr(owner, where[op][1]), fmt))
-            stats[op] += 1
-    return stats
+    return _patch_linears(model, ops, lambda lin: MXLinear(lin, fmt))
+
+
+def patch_vit_fp8(model: ViTClassifier, ops: Iterable[str] = MX_OPS, *,
+                  train: bool = False) -> dict:
+    """Put the named linears of every block (the op names of ``patch_vit``) in 8
+    bits: ``fp8.FP8Linear`` from the present weights, which must be on the GPU, or
+    with ``train`` on the present parameters, which stay trainable."""
+    return _patch_linears(model, ops, lambda lin: FP8Linear(lin, train))
+
+
+def set_dropout(model: ViTClassifier, p: float = 0.0, drop_path=0.0, *, seed: int = 0) -> None:
+    """Dropout with probability ``p`` behind every block's projection and MLP, and
+    stochastic depth with probability ``drop_path`` (one number, or one per block) of
+    each branch, from one ``seed``; active in training mode.  0 takes them out."""
+    blocks = model.backbone.blocks
+    rates = [float(drop_path)] * len(blocks) if isinstance(drop_path, (int, float)) else [
+        float(r) for r in drop_path]
+    if len(rates) != len(blocks):
+        raise ValueError(f"{len(rates)} drop_path rates for {len(blocks)} blocks")
+    for i, (blk, rate) in enumerate(zip(blocks, rates)):
+        made = [Dropout(q, per=per, seed=seed, index=3 * i + j).to(blk.ls1.gamma.device).train(
+            blk.training) if q else None
+                for j, (q, per) in enumerate(((p, "element"), (p, "element"), (rate, "sample")))]
+        blk.attn.proj_drop = made[0] or nn.Identity()
+        blk.mlp.drop = made[1] or nn.Identity()
+        blk.drop_path = made[2]
