@@ -436,15 +436,12 @@ int scmp_split_qkv_norm(const scmp_qknorm_args *args, void *stream) {
   p.param_dtype = args->param_dtype;
   p.eps = args->eps;
   p.rms = args->rms != 0;
-  auto s = static_cast<cudaStream_t>(stream);
   void *const grads[4] = {args->dq_weight, args->dq_bias, args->dk_weight, args->dk_bias};
-  bool sums = false;
   if (x.inverse) {
     if (!args->x) return fail(SCMP_EINVAL, "x (the forward's qkv) must be non-NULL");
     if ((rc = check_elements({args->x}, x.dtype)) != SCMP_OK) return rc;
     p.x = args->x;
-    sums = grads[0] || grads[1] || grads[2] || grads[3];
-    if (sums) {
+    if (grads[0] || grads[1] || grads[2] || grads[3]) {
       const size_t need = scmp_split_qkv_norm_workspace(x.H, x.Hk, x.D);
       if (!args->workspace || args->workspace_bytes < need)
         return fail(SCMP_EWORKSPACE, "workspace needs %zu bytes, got %zu", need,
@@ -452,22 +449,18 @@ int scmp_split_qkv_norm(const scmp_qknorm_args *args, void *stream) {
       if (!aligned({args->workspace}, 4))
         return fail(SCMP_EINVAL, "workspace must be 4-byte aligned");
       p.part = static_cast<float *>(args->workspace);
+      for (int i = 0; i < 4; ++i) p.grads[i] = grads[i];
     }
   }
-  cudaError_t e = launch_qknorm(p, x.dtype, s);
+  const cudaError_t e = launch_qknorm(p, x.dtype, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return cuda_fail(e, "split_qkv_norm launch");
-  add_launches(1);
-  if (sums) {
-    if ((e = launch_qknorm_sum(p, grads, s)) != cudaSuccess)
-      return cuda_fail(e, "split_qkv_norm launch");
-    add_launches(1);
-  }
+  add_launches(p.part ? 2 : 1);
   return SCMP_OK;
 }
 
 size_t scmp_split_qkv_norm_workspace(int64_t H, int64_t Hk, int64_t D) {
   if (H < 1 || Hk < 1 || H > 65535 || Hk > 65535 || D < 1 || D > 256) return 0;
-  return (size_t)qknorm_bwd_blocks(H, Hk).qk * 2 * (size_t)D * sizeof(float);
+  return qknorm_part_floats(H, Hk, D) * sizeof(float);
 }
 
 int scmp_dropout(const scmp_dropout_args *args, void *stream) {
@@ -491,12 +484,13 @@ int scmp_dropout(const scmp_dropout_args *args, void *stream) {
   p.y = x.y;
   p.n = x.n;
   p.span = x.span;
-  p.seed = x.seed;
   p.offset = x.offset;
   p.state = x.state;
-  p.threshold = (uint64_t)nearbyint(x.p * 4294967296.0);
+  const uint64_t below = (uint64_t)nearbyint(x.p * 4294967296.0);  // draws below it are dropped
+  p.none = below == 0;
+  p.limit = (uint32_t)(below - 1);
   p.scale = x.p < 1.0 ? (float)(1.0 / (1.0 - x.p)) : 0.0f;
-  const cudaError_t e = launch_dropout(p, x.dtype, static_cast<cudaStream_t>(stream));
+  const cudaError_t e = launch_dropout(p, x.seed, x.dtype, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return cuda_fail(e, "dropout launch");
   add_launches(1);
   return SCMP_OK;

@@ -8,6 +8,7 @@
 // a second pass over the registers.
 #include "norm.cuh"
 
+#include "f32x2.cuh"
 #include "mx_common.cuh"
 
 namespace scmp {
@@ -68,34 +69,6 @@ template <typename T, int V> __device__ __forceinline__ void store_rounded(T *p,
     unpack16<T>(u, v + i);
   }
 }
-
-// Two fp32 operations in one instruction: rows of 16-bit types are bound by
-// instructions, not by HBM.
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-  float2 r;
-  asm("{\n.reg .b64 a, b;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\n"
-      "add.rn.f32x2 a, a, b;\nmov.b64 {%0, %1}, a;\n}\n"
-      : "=f"(r.x), "=f"(r.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return r;
-}
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-  float2 r;
-  asm("{\n.reg .b64 a, b;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\n"
-      "mul.rn.f32x2 a, a, b;\nmov.b64 {%0, %1}, a;\n}\n"
-      : "=f"(r.x), "=f"(r.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return r;
-}
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  float2 r;
-  asm("{\n.reg .b64 a, b, c;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nmov.b64 c, {%6, %7};\n"
-      "fma.rn.f32x2 a, a, b, c;\nmov.b64 {%0, %1}, a;\n}\n"
-      : "=f"(r.x), "=f"(r.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-  return r;
-}
-__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
 // The E values of a lane, chunk j's V from element j V on, as pairs.
 template <int E> struct Values {

@@ -11,6 +11,7 @@
 // row are shuffles inside the group, and a few heads are in flight at a time.  The
 // partner of a pair half a section apart is loaded again (from L1) and normalised
 // by its own weight.  HBM-bound: each element is read once and written once.
+#include "f32x2.cuh"
 #include "mx_common.cuh"
 #include "qknorm.cuh"
 #include "rotary_device.cuh"
@@ -19,19 +20,26 @@ namespace scmp {
 namespace {
 
 constexpr int kMaxD = 256;
+// Blocks of the backward pass on an SM, by the elements of a thread.
+__host__ __device__ constexpr int blocks_per_sm(int elements) { return elements > 4 ? 2 : 3; }
 
-// What a thread holds of one head row: kP pieces of V elements, piece i at element
-// (lane + i lanes) V of D.
+// A thread holds kP pieces of V elements of a head row, piece i at element (lane + i
+// lanes) V of D: E = V kP values, flat, as pairs.
 template <int V, int kP> struct Mine {
+  static constexpr int E = V * kP;
   int e0[kP], partner[kP];
   uint32_t mask[kP];  // elements that turn
   bool in[kP];
-  float c[kP][V], s[kP][V];
+};
+template <int E> struct Pairs {
+  float2 p[E / 2];
+  __device__ __forceinline__ float &operator[](int e) { return reinterpret_cast<float *>(p)[e]; }
 };
 
+// Pieces, and the cos and signed sin of their elements (1 and 0 where none turns).
 template <int V, int kP, bool kInterleaved, bool kBackward>
 __device__ __forceinline__ void set_up(const QkNormParams &p, uint32_t tok, uint32_t n, bool turns,
-                                       Mine<V, kP> &m) {
+                                       Mine<V, kP> &m, Pairs<V * kP> &c, Pairs<V * kP> &s) {
   const int lane = threadIdx.x & (p.lanes - 1);
 #pragma unroll
   for (int i = 0; i < kP; ++i) {
@@ -39,9 +47,20 @@ __device__ __forceinline__ void set_up(const QkNormParams &p, uint32_t tok, uint
     m.in[i] = m.e0[i] < p.r.D;
     m.mask[i] = 0;
     m.partner[i] = m.e0[i];
+    float ci[V], si[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      ci[j] = 1.0f;
+      si[j] = 0.0f;
+    }
     if (turns && m.in[i])
       m.mask[i] = angles_of<V, kInterleaved, kBackward>(p.r, p.r.pos_batched ? tok : n, m.e0[i],
-                                                        m.c[i], m.s[i], m.partner[i]);
+                                                        ci, si, m.partner[i]);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      c[i * V + j] = ci[j];
+      s[i * V + j] = si[j];
+    }
   }
 }
 
@@ -60,11 +79,21 @@ template <typename T, int V> __device__ __forceinline__ void zero(Piece<T, V> &x
     for (int i = 0; i < Piece<T, V>::kWords; ++i) x.u[i] = 0;
   }
 }
-template <typename T, int V> __device__ __forceinline__ void values(const Piece<T, V> &x, float *v) {
-  if constexpr (V == 1)
-    v[0] = to_f32(x.u[0]);
-  else
-    x.get(v);
+template <typename T, int V, int kP>
+__device__ __forceinline__ Pairs<V * kP> values(const Piece<T, V> (&x)[kP]) {
+  Pairs<V * kP> r;
+#pragma unroll
+  for (int i = 0; i < kP; ++i) {
+    if constexpr (V == 1) {
+      r[i] = to_f32(x[i].u[0]);
+    } else {
+      float v[V];
+      x[i].get(v);
+#pragma unroll
+      for (int j = 0; j < V; ++j) r[i * V + j] = v[j];
+    }
+  }
+  return r;
 }
 template <typename T, int V> __device__ __forceinline__ void store(T *p, const float *v) {
   Piece<T, V> x;
@@ -76,103 +105,118 @@ template <typename T, int V> __device__ __forceinline__ void store(T *p, const f
   }
   x.store(p);
 }
+// Every element's partner within a thread's pieces (pairs side by side).
+template <int E> __device__ __forceinline__ Pairs<E> swapped(const Pairs<E> &x) {
+  Pairs<E> r;
+#pragma unroll
+  for (int i = 0; i < E / 2; ++i) r.p[i] = make_float2(x.p[i].y, x.p[i].x);
+  return r;
+}
 
-// mean and 1 / deviation of A head rows (mean 0 for rms).
+// mean and 1 / deviation of A head rows (mean 0 for rms); the variance is a second
+// pass over the registers.
 template <typename T, int V, int kP, int A>
 __device__ __forceinline__ void statistics(const QkNormParams &p, const Piece<T, V> (&x)[A][kP],
                                            const Mine<V, kP> &m, float (&mean)[A],
                                            float (&rstd)[A]) {
+  constexpr int E = V * kP;
   const float inv = 1.0f / (float)p.r.D;
 #pragma unroll
   for (int q = 0; q < A; ++q) mean[q] = 0.0f;
   if (!p.rms) {
 #pragma unroll
-    for (int q = 0; q < A; ++q)
+    for (int q = 0; q < A; ++q) {
+      const Pairs<E> v = values<T, V, kP>(x[q]);
+      float2 t = v.p[0];
 #pragma unroll
-      for (int i = 0; i < kP; ++i) {
-        float v[V];
-        values<T, V>(x[q][i], v);
-#pragma unroll
-        for (int j = 0; j < V; ++j) mean[q] += v[j];  // (0 past D)
-      }
+      for (int i = 1; i < E / 2; ++i) t = add2(t, v.p[i]);  // (0 past D)
+      mean[q] = t.x + t.y;
+    }
     group_sum<A>(p.lanes, mean);
 #pragma unroll
     for (int q = 0; q < A; ++q) mean[q] *= inv;
   }
 #pragma unroll
   for (int q = 0; q < A; ++q) {
-    rstd[q] = 0.0f;
+    Pairs<E> v = values<T, V, kP>(x[q]);
+    if (!p.rms) {
 #pragma unroll
-    for (int i = 0; i < kP; ++i) {
-      if (!m.in[i]) continue;
-      float v[V];
-      values<T, V>(x[q][i], v);
+      for (int i = 0; i < E / 2; ++i) v.p[i] = add2(v.p[i], both(-mean[q]));
+      if (!p.whole) {
 #pragma unroll
-      for (int j = 0; j < V; ++j) rstd[q] = __fmaf_rn(v[j] - mean[q], v[j] - mean[q], rstd[q]);
+        for (int i = 0; i < kP; ++i)
+#pragma unroll
+          for (int j = 0; j < V; ++j)
+            if (!m.in[i]) v[i * V + j] = 0.0f;
+      }
     }
+    float2 t = mul2(v.p[0], v.p[0]);
+#pragma unroll
+    for (int i = 1; i < E / 2; ++i) t = fma2(v.p[i], v.p[i], t);
+    rstd[q] = t.x + t.y;
   }
   group_sum<A>(p.lanes, rstd);
 #pragma unroll
   for (int q = 0; q < A; ++q) rstd[q] = rsqrtf(__fmaf_rn(rstd[q], inv, p.eps));
 }
 
-// Heads in flight: eight fp32 elements per lane and head are 8 registers, twice.
+// Heads in flight: up to 32 bytes of x per thread.
 template <typename T, int V, int kP, bool kBackward>
 __host__ __device__ constexpr int at_once() {
-  return V * kP * (int)sizeof(T) > 16 || kBackward ? 2 : 4;
+  return kBackward ? (V * kP > 4 ? 1 : 2) : V * kP * (int)sizeof(T) > 16 ? 2 : 4;
 }
 
-// Element (token, head) row of q, k or v: [B, heads, N, D].
-template <typename T>
-__device__ __forceinline__ T *head_row(void *base, const RotaryParams &r, uint32_t b, uint32_t n,
-                                       int64_t heads, int h) {
-  return static_cast<T *>(base) + (((int64_t)b * heads + h) * r.N + n) * r.D;
-}
-
-// Heads [h0, h1) of role 0 (q), 1 (k) or 2 (v) of one token.
+// Heads [h0, h1) of role 0 (q), 1 (k) or 2 (v) of one token.  With the rotation's c
+// and s and the partner's weight w', an element of the output is
+//   rstd (x w c + x' w' s - mean (w c + w' s)) + b c + b' s,
+// whose products of weights and angles are made once per token.
 template <typename T, int V, int kP, bool kInterleaved>
 __device__ __forceinline__ void forward_heads(const QkNormParams &p, uint32_t tok, int role, int h0,
                                               int h1) {
-  constexpr int A = at_once<T, V, kP, false>();
+  constexpr int A = at_once<T, V, kP, false>(), E = V * kP;
+  constexpr bool kApart = !kInterleaved || V == 1;  // partners are other threads'
   const RotaryParams &r = p.r;
   const bool live = tok < (uint32_t)(r.B * r.N);
   if (!live) tok = (uint32_t)(r.B * r.N) - 1;
   const uint32_t b = r.tokens.quotient(tok), n = tok - b * (uint32_t)r.N;
-  Mine<V, kP> m;
-  set_up<V, kP, kInterleaved, false>(p, tok, n, role < 2 && r.axes > 0, m);
-  float w[kP][V], bias[kP][V], wo[kP][V], bo[kP][V];
-#pragma unroll
-  for (int i = 0; i < kP; ++i)
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      w[i][j] = wo[i][j] = 1.0f;
-      bias[i][j] = bo[i][j] = 0.0f;
-      if (role == 2 || !m.in[i]) continue;
-      const int o = kInterleaved && V > 1 ? m.e0[i] + (j ^ 1) : m.partner[i] + j;
-      w[i][j] = load_as_f32(p.weight[role], p.param_dtype, m.e0[i] + j);
-      wo[i][j] = load_as_f32(p.weight[role], p.param_dtype, o);
-      if (p.bias[role]) {
-        bias[i][j] = load_as_f32(p.bias[role], p.param_dtype, m.e0[i] + j);
-        bo[i][j] = load_as_f32(p.bias[role], p.param_dtype, o);
-      }
-    }
   const int64_t heads = role == 0 ? r.H : r.Hk;
   const int before = role == 0 ? 0 : (int)(role == 1 ? r.H : r.H + r.Hk);
-  void *const out = role == 0 ? r.q : role == 1 ? r.k : r.v;
-  const T *const fused = static_cast<const T *>(r.qkv) +
-                         ((int64_t)tok * (r.H + 2 * r.Hk) + before) * r.D;
-  for (int h = h0; h < h1; h += A) {
+  const T *from = static_cast<const T *>(r.qkv) +
+                  ((int64_t)tok * (r.H + 2 * r.Hk) + before + h0) * r.D;
+  const int64_t apart = r.N * r.D;  // of a token's rows in q, k and v
+  T *to = static_cast<T *>(role == 0 ? r.q : role == 1 ? r.k : r.v) +
+          (((int64_t)b * heads + h0) * r.N + n) * r.D;
+  Mine<V, kP> m;
+  Pairs<E> wc, ws, shift, c, s;
+  set_up<V, kP, kInterleaved, false>(p, tok, n, role < 2 && r.axes > 0, m, c, s);
+  if (role < 2) {
+#pragma unroll
+    for (int i = 0; i < kP; ++i)
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const int e = i * V + j, at = m.e0[i] + j;
+        const int o = kApart ? m.partner[i] + j : m.e0[i] + (j ^ 1);
+        wc[e] = ws[e] = shift[e] = 0.0f;
+        if (!m.in[i]) continue;
+        wc[e] = load_as_f32(p.weight[role], p.param_dtype, at) * c[e];
+        ws[e] = load_as_f32(p.weight[role], p.param_dtype, o) * s[e];
+        if (p.bias[role])
+          shift[e] = __fmaf_rn(load_as_f32(p.bias[role], p.param_dtype, at), c[e],
+                               load_as_f32(p.bias[role], p.param_dtype, o) * s[e]);
+      }
+  }
+  for (int h = h0; h < h1; h += A, from += A * r.D, to += A * apart) {
     Piece<T, V> x[A][kP], o[A][kP];
 #pragma unroll
     for (int q = 0; q < A; ++q) {
-      const T *row = fused + (int64_t)(h + q < h1 ? h + q : h1 - 1) * r.D;
+      const T *row = from + (h + q < h1 ? q : h1 - 1 - h) * r.D;
 #pragma unroll
       for (int i = 0; i < kP; ++i) {
         if (m.in[i])
           x[q][i].load(row + m.e0[i]);
         else
           zero<T, V>(x[q][i]);
-        if (!kInterleaved || V == 1) {
+        if (kApart) {
           if (m.mask[i])
             o[q][i].load(row + m.partner[i]);
           else
@@ -185,8 +229,7 @@ __device__ __forceinline__ void forward_heads(const QkNormParams &p, uint32_t to
       for (int q = 0; q < A; ++q)
 #pragma unroll
         for (int i = 0; i < kP; ++i)
-          if (live && h + q < h1 && m.in[i])
-            x[q][i].store(head_row<T>(out, r, b, n, heads, h + q) + m.e0[i]);
+          if (live && h + q < h1 && m.in[i]) x[q][i].store(to + q * apart + m.e0[i]);
       continue;
     }
     float mean[A], rstd[A];
@@ -194,25 +237,21 @@ __device__ __forceinline__ void forward_heads(const QkNormParams &p, uint32_t to
 #pragma unroll
     for (int q = 0; q < A; ++q) {
       if (h + q >= h1) break;
+      const Pairs<E> v = values<T, V, kP>(x[q]);
+      Pairs<E> u, y;
+      if constexpr (kApart)
+        u = values<T, V, kP>(o[q]);
+      else
+        u = swapped<E>(v);
 #pragma unroll
-      for (int i = 0; i < kP; ++i) {
-        float v[V], u[V];
-        values<T, V>(x[q][i], v);
-        if (!kInterleaved || V == 1) {
-          values<T, V>(o[q][i], u);
-        } else {
-#pragma unroll
-          for (int j = 0; j < V; ++j) u[j] = v[j ^ 1];
-        }
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          v[j] = __fmaf_rn((v[j] - mean[q]) * rstd[q], w[i][j], bias[i][j]);
-          u[j] = __fmaf_rn((u[j] - mean[q]) * rstd[q], wo[i][j], bo[i][j]);
-          if (m.mask[i] >> j & 1) v[j] = __fmaf_rn(v[j], m.c[i][j], u[j] * m.s[i][j]);
-        }
-        if (live && m.in[i])
-          store<T, V>(head_row<T>(out, r, b, n, heads, h + q) + m.e0[i], v);
+      for (int i = 0; i < E / 2; ++i) {
+        float2 t = fma2(v.p[i], wc.p[i], mul2(u.p[i], ws.p[i]));
+        if (!p.rms) t = fma2(both(-mean[q]), add2(wc.p[i], ws.p[i]), t);
+        y.p[i] = fma2(both(rstd[q]), t, shift.p[i]);
       }
+#pragma unroll
+      for (int i = 0; i < kP; ++i)
+        if (live && m.in[i]) store<T, V>(to + q * apart + m.e0[i], &y[i * V]);
     }
   }
 }
@@ -220,45 +259,49 @@ __device__ __forceinline__ void forward_heads(const QkNormParams &p, uint32_t to
 // The same heads' gradients; dw and db add up in the thread.
 template <typename T, int V, int kP, bool kInterleaved>
 __device__ __forceinline__ void backward_heads(const QkNormParams &p, uint32_t tok, int role,
-                                               int h0, int h1, float (&dw)[kP][V],
-                                               float (&db)[kP][V]) {
-  constexpr int A = at_once<T, V, kP, true>();
+                                               int h0, int h1, Pairs<V * kP> &dw,
+                                               Pairs<V * kP> &db) {
+  constexpr int A = at_once<T, V, kP, true>(), E = V * kP;
+  constexpr bool kApart = !kInterleaved || V == 1;
   const RotaryParams &r = p.r;
   const bool live = tok < (uint32_t)(r.B * r.N);
   if (!live) tok = (uint32_t)(r.B * r.N) - 1;
   const uint32_t b = r.tokens.quotient(tok), n = tok - b * (uint32_t)r.N;
+  const int64_t heads = role == 0 ? r.H : r.Hk;
+  const int before = role == 0 ? 0 : (int)(role == 1 ? r.H : r.H + r.Hk);
+  const int64_t at = ((int64_t)tok * (r.H + 2 * r.Hk) + before + h0) * r.D;
+  const T *from = static_cast<const T *>(p.x) + at;
+  T *to = static_cast<T *>(r.qkv) + at;
+  const int64_t apart = r.N * r.D;
+  const T *grad = static_cast<const T *>(role == 0 ? r.q : role == 1 ? r.k : r.v) +
+                  (((int64_t)b * heads + h0) * r.N + n) * r.D;
   Mine<V, kP> m;
-  set_up<V, kP, kInterleaved, true>(p, tok, n, role < 2 && r.axes > 0, m);
-  float w[kP][V];
+  Pairs<E> c, s, w;
+  set_up<V, kP, kInterleaved, true>(p, tok, n, role < 2 && r.axes > 0, m, c, s);
 #pragma unroll
   for (int i = 0; i < kP; ++i)
 #pragma unroll
     for (int j = 0; j < V; ++j)
-      w[i][j] = role < 2 && m.in[i] ? load_as_f32(p.weight[role], p.param_dtype, m.e0[i] + j) : 0.f;
-  const int64_t heads = role == 0 ? r.H : r.Hk;
-  const int before = role == 0 ? 0 : (int)(role == 1 ? r.H : r.H + r.Hk);
-  void *const from = role == 0 ? r.q : role == 1 ? r.k : r.v;
-  const int64_t at = ((int64_t)tok * (r.H + 2 * r.Hk) + before) * r.D;
-  const T *const fused = static_cast<const T *>(p.x) + at;
-  T *const out = static_cast<T *>(r.qkv) + at;
+      w[i * V + j] =
+          role < 2 && m.in[i] ? load_as_f32(p.weight[role], p.param_dtype, m.e0[i] + j) : 0.0f;
   const float inv = 1.0f / (float)r.D;
-  for (int h = h0; h < h1; h += A) {
+  for (int h = h0; h < h1; h += A, from += A * r.D, to += A * r.D, grad += A * apart) {
     Piece<T, V> x[A][kP], g[A][kP], o[A][kP];
 #pragma unroll
     for (int q = 0; q < A; ++q) {
-      const int hh = h + q < h1 ? h + q : h1 - 1;
-      const T *grad = head_row<const T>(from, r, b, n, heads, hh);
-      const T *row = fused + (int64_t)hh * r.D;
+      // (what counts for no row has gradients of zero)
+      const bool counts = live && h + q < h1;
+      const int64_t hh = h + q < h1 ? q : h1 - 1 - h;
 #pragma unroll
       for (int i = 0; i < kP; ++i) {
         zero<T, V>(x[q][i]);
         zero<T, V>(g[q][i]);
         zero<T, V>(o[q][i]);
         if (!m.in[i]) continue;
-        g[q][i].load(grad + m.e0[i]);
+        if (counts) g[q][i].load(grad + hh * apart + m.e0[i]);
         if (role == 2) continue;
-        x[q][i].load(row + m.e0[i]);
-        if ((!kInterleaved || V == 1) && m.mask[i]) o[q][i].load(grad + m.partner[i]);
+        x[q][i].load(from + hh * r.D + m.e0[i]);
+        if (kApart && counts && m.mask[i]) o[q][i].load(grad + hh * apart + m.partner[i]);
       }
     }
     if (role == 2) {
@@ -266,61 +309,47 @@ __device__ __forceinline__ void backward_heads(const QkNormParams &p, uint32_t t
       for (int q = 0; q < A; ++q)
 #pragma unroll
         for (int i = 0; i < kP; ++i)
-          if (live && h + q < h1 && m.in[i])
-            g[q][i].store(out + (int64_t)(h + q) * r.D + m.e0[i]);
+          if (live && h + q < h1 && m.in[i]) g[q][i].store(to + q * r.D + m.e0[i]);
       continue;
     }
-    float mean[A], rstd[A];
+    float mean[A], rstd[A], sum_gn[A], sum_g[A];
     statistics<T, V, kP, A>(p, x, m, mean, rstd);
-    float dt[A][kP][V], sum_gn[A], sum_g[A];
+    Pairs<E> norm[A], gw[A];
 #pragma unroll
     for (int q = 0; q < A; ++q) {
-      sum_gn[q] = sum_g[q] = 0.0f;
-      const bool counts = live && h + q < h1;
+      const Pairs<E> v = values<T, V, kP>(x[q]), t = values<T, V, kP>(g[q]);
+      Pairs<E> u;
+      if constexpr (kApart)
+        u = values<T, V, kP>(o[q]);
+      else
+        u = swapped<E>(t);
+      float2 gn = make_float2(0.f, 0.f), gs = gn;
 #pragma unroll
-      for (int i = 0; i < kP; ++i) {
-        float v[V], u[V], t[V];
-        values<T, V>(x[q][i], v);
-        values<T, V>(g[q][i], t);
-        if (!kInterleaved || V == 1) {
-          values<T, V>(o[q][i], u);
-        } else {
-#pragma unroll
-          for (int j = 0; j < V; ++j) u[j] = t[j ^ 1];
-        }
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const float y = m.mask[i] >> j & 1 ? __fmaf_rn(t[j], m.c[i][j], u[j] * m.s[i][j]) : t[j];
-          const float norm = (v[j] - mean[q]) * rstd[q];
-          dt[q][i][j] = y * w[i][j];
-          if (m.in[i]) {
-            sum_g[q] += dt[q][i][j];
-            sum_gn[q] = __fmaf_rn(dt[q][i][j], norm, sum_gn[q]);
-            if (counts) {
-              dw[i][j] = __fmaf_rn(y, norm, dw[i][j]);
-              db[i][j] += y;
-            }
-          }
-        }
+      for (int i = 0; i < E / 2; ++i) {
+        const float2 dt = fma2(t.p[i], c.p[i], mul2(u.p[i], s.p[i]));
+        norm[q].p[i] = mul2(add2(v.p[i], both(-mean[q])), both(rstd[q]));
+        gw[q].p[i] = mul2(dt, w.p[i]);  // (0 past D)
+        gn = fma2(gw[q].p[i], norm[q].p[i], gn);
+        gs = add2(gs, gw[q].p[i]);
+        dw.p[i] = fma2(dt, norm[q].p[i], dw.p[i]);
+        db.p[i] = add2(db.p[i], dt);
       }
+      sum_gn[q] = gn.x + gn.y;
+      sum_g[q] = gs.x + gs.y;
     }
     group_sum<A>(p.lanes, sum_gn);
     if (!p.rms) group_sum<A>(p.lanes, sum_g);
 #pragma unroll
     for (int q = 0; q < A; ++q) {
       if (h + q >= h1) break;
-      const float a = sum_gn[q] * inv, c = p.rms ? 0.0f : sum_g[q] * inv;
+      const float2 a = both(-sum_gn[q] * inv), d = both(p.rms ? 0.0f : -sum_g[q] * inv);
+      Pairs<E> y;
 #pragma unroll
-      for (int i = 0; i < kP; ++i) {
-        float v[V];
-        values<T, V>(x[q][i], v);
+      for (int i = 0; i < E / 2; ++i)
+        y.p[i] = mul2(fma2(norm[q].p[i], a, add2(gw[q].p[i], d)), both(rstd[q]));
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const float norm = (v[j] - mean[q]) * rstd[q];
-          v[j] = (dt[q][i][j] - c - norm * a) * rstd[q];
-        }
-        if (live && m.in[i]) store<T, V>(out + (int64_t)(h + q) * r.D + m.e0[i], v);
-      }
+      for (int i = 0; i < kP; ++i)
+        if (live && m.in[i]) store<T, V>(to + q * r.D + m.e0[i], &y[i * V]);
     }
   }
 }
@@ -351,7 +380,7 @@ __global__ void __launch_bounds__(kThreads)
 // Blocks [0, blocks_q) take q's units in turn, those up to blocks_qk k's, the rest
 // v's (then v's transposed tiles, a block each).
 template <typename T, int V, int kP, bool kInterleaved>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, blocks_per_sm(V * kP))
     qknorm_bwd_kernel(const __grid_constant__ QkNormParams p) {
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ float sums[kThreads / 32][2][kMaxD];
@@ -365,11 +394,9 @@ __global__ void __launch_bounds__(kThreads)
   const uint32_t blocks = (role == 0 ? p.blocks_q : role == 1 ? p.blocks_qk : p.blocks_all) - first;
   const int unit0 = role == 0 ? 0 : role == 1 ? p.units_q : p.units_qk;
   const uint32_t per = (role == 0 ? p.units_q : role == 1 ? p.units_qk : p.units_all) - unit0;
-  float dw[kP][V], db[kP][V];
+  Pairs<V * kP> dw, db;
 #pragma unroll
-  for (int i = 0; i < kP; ++i)
-#pragma unroll
-    for (int j = 0; j < V; ++j) dw[i][j] = db[i][j] = 0.0f;
+  for (int e = 0; e < V * kP; ++e) dw[e] = db[e] = 0.0f;
   for (uint64_t u = blockIdx.x - first; u < (uint64_t)p.token_blocks * per; u += blocks) {
     const uint32_t tb = (uint32_t)(u / per);
     int same, h0, h1;
@@ -385,13 +412,13 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       for (int o = p.lanes; o < 32; o <<= 1) {
-        dw[i][j] += __shfl_xor_sync(~0u, dw[i][j], o);
-        db[i][j] += __shfl_xor_sync(~0u, db[i][j], o);
+        dw[i * V + j] += __shfl_xor_sync(~0u, dw[i * V + j], o);
+        db[i * V + j] += __shfl_xor_sync(~0u, db[i * V + j], o);
       }
       const int e = ((lane & (p.lanes - 1)) + i * p.lanes) * V + j;
       if (lane < p.lanes && e < p.r.D) {
-        sums[warp][0][e] = dw[i][j];
-        sums[warp][1][e] = db[i][j];
+        sums[warp][0][e] = dw[i * V + j];
+        sums[warp][1][e] = db[i * V + j];
       }
     }
   __syncthreads();
@@ -437,6 +464,22 @@ __global__ void __launch_bounds__(kThreads) qknorm_sum_kernel(const __grid_const
     static_cast<__half *>(a.out[y])[d] = from_f32<__half>(t);
 }
 
+// As many blocks as run at once on the 148 SMs, shared out by heads: of q, of q and k,
+// of all.
+struct Blocks {
+  uint32_t q, qk, all;
+};
+Blocks bwd_blocks(int64_t H, int64_t Hk, int per_sm) {
+  const int64_t all = 148 * per_sm;
+  int64_t k = all * Hk / (H + 2 * Hk);
+  k = k < 1 ? 1 : k;
+  Blocks n;
+  n.q = (uint32_t)(all - 2 * k);
+  n.qk = n.q + (uint32_t)k;
+  n.all = n.qk + (uint32_t)k;
+  return n;
+}
+
 int units(int64_t heads, int per) { return (int)((heads + per - 1) / per); }
 
 template <typename T, int V, int kP, bool kInterleaved>
@@ -446,6 +489,7 @@ cudaError_t launch_p(QkNormParams p, cudaStream_t s) {
   const int pieces = (r.D / V + kP - 1) / kP;
   p.lanes = 1;
   while (p.lanes < pieces) p.lanes *= 2;
+  p.whole = p.lanes * kP * V == r.D;
   const int64_t tokens = r.B * r.N, per_block = kThreads / p.lanes;
   const int64_t token_blocks = (tokens + per_block - 1) / per_block;
   p.token_blocks = (uint32_t)token_blocks;
@@ -460,7 +504,7 @@ cudaError_t launch_p(QkNormParams p, cudaStream_t s) {
   const size_t smem = r.v_transposed ? (size_t)(kTile + 2) * r.D * sizeof(T) : 0;  // <= 66 KB
   int64_t blocks = token_blocks * p.units_all;
   if (r.inverse) {
-    const QkNormBlocks n = qknorm_bwd_blocks(r.H, r.Hk);
+    const Blocks n = bwd_blocks(r.H, r.Hk, blocks_per_sm(V * kP));
     p.blocks_q = n.q;
     p.blocks_qk = n.qk;
     p.blocks_all = r.v_transposed ? n.qk : n.all;
@@ -479,6 +523,18 @@ cudaError_t launch_p(QkNormParams p, cudaStream_t s) {
     if (e != cudaSuccess) return e;
   }
   kern<<<(unsigned)(blocks + tiles), kThreads, smem, s>>>(p);
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess || !p.part) return e;
+  SumArgs a;
+  a.part = p.part;
+  a.D = r.D;
+  a.dtype = p.param_dtype;
+  for (int y = 0; y < 4; ++y) {
+    a.out[y] = p.grads[y];
+    a.first[y] = y < 2 ? 0 : p.blocks_q;
+    a.last[y] = y < 2 ? p.blocks_q : p.blocks_qk;
+  }
+  qknorm_sum_kernel<<<dim3((unsigned)((r.D + 31) / 32), 4), kThreads, 0, s>>>(a);
   return cudaGetLastError();
 }
 template <typename T, int V, int kP>
@@ -501,37 +557,14 @@ template <typename T> cudaError_t launch(const QkNormParams &p, cudaStream_t s) 
 
 }  // namespace
 
-// Four blocks for each of the 148 SMs, shared out by heads.
-QkNormBlocks qknorm_bwd_blocks(int64_t H, int64_t Hk) {
-  constexpr int64_t kAll = 148 * 4;
-  int64_t k = kAll * Hk / (H + 2 * Hk);
-  k = k < 1 ? 1 : k;
-  QkNormBlocks n;
-  n.q = (uint32_t)(kAll - 2 * k);
-  n.qk = n.q + (uint32_t)k;
-  n.all = n.qk + (uint32_t)k;
-  return n;
+size_t qknorm_part_floats(int64_t H, int64_t Hk, int64_t D) {
+  return (size_t)bwd_blocks(H, Hk, blocks_per_sm(1)).qk * 2 * (size_t)D;
 }
 
 cudaError_t launch_qknorm(const QkNormParams &p, int dtype, cudaStream_t s) {
   if (dtype == SCMP_F32) return launch<float>(p, s);
   if (dtype == SCMP_BF16) return launch<__nv_bfloat16>(p, s);
   return launch<__half>(p, s);
-}
-
-cudaError_t launch_qknorm_sum(const QkNormParams &p, void *const (&grads)[4], cudaStream_t s) {
-  const QkNormBlocks n = qknorm_bwd_blocks(p.r.H, p.r.Hk);
-  SumArgs a;
-  a.part = p.part;
-  a.D = p.r.D;
-  a.dtype = p.param_dtype;
-  for (int y = 0; y < 4; ++y) {
-    a.out[y] = grads[y];
-    a.first[y] = y < 2 ? 0 : n.q;
-    a.last[y] = y < 2 ? n.q : n.qk;
-  }
-  qknorm_sum_kernel<<<dim3((unsigned)((p.r.D + 31) / 32), 4), kThreads, 0, s>>>(a);
-  return cudaGetLastError();
 }
 
 }  // namespace scmp

@@ -11,21 +11,17 @@ struct QkNormParams {
   const void *weight[2], *bias[2];  // of q, k: [D] of param_dtype; biases nullable
   int param_dtype;
   float eps;
-  bool rms;
+  bool rms, whole;  // whole (set by the launcher): the lanes hold exactly D elements
   float *part;  // inverse: [blocks of q, then of k][2][D] partial sums, nullable
+  void *grads[4];  // with part: of q's weight and bias, k's weight and bias, each nullable
   // set by the launcher: lanes per head row; heads per thread of a unit; units per
   // token block, of q, of q and k, of all; backward: blocks of q, of q and k, of all
   int lanes, heads_per, units_q, units_qk, units_all;
   uint32_t token_blocks, blocks_q, blocks_qk, blocks_all;
 };
-// Partial sums of a backward pass: blocks of q and of q and k.
-struct QkNormBlocks {
-  uint32_t q, qk, all;
-};
-QkNormBlocks qknorm_bwd_blocks(int64_t H, int64_t Hk);
-
+// Floats of workspace of a backward pass with gradients of parameters.
+size_t qknorm_part_floats(int64_t H, int64_t Hk, int64_t D);
+// One launch, two with part.
 cudaError_t launch_qknorm(const QkNormParams &p, int dtype, cudaStream_t s);
-// grads: of q's weight and bias, k's weight and bias (each nullable).
-cudaError_t launch_qknorm_sum(const QkNormParams &p, void *const (&grads)[4], cudaStream_t s);
 
 }  // namespace scmp

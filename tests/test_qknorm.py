@@ -378,11 +378,14 @@ def test_strides_streams_graph_empty_repeats(cuda_device):
     w = torch.randn(65, device=dev).half()
     kw = dict(axes=axes, pos=pos)
     big = torch.randn(2, 26, 200, device=dev).half()
-    for qkv in (big[..., 3:195], big[..., :192].contiguous(),
-                torch.randn(2 * 26 * 192 + 1, device=dev).half()[1:].view(2, 26, 192)):
+    for qkv in (big[..., 3:195], big[..., :192].contiguous()):
         got = split_qkv_norm(qkv, 2, w[::2][:32], w[1:33], **kw)
         ref = split_qkv_norm(qkv.clone(), 2, w[::2][:32].clone(), w[1:33].clone(), **kw)
         assert all(torch.equal(a, b) for a, b in zip(got, ref))
+    # an odd address takes narrower pieces, whose sums have another order
+    odd = torch.randn(2 * 26 * 192 + 1, device=dev).half()[1:].view(2, 26, 192)
+    grads = [torch.randn(2, 2, 26, 32, device=dev).half() for _ in range(3)]
+    check(odd, 2, 2, [w[::2][:32], w[1:33], None, None], "rms", 1e-6, axes, pos, True, grads)
     wc = w[:32].contiguous()
     ref = split_qkv_norm(qkv, 2, wc, wc, **kw)
     side = torch.cuda.Stream()
