@@ -42,11 +42,9 @@ constexpr uint32_t kFp8Nan = 0xFF;  // e8m0 NaN: a block that holds a NaN or an 
 // floating point), at most one of e4m3's 18 binades, and let the tensor core
 // apply them.
 __device__ __forceinline__ uint32_t fp8_scale(uint32_t amax) {
-  const uint32_t field = amax >> 23;
-  if (field == 0xFFu) return kFp8Nan;
-  const uint32_t up = (amax & 0x7FFFFFu) > 0x600000u ? 1u : 0u;  // significand above 1.75
-  const uint32_t e = field + up;                                 // exponent field of E + 8
-  return e > 8u ? e - 8u : 0u;
+  // a significand above 1.75 (0x600000) carries into the exponent field of E + 8
+  const uint32_t e = (amax + 0x1FFFFFu) >> 23;
+  return amax >= 0x7F800000u ? kFp8Nan : max(e, 8u) - 8u;
 }
 // What values are multiplied by before they are rounded: 2^-E, and NaN blocks by
 // 0 (their codes do not matter).  2^127 is a normal number, and code 0's; the

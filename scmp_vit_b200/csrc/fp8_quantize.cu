@@ -80,18 +80,45 @@ struct TileArgs {
   FastDiv tiles_c{1};
 };
 
-// Pitch of a transposed row in shared memory: 8-byte stores of a warp (16 columns
-// 8 apart, 2 row groups) and 16-byte loads of neighbours both go without conflicts
-// beyond their size.
-constexpr int kTilePitch = 128 + 16;
+// Largest magnitudes: 32-bit patterns of fp32, whose order is the numbers' with every
+// NaN above the infinities; pairs of 16-bit numbers as such, where a NaN wins too.
+template <typename T> struct Magnitude {
+  static constexpr int kWords = 8 * (int)sizeof(T) / 4;  // of eight elements
+  // of m (magnitudes) and the values of w
+  static __device__ __forceinline__ uint32_t most(uint32_t m, uint32_t w) {
+    if constexpr (sizeof(T) == 4) {
+      return max(m, w & 0x7FFFFFFFu);
+    } else if constexpr (__is_same(T, __nv_bfloat16)) {
+      const __nv_bfloat162 r = __hmax2_nan(*reinterpret_cast<const __nv_bfloat162 *>(&m),
+                                           __habs2(*reinterpret_cast<const __nv_bfloat162 *>(&w)));
+      return *reinterpret_cast<const uint32_t *>(&r);
+    } else {
+      const __half2 r = __hmax2_nan(*reinterpret_cast<const __half2 *>(&m),
+                                    __habs2(*reinterpret_cast<const __half2 *>(&w)));
+      return *reinterpret_cast<const uint32_t *>(&r);
+    }
+  }
+  // bits of the fp32 magnitude in the low half (or the word)
+  static __device__ __forceinline__ uint32_t bits(uint32_t m) {
+    if (sizeof(T) == 4) return m;
+    if (__is_same(T, __nv_bfloat16)) return m << 16;
+    return __float_as_uint(__half2float(__ushort_as_half((unsigned short)m)));
+  }
+};
 
 // Thread t holds rows 8 (t / 16) + i and columns 8 (t % 16) + j of the tile, i, j < 8.
+// The transpose is kept in shared memory as 128 rows of 16 pieces of 8 bytes, piece u
+// of row c at u ^ (c / 8 % 16): what 16 threads store at a time, 8 rows apart, and
+// what they load along a row both spread over all banks (in plain order the stores'
+// conflicts took the bf16 tile of 128 x 128 from 4 to 12 us).
 template <typename T, bool kVec, bool kSquare, bool kSums>
 __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : 3)
     fp8_tile_kernel(const T *__restrict__ x, const __grid_constant__ TileArgs a) {
-  __shared__ __align__(16) uint8_t turned[128 * kTilePitch];
-  __shared__ uint32_t warp_max[8][128];
-  __shared__ float warp_sum[kSums ? 8 : 1][128];
+  using Mag = Magnitude<T>;
+  constexpr int kWords = Mag::kWords;
+  __shared__ __align__(16) uint8_t turned[128 * 128];
+  __shared__ __align__(16) uint32_t warp_max[8][16 * kWords];
+  __shared__ __align__(16) float warp_sum[kSums ? 8 : 1][128];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int rg = threadIdx.x >> 4, piece = threadIdx.x & 15;
@@ -101,15 +128,19 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : 3)
   const int64_t rows = a.rows.rows, K = a.rows.K;
 
   // the tile, as loaded
-  constexpr int kWords = 2 * (int)sizeof(T);  // of eight elements
   uint32_t e[8][kWords];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const T *p = x + (r0 + i) * a.ld + c0;
     if (kVec && r0 + i < rows && c0 + 8 <= K) {
 #pragma unroll
-      for (int h = 0; h < kWords / 4; ++h)
-        *reinterpret_cast<uint4 *>(&e[i][4 * h]) = __ldg(reinterpret_cast<const uint4 *>(p) + h);
+      for (int h = 0; h < kWords / 4; ++h) {
+        const uint4 u = __ldg(reinterpret_cast<const uint4 *>(p) + h);
+        e[i][4 * h] = u.x;
+        e[i][4 * h + 1] = u.y;
+        e[i][4 * h + 2] = u.z;
+        e[i][4 * h + 3] = u.w;
+      }
     } else {
       T v[8];
 #pragma unroll
@@ -118,74 +149,113 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : 3)
       memcpy(e[i], v, sizeof(v));
     }
   }
-  const auto values = [&](int i, float *v) {
-    unpack16<T>(*reinterpret_cast<const uint4 *>(&e[i][0]), v);
-    if (sizeof(T) == 4) unpack16<T>(*reinterpret_cast<const uint4 *>(&e[i][kWords - 4]), v + 4);
+  // columns j and j + 1 (j even) of row i
+  const auto two = [&](int i, int j) {
+    if constexpr (sizeof(T) == 4)
+      return make_float2(__uint_as_float(e[i][j]), __uint_as_float(e[i][j + 1]));
+    else
+      return unpack2<T>(e[i][j / 2]);
   };
 
-  // largest magnitudes: of the thread's part of each row and each column
-  uint32_t row_max[8], col_max[8];
-  float sums[8];
+  // largest magnitudes: of the thread's part of each row and of each column
+  uint32_t row_max[8], col_max[kWords];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    col_max[j] = 0;
-    sums[j] = 0.0f;
-  }
+  for (int w = 0; w < kWords; ++w) col_max[w] = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    float v[8];
-    values(i, v);
-    row_max[i] = 0;
+    uint32_t m = 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint32_t bits = __float_as_uint(v[j]) & 0x7FFFFFFFu;
-      row_max[i] = max(row_max[i], bits);
-      col_max[j] = max(col_max[j], bits);
-      if (kSums) sums[j] += v[j];
+    for (int w = 0; w < kWords; ++w) {
+      m = Mag::most(m, e[i][w]);
+      col_max[w] = Mag::most(col_max[w], e[i][w]);
     }
+    row_max[i] = sizeof(T) == 4 ? m : Mag::most(m, __funnelshift_r(m, m, 16));
   }
   uint32_t row_scale[8], col_scale[8];
   if (kSquare) {
-    uint32_t m = 0;
+    uint32_t m = row_max[0];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, row_max[i]);
-    m = __reduce_max_sync(~0u, m);
+    for (int i = 1; i < 8; ++i) m = Mag::most(m, row_max[i]);
+    m = __reduce_max_sync(~0u, sizeof(T) == 4 ? m : m & 0xFFFFu);  // (a NaN's pattern is the largest)
     if (lane == 0) warp_max[0][warp] = m;
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < 8; ++w) m = max(m, warp_max[0][w]);
-    const uint32_t s = fp8_scale(m);
+    const uint32_t s = fp8_scale(Mag::bits(m));
 #pragma unroll
     for (int i = 0; i < 8; ++i) row_scale[i] = col_scale[i] = s;
   } else {
     if (a.data) {
+      if constexpr (sizeof(T) == 2) {  // two rows at a time
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < 8; i += 2) {
+          uint32_t m = __byte_perm(row_max[i], row_max[i + 1], 0x5410);
 #pragma unroll
-        for (int o = 1; o < 16; o <<= 1)
-          row_max[i] = max(row_max[i], __shfl_xor_sync(~0u, row_max[i], o));
-        row_scale[i] = fp8_scale(row_max[i]);
+          for (int o = 1; o < 16; o <<= 1) m = Mag::most(m, __shfl_xor_sync(~0u, m, o));
+          row_scale[i] = fp8_scale(Mag::bits(m & 0xFFFFu));
+          row_scale[i + 1] = fp8_scale(Mag::bits(m >> 16));
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          uint32_t m = row_max[i];
+#pragma unroll
+          for (int o = 1; o < 16; o <<= 1) m = max(m, __shfl_xor_sync(~0u, m, o));
+          row_scale[i] = fp8_scale(m);
+        }
       }
     }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      col_max[j] = max(col_max[j], __shfl_xor_sync(~0u, col_max[j], 16));
-      if (kSums) sums[j] += __shfl_xor_sync(~0u, sums[j], 16);
-    }
+    for (int w = 0; w < kWords; ++w)
+      col_max[w] = Mag::most(col_max[w], __shfl_xor_sync(~0u, col_max[w], 16));
     if (lane < 16) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        warp_max[warp][piece * 8 + j] = col_max[j];
-        if (kSums) warp_sum[warp][piece * 8 + j] = sums[j];
+      for (int w = 0; w < kWords; w += 4)
+        *reinterpret_cast<uint4 *>(&warp_max[warp][piece * kWords + w]) =
+            make_uint4(col_max[w], col_max[w + 1], col_max[w + 2], col_max[w + 3]);
+    }
+    if (kSums) {
+      float2 sums[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        sums[j] = two(0, 2 * j);
+#pragma unroll
+        for (int i = 1; i < 8; ++i) {
+          const float2 v = two(i, 2 * j);
+          sums[j].x += v.x;
+          sums[j].y += v.y;
+        }
+        sums[j].x += __shfl_xor_sync(~0u, sums[j].x, 16);
+        sums[j].y += __shfl_xor_sync(~0u, sums[j].y, 16);
+      }
+      if (lane < 16) {
+        float4 *to = reinterpret_cast<float4 *>(&warp_sum[warp][piece * 8]);
+        to[0] = make_float4(sums[0].x, sums[0].y, sums[1].x, sums[1].y);
+        to[1] = make_float4(sums[2].x, sums[2].y, sums[3].x, sums[3].y);
       }
     }
     __syncthreads();
+    if (a.t_data) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      uint32_t m = 0;
+      for (int w = 0; w < kWords; w += 4) {
+        uint4 m = make_uint4(0, 0, 0, 0);
 #pragma unroll
-      for (int w = 0; w < 8; ++w) m = max(m, warp_max[w][piece * 8 + j]);
-      col_scale[j] = fp8_scale(m);
+        for (int q = 0; q < 8; ++q) {
+          const uint4 v = *reinterpret_cast<const uint4 *>(&warp_max[q][piece * kWords + w]);
+          m = make_uint4(Mag::most(m.x, v.x), Mag::most(m.y, v.y), Mag::most(m.z, v.z),
+                         Mag::most(m.w, v.w));
+        }
+        const uint32_t ms[4] = {m.x, m.y, m.z, m.w};
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          if constexpr (sizeof(T) == 4) {
+            col_scale[w + q] = fp8_scale(ms[q]);
+          } else {
+            col_scale[2 * q] = fp8_scale(Mag::bits(ms[q] & 0xFFFFu));
+            col_scale[2 * q + 1] = fp8_scale(Mag::bits(ms[q] >> 16));
+          }
+        }
+      }
     }
     if (kSums && threadIdx.x < 128 && tile_c * 128 + threadIdx.x < K) {
       float t = 0.0f;
@@ -195,20 +265,25 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : 3)
     }
   }
 
+  const int live_r = (int)(rows - r0 < 8 ? rows - r0 : 8), live_c = (int)(K - c0 < 8 ? K - c0 : 8);
   if (a.data) {
+    uint8_t *to = a.data + r0 * a.rows.kp + c0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      float v[8];
-      values(i, v);
+    for (int i = 0; i < 8; ++i, to += a.rows.kp) {
       const float inv = fp8_inverse(row_scale[i]);
+      uint32_t codes[2];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] *= inv;
-      if (r0 + i < rows && c0 < a.rows.kp)
-        *reinterpret_cast<uint2 *>(a.data + (r0 + i) * a.rows.kp + c0) =
-            make_uint2(e4m3x4(v[0], v[1], v[2], v[3]), e4m3x4(v[4], v[5], v[6], v[7]));
-      if (piece == 0)
-        a.scales[fp8_scale_at(r0 + i, tile_c, a.rows.groups)] =
-            (uint8_t)(r0 + i < rows ? row_scale[i] : 0u);
+      for (int h = 0; h < 2; ++h) {
+        const float2 u = two(i, 4 * h), w = two(i, 4 * h + 2);
+        codes[h] = e4m3x4(u.x * inv, u.y * inv, w.x * inv, w.y * inv);
+      }
+      if (i < live_r)  // (columns up to the end of the block are the row's)
+        *reinterpret_cast<uint2 *>(to) = make_uint2(codes[0], codes[1]);
+    }
+    if (piece == 0) {  // (eight rows of a scale atom are 16 bytes apart)
+      uint8_t *at = a.scales + fp8_scale_at(r0, tile_c, a.rows.groups);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) at[16 * i] = (uint8_t)(i < live_r ? row_scale[i] : 0u);
     }
     // the last tile of a row also fills its last scale word
     if (tile_c == a.rows.blocks - 1 && threadIdx.x < 128)
@@ -219,58 +294,61 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : 3)
     // column j's eight rows are eight neighbouring bytes of the transpose
 #pragma unroll
     for (int j = 0; j < 8; j += 2) {
-      float u[8], w[8];
       const float iu = fp8_inverse(col_scale[j]), iw = fp8_inverse(col_scale[j + 1]);
+      uint32_t u[2], w[2];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        float v[8];
-        values(i, v);
-        u[i] = v[j] * iu;
-        w[i] = v[j + 1] * iw;
+      for (int h = 0; h < 2; ++h) {
+        const float2 p = two(4 * h, j), q = two(4 * h + 1, j), r = two(4 * h + 2, j),
+                     t = two(4 * h + 3, j);
+        u[h] = e4m3x4(p.x * iu, q.x * iu, r.x * iu, t.x * iu);
+        w[h] = e4m3x4(p.y * iw, q.y * iw, r.y * iw, t.y * iw);
       }
-      uint8_t *at = turned + (piece * 8 + j) * kTilePitch + rg * 8;
-      *reinterpret_cast<uint2 *>(at) =
-          make_uint2(e4m3x4(u[0], u[1], u[2], u[3]), e4m3x4(u[4], u[5], u[6], u[7]));
-      *reinterpret_cast<uint2 *>(at + kTilePitch) =
-          make_uint2(e4m3x4(w[0], w[1], w[2], w[3]), e4m3x4(w[4], w[5], w[6], w[7]));
+      uint8_t *at = turned + (piece * 8 + j) * 128 + (rg ^ piece) * 8;
+      *reinterpret_cast<uint2 *>(at) = make_uint2(u[0], u[1]);
+      *reinterpret_cast<uint2 *>(at + 128) = make_uint2(w[0], w[1]);
     }
     if (rg == 0) {
+      uint8_t *to = a.t_scales + fp8_scale_at(c0, tile_r, a.cols.groups);
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        a.t_scales[fp8_scale_at(c0 + j, tile_r, a.cols.groups)] =
-            (uint8_t)(c0 + j < K ? col_scale[j] : 0u);
+      for (int j = 0; j < 8; ++j) to[16 * j] = (uint8_t)(j < live_c ? col_scale[j] : 0u);
     }
     if (tile_r == a.cols.blocks - 1 && threadIdx.x < 128)
       for (int64_t b = a.cols.blocks; b < a.cols.groups * 4; ++b)
         a.t_scales[fp8_scale_at(tile_c * 128 + threadIdx.x, b, a.cols.groups)] = 0;
     __syncthreads();
+    const int m = threadIdx.x & 7, left = (int)(K - tile_c * 128 < 128 ? K - tile_c * 128 : 128);
+    uint8_t *to = a.t_data + (tile_c * 128 + (threadIdx.x >> 3)) * a.cols.kp + tile_r * 128 + m * 16;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int q = threadIdx.x + i * kThreads, c = q >> 3, m = (q & 7) * 16;
-      if (tile_c * 128 + c < K && tile_r * 128 + m < a.cols.kp)
-        *reinterpret_cast<uint4 *>(a.t_data + (tile_c * 128 + c) * a.cols.kp + tile_r * 128 + m) =
-            *reinterpret_cast<const uint4 *>(turned + c * kTilePitch + m);
+    for (int i = 0; i < 4; ++i, to += 32 * a.cols.kp) {
+      const int c = (threadIdx.x >> 3) + i * 32, at = c >> 3;
+      uint4 v = *reinterpret_cast<const uint4 *>(turned + c * 128 + (m ^ at >> 1) * 16);
+      if (at & 1) v = make_uint4(v.z, v.w, v.x, v.y);
+      if (c < left) *reinterpret_cast<uint4 *>(to) = v;
     }
   }
 }
 
 // Sums of columns over the tiles' parts, in a fixed order.
 template <typename T>
-__global__ void __launch_bounds__(128)
+__global__ void __launch_bounds__(512)
     fp8_sum_kernel(const float *__restrict__ sums, int64_t parts, int64_t K, T *__restrict__ out) {
-  // 32 columns, four threads each: part p of a column goes to thread p % 4
-  __shared__ float part[4][32];
+  // 32 columns, a thread of each of 16 warps: part p of a column goes to warp p % 16
+  __shared__ float part[16][32];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int64_t c = (int64_t)blockIdx.x * 32 + lane;
   float t = 0.0f;
   if (c < K) {
 #pragma unroll 8
-    for (int64_t p = w; p < parts; p += 4) t += sums[p * K + c];
+    for (int64_t p = w; p < parts; p += 16) t += sums[p * K + c];
   }
   part[w][lane] = t;
   __syncthreads();
-  if (w == 0 && c < K)
-    out[c] = from_f32<T>((part[0][lane] + part[1][lane]) + (part[2][lane] + part[3][lane]));
+  if (w == 0 && c < K) {
+    t = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) t += part[i][lane];
+    out[c] = from_f32<T>(t);
+  }
 }
 
 // ------------------------------------------------------------------- back
@@ -422,12 +500,12 @@ cudaError_t launch_fp8_sum_columns(const float *sums, int64_t parts, int64_t K, 
                                    int dtype, cudaStream_t s) {
   const unsigned grid = (unsigned)((K + 31) / 32);
   if (dtype == SCMP_F32)
-    fp8_sum_kernel<float><<<grid, 128, 0, s>>>(sums, parts, K, static_cast<float *>(out));
+    fp8_sum_kernel<float><<<grid, 512, 0, s>>>(sums, parts, K, static_cast<float *>(out));
   else if (dtype == SCMP_BF16)
     fp8_sum_kernel<__nv_bfloat16>
-        <<<grid, 128, 0, s>>>(sums, parts, K, static_cast<__nv_bfloat16 *>(out));
+        <<<grid, 512, 0, s>>>(sums, parts, K, static_cast<__nv_bfloat16 *>(out));
   else
-    fp8_sum_kernel<__half><<<grid, 128, 0, s>>>(sums, parts, K, static_cast<__half *>(out));
+    fp8_sum_kernel<__half><<<grid, 512, 0, s>>>(sums, parts, K, static_cast<__half *>(out));
   return cudaGetLastError();
 }
 
