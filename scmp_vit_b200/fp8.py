@@ -51,8 +51,8 @@ class FP8Tensor:
     (for the record: both have one layout); ``dtype`` is the type of the tensor it
     was made from, which products of it come out in by default."""
 
-    __slots__ = ("shape", "rows", "blocks", "dtype", "data", "scales", "data_ptr", "scales_ptr",
-                 "index")
+    __slots__ = ("shape", "rows", "blocks", "dtype", "_data", "_scales", "_buf", "data_ptr",
+                 "scales_ptr", "index")
 
     def __init__(self, data: torch.Tensor, scales: torch.Tensor, shape: Sequence[int],
                  blocks: str = "row", dtype: torch.dtype = torch.float32):
@@ -68,13 +68,31 @@ class FP8Tensor:
             raise ValueError(f"data on {data.device}, scales on {scales.device}")
         if data.data_ptr() % 16 or scales.data_ptr() % 16:
             raise ValueError("data and scales must be 16-byte aligned")
-        self.data, self.scales = data, scales
-        self.data_ptr, self.scales_ptr = data.data_ptr(), scales.data_ptr()
-        self.index, self.shape, self.blocks, self.dtype = data.get_device(), shape, blocks, dtype
+        self._set(data, scales, None, data.data_ptr(), scales.data_ptr(), data.get_device(), shape,
+                  self.rows, blocks, dtype)
+
+    def _set(self, data, scales, buf, data_ptr, scales_ptr, index, shape, rows, blocks, dtype):
+        self._data, self._scales, self._buf = data, scales, buf
+        self.data_ptr, self.scales_ptr, self.index = data_ptr, scales_ptr, index
+        self.shape, self.rows, self.blocks, self.dtype = shape, rows, blocks, dtype
+        return self
+
+    @property
+    def data(self) -> torch.Tensor:
+        if self._data is None:
+            self._data = self._buf[:_sizes(self.rows, self.shape[-1])[0]]
+        return self._data
+
+    @property
+    def scales(self) -> torch.Tensor:
+        if self._scales is None:
+            at = self.scales_ptr - self.data_ptr
+            self._scales = self._buf[at:at + _sizes(self.rows, self.shape[-1])[1]]
+        return self._scales
 
     @property
     def device(self) -> torch.device:
-        return self.data.device
+        return (self._data if self._buf is None else self._buf).device
 
     @property
     def is_cuda(self) -> bool:
@@ -93,7 +111,9 @@ class FP8Tensor:
         shape = torch.empty(self.shape, device="meta").reshape(*shape).shape
         if not shape or shape[-1] != self.shape[-1]:
             raise ValueError("an FP8Tensor keeps its last dimension")
-        return FP8Tensor(self.data, self.scales, shape, self.blocks, self.dtype)
+        return FP8Tensor.__new__(FP8Tensor)._set(
+            self._data, self._scales, self._buf, self.data_ptr, self.scales_ptr, self.index, shape,
+            self.rows, self.blocks, self.dtype)
 
     def dequantize(self, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
         """The values that the codes stand for, ``[..., K]`` (default: the type
@@ -115,10 +135,13 @@ class FP8Tensor:
 def fp8_empty(shape: Sequence[int], device: torch.device, dtype: torch.dtype,
               blocks: str = "row") -> FP8Tensor:
     """An FP8Tensor whose codes and scales (one allocation) are still to be written."""
-    data, scales = _sizes(math.prod(shape[:-1]), shape[-1])
-    at = (data + 255) & ~255
-    buf = torch.empty(at + scales, dtype=torch.uint8, device=device)
-    return FP8Tensor(buf[:data], buf[at:], shape, blocks, dtype)
+    shape = torch.Size(shape)
+    rows = math.prod(shape[:-1])
+    data, scales = _sizes(rows, shape[-1])
+    buf = torch.empty(data + scales, dtype=torch.uint8, device=device)
+    ptr = buf.data_ptr()  # (rows of codes are whole 128-byte blocks: the scales are aligned)
+    return FP8Tensor.__new__(FP8Tensor)._set(None, None, buf, ptr, ptr + data, buf.get_device(),
+                                             shape, rows, blocks, dtype)
 
 
 def fp8_quantize(x: torch.Tensor, blocks: str = "row", *, transpose: bool = False
@@ -177,13 +200,18 @@ def fp8_matmul(a: Union[torch.Tensor, FP8Tensor], b: FP8Tensor, *,
         raise ValueError(f"operands on different devices: {a.device} vs {b.device}")
     if len(a.shape) < 1 or a.shape[-1] != K:
         raise ValueError(f"inner-dim mismatch: a {tuple(a.shape)}, b {tuple(b.shape)}")
-    qa = a
+    codes = None  # of a plain a: freed to the stream's later calls when this one returns
+    a_ptr = a_scales_ptr = 0
     if plain:
         x_code = _check_input(a, "fp8_matmul")
         rows = a.numel() // K
-        qa = None if _thin(rows, N, K) else fp8_empty(a.shape, a.device, a.dtype)
+        if not _thin(rows, N, K):
+            data, scales = _sizes(rows, K)
+            codes = torch.empty(data + scales, dtype=torch.uint8, device=a.device)
+            a_ptr = codes.data_ptr()
+            a_scales_ptr = a_ptr + data
     else:
-        rows = a.rows
+        rows, a_ptr, a_scales_ptr = a.rows, a.data_ptr, a.scales_ptr
     _no_grad_wanted("fp8_matmul", a if plain else None, bias, out)
     shape = (*a.shape[:-1], N)
     given = out is not None
@@ -205,9 +233,8 @@ def fp8_matmul(a: Union[torch.Tensor, FP8Tensor], b: FP8Tensor, *,
         bias = bias if bias.is_contiguous() else bias.detach().contiguous()
         bias_ptr = bias.data_ptr()
     args = _lib.PACK_FP8_MATMUL.pack(
-        _lib.ABI_VERSION, bias_code, 0 if qa is None else qa.data_ptr,
-        0 if qa is None else qa.scales_ptr, b.data_ptr, b.scales_ptr, rows, N, K, bias_ptr,
-        out.data_ptr(), out_code, 0)
+        _lib.ABI_VERSION, bias_code, a_ptr, a_scales_ptr, b.data_ptr, b.scales_ptr, rows, N, K,
+        bias_ptr, out.data_ptr(), out_code, 0)
     if plain:
         x, ld = _rows_of(a)
         call(_lib.load().scmp_fp8_linear, index, x.data_ptr(), x_code, ld, args)
@@ -234,38 +261,41 @@ def _train_sizes(M: int, N: int, K: int) -> Tuple[int, int, int, int]:
 
 
 def _train_forward(x, weight, bias, save_x: bool, save_weight: bool):
-    """(y, codes of x^T or None, codes of weight^T or None)."""
+    """(y, codes of x^T and of weight^T in one buffer or None, where the second begins)."""
     N, K = weight.shape
     y = torch.empty((*x.shape[:-1], N), dtype=x.dtype, device=x.device)
     index = x.get_device()
     xr, ld = _rows_of(x)
     M = x.numel() // K
     if M == 0:
-        return y, None, None
+        return y, None, 0
     wr, weight_ld = _rows_of(weight)
     bias = bias if bias is None or bias.is_contiguous() else bias.detach().contiguous()
     workspace, _, x_bytes, w_bytes = _train_sizes(M, N, K)
     ws = torch.empty(workspace, dtype=torch.uint8, device=x.device)
-    saved_x = torch.empty(x_bytes, dtype=torch.uint8, device=x.device) if save_x else None
-    saved_w = torch.empty(w_bytes, dtype=torch.uint8, device=x.device) if save_weight else None
+    x_bytes = x_bytes if save_x else 0  # (multiples of 256)
+    saved, ptr = None, 0
+    if save_x or save_weight:
+        saved = torch.empty(x_bytes + (w_bytes if save_weight else 0), dtype=torch.uint8,
+                            device=x.device)
+        ptr = saved.data_ptr()
     args = _lib.PACK_FP8_TRAIN.pack(
         _lib.ABI_VERSION, DTYPE[x.dtype], DTYPE[weight.dtype],
         0 if bias is None else DTYPE[bias.dtype], xr.data_ptr(), wr.data_ptr(),
         0 if bias is None else bias.data_ptr(), y.data_ptr(),
-        0 if saved_x is None else saved_x.data_ptr(),
-        0 if saved_w is None else saved_w.data_ptr(), ws.data_ptr(), workspace, M, N, K, ld,
-        weight_ld)
+        ptr if save_x else 0, ptr + x_bytes if save_weight else 0, ws.data_ptr(), workspace, M, N,
+        K, ld, weight_ld)
     call(_lib.load().scmp_fp8_train_forward, index, args)
-    return y, saved_x, saved_w
+    return y, saved, x_bytes
 
 
 class _FP8Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias):
         wants = ctx.needs_input_grad
-        y, saved_x, saved_w = _train_forward(x, weight, bias, wants[1], wants[0])
+        y, saved, ctx.weight_at = _train_forward(x, weight, bias, wants[1], wants[0])
         # (codes alone: nothing of x or weight is kept for the backward pass)
-        ctx.save_for_backward(saved_x, saved_w)
+        ctx.save_for_backward(saved)
         ctx.like = (x.shape, weight.shape, x.dtype, weight.dtype,
                     None if bias is None else bias.dtype)
         return y
@@ -273,7 +303,7 @@ class _FP8Linear(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        saved_x, saved_w = ctx.saved_tensors
+        (saved,) = ctx.saved_tensors
         x_shape, (N, K), dtype, weight_dtype, bias_dtype = ctx.like
         wants, device = ctx.needs_input_grad, dy.device
         M = math.prod(x_shape[:-1])
@@ -284,12 +314,12 @@ class _FP8Linear(torch.autograd.Function):
         if M:
             dyr, ld = _rows_of(dy)
             size = _train_sizes(M, N, K)[1]
+            ptr = 0 if saved is None else saved.data_ptr()
             ws = torch.empty(size, dtype=torch.uint8, device=device)
             args = _lib.PACK_FP8_TRAIN_BWD.pack(
                 _lib.ABI_VERSION, DTYPE[dtype], DTYPE[weight_dtype],
                 0 if db is None else DTYPE[bias_dtype], dyr.data_ptr(),
-                0 if saved_x is None else saved_x.data_ptr(),
-                0 if saved_w is None else saved_w.data_ptr(),
+                ptr if wants[1] else 0, ptr + ctx.weight_at if wants[0] else 0,
                 *[0 if t is None else t.data_ptr() for t in (dx, dw, db)], ws.data_ptr(), size,
                 M, N, K, ld)
             call(_lib.load().scmp_fp8_train_backward, dy.get_device(), args)

@@ -349,3 +349,20 @@ def test_in_the_blocks(cuda_device, fused):
         assert all(p.grad is None or bool(p.grad.isfinite().all()) for p in m.parameters())
     finally:
         vit.set_fused_norm(False)
+
+
+@pytest.mark.gpu
+def test_more_elements_than_32_bits(cuda_device):
+    """Past 2^31 elements counters are 64 bits wide; the ends and the middle."""
+    n = (1 << 31) + 40
+    if torch.cuda.mem_get_info()[0] < 6 * n:
+        pytest.skip("needs 13 GB of device memory")
+    x = torch.ones(n, dtype=torch.bfloat16, device=cuda_device)
+    y = vit.dropout(x, 0.5, 21, 22)
+    z = vit.dropout(x.view(8, n // 8), 0.5, 21, 22, per="sample")
+    row = words(8, 21, 22)
+    for at in (0, 1 << 30, (1 << 31) - 20, n - 36):
+        keep = torch.from_numpy(words(36, 21, 22, at) >= np.uint64(1 << 31))
+        assert torch.equal(y[at:at + 36].cpu() != 0, keep)
+        assert torch.equal(z.view(-1)[at:at + 36].cpu() != 0, torch.from_numpy(
+            row[np.arange(at, at + 36) // (n // 8)] >= np.uint64(1 << 31)))
