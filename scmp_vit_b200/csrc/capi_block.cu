@@ -460,7 +460,7 @@ int scmp_split_qkv_norm(const scmp_qknorm_args *args, void *stream) {
 
 size_t scmp_split_qkv_norm_workspace(int64_t H, int64_t Hk, int64_t D) {
   if (H < 1 || Hk < 1 || H > 65535 || Hk > 65535 || D < 1 || D > 256) return 0;
-  return qknorm_part_floats(H, Hk, D) * sizeof(float);
+  return qknorm_part_floats(D) * sizeof(float);
 }
 
 int scmp_dropout(const scmp_dropout_args *args, void *stream) {

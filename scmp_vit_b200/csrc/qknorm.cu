@@ -6,11 +6,13 @@
 //   du = (g - mean(g) - n mean(g n)) / sqrt(var + eps)     (rms: without mean(g))
 // Statistics are fp32 and not stored: the backward pass reads u in any case.
 //
-// A group of 1 to 32 lanes owns a token and walks its heads: cos, sin and the
-// weights stay in registers, a head's row is one piece per lane, sums over the
-// row are shuffles inside the group, and a few heads are in flight at a time.  The
-// partner of a pair half a section apart is loaded again (from L1) and normalised
-// by its own weight.  HBM-bound: each element is read once and written once.
+// A group of 1 to 32 lanes owns a token and walks some of its heads (a unit is a
+// block's tokens by those heads): cos and sin stay in registers, a lane holds 4 or 8
+// elements of a head row, sums over the row are shuffles inside the group, and a few
+// heads are in flight at a time.  The partner of a pair half a section apart is loaded
+// again (from L1).  Weights are kept in shared memory in fp32.  What fp32 rows are
+// bound by is HBM, each element read once and written once; 16-bit rows are bound by
+// instructions, so sums and products go two at a time.
 #include "f32x2.cuh"
 #include "mx_common.cuh"
 #include "qknorm.cuh"
@@ -20,48 +22,199 @@ namespace scmp {
 namespace {
 
 constexpr int kMaxD = 256;
-// Blocks of the backward pass on an SM, by the elements of a thread.
-__host__ __device__ constexpr int blocks_per_sm(int elements) { return elements > 4 ? 2 : 3; }
 
-// A thread holds kP pieces of V elements of a head row, piece i at element (lane + i
-// lanes) V of D: E = V kP values, flat, as pairs.
-template <int V, int kP> struct Mine {
-  static constexpr int E = V * kP;
-  int e0[kP], partner[kP];
-  uint32_t mask[kP];  // elements that turn
-  bool in[kP];
+// E elements of a head row per lane: x and the outputs are accessed L at a time, the
+// pairs' partners (half a section apart) and the angles V at a time, V dividing L.
+// Lanes hold E consecutive elements; single ones (V = 1) lie a lane apart instead.
+template <typename T_, int L_, int V_, int E_, bool kInterleaved_> struct Form {
+  using T = T_;
+  static constexpr int L = L_, V = V_, E = E_, kLoads = E_ / L_, kPieces = E_ / V_;
+  static constexpr bool kInterleaved = kInterleaved_, kApart = !kInterleaved_ || V_ == 1;
+  static __device__ __forceinline__ int element(int lane, int lanes, int e) {
+    return V == 1 ? lane + e * lanes : lane * E + e;
+  }
 };
+
 template <int E> struct Pairs {
   float2 p[E / 2];
   __device__ __forceinline__ float &operator[](int e) { return reinterpret_cast<float *>(p)[e]; }
 };
 
-// Pieces, and the cos and signed sin of their elements (1 and 0 where none turns).
-template <int V, int kP, bool kInterleaved, bool kBackward>
-__device__ __forceinline__ void set_up(const QkNormParams &p, uint32_t tok, uint32_t n, bool turns,
-                                       Mine<V, kP> &m, Pairs<V * kP> &c, Pairs<V * kP> &s) {
-  const int lane = threadIdx.x & (p.lanes - 1);
+// E elements as loaded, N at a time.
+template <typename T, int E, int N> struct Raw {
+  Piece<T, N> u[E / N];
+  __device__ __forceinline__ void zero(int i) {
+    if constexpr (N == 1) {
+      u[i].u[0] = from_f32<T>(0.0f);
+    } else {
 #pragma unroll
-  for (int i = 0; i < kP; ++i) {
-    m.e0[i] = (lane + i * p.lanes) * V;
-    m.in[i] = m.e0[i] < p.r.D;
-    m.mask[i] = 0;
-    m.partner[i] = m.e0[i];
-    float ci[V], si[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      ci[j] = 1.0f;
-      si[j] = 0.0f;
-    }
-    if (turns && m.in[i])
-      m.mask[i] = angles_of<V, kInterleaved, kBackward>(p.r, p.r.pos_batched ? tok : n, m.e0[i],
-                                                        ci, si, m.partner[i]);
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      c[i * V + j] = ci[j];
-      s[i * V + j] = si[j];
+      for (int w = 0; w < Piece<T, N>::kWords; ++w) u[i].u[w] = 0;
     }
   }
+  __device__ __forceinline__ Pairs<E> values() const {
+    Pairs<E> r;
+#pragma unroll
+    for (int i = 0; i < E / N; ++i) {
+      if constexpr (N == 1) {
+        r[i] = to_f32(u[i].u[0]);
+      } else {
+        float v[N];
+        u[i].get(v);
+#pragma unroll
+        for (int j = 0; j < N; ++j) r[i * N + j] = v[j];
+      }
+    }
+    return r;
+  }
+  __device__ __forceinline__ void set(Pairs<E> &v) {
+#pragma unroll
+    for (int i = 0; i < E / N; ++i) {
+      if constexpr (N == 1) {
+        u[i].u[0] = from_f32<T>(v[i]);
+      } else {
+#pragma unroll
+        for (int w = 0; w < Piece<T, N>::kWords; ++w)
+          u[i].u[w] = Piece<T, N>::word(&v[i * N], w);
+      }
+    }
+  }
+};
+
+// Every element's partner within a thread's pieces (pairs side by side).
+template <int E> __device__ __forceinline__ Pairs<E> swapped(const Pairs<E> &x) {
+  Pairs<E> r;
+#pragma unroll
+  for (int i = 0; i < E / 2; ++i) r.p[i] = make_float2(x.p[i].y, x.p[i].x);
+  return r;
+}
+
+// What a thread's elements are, for every token: where they lie, and the section of
+// an axis that each piece belongs to.
+template <typename F> struct Lane {
+  int at[F::kLoads];                  // first element of each load
+  bool in[F::kLoads];                 // below D
+  int partner[F::kPieces];            // first element of each piece's partners
+  int axis[F::kPieces];               // -1: turned by none
+  const float2 *table[F::kPieces];    // the piece's first cos and sin at coordinate 0
+  int half[F::kPieces], size[F::kPieces];  // the axis's table: [size][half]
+  bool second[F::kPieces];            // of a pair's members (V = 1 or apart)
+
+  __device__ __forceinline__ Lane(const QkNormParams &p) {
+    const int lane = threadIdx.x & (p.lanes - 1);
+#pragma unroll
+    for (int i = 0; i < F::kLoads; ++i) {
+      at[i] = F::element(lane, p.lanes, i * F::L);
+      in[i] = at[i] < p.r.D;
+    }
+#pragma unroll
+    for (int i = 0; i < F::kPieces; ++i) {
+      const int e = F::element(lane, p.lanes, i * F::V);
+      partner[i] = e;
+      axis[i] = -1;
+      table[i] = p.r.table;
+      half[i] = size[i] = 0;
+      second[i] = false;
+      int begin = 0;
+#pragma unroll
+      for (int a = 0; a < SCMP_MAX_AXES; ++a) {
+        if (a >= p.r.axes) break;
+        const int h = p.r.dims[a] >> 1, o = e - begin;
+        begin += p.r.dims[a];
+        if (o < 0 || e >= begin) continue;
+        axis[i] = a;
+        half[i] = h;
+        size[i] = p.r.sizes[a];
+        second[i] = F::kInterleaved ? (o & 1) : o >= h;
+        partner[i] = F::kInterleaved ? e ^ 1 : second[i] ? e - h : e + h;
+        table[i] += p.r.table_at[a] + (F::kInterleaved ? o >> 1 : second[i] ? o - h : o);
+      }
+    }
+  }
+};
+
+// A group's token.
+struct Token {
+  uint32_t tok, b, n;
+  bool live;  // (one past the last stands for that one)
+  __device__ __forceinline__ Token(const QkNormParams &p, uint32_t token_block) {
+    const uint32_t tokens = (uint32_t)(p.r.B * p.r.N);
+    tok = token_block * (kThreads / p.lanes) + threadIdx.x / p.lanes;
+    live = tok < tokens;
+    if (!live) tok = tokens - 1;
+    b = p.r.tokens.quotient(tok);
+    n = tok - b * (uint32_t)p.r.N;
+  }
+};
+
+// cos and signed sin of a thread's elements for one token (1 and 0 where nothing
+// turns; a negative coordinate leaves its axis, one past the table gives NaN), and
+// which pieces turn.
+template <typename F, bool kBackward>
+__device__ __forceinline__ void angles(const QkNormParams &p, const Lane<F> &m, const Token &t,
+                                       Pairs<F::E> &c, Pairs<F::E> &s, bool (&turns)[F::kPieces]) {
+  constexpr int V = F::V;
+  constexpr bool kPaired = F::kInterleaved && V > 1;  // both members of each pair
+  constexpr int N = kPaired ? V / 2 : V;
+  const int64_t row = (int64_t)(p.r.pos_batched ? t.tok : t.n) * p.r.axes;
+#pragma unroll
+  for (int i = 0; i < F::kPieces; ++i) {
+    const int coord = m.axis[i] >= 0 ? __ldg(p.r.pos + row + m.axis[i]) : -1;
+    turns[i] = coord >= 0;
+    float2 cs[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) cs[j] = make_float2(1.0f, 0.0f);
+    if (turns[i]) {
+      const float2 *at = m.table[i] + (int64_t)coord * m.half[i];
+      const float nan = __uint_as_float(0x7FC00000u);
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        cs[j] = coord < m.size[i] ? __ldg(at + j) : make_float2(nan, nan);
+    }
+    // the first member of a pair subtracts (adds, going back)
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      if constexpr (kPaired) {
+        const int e = i * V + 2 * j;
+        c[e] = c[e + 1] = cs[j].x;
+        s[e] = kBackward ? cs[j].y : -cs[j].y;
+        s[e + 1] = -s[e];
+      } else {
+        c[i * V + j] = cs[j].x;
+        s[i * V + j] = m.second[i] != kBackward ? cs[j].y : -cs[j].y;
+      }
+    }
+  }
+}
+
+template <typename F>
+__device__ __forceinline__ void load_row(const Lane<F> &m, const typename F::T *row,
+                                         Raw<typename F::T, F::E, F::L> &x) {
+#pragma unroll
+  for (int i = 0; i < F::kLoads; ++i) {
+    if (m.in[i])
+      x.u[i].load(row + m.at[i]);
+    else
+      x.zero(i);
+  }
+}
+template <typename F>
+__device__ __forceinline__ void load_partners(const Lane<F> &m, const bool (&turns)[F::kPieces],
+                                              const typename F::T *row,
+                                              Raw<typename F::T, F::E, F::V> &x) {
+#pragma unroll
+  for (int i = 0; i < F::kPieces; ++i) {
+    if (turns[i])
+      x.u[i].load(row + m.partner[i]);
+    else
+      x.zero(i);
+  }
+}
+template <typename F>
+__device__ __forceinline__ void store_row(const Lane<F> &m, bool live, typename F::T *row,
+                                          const Raw<typename F::T, F::E, F::L> &x) {
+#pragma unroll
+  for (int i = 0; i < F::kLoads; ++i)
+    if (live && m.in[i]) x.u[i].store(row + m.at[i]);
 }
 
 // Sums over a group of lanes, of several values at a time.
@@ -71,62 +224,20 @@ template <int A> __device__ __forceinline__ void group_sum(int lanes, float (&v)
     for (int q = 0; q < A; ++q) v[q] += __shfl_xor_sync(~0u, v[q], o);
 }
 
-template <typename T, int V> __device__ __forceinline__ void zero(Piece<T, V> &x) {
-  if constexpr (V == 1) {
-    x.u[0] = from_f32<T>(0.0f);
-  } else {
-#pragma unroll
-    for (int i = 0; i < Piece<T, V>::kWords; ++i) x.u[i] = 0;
-  }
-}
-template <typename T, int V, int kP>
-__device__ __forceinline__ Pairs<V * kP> values(const Piece<T, V> (&x)[kP]) {
-  Pairs<V * kP> r;
-#pragma unroll
-  for (int i = 0; i < kP; ++i) {
-    if constexpr (V == 1) {
-      r[i] = to_f32(x[i].u[0]);
-    } else {
-      float v[V];
-      x[i].get(v);
-#pragma unroll
-      for (int j = 0; j < V; ++j) r[i * V + j] = v[j];
-    }
-  }
-  return r;
-}
-template <typename T, int V> __device__ __forceinline__ void store(T *p, const float *v) {
-  Piece<T, V> x;
-  if constexpr (V == 1) {
-    x.u[0] = from_f32<T>(v[0]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < Piece<T, V>::kWords; ++i) x.u[i] = Piece<T, V>::word(v, i);
-  }
-  x.store(p);
-}
-// Every element's partner within a thread's pieces (pairs side by side).
-template <int E> __device__ __forceinline__ Pairs<E> swapped(const Pairs<E> &x) {
-  Pairs<E> r;
-#pragma unroll
-  for (int i = 0; i < E / 2; ++i) r.p[i] = make_float2(x.p[i].y, x.p[i].x);
-  return r;
-}
-
 // mean and 1 / deviation of A head rows (mean 0 for rms); the variance is a second
 // pass over the registers.
-template <typename T, int V, int kP, int A>
-__device__ __forceinline__ void statistics(const QkNormParams &p, const Piece<T, V> (&x)[A][kP],
-                                           const Mine<V, kP> &m, float (&mean)[A],
-                                           float (&rstd)[A]) {
-  constexpr int E = V * kP;
+template <typename F, int A>
+__device__ __forceinline__ void statistics(const QkNormParams &p, const Lane<F> &m,
+                                           const Raw<typename F::T, F::E, F::L> (&x)[A],
+                                           float (&mean)[A], float (&rstd)[A]) {
+  constexpr int E = F::E;
   const float inv = 1.0f / (float)p.r.D;
 #pragma unroll
   for (int q = 0; q < A; ++q) mean[q] = 0.0f;
   if (!p.rms) {
 #pragma unroll
     for (int q = 0; q < A; ++q) {
-      const Pairs<E> v = values<T, V, kP>(x[q]);
+      const Pairs<E> v = x[q].values();
       float2 t = v.p[0];
 #pragma unroll
       for (int i = 1; i < E / 2; ++i) t = add2(t, v.p[i]);  // (0 past D)
@@ -138,16 +249,14 @@ __device__ __forceinline__ void statistics(const QkNormParams &p, const Piece<T,
   }
 #pragma unroll
   for (int q = 0; q < A; ++q) {
-    Pairs<E> v = values<T, V, kP>(x[q]);
+    Pairs<E> v = x[q].values();
     if (!p.rms) {
 #pragma unroll
       for (int i = 0; i < E / 2; ++i) v.p[i] = add2(v.p[i], both(-mean[q]));
       if (!p.whole) {
 #pragma unroll
-        for (int i = 0; i < kP; ++i)
-#pragma unroll
-          for (int j = 0; j < V; ++j)
-            if (!m.in[i]) v[i * V + j] = 0.0f;
+        for (int e = 0; e < E; ++e)
+          if (!m.in[e / F::L]) v[e] = 0.0f;
       }
     }
     float2 t = mul2(v.p[0], v.p[0]);
@@ -160,179 +269,203 @@ __device__ __forceinline__ void statistics(const QkNormParams &p, const Piece<T,
   for (int q = 0; q < A; ++q) rstd[q] = rsqrtf(__fmaf_rn(rstd[q], inv, p.eps));
 }
 
-// Heads in flight: up to 32 bytes of x per thread.
-template <typename T, int V, int kP, bool kBackward>
-__host__ __device__ constexpr int at_once() {
-  return kBackward ? (V * kP > 4 ? 1 : 2) : V * kP * (int)sizeof(T) > 16 ? 2 : 4;
+// Weights and biases of q and k in shared memory, [q, k][weight, bias][kMaxD].
+using Shared = float[2][2][kMaxD];  // (on 16 bytes)
+__device__ __forceinline__ void load_weights(const QkNormParams &p, Shared &w) {
+  for (int i = threadIdx.x; i < p.r.D; i += kThreads)
+#pragma unroll
+    for (int role = 0; role < 2; ++role) {
+      w[role][0][i] = load_as_f32(p.weight[role], p.param_dtype, i);
+      w[role][1][i] = p.bias[role] ? load_as_f32(p.bias[role], p.param_dtype, i) : 0.0f;
+    }
 }
 
-// Heads [h0, h1) of role 0 (q), 1 (k) or 2 (v) of one token.  With the rotation's c
-// and s and the partner's weight w', an element of the output is
-//   rstd (x w c + x' w' s - mean (w c + w' s)) + b c + b' s,
-// whose products of weights and angles are made once per token.
-template <typename T, int V, int kP, bool kInterleaved>
-__device__ __forceinline__ void forward_heads(const QkNormParams &p, uint32_t tok, int role, int h0,
-                                              int h1) {
-  constexpr int A = at_once<T, V, kP, false>(), E = V * kP;
-  constexpr bool kApart = !kInterleaved || V == 1;  // partners are other threads'
-  const RotaryParams &r = p.r;
-  const bool live = tok < (uint32_t)(r.B * r.N);
-  if (!live) tok = (uint32_t)(r.B * r.N) - 1;
-  const uint32_t b = r.tokens.quotient(tok), n = tok - b * (uint32_t)r.N;
-  const int64_t heads = role == 0 ? r.H : r.Hk;
-  const int before = role == 0 ? 0 : (int)(role == 1 ? r.H : r.H + r.Hk);
-  const T *from = static_cast<const T *>(r.qkv) +
-                  ((int64_t)tok * (r.H + 2 * r.Hk) + before + h0) * r.D;
-  const int64_t apart = r.N * r.D;  // of a token's rows in q, k and v
-  T *to = static_cast<T *>(role == 0 ? r.q : role == 1 ? r.k : r.v) +
-          (((int64_t)b * heads + h0) * r.N + n) * r.D;
-  Mine<V, kP> m;
-  Pairs<E> wc, ws, shift, c, s;
-  set_up<V, kP, kInterleaved, false>(p, tok, n, role < 2 && r.axes > 0, m, c, s);
-  if (role < 2) {
+// A thread's elements (kOwn), or their partners, of such a row; 0 past D.
+template <typename F, bool kOwn>
+__device__ __forceinline__ Pairs<F::E> shared_values(const Lane<F> &m, const float *row) {
+  Pairs<F::E> r;
 #pragma unroll
-    for (int i = 0; i < kP; ++i)
+  for (int i = 0; i < F::kPieces; ++i) {
+    const int l = i * F::V / F::L, own = m.at[l] + i * F::V % F::L;
+    const int at = kOwn || !F::kApart ? own : m.partner[i];
+    const bool in = m.in[l];
+    if constexpr (F::V % 4 == 0) {
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const int e = i * V + j, at = m.e0[i] + j;
-        const int o = kApart ? m.partner[i] + j : m.e0[i] + (j ^ 1);
-        wc[e] = ws[e] = shift[e] = 0.0f;
-        if (!m.in[i]) continue;
-        wc[e] = load_as_f32(p.weight[role], p.param_dtype, at) * c[e];
-        ws[e] = load_as_f32(p.weight[role], p.param_dtype, o) * s[e];
-        if (p.bias[role])
-          shift[e] = __fmaf_rn(load_as_f32(p.bias[role], p.param_dtype, at), c[e],
-                               load_as_f32(p.bias[role], p.param_dtype, o) * s[e]);
+      for (int j = 0; j < F::V; j += 4) {
+        const float4 f = in ? *reinterpret_cast<const float4 *>(row + at + j)
+                            : make_float4(0.f, 0.f, 0.f, 0.f);
+        r[i * F::V + j] = f.x;
+        r[i * F::V + j + 1] = f.y;
+        r[i * F::V + j + 2] = f.z;
+        r[i * F::V + j + 3] = f.w;
       }
+    } else {
+#pragma unroll
+      for (int j = 0; j < F::V; ++j) r[i * F::V + j] = in ? row[at + j] : 0.0f;
+    }
   }
-  for (int h = h0; h < h1; h += A, from += A * r.D, to += A * apart) {
-    Piece<T, V> x[A][kP], o[A][kP];
+  if constexpr (!kOwn && !F::kApart) return swapped<F::E>(r);
+  return r;
+}
+
+// What is the same for all heads of role 0 (q), 1 (k) or 2 (v): a token's rows in the
+// fused tensor are D apart, in q, k and v N D.
+template <typename T> struct Rows {
+  T *fused, *split;
+  int64_t apart;
+  __device__ __forceinline__ Rows(const RotaryParams &r, void *fused_base, const Token &t,
+                                  int role, int h0) {
+    const int64_t heads = role == 0 ? r.H : r.Hk;
+    const int64_t before = role == 0 ? 0 : role == 1 ? r.H : r.H + r.Hk;
+    fused = static_cast<T *>(fused_base) + ((int64_t)t.tok * (r.H + 2 * r.Hk) + before + h0) * r.D;
+    split = static_cast<T *>(role == 0 ? r.q : role == 1 ? r.k : r.v) +
+            (((int64_t)t.b * heads + h0) * r.N + t.n) * r.D;
+    apart = r.N * r.D;
+  }
+};
+
+// Heads [h0, h1) of v, either way.
+template <typename F, bool kBackward>
+__device__ __forceinline__ void copy_heads(const QkNormParams &p, const Lane<F> &m,
+                                           const Token &t, int h0, int h1) {
+  constexpr int A = 4;
+  const Rows<typename F::T> rows(p.r, p.r.qkv, t, 2, h0);
+  for (int h = h0; h < h1; h += A) {
+    Raw<typename F::T, F::E, F::L> x[A];
 #pragma unroll
     for (int q = 0; q < A; ++q) {
-      const T *row = from + (h + q < h1 ? q : h1 - 1 - h) * r.D;
-#pragma unroll
-      for (int i = 0; i < kP; ++i) {
-        if (m.in[i])
-          x[q][i].load(row + m.e0[i]);
-        else
-          zero<T, V>(x[q][i]);
-        if (kApart) {
-          if (m.mask[i])
-            o[q][i].load(row + m.partner[i]);
-          else
-            zero<T, V>(o[q][i]);
-        }
-      }
+      const int64_t i = (h + q < h1 ? h + q : h1 - 1) - h0;
+      load_row<F>(m, kBackward ? rows.split + i * rows.apart : rows.fused + i * p.r.D, x[q]);
     }
-    if (role == 2) {
 #pragma unroll
-      for (int q = 0; q < A; ++q)
+    for (int q = 0; q < A; ++q) {
+      const int64_t i = h + q - h0;
+      if (h + q < h1)
+        store_row<F>(m, t.live, kBackward ? rows.fused + i * p.r.D : rows.split + i * rows.apart,
+                     x[q]);
+    }
+  }
+}
+
+// Heads [h0, h1) of q (role 0) or k (1).  With the partner's weight w', an element of
+// the output is
+//   rstd (x w c + x' w' s - mean (w c + w' s)) + b c + b' s,
+// whose products of weights and angles are made once per token.
+template <typename F, bool kBias>
+__device__ __forceinline__ void forward_heads(const QkNormParams &p, const Lane<F> &m,
+                                              const Token &t, const Shared &weights, int role,
+                                              int h0, int h1) {
+  using T = typename F::T;
+  constexpr int A = F::E > 4 ? 2 : 4, E = F::E;
+  const Rows<T> rows(p.r, p.r.qkv, t, role, h0);
+  const T *from = rows.fused;
+  T *to = rows.split;
+  Pairs<E> wc, ws, shift;
+  bool turns[F::kPieces];
+  angles<F, false>(p, m, t, wc, ws, turns);
+  if constexpr (kBias) {
+    const Pairs<E> b = shared_values<F, true>(m, weights[role][1]);
+    const Pairs<E> o = shared_values<F, false>(m, weights[role][1]);
 #pragma unroll
-        for (int i = 0; i < kP; ++i)
-          if (live && h + q < h1 && m.in[i]) x[q][i].store(to + q * apart + m.e0[i]);
-      continue;
+    for (int i = 0; i < E / 2; ++i) shift.p[i] = fma2(b.p[i], wc.p[i], mul2(o.p[i], ws.p[i]));
+  }
+  {
+    const Pairs<E> w = shared_values<F, true>(m, weights[role][0]);
+    const Pairs<E> o = shared_values<F, false>(m, weights[role][0]);
+#pragma unroll
+    for (int i = 0; i < E / 2; ++i) {
+      wc.p[i] = mul2(w.p[i], wc.p[i]);
+      ws.p[i] = mul2(o.p[i], ws.p[i]);
+    }
+  }
+  for (int h = h0; h < h1; h += A, from += A * p.r.D, to += A * rows.apart) {
+    Raw<T, E, F::L> x[A];
+    Raw<T, E, F::V> o[A];
+#pragma unroll
+    for (int q = 0; q < A; ++q) {
+      const T *row = from + (h + q < h1 ? q : h1 - 1 - h) * p.r.D;
+      load_row<F>(m, row, x[q]);
+      if (F::kApart) load_partners<F>(m, turns, row, o[q]);
     }
     float mean[A], rstd[A];
-    statistics<T, V, kP, A>(p, x, m, mean, rstd);
+    statistics<F, A>(p, m, x, mean, rstd);
 #pragma unroll
     for (int q = 0; q < A; ++q) {
       if (h + q >= h1) break;
-      const Pairs<E> v = values<T, V, kP>(x[q]);
+      const Pairs<E> v = x[q].values();
       Pairs<E> u, y;
-      if constexpr (kApart)
-        u = values<T, V, kP>(o[q]);
+      if constexpr (F::kApart)
+        u = o[q].values();
       else
         u = swapped<E>(v);
 #pragma unroll
       for (int i = 0; i < E / 2; ++i) {
-        float2 t = fma2(v.p[i], wc.p[i], mul2(u.p[i], ws.p[i]));
-        if (!p.rms) t = fma2(both(-mean[q]), add2(wc.p[i], ws.p[i]), t);
-        y.p[i] = fma2(both(rstd[q]), t, shift.p[i]);
+        float2 r = fma2(v.p[i], wc.p[i], mul2(u.p[i], ws.p[i]));
+        if (!p.rms) r = fma2(both(-mean[q]), add2(wc.p[i], ws.p[i]), r);
+        if constexpr (kBias)
+          y.p[i] = fma2(both(rstd[q]), r, shift.p[i]);
+        else
+          y.p[i] = mul2(both(rstd[q]), r);
       }
-#pragma unroll
-      for (int i = 0; i < kP; ++i)
-        if (live && m.in[i]) store<T, V>(to + q * apart + m.e0[i], &y[i * V]);
+      x[q].set(y);
+      store_row<F>(m, t.live, to + q * rows.apart, x[q]);
     }
   }
 }
 
 // The same heads' gradients; dw and db add up in the thread.
-template <typename T, int V, int kP, bool kInterleaved>
-__device__ __forceinline__ void backward_heads(const QkNormParams &p, uint32_t tok, int role,
-                                               int h0, int h1, Pairs<V * kP> &dw,
-                                               Pairs<V * kP> &db) {
-  constexpr int A = at_once<T, V, kP, true>(), E = V * kP;
-  constexpr bool kApart = !kInterleaved || V == 1;
-  const RotaryParams &r = p.r;
-  const bool live = tok < (uint32_t)(r.B * r.N);
-  if (!live) tok = (uint32_t)(r.B * r.N) - 1;
-  const uint32_t b = r.tokens.quotient(tok), n = tok - b * (uint32_t)r.N;
-  const int64_t heads = role == 0 ? r.H : r.Hk;
-  const int before = role == 0 ? 0 : (int)(role == 1 ? r.H : r.H + r.Hk);
-  const int64_t at = ((int64_t)tok * (r.H + 2 * r.Hk) + before + h0) * r.D;
-  const T *from = static_cast<const T *>(p.x) + at;
-  T *to = static_cast<T *>(r.qkv) + at;
-  const int64_t apart = r.N * r.D;
-  const T *grad = static_cast<const T *>(role == 0 ? r.q : role == 1 ? r.k : r.v) +
-                  (((int64_t)b * heads + h0) * r.N + n) * r.D;
-  Mine<V, kP> m;
-  Pairs<E> c, s, w;
-  set_up<V, kP, kInterleaved, true>(p, tok, n, role < 2 && r.axes > 0, m, c, s);
-#pragma unroll
-  for (int i = 0; i < kP; ++i)
-#pragma unroll
-    for (int j = 0; j < V; ++j)
-      w[i * V + j] =
-          role < 2 && m.in[i] ? load_as_f32(p.weight[role], p.param_dtype, m.e0[i] + j) : 0.0f;
-  const float inv = 1.0f / (float)r.D;
-  for (int h = h0; h < h1; h += A, from += A * r.D, to += A * r.D, grad += A * apart) {
-    Piece<T, V> x[A][kP], g[A][kP], o[A][kP];
+template <typename F, bool kBias>
+__device__ __forceinline__ void backward_heads(const QkNormParams &p, const Lane<F> &m,
+                                               const Token &t, const Shared &weights,
+                                               const Pairs<F::E> &c, const Pairs<F::E> &s,
+                                               const bool (&turns)[F::kPieces], int role, int h0,
+                                               int h1, Pairs<F::E> &dw, Pairs<F::E> &db) {
+  using T = typename F::T;
+  constexpr int A = F::E > 4 ? 1 : 2, E = F::E;
+  const Rows<T> rows(p.r, p.r.qkv, t, role, h0);
+  const T *from = static_cast<const T *>(p.x) + (rows.fused - static_cast<T *>(p.r.qkv));
+  T *to = rows.fused;
+  const T *grad = rows.split;
+  const Pairs<E> w = shared_values<F, true>(m, weights[role][0]);
+  const float inv = 1.0f / (float)p.r.D;
+  for (int h = h0; h < h1; h += A, from += A * p.r.D, to += A * p.r.D, grad += A * rows.apart) {
+    Raw<T, E, F::L> x[A], g[A];
+    Raw<T, E, F::V> o[A];
 #pragma unroll
     for (int q = 0; q < A; ++q) {
-      // (what counts for no row has gradients of zero)
-      const bool counts = live && h + q < h1;
-      const int64_t hh = h + q < h1 ? q : h1 - 1 - h;
+      const int64_t i = h + q < h1 ? q : h1 - 1 - h;
+      load_row<F>(m, from + i * p.r.D, x[q]);
+      if (t.live && h + q < h1) {
+        load_row<F>(m, grad + i * rows.apart, g[q]);
+        if (F::kApart) load_partners<F>(m, turns, grad + i * rows.apart, o[q]);
+      } else {  // (what counts for no row has gradients of zero)
 #pragma unroll
-      for (int i = 0; i < kP; ++i) {
-        zero<T, V>(x[q][i]);
-        zero<T, V>(g[q][i]);
-        zero<T, V>(o[q][i]);
-        if (!m.in[i]) continue;
-        if (counts) g[q][i].load(grad + hh * apart + m.e0[i]);
-        if (role == 2) continue;
-        x[q][i].load(from + hh * r.D + m.e0[i]);
-        if (kApart && counts && m.mask[i]) o[q][i].load(grad + hh * apart + m.partner[i]);
+        for (int l = 0; l < F::kLoads; ++l) g[q].zero(l);
+#pragma unroll
+        for (int l = 0; l < F::kPieces; ++l) o[q].zero(l);
       }
     }
-    if (role == 2) {
-#pragma unroll
-      for (int q = 0; q < A; ++q)
-#pragma unroll
-        for (int i = 0; i < kP; ++i)
-          if (live && h + q < h1 && m.in[i]) g[q][i].store(to + q * r.D + m.e0[i]);
-      continue;
-    }
     float mean[A], rstd[A], sum_gn[A], sum_g[A];
-    statistics<T, V, kP, A>(p, x, m, mean, rstd);
+    statistics<F, A>(p, m, x, mean, rstd);
     Pairs<E> norm[A], gw[A];
 #pragma unroll
     for (int q = 0; q < A; ++q) {
-      const Pairs<E> v = values<T, V, kP>(x[q]), t = values<T, V, kP>(g[q]);
+      const Pairs<E> v = x[q].values(), y = g[q].values();
       Pairs<E> u;
-      if constexpr (kApart)
-        u = values<T, V, kP>(o[q]);
+      if constexpr (F::kApart)
+        u = o[q].values();
       else
-        u = swapped<E>(t);
+        u = swapped<E>(y);
       float2 gn = make_float2(0.f, 0.f), gs = gn;
 #pragma unroll
       for (int i = 0; i < E / 2; ++i) {
-        const float2 dt = fma2(t.p[i], c.p[i], mul2(u.p[i], s.p[i]));
+        const float2 dt = fma2(y.p[i], c.p[i], mul2(u.p[i], s.p[i]));
         norm[q].p[i] = mul2(add2(v.p[i], both(-mean[q])), both(rstd[q]));
         gw[q].p[i] = mul2(dt, w.p[i]);  // (0 past D)
         gn = fma2(gw[q].p[i], norm[q].p[i], gn);
         gs = add2(gs, gw[q].p[i]);
         dw.p[i] = fma2(dt, norm[q].p[i], dw.p[i]);
-        db.p[i] = add2(db.p[i], dt);
+        if (kBias) db.p[i] = add2(db.p[i], dt);
       }
       sum_gn[q] = gn.x + gn.y;
       sum_g[q] = gs.x + gs.y;
@@ -347,218 +480,233 @@ __device__ __forceinline__ void backward_heads(const QkNormParams &p, uint32_t t
 #pragma unroll
       for (int i = 0; i < E / 2; ++i)
         y.p[i] = mul2(fma2(norm[q].p[i], a, add2(gw[q].p[i], d)), both(rstd[q]));
-#pragma unroll
-      for (int i = 0; i < kP; ++i)
-        if (live && m.in[i]) store<T, V>(to + q * r.D + m.e0[i], &y[i * V]);
+      x[q].set(y);
+      store_row<F>(m, t.live, to + q * p.r.D, x[q]);
     }
   }
 }
 
-__device__ __forceinline__ void unit_of(const QkNormParams &p, int u, int &role, int &h0, int &h1) {
-  role = u < p.units_q ? 0 : u < p.units_qk ? 1 : 2;
-  h0 = (role == 0 ? u : role == 1 ? u - p.units_q : u - p.units_qk) * p.heads_per;
-  const int heads = (int)(role == 0 ? p.r.H : p.r.Hk);
-  h1 = h0 + p.heads_per < heads ? h0 + p.heads_per : heads;
+// A unit's heads among q's, k's and v's in a row: f(role, first, last).
+template <typename Fn>
+__device__ __forceinline__ void for_roles(const QkNormParams &p, uint32_t split, Fn &&f) {
+  const int H = (int)p.r.H, Hk = (int)p.r.Hk, all = H + Hk + (p.r.v_transposed ? 0 : Hk);
+  const int first = (int)split * p.heads_per;
+  const int last = first + p.heads_per < all ? first + p.heads_per : all;
+  if (first < H) f(0, first, last < H ? last : H);
+  if (last > H && first < H + Hk)
+    f(1, first > H ? first - H : 0, last < H + Hk ? last - H : Hk);
+  if (last > H + Hk) f(2, first > H + Hk ? first - H - Hk : 0, last - H - Hk);
 }
 
-template <typename T, int V, int kP, bool kInterleaved>
-__global__ void __launch_bounds__(kThreads)
+// Blocks take units in turn (behind them v's transposed tiles, a block each).
+// (single elements keep a place each, which takes registers)
+template <typename F, bool kBackward> __host__ __device__ constexpr int blocks_per_sm() {
+  return F::V == 1 ? 1 : F::V == 2 || (kBackward && F::E > 4) ? 2 : 3;
+}
+template <typename F, bool kBias>
+__global__ void __launch_bounds__(kThreads, (blocks_per_sm<F, false>()))
     qknorm_kernel(const __grid_constant__ QkNormParams p) {
   extern __shared__ __align__(16) unsigned char smem[];
+  __shared__ __align__(16) Shared weights;
   if (blockIdx.x >= p.r.turn_blocks) {
-    transpose_tile<T, kP == 1 ? V : 1, false>(p.r, blockIdx.x - p.r.turn_blocks,
-                                              reinterpret_cast<T *>(smem));
+    transpose_tile<typename F::T, F::L, false>(p.r, blockIdx.x - p.r.turn_blocks,
+                                               reinterpret_cast<typename F::T *>(smem));
     return;
   }
-  const uint32_t tb = blockIdx.x / (uint32_t)p.units_all;
-  int role, h0, h1;
-  unit_of(p, (int)(blockIdx.x - tb * (uint32_t)p.units_all), role, h0, h1);
-  const uint32_t tok = tb * (kThreads / p.lanes) + threadIdx.x / p.lanes;
-  forward_heads<T, V, kP, kInterleaved>(p, tok, role, h0, h1);
+  load_weights(p, weights);
+  const Lane<F> m(p);
+  __syncthreads();
+  for (uint32_t u = blockIdx.x; u < p.units; u += p.r.turn_blocks) {
+    const uint32_t tb = u / p.splits;
+    const Token t(p, tb);
+    for_roles(p, u - tb * p.splits, [&](int role, int h0, int h1) {
+      if (role == 2)
+        copy_heads<F, false>(p, m, t, h0, h1);
+      else
+        forward_heads<F, kBias>(p, m, t, weights, role, h0, h1);
+    });
+  }
 }
 
-// Blocks [0, blocks_q) take q's units in turn, those up to blocks_qk k's, the rest
-// v's (then v's transposed tiles, a block each).
-template <typename T, int V, int kP, bool kInterleaved>
-__global__ void __launch_bounds__(kThreads, blocks_per_sm(V * kP))
+
+template <typename F, bool kBias>
+__global__ void __launch_bounds__(kThreads, (blocks_per_sm<F, true>()))
     qknorm_bwd_kernel(const __grid_constant__ QkNormParams p) {
+  constexpr int E = F::E;
   extern __shared__ __align__(16) unsigned char smem[];
+  __shared__ __align__(16) Shared weights;
   __shared__ float sums[kThreads / 32][2][kMaxD];
-  if (blockIdx.x >= p.blocks_all) {
-    transpose_tile<T, kP == 1 ? V : 1, true>(p.r, blockIdx.x - p.blocks_all,
-                                             reinterpret_cast<T *>(smem));
+  if (blockIdx.x >= p.r.turn_blocks) {
+    transpose_tile<typename F::T, F::L, true>(p.r, blockIdx.x - p.r.turn_blocks,
+                                              reinterpret_cast<typename F::T *>(smem));
     return;
   }
-  const int role = blockIdx.x < p.blocks_q ? 0 : blockIdx.x < p.blocks_qk ? 1 : 2;
-  const uint32_t first = role == 0 ? 0 : role == 1 ? p.blocks_q : p.blocks_qk;
-  const uint32_t blocks = (role == 0 ? p.blocks_q : role == 1 ? p.blocks_qk : p.blocks_all) - first;
-  const int unit0 = role == 0 ? 0 : role == 1 ? p.units_q : p.units_qk;
-  const uint32_t per = (role == 0 ? p.units_q : role == 1 ? p.units_qk : p.units_all) - unit0;
-  Pairs<V * kP> dw, db;
+  load_weights(p, weights);
+  const Lane<F> m(p);
+  __syncthreads();
+  Pairs<E> dw[2], db[2];
 #pragma unroll
-  for (int e = 0; e < V * kP; ++e) dw[e] = db[e] = 0.0f;
-  for (uint64_t u = blockIdx.x - first; u < (uint64_t)p.token_blocks * per; u += blocks) {
-    const uint32_t tb = (uint32_t)(u / per);
-    int same, h0, h1;
-    unit_of(p, unit0 + (int)(u - (uint64_t)tb * per), same, h0, h1);
-    const uint32_t tok = tb * (kThreads / p.lanes) + threadIdx.x / p.lanes;
-    backward_heads<T, V, kP, kInterleaved>(p, tok, role, h0, h1, dw, db);
+  for (int e = 0; e < E; ++e) dw[0][e] = dw[1][e] = db[0][e] = db[1][e] = 0.0f;
+  for (uint32_t u = blockIdx.x; u < p.units; u += p.r.turn_blocks) {
+    const uint32_t tb = u / p.splits;
+    const Token t(p, tb);
+    Pairs<E> c, s;
+    bool turns[F::kPieces];
+    angles<F, true>(p, m, t, c, s, turns);
+    for_roles(p, u - tb * p.splits, [&](int role, int h0, int h1) {
+      if (role == 0)
+        backward_heads<F, kBias>(p, m, t, weights, c, s, turns, 0, h0, h1, dw[0], db[0]);
+      else if (role == 1)
+        backward_heads<F, kBias>(p, m, t, weights, c, s, turns, 1, h0, h1, dw[1], db[1]);
+      else
+        copy_heads<F, true>(p, m, t, h0, h1);
+    });
   }
-  if (role == 2 || !p.part) return;
+  if (!p.part) return;
   // the block's sums: over the groups of a warp, then over the warps
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
-  for (int i = 0; i < kP; ++i)
+  for (int role = 0; role < 2; ++role) {
+    __syncthreads();
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
+    for (int e = 0; e < E; ++e) {
+      float a = dw[role][e], b = db[role][e];
       for (int o = p.lanes; o < 32; o <<= 1) {
-        dw[i * V + j] += __shfl_xor_sync(~0u, dw[i * V + j], o);
-        db[i * V + j] += __shfl_xor_sync(~0u, db[i * V + j], o);
+        a += __shfl_xor_sync(~0u, a, o);
+        if (kBias) b += __shfl_xor_sync(~0u, b, o);
       }
-      const int e = ((lane & (p.lanes - 1)) + i * p.lanes) * V + j;
-      if (lane < p.lanes && e < p.r.D) {
-        sums[warp][0][e] = dw[i * V + j];
-        sums[warp][1][e] = db[i * V + j];
+      const int at = F::element(lane & (p.lanes - 1), p.lanes, e);
+      if (lane < p.lanes && at < p.r.D) {
+        sums[warp][0][at] = a;
+        if (kBias) sums[warp][1][at] = b;
       }
     }
-  __syncthreads();
-  for (int e = threadIdx.x; e < 2 * p.r.D; e += kThreads) {
-    const int which = e >= p.r.D, d = e - which * p.r.D;
-    float t = 0.0f;
+    __syncthreads();
+    for (int e = threadIdx.x; e < (kBias ? 2 : 1) * p.r.D; e += kThreads) {
+      const int which = e >= p.r.D, d = e - which * p.r.D;
+      float t = 0.0f;
 #pragma unroll
-    for (int i = 0; i < kThreads / 32; ++i) t += sums[i][which][d];
-    p.part[((int64_t)blockIdx.x * 2 + which) * p.r.D + d] = t;
+      for (int i = 0; i < kThreads / 32; ++i) t += sums[i][which][d];
+      p.part[(((int64_t)blockIdx.x * 2 + role) * 2 + which) * p.r.D + d] = t;
+    }
   }
 }
 
 // Block (x, y): 32 columns of gradient y (q's weight and bias, k's weight and bias);
-// eight warps take every eighth part.
+// 32 warps take every 32nd part.
 struct SumArgs {
   const float *part;
   void *out[4];
-  uint32_t first[4], last[4];
+  uint32_t parts;
   int D, dtype;
 };
-__global__ void __launch_bounds__(kThreads) qknorm_sum_kernel(const __grid_constant__ SumArgs a) {
-  __shared__ float sums[kThreads / 32][32];
+__global__ void __launch_bounds__(1024) qknorm_sum_kernel(const __grid_constant__ SumArgs a) {
+  __shared__ float sums[32][33];
   const int y = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int d = blockIdx.x * 32 + lane;
   if (!a.out[y]) return;
   float t = 0.0f;
   if (d < a.D) {
 #pragma unroll 8
-    for (uint32_t i = a.first[y] + warp; i < a.last[y]; i += kThreads / 32)
-      t += a.part[((int64_t)i * 2 + (y & 1)) * a.D + d];
+    for (uint32_t i = warp; i < a.parts; i += 32) t += a.part[((int64_t)i * 4 + y) * a.D + d];
   }
   sums[warp][lane] = t;
   __syncthreads();
-  if (warp != 0 || d >= a.D) return;
-  t = 0.0f;
+  t = sums[lane][warp];  // column `warp` of the block, its parts over the lanes
 #pragma unroll
-  for (int i = 0; i < kThreads / 32; ++i) t += sums[i][lane];
+  for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(~0u, t, o);
+  const int c = blockIdx.x * 32 + warp;
+  if (lane != 0 || c >= a.D) return;
   if (a.dtype == SCMP_F32)
-    static_cast<float *>(a.out[y])[d] = t;
+    static_cast<float *>(a.out[y])[c] = t;
   else if (a.dtype == SCMP_BF16)
-    static_cast<__nv_bfloat16 *>(a.out[y])[d] = from_f32<__nv_bfloat16>(t);
+    static_cast<__nv_bfloat16 *>(a.out[y])[c] = from_f32<__nv_bfloat16>(t);
   else
-    static_cast<__half *>(a.out[y])[d] = from_f32<__half>(t);
+    static_cast<__half *>(a.out[y])[c] = from_f32<__half>(t);
 }
 
-// As many blocks as run at once on the 148 SMs, shared out by heads: of q, of q and k,
-// of all.
-struct Blocks {
-  uint32_t q, qk, all;
-};
-Blocks bwd_blocks(int64_t H, int64_t Hk, int per_sm) {
-  const int64_t all = 148 * per_sm;
-  int64_t k = all * Hk / (H + 2 * Hk);
-  k = k < 1 ? 1 : k;
-  Blocks n;
-  n.q = (uint32_t)(all - 2 * k);
-  n.qk = n.q + (uint32_t)k;
-  n.all = n.qk + (uint32_t)k;
-  return n;
-}
-
-int units(int64_t heads, int per) { return (int)((heads + per - 1) / per); }
-
-template <typename T, int V, int kP, bool kInterleaved>
-cudaError_t launch_p(QkNormParams p, cudaStream_t s) {
+template <typename F> cudaError_t launch_form(QkNormParams p, cudaStream_t s) {
+  using T = typename F::T;
   RotaryParams &r = p.r;
   r.tokens = FastDiv((uint32_t)r.N);
-  const int pieces = (r.D / V + kP - 1) / kP;
   p.lanes = 1;
-  while (p.lanes < pieces) p.lanes *= 2;
-  p.whole = p.lanes * kP * V == r.D;
+  while (p.lanes * F::E < r.D) p.lanes *= 2;
+  p.whole = p.lanes * F::E == r.D;
   const int64_t tokens = r.B * r.N, per_block = kThreads / p.lanes;
   const int64_t token_blocks = (tokens + per_block - 1) / per_block;
-  p.token_blocks = (uint32_t)token_blocks;
-  // as many heads per thread as leave six units for each of the 148 SMs
+  // as many heads per unit as leave 24 units for each of the 148 SMs: the last ones
+  // to run are then a small part
   const int64_t all = r.H + r.Hk + (r.v_transposed ? 0 : r.Hk);
-  const int64_t fit = all * token_blocks / (148 * 6);
-  p.heads_per = (int)(fit < 1 ? 1 : fit > r.H ? r.H : fit);
-  p.units_q = units(r.H, p.heads_per);
-  p.units_qk = p.units_q + units(r.Hk, p.heads_per);
-  p.units_all = p.units_qk + (r.v_transposed ? 0 : units(r.Hk, p.heads_per));
+  int64_t splits = (148 * 24 + token_blocks - 1) / token_blocks;
+  splits = splits > all ? all : splits;
+  p.heads_per = (int)((all + splits - 1) / splits);
+  p.splits = (uint32_t)((all + p.heads_per - 1) / p.heads_per);
   const int64_t tiles = r.v_transposed ? r.B * r.Hk * ((r.N + kTile - 1) / kTile) : 0;
   const size_t smem = r.v_transposed ? (size_t)(kTile + 2) * r.D * sizeof(T) : 0;  // <= 66 KB
-  int64_t blocks = token_blocks * p.units_all;
-  if (r.inverse) {
-    const Blocks n = bwd_blocks(r.H, r.Hk, blocks_per_sm(V * kP));
-    p.blocks_q = n.q;
-    p.blocks_qk = n.qk;
-    p.blocks_all = r.v_transposed ? n.qk : n.all;
-    blocks = p.blocks_all;
-  }
-  if (blocks + tiles > INT32_MAX) return cudaErrorInvalidConfiguration;
-  r.turn_blocks = (uint32_t)blocks;
-  r.per = FastDiv((uint32_t)(r.D / V));
-  auto kern = r.inverse ? qknorm_bwd_kernel<T, V, kP, kInterleaved>
-                        : qknorm_kernel<T, V, kP, kInterleaved>;
-  // (always the most that this kernel uses: calls at the same time agree on it)
-  const int most = (kTile + 2) * kMaxD * (int)sizeof(T);
-  if (most + (int)sizeof(float) * kThreads / 32 * 2 * kMaxD > 48 * 1024 && smem > 0) {
-    const cudaError_t e =
-        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+  const int64_t units = token_blocks * p.splits;
+  if (units + tiles > INT32_MAX) return cudaErrorInvalidConfiguration;
+  p.units = (uint32_t)units;
+  const uint32_t most = 148u * (r.inverse ? blocks_per_sm<F, true>() : blocks_per_sm<F, false>());
+  r.turn_blocks = p.units < most ? p.units : most;
+  r.per = FastDiv((uint32_t)(r.D / F::L));
+  const bool bias = r.inverse ? p.grads[1] || p.grads[3] : p.bias[0] || p.bias[1];
+  auto kern = r.inverse ? (bias ? qknorm_bwd_kernel<F, true> : qknorm_bwd_kernel<F, false>)
+                        : (bias ? qknorm_kernel<F, true> : qknorm_kernel<F, false>);
+  if (smem > 0) {
+    // (always the most that this kernel uses: calls at the same time agree on it)
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               (kTile + 2) * kMaxD * (int)sizeof(T));
     if (e != cudaSuccess) return e;
   }
-  kern<<<(unsigned)(blocks + tiles), kThreads, smem, s>>>(p);
+  kern<<<(unsigned)(r.turn_blocks + tiles), kThreads, smem, s>>>(p);
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess || !p.part) return e;
   SumArgs a;
   a.part = p.part;
+  a.parts = r.turn_blocks;
   a.D = r.D;
   a.dtype = p.param_dtype;
-  for (int y = 0; y < 4; ++y) {
-    a.out[y] = p.grads[y];
-    a.first[y] = y < 2 ? 0 : p.blocks_q;
-    a.last[y] = y < 2 ? p.blocks_q : p.blocks_qk;
-  }
-  qknorm_sum_kernel<<<dim3((unsigned)((r.D + 31) / 32), 4), kThreads, 0, s>>>(a);
+  for (int y = 0; y < 4; ++y) a.out[y] = p.grads[y];
+  qknorm_sum_kernel<<<dim3((unsigned)((r.D + 31) / 32), 4), 1024, 0, s>>>(a);
   return cudaGetLastError();
 }
-template <typename T, int V, int kP>
+template <typename T, int L, int V, int E>
 cudaError_t launch_order(const QkNormParams &p, cudaStream_t s) {
-  return p.r.interleaved ? launch_p<T, V, kP, true>(p, s) : launch_p<T, V, kP, false>(p, s);
+  return p.r.interleaved ? launch_form<Form<T, L, V, E, true>>(p, s)
+                         : launch_form<Form<T, L, V, E, false>>(p, s);
 }
-template <typename T, int V> bool fits(const QkNormParams &p) {
-  return pieces<T, V>(p.r) && reinterpret_cast<uintptr_t>(p.x) % (V * sizeof(T)) == 0;
+// Whether rows can be accessed L elements at a time, and pairs V.
+template <typename T, int L, int V> bool fits(const QkNormParams &p) {
+  const uintptr_t at = reinterpret_cast<uintptr_t>(p.r.qkv) | reinterpret_cast<uintptr_t>(p.r.q) |
+                       reinterpret_cast<uintptr_t>(p.r.k) | reinterpret_cast<uintptr_t>(p.r.v) |
+                       reinterpret_cast<uintptr_t>(p.x);
+  bool ok = p.r.D % L == 0 && at % (L * sizeof(T)) == 0;
+  // (a piece lies in one section, and in one half of it where pairs are apart)
+  for (int a = 0; a < p.r.axes; ++a)
+    ok = ok && p.r.dims[a] / (p.r.interleaved ? 1 : 2) % V == 0;
+  return ok;
 }
-// The widest pieces (16 bytes at most) that divide every head row and half section,
-// up to eight elements per lane.
+// The widest accesses (16 bytes at most) that rows and half sections allow.  Eight
+// elements per lane; four of fp32 in the forward pass where 32 lanes hold the row so
+// (64 images of 16 heads of 64: 72 us, with eight 75; backward 131 and 120).
 template <typename T> cudaError_t launch(const QkNormParams &p, cudaStream_t s) {
-  if constexpr (sizeof(T) == 2)
-    if (fits<T, 8>(p)) return launch_order<T, 8, 1>(p, s);
-  if (fits<T, 4>(p))
-    return p.r.D <= 128 ? launch_order<T, 4, 1>(p, s) : launch_order<T, 4, 2>(p, s);
-  if (fits<T, 2>(p)) return launch_order<T, 2, 4>(p, s);
-  return launch_order<T, 1, 8>(p, s);
+  if constexpr (sizeof(T) == 2) {
+    if (fits<T, 8, 8>(p)) return launch_order<T, 8, 8, 8>(p, s);
+    if (fits<T, 8, 4>(p)) return launch_order<T, 8, 4, 8>(p, s);
+    if (fits<T, 4, 4>(p)) return launch_order<T, 4, 4, 8>(p, s);
+  } else {
+    if (fits<T, 4, 4>(p))
+      return p.r.D <= 128 && !p.r.inverse ? launch_order<T, 4, 4, 4>(p, s)
+                                          : launch_order<T, 4, 4, 8>(p, s);
+  }
+  if (fits<T, 2, 2>(p)) return launch_order<T, 2, 2, 8>(p, s);
+  return launch_order<T, 1, 1, 8>(p, s);
 }
 
 }  // namespace
 
-size_t qknorm_part_floats(int64_t H, int64_t Hk, int64_t D) {
-  return (size_t)bwd_blocks(H, Hk, blocks_per_sm(1)).qk * 2 * (size_t)D;
+size_t qknorm_part_floats(int64_t D) {
+  return (size_t)148 * blocks_per_sm<Form<float, 4, 4, 4, true>, true>() * 4 * (size_t)D;
 }
 
 cudaError_t launch_qknorm(const QkNormParams &p, int dtype, cudaStream_t s) {
