@@ -1,9 +1,9 @@
 """Build the in-tree engine library ``scmp_vit_b200/libscmp_b200.so``.
 
 nvcc compiles every ``csrc/*.cu`` for sm_100a only (``-gencode
-arch=compute_100a,code=sm_100a``) into one shared object with a plain C ABI
-(``include/scmp_b200.h``).  No torch headers are involved; Python binds the
-library with ctypes (``scmp_vit_b200/_lib.py``).
+arch=compute_100a,code=sm_100a``), one process per core, and links them into one
+shared object with a plain C ABI (``include/scmp_b200.h``).  No torch headers are
+involved; Python binds the library with ctypes (``scmp_vit_b200/_lib.py``).
 """
 from __future__ import annotations
 
@@ -11,6 +11,8 @@ import os
 import shutil
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -18,10 +20,11 @@ CSRC = PKG / "csrc"
 LIB = PKG / "libscmp_b200.so"
 ROOT = PKG.parent
 
+ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = [
-    "-gencode", "arch=compute_100a,code=sm_100a",
+    *ARCH,
     "-O3", "-lineinfo", "-std=c++17",
-    "--shared", "-Xcompiler", "-fPIC,-fvisibility=hidden",
+    "-Xcompiler", "-fPIC,-fvisibility=hidden",
     "-Xptxas", "-warn-spills",
     # IEEE float everywhere: the rescale must match the oracle bit for bit.
     "-prec-div=true", "-prec-sqrt=true", "-fmad=false", "-ftz=false",
@@ -50,15 +53,25 @@ def needs_build() -> bool:
 def build(force: bool = False, verbose: bool = False) -> Path:
     if not force and not needs_build():
         return LIB
-    cmd = [_nvcc(), *NVCC_FLAGS, "-I", str(ROOT / "include"),
-           *[str(s) for s in sources()], "-o", str(LIB) + ".tmp"]
-    if verbose:
-        print(" ".join(cmd), file=sys.stderr)
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    if res.returncode != 0:
-        raise RuntimeError(f"nvcc failed ({res.returncode}):\n{res.stdout}\n{res.stderr}")
-    if verbose and (res.stdout or res.stderr):
-        print(res.stdout + res.stderr, file=sys.stderr)
+    def run(cmd):
+        if verbose:
+            print(" ".join(cmd), file=sys.stderr)
+        res = subprocess.run(cmd, capture_output=True, text=True)
+        if res.returncode != 0:
+            raise RuntimeError(f"nvcc failed ({res.returncode}):\n{res.stdout}\n{res.stderr}")
+        if verbose and (res.stdout or res.stderr):
+            print(res.stdout + res.stderr, file=sys.stderr)
+
+    nvcc, files = _nvcc(), sources()
+    with tempfile.TemporaryDirectory() as tmp:
+        objects = [str(Path(tmp) / (f.stem + ".o")) for f in files]
+        jobs = [[nvcc, *NVCC_FLAGS, "-I", str(ROOT / "include"), "-c", str(f), "-o", o]
+                for f, o in zip(files, objects)]
+        # (the longest first: they decide when the last one ends)
+        jobs.sort(key=lambda job: -os.path.getsize(job[-3]))
+        with ThreadPoolExecutor(max_workers=max(1, os.cpu_count() or 1)) as pool:
+            list(pool.map(run, jobs))
+        run([nvcc, *ARCH, "--shared", "-Xcompiler", "-fPIC", *objects, "-o", str(LIB) + ".tmp"])
     os.replace(str(LIB) + ".tmp", LIB)
     return LIB
 
