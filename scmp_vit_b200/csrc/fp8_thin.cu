@@ -12,7 +12,7 @@ namespace scmp {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kAhead = 2;        // steps of a weight row in flight
+constexpr int kAhead = 2;  // steps of a weight row in flight (four: [4096, 4096] 9.3 -> 10.5 us)
 constexpr int kStepValues = 512;  // values of a warp's step
 
 __device__ __forceinline__ void store_as(void *p, int dtype, int64_t i, float v) {
@@ -208,9 +208,15 @@ cudaError_t launch_m(const Fp8Product &p, const void *x, int64_t ld, const Fp8La
 
 bool fp8_thin_fits(int64_t M, int64_t K) { return M <= SCMP_FP8_THIN_ROWS && K <= SCMP_FP8_THIN_K; }
 
+// With k = K / 1024 and n = N / 1024 this launch takes about 2 + k n (0.13 + 0.17 M)
+// + k (0.2 + 0.2 M) us, quantise + tensor-core tiles 5.2 + 1.8 k + 0.1 k n.  [N, K]
+// and rows, this / the other (us, weights from HBM):
+//   [1024, 1024]  1: 2.6 / 6.9   4: 4.1 / 6.9     [4096, 1024]  1: 4.2 / 8.3   4: 7.1 / 8.3
+//   [1024, 4096]  1: 6.2 / 13.0  4: 10.6 / 13.0   [4096, 4096]  1: 9.3 / 13.5  2: 13.0 / 13.5
+//   [16384, 1024] 1: 8.0 / 9.5   2: 11.5 / 9.5    [6144, 6144]  1: 15.9 / 17.9 2: 24.4 / 17.9
 bool fp8_thin(int64_t M, int64_t N, int64_t K) {
   return fp8_thin_fits(M, K) &&
-         K / 1024.0 * (N / 1024.0 * (1 + 0.7 * M) + (double)M - 5) < 12;
+         K / 1024.0 * (N / 1024.0 * (0.03 + 0.17 * M) + 0.2 * M - 1.6) < 3.2;
 }
 
 cudaError_t launch_fp8_thin(const Fp8Product &p, const void *x, int x_dtype, int64_t ld,

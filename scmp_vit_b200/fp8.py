@@ -173,7 +173,7 @@ def _thin(rows: int, N: int, K: int) -> bool:
     """Whether a few rows are quantised inside the product's own launch, which
     needs no buffers (the engine's rule for products of codes)."""
     return (rows <= _lib.FP8_THIN_ROWS and K <= _lib.FP8_THIN_K
-            and K / 1024 * (N / 1024 * (1 + 0.7 * rows) + rows - 5) < 12)
+            and K / 1024 * (N / 1024 * (0.03 + 0.17 * rows) + 0.2 * rows - 1.6) < 3.2)
 
 
 def _overlap_codes(out: torch.Tensor, q: FP8Tensor) -> bool:

@@ -253,6 +253,14 @@ def no_launch(monkeypatch):
     return launched
 
 
+def test_few_rows_rule_in_both_places():
+    """The Python side allocates no buffers where the engine needs none."""
+    for M in (1, 2, 3, 4, 5):
+        for N in (1, 300, 1024, 4096, 16384):
+            for K in (1, 700, 1024, 4096, 6144, 6145):
+                assert _lib.fp8_plan(M, N, K)[0] == fp8._thin(M, N, K)
+
+
 def test_shapes_and_types_are_checked(no_launch):
     x, w = torch.zeros(6, 32), torch.zeros(8, 32)
     q = fp8.fp8_empty((8, 32), x.device, x.dtype)
