@@ -14,6 +14,7 @@ numerics per slice, but without their host loops:
 """
 from __future__ import annotations
 
+import functools
 import math
 from typing import Callable, Optional
 
@@ -534,6 +535,12 @@ def _split_norm(src, weights, pos, table, spec):
     return q, k, v.transpose(-1, -2) if transpose_v else v
 
 
+@functools.lru_cache(maxsize=64)
+def _norm_workspace(H: int, Hk: int, D: int) -> int:
+    """Bytes, a function of the sizes alone."""
+    return _lib.load().scmp_split_qkv_norm_workspace(H, Hk, D)
+
+
 class _SplitQkvNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, qkv, q_weight, k_weight, q_bias, k_bias, pos, table, spec):
@@ -559,8 +566,7 @@ class _SplitQkvNorm(torch.autograd.Function):
             dq, dk = dq.contiguous(), dk.contiguous()
             size, ws = 0, None
             if any([t is not None for t in params]):
-                size = _lib.load().scmp_split_qkv_norm_workspace(dq.shape[1], dk.shape[1],
-                                                                 dq.shape[3])
+                size = _norm_workspace(dq.shape[1], dk.shape[1], dq.shape[3])
                 ws = torch.empty(size, dtype=torch.uint8, device=src.device)
             _norm_args(grad, dq, dk, dv, src, weights, pos, table, spec, True, transposed,
                        [0 if t is None else t.data_ptr() for t in params],

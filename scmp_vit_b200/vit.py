@@ -390,9 +390,9 @@ def dropout(x: torch.Tensor, p: float, seed, offset: int = 0, *, per: str = "ele
 class Dropout(nn.Module):
     """``dropout`` in a model: in training every call takes the next mask, in
     evaluation it passes through.  ``index`` tells the modules of a model apart, which
-    may then share ``seed``.  ``calls`` counts (and, set, repeats) the eager masks;
-    calls that a graph captures count on the device, so that every replay draws
-    masks of its own."""
+    may then share ``seed``; ranks that are to draw apart take seeds of their own.
+    ``calls`` counts (and, set, repeats) the eager masks; calls that a graph captures
+    count on the device, so that every replay draws masks of its own."""
 
     def __init__(self, p: float, *, per: str = "element", seed: int = 0, index: int = 0):
         super().__init__()
@@ -402,7 +402,11 @@ class Dropout(nn.Module):
             raise ValueError(f"p must be within 0 and 1, got {p!r}")
         if not 0 <= index < 1 << 16:
             raise ValueError(f"index must be within 0 and 65535, got {index}")
-        self.p, self.per, self.seed, self.index, self.calls = float(p), per, int(seed), index, 0
+        seed = int(seed)
+        if not -1 << 63 <= seed < 1 << 64:
+            raise ValueError(f"seed is 64-bit, got {seed}")
+        self.p, self.per, self.index, self.calls = float(p), per, index, 0
+        self.seed = seed - (1 << 64) if seed >= 1 << 63 else seed  # (as int64 holds it)
         self.register_buffer("state", torch.tensor([self.seed, 0]), persistent=False)
 
     @property

@@ -132,12 +132,13 @@ def test_python_refusals(monkeypatch):
 
 def test_modules_on_cpu():
     for kw, match in ((dict(p=-1.0), "p must"), (dict(p=0.1, per="x"), "per"),
-                      (dict(p=0.1, index=1 << 16), "index")):
+                      (dict(p=0.1, index=1 << 16), "index"), (dict(p=0.1, seed=1 << 64), "seed")):
         with pytest.raises(ValueError, match=match):
             vit.Dropout(**kw)
     x = torch.randn(2, 3)
     for m in (vit.Dropout(0.5).eval(), vit.Dropout(0.0)):
         assert m(x) is x and torch.equal(m(x, x), x + x) and m.calls == 0
+    assert vit.Dropout(0.1, seed=(1 << 64) - 2).seed == vit.Dropout(0.1, seed=-2).state[0] == -2
     m = vit.vit_l14(dim=64, depth=3, heads=1, hidden=64, img=28)
     names = set(m.state_dict())
     with pytest.raises(ValueError, match="rates"):
