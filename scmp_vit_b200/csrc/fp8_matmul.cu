@@ -46,14 +46,14 @@ constexpr uint32_t kStage = kPerStage * (kW + kX);
 constexpr uint32_t kScales = 4 * 512;  // one row group of B, up to three of A
 constexpr uint32_t kScalesAt = kStages * kStage;
 // 16-bit outputs are stored through pieces of 16 rows x 32 features, one per epilogue
-// warp (of 32 rows they do not fit; stored from registers instead, two rows of 64
-// bytes at a time, products of short K take 3% longer).
+// warp (of 32 rows they do not fit).
 constexpr int kPieceRows = 16;
 constexpr uint32_t kPiece = kPieceRows * 64;
 constexpr uint32_t kOutAt = kScalesAt + kStages * kScales;
 constexpr uint32_t kBarsAt = kOutAt + kEpilogueWarps * kPiece;
 constexpr size_t kSmem = (size_t)kBarsAt + 1024 /*align*/ + 256;
-static_assert(kStage % 1024 == 0, "swizzle atoms stay aligned");
+static_assert(kStage % 1024 == 0 && kOutAt % 512 == 0 && kPiece % 512 == 0,
+              "swizzle atoms stay aligned");
 static_assert(kScaleCol + 2 * kScaleCols <= 512, "two sets of scales behind the accumulators");
 static_assert(kSmem <= 227 * 1024, "shared memory per CTA");
 
@@ -106,6 +106,31 @@ __device__ __forceinline__ void mma_pair(uint32_t d, uint64_t a, uint64_t b, uin
       "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.block32 [%0], %1, %2, %3, [%5], [%6], "
       "p;\n}\n" ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(accumulate), "r"(sfa), "r"(sfb)
       : "memory");
+}
+
+// 32 lanes x 32 columns of tensor memory as fragments of 8 x 8 (lanes x columns):
+// thread t holds lane t / 4 and columns 2 (t % 4), + 1 of each, in v[16 h + 4 c + 2 l]
+// and the next for lanes 16 h + 8 l .. and columns 8 c ...
+__device__ __forceinline__ void tmem_ld_fragments(uint32_t taddr, uint32_t (&v)[32]) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    uint32_t *r = v + 16 * h;
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+          "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+          "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr + ((uint32_t)(16 * h) << 16)));
+  }
+}
+// Four 8 x 8 matrices of 16-bit values, a fragment register each, transposed into
+// shared memory: thread t gives the address of row t % 8 of matrix t / 8 (16 bytes).
+__device__ __forceinline__ void store_transposed(uint32_t addr, uint32_t a, uint32_t b, uint32_t c,
+                                                 uint32_t d) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(addr),
+               "r"(a), "r"(b), "r"(c), "r"(d)
+               : "memory");
 }
 
 template <typename T>
@@ -272,15 +297,26 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
     // that the tiles of the two accumulators are read and stored side by side.  An
     // accumulator's next tile waits for the last load from it: two pieces are
     // loaded at once and stored while the next are on their way.
+    //
+    // 16-bit rows that a TMA store can write are loaded as 8 x 8 fragments, which go to
+    // shared memory transposed, 512 bytes at a time, in the order of the store's
+    // 64-byte swizzle (no conflicts; two bytes at a time they took 72 shared-memory
+    // cycles a piece, which the MMAs' operands compete for).  Others go from
+    // registers: a lane holds a feature.
+    const bool by_tma = sizeof(T) == 2 && t.tma_out;
     const uint32_t mine = (uint32_t)(warp - 4) >> 3, half = (uint32_t)(warp - 4) >> 2 & 1;
     const int first = (int)(alone ? 2 * mine + half : half) * 32, stride = alone ? 128 : 64;
+    const uint32_t piece = smem0 + kOutAt + (uint32_t)(warp - 4) * kPiece;
     uint32_t turn = 0;
     for_tiles(t, [&](int f0, int n0, int sub, uint32_t buf) {
       if (!alone && buf != mine) return true;
       f0 += (int)rank * 128 + (warp & 3) * 32;
-      const int64_t f = f0 + lane;
-      const float bias =
-          t.p.bias && f < t.p.N ? load_as_f32(t.p.bias, t.p.bias_dtype, f) : 0.0f;
+      const auto bias_of = [&](int f) {
+        return t.p.bias && f < t.p.N ? load_as_f32(t.p.bias, t.p.bias_dtype, f) : 0.0f;
+      };
+      float bias[4];  // of a fragment's features, or of the lane's
+#pragma unroll
+      for (int i = 0; i < 4; ++i) bias[i] = bias_of(f0 + (by_tma ? 8 * i + (lane >> 2) : lane));
       const int64_t left = t.p.M - n0;
       const int w = t.plan.w[sub], rows = left < w ? (int)left : w;
       if (!warp_wait_cl(&tfull[buf], turn++ & 1, abort)) return false;
@@ -291,45 +327,56 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
         __syncwarp();
         if (lane == 0) arrive_remote(mapa_shared(smem_u32(&tempty[buf]), 0));
       };
+      const auto load = [&](int j0, uint32_t (&v)[32]) {
+        if (by_tma)
+          tmem_ld_fragments(acc + j0, v);
+        else
+          tmem_ld32(acc + j0, v);
+      };
       const auto store = [&](int j0, uint32_t (&v)[32]) {
         if (j0 >= rows || f0 >= t.p.N) return;
+        if constexpr (sizeof(T) == 2) if (by_tma) {
+          // (a TMA store clips what lies past M and N)
+#pragma unroll
+          for (int h = 0; h < 32; h += kPieceRows) {
+            asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+            __syncwarp();
+#pragma unroll
+            for (int c = 0; c < kPieceRows / 8; ++c) {
+              uint32_t m[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const uint32_t *r = v + 16 * (i >> 1) + 4 * (h / 8 + c) + 2 * (i & 1);
+                m[i] = pack2<T>(__uint_as_float(r[0]) + bias[i], __uint_as_float(r[1]) + bias[i]);
+              }
+              const int row = 8 * c + (lane & 7), chunk = lane >> 3;
+              store_transposed(piece + row * 64 + (chunk ^ (row >> 1 & 3)) * 16, m[0], m[1], m[2],
+                               m[3]);
+            }
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0 && j0 + h < rows) tma_store_2d(&omap, f0, n0 + j0 + h, piece);
+          }
+          return;
+        }
+        const int64_t f = f0 + lane;
         if constexpr (sizeof(T) == 4) if (t.add && f < t.p.N) {
           const float *out = static_cast<const float *>(t.p.out) + (int64_t)(n0 + j0) * t.p.N + f;
 #pragma unroll
           for (int j = 0; j < 32; ++j)
             if (j0 + j < rows) v[j] = __float_as_uint(__uint_as_float(v[j]) + out[j * t.p.N]);
         }
-        if constexpr (sizeof(T) == 2) if (t.tma_out) {
-          // (a TMA store clips what lies past M and N)
-          uint16_t *piece = reinterpret_cast<uint16_t *>(smem + kOutAt + (warp - 4) * kPiece);
-#pragma unroll
-          for (int h = 0; h < 32; h += kPieceRows) {
-            asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-            __syncwarp();
-#pragma unroll
-            for (int j = 0; j < kPieceRows; j += 2) {
-              const uint32_t two = pack2<T>(__uint_as_float(v[h + j]) + bias,
-                                            __uint_as_float(v[h + j + 1]) + bias);
-              piece[j * 32 + lane] = (uint16_t)two;
-              piece[(j + 1) * 32 + lane] = (uint16_t)(two >> 16);
-            }
-            fence_async_smem();
-            __syncwarp();
-            if (lane == 0 && j0 + h < rows) tma_store_2d(&omap, f0, n0 + j0 + h, smem_u32(piece));
-          }
-          return;
-        }
         if (j0 + 32 <= rows)
-          store_chunk<T, true>(t.p, 1.0f, t.words, v, bias, n0 + j0, f, 32, lane);
+          store_chunk<T, true>(t.p, 1.0f, t.words, v, bias[0], n0 + j0, f, 32, lane);
         else
-          store_chunk<T, false>(t.p, 1.0f, t.words, v, bias, n0 + j0, f, rows - j0, lane);
+          store_chunk<T, false>(t.p, 1.0f, t.words, v, bias[0], n0 + j0, f, rows - j0, lane);
       };
       uint32_t v[2][32];
       if (first >= w) hand_back();
 #pragma unroll 1
       for (int j0 = first; j0 < w; j0 += 2 * stride) {
-        tmem_ld32(acc + j0, v[0]);
-        if (j0 + stride < w) tmem_ld32(acc + j0 + stride, v[1]);
+        load(j0, v[0]);
+        if (j0 + stride < w) load(j0 + stride, v[1]);
         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
         if (j0 + 2 * stride >= w) hand_back();
         store(j0, v[0]);
@@ -453,7 +500,8 @@ template <typename T> cudaError_t launch(Fp8Tiles t, const Fp8Layout &l, cudaStr
       !encode_blocks(&xmap1, t.p.a, t.p.M, l, (uint32_t)(w[1] ? w[1] : w[0]) / 2) ||
       !encode_scales(&wsmap, t.p.b_scales, t.p.N, l.groups, 1, 1) ||
       !encode_scales(&xsmap, t.p.a_scales, t.p.M, l.groups, 1, (uint32_t)t.xrows) ||
-      (t.tma_out && !encode_out(&omap, t.p.out, t.p.M, t.p.N, kPieceRows)))
+      (t.tma_out && !encode_out(&omap, t.p.out, t.p.M, t.p.N, kPieceRows,
+                                 CU_TENSOR_MAP_SWIZZLE_64B)))
     return cudaErrorInvalidValue;
   const unsigned grid = t.plan.units < (uint32_t)clusters ? t.plan.units : (unsigned)clusters;
   cudaLaunchAttribute early[1];

@@ -404,7 +404,7 @@ cudaError_t launch(MxTiles t, int64_t kp, int64_t groups, cudaStream_t s) {
       !encode_rows(&xmap, t.p.a, t.p.M, kp / 2, (uint32_t)t.nt / 2) ||
       !encode_scales(&wsmap, t.p.b_scales, t.p.N, groups, Cfg::kGroups, 1) ||
       !encode_scales(&xsmap, t.p.a_scales, t.p.M, groups, Cfg::kGroups, (uint32_t)t.xrows) ||
-      (t.tma_out && !encode_out(&omap, t.p.out, t.p.M, t.p.N, 32)))
+      (t.tma_out && !encode_out(&omap, t.p.out, t.p.M, t.p.N, 32, CU_TENSOR_MAP_SWIZZLE_NONE)))
     return cudaErrorInvalidValue;
   const unsigned grid = t.tiles < (uint32_t)clusters ? t.tiles : (unsigned)clusters;
   cudaLaunchAttribute early[1];

@@ -137,7 +137,8 @@ bool encode_scales(CUtensorMap *map, const uint8_t *scales, int64_t rows, int64_
 }
 
 // 16-bit outputs in pieces of 32 features.
-bool encode_out(CUtensorMap *map, void *out, int64_t rows, int64_t features, uint32_t box_rows) {
+bool encode_out(CUtensorMap *map, void *out, int64_t rows, int64_t features, uint32_t box_rows,
+                CUtensorMapSwizzle swizzle) {
   PFN_cuTensorMapEncodeTiled_v12000 enc = tensor_map_encoder();
   if (!enc) return false;
   cuuint64_t gdim[2] = {(cuuint64_t)features, (cuuint64_t)rows};
@@ -145,7 +146,7 @@ bool encode_out(CUtensorMap *map, void *out, int64_t rows, int64_t features, uin
   cuuint32_t box[2] = {32, box_rows};
   cuuint32_t estride[2] = {1u, 1u};
   return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, out, gdim, gstride, box, estride,
-             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
              CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
