@@ -60,6 +60,7 @@ static_assert(kSmem <= 227 * 1024, "shared memory per CTA");
 struct Fp8Tiles {
   Fp8Product p;
   Fp8TilePlan plan;
+  uint32_t group, group_units;  // tiles of B's rows that are walked together; their units
   int xrows;               // row groups (of 128) that a tile's scales of A touch, at most
   int block0, blocks;      // blocks of K of this launch
   int steps;               // stages per tile
@@ -76,8 +77,15 @@ __device__ __forceinline__ void for_tiles(const Fp8Tiles &t, F &&f) {
   const uint32_t clusters = gridDim.x >> 1;
   uint32_t it = 0;
   for (uint32_t u = blockIdx.x >> 1; u < t.plan.units; u += clusters) {
-    const uint32_t q = u / t.plan.tiles_f;
-    const int f0 = (int)(u - q * t.plan.tiles_f) * 256;
+    uint32_t begin = 0, width = t.group, at = u;
+    if (width < t.plan.tiles_f) {
+      const uint32_t group = u / t.group_units;
+      begin = group * width;
+      at -= group * t.group_units;
+      if (t.plan.tiles_f - begin < width) width = t.plan.tiles_f - begin;
+    }
+    const uint32_t q = at / width;
+    const int f0 = (int)(begin + at - q * width) * 256;
     int64_t n0 = (int64_t)q * (t.plan.w[0] + t.plan.w[1]);
     for (int sub = 0; sub < 2; ++sub) {
       if (t.plan.w[sub] == 0 || n0 >= t.p.M) break;
@@ -503,6 +511,13 @@ template <typename T> cudaError_t launch(Fp8Tiles t, const Fp8Layout &l, cudaStr
       (t.tma_out && !encode_out(&omap, t.p.out, t.p.M, t.p.N, kPieceRows,
                                  CU_TENSOR_MAP_SWIZZLE_64B)))
     return cudaErrorInvalidValue;
+  // As many tiles of B's rows at a time as stay in L2 beside what streams past them
+  // (16 MB), unless all of them do (8192^3: 450 -> 422 us).
+  const int64_t bytes = 256 * l.kp;
+  t.group = t.plan.tiles_f;
+  if (t.plan.tiles_f * bytes > (24 << 20))
+    t.group = bytes < (16 << 20) ? (uint32_t)((16 << 20) / bytes) : 1u;
+  t.group_units = t.group * (t.plan.units / t.plan.tiles_f);
   const unsigned grid = t.plan.units < (uint32_t)clusters ? t.plan.units : (unsigned)clusters;
   cudaLaunchAttribute early[1];
   early[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -512,10 +512,11 @@ def test_product_ranges_and_nan(cuda_device, M):
 @pytest.mark.parametrize("M,N,K,widths,units", [
     (16135, 952, 640, (256, 192), 148), (7299, 1817, 1100, (256, 192), 136),
     (9000, 1152, 1024, (192, 0), 235), (16697, 80, 71, (128, 0), 131),
-    (788, 333, 1000, (64, 0), 26), (1024, 4096, 4300, (256, 0), 64)])
+    (788, 333, 1000, (64, 0), 26), (1024, 4096, 4300, (256, 0), 64),
+    (1500, 4100, 6200, (192, 0), 136)])
 def test_product_many_tiles(cuda_device, M, N, K, widths, units):
-    """Every choice of tile widths, several units per pair where it has them, and
-    ragged ends."""
+    """Every choice of tile widths, several units per pair where it has them, ragged
+    ends, and (the last) a weight that is walked in groups of its rows."""
     assert _lib.fp8_plan(M, N, K)[1:] == (widths, units)
     g = torch.Generator().manual_seed(M)
     a = torch.randn(M, K, generator=g).to(torch.bfloat16).to(cuda_device)
