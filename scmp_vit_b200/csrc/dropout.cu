@@ -91,17 +91,19 @@ __device__ __forceinline__ uint64_t quotient(const DropoutParams &p, uint64_t i)
   return i / (uint64_t)p.span;
 }
 
-// The draws of eight elements from i on.
+// The draws of eight elements from i on; `last` and `w` are a span and its draw, the
+// last ones used.
 template <int kDraw, typename I>
 __device__ __forceinline__ void draws(const DropoutParams &p, I i, uint64_t offset,
-                                      const uint32_t *keys, uint32_t (&u)[8]) {
+                                      const uint32_t *keys, I &last, uint32_t &w,
+                                      uint32_t (&u)[8]) {
   if (kDraw == 1) {
     const uint4 a = philox<I>(i >> 2, offset, keys), b = philox<I>((i >> 2) + 1, offset, keys);
     u[0] = a.x; u[1] = a.y; u[2] = a.z; u[3] = a.w;
     u[4] = b.x; u[5] = b.y; u[6] = b.z; u[7] = b.w;
   } else if (kDraw == 2) {
     I d = quotient(p, i), end = (d + 1) * (I)p.span;
-    uint32_t w = word(philox<I>(d >> 2, offset, keys), (uint32_t)d & 3);
+    if (d != last) w = word(philox<I>(d >> 2, offset, keys), (uint32_t)d & 3);
     if (i + 8 <= end) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) u[j] = w;
@@ -116,14 +118,18 @@ __device__ __forceinline__ void draws(const DropoutParams &p, I i, uint64_t offs
         u[j] = w;
       }
     }
+    last = d;
   }
 }
 
-// kSteps x 8 elements per thread, all loads first (16-bit types: with one step in
-// flight 3.4 TB/s).  kDraw 0: nothing is dropped, 1: a draw per element, 2: per span.
+// steps() x 8 elements per thread, all loads first.  kDraw 0: nothing is dropped, 1: a
+// draw per element, 2: per span.
+template <typename T, int kDraw> __host__ __device__ constexpr int steps() {
+  return sizeof(T) == 2 && kDraw != 1 ? 2 : 1;
+}
 template <typename T, bool kVec, bool kResidual, int kDraw, bool kState, typename I>
 __global__ void __launch_bounds__(kThreads) dropout_kernel(const __grid_constant__ DropoutParams p) {
-  constexpr int kSteps = sizeof(T) == 2 ? 2 : 1;
+  constexpr int kSteps = steps<T, kDraw>();
   constexpr int64_t kBlock = kThreads * 8;
   uint64_t offset = p.offset;
   uint32_t own[20];
@@ -133,6 +139,8 @@ __global__ void __launch_bounds__(kThreads) dropout_kernel(const __grid_constant
   }
   const T *x = static_cast<const T *>(p.x), *residual = static_cast<const T *>(p.residual);
   T *y = static_cast<T *>(p.y);
+  I last = ~(I)0;
+  uint32_t w = 0;
   for (int64_t i0 = blockIdx.x * kBlock * kSteps + threadIdx.x * 8; i0 < p.n;
        i0 += gridDim.x * kBlock * kSteps) {
     Eight<T, kVec> xs[kSteps], rs[kSteps];
@@ -147,7 +155,7 @@ __global__ void __launch_bounds__(kThreads) dropout_kernel(const __grid_constant
       const int64_t i = i0 + q * kBlock;
       if (i >= p.n) break;
       uint32_t u[8];
-      draws<kDraw, I>(p, (I)i, offset, kState ? own : p.keys, u);
+      draws<kDraw, I>(p, (I)i, offset, kState ? own : p.keys, last, w, u);
       float v[8], r[8];
 #pragma unroll
       for (int l = 0; l < Eight<T, kVec>::kLoads; ++l) {
@@ -166,40 +174,43 @@ __global__ void __launch_bounds__(kThreads) dropout_kernel(const __grid_constant
   }
 }
 
+template <typename T, bool kVec, bool kResidual, int kDraw, bool kState, typename I>
+void launch_kernel(const DropoutParams &p, cudaStream_t s) {
+  const int64_t per = kThreads * 8 * steps<T, kDraw>(), blocks = (p.n + per - 1) / per;
+  const unsigned grid = (unsigned)(blocks < 148 * 16 ? blocks : 148 * 16);
+  dropout_kernel<T, kVec, kResidual, kDraw, kState, I><<<grid, kThreads, 0, s>>>(p);
+}
 template <typename T, bool kVec, bool kResidual, typename I>
-void launch_draw(const DropoutParams &p, unsigned grid, cudaStream_t s) {
+void launch_draw(const DropoutParams &p, cudaStream_t s) {
   if (p.none)
-    dropout_kernel<T, kVec, kResidual, 0, false, I><<<grid, kThreads, 0, s>>>(p);
+    launch_kernel<T, kVec, kResidual, 0, false, I>(p, s);
   else if (p.span == 1 && !p.state)
-    dropout_kernel<T, kVec, kResidual, 1, false, I><<<grid, kThreads, 0, s>>>(p);
+    launch_kernel<T, kVec, kResidual, 1, false, I>(p, s);
   else if (p.span == 1)
-    dropout_kernel<T, kVec, kResidual, 1, true, I><<<grid, kThreads, 0, s>>>(p);
+    launch_kernel<T, kVec, kResidual, 1, true, I>(p, s);
   else if (!p.state)
-    dropout_kernel<T, kVec, kResidual, 2, false, I><<<grid, kThreads, 0, s>>>(p);
+    launch_kernel<T, kVec, kResidual, 2, false, I>(p, s);
   else
-    dropout_kernel<T, kVec, kResidual, 2, true, I><<<grid, kThreads, 0, s>>>(p);
+    launch_kernel<T, kVec, kResidual, 2, true, I>(p, s);
 }
 // Elements counted in 32 bits where they and the end of their last span fit.
 template <typename T, bool kVec, bool kResidual>
-void launch_index(DropoutParams p, unsigned grid, cudaStream_t s) {
+void launch_index(DropoutParams p, cudaStream_t s) {
   if (p.n <= INT32_MAX && p.span <= INT32_MAX) {
     p.per_span = FastDiv((uint32_t)p.span);
-    launch_draw<T, kVec, kResidual, uint32_t>(p, grid, s);
+    launch_draw<T, kVec, kResidual, uint32_t>(p, s);
   } else {
-    launch_draw<T, kVec, kResidual, uint64_t>(p, grid, s);
+    launch_draw<T, kVec, kResidual, uint64_t>(p, s);
   }
 }
 template <typename T> cudaError_t launch(const DropoutParams &p, cudaStream_t s) {
   const uintptr_t at = reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.residual) |
                        reinterpret_cast<uintptr_t>(p.y);
   const bool vec = at % 16 == 0;
-  const int64_t per = kThreads * (sizeof(T) == 2 ? 16 : 8), blocks = (p.n + per - 1) / per;
-  const unsigned grid = (unsigned)(blocks < 148 * 16 ? blocks : 148 * 16);
   if (vec)
-    p.residual ? launch_index<T, true, true>(p, grid, s) : launch_index<T, true, false>(p, grid, s);
+    p.residual ? launch_index<T, true, true>(p, s) : launch_index<T, true, false>(p, s);
   else
-    p.residual ? launch_index<T, false, true>(p, grid, s)
-               : launch_index<T, false, false>(p, grid, s);
+    p.residual ? launch_index<T, false, true>(p, s) : launch_index<T, false, false>(p, s);
   return cudaGetLastError();
 }
 

@@ -429,7 +429,8 @@ double block_ns(int w) {
 // The same of a tile's part that no MMA hides.
 constexpr double kTileNs = 250, kAloneNs = 2000;
 
-// Widths: one tile for up to 32 rows; else what costs least among 64, 128 and 192
+// Widths: one tile for up to 32 rows (16 rows by [16384, 1024]: 6.0 us, a tile of 64
+// 6.7; 32 rows 6.1 and 6.5; [4096, 4096] 9.0 and 9.1); else what costs least among 64, 128 and 192
 // throughout, 256 alone, and 256 and 192 in turn, whose starts are all multiples of
 // 64 rows (the scale columns they begin at are even).
 Fp8TilePlan plan_of(int64_t M, int64_t N, int64_t blocks, int pairs) {
@@ -512,7 +513,8 @@ template <typename T> cudaError_t launch(Fp8Tiles t, const Fp8Layout &l, cudaStr
                                  CU_TENSOR_MAP_SWIZZLE_64B)))
     return cudaErrorInvalidValue;
   // As many tiles of B's rows at a time as stay in L2 beside what streams past them
-  // (16 MB), unless all of them do (8192^3: 450 -> 422 us).
+  // (16 MB), unless all of them do.  In groups / not: 8192^3 410 / 438 us, 8192 x 8192 x
+  // 4096 211 / 236, 2048 rows by [8192, 8192] 108 / 114, 4096 by [8192, 4096] 110 / 106.
   const int64_t bytes = 256 * l.kp;
   t.group = t.plan.tiles_f;
   if (t.plan.tiles_f * bytes > (24 << 20))

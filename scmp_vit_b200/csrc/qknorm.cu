@@ -665,7 +665,8 @@ template <typename F> cudaError_t launch_form(QkNormParams p, cudaStream_t s) {
   const int64_t token_blocks = (tokens + per_block - 1) / per_block;
   // as many heads per unit as leave 24 units for each of the 148 SMs, so that the last
   // ones to run are a small part (12: 8 clips forward 36 us instead of 34); 8 where
-  // elements go one at a time, whose angles cost a unit more than its heads do
+  // elements go one at a time, whose angles cost a unit more than its heads do (odd half
+  // sections, bf16 [32, 257], 24 heads of 128: 87 + 119 us, with 24 units 122 + 152)
   const int64_t all = r.H + r.Hk + (r.v_transposed ? 0 : r.Hk);
   int64_t splits = (148 * (F::V == 1 ? 8 : 24) + token_blocks - 1) / token_blocks;
   splits = splits > all ? all : splits;
