@@ -392,7 +392,10 @@ class Dropout(nn.Module):
     evaluation it passes through.  ``index`` tells the modules of a model apart, which
     may then share ``seed``; ranks that are to draw apart take seeds of their own.
     ``calls`` counts (and, set, repeats) the eager masks; calls that a graph captures
-    count on the device, so that every replay draws masks of its own."""
+    count on the device, so that every replay draws masks of its own.  A call made
+    while a backward pass runs (a checkpoint's recomputation) would take the next mask
+    instead of the one to be repeated, and raises: ``dropout`` with an offset of the
+    caller's own repeats it."""
 
     def __init__(self, p: float, *, per: str = "element", seed: int = 0, index: int = 0):
         super().__init__()
@@ -416,6 +419,10 @@ class Dropout(nn.Module):
     def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
         if not self.active:
             return x if residual is None else residual + x
+        if torch._C._current_graph_task_id() >= 0:
+            raise RuntimeError("a Dropout module called inside a backward pass (by an activation "
+                               "checkpoint?) cannot repeat the mask of its first call; use "
+                               "dropout() with an offset of your own there")
         at = self.index << 48  # (its calls below 2^47, the captured ones above)
         if x.is_cuda and torch.cuda.is_current_stream_capturing():
             state = self.state.clone()

@@ -157,6 +157,28 @@ def test_modules_on_cpu():
     assert not any(type(d) is vit.Dropout for d in m.modules())
 
 
+def test_module_refused_inside_a_backward_pass():
+    """A recomputation would draw the next mask, not the first call's."""
+    m = vit.Dropout(0.5)
+    message = []
+
+    class Recomputed(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x):
+            return x * 1
+
+        @staticmethod
+        def backward(ctx, dy):
+            with pytest.raises(RuntimeError, match="inside a backward pass") as e:
+                m(dy)
+            message.append(e.value)
+            return m.eval()(dy)  # (what drops nothing may be called)
+
+    x = torch.ones(3, requires_grad=True)
+    Recomputed.apply(x).sum().backward()
+    assert message and m.calls == 0 and torch.equal(x.grad, torch.ones(3))
+
+
 # ------------------------------------------------------------ GPU
 
 @pytest.mark.gpu
@@ -350,6 +372,26 @@ def test_in_the_blocks(cuda_device, fused):
         assert all(p.grad is None or bool(p.grad.isfinite().all()) for p in m.parameters())
     finally:
         vit.set_fused_norm(False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_checkpointed_module_is_refused(cuda_device, reentrant):
+    """With an offset of the caller's own a checkpoint repeats the mask."""
+    from torch.utils.checkpoint import checkpoint
+
+    x = torch.randn(5, 40, device=cuda_device, requires_grad=True)
+    m = vit.Dropout(0.5)
+    with pytest.raises(RuntimeError, match="inside a backward pass"):
+        checkpoint(lambda t: m(t).square(), x, use_reentrant=reentrant).sum().backward()
+
+    def f(t):
+        return vit.dropout(t, 0.5, 3, 4).square().sum()
+
+    checkpoint(f, x, use_reentrant=reentrant).backward()
+    want = x.detach().clone().requires_grad_()
+    f(want).backward()
+    assert torch.equal(x.grad, want.grad)
 
 
 @pytest.mark.gpu
