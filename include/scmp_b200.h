@@ -290,7 +290,11 @@ SCMP_API int scmp_fp8_quantize(const scmp_fp8_quantize_args *args, void *stream)
 SCMP_API int scmp_fp8_dequantize(const void *data, const void *scales, int64_t rows, int64_t K,
                                  void *out, int dtype, void *stream);
 /* out [M, N] = A B^T (+ bias [N]) for quantised A [M, K] and B [N, K]: fp32 sums,
- * rounded once to out_dtype. */
+ * rounded once to out_dtype.  Up to SCMP_FP8_THIN_ROWS rows may take a kernel of their
+ * own (a rule on the sizes).  The tensor core cuts its running sum's low bits off, so
+ * fp32 outputs of more than 4096 values each are summed in pieces of at most that
+ * many, one launch each, added up in out; all others take one launch.  Numbers below
+ * fp32's normal range may become 0. */
 typedef struct scmp_fp8_matmul_args {
   int32_t abi_version;
   int32_t bias_dtype;
@@ -314,7 +318,8 @@ SCMP_API int scmp_fp8_linear(const void *x, int x_dtype, int64_t ld,
  * rows and W [N, K] in squares; y is of x's type.  saved_x and saved_weight
  * (nullable: not wanted) receive the transposes' codes for the backward pass,
  * scmp_fp8_train_saved_size(M, K) and (N, K) bytes.  The workspace
- * (scmp_fp8_train_workspace, backward 0) holds codes.  Three launches. */
+ * (scmp_fp8_train_workspace, backward 0) holds codes.  Two launches and the
+ * product's. */
 typedef struct scmp_fp8_train_args {
   int32_t abi_version;
   int32_t dtype, weight_dtype, bias_dtype;
@@ -331,7 +336,8 @@ SCMP_API int scmp_fp8_train_forward(const scmp_fp8_train_args *args, void *strea
 /* Its gradients from dy [M, N] of y's type, rows `ld` apart (each nullable: not
  * wanted): dx [M, K] = Q(dy) Q(W), dy quantised along its rows; dweight [N, K] =
  * Q(dy)^T Q(x), both quantised along their columns; dbias [N] = the column sums of dy
- * (not quantised).  Deterministic.  Up to four launches. */
+ * (not quantised).  Deterministic.  One launch, one more with dbias, and the
+ * products'. */
 typedef struct scmp_fp8_train_bwd_args {
   int32_t abi_version;
   int32_t dtype, weight_dtype, bias_dtype;
@@ -501,7 +507,7 @@ SCMP_API int scmp_debug_mx_plan(int64_t M, int64_t N, int64_t K, int pairs, int3
 
 /* The same for an 8-bit product: plan[0] as above, plan[1] and plan[2] = rows of A
  * per tile, in turn (plan[2] 0: all alike), plan[3] = units of 256 rows of B by
- * the sum of the two. */
+ * the sum of the two, of a launch that sums all of K. */
 SCMP_API int scmp_debug_fp8_plan(int64_t M, int64_t N, int64_t K, int pairs, int32_t *plan);
 
 /* Roofline probe (synchronous; allocates a small scratch buffer): runs a

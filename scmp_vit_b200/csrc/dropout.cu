@@ -5,9 +5,11 @@
 // No mask is stored: the backward pass calls the same kernel on the gradient and
 // draws the same words.
 //
-// span 1: a thread takes eight consecutive elements, two blocks of the generator
-// (40 wide multiplications), which HBM hides: 16-byte loads, one launch, each
-// element read and written once.  Longer spans draw once per piece of elements.
+// A thread takes eight consecutive elements: 16-byte loads, one launch, each element
+// read and written once.  With spans of many elements that is bound by HBM: bf16
+// [64, 257, 4096] per sample 43 us, a copy of it 42.6; fp32 per element 84 us (6.4 TB/s).
+// 16-bit elements that all draw are bound by instructions: two blocks of the generator
+// (40 wide multiplications) for 32 bytes moved, 59 us, with a residual 64.
 #include "dropout.cuh"
 
 #include <cstring>
@@ -123,7 +125,9 @@ __device__ __forceinline__ void draws(const DropoutParams &p, I i, uint64_t offs
 }
 
 // steps() x 8 elements per thread, all loads first.  kDraw 0: nothing is dropped, 1: a
-// draw per element, 2: per span.
+// draw per element, 2: per span.  Two steps for 16-bit types that HBM bounds (bf16 as
+// above, per sample 43 us, with one step 58; per element 61, one 59; fp32 84 either way,
+// [257, 1024] 2.0 and 1.7).
 template <typename T, int kDraw> __host__ __device__ constexpr int steps() {
   return sizeof(T) == 2 && kDraw != 1 ? 2 : 1;
 }

@@ -3,7 +3,10 @@
 // Rows alone: a warp takes 512 or 1024 columns of a row, a half-warp a block.
 // With the transpose, or in squares: a block of threads takes a 128 x 128 tile,
 // which it reads once; its columns' codes leave through shared memory as rows of
-// the transpose.  Both are bound by HBM (read once, written once or twice).
+// the transpose.  Rows are bound by HBM, read once and written once (bf16 16448 x 4096:
+// 37 us, 5.5 TB/s; fp32 51 us, 6.6 TB/s; back to bf16 33 us); tiles by instructions, two
+// roundings and a scale's search per element (bf16 both orders 55 us where the bytes
+// take 41, squares in both 49).
 #include "chunk.cuh"
 #include "fp8_common.cuh"
 

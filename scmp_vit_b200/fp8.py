@@ -340,7 +340,8 @@ def fp8_linear(x: torch.Tensor, weight: torch.Tensor,
     Sums in fp32, each result rounded once to its tensor's type.  Differentiable
     (once, backward) in all three, as if Q passed gradients through.  Kept for the
     backward pass are codes only, one byte per element of ``x`` and ``weight``.
-    The weight is quantised in every call."""
+    The weight is quantised in every call.  Under autocast as anywhere else y is of
+    x's own type."""
     _check_input(x, "fp8_linear")
     dtype_code(weight.dtype, "weight")
     if weight.dim() != 2 or weight.shape[0] < 1 or weight.shape[1] < 1:
