@@ -619,10 +619,12 @@ def split_qkv_norm(qkv: torch.Tensor, num_heads: int, q_weight: torch.Tensor,
     if param_dtype != qkv.dtype and param_dtype != torch.float32:
         raise TypeError(f"parameters must be {qkv.dtype} or float32, got {param_dtype}")
     weights = (q_weight, k_weight, q_bias, k_bias)
-    for name, w in zip(("q_weight", "k_weight", "q_bias", "k_bias"), weights):
-        if w is None and "bias" in name:
+    size = (D,)
+    for i, w in enumerate(weights):
+        if w is None and i >= 2:
             continue
-        if w.shape != (D,) or w.dtype != param_dtype or w.get_device() != index:
+        if w.shape != size or w.dtype != param_dtype or w.get_device() != index:
+            name = ("q_weight", "k_weight", "q_bias", "k_bias")[i]
             raise ValueError(f"{name} must be [{D}] of {param_dtype} on {qkv.device}, got "
                              f"{tuple(w.shape)} {w.dtype} {w.device}")
     if (axes is None) != (pos is None):
@@ -630,7 +632,7 @@ def split_qkv_norm(qkv: torch.Tensor, num_heads: int, q_weight: torch.Tensor,
     table = None
     if axes is not None:
         if (pos.dtype != torch.int32 or pos.get_device() != index
-                or tuple(pos.shape) not in ((N, n_axes), (B, N, n_axes))):
+                or pos.shape != (N, n_axes) and pos.shape != (B, N, n_axes)):
             raise ValueError(f"pos must be int32 [{N}, {n_axes}] or [{B}, {N}, {n_axes}] on "
                              f"{qkv.device}, got {pos.dtype} {tuple(pos.shape)} {pos.device}")
         table = axes.table_bits

@@ -207,7 +207,7 @@ def fp8_matmul(a: Union[torch.Tensor, FP8Tensor], b: FP8Tensor, *,
         rows = a.numel() // K
         if not _thin(rows, N, K):
             data, scales = _sizes(rows, K)
-            codes = torch.empty(data + scales, dtype=torch.uint8, device=a.device)
+            codes = a.new_empty(data + scales, dtype=torch.uint8)  # (cheaper than torch.empty)
             a_ptr = codes.data_ptr()
             a_scales_ptr = a_ptr + data
     else:
@@ -218,7 +218,8 @@ def fp8_matmul(a: Union[torch.Tensor, FP8Tensor], b: FP8Tensor, *,
     if not given:
         dtype = a.dtype if out_dtype is None else out_dtype
         out_code = dtype_code(dtype, "out")
-        out = torch.empty(shape, dtype=dtype, device=b.device)
+        out = (a.new_empty(shape, dtype=dtype) if plain else
+               torch.empty(shape, dtype=dtype, device=b.device))
     else:
         if (tuple(out.shape) != shape or not out.is_contiguous() or out.get_device() != index
                 or out_dtype not in (None, out.dtype)):
@@ -263,7 +264,7 @@ def _train_sizes(M: int, N: int, K: int) -> Tuple[int, int, int, int]:
 def _train_forward(x, weight, bias, save_x: bool, save_weight: bool):
     """(y, codes of x^T and of weight^T in one buffer or None, where the second begins)."""
     N, K = weight.shape
-    y = torch.empty((*x.shape[:-1], N), dtype=x.dtype, device=x.device)
+    y = x.new_empty((*x.shape[:-1], N))
     index = x.get_device()
     xr, ld = _rows_of(x)
     M = x.numel() // K
@@ -272,12 +273,11 @@ def _train_forward(x, weight, bias, save_x: bool, save_weight: bool):
     wr, weight_ld = _rows_of(weight)
     bias = bias if bias is None or bias.is_contiguous() else bias.detach().contiguous()
     workspace, _, x_bytes, w_bytes = _train_sizes(M, N, K)
-    ws = torch.empty(workspace, dtype=torch.uint8, device=x.device)
+    ws = x.new_empty(workspace, dtype=torch.uint8)
     x_bytes = x_bytes if save_x else 0  # (multiples of 256)
     saved, ptr = None, 0
     if save_x or save_weight:
-        saved = torch.empty(x_bytes + (w_bytes if save_weight else 0), dtype=torch.uint8,
-                            device=x.device)
+        saved = x.new_empty(x_bytes + (w_bytes if save_weight else 0), dtype=torch.uint8)
         ptr = saved.data_ptr()
     args = _lib.PACK_FP8_TRAIN.pack(
         _lib.ABI_VERSION, DTYPE[x.dtype], DTYPE[weight.dtype],
@@ -305,17 +305,17 @@ class _FP8Linear(torch.autograd.Function):
     def backward(ctx, dy):
         (saved,) = ctx.saved_tensors
         x_shape, (N, K), dtype, weight_dtype, bias_dtype = ctx.like
-        wants, device = ctx.needs_input_grad, dy.device
+        wants = ctx.needs_input_grad
         M = math.prod(x_shape[:-1])
-        new = torch.zeros if M == 0 else torch.empty  # (no rows: sums of nothing)
-        dx = new(x_shape, dtype=dtype, device=device) if wants[0] else None
-        dw = new((N, K), dtype=weight_dtype, device=device) if wants[1] else None
-        db = new(N, dtype=bias_dtype, device=device) if wants[2] else None
+        new = dy.new_zeros if M == 0 else dy.new_empty  # (no rows: sums of nothing)
+        dx = new(x_shape, dtype=dtype) if wants[0] else None
+        dw = new((N, K), dtype=weight_dtype) if wants[1] else None
+        db = new(N, dtype=bias_dtype) if wants[2] else None
         if M:
             dyr, ld = _rows_of(dy)
             size = _train_sizes(M, N, K)[1]
             ptr = 0 if saved is None else saved.data_ptr()
-            ws = torch.empty(size, dtype=torch.uint8, device=device)
+            ws = dy.new_empty(size, dtype=torch.uint8)
             args = _lib.PACK_FP8_TRAIN_BWD.pack(
                 _lib.ABI_VERSION, DTYPE[dtype], DTYPE[weight_dtype],
                 0 if db is None else DTYPE[bias_dtype], dyr.data_ptr(),
