@@ -5,9 +5,10 @@
 // which it reads once; its columns' codes leave through shared memory as rows of
 // the transpose.  Rows are bound by HBM, read once and written once (bf16 16448 x 4096:
 // 37 us, 5.5 TB/s; fp32 51 us, 6.6 TB/s; back to bf16 33 us); tiles by instructions, two
-// roundings and a scale's search per element (bf16 both orders 55 us where the bytes
-// take 41, squares in both 49).
+// roundings and a scale's search per element (bf16 both orders 50 us where the bytes
+// take 41, squares in both 45).
 #include "chunk.cuh"
+#include "f32x2.cuh"
 #include "fp8_common.cuh"
 
 namespace scmp {
@@ -114,8 +115,10 @@ template <typename T> struct Magnitude {
 // of row c at u ^ (c / 8 % 16): what 16 threads store at a time, 8 rows apart, and
 // what they load along a row both spread over all banks (in plain order the stores'
 // conflicts took the bf16 tile of 128 x 128 from 4 to 12 us).
+// (16-bit tiles in both orders with three blocks an SM 53 us, with four 50; with sums or
+// unaligned they would spill: a step with a bias 2 us more)
 template <typename T, bool kVec, bool kSquare, bool kSums>
-__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : 3)
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : kVec && !kSums ? 4 : 3)
     fp8_tile_kernel(const T *__restrict__ x, const __grid_constant__ TileArgs a) {
   using Mag = Magnitude<T>;
   constexpr int kWords = Mag::kWords;
@@ -277,8 +280,8 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : 3)
       uint32_t codes[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const float2 u = two(i, 4 * h), w = two(i, 4 * h + 2);
-        codes[h] = e4m3x4(u.x * inv, u.y * inv, w.x * inv, w.y * inv);
+        const float2 u = mul2(two(i, 4 * h), both(inv)), w = mul2(two(i, 4 * h + 2), both(inv));
+        codes[h] = e4m3x4(u.x, u.y, w.x, w.y);
       }
       if (i < live_r)  // (columns up to the end of the block are the row's)
         *reinterpret_cast<uint2 *>(to) = make_uint2(codes[0], codes[1]);
@@ -297,14 +300,14 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : 3)
     // column j's eight rows are eight neighbouring bytes of the transpose
 #pragma unroll
     for (int j = 0; j < 8; j += 2) {
-      const float iu = fp8_inverse(col_scale[j]), iw = fp8_inverse(col_scale[j + 1]);
+      const float2 inv = make_float2(fp8_inverse(col_scale[j]), fp8_inverse(col_scale[j + 1]));
       uint32_t u[2], w[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const float2 p = two(4 * h, j), q = two(4 * h + 1, j), r = two(4 * h + 2, j),
-                     t = two(4 * h + 3, j);
-        u[h] = e4m3x4(p.x * iu, q.x * iu, r.x * iu, t.x * iu);
-        w[h] = e4m3x4(p.y * iw, q.y * iw, r.y * iw, t.y * iw);
+        const float2 p = mul2(two(4 * h, j), inv), q = mul2(two(4 * h + 1, j), inv),
+                     r = mul2(two(4 * h + 2, j), inv), t = mul2(two(4 * h + 3, j), inv);
+        u[h] = e4m3x4(p.x, q.x, r.x, t.x);
+        w[h] = e4m3x4(p.y, q.y, r.y, t.y);
       }
       uint8_t *at = turned + (piece * 8 + j) * 128 + (rg ^ piece) * 8;
       *reinterpret_cast<uint2 *>(at) = make_uint2(u[0], u[1]);
