@@ -5,8 +5,8 @@
 // which it reads once; its columns' codes leave through shared memory as rows of
 // the transpose.  Rows are bound by HBM, read once and written once (bf16 16448 x 4096:
 // 37 us, 5.5 TB/s; fp32 51 us, 6.6 TB/s; back to bf16 33 us); tiles by instructions, two
-// roundings and a scale's search per element (bf16 both orders 50 us where the bytes
-// take 41, squares in both 45).
+// roundings and the search for two scales per element (bf16 both orders 45 us where the
+// bytes take 41, squares in both 45, squares alone 32).
 #include "chunk.cuh"
 #include "f32x2.cuh"
 #include "fp8_common.cuh"
@@ -115,8 +115,9 @@ template <typename T> struct Magnitude {
 // of row c at u ^ (c / 8 % 16): what 16 threads store at a time, 8 rows apart, and
 // what they load along a row both spread over all banks (in plain order the stores'
 // conflicts took the bf16 tile of 128 x 128 from 4 to 12 us).
-// (16-bit tiles in both orders with three blocks an SM 53 us, with four 50; with sums or
-// unaligned they would spill: a step with a bias 2 us more)
+// (16-bit tiles in both orders with three blocks an SM 53 us, with four 50, and 45 since
+// each scale is found by one thread instead of sixteen; with sums or unaligned, four would
+// spill: a step with a bias 2 us more)
 template <typename T, bool kVec, bool kSquare, bool kSums>
 __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : kVec && !kSums ? 4 : 3)
     fp8_tile_kernel(const T *__restrict__ x, const __grid_constant__ TileArgs a) {
@@ -125,6 +126,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : kVec && !kSums 
   __shared__ __align__(16) uint8_t turned[128 * 128];
   __shared__ __align__(16) uint32_t warp_max[8][16 * kWords];
   __shared__ __align__(16) float warp_sum[kSums ? 8 : 1][128];
+  __shared__ __align__(16) float col_inv[128];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int rg = threadIdx.x >> 4, piece = threadIdx.x & 15;
@@ -177,7 +179,10 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : kVec && !kSums 
     }
     row_max[i] = sizeof(T) == 4 ? m : Mag::most(m, __funnelshift_r(m, m, 16));
   }
-  uint32_t row_scale[8], col_scale[8];
+  // scales: of a row from the lane of its number (the half-warp's rows), of a column from
+  // the thread of its number, others get what to multiply by
+  uint32_t row_scale = 0, square_scale = 0;
+  float row_inv[8];
   if (kSquare) {
     uint32_t m = row_max[0];
 #pragma unroll
@@ -187,29 +192,34 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : kVec && !kSums 
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < 8; ++w) m = max(m, warp_max[0][w]);
-    const uint32_t s = fp8_scale(Mag::bits(m));
+    row_scale = square_scale = fp8_scale(Mag::bits(m));
 #pragma unroll
-    for (int i = 0; i < 8; ++i) row_scale[i] = col_scale[i] = s;
+    for (int i = 0; i < 8; ++i) row_inv[i] = fp8_inverse(row_scale);
   } else {
     if (a.data) {
+      uint32_t m = 0;  // of row piece % 8
       if constexpr (sizeof(T) == 2) {  // two rows at a time
 #pragma unroll
         for (int i = 0; i < 8; i += 2) {
-          uint32_t m = __byte_perm(row_max[i], row_max[i + 1], 0x5410);
+          uint32_t u = __byte_perm(row_max[i], row_max[i + 1], 0x5410);
 #pragma unroll
-          for (int o = 1; o < 16; o <<= 1) m = Mag::most(m, __shfl_xor_sync(~0u, m, o));
-          row_scale[i] = fp8_scale(Mag::bits(m & 0xFFFFu));
-          row_scale[i + 1] = fp8_scale(Mag::bits(m >> 16));
+          for (int o = 1; o < 16; o <<= 1) u = Mag::most(u, __shfl_xor_sync(~0u, u, o));
+          if ((piece & 6) == i) m = u;
         }
+        m = piece & 1 ? m >> 16 : m & 0xFFFFu;
       } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          uint32_t m = row_max[i];
+          uint32_t u = row_max[i];
 #pragma unroll
-          for (int o = 1; o < 16; o <<= 1) m = max(m, __shfl_xor_sync(~0u, m, o));
-          row_scale[i] = fp8_scale(m);
+          for (int o = 1; o < 16; o <<= 1) u = max(u, __shfl_xor_sync(~0u, u, o));
+          if ((piece & 7) == i) m = u;
         }
       }
+      row_scale = fp8_scale(Mag::bits(m));
+      const float inv = fp8_inverse(row_scale);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) row_inv[i] = __shfl_sync(~0u, inv, (lane & 16) + i);
     }
 #pragma unroll
     for (int w = 0; w < kWords; ++w)
@@ -241,27 +251,17 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : kVec && !kSums 
       }
     }
     __syncthreads();
-    if (a.t_data) {
+    if (a.t_data && threadIdx.x < 128) {
+      uint32_t m = 0;  // (patterns of magnitudes, a NaN's the largest)
 #pragma unroll
-      for (int w = 0; w < kWords; w += 4) {
-        uint4 m = make_uint4(0, 0, 0, 0);
-#pragma unroll
-        for (int q = 0; q < 8; ++q) {
-          const uint4 v = *reinterpret_cast<const uint4 *>(&warp_max[q][piece * kWords + w]);
-          m = make_uint4(Mag::most(m.x, v.x), Mag::most(m.y, v.y), Mag::most(m.z, v.z),
-                         Mag::most(m.w, v.w));
-        }
-        const uint32_t ms[4] = {m.x, m.y, m.z, m.w};
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          if constexpr (sizeof(T) == 4) {
-            col_scale[w + q] = fp8_scale(ms[q]);
-          } else {
-            col_scale[2 * q] = fp8_scale(Mag::bits(ms[q] & 0xFFFFu));
-            col_scale[2 * q + 1] = fp8_scale(Mag::bits(ms[q] >> 16));
-          }
-        }
-      }
+      for (int q = 0; q < 8; ++q)
+        m = max(m, sizeof(T) == 4
+                       ? warp_max[q][threadIdx.x]
+                       : (uint32_t) reinterpret_cast<const uint16_t *>(warp_max[q])[threadIdx.x]);
+      const uint32_t scale = fp8_scale(Mag::bits(m));
+      const int64_t c = tile_c * 128 + threadIdx.x;
+      col_inv[threadIdx.x] = fp8_inverse(scale);
+      a.t_scales[fp8_scale_at(c, tile_r, a.cols.groups)] = (uint8_t)(c < K ? scale : 0u);
     }
     if (kSums && threadIdx.x < 128 && tile_c * 128 + threadIdx.x < K) {
       float t = 0.0f;
@@ -271,36 +271,36 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : kVec && !kSums 
     }
   }
 
-  const int live_r = (int)(rows - r0 < 8 ? rows - r0 : 8), live_c = (int)(K - c0 < 8 ? K - c0 : 8);
+  const int live_r = (int)(rows - r0 < 8 ? rows - r0 : 8);
   if (a.data) {
     uint8_t *to = a.data + r0 * a.rows.kp + c0;
 #pragma unroll
     for (int i = 0; i < 8; ++i, to += a.rows.kp) {
-      const float inv = fp8_inverse(row_scale[i]);
       uint32_t codes[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const float2 u = mul2(two(i, 4 * h), both(inv)), w = mul2(two(i, 4 * h + 2), both(inv));
+        const float2 u = mul2(two(i, 4 * h), both(row_inv[i])),
+                     w = mul2(two(i, 4 * h + 2), both(row_inv[i]));
         codes[h] = e4m3x4(u.x, u.y, w.x, w.y);
       }
       if (i < live_r)  // (columns up to the end of the block are the row's)
         *reinterpret_cast<uint2 *>(to) = make_uint2(codes[0], codes[1]);
     }
-    if (piece == 0) {  // (eight rows of a scale atom are 16 bytes apart)
-      uint8_t *at = a.scales + fp8_scale_at(r0, tile_c, a.rows.groups);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) at[16 * i] = (uint8_t)(i < live_r ? row_scale[i] : 0u);
-    }
+    if (piece < 8)  // (eight rows of a scale atom are 16 bytes apart)
+      a.scales[fp8_scale_at(r0, tile_c, a.rows.groups) + 16 * piece] =
+          (uint8_t)(piece < live_r ? row_scale : 0u);
     // the last tile of a row also fills its last scale word
     if (tile_c == a.rows.blocks - 1 && threadIdx.x < 128)
       for (int64_t b = a.rows.blocks; b < a.rows.groups * 4; ++b)
         a.scales[fp8_scale_at(tile_r * 128 + threadIdx.x, b, a.rows.groups)] = 0;
   }
   if (a.t_data) {
+    if (!kSquare) __syncthreads();  // col_inv
     // column j's eight rows are eight neighbouring bytes of the transpose
 #pragma unroll
     for (int j = 0; j < 8; j += 2) {
-      const float2 inv = make_float2(fp8_inverse(col_scale[j]), fp8_inverse(col_scale[j + 1]));
+      const float2 inv = kSquare ? both(row_inv[0])
+                                 : *reinterpret_cast<const float2 *>(&col_inv[piece * 8 + j]);
       uint32_t u[2], w[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -313,10 +313,9 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : kVec && !kSums 
       *reinterpret_cast<uint2 *>(at) = make_uint2(u[0], u[1]);
       *reinterpret_cast<uint2 *>(at + 128) = make_uint2(w[0], w[1]);
     }
-    if (rg == 0) {
-      uint8_t *to = a.t_scales + fp8_scale_at(c0, tile_r, a.cols.groups);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) to[16 * j] = (uint8_t)(j < live_c ? col_scale[j] : 0u);
+    if (kSquare && threadIdx.x < 128) {
+      const int64_t c = tile_c * 128 + threadIdx.x;
+      a.t_scales[fp8_scale_at(c, tile_r, a.cols.groups)] = (uint8_t)(c < K ? square_scale : 0u);
     }
     if (tile_r == a.cols.blocks - 1 && threadIdx.x < 128)
       for (int64_t b = a.cols.blocks; b < a.cols.groups * 4; ++b)
