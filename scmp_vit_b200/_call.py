@@ -19,6 +19,18 @@ except AttributeError:
     _current_device = torch.cuda.current_device
 
 
+try:
+    _graph_task = torch._C._current_graph_task_id
+except AttributeError:  # (a torch that does not tell)
+    def _graph_task() -> int:
+        return -1
+
+
+def in_backward() -> bool:
+    """Whether this thread is inside a backward pass."""
+    return _graph_task() >= 0
+
+
 def call(fn, index: int, *args) -> None:
     """``fn(*args, stream)`` on CUDA device ``index`` and its current stream;
     raises on a non-zero status."""

@@ -31,7 +31,8 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from . import _lib
-from ._call import DTYPE, call, has_tangent, in_dual_level, once_differentiable
+from ._call import (DTYPE, call, has_tangent, in_backward, in_dual_level,
+                    once_differentiable)
 from .attention import GridRotary, QKNorm, make_sc_attention_forward
 from .fp8 import FP8Linear
 from .head_aligned_comp import HeadAlignedSCLinear
@@ -419,7 +420,7 @@ class Dropout(nn.Module):
     def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
         if not self.active:
             return x if residual is None else residual + x
-        if torch._C._current_graph_task_id() >= 0:
+        if in_backward():
             raise RuntimeError("a Dropout module called inside a backward pass (by an activation "
                                "checkpoint?) cannot repeat the mask of its first call; use "
                                "dropout() with an offset of your own there")
