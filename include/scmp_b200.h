@@ -291,10 +291,12 @@ SCMP_API int scmp_fp8_dequantize(const void *data, const void *scales, int64_t r
                                  void *out, int dtype, void *stream);
 /* out [M, N] = A B^T (+ bias [N]) for quantised A [M, K] and B [N, K]: fp32 sums,
  * rounded once to out_dtype.  Up to SCMP_FP8_THIN_ROWS rows may take a kernel of their
- * own (a rule on the sizes).  The tensor core cuts its running sum's low bits off, so
- * fp32 outputs of more than 4096 values each are summed in pieces of at most that
- * many, one launch each, added up in out; all others take one launch.  Numbers below
- * fp32's normal range may become 0. */
+ * own (a rule on the sizes).  The tensor core cuts its running sum's low bits off, at
+ * most 9 * 2^-23 of it per 32 values (of positive values over many powers of two a
+ * twentieth of that on average over 4096, a ninth over 500000).  So fp32 outputs of more than 4096 values each are summed
+ * in pieces of at most that many, one launch each, added up rounded in out; 16-bit
+ * outputs take one launch, and above 16384 values (fp16) or 131072 (bf16) go in pieces of
+ * 1024, added up rounded in fp32.  Numbers below fp32's normal range may become 0. */
 typedef struct scmp_fp8_matmul_args {
   int32_t abi_version;
   int32_t bias_dtype;
@@ -507,7 +509,7 @@ SCMP_API int scmp_debug_mx_plan(int64_t M, int64_t N, int64_t K, int pairs, int3
 
 /* The same for an 8-bit product: plan[0] as above, plan[1] and plan[2] = rows of A
  * per tile, in turn (plan[2] 0: all alike), plan[3] = units of 256 rows of B by
- * the sum of the two, of a launch that sums all of K. */
+ * the sum of the two, of a launch that sums all of K, in one piece. */
 SCMP_API int scmp_debug_fp8_plan(int64_t M, int64_t N, int64_t K, int pairs, int32_t *plan);
 
 /* Roofline probe (synchronous; allocates a small scratch buffer): runs a

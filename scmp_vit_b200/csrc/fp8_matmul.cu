@@ -27,6 +27,9 @@
 // registers 42), and operands on their way in wait.  One stage of B for both accumulators
 // loads 27 % less, but then their tiles end together: fc1 63 us, K = 4096 186 for 193.
 //
+// Where a sum is so long that the bits that the tensor core cuts off would show, it is
+// made in pieces (kPieces, kWholeBlocks).
+//
 // Warps: 0 loads, 1 issues MMAs (even CTA), 2 owns the tensor memory, 4-19 run
 // the epilogue.  Every wait is bounded: a wait that gives up raises the error
 // word and the pair drains.
@@ -44,6 +47,7 @@ constexpr int kEpilogueWarps = 16;
 constexpr int kWide = 256, kNarrow = 192;  // rows of A: the accumulators' columns
 constexpr int kPerStage = 2;               // blocks of K per stage
 constexpr int kStages = 3;
+constexpr int kPieceCols = 128;            // of a sum in pieces, at most
 constexpr uint32_t kScaleCol = kWide + kNarrow;
 constexpr uint32_t kScaleCols = 4 + 12;  // of an atom of B, three of A
 
@@ -71,6 +75,7 @@ struct Fp8Tiles {
   int xrows;               // row groups (of 128) that a tile's scales of A touch, at most
   int block0, blocks;      // blocks of K of this launch
   int steps;               // stages per tile
+  int piece;               // stages per piece of a sum in pieces
   bool tma_out;            // 16-bit rows of whole 16-byte pieces: stored by TMA
   bool words;              // else: 16-bit outputs are stored two features at a time
   bool add;                // fp32 outputs: added to what is there
@@ -148,7 +153,9 @@ __device__ __forceinline__ void store_transposed(uint32_t addr, uint32_t a, uint
                : "memory");
 }
 
-template <typename T>
+// kPieces: a tile's sum in pieces, each in the one or the other accumulator, which the
+// epilogue's warps add up in registers, 32 of at most 128 columns each.
+template <typename T, bool kPieces>
 __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
     fp8_pair_kernel(const __grid_constant__ Fp8Tiles t, const __grid_constant__ CUtensorMap wmap,
                     const __grid_constant__ CUtensorMap xmap0,
@@ -166,8 +173,8 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
   volatile int *abort = reinterpret_cast<volatile int *>(tmem_slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
-  // one accumulator: all epilogue warps read it
-  const bool alone = t.plan.w[1] == 0 && t.plan.w[0] > kNarrow;
+  // one accumulator (or one at a time): all epilogue warps read it
+  const bool alone = kPieces || (t.plan.w[1] == 0 && t.plan.w[0] > kNarrow);
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
@@ -256,50 +263,55 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
     // the whole warp walks the stages and one elected lane issues: loop state
     // and descriptors stay warp-uniform, and so does what the instructions read
     int stage = 0;
-    uint32_t phase = 0, set = 0, uses[2] = {0, 0};
+    uint32_t phase = 0, set = 0, turn = 0, uses[2] = {0, 0};
     const uint64_t desc0 = smem_desc_sw128(smem0);
     const uint64_t sdesc0 = scale_desc(smem0 + kScalesAt);
-    for_tiles(t, [&](int, int n0, int sub, uint32_t buf) {
-      const uint32_t use = buf ? uses[1]++ : uses[0]++;
-      if (use > 0 && !warp_wait_cl(&tempty[buf], (use - 1) & 1, abort)) return false;
-      tc_fence_after();
-      const uint32_t acc = tmem + buf * kWide;
+    for_tiles(t, [&](int, int n0, int sub, uint32_t of_tile) {
       const uint32_t w = (uint32_t)t.plan.w[sub], id0 = idesc((int)w);
       const uint32_t xblock = w / 2 * kRowBytes, offset = ((uint32_t)n0 & 127u) / 32;
-      for (int kb = 0; kb < t.steps; ++kb) {
-        if (!warp_wait_cl(&full[stage], phase, abort)) return false;
+      int kb = 0;
+      do {
+        const uint32_t buf = kPieces ? turn++ & 1 : of_tile;
+        const uint32_t use = buf ? uses[1]++ : uses[0]++;
+        if (use > 0 && !warp_wait_cl(&tempty[buf], (use - 1) & 1, abort)) return false;
         tc_fence_after();
-        // consecutive atoms of scales use two sets of columns in turn
-        const bool first = kb % (4 / kPerStage) == 0;
-        if (first) set ^= 1;
-        const uint32_t sw = tmem + kScaleCol + set * kScaleCols, sx = sw + 4;
-        const uint64_t d = desc_add(desc0, (uint32_t)stage * kStage);
-        const uint64_t dx = desc_add(d, kPerStage * kW);
-        if (elect_one()) {
-          if (first) {
-            const uint64_t ds = desc_add(sdesc0, (uint32_t)stage * kScales);
-            copy_scales(sw, ds);
-            for (int i = 0; i < t.xrows; ++i)
-              copy_scales(sx + 4 * i, desc_add(ds, 512 + 512 * i));
-          }
+        const uint32_t acc = tmem + buf * kWide;
+        const int begin = kb, end = kPieces && kb + t.piece < t.steps ? kb + t.piece : t.steps;
+        for (; kb < end; ++kb) {
+          if (!warp_wait_cl(&full[stage], phase, abort)) return false;
+          tc_fence_after();
+          // consecutive atoms of scales use two sets of columns in turn
+          const bool first = kb % (4 / kPerStage) == 0;
+          if (first) set ^= 1;
+          const uint32_t sw = tmem + kScaleCol + set * kScaleCols, sx = sw + 4;
+          const uint64_t d = desc_add(desc0, (uint32_t)stage * kStage);
+          const uint64_t dx = desc_add(d, kPerStage * kW);
+          if (elect_one()) {
+            if (first) {
+              const uint64_t ds = desc_add(sdesc0, (uint32_t)stage * kScales);
+              copy_scales(sw, ds);
+              for (int i = 0; i < t.xrows; ++i)
+                copy_scales(sx + 4 * i, desc_add(ds, 512 + 512 * i));
+            }
 #pragma unroll
-          for (int b = 0; b < kPerStage; ++b) {
-            if (b > 0 && kb * kPerStage + b >= t.blocks) break;  // past K
-            const uint32_t id = idesc_byte(id0, (uint32_t)(kb * kPerStage + b) & 3u);
+            for (int b = 0; b < kPerStage; ++b) {
+              if (b > 0 && kb * kPerStage + b >= t.blocks) break;  // past K
+              const uint32_t id = idesc_byte(id0, (uint32_t)(kb * kPerStage + b) & 3u);
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk)
-              mma_pair(acc, desc_add(d, b * kW + kk * 32), desc_add(dx, b * xblock + kk * 32), id,
-                       sw, sx + offset, (kb > 0 || b > 0 || kk > 0) ? 1u : 0u);
+              for (int kk = 0; kk < 4; ++kk)
+                mma_pair(acc, desc_add(d, b * kW + kk * 32), desc_add(dx, b * xblock + kk * 32),
+                         id, sw, sx + offset, (kb > begin || b > 0 || kk > 0) ? 1u : 0u);
+            }
+            tc_commit_pair_both(&empty[stage]);
+            if (kb == end - 1) tc_commit_pair_both(&tfull[buf]);
           }
-          tc_commit_pair_both(&empty[stage]);
-          if (kb == t.steps - 1) tc_commit_pair_both(&tfull[buf]);
+          __syncwarp();
+          if (++stage == kStages) {
+            stage = 0;
+            phase ^= 1;
+          }
         }
-        __syncwarp();
-        if (++stage == kStages) {
-          stage = 0;
-          phase ^= 1;
-        }
-      }
+      } while (kPieces && kb < t.steps);
       return true;
     });
     if (elect_one()) {
@@ -323,8 +335,8 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
     const int first = (int)(alone ? 2 * mine + half : half) * 32, stride = alone ? 128 : 64;
     const uint32_t piece = smem0 + kOutAt + (uint32_t)(warp - 4) * kPiece;
     uint32_t turn = 0;
-    for_tiles(t, [&](int f0, int n0, int sub, uint32_t buf) {
-      if (!alone && buf != mine) return true;
+    for_tiles(t, [&](int f0, int n0, int sub, uint32_t of_tile) {
+      if (!alone && of_tile != mine) return true;
       f0 += (int)rank * 128 + (warp & 3) * 32;
       const auto bias_of = [&](int f) {
         return t.p.bias && f < t.p.N ? load_as_f32(t.p.bias, t.p.bias_dtype, f) : 0.0f;
@@ -334,9 +346,11 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
       for (int i = 0; i < 4; ++i) bias[i] = bias_of(f0 + (by_tma ? 8 * i + (lane >> 2) : lane));
       const int64_t left = t.p.M - n0;
       const int w = t.plan.w[sub], rows = left < w ? (int)left : w;
-      if (!warp_wait_cl(&tfull[buf], turn++ & 1, abort)) return false;
+      uint32_t buf = kPieces ? turn & 1 : of_tile;
+      if (!warp_wait_cl(&tfull[buf], (kPieces ? turn >> 1 : turn) & 1, abort)) return false;
+      ++turn;
       tc_fence_after();
-      const uint32_t acc = tmem + ((uint32_t)((warp & 3) * 32) << 16) + buf * kWide;
+      uint32_t acc = tmem + ((uint32_t)((warp & 3) * 32) << 16) + buf * kWide;
       const auto hand_back = [&] {
         tc_fence_before();
         __syncwarp();
@@ -387,6 +401,30 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
           store_chunk<T, false>(t.p, 1.0f, t.words, v, bias[0], n0 + j0, f, rows - j0, lane);
       };
       uint32_t v[2][32];
+      if constexpr (kPieces) {
+        // v[1]: the sum of the pieces so far
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[1][j] = 0;
+#pragma unroll 1
+        for (int kb = 0;;) {
+          if (first < w) {
+            load(first, v[0]);
+            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              v[1][j] = __float_as_uint(__uint_as_float(v[1][j]) + __uint_as_float(v[0][j]));
+          }
+          hand_back();
+          if ((kb += t.piece) >= t.steps) break;
+          buf = turn & 1;
+          if (!warp_wait_cl(&tfull[buf], turn >> 1 & 1, abort)) return false;
+          ++turn;
+          tc_fence_after();
+          acc = tmem + ((uint32_t)((warp & 3) * 32) << 16) + buf * kWide;
+        }
+        if (first < w) store(first, v[1]);
+        return true;
+      }
       if (first >= w) hand_back();
 #pragma unroll 1
       for (int j0 = first; j0 < w; j0 += 2 * stride) {
@@ -439,8 +477,9 @@ constexpr double kTileNs = 250, kAloneNs = 2000;
 // Widths: one tile for up to 32 rows (16 rows by [16384, 1024]: 6.0 us, a tile of 64
 // 6.7; 32 rows 6.1 and 6.5; [4096, 4096] 9.0 and 9.1); else what costs least among 64, 128 and 192
 // throughout, 256 alone, and 256 and 192 in turn, whose starts are all multiples of
-// 64 rows (the scale columns they begin at are even).
-Fp8TilePlan plan_of(int64_t M, int64_t N, int64_t blocks, int pairs) {
+// 64 rows (the scale columns they begin at are even); among 64 and 128 for a sum in
+// pieces.
+Fp8TilePlan plan_of(int64_t M, int64_t N, int64_t blocks, int pairs, bool pieces = false) {
   Fp8TilePlan best{};
   best.tiles_f = (uint32_t)((N + 255) / 256);
   best.units = best.tiles_f;
@@ -451,6 +490,7 @@ Fp8TilePlan plan_of(int64_t M, int64_t N, int64_t blocks, int pairs) {
   constexpr int kWidths[5][2] = {{kWide, kNarrow}, {kNarrow, 0}, {128, 0}, {64, 0}, {kWide, 0}};
   double best_ns = 0;
   for (const auto &w : kWidths) {
+    if (pieces && w[0] > kPieceCols) continue;
     const int pitch = w[0] + w[1];
     const int64_t units = best.tiles_f * ((M + pitch - 1) / pitch);
     double ns = blocks * block_ns(w[0]) + (w[0] > kNarrow && !w[1] ? kAloneNs : kTileNs);
@@ -467,14 +507,30 @@ Fp8TilePlan plan_of(int64_t M, int64_t N, int64_t blocks, int pairs) {
   return best;
 }
 
-// fp32 outputs of long sums: the tensor core cuts its running sum's low bits off at
-// every MMA, which leaves a relative 3e-6 after 16384 values (1e-7 rounded), so
-// those go in launches of at most this many blocks that add up in the outputs (0.5e-6
-// at 4096 values).  16-bit outputs do not show it.
+// Long sums.  An MMA cuts each of its 32 products off at 2^-25 of the power of two of
+// the largest term (the running sum is one) and what comes out at 2^-23: at most 9 * 2^-23
+// of the running sum per 32 values, all in one direction where all products have one
+// sign.  Positive values over many powers of two (e^(2 z), z normal) lose 0.4 * 2^-23 per
+// 32 on average over 4096 of them (6e-6 of the sum, 3e-5 at most), 0.6 over 16384, 1 over
+// 524288; normal values of both signs a root mean square of 5e-7 of the outputs' over
+// 4096 and 3e-6 over 16384 (rounded 1e-7).
+//
+// fp32 outputs of more than kSumBlocks go in launches of at most so many that add up
+// in the outputs.  16-bit outputs go in one launch, and in pieces of kPieceBlocks that
+// the epilogue adds up, rounded, from where the cut bits would come near the type's
+// half step (2.4e-4 to 4.9e-4 for fp16): above 16384 values for fp16 (4e-5 on average in
+// the case above), eight times that for bf16.  In fp16 that case is 2e-4 off on average
+// over 65536 in one piece and 2e-3 over 524288, in pieces 3e-6 and 1e-6.  Narrower tiles
+// cost time: fp16 1024 rows by [4096, 16512] 71 us (in one piece 53), 4096 by [4096, 32768]
+// 533 (474).
 constexpr int64_t kSumBlocks = 32;
+constexpr int64_t kPieceBlocks = 8;
+template <typename T> constexpr int64_t kWholeBlocks = __is_same(T, __half) ? 128 : 1024;
+static_assert(kPieceBlocks % 4 == 0, "a piece begins with an atom of scales");
 
-template <typename T> cudaError_t launch(Fp8Tiles t, const Fp8Layout &l, cudaStream_t s) {
-  auto kern = fp8_pair_kernel<T>;
+template <typename T, bool kPieces>
+cudaError_t launch(Fp8Tiles t, const Fp8Layout &l, cudaStream_t s) {
+  auto kern = fp8_pair_kernel<T, kPieces>;
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
@@ -504,8 +560,9 @@ template <typename T> cudaError_t launch(Fp8Tiles t, const Fp8Layout &l, cudaStr
   const int64_t launches =
       sizeof(T) == 4 ? (l.blocks + kSumBlocks - 1) / kSumBlocks : 1;
   const int64_t share = ((l.blocks + launches - 1) / launches + 3) / 4 * 4;  // whole scale atoms
-  t.plan = plan_of(t.p.M, t.p.N, launches > 1 ? share : l.blocks, clusters);
+  t.plan = plan_of(t.p.M, t.p.N, launches > 1 ? share : l.blocks, clusters, kPieces);
   const int *w = t.plan.w;
+  t.piece = (int)kPieceBlocks / kPerStage;
   t.xrows = w[0] > kNarrow ? 3 : w[0] > 128 ? 2 : 1;
   t.words = t.p.N % 2 == 0 && (reinterpret_cast<uintptr_t>(t.p.out) & 3) == 0;
   t.tma_out = sizeof(T) == 2 && t.p.N % 8 == 0 &&
@@ -553,6 +610,10 @@ template <typename T> cudaError_t launch(Fp8Tiles t, const Fp8Layout &l, cudaStr
   return cudaSuccess;
 }
 
+template <typename T> cudaError_t launch_16(const Fp8Tiles &t, const Fp8Layout &l, cudaStream_t s) {
+  return l.blocks > kWholeBlocks<T> ? launch<T, true>(t, l, s) : launch<T, false>(t, l, s);
+}
+
 }  // namespace
 
 Fp8TilePlan fp8_tile_plan(int64_t M, int64_t N, int64_t K, int pairs) {
@@ -564,9 +625,9 @@ cudaError_t launch_fp8_matmul(const Fp8Product &p, unsigned int *error, cudaStre
   Fp8Tiles t{};
   t.p = p;
   t.error = error;
-  if (p.out_dtype == SCMP_F32) return launch<float>(t, l, s);
-  if (p.out_dtype == SCMP_BF16) return launch<__nv_bfloat16>(t, l, s);
-  return launch<__half>(t, l, s);
+  if (p.out_dtype == SCMP_F32) return launch<float, false>(t, l, s);
+  if (p.out_dtype == SCMP_BF16) return launch_16<__nv_bfloat16>(t, l, s);
+  return launch_16<__half>(t, l, s);
 }
 
 cudaError_t fp8_set_wait_limit(unsigned long long ns) {

@@ -337,7 +337,8 @@ def fp8_linear(x: torch.Tensor, weight: torch.Tensor,
         dW = Q(dy)^T Q(x)          both in blocks of 128 tokens along their columns
         db = sum of dy over tokens
 
-    Sums in fp32, each result rounded once to its tensor's type.  Differentiable
+    Sums in fp32 (the tensor core's, which are cut off and not rounded; long ones in
+    pieces: ``scmp_fp8_matmul``), each result rounded once to its tensor's type.  Differentiable
     (once, backward) in all three, as if Q passed gradients through.  Kept for the
     backward pass are codes only, one byte per element of ``x`` and ``weight``.
     The weight is quantised in every call.  Under autocast as anywhere else y is of

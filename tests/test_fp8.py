@@ -546,6 +546,94 @@ def test_long_sums(cuda_device):
     close(y, values(qa), values(qw), bias)
 
 
+def one_sign(rows, K, g, device):
+    """Positive values of many magnitudes, rows of different size, whose products sum
+    to a few units: every addition to a long sum has bits below the sum's last one."""
+    x = torch.exp(2 * torch.randn(rows, K, generator=g, device=device) - 2)
+    return x.mul_((1 + torch.rand(rows, 1, generator=g, device=device)) / K ** 0.5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,M,N,K", [
+    (torch.float16, 300, 296, 16384), (torch.float16, 300, 300, 16385),
+    (torch.float16, 40, 299, 70000),
+    (torch.float16, 5, 4100, 20000), (torch.float16, 17, 520, 300000),
+    (torch.float16, 500, 296, 524288), (torch.bfloat16, 300, 296, 131072),
+    (torch.bfloat16, 300, 296, 131073), (torch.bfloat16, 260, 299, 1048576),
+    (torch.float32, 300, 296, 16500)])
+def test_long_sums_of_one_sign(cuda_device, dtype, M, N, K):
+    """Sums of positive products, where cut-off bits all point one way.  An addition
+    of 32 products to a sum cuts each product off at 2^-25 of the sum's power of two and
+    the new sum at 2^-23: at most 32 * 2^-25 + 2^-23 = 9 * 2^-23 of the sum.  Up to 16384
+    values (fp16 outputs) and 131072 (bf16) are one sum, fp32 outputs add up launches of
+    at most 4096; longer 16-bit ones go in pieces of 1024 (32 additions), which are added
+    up rounded (2^-24 each, the bias 2^-24)."""
+    g = torch.Generator(device=cuda_device).manual_seed(K)
+    qa, qw = (fp8.fp8_quantize(one_sign(rows, K, g, cuda_device)) for rows in (M, N))
+    bias = torch.rand(N, generator=g, device=cuda_device)
+    y = fp8.fp8_matmul(qa, qw, bias=bias, out_dtype=dtype)
+    torch.cuda.synchronize()
+    assert _lib.engine_status() == 0
+    ref = torch.zeros(M, N, dtype=torch.float64, device=cuda_device)
+    a, w = (q.dequantize(torch.float32) for q in (qa, qw))
+    for k in range(0, K, 65536):
+        ref += a[:, k:k + 65536].double() @ w[:, k:k + 65536].double().t()
+    ref += bias.double()
+    whole, piece = {torch.float16: (16384, 1024), torch.bfloat16: (131072, 1024),
+                    torch.float32: (4096, 4096)}[dtype]
+    pieces = 1 if K <= whole else -(-K // piece)
+    cut = (K if K <= whole else piece) / 32 * 9 * 2.0 ** -23
+    half = torch.finfo(dtype).eps / 2
+    err = ((y.double() - ref) / ref).abs()
+    assert float(err.max()) <= (cut + (pieces + 2) * 2.0 ** -24) * (1 + half) + half
+    assert torch.equal(y, fp8.fp8_matmul(qa, qw, bias=bias, out_dtype=dtype))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,N", [(16, 264), (40, 257), (300, 130), (1500, 2100)])
+def test_long_sums_are_exact_where_sums_are(cuda_device, M, N):
+    """Sums in pieces of whole numbers, both signs: every partial sum is exact, so each
+    piece, and what the last one leaves, counts once; several tiles per pair."""
+    g = torch.Generator().manual_seed(M)
+    K = 20 * 4096 + 300
+    a = torch.randint(-2, 3, (M, K), generator=g, dtype=torch.int8).to(cuda_device).half()
+    w = torch.randint(-2, 3, (N, K), generator=g, dtype=torch.int8).to(cuda_device).half()
+    bias = torch.randint(-500, 501, (N,), generator=g).float().to(cuda_device)
+    ref = a.double() @ w.double().t() + bias.double()
+    y = fp8.fp8_matmul(fp8.fp8_quantize(a), fp8.fp8_quantize(w), bias=bias)
+    assert y.dtype == torch.float16 and torch.equal(y, ref.to(torch.float16))
+
+
+@pytest.mark.gpu
+def test_long_sums_give_up_and_recover(cuda_device):
+    """A sum in pieces whose loaders are held: every wait runs out, the next call is right."""
+    g = torch.Generator(device=cuda_device).manual_seed(8)
+    qa, qw = (fp8.fp8_quantize(one_sign(300, 20000, g, cuda_device)) for _ in range(2))
+    want = fp8.fp8_matmul(qa, qw, out_dtype=torch.float16)
+    torch.cuda.synchronize()
+    _lib.engine_status(reset=True)
+    _lib.set_wait_limit(20_000_000)
+    _lib.hold_producers(True)
+    try:
+        fp8.fp8_matmul(qa, qw, out_dtype=torch.float16)
+        torch.cuda.synchronize()
+        status = _lib.engine_status(reset=True)
+    finally:
+        _lib.hold_producers(False)
+        _lib.set_wait_limit(2_000_000_000)
+    assert status & 1
+    assert torch.equal(fp8.fp8_matmul(qa, qw, out_dtype=torch.float16), want)
+
+
+@pytest.mark.gpu
+def test_training_over_many_tokens(cuda_device):
+    """A weight gradient that is a sum in pieces, in fp16."""
+    g = torch.Generator().manual_seed(17)
+    x, dy = (torch.randn(17000, n, generator=g).half().to(cuda_device) for n in (40, 72))
+    w = (torch.randn(72, 40, generator=g) * 0.05).half().to(cuda_device)
+    check_training(x, w, None, dy * 0.1)
+
+
 @pytest.mark.gpu
 def test_out_and_its_refusals(cuda_device):
     a = torch.randn(30, 64, device=cuda_device)
