@@ -259,7 +259,11 @@ __device__ __forceinline__ void statistics(const QkNormParams &p, const Lane<F> 
     }
     group_sum<A>(p.lanes, mean);
 #pragma unroll
-    for (int q = 0; q < A; ++q) mean[q] *= inv;
+    for (int q = 0; q < A; ++q) {
+      // (the rounded quotient: of equal values the value itself, whatever D)
+      const float m = mean[q] * inv;
+      mean[q] = __fmaf_rn(__fmaf_rn(-m, (float)p.r.D, mean[q]), inv, m);
+    }
   }
 #pragma unroll
   for (int q = 0; q < A; ++q) {
@@ -366,8 +370,10 @@ __device__ __forceinline__ void copy_heads(const QkNormParams &p, const Lane<F> 
 
 // Heads [h0, h1) of q (role 0) or k (1).  With the partner's weight w', an element of
 // the output is
-//   rstd (x w c + x' w' s - mean (w c + w' s)) + b c + b' s,
-// whose products of weights and angles are made once per token.
+//   rstd ((x - mean) w c + (x' - mean) w' s) + b c + b' s,
+// whose products of weights and angles are made once per token.  The mean is taken off
+// first: products with x lose what lies below the mean's last bits, a thousand times
+// enlarged by the rstd of a row that is nearly constant.
 template <typename F, bool kBias>
 __device__ __forceinline__ void forward_heads(const QkNormParams &p, const Lane<F> &m,
                                               const Token &t, const Shared &weights, int role,
@@ -409,16 +415,19 @@ __device__ __forceinline__ void forward_heads(const QkNormParams &p, const Lane<
 #pragma unroll
     for (int q = 0; q < A; ++q) {
       if (h + q >= h1) break;
-      const Pairs<E> v = x[q].values();
-      Pairs<E> u, y;
-      if constexpr (F::kApart)
-        u = o[q].values();
-      else
-        u = swapped<E>(v);
+      Pairs<E> v = x[q].values(), u, y;
+      if constexpr (F::kApart) u = o[q].values();
+      if (!p.rms) {  // (what is past D or does not turn is multiplied by 0)
+#pragma unroll
+        for (int i = 0; i < E / 2; ++i) {
+          v.p[i] = add2(v.p[i], both(-mean[q]));
+          if constexpr (F::kApart) u.p[i] = add2(u.p[i], both(-mean[q]));
+        }
+      }
+      if constexpr (!F::kApart) u = swapped<E>(v);
 #pragma unroll
       for (int i = 0; i < E / 2; ++i) {
-        float2 r = fma2(v.p[i], wc.p[i], mul2(u.p[i], ws.p[i]));
-        if (!p.rms) r = fma2(both(-mean[q]), add2(wc.p[i], ws.p[i]), r);
+        const float2 r = fma2(v.p[i], wc.p[i], mul2(u.p[i], ws.p[i]));
         if constexpr (kBias)
           y.p[i] = fma2(both(rstd[q]), r, shift.p[i]);
         else

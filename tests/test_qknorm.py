@@ -349,6 +349,56 @@ def test_rows_that_are_odd(cuda_device):
         assert all(torch.equal(a, b) for a, b in ((q, q2), (k, k2), (v, v2)))
 
 
+FAR = [  # D, dims, grid: every width of pieces
+    (64, [32, 32], (4, 5)), (40, [20, 20], (5, 4)), (48, [24, 12], (3, 6)), (22, [10, 6, 4], (2, 3, 3)),
+    (128, [44, 42, 42], (2, 3, 3)), (256, [128, 128], (4, 4)), (34, [30], (19,)), (2, [2], (7,))]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("interleaved", [True, False])
+@pytest.mark.parametrize("D,dims,grid", FAR)
+def test_layer_norm_far_from_zero(cuda_device, D, dims, grid, interleaved):
+    """Rows whose mean is 100 to 1000 deviations, and constant ones, turned: what is
+    normalised is x - mean, whose terms are no larger than the deviation.  Rows are m + d
+    and m - d with few bits, so that every sum of them is exact, m is a representable mean
+    and x - m exact: the error is the deviation's (D / 2 + 8) u and a few u of each
+    product, all relative to |n|.  A constant row leaves 0, turned biases."""
+    dev, g = cuda_device, torch.Generator().manual_seed(D)
+    pos = positions(grid, 1).to(dev)
+    axes = RotaryAxes(dims, grid, interleaved=interleaved, device=dev)
+    N = pos.shape[0]
+    for i, dtype in enumerate(DTYPES):
+        step = (2.0 ** -14, 2.0 ** -4, 2.0 ** -7)[i]  # (8 + d is a number of each type)
+        for size, deviation in ((8.0, 0.08), (8.0, 0.02 if i != 1 else 0.1), (0.0, 1.0)):
+            d = (torch.randn(1, N, 3, D // 2, generator=g) * deviation / step).round() * step
+            x = torch.cat([size + d, size - d], -1)[..., torch.randperm(D, generator=g)]
+            qkv = x.reshape(1, N, 3 * D).to(dtype).to(dev)
+            assert torch.equal(qkv.cpu().float(), x.reshape(1, N, 3 * D))
+            w = [(1 + 0.3 * torch.randn(D, generator=g)).to(dev) for _ in range(2)]
+            b = [0.2 * torch.randn(D, generator=g).to(dev) for _ in range(2)]
+            for bias in ([None, None], b):
+                q, k, _ = split_qkv_norm(qkv, 1, *w, *bias, kind="layer", axes=axes, pos=pos)
+                heads = qkv.double().reshape(1, N, 3, D).transpose(1, 2)
+                for j, got in enumerate((q, k)):
+                    wj, bj = w[j].double(), None if bias[j] is None else bias[j].double()
+                    t, n, _ = norm64(heads[:, j:j + 1], wj, bj, "layer", 1e-6)
+                    mag = wj.abs() * n.abs() + (0 if bj is None else bj.abs())
+                    close(got, turn64(t, dims, pos, interleaved),
+                          (D / 2 + 16) * U * spread64(mag.expand_as(n), dims, interleaved))
+        for c in (100.0, -10.0, 7.5, 0.375, 3000.0 if i != 1 else 3008.0):
+            qkv = torch.full((1, N, 3 * D), c, dtype=dtype, device=dev)
+            leaves = [t.detach().requires_grad_() for t in (qkv, *w)]
+            q, k, _ = split_qkv_norm(leaves[0], 1, *leaves[1:], kind="layer", axes=axes, pos=pos)
+            assert not q.any() and not k.any()
+            _, dwq, dwk = torch.autograd.grad((q, k), leaves, (torch.ones_like(q),) * 2)
+            assert not dwq.any() and not dwk.any()
+            q, k, _ = split_qkv_norm(qkv, 1, *w, *b, kind="layer", axes=axes, pos=pos)
+            for got, bj in ((q, b[0]), (k, b[1])):
+                bj = bj.double().expand(1, 1, N, D)
+                close(got, turn64(bj, dims, pos, interleaved),
+                      4 * U * spread64(bj.abs(), dims, interleaved))
+
+
 @pytest.mark.gpu
 def test_batched_positions_and_range(cuda_device):
     dev, g = cuda_device, torch.Generator().manual_seed(1)
