@@ -24,6 +24,7 @@ LFSR-16 pool seeded per block) and optional head-aligned compensation
 from __future__ import annotations
 
 import functools
+import threading
 from typing import Callable, Dict, Iterable, Optional
 
 import torch
@@ -388,12 +389,37 @@ def dropout(x: torch.Tensor, p: float, seed, offset: int = 0, *, per: str = "ele
     return _dropout_launch(_dense(x), _dense(residual), float(p), seed, offset, state, span)
 
 
+class _Calls:
+    """Numbers of a module's calls, each given out once: to its threads, and to its
+    data-parallel replicas, which are copies made for one call and hold this same object
+    (a sequence for each of their devices, so that what one draws does not depend on when
+    the others run)."""
+
+    def __init__(self, start: int = 0):
+        self.start, self.taken, self.lock = start, {}, threading.Lock()
+
+    def take(self, device: Optional[int] = None) -> int:
+        with self.lock:
+            n = self.taken.get(device, self.start)
+            self.taken[device] = n + 1
+        return n if device is None else (device + 1 << 40) + n
+
+    def most(self) -> int:
+        with self.lock:
+            return max(self.taken.values(), default=self.start)
+
+    def __reduce__(self):  # (copies count for themselves)
+        return _Calls, (self.most(),)
+
+
 class Dropout(nn.Module):
     """``dropout`` in a model: in training every call takes the next mask, in
     evaluation it passes through.  ``index`` tells the modules of a model apart, which
     may then share ``seed``; ranks that are to draw apart take seeds of their own.
-    ``calls`` counts (and, set, repeats) the eager masks; calls that a graph captures
-    count on the device, so that every replay draws masks of its own.  A call made
+    ``calls`` counts (and, set, repeats) the eager masks, over threads (who takes which is
+    theirs to order) and data-parallel replicas (whose devices draw masks of their own);
+    calls that a graph captures count on the device, so that every replay draws masks of
+    its own.  A call made
     while a backward pass runs (a checkpoint's recomputation) would take the next mask
     instead of the one to be repeated, and raises: ``dropout`` with an offset of the
     caller's own repeats it."""
@@ -409,13 +435,26 @@ class Dropout(nn.Module):
         seed = int(seed)
         if not -1 << 63 <= seed < 1 << 64:
             raise ValueError(f"seed is 64-bit, got {seed}")
-        self.p, self.per, self.index, self.calls = float(p), per, index, 0
+        self.p, self.per, self.index, self._calls = float(p), per, index, _Calls()
         self.seed = seed - (1 << 64) if seed >= 1 << 63 else seed  # (as int64 holds it)
         self.register_buffer("state", torch.tensor([self.seed, 0]), persistent=False)
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        if "_calls" not in self.__dict__:  # (saved whole by an earlier version)
+            self._calls = _Calls(self.__dict__.pop("calls", 0))
 
     @property
     def active(self) -> bool:
         return self.training and self.p > 0
+
+    @property
+    def calls(self) -> int:
+        return self._calls.most()
+
+    @calls.setter
+    def calls(self, n: int) -> None:
+        self._calls = _Calls(int(n))
 
     def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
         if not self.active:
@@ -424,13 +463,13 @@ class Dropout(nn.Module):
             raise RuntimeError("a Dropout module called inside a backward pass (by an activation "
                                "checkpoint?) cannot repeat the mask of its first call; use "
                                "dropout() with an offset of your own there")
-        at = self.index << 48  # (its calls below 2^47, the captured ones above)
+        at = self.index << 48  # (its calls below 2^40, replicas' and, from 2^47, captured ones above)
         if x.is_cuda and torch.cuda.is_current_stream_capturing():
             state = self.state.clone()
             self.state[1:] += 1
             return dropout(x, self.p, state, at + (1 << 47), per=self.per, residual=residual)
-        offset = at + self.calls
-        self.calls += 1
+        replica = getattr(self, "_is_replica", False)
+        offset = at + self._calls.take(x.get_device() if replica else None)
         return dropout(x, self.p, self.seed, offset, per=self.per, residual=residual)
 
     def extra_repr(self) -> str:

@@ -3,6 +3,9 @@ modules in a block, and the refusals."""
 import copy
 import ctypes
 import math
+import pickle
+import sys
+import threading
 
 import numpy as np
 import pytest
@@ -177,6 +180,62 @@ def test_module_refused_inside_a_backward_pass():
     x = torch.ones(3, requires_grad=True)
     Recomputed.apply(x).sum().backward()
     assert message and m.calls == 0 and torch.equal(x.grad, torch.ones(3))
+
+
+@pytest.fixture
+def offsets(monkeypatch):
+    """Dropout modules record the offsets of their calls instead of launching."""
+    seen = []
+    monkeypatch.setattr(vit, "dropout", lambda x, p, seed, offset, **kw: (seen.append(offset), x)[1])
+    return seen
+
+
+def test_threads_take_a_mask_each(offsets):
+    """No two calls of a shared module draw the same mask."""
+    m, x = vit.Dropout(0.5, index=1), torch.ones(2)
+    old, go = sys.getswitchinterval(), threading.Barrier(8)
+
+    def run():
+        go.wait()
+        for _ in range(1500):
+            m(x)
+    sys.setswitchinterval(1e-6)
+    try:
+        threads = [threading.Thread(target=run) for _ in range(8)]
+        [t.start() for t in threads]
+        [t.join() for t in threads]
+    finally:
+        sys.setswitchinterval(old)
+    assert sorted(offsets) == [(1 << 48) + i for i in range(12000)] and m.calls == 12000
+
+
+def test_data_parallel_replicas_draw_on(offsets, monkeypatch):
+    """Replicas live for one call: what they count stays with the module, on each
+    device a sequence of its own."""
+    monkeypatch.setattr(torch.Tensor, "get_device", lambda t: int(t[0]))
+    m = vit.Dropout(0.5, index=2)
+    for step in range(2):
+        for device in (1, 0):
+            m._replicate_for_data_parallel()(torch.tensor([float(device)]))
+    assert offsets == [(2 << 48) + (d + 1 << 40) + i for i in range(2) for d in (1, 0)]
+    m(torch.ones(1))
+    assert offsets[4:] == [2 << 48] and m.calls == 2
+    for c in (copy.deepcopy(m), pickle.loads(pickle.dumps(m))):
+        c(torch.ones(1))
+        assert offsets[-1] == (2 << 48) + 2 and c.calls == 3 and m.calls == 2
+    m.calls = 7
+    m(torch.ones(1))
+    m._replicate_for_data_parallel()(torch.zeros(1))
+    assert offsets[-2:] == [(2 << 48) + 7, (2 << 48) + (1 << 40) + 7] and m.calls == 8
+
+
+def test_modules_saved_whole_before_replicas_counted():
+    m = vit.Dropout(0.5)
+    state = m.__dict__.copy()
+    del state["_calls"]
+    old = vit.Dropout.__new__(vit.Dropout)
+    old.__setstate__(dict(state, calls=5))
+    assert old.calls == 5 and old._calls.take() == 5 and old.calls == 6
 
 
 # ------------------------------------------------------------ GPU
