@@ -419,7 +419,9 @@ class Dropout(nn.Module):
     ``calls`` counts (and, set, repeats) the eager masks, over threads (who takes which is
     theirs to order) and data-parallel replicas (whose devices draw masks of their own);
     calls that a graph captures count on the device, so that every replay draws masks of
-    its own.  A call made
+    its own.  Both counts go with a state dict, in its metadata (its keys are those of a
+    model without dropout, so that either loads the other's), and a run that loads it draws
+    on where the saved one stopped.  A call made
     while a backward pass runs (a checkpoint's recomputation) would take the next mask
     instead of the one to be repeated, and raises: ``dropout`` with an offset of the
     caller's own repeats it."""
@@ -436,11 +438,30 @@ class Dropout(nn.Module):
         if not -1 << 63 <= seed < 1 << 64:
             raise ValueError(f"seed is 64-bit, got {seed}")
         self.p, self.per, self.index, self._calls = float(p), per, index, _Calls()
+        self._captured = False  # whether a graph has captured a call
         self.seed = seed - (1 << 64) if seed >= 1 << 63 else seed  # (as int64 holds it)
         self.register_buffer("state", torch.tensor([self.seed, 0]), persistent=False)
 
+    def _save_to_state_dict(self, destination, prefix, keep_vars):
+        super()._save_to_state_dict(destination, prefix, keep_vars)
+        metadata = getattr(destination, "_metadata", None)
+        if metadata is not None:
+            counts = metadata.setdefault(prefix[:-1], {})
+            counts["calls"] = self.calls
+            if self._captured:  # (read back from the device)
+                counts["captured"] = int(self.state[1])
+
+    def _load_from_state_dict(self, state_dict, prefix, local_metadata, *args):
+        super()._load_from_state_dict(state_dict, prefix, local_metadata, *args)
+        if "calls" in local_metadata:
+            self.calls = local_metadata["calls"]
+        if "captured" in local_metadata:
+            self._captured = True
+            self.state[1:].fill_(local_metadata["captured"])
+
     def __setstate__(self, state):
         super().__setstate__(state)
+        self.__dict__.setdefault("_captured", True)
         if "_calls" not in self.__dict__:  # (saved whole by an earlier version)
             self._calls = _Calls(self.__dict__.pop("calls", 0))
 
@@ -465,6 +486,7 @@ class Dropout(nn.Module):
                                "dropout() with an offset of your own there")
         at = self.index << 48  # (its calls below 2^40, replicas' and, from 2^47, captured ones above)
         if x.is_cuda and torch.cuda.is_current_stream_capturing():
+            self._captured = True
             state = self.state.clone()
             self.state[1:] += 1
             return dropout(x, self.p, state, at + (1 << 47), per=self.per, residual=residual)

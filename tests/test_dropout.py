@@ -2,6 +2,7 @@
 modules in a block, and the refusals."""
 import copy
 import ctypes
+import io
 import math
 import pickle
 import sys
@@ -228,6 +229,45 @@ def test_data_parallel_replicas_draw_on(offsets, monkeypatch):
     m._replicate_for_data_parallel()(torch.zeros(1))
     assert offsets[-2:] == [(2 << 48) + 7, (2 << 48) + (1 << 40) + 7] and m.calls == 8
 
+def saved(module):
+    """Its state dict, written to a file and read again."""
+    f = io.BytesIO()
+    torch.save(module.state_dict(), f)
+    f.seek(0)
+    return torch.load(f, weights_only=True)
+
+
+def test_a_resumed_run_draws_on(offsets):
+    """Counts go with the state dict, whose keys stay; models with and without dropout
+    load each other's."""
+    def model():
+        m = torch.nn.Sequential(torch.nn.Linear(2, 2), vit.Dropout(0.5, index=1),
+                                torch.nn.Sequential(vit.Dropout(0.5, index=2)))
+        return m.train()
+    m, x = model(), torch.ones(1, 2)
+    for _ in range(3):
+        m(x)
+    m[1](x)
+    state = saved(m)
+    assert set(state) == {"0.weight", "0.bias"}
+    again = model()
+    again.load_state_dict(state)
+    del offsets[:]
+    again(x)
+    assert offsets == [(1 << 48) + 4, (2 << 48) + 3]
+    assert (m[1].calls, m[2][0].calls) == (4, 3)
+    plain = torch.nn.Sequential(torch.nn.Linear(2, 2), torch.nn.Identity(), torch.nn.Identity())
+    plain.load_state_dict(state)
+    again.load_state_dict(saved(plain))
+    again.load_state_dict(dict(state))  # (no metadata: the counts stay)
+    assert (again[1].calls, again[2][0].calls) == (5, 4)
+    with torch.no_grad():  # captured calls count in `state`
+        m[1].state[1], m[1]._captured = 9, True
+    again.load_state_dict(saved(m))
+    assert int(again[1].state[1]) == 9 and int(again[2][0].state[1]) == 0
+    assert saved(again)._metadata["1"]["captured"] == 9
+
+
 
 def test_modules_saved_whole_before_replicas_counted():
     m = vit.Dropout(0.5)
@@ -381,6 +421,33 @@ def test_module_masks(cuda_device):
             seen.append(t.clone())
             assert torch.equal(t, expect(x, 0.5, 3, (2 << 48) + (1 << 47) + 2 * i + j, "element"))
     assert all(not torch.equal(s, t) for i, s in enumerate(seen) for t in seen[:i])
+
+
+@pytest.mark.gpu
+def test_captured_masks_of_a_resumed_run(cuda_device):
+    x = torch.randn(64, 96, device=cuda_device)
+    m = vit.Dropout(0.5, seed=3, index=2).to(cuda_device)
+
+    def captured(m):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = m(x)
+        return graph, y
+    graph, y = captured(m)
+    for _ in range(3):
+        graph.replay()
+    state = saved(m)
+    for loaded_first in (True, False):
+        n = vit.Dropout(0.5, seed=3, index=2).to(cuda_device)
+        if loaded_first:
+            n.load_state_dict(state)
+        graph, y = captured(n)
+        if not loaded_first:
+            n.load_state_dict(state)
+        for i in (3, 4):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(y, expect(x, 0.5, 3, (2 << 48) + (1 << 47) + i, "element"))
 
 
 def small(dev, **kw):
