@@ -440,7 +440,16 @@ class Dropout(nn.Module):
         self.p, self.per, self.index, self._calls = float(p), per, index, _Calls()
         self._captured = False  # whether a graph has captured a call
         self.seed = seed - (1 << 64) if seed >= 1 << 63 else seed  # (as int64 holds it)
-        self.register_buffer("state", torch.tensor([self.seed, 0]), persistent=False)
+        # (no buffer: wrappers that broadcast buffers would give every rank the first one's seed)
+        self.state = torch.tensor([self.seed, 0])
+
+    def _apply(self, fn, *args):
+        super()._apply(fn, *args)
+        device = fn(self.state).device  # (its values stay, where fn only allocates too)
+        if device != self.state.device:
+            state = torch.tensor([self.seed, 0], device="cpu") if self.state.is_meta else self.state
+            self.state = state.to(device)
+        return self
 
     def _save_to_state_dict(self, destination, prefix, keep_vars):
         super()._save_to_state_dict(destination, prefix, keep_vars)
@@ -462,6 +471,10 @@ class Dropout(nn.Module):
     def __setstate__(self, state):
         super().__setstate__(state)
         self.__dict__.setdefault("_captured", True)
+        if "state" in self._buffers:
+            state = self._buffers.pop("state")
+            self._non_persistent_buffers_set.discard("state")
+            self.state = state
         if "_calls" not in self.__dict__:  # (saved whole by an earlier version)
             self._calls = _Calls(self.__dict__.pop("calls", 0))
 

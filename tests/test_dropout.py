@@ -2,15 +2,20 @@
 modules in a block, and the refusals."""
 import copy
 import ctypes
+import datetime
 import io
 import math
+import os
 import pickle
+import socket
 import sys
 import threading
 
 import numpy as np
 import pytest
 import torch
+import torch.distributed as dist
+import torch.multiprocessing as mp
 
 from scmp_vit_b200 import _lib, vit
 
@@ -276,6 +281,48 @@ def test_modules_saved_whole_before_replicas_counted():
     old = vit.Dropout.__new__(vit.Dropout)
     old.__setstate__(dict(state, calls=5))
     assert old.calls == 5 and old._calls.take() == 5 and old.calls == 6
+
+
+def _rank(rank, port, q):
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port))
+    dist.init_process_group("gloo", rank=rank, world_size=2,
+                            timeout=datetime.timedelta(seconds=60))
+    m = torch.nn.Sequential(torch.nn.Linear(2, 2), vit.Dropout(0.5, seed=10 + rank)).eval()
+    wrapped = torch.nn.parallel.DistributedDataParallel(m)
+    wrapped(torch.ones(1, 2)).sum().backward()
+    q.put((rank, m[1].state.tolist()))
+    dist.barrier()
+    dist.destroy_process_group()
+
+
+def test_ranks_keep_their_seeds():
+    """What a data-parallel wrapper makes alike on all ranks leaves the seeds apart."""
+    with socket.socket() as s:
+        s.bind(("127.0.0.1", 0))
+        port = s.getsockname()[1]
+    ctx = mp.get_context("spawn")
+    q = ctx.Queue()
+    ranks = [ctx.Process(target=_rank, args=(r, port, q)) for r in range(2)]
+    [r.start() for r in ranks]
+    got = dict(q.get(timeout=120) for _ in ranks)
+    [r.join(60) for r in ranks]
+    assert got == {0: [10, 0], 1: [11, 0]} and all(r.exitcode == 0 for r in ranks)
+
+
+def test_the_captured_state_moves_with_its_module():
+    m = torch.nn.Sequential(vit.Dropout(0.5, seed=-4))
+    assert not list(m.buffers()) and m.half()[0].state.tolist() == [-4, 0]
+    m[0].state[1] = 3
+    assert copy.deepcopy(m)[0].state.tolist() == [-4, 3]
+    assert m.to_empty(device="cpu")[0].state.tolist() == [-4, 3]
+    assert m.to("meta")[0].state.is_meta
+    assert m.to_empty(device="cpu")[0].state.tolist() == [-4, 0]
+    old = vit.Dropout(0.5, seed=6)  # as earlier versions kept it
+    state = dict(old.__dict__, _buffers={"state": old.state}, _non_persistent_buffers_set={"state"})
+    del state["state"]
+    new = vit.Dropout.__new__(vit.Dropout)
+    new.__setstate__(state)
+    assert new.state.tolist() == [6, 0] and not list(new.buffers())
 
 
 # ------------------------------------------------------------ GPU
