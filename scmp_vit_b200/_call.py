@@ -1,6 +1,8 @@
 """Calls into the engine library on a tensor's device and current stream."""
 from __future__ import annotations
 
+from typing import Optional
+
 import torch
 import torch.autograd.forward_ad as _forward_ad
 
@@ -19,16 +21,12 @@ except AttributeError:
     _current_device = torch.cuda.current_device
 
 
-try:
-    _graph_task = torch._C._current_graph_task_id
-except AttributeError:  # (a torch that does not tell)
-    def _graph_task() -> int:
-        return -1
+_graph_task = getattr(torch._C, "_current_graph_task_id", None)
 
 
-def in_backward() -> bool:
-    """Whether this thread is inside a backward pass."""
-    return _graph_task() >= 0
+def in_backward() -> Optional[bool]:
+    """Whether this thread is inside a backward pass; None where torch does not tell."""
+    return None if _graph_task is None else _graph_task() >= 0
 
 
 def call(fn, index: int, *args) -> None:

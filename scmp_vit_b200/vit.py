@@ -493,7 +493,12 @@ class Dropout(nn.Module):
     def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
         if not self.active:
             return x if residual is None else residual + x
-        if in_backward():
+        inside = in_backward()
+        if inside is None:
+            raise RuntimeError("this torch does not tell whether a backward pass runs, in which a "
+                               "Dropout module must not take the next mask; use dropout() with "
+                               "an offset of your own")
+        if inside:
             raise RuntimeError("a Dropout module called inside a backward pass (by an activation "
                                "checkpoint?) cannot repeat the mask of its first call; use "
                                "dropout() with an offset of your own there")

@@ -188,6 +188,16 @@ def test_module_refused_inside_a_backward_pass():
     assert message and m.calls == 0 and torch.equal(x.grad, torch.ones(3))
 
 
+def test_module_refused_where_torch_does_not_tell(monkeypatch):
+    """Without the query a recomputation would draw another mask in silence."""
+    from scmp_vit_b200 import _call
+    monkeypatch.setattr(_call, "_graph_task", None)
+    m, x = vit.Dropout(0.5), torch.ones(3)
+    with pytest.raises(RuntimeError, match="does not tell"):
+        m(x)
+    assert m.calls == 0 and m.eval()(x) is x
+
+
 @pytest.fixture
 def offsets(monkeypatch):
     """Dropout modules record the offsets of their calls instead of launching."""
