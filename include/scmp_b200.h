@@ -434,8 +434,8 @@ SCMP_API int scmp_split_qkv_rotary(const scmp_rotary_args *args, void *stream);
  * split.inverse: the gradients, from q, k, v (their gradients) and x (the forward's
  * qkv) to qkv, and to dq_weight, dk_weight, dq_bias, dk_bias (each nullable: not
  * wanted), for which the workspace holds partial sums
- * (scmp_split_qkv_norm_workspace).  Deterministic.  One launch, two with gradients of
- * parameters. */
+ * (scmp_split_qkv_norm_workspace; a function of D so far); of no rows they are 0.
+ * Deterministic.  One launch, two with gradients of parameters. */
 typedef struct scmp_qknorm_args {
   scmp_rotary_args split;
   const void *x;

@@ -421,14 +421,24 @@ int scmp_split_qkv_norm(const scmp_qknorm_args *args, void *stream) {
   if (!(args->eps >= 0.0f)) return fail(SCMP_EINVAL, "eps must be >= 0");
   QkNormParams p{};
   int rc = check_rotary("split_qkv_norm", x, p.r);
-  if (rc != SCMP_OK) return rc;
-  if (x.B == 0 || x.N == 0) return SCMP_OK;
-  if (!args->q_weight || !args->k_weight)
-    return fail(SCMP_EINVAL, "q_weight and k_weight must be non-NULL");
-  if ((rc = check_elements({args->q_weight, args->k_weight, args->q_bias, args->k_bias,
+  if (rc != SCMP_OK ||
+      (rc = check_elements({args->q_weight, args->k_weight, args->q_bias, args->k_bias,
                             args->dq_weight, args->dk_weight, args->dq_bias, args->dk_bias},
                            args->param_dtype)) != SCMP_OK)
     return rc;
+  void *const grads[4] = {args->dq_weight, args->dq_bias, args->dk_weight, args->dk_bias};
+  if (x.B == 0 || x.N == 0) {
+    if (x.inverse)  // (sums over no rows)
+      for (void *g : grads) {
+        const size_t bytes = (size_t)(x.D * dtype_bytes(args->param_dtype));
+        const cudaError_t e =
+            g ? cudaMemsetAsync(g, 0, bytes, static_cast<cudaStream_t>(stream)) : cudaSuccess;
+        if (e != cudaSuccess) return cuda_fail(e, "split_qkv_norm gradients of no rows");
+      }
+    return SCMP_OK;
+  }
+  if (!args->q_weight || !args->k_weight)
+    return fail(SCMP_EINVAL, "q_weight and k_weight must be non-NULL");
   p.weight[0] = args->q_weight;
   p.weight[1] = args->k_weight;
   p.bias[0] = args->q_bias;
@@ -436,7 +446,6 @@ int scmp_split_qkv_norm(const scmp_qknorm_args *args, void *stream) {
   p.param_dtype = args->param_dtype;
   p.eps = args->eps;
   p.rms = args->rms != 0;
-  void *const grads[4] = {args->dq_weight, args->dq_bias, args->dk_weight, args->dk_bias};
   if (x.inverse) {
     if (!args->x) return fail(SCMP_EINVAL, "x (the forward's qkv) must be non-NULL");
     if ((rc = check_elements({args->x}, x.dtype)) != SCMP_OK) return rc;

@@ -470,6 +470,30 @@ def test_strides_streams_graph_empty_repeats(cuda_device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("empty", ["B", "N"])
+def test_parameter_gradients_of_no_rows_at_the_c_entry(cuda_device, dtype, empty):
+    """Sums over nothing: 0 in each gradient that is wanted, nothing behind it."""
+    code = DTYPES.index(dtype)
+    for wanted in range(16):
+        out = torch.full((4, 40), math.nan, dtype=dtype, device=cuda_device)
+        names = ("dq_weight", "dk_weight", "dq_bias", "dk_bias")
+        at = {n: out[i].data_ptr() for i, n in enumerate(names) if wanted >> i & 1}
+        a = args(inverse=1, D=32, dtype=code, param_dtype=code, **{empty: 0}, **at)
+        attention.call(_lib.load().scmp_split_qkv_norm, 0, bytes(a))
+        for i in range(4):
+            n = 32 if wanted >> i & 1 else 0
+            assert not out[i, :n].any() and bool(out[i, n:].isnan().all())
+
+
+def test_no_rows_on_the_cpu():
+    lib = _lib.load()
+    assert lib.scmp_split_qkv_norm(ctypes.byref(args(inverse=1, B=0)), None) == 0
+    assert lib.scmp_split_qkv_norm(ctypes.byref(args(inverse=1, N=0, dk_bias=18)), None) == -1
+    assert "aligned to its elements" in _lib.last_error()
+
+
+@pytest.mark.gpu
 def test_wants_and_second_derivative(cuda_device):
     dev, g = cuda_device, torch.Generator().manual_seed(2)
     qkv, w, b = (torch.randn(*s, generator=g).to(dev) for s in ((2, 9, 96), (16,), (16,)))
