@@ -403,6 +403,30 @@ def test_dropped_values_leave_nothing(cuda_device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("per", vit.PER)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_dropped_values_leave_nothing_either_way(cuda_device, dtype, bad, per):
+    """The same of gradients, for every draw and type: what comes in at a dropped place
+    is 0 in x's gradient and comes through in the residual's, whose value is y's there."""
+    shape = (33, 7, 24)
+    keep = keep_of(shape, 0.5, 1, 2, per).to(cuda_device)
+    g = torch.Generator().manual_seed(7)
+    x, r, dy = (torch.randn(*shape, generator=g).to(dtype).to(cuda_device) for _ in range(3))
+    x[~keep] = bad
+    dy[~keep] = bad
+    leaves = [x.requires_grad_(), r.requires_grad_()]
+    y = vit.dropout(x, 0.5, 1, 2, per=per, residual=r)
+    assert torch.equal(y[~keep], r[~keep]) and bool(y.isfinite().all())
+    dx, dr = torch.autograd.grad(y, leaves, dy)
+    assert not dx[~keep].any() and torch.equal(dx[keep], 2 * dy[keep])
+    assert torch.equal(dr.nan_to_num(7.0), dy.nan_to_num(7.0))
+    y = vit.dropout(x, 0.5, 1, 2, per=per)
+    (dx2,) = torch.autograd.grad(y, x, dy)
+    assert not y[~keep].any() and torch.equal(dx2, dx)
+
+
+@pytest.mark.gpu
 def test_in_place_at_the_c_entry(cuda_device):
     """y may be x or residual."""
     x = torch.randn(1000, device=cuda_device)
