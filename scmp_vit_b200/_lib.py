@@ -26,7 +26,6 @@ ENGINE = {"auto": 0, "popc": 1, "tcgen05": 2}
 MX_FORMAT = {"mxfp4": 0, "nvfp4": 1}
 MX_BLOCK = {"mxfp4": 32, "nvfp4": 16}
 MX_THIN_ROWS, MX_THIN_K = 4, 6144  # SCMP_MX_THIN_ROWS, SCMP_MX_THIN_K
-FP8_BLOCK = 128
 FP8_THIN_ROWS, FP8_THIN_K = 4, 6144  # SCMP_FP8_THIN_ROWS, SCMP_FP8_THIN_K
 MAX_AXES = 4  # SCMP_MAX_AXES
 IO_A_BF16, IO_B_BF16, IO_OUT_BF16, IO_B_PACKED, IO_A_QUANT = 1, 2, 4, 8, 16  # io_flags bits

@@ -688,7 +688,6 @@ template <typename F> cudaError_t launch_form(QkNormParams p, cudaStream_t s) {
   p.units = (uint32_t)units;
   const uint32_t most = 148u * (r.inverse ? blocks_per_sm<F, true>() : blocks_per_sm<F, false>());
   r.turn_blocks = p.units < most ? p.units : most;
-  r.per = FastDiv((uint32_t)(r.D / F::L));
   const bool bias = r.inverse ? p.grads[1] || p.grads[3] : p.bias[0] || p.bias[1];
   auto kern = r.inverse ? (bias ? qknorm_bwd_kernel<F, true> : qknorm_bwd_kernel<F, false>)
                         : (bias ? qknorm_kernel<F, true> : qknorm_kernel<F, false>);
