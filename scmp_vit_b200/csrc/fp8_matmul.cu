@@ -22,9 +22,10 @@
 //
 // Long sums are bound by power (8192^3: 410 us at 1.1 GHz, 343 of zeros at 1.97), fc1 of 64
 // images ([16448, 1024] by [4096, 1024], bf16: 62 us) by its outputs besides: without
-// their stores it takes 47.  An SM writes some 14 bytes a clock however it does it (K =
-// 128, which leaves little else: pieces of 64-byte rows 33 us, of 128-byte rows 38, from
-// registers 42), and operands on their way in wait.  One stage of B for both accumulators
+// their stores it takes 47.  At K = 128, which leaves little but the stores, pieces of
+// 64-byte rows take 33 us, of 128-byte rows 38, from registers 42: what these stores cost
+// beside these loads, not what an SM can write (the dequantiser's fp32 leave at 17
+// bytes a clock and SM, 33 us are 14).  One stage of B for both accumulators
 // loads 27 % less, but then their tiles end together: fc1 63 us, K = 4096 186 for 193.
 //
 // Where a sum is so long that the bits that the tensor core cuts off would show, it is
