@@ -443,8 +443,8 @@ class Dropout(nn.Module):
         # (no buffer: wrappers that broadcast buffers would give every rank the first one's seed)
         self.state = torch.tensor([self.seed, 0])
 
-    def _apply(self, fn, *args):
-        super()._apply(fn, *args)
+    def _apply(self, fn, *args, **kwargs):
+        super()._apply(fn, *args, **kwargs)
         device = fn(self.state).device  # (its values stay, where fn only allocates too)
         if device != self.state.device:
             state = torch.tensor([self.seed, 0], device="cpu") if self.state.is_meta else self.state

@@ -327,6 +327,9 @@ def test_the_captured_state_moves_with_its_module():
     assert m.to_empty(device="cpu")[0].state.tolist() == [-4, 3]
     assert m.to("meta")[0].state.is_meta
     assert m.to_empty(device="cpu")[0].state.tolist() == [-4, 0]
+    d = vit.Dropout(0.5, seed=5)  # (the module itself, which passes `recurse` on)
+    assert d.to_empty(device="meta", recurse=False).state.is_meta
+    assert d.to_empty(device="cpu").state.tolist() == [5, 0]
     old = vit.Dropout(0.5, seed=6)  # as earlier versions kept it
     state = dict(old.__dict__, _buffers={"state": old.state}, _non_persistent_buffers_set={"state"})
     del state["state"]
