@@ -419,7 +419,8 @@ class Dropout(nn.Module):
     ``calls`` counts (and, set, repeats) the eager masks, over threads (who takes which is
     theirs to order) and data-parallel replicas (whose devices draw masks of their own);
     calls that a graph captures count on the device, so that every replay draws masks of
-    its own.  Both counts go with a state dict, in its metadata (its keys are those of a
+    its own (replays that share a module follow one another, as they do for its weights'
+    sake).  Both counts go with a state dict, in its metadata (its keys are those of a
     model without dropout, so that either loads the other's), and a run that loads it draws
     on where the saved one stopped.  A call made
     while a backward pass runs (a checkpoint's recomputation) would take the next mask
